@@ -701,6 +701,94 @@ int cubic_embedding(const void* ids, int id_bytes, int64_t tokens, int fmt, cons
 }
 
 // ---------------------------------------------------------------------------
+// Low-rank adapters
+// ---------------------------------------------------------------------------
+int64_t cubic_adapters_workspace_bytes(int64_t m, int64_t k, int members, const int* max_ranks) {
+    if (m <= 0 || m >= (1 << 24) || k <= 0 || k > (1 << 20) || members < 1 ||
+        members > cubic::kMaxGemmMembers || !max_ranks)
+        return -1;
+    int64_t tiles = 0;
+    for (int j = 0; j < members; ++j) {
+        if (max_ranks[j] < 8 || max_ranks[j] > cubic::kMaxAdapterRank || max_ranks[j] % 8) return -1;
+        tiles += ceil_div(max_ranks[j], 16);
+    }
+    return ceil_div(k, cubic::kAdapterDownK) * m * tiles * 16 * (int64_t)sizeof(float);
+}
+
+int cubic_adapters(const void* x, int64_t ldx, const int32_t* row_slots, int64_t m, int64_t k, int slots,
+                   int members, const int64_t* ns, const int* max_ranks, const void* const* downs,
+                   const void* const* ups, const float* const* scales, const int32_t* const* ranks,
+                   const void* const* bases, const int64_t* ldbases, void* const* ys, const int64_t* ldys,
+                   int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+    if (!x || !row_slots || !ns || !max_ranks || !downs || !ups || !scales || !ranks || !bases ||
+        !ldbases || !ys || !ldys)
+        return fail(CUBIC_EINVAL, "adapters: null operand");
+    if (dtype != CUBIC_DTYPE_BF16 && dtype != CUBIC_DTYPE_F16) return fail(CUBIC_ENOTSUP, "dtype=%d", dtype);
+    if (members < 1 || members > cubic::kMaxGemmMembers)
+        return fail(CUBIC_EINVAL, "members=%d outside 1..%d", members, cubic::kMaxGemmMembers);
+    if (m <= 0 || m >= (1 << 24) || k <= 0 || k > (1 << 20) || slots <= 0 || slots >= (1 << 20))
+        return fail(CUBIC_EINVAL, "adapters extents: m=%lld k=%lld slots=%d", (long long)m, (long long)k, slots);
+    if (k % 8 || ldx % 8 || ldx < k || ldx > (1 << 23) || !aligned16(x))
+        return fail(CUBIC_ENOTSUP, "activations need k %% 8 == 0, ldx %% 8 == 0, ldx <= 2^23 and 16-byte alignment");
+    cubic::AdapterArgs a = {};
+    a.x = (const uint16_t*)x;
+    a.row_slots = row_slots;
+    a.ldx = ldx;
+    a.m = (int)m;
+    a.k = (int)k;
+    a.slots = slots;
+    a.f16 = dtype == CUBIC_DTYPE_F16;
+    a.split = (int)ceil_div(k, cubic::kAdapterDownK);
+    a.vectors = 1;
+    int64_t columns = 0;
+    int largest = 0;
+    for (int j = 0; j < members; ++j) {
+        if (!downs[j] || !ups[j] || !scales[j] || !ranks[j] || !bases[j] || !ys[j])
+            return fail(CUBIC_EINVAL, "adapters: null operand of member %d", j);
+        if (max_ranks[j] < 8 || max_ranks[j] > cubic::kMaxAdapterRank || max_ranks[j] % 8)
+            return fail(CUBIC_ENOTSUP, "adapter rank capacity %d must be a multiple of 8 in 8..%d",
+                        max_ranks[j], cubic::kMaxAdapterRank);
+        if (ns[j] <= 0 || ns[j] * max_ranks[j] >= (1 << 30) || ns[j] >= (1 << 30))
+            return fail(CUBIC_EINVAL, "adapter width %lld of member %d", (long long)ns[j], j);
+        if (ldbases[j] < ns[j] || ldys[j] < ns[j])
+            return fail(CUBIC_EINVAL, "output leading dimension too small");
+        if (!aligned16(downs[j]) || !aligned16(ups[j]))
+            return fail(CUBIC_ENOTSUP, "adapters need 16-byte alignment");
+        cubic::AdapterMember& b = a.member[j];
+        b = {(const uint16_t*)downs[j], (const uint16_t*)ups[j], scales[j], ranks[j],
+             (const uint16_t*)bases[j], (uint16_t*)ys[j], ldbases[j], ldys[j], (int)ns[j], max_ranks[j],
+             a.tiles, a.tiles + (int)ceil_div(max_ranks[j], 16), 0, 0};
+        a.tiles = b.tile1;
+        a.vectors &= ns[j] % 8 == 0 && ldbases[j] % 8 == 0 && ldys[j] % 8 == 0 && aligned16(bases[j]) &&
+                     aligned16(ys[j]);
+        columns += ns[j];
+        largest = std::max(largest, max_ranks[j]);
+    }
+    a.width = 16 * a.tiles;
+    a.rank_steps = (int)ceil_div(largest, 32);
+    const int64_t need = (int64_t)a.split * m * a.width * (int64_t)sizeof(float);
+    if (workspace_bytes < need)
+        return fail(CUBIC_EWORKSPACE, "adapter workspace %lld < %lld bytes", (long long)workspace_bytes, (long long)need);
+    if (!workspace || !aligned16(workspace)) return fail(CUBIC_EINVAL, "adapter workspace must be 16-byte aligned");
+    a.partial = (float*)workspace;
+    a.down_rows = m <= 128 ? 1 : m <= 1024 ? 2 : 4;
+    a.up_rows = a.rank_steps > 4 ? std::min(a.down_rows, 2) : a.down_rows;
+    auto groups = [&](int rows) { return rows == 1 ? (int)std::min<int64_t>(16, m) : rows == 2 ? 4 : 1; };
+    a.down_groups = groups(a.down_rows);
+    a.up_groups = groups(a.up_rows);
+    const int64_t rows = ceil_div(m, 16 * a.up_rows) * a.up_groups;
+    a.chunk_cols = 128;
+    while (a.chunk_cols < 2048 && rows * ceil_div(columns, 2 * a.chunk_cols) >= 1024) a.chunk_cols *= 2;
+    for (int j = 0; j < members; ++j) {
+        a.member[j].chunk0 = a.chunks;
+        a.chunks += (int)ceil_div(ns[j], a.chunk_cols);
+        a.member[j].chunk1 = a.chunks;
+    }
+    if (a.chunks > 65535) return fail(CUBIC_ENOTSUP, "adapter widths too large");
+    return hip_status(cubic::launch_adapters(a, (hipStream_t)stream), "cubic_adapters launch");
+}
+
+// ---------------------------------------------------------------------------
 // Routed experts (MoE)
 // ---------------------------------------------------------------------------
 int cubic_moe_pad_routes(const int32_t* counts, const int32_t* starts, const int32_t* block_starts,

@@ -250,6 +250,37 @@ struct GuardArgs {
     uint8_t* valid;               // [1]
 };
 
+// Low-rank adapters beside a shared projection (cubic_adapters.hip)
+constexpr int kAdapterDownK = 1024;  // columns of x per K partition
+constexpr int kMaxAdapterRank = 256;
+struct AdapterMember {
+    const uint16_t* down;         // [slots, max_rank, k]
+    const uint16_t* up;           // [slots, n, max_rank]
+    const float* scales;          // [slots]
+    const int32_t* ranks;         // [slots]: 0 = empty
+    const uint16_t* base;         // [m, ldbase]
+    uint16_t* y;                  // [m, ldy]
+    int64_t ldbase, ldy;
+    int n, max_rank;              // max_rank % 8 == 0
+    int tile0, tile1;             // its 16-rank tiles among all members'
+    int chunk0, chunk1;           // its column chunks (up kernel) among all members'
+};
+struct AdapterArgs {
+    const uint16_t* x;            // [m, k] bf16 or fp16 (f16), row stride ldx
+    const int32_t* row_slots;     // [m]: adapter slot, outside [0, slots): none
+    float* partial;               // [split, m, width] binary32 partial sums of t
+    int64_t ldx;
+    int m, k, slots, f16;
+    int split, tiles, width;      // K partitions; 16-rank tiles of all members; 16 * tiles
+    int rank_steps;               // ceil(largest max_rank / 32)
+    int vectors;                  // every member: 16-byte base and output accesses
+    int down_rows, up_rows;       // 16-row tiles per workgroup (1, 2 or 4)
+    int down_groups, up_groups;   // workgroups that share a tile's distinct adapters
+    int chunks, chunk_cols;       // column chunks of all members; columns per chunk (32 * 4 * i)
+    AdapterMember member[kMaxGemmMembers];  // unused ones: empty tile and chunk ranges
+};
+
+hipError_t launch_adapters(const AdapterArgs& a, hipStream_t s);
 hipError_t launch_accept(const AcceptArgs& a, bool fused, hipStream_t s);
 hipError_t launch_greedy(const GreedyArgs& a, hipStream_t s);
 hipError_t launch_greedy_root(const GreedyRootArgs& a, hipStream_t s);

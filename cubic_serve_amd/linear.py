@@ -404,6 +404,26 @@ class PackedLinearOperators:
                          for l in bind_linear(self, x, w, y, params)._launches)
         return PackedOperatorBinding(outputs, launches)
 
+    def bind_adapters(self, x: Tensor, banks, row_slots: Tensor, outputs, *, bases=None) -> PackedOperatorBinding:
+        """Add each row's low-rank adapter to projection outputs (adapters.bind_adapters)."""
+        from . import adapters
+
+        return adapters.bind_adapters(x, banks, row_slots, outputs, bases=bases)
+
+    def bind_adapted_linear(self, x: Tensor, weights: Sequence[QuantizedMatrix] | QuantizedMatrix,
+                            outputs: Sequence[Tensor] | Tensor, banks, row_slots: Tensor,
+                            params: CubicLinearParameters | None = None) -> PackedOperatorBinding:
+        """Bind the shared projection (or a group on one x) and the adapters of
+        its rows, one bank per matrix: bind_linear / bind_linear_group, then
+        bind_adapters in place."""
+        if isinstance(weights, QuantizedMatrix):
+            shared = self.bind_linear(x, weights, outputs, params)
+        else:
+            shared = self.bind_linear_group(x, weights, outputs, params)
+        added = self.bind_adapters(x, banks, row_slots, outputs)
+        return PackedOperatorBinding(shared.output, (*shared._launches, *added._launches),
+                                     scratch=(*shared.scratch, *added.scratch))
+
     def embedding(self, input_ids: Tensor, weight: QuantizedMatrix, *, dtype: torch.dtype) -> Tensor:
         """Eager lookup (quantized.py:776-784)."""
         output = torch.empty((*input_ids.shape, weight.shape[1]), dtype=dtype, device=input_ids.device)

@@ -157,6 +157,40 @@ CUBIC_API int cubic_gemm_grouped(const void* x, int64_t ldx, const uint32_t* cod
                        int64_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------------------
+ * Low-rank adapters of many requests beside a shared projection (no reference
+ * counterpart): for row i with adapter slot e = row_slots[i] and every member
+ * j of up to 8 projections that share x,
+ *   y_j[i, :] = base_j[i, :] + scales_j[e] * up_j[e] . (down_j[e] . x[i, :])
+ * rounded once to dtype; everything before is held in 32 bits (the rank-wide
+ * intermediate enters the second product as two 16-bit parts whose sum is it to
+ * 17 bits or more).  A slot outside [0, slots) or of rank 0 leaves y = base.
+ *   x          dtype [m, ldx], 16-byte aligned, k % 8 == 0, ldx % 8 == 0
+ *   row_slots  int32 [m], any order
+ *   downs[j]   dtype [slots, max_ranks[j], k], 16-byte aligned
+ *   ups[j]     dtype [slots, ns[j], max_ranks[j]], 16-byte aligned; entries at or
+ *              past a slot's rank, up to the next multiple of 8, must be zero
+ *   scales[j]  f32 [slots]; ranks[j] int32 [slots], 0 = empty slot; a rank past
+ *              max_ranks[j] counts as max_ranks[j]
+ *   max_ranks[j] % 8 == 0, 8..256; bases[j] [m, ldbases[j]], ys[j] [m, ldys[j]];
+ *              ys[j] == bases[j] adds in place
+ * The pointer and extent tables are host arrays of `members` entries.  A row's
+ * result does not depend on m or on the other rows, bit for bit.  No output may
+ * overlap x, another member's output or base, or the adapters.  1 <= m < 2^24,
+ * slots < 2^20, k <= 2^20, ldx <= 2^23, ns[j] * max_ranks[j] < 2^30.
+ * Workspace: cubic_adapters_workspace_bytes(m, k, members, max_ranks) bytes, not
+ * initialised, 16-byte aligned; one per concurrently running launch.  It covers
+ * every smaller m.
+ * ------------------------------------------------------------------------- */
+CUBIC_API int64_t cubic_adapters_workspace_bytes(int64_t m, int64_t k, int members, const int* max_ranks);
+CUBIC_API int cubic_adapters(const void* x, int64_t ldx, const int32_t* row_slots, int64_t m, int64_t k,
+                             int slots, int members, const int64_t* ns, const int* max_ranks,
+                             const void* const* downs, const void* const* ups,
+                             const float* const* scales, const int32_t* const* ranks,
+                             const void* const* bases, const int64_t* ldbases, void* const* ys,
+                             const int64_t* ldys, int dtype, void* workspace, int64_t workspace_bytes,
+                             void* stream);
+
+/* ---------------------------------------------------------------------------
  * Routed experts (MoE).  Replaces the Cubic Marlin MoE bind
  * (quantization/extensions/cubic/marlin.py:84-253: bind_grouped, bind_routed)
  * with its route padding (quantization/common/marlin/repack.py:253-277,
