@@ -5,18 +5,18 @@
 //
 // for up to kMaxGemmMembers projections that share x, in two launches: the
 // down kernel writes t as binary32 partial sums over K partitions, the up
-// kernel adds the partitions in ascending order and finishes the rows.
+// kernel adds the partitions and finishes the rows.
 //
 // Rows come in any order.  A tile of consecutive rows is walked once per
 // distinct adapter in it (a ballot over the tile's slots finds the rows of
 // each), so a prompt's rows, which share an adapter, are one matrix product and
 // a decode batch whose rows all differ reads each adapter once, without a
-// grouping launch or any host knowledge of the slots.
+// grouping launch or any host knowledge of the slots.  `groups` workgroups may
+// share a tile's adapters: number j takes those at j, j + groups, ...
 //
-// Arithmetic order: K partitions of kDownK columns, a quarter per wave, the
-// quarters added as (0 + 1) + (2 + 3); then the rank in steps of 32.  Nothing
-// of it depends on m, on the tile or on the other rows, so a row's result is
-// the same bit for bit whichever batch it is in.
+// Arithmetic order: K partitions of kDownK columns, each a sum of four quarters
+// (0 + 1) + (2 + 3), partitions added in ascending order; then the rank in steps
+// of 32.  Nothing of it depends on m, on the tile or on the other rows, so a row's result is the same bit for bit whichever batch it is in.
 #include "cubic_gemm_common.h"
 
 namespace cubic {
@@ -27,9 +27,9 @@ using gemm::mfma16;
 
 constexpr int kThreads = 256;
 constexpr int kWaves = 4;
-constexpr int kDownK = kAdapterDownK;       // columns of x per workgroup
-constexpr int kWaveK = kDownK / kWaves;     // ... per wave
-constexpr int kSteps = kWaveK / 32;         // MFMA steps per wave
+constexpr int kDownK = kAdapterDownK;       // columns of x per K partition
+constexpr int kQuarter = kDownK / 4;
+constexpr int kSteps = kQuarter / 32;       // MFMA steps of a quarter
 constexpr uint32_t kOutside = 0x80000000u;  // added to a byte offset: past every buffer, reads 0
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void* base, int64_t bytes) {
@@ -44,60 +44,80 @@ __device__ __forceinline__ uint4 load16(__amdgpu_buffer_rsrc_t r, uint32_t byte_
 // adapter), the same in every wave: one wave reads them, so that waves cannot
 // disagree on the walk (and its barriers) if the caller rewrites them meanwhile.
 constexpr int kNone = -2;
-template <int ROWS>
-__device__ __forceinline__ int tile_slots(const AdapterArgs& a, int row0, int* lds) {
-    if (threadIdx.x < 64) {
-        int slot = -1;
-        if ((int)threadIdx.x < ROWS && row0 + (int)threadIdx.x < a.m) {
-            slot = a.row_slots[row0 + threadIdx.x];
-            if (slot < 0 || slot >= a.slots) slot = kNone;
-        }
-        lds[threadIdx.x] = slot;
-    }
+__device__ __forceinline__ int row_slot(const AdapterArgs& a, int row0, int rows, int lane) {
+    if (lane >= rows || row0 + lane >= a.m) return -1;
+    const int slot = a.row_slots[row0 + lane];
+    return slot < 0 || slot >= a.slots ? kNone : slot;
+}
+__device__ __forceinline__ int tile_slots(const AdapterArgs& a, int row0, int rows, int* lds) {
+    if (threadIdx.x < 64) lds[threadIdx.x] = row_slot(a, row0, rows, threadIdx.x);
     __syncthreads();
     return lds[threadIdx.x & 63];
 }
 
+// One quarter of t for 16 * MT rows x RT 16-rank tiles, every load in flight at
+// once.  MFMA operands straight from memory: the first is A (its rows are the
+// ranks), the second x, so a lane ends with four consecutive ranks of one row.
+// x goes out ahead of A in runs of four steps (256 bytes of every row).
+template <bool F16, int MT, int RT>
+__device__ __forceinline__ void quarter_product(__amdgpu_buffer_rsrc_t x, const uint32_t (&xoff)[MT],
+                                                __amdgpu_buffer_rsrc_t d, const uint32_t (&doff)[RT], int k0,
+                                                int k, floatx4_t (&acc)[MT][RT]) {
+    uint4 xf[kSteps][MT], df[kSteps][RT];
+#pragma unroll
+    for (int h = 0; h < kSteps; h += 4) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int s = h; s < h + 4; ++s) {
+                const int kk = k0 + s * 32;
+                xf[s][i] = load16(x, kk < k ? xoff[i] + (uint32_t)kk * 2 : kOutside);
+            }
+#pragma unroll
+        for (int t = 0; t < RT; ++t)
+#pragma unroll
+            for (int s = h; s < h + 4; ++s) {
+                const int kk = k0 + s * 32;
+                df[s][t] = load16(d, kk < k && doff[t] != kOutside ? doff[t] + (uint32_t)kk * 2 : kOutside);
+            }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int t = 0; t < RT; ++t) acc[i][t] = floatx4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int t = 0; t < RT; ++t) acc[i][t] = mfma16<F16>(df[s][t], xf[s][i], acc[i][t]);
+}
+
 // ---------------------------------------------------------------------------
-// t = A x.  Workgroup: 16 * MT rows x RT 16-rank tiles x kDownK columns.  MFMA
-// operands straight from memory: the first is A (its rows are the ranks), the
-// second x, so a lane ends with four consecutive ranks of one row.
+// t = A x into the partial sums.  Workgroup: 16 * MT rows x RT rank tiles x one K
+// partition, a quarter per wave.
 // ---------------------------------------------------------------------------
-template <bool F16, int MT, int RT, int S>
+template <bool F16, int MT, int RT>
 __global__ __launch_bounds__(kThreads) void adapter_down_kernel(AdapterArgs a) {
     constexpr int kRows = 16 * MT;
     __shared__ int slots_lds[64];
     __shared__ floatx4_t red[2][MT * RT][64];
+    const AdapterMember& mb = a.member[blockIdx.z];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, q = lane >> 4;
-    const int tile = blockIdx.x / a.down_groups, group = blockIdx.x % a.down_groups;
-    const int row0 = tile * kRows;
-    const int slot = tile_slots<kRows>(a, row0, slots_lds);
+    // K partitions first: workgroups that run together spread over all of a
+    // row (tiles first, they meet on the few memory channels of one column
+    // range: 4096 x 8192 at rank 128, 76 -> 57 us)
+    const int part = blockIdx.x % a.split, item = blockIdx.x / a.split;
+    const int tile = item / a.down_groups, group = item % a.down_groups;
+    const int row0 = tile * kRows, rank0 = blockIdx.y * RT * 16;
+    if (rank0 >= mb.max_rank) return;
+    const int slot = tile_slots(a, row0, kRows, slots_lds);
 
     const int rows = min(kRows, a.m - row0);
     const auto x = buffer(a.x + (int64_t)row0 * a.ldx, ((int64_t)(rows - 1) * a.ldx + a.k) * 2);
-    const int k0 = blockIdx.y * kDownK + wave * kWaveK + q * 8;
-    // the rank tiles of this workgroup: member and first rank of each
-    const uint16_t* down[RT];
-    const int32_t* ranks[RT];
-    int max_rank[RT], first[RT];
-#pragma unroll
-    for (int t = 0; t < RT; ++t) {
-        const int v = blockIdx.z * RT + t;
-        down[t] = a.member[0].down;
-        ranks[t] = a.member[0].ranks;
-        max_rank[t] = 0;
-        first[t] = 0;
-#pragma unroll
-        for (int j = 0; j < kMaxGemmMembers; ++j)
-            if (v >= a.member[j].tile0 && v < a.member[j].tile1) {
-                down[t] = a.member[j].down;
-                ranks[t] = a.member[j].ranks;
-                max_rank[t] = a.member[j].max_rank;
-                first[t] = (v - a.member[j].tile0) * 16;
-            }
-    }
-
+    const int k0 = part * kDownK + wave * kQuarter + q * 8;
     uint64_t left = __ballot(slot >= 0);
     for (int order = 0; left; ++order) {
         const int lead = __builtin_ctzll(left);
@@ -105,45 +125,23 @@ __global__ __launch_bounds__(kThreads) void adapter_down_kernel(AdapterArgs a) {
         const uint64_t mine = __ballot(slot == e);
         left &= ~mine;
         if (order % a.down_groups != group) continue;
+        // rows of other adapters repeat the first row: their columns of the
+        // product are not stored
         uint32_t xoff[MT], doff[RT];
-        __amdgpu_buffer_rsrc_t d[RT];
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            // rows of other adapters repeat the first row: their columns of
-            // the product are not stored
-            const int r = (mine >> (16 * i + col)) & 1 ? 16 * i + col : lead;
-            xoff[i] = (uint32_t)r * (uint32_t)(a.ldx * 2);
-        }
-#pragma unroll
-        for (int t = 0; t < RT; ++t) {
-            const int rank = max_rank[t] ? min(ranks[t][e], max_rank[t]) : 0;
-            d[t] = buffer(down[t] + (int64_t)e * max_rank[t] * a.k, (int64_t)max_rank[t] * a.k * 2);
-            doff[t] = first[t] + col < rank ? (uint32_t)(first[t] + col) * (uint32_t)(a.k * 2) : kOutside;
-        }
-        uint4 xf[S][MT], df[S][RT];
-        auto issue = [&](int s) {
-            const int kk = k0 + s * 32;
-            const uint32_t ko = kk < a.k ? (uint32_t)kk * 2 : kOutside;
-#pragma unroll
-            for (int t = 0; t < RT; ++t) df[s % S][t] = load16(d[t], doff[t] == kOutside ? kOutside : doff[t] + ko);
-#pragma unroll
-            for (int i = 0; i < MT; ++i) xf[s % S][i] = load16(x, xoff[i] + ko);
-        };
-        floatx4_t acc[MT][RT];
 #pragma unroll
         for (int i = 0; i < MT; ++i)
+            xoff[i] = (uint32_t)((mine >> (16 * i + col)) & 1 ? 16 * i + col : lead) * (uint32_t)(a.ldx * 2);
+        // the first tile does not wait for the slot's rank (what lies past it
+        // the up kernel leaves out); the others are read only below it
+        const int rank = RT > 1 || rank0 ? min(mb.ranks[e], mb.max_rank) : mb.max_rank;
 #pragma unroll
-            for (int t = 0; t < RT; ++t) acc[i][t] = floatx4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int s = 0; s < S; ++s) issue(s);
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-#pragma unroll
-            for (int i = 0; i < MT; ++i)
-#pragma unroll
-                for (int t = 0; t < RT; ++t) acc[i][t] = mfma16<F16>(df[s % S][t], xf[s % S][i], acc[i][t]);
-            if (s + S < kSteps) issue(s + S);
+        for (int t = 0; t < RT; ++t) {
+            const int r = rank0 + 16 * t + col;
+            doff[t] = r < (rank0 + t == 0 ? mb.max_rank : rank) ? (uint32_t)r * (uint32_t)(a.k * 2) : kOutside;
         }
+        const auto d = buffer(mb.down + (int64_t)e * mb.max_rank * a.k, (int64_t)mb.max_rank * a.k * 2);
+        floatx4_t acc[MT][RT];
+        quarter_product<F16, MT, RT>(x, xoff, d, doff, k0, a.k, acc);
         // (0 + 1) + (2 + 3); the walk's next turn writes red only after the
         // last barrier, which follows every read of it
         if (wave & 1)
@@ -168,11 +166,11 @@ __global__ __launch_bounds__(kThreads) void adapter_down_kernel(AdapterArgs a) {
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
                 if (!((mine >> (16 * i + col)) & 1)) continue;
-                float* out = a.partial + ((int64_t)blockIdx.y * a.m + row0 + 16 * i + col) * a.width +
-                             blockIdx.z * RT * 16 + 4 * q;
+                float* out = a.partial + ((int64_t)part * a.m + row0 + 16 * i + col) * a.width + mb.rank0 +
+                             rank0 + 4 * q;
 #pragma unroll
                 for (int t = 0; t < RT; ++t)
-                    if (blockIdx.z * RT + t < a.tiles)
+                    if (rank0 + 16 * t < mb.max_rank)
                         *(floatx4_t*)(out + 16 * t) = acc[i][t] + red[0][i * RT + t][lane];
             }
         __syncthreads();
@@ -180,11 +178,16 @@ __global__ __launch_bounds__(kThreads) void adapter_down_kernel(AdapterArgs a) {
 }
 
 // ---------------------------------------------------------------------------
-// y = base + s B t.  Workgroup: 16 * MT rows x a chunk of one member's columns,
-// 32 columns per wave and turn.  The first MFMA operand is B with its rows
-// (columns of y) permuted so that a lane ends with eight consecutive columns of
-// one row: two 16-row tiles, row 4 q + s of tile u standing for column 8 q + 4 u
-// + s.  t is split into two 16-bit parts, t = hi + lo with an error below 2^-17
+// y = base + s B t.  A wave takes 16 rows x kTurn columns per turn; the four
+// waves of a workgroup stand side by side over columns (WR = 1: few rows) or
+// one below the other (WR = 4: they read the same B, which their CU's cache
+// holds).  The first MFMA operand is B, so a lane ends with four consecutive
+// columns of one row; the product passes through LDS (the wave's own, no
+// barrier) so that base and y move as whole 256-byte pieces of rows: a copy in
+// that pattern runs at 4.6 - 4.8 TB/s where 64-byte pieces of 16 rows, which
+// the product's own layout gives, run at 3.1 - 3.7 (2048 x 24576 and 4096 x 8192).
+//
+// t is split into two 16-bit parts, t = hi + lo with an error below 2^-17
 // (bf16) or 2^-22 of the row's largest (fp16) of t, so that the only rounding
 // to 16 bits that counts is y's; the operator is bound by y's bytes, and the
 // second product costs matrix time that is idle.  fp16 parts are taken of t
@@ -213,24 +216,99 @@ __device__ __forceinline__ void split_parts(const float* t, uint4& hi, uint4& lo
     lo = uint4{l[0], l[1], l[2], l[3]};
 }
 
-template <bool F16, int MT, int KS, bool VEC>
+// The parts of a row of t (this lane's eight ranks of every step; lanes of one
+// column hold the row): scaled, cut at the rank; returns what the product has
+// to be multiplied by.
+template <bool F16, int KS>
+__device__ __forceinline__ float split_row(const floatx4_t (&v)[KS][2], int rank, float scale, int q,
+                                           uint4 (&hi)[KS], uint4 (&lo)[KS]) {
+    float t[KS][8];
+    float top = 0.f, back = 1.f;
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            t[s][c] = s * 32 + q * 8 + c < rank ? v[s][c >> 2][c & 3] * scale : 0.f;
+            top = fmaxf(top, fabsf(t[s][c]));
+        }
+    if constexpr (F16) {
+        top = fmaxf(top, __uint_as_float(xor16_u32(__float_as_uint(top))));
+        top = fmaxf(top, __uint_as_float(xor32_u32(__float_as_uint(top))));
+        // 2^-(exponent + 1) of the row's largest, kept within normal numbers
+        int ex = (int)(__float_as_uint(top) >> 23) - 126;
+        ex = top == 0.f || !__builtin_isfinite(top) ? 0 : min(max(ex, -120), 120);
+        const float down = __uint_as_float((uint32_t)(127 - ex) << 23);
+        back = __uint_as_float((uint32_t)(127 + ex) << 23);
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+            for (int c = 0; c < 8; ++c) t[s][c] *= down;
+    }
+#pragma unroll
+    for (int s = 0; s < KS; ++s) split_parts<F16>(t[s], hi[s], lo[s]);
+    return back;
+}
+
+// Eight 16-bit values of a row at column c: one access, or (rows that are not
+// 16-byte aligned) eight, those past column n left out.
+template <bool VEC>
+__device__ __forceinline__ uint4 load8(__amdgpu_buffer_rsrc_t r, uint32_t row, int c, int n) {
+    if constexpr (VEC) {
+        return load16(r, row + 2 * c);
+    } else {
+        uint32_t v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            v[i] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(r, (int)(c + i < n ? row + 2 * (c + i) : kOutside), 0, 0);
+        return uint4{v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16};
+    }
+}
+
+template <bool VEC>
+__device__ __forceinline__ void store8(__amdgpu_buffer_rsrc_t r, uint32_t row, int c, int n, uint4 v) {
+    if constexpr (VEC) {
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_dev_t, v), r, (int)(row + 2 * c), 0, 0);
+    } else {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            __builtin_amdgcn_raw_buffer_store_b16((short)(w[i / 2] >> (16 * (i & 1))), r,
+                                                  (int)(c + i < n ? row + 2 * (c + i) : kOutside), 0, 0);
+    }
+}
+
+// Two 16-bit values plus two binary32 ones, each sum rounded once.
+template <bool F16>
+__device__ __forceinline__ uint32_t add_pair(uint32_t in, float lo, float hi) {
+    if constexpr (F16) return gemm::pack_level2<true>(half_bits_to_float(in & 0xffffu) + lo, half_bits_to_float(in >> 16) + hi);
+    else return gemm::pack_level2<false>(bf16_bits_to_float(in & 0xffffu) + lo, __uint_as_float(in & 0xffff0000u) + hi);
+}
+
+template <bool F16, int KS, int WR, bool VEC>
 __global__ __launch_bounds__(kThreads) void adapter_up_kernel(AdapterArgs a) {
-    constexpr int kRows = 16 * MT, kPitch = KS * 32 + 4;
-    __shared__ int slots_lds[64];
-    __shared__ __attribute__((aligned(16))) float tl[kRows][kPitch];
+    constexpr int kColWaves = kWaves / WR;  // waves side by side
+    constexpr int kTurn = kAdapterUpTurn, kPitch = kTurn + 4;
+    __shared__ __attribute__((aligned(16))) float product[kWaves][16][kPitch];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, q = lane >> 4;
-    const int tile = blockIdx.x / a.up_groups, group = blockIdx.x % a.up_groups;
-    const int row0 = tile * kRows;
-    const int slot = tile_slots<kRows>(a, row0, slots_lds);
-
-    // member of this column chunk
-    AdapterMember mb = a.member[0];
+    const int chunk = blockIdx.x % a.chunks, item = blockIdx.x / a.chunks;
+    const int tile = item / a.up_groups, group = item % a.up_groups;
+    const int row0 = (tile * WR + wave / kColWaves) * 16;
+    // every wave walks its own rows
+    const int slot = row_slot(a, row0, 16, lane);
+    // the member of this column chunk (a grid of members x the widest one's
+    // chunks leaves workgroups that only end: m = 64, q k v: 7.4 -> 13 us)
+    int j = 0;
 #pragma unroll
-    for (int j = 1; j < kMaxGemmMembers; ++j)
-        if ((int)blockIdx.y >= a.member[j].chunk0 && (int)blockIdx.y < a.member[j].chunk1) mb = a.member[j];
-    const int c_begin = ((int)blockIdx.y - mb.chunk0) * a.chunk_cols;
-    const int c_end = min(mb.n, c_begin + a.chunk_cols);
+    for (int i = 0; i < kMaxGemmMembers; ++i) j += chunk >= a.chunk_end[i];
+    const AdapterMember& mb = a.member[j];
+    const int n = mb.n, max_rank = mb.max_rank;
+    const int c_begin = (chunk - mb.chunk0) * a.chunk_cols + wave % kColWaves * kTurn;
+    const int c_end = min(n, (chunk - mb.chunk0 + 1) * a.chunk_cols);
+    const uint32_t ldbase = (uint32_t)mb.ldbase * 2, ldy = (uint32_t)mb.ldy * 2;  // bytes
+    const auto base = buffer(mb.base + (int64_t)row0 * mb.ldbase, 15 * (int64_t)ldbase + 2 * n);
+    const auto y = buffer(mb.y + (int64_t)row0 * mb.ldy, 15 * (int64_t)ldy + 2 * n);
+    const bool in_place = mb.base == mb.y;
 
     uint64_t left = __ballot(slot != -1);
     for (int order = 0; left; ++order) {
@@ -239,145 +317,141 @@ __global__ __launch_bounds__(kThreads) void adapter_up_kernel(AdapterArgs a) {
         const uint64_t mine = __ballot(slot == e);
         left &= ~mine;
         if (order % a.up_groups != group) continue;
-        const int rank = e >= 0 ? min(mb.ranks[e], mb.max_rank) : 0;
+        const int rank = e >= 0 ? min(mb.ranks[e], max_rank) : 0;
+        if (rank <= 0 && in_place) continue;
         const float scale = e >= 0 ? mb.scales[e] : 0.f;
-        __syncthreads();  // the last turn's reads of tl
-        for (int i = threadIdx.x; i < kRows * KS * 8; i += kThreads) {
-            const int r = i / (KS * 8), f = (i % (KS * 8)) * 4;
-            floatx4_t v = {0.f, 0.f, 0.f, 0.f};
-            if (f < rank && ((mine >> r) & 1)) {
-                const float* p = a.partial + (int64_t)(row0 + r) * a.width + mb.tile0 * 16 + f;
-                for (int s = 0; s < a.split; ++s) v += *(const floatx4_t*)(p + (int64_t)s * a.m * a.width);
-#pragma unroll
-                for (int c = 0; c < 4; ++c) v[c] = f + c < rank ? v[c] * scale : 0.f;
-            }
-            *(floatx4_t*)&tl[r][f] = v;
-        }
-        __syncthreads();
-        uint4 hi[MT][KS], lo[MT][KS];
-        float back[MT];
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            float t[KS][8];
-            float top = 0.f;
+        uint4 hi[KS], lo[KS];
+        float back = 1.f;
+        {
+            // the partitions in ascending order, kParts requested together;
+            // what is not there (another row, past the rank) reads as 0
+            constexpr int kParts = KS < 8 ? 8 / KS : 1;
+            const bool own = (mine >> col) & 1;
+            uint32_t off[KS][2];
+            floatx4_t v[KS][2];
 #pragma unroll
             for (int s = 0; s < KS; ++s)
 #pragma unroll
-                for (int c = 0; c < 8; c += 4) {
-                    const floatx4_t v = *(const floatx4_t*)&tl[16 * i + col][s * 32 + q * 8 + c];
-#pragma unroll
-                    for (int d = 0; d < 4; ++d) {
-                        t[s][c + d] = v[d];
-                        top = fmaxf(top, fabsf(v[d]));
-                    }
+                for (int c = 0; c < 2; ++c) {
+                    const int f = s * 32 + q * 8 + 4 * c;
+                    off[s][c] = own && f < rank ? (uint32_t)(col * a.width + mb.rank0 + f) * 4 : kOutside;
+                    v[s][c] = floatx4_t{0.f, 0.f, 0.f, 0.f};
                 }
-            back[i] = 1.f;
-            if constexpr (F16) {
-                top = fmaxf(top, __uint_as_float(xor16_u32(__float_as_uint(top))));
-                top = fmaxf(top, __uint_as_float(xor32_u32(__float_as_uint(top))));
-                // 2^-(exponent + 1) of the row's largest, kept within normal numbers
-                int ex = (int)(__float_as_uint(top) >> 23) - 126;
-                ex = top == 0.f || !__builtin_isfinite(top) ? 0 : min(max(ex, -120), 120);
-                const float down = __uint_as_float((uint32_t)(127 - ex) << 23);
-                back[i] = __uint_as_float((uint32_t)(127 + ex) << 23);
+            for (int part = 0; part < a.split; part += kParts) {
+                floatx4_t in[kParts][KS][2];
 #pragma unroll
-                for (int s = 0; s < KS; ++s)
+                for (int p = 0; p < kParts; ++p) {
+                    const int64_t at = ((int64_t)min(part + p, a.split - 1) * a.m + row0) * a.width;
+                    const auto buf = buffer(a.partial + at, part + p < a.split ? 16 * a.width * 4 : 0);
 #pragma unroll
-                    for (int c = 0; c < 8; ++c) t[s][c] *= down;
+                    for (int s = 0; s < KS; ++s)
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) in[p][s][c] = __builtin_bit_cast(floatx4_t, load16(buf, off[s][c]));
+                }
+#pragma unroll
+                for (int p = 0; p < kParts; ++p)
+#pragma unroll
+                    for (int s = 0; s < KS; ++s)
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) v[s][c] += in[p][s][c];
             }
-#pragma unroll
-            for (int s = 0; s < KS; ++s) split_parts<F16>(t[s], hi[i][s], lo[i][s]);
+            back = split_row<F16, KS>(v, rank, scale, q, hi, lo);
         }
-        const auto up = buffer(mb.up + (e >= 0 ? (int64_t)e * mb.n * mb.max_rank : 0), (int64_t)mb.n * mb.max_rank * 2);
-        for (int c0 = c_begin + wave * 32; c0 < c_end; c0 += kWaves * 32) {
-            floatx4_t acc[MT][2];
+        const auto up = buffer(mb.up + (e >= 0 ? (int64_t)e * n * max_rank : 0), (int64_t)n * max_rank * 2);
+        for (int c0 = c_begin; c0 < c_end; c0 += kColWaves * kTurn) {
+            // base and y: rows q, q + 4, ..., eight columns per lane; what is
+            // not this turn's reads 0 and is not written
+            const int cy = c0 + 8 * col;
+            uint4 in[4];
+            uint32_t at[4];  // row offsets are the caller's strides times this lane's rows
 #pragma unroll
-            for (int i = 0; i < MT; ++i) acc[i][0] = acc[i][1] = floatx4_t{0.f, 0.f, 0.f, 0.f};
+            for (int i = 0; i < 4; ++i) {
+                const bool own = ((mine >> (4 * i + q)) & 1) && cy < n;
+                at[i] = own ? (uint32_t)(4 * i + q) : kOutside;
+                in[i] = load8<VEC>(base, own ? (4 * i + q) * ldbase : kOutside, cy, n);
+            }
             if (rank > 0) {
+                constexpr int kTiles = kTurn / 16, kHalf = kTiles / 2;
+                auto fetch = [&](int h, int s, uint4 (&b)[kHalf]) {
 #pragma unroll
-                for (int s = 0; s < KS; ++s)
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const int c = c0 + 8 * (col >> 2) + 4 * u + (col & 3), r = s * 32 + q * 8;
-                        const uint4 b = load16(up, r < rank && c < mb.n ? (uint32_t)(c * mb.max_rank + r) * 2 : kOutside);
-#pragma unroll
-                        for (int i = 0; i < MT; ++i) {
-                            acc[i][u] = mfma16<F16>(b, lo[i][s], acc[i][u]);
-                            acc[i][u] = mfma16<F16>(b, hi[i][s], acc[i][u]);
-                        }
+                    for (int u = 0; u < kHalf; ++u) {
+                        const int c = c0 + 16 * (h * kHalf + u) + col, r = s * 32 + q * 8;
+                        b[u] = load16(up, r < rank && c < n ? (uint32_t)(c * max_rank + r) * 2 : kOutside);
                     }
+                };
+                uint4 b[2][kHalf];
+                fetch(0, 0, b[0]);
+                floatx4_t acc[kHalf];
+#pragma unroll
+                for (int v = 0; v < 2 * KS; ++v) {  // half v / KS, rank step v % KS
+                    const int s = v % KS;
+                    if (v + 1 < 2 * KS) fetch((v + 1) / KS, (v + 1) % KS, b[(v + 1) & 1]);
+                    __builtin_amdgcn_sched_barrier(0);  // the next loads go out before these are waited for
+#pragma unroll
+                    for (int u = 0; u < kHalf; ++u) {
+                        if (s == 0) acc[u] = floatx4_t{0.f, 0.f, 0.f, 0.f};
+                        acc[u] = mfma16<F16>(b[v & 1][u], lo[s], acc[u]);
+                        acc[u] = mfma16<F16>(b[v & 1][u], hi[s], acc[u]);
+                        if (s == KS - 1)
+                            *(floatx4_t*)&product[wave][col][16 * (v / KS * kHalf + u) + 4 * q] = acc[u] * back;
+                    }
+                }
+                __builtin_amdgcn_wave_barrier();
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const floatx4_t d0 = *(const floatx4_t*)&product[wave][4 * i + q][8 * col];
+                    const floatx4_t d1 = *(const floatx4_t*)&product[wave][4 * i + q][8 * col + 4];
+                    in[i].x = add_pair<F16>(in[i].x, d0[0], d0[1]);
+                    in[i].y = add_pair<F16>(in[i].y, d0[2], d0[3]);
+                    in[i].z = add_pair<F16>(in[i].z, d1[0], d1[1]);
+                    in[i].w = add_pair<F16>(in[i].w, d1[2], d1[3]);
+                }
+                __builtin_amdgcn_wave_barrier();
             }
-            const int cy = c0 + 8 * q;
 #pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                if (!((mine >> (16 * i + col)) & 1) || cy >= mb.n) continue;
-                const int64_t row = row0 + 16 * i + col;
-                const uint16_t* base = mb.base + row * mb.ldbase + cy;
-                uint16_t* y = mb.y + row * mb.ldy + cy;
-                uint16_t in[8], out[8];
-                if constexpr (VEC) {
-                    *(uint4*)in = *(const uint4*)base;
-                } else {
-#pragma unroll
-                    for (int c = 0; c < 8; ++c) in[c] = cy + c < mb.n ? base[c] : 0;
-                }
-#pragma unroll
-                for (int c = 0; c < 8; ++c) {
-                    const float b = F16 ? half_bits_to_float(in[c]) : bf16_bits_to_float(in[c]);
-                    const float d = acc[i][c >> 2][c & 3] * back[i];
-                    out[c] = rank > 0 ? gemm::out_bits<F16>(b + d) : in[c];
-                }
-                if constexpr (VEC) {
-                    *(uint4*)y = *(const uint4*)out;
-                } else {
-#pragma unroll
-                    for (int c = 0; c < 8; ++c)
-                        if (cy + c < mb.n) y[c] = out[c];
-                }
-            }
+            for (int i = 0; i < 4; ++i) store8<VEC>(y, at[i] == kOutside ? kOutside : at[i] * ldy, cy, n, in[i]);
         }
     }
 }
 
-template <bool F16, int MT, int RT, int S>
+template <bool F16, int MT, int RT>
 void start_down(const AdapterArgs& a, hipStream_t s) {
-    const dim3 grid((a.m + 16 * MT - 1) / (16 * MT) * a.down_groups, a.split, (a.tiles + RT - 1) / RT);
-    adapter_down_kernel<F16, MT, RT, S><<<grid, kThreads, 0, s>>>(a);
+    const dim3 grid((a.m + 16 * MT - 1) / (16 * MT) * a.down_groups * a.split,
+                    (a.rank_tiles + RT - 1) / RT, a.members);
+    adapter_down_kernel<F16, MT, RT><<<grid, kThreads, 0, s>>>(a);
 }
 
 template <bool F16, int MT>
 void start_down_tiles(const AdapterArgs& a, hipStream_t s) {
-    if (a.tiles == 1) start_down<F16, MT, 1, 8>(a, s);
-    else if (a.tiles == 2) start_down<F16, MT, 2, MT == 4 ? 4 : 8>(a, s);
-    else if (a.tiles <= 4) start_down<F16, MT, 4, 4>(a, s);
-    else start_down<F16, MT, 8, MT == 4 ? 2 : 4>(a, s);
+    if (a.rank_tiles == 1) start_down<F16, MT, 1>(a, s);
+    else if (a.rank_tiles == 2) start_down<F16, MT, 2>(a, s);
+    else start_down<F16, MT, 4>(a, s);
 }
 
-template <bool F16, int MT, int KS>
+template <bool F16, int KS, int WR>
 void start_up(const AdapterArgs& a, hipStream_t s) {
-    const dim3 grid((a.m + 16 * MT - 1) / (16 * MT) * a.up_groups, a.chunks);
-    if (a.vectors) adapter_up_kernel<F16, MT, KS, true><<<grid, kThreads, 0, s>>>(a);
-    else adapter_up_kernel<F16, MT, KS, false><<<grid, kThreads, 0, s>>>(a);
+    const dim3 grid((a.m + 16 * WR - 1) / (16 * WR) * a.up_groups * a.chunks);
+    if (a.vectors) adapter_up_kernel<F16, KS, WR, true><<<grid, kThreads, 0, s>>>(a);
+    else adapter_up_kernel<F16, KS, WR, false><<<grid, kThreads, 0, s>>>(a);
 }
 
-template <bool F16, int MT>
-void start_up_steps(const AdapterArgs& a, hipStream_t s) {
-    if (a.rank_steps == 1) start_up<F16, MT, 1>(a, s);
-    else if (a.rank_steps == 2) start_up<F16, MT, 2>(a, s);
-    else if (a.rank_steps <= 4) start_up<F16, MT, 4>(a, s);
-    else if constexpr (MT < 4) start_up<F16, MT, 8>(a, s);
+template <bool F16, int KS>
+void start_up_rows(const AdapterArgs& a, hipStream_t s) {
+    if (a.up_rows == 1) start_up<F16, KS, 1>(a, s);
+    else start_up<F16, KS, 4>(a, s);
 }
 
 template <bool F16>
 hipError_t start(const AdapterArgs& a, hipStream_t s) {
     if (a.down_rows == 1) start_down_tiles<F16, 1>(a, s);
-    else if (a.down_rows == 2) start_down_tiles<F16, 2>(a, s);
-    else start_down_tiles<F16, 4>(a, s);
+    else start_down_tiles<F16, 2>(a, s);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    if (a.up_rows == 1) start_up_steps<F16, 1>(a, s);
-    else if (a.up_rows == 2) start_up_steps<F16, 2>(a, s);
-    else start_up_steps<F16, 4>(a, s);
+    const int steps = (a.rank_tiles + 1) / 2;
+    if (steps == 1) start_up_rows<F16, 1>(a, s);
+    else if (steps == 2) start_up_rows<F16, 2>(a, s);
+    else if (steps <= 4) start_up_rows<F16, 4>(a, s);
+    else start_up_rows<F16, 8>(a, s);
     return hipGetLastError();
 }
 

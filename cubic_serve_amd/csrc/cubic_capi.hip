@@ -750,41 +750,42 @@ int cubic_adapters(const void* x, int64_t ldx, const int32_t* row_slots, int64_t
                         max_ranks[j], cubic::kMaxAdapterRank);
         if (ns[j] <= 0 || ns[j] * max_ranks[j] >= (1 << 30) || ns[j] >= (1 << 30))
             return fail(CUBIC_EINVAL, "adapter width %lld of member %d", (long long)ns[j], j);
-        if (ldbases[j] < ns[j] || ldys[j] < ns[j])
-            return fail(CUBIC_EINVAL, "output leading dimension too small");
+        if (ldbases[j] < ns[j] || ldys[j] < ns[j] || ldbases[j] > (1 << 25) || ldys[j] > (1 << 25))
+            return fail(CUBIC_EINVAL, "output leading dimension outside n..2^25");
         if (!aligned16(downs[j]) || !aligned16(ups[j]))
             return fail(CUBIC_ENOTSUP, "adapters need 16-byte alignment");
         cubic::AdapterMember& b = a.member[j];
         b = {(const uint16_t*)downs[j], (const uint16_t*)ups[j], scales[j], ranks[j],
              (const uint16_t*)bases[j], (uint16_t*)ys[j], ldbases[j], ldys[j], (int)ns[j], max_ranks[j],
-             a.tiles, a.tiles + (int)ceil_div(max_ranks[j], 16), 0, 0};
-        a.tiles = b.tile1;
+             a.width, 0};
+        a.width += (int)ceil_div(max_ranks[j], 16) * 16;
         a.vectors &= ns[j] % 8 == 0 && ldbases[j] % 8 == 0 && ldys[j] % 8 == 0 && aligned16(bases[j]) &&
                      aligned16(ys[j]);
         columns += ns[j];
         largest = std::max(largest, max_ranks[j]);
     }
-    a.width = 16 * a.tiles;
-    a.rank_steps = (int)ceil_div(largest, 32);
+    a.members = members;
+    a.rank_tiles = (int)ceil_div(largest, 16);
     const int64_t need = (int64_t)a.split * m * a.width * (int64_t)sizeof(float);
     if (workspace_bytes < need)
         return fail(CUBIC_EWORKSPACE, "adapter workspace %lld < %lld bytes", (long long)workspace_bytes, (long long)need);
     if (!workspace || !aligned16(workspace)) return fail(CUBIC_EINVAL, "adapter workspace must be 16-byte aligned");
     a.partial = (float*)workspace;
-    a.down_rows = m <= 128 ? 1 : m <= 1024 ? 2 : 4;
-    a.up_rows = a.rank_steps > 4 ? std::min(a.down_rows, 2) : a.down_rows;
-    auto groups = [&](int rows) { return rows == 1 ? (int)std::min<int64_t>(16, m) : rows == 2 ? 4 : 1; };
-    a.down_groups = groups(a.down_rows);
-    a.up_groups = groups(a.up_rows);
-    const int64_t rows = ceil_div(m, 16 * a.up_rows) * a.up_groups;
-    a.chunk_cols = 128;
-    while (a.chunk_cols < 2048 && rows * ceil_div(columns, 2 * a.chunk_cols) >= 1024) a.chunk_cols *= 2;
-    for (int j = 0; j < members; ++j) {
-        a.member[j].chunk0 = a.chunks;
-        a.chunks += (int)ceil_div(ns[j], a.chunk_cols);
-        a.member[j].chunk1 = a.chunks;
+    a.down_rows = m <= 1024 ? 1 : 2;
+    a.up_rows = m <= 128 ? 1 : 4;
+    a.down_groups = m <= 128 ? (int)std::min<int64_t>(16, m) : m <= 1024 ? 4 : 1;
+    a.up_groups = m <= 128 ? (int)std::min<int64_t>(16, m) : m <= 1024 ? 4 : 1;
+    const int64_t items = ceil_div(m, 16 * a.up_rows) * a.up_groups;
+    a.chunk_cols = 4 * cubic::kAdapterUpTurn;
+    while (a.chunk_cols > cubic::kAdapterUpTurn && items * ceil_div(columns, a.chunk_cols) < 512) a.chunk_cols /= 2;
+    int64_t chunks = 0;
+    for (int j = 0; j < cubic::kMaxGemmMembers; ++j) {
+        a.member[j].chunk0 = (int)chunks;
+        if (j < members) chunks += ceil_div(ns[j], a.chunk_cols);
+        a.chunk_end[j] = (int)chunks;
     }
-    if (a.chunks > 65535) return fail(CUBIC_ENOTSUP, "adapter widths too large");
+    a.chunks = (int)chunks;
+    if (items * chunks >= INT_MAX) return fail(CUBIC_ENOTSUP, "adapter extents too large");
     return hip_status(cubic::launch_adapters(a, (hipStream_t)stream), "cubic_adapters launch");
 }
 

@@ -252,6 +252,7 @@ struct GuardArgs {
 
 // Low-rank adapters beside a shared projection (cubic_adapters.hip)
 constexpr int kAdapterDownK = 1024;  // columns of x per K partition
+constexpr int kAdapterUpTurn = 128;  // columns of y per wave and turn
 constexpr int kMaxAdapterRank = 256;
 struct AdapterMember {
     const uint16_t* down;         // [slots, max_rank, k]
@@ -262,22 +263,23 @@ struct AdapterMember {
     uint16_t* y;                  // [m, ldy]
     int64_t ldbase, ldy;
     int n, max_rank;              // max_rank % 8 == 0
-    int tile0, tile1;             // its 16-rank tiles among all members'
-    int chunk0, chunk1;           // its column chunks (up kernel) among all members'
+    int rank0;                    // its first column of the partial sums
+    int chunk0;                   // its first column chunk
 };
 struct AdapterArgs {
     const uint16_t* x;            // [m, k] bf16 or fp16 (f16), row stride ldx
     const int32_t* row_slots;     // [m]: adapter slot, outside [0, slots): none
     float* partial;               // [split, m, width] binary32 partial sums of t
     int64_t ldx;
-    int m, k, slots, f16;
-    int split, tiles, width;      // K partitions; 16-rank tiles of all members; 16 * tiles
-    int rank_steps;               // ceil(largest max_rank / 32)
+    int m, k, slots, members, f16;
+    int split, width;             // K partitions; ranks of all members, each rounded up to 16
+    int rank_tiles;               // ceil(largest max_rank / 16)
     int vectors;                  // every member: 16-byte base and output accesses
-    int down_rows, up_rows;       // 16-row tiles per workgroup (1, 2 or 4)
+    int down_rows, up_rows;       // 16-row tiles per workgroup: 1 or 2; 1 or 4
     int down_groups, up_groups;   // workgroups that share a tile's distinct adapters
-    int chunks, chunk_cols;       // column chunks of all members; columns per chunk (32 * 4 * i)
-    AdapterMember member[kMaxGemmMembers];  // unused ones: empty tile and chunk ranges
+    int chunks, chunk_cols;       // column chunks of all members; columns per chunk
+    int chunk_end[kMaxGemmMembers];  // ends of the members' chunks
+    AdapterMember member[kMaxGemmMembers];
 };
 
 hipError_t launch_adapters(const AdapterArgs& a, hipStream_t s);

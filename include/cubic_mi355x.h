@@ -176,7 +176,8 @@ CUBIC_API int cubic_gemm_grouped(const void* x, int64_t ldx, const uint32_t* cod
  * The pointer and extent tables are host arrays of `members` entries.  A row's
  * result does not depend on m or on the other rows, bit for bit.  No output may
  * overlap x, another member's output or base, or the adapters.  1 <= m < 2^24,
- * slots < 2^20, k <= 2^20, ldx <= 2^23, ns[j] * max_ranks[j] < 2^30.
+ * slots < 2^20, k <= 2^20, ldx <= 2^23, ldbases and ldys <= 2^25, ns[j] *
+ * max_ranks[j] < 2^30.
  * Workspace: cubic_adapters_workspace_bytes(m, k, members, max_ranks) bytes, not
  * initialised, 16-byte aligned; one per concurrently running launch.  It covers
  * every smaller m.

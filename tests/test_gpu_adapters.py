@@ -129,8 +129,10 @@ def test_against_the_formula(m, k, ns, ranks, capacity, pattern, dtype):
 
 def test_a_row_does_not_depend_on_its_batch():
     print("adapters: rows of m=1300, 300, 40 and 1 agree bit for bit", flush=True)
-    for dtype in (torch.bfloat16, torch.float16):
-        x, (base,), (bank,), _, slots = case(1300, 2056, (264,), (64, 16, 40), 64, dtype, "mixed", seed=3)
+    # ranks past and within what the one-launch kernel of few rows takes
+    for dtype, ranks in ((torch.bfloat16, (64, 16, 40)), (torch.float16, (64, 16, 40)),
+                         (torch.bfloat16, (16, 3, 9)), (torch.float16, (24, 32, 7))):
+        x, (base,), (bank,), _, slots = case(1300, 2056, (264,), ranks, max(ranks), dtype, "mixed", seed=3)
         whole = torch.empty_like(base)
         ops = linear.PackedLinearOperators()
         ops.bind_adapters(x, bank, slots, whole, bases=base).launch()
