@@ -34,6 +34,8 @@ SIGNATURES: dict[str, tuple] = {
     "cubic_gemm": (I32, [P, I64, P, P, I64, I64, I64, I32, I32, I32, P, I64, P, I64, P]),
     "cubic_gemm_grouped": (I32, [P, I64, P, P, I64, I64, I64, I64, I32, I32, I32, P, I64, P, I64, P,
                                  I64, P]),
+    "cubic_vocab_sample_workspace_bytes": (I64, [I32, I32, I32]),
+    "cubic_vocab_sample": (I32, [P, I32, I64, I32, I32, I32, P, P, P, P, P, P, P, P, P, P, I64, P]),
     "cubic_adapters_workspace_bytes": (I64, [I64, I64, I32, P]),
     "cubic_adapters": (I32, [P, I64, P, I64, I64, I32, I32, P, P, P, P, P, P, P, P, P, P, I32, P, I64, P]),
     "cubic_moe_pad_routes": (I32, [P, P, P, P, P, I32, I32, I32, P, P, P, P]),

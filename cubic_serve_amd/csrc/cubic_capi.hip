@@ -701,6 +701,54 @@ int cubic_embedding(const void* ids, int id_bytes, int64_t tokens, int fmt, cons
 }
 
 // ---------------------------------------------------------------------------
+// Sampling from the whole vocabulary
+// ---------------------------------------------------------------------------
+int64_t cubic_vocab_sample_workspace_bytes(int rows, int width, int dtype) {
+    if (rows < 1 || rows >= (1 << 24) || width < 1 || width > cubic::kMaxSampleWidth || dtype < 0 || dtype > 2)
+        return -1;
+    return 0;
+}
+
+int cubic_vocab_sample(const void* logits, int dtype, int64_t row_stride, int rows, int width, int live_rows,
+                       const int32_t* live_count, const float* temperatures, const int64_t* top_ks,
+                       const float* top_ps, const float* min_ps, const float* uniforms, int64_t* tokens,
+                       uint8_t* valid, float* logprobs, void* workspace, int64_t workspace_bytes,
+                       void* stream) {
+    if (!logits || !temperatures || !top_ks || !top_ps || !min_ps || !uniforms || !tokens || !valid)
+        return fail(CUBIC_EINVAL, "vocabulary sampling: null operand");
+    if (dtype != CUBIC_DTYPE_BF16 && dtype != CUBIC_DTYPE_F16 && dtype != CUBIC_DTYPE_F32)
+        return fail(CUBIC_EINVAL, "vocabulary sampling: dtype must be CUBIC_DTYPE_BF16, _F16 or _F32");
+    if (rows < 1 || rows >= (1 << 24) || width < 1 || width > cubic::kMaxSampleWidth || row_stride < width)
+        return fail(CUBIC_EINVAL, "vocabulary sampling: rows=%d width=%d row_stride=%lld", rows, width,
+                    (long long)row_stride);
+    if ((uintptr_t)logits % (dtype == CUBIC_DTYPE_F32 ? 4 : 2))
+        return fail(CUBIC_EINVAL, "vocabulary sampling: logits are not aligned to their element");
+    if (live_rows < 0 || live_rows > rows) return fail(CUBIC_EINVAL, "live_rows outside 0..rows");
+    const int64_t need = cubic_vocab_sample_workspace_bytes(rows, width, dtype);
+    if (workspace_bytes < need)
+        return fail(CUBIC_EWORKSPACE, "vocabulary sampling workspace %lld < %lld", (long long)workspace_bytes,
+                    (long long)need);
+    if (need && !workspace) return fail(CUBIC_EINVAL, "null workspace");
+    cubic::VocabSampleArgs a = {};
+    a.logits = logits;
+    a.row_stride = row_stride;
+    a.dtype = dtype;
+    a.rows = rows;
+    a.width = width;
+    a.live_rows = live_rows;
+    a.live_count = live_count;
+    a.temperatures = temperatures;
+    a.top_ks = top_ks;
+    a.top_ps = top_ps;
+    a.min_ps = min_ps;
+    a.uniforms = uniforms;
+    a.tokens = tokens;
+    a.valid = valid;
+    a.logprobs = logprobs;
+    return hip_status(cubic::launch_vocab_sample(a, (hipStream_t)stream), "cubic_vocab_sample launch");
+}
+
+// ---------------------------------------------------------------------------
 // Low-rank adapters
 // ---------------------------------------------------------------------------
 int64_t cubic_adapters_workspace_bytes(int64_t m, int64_t k, int members, const int* max_ranks) {

@@ -250,6 +250,25 @@ struct GuardArgs {
     uint8_t* valid;               // [1]
 };
 
+// Sampling from the whole vocabulary (cubic_sample.hip)
+constexpr int kMaxSampleWidth = 1 << 20;
+struct VocabSampleArgs {
+    const void* logits;           // [rows, row_stride] bf16, fp16 or fp32 (dtype)
+    int64_t row_stride;           // elements
+    int dtype, rows, width;
+    int live_rows;                // rows below it are sampled, the others left as they are
+    const int32_t* live_count;    // device int32 that replaces live_rows, or null
+    const float* temperatures;    // [rows]
+    const int64_t* top_ks;
+    const float* top_ps;
+    const float* min_ps;
+    const float* uniforms;
+    int64_t* tokens;              // [rows]
+    uint8_t* valid;               // [rows]
+    float* logprobs;              // [rows] or null
+};
+hipError_t launch_vocab_sample(const VocabSampleArgs& a, hipStream_t s);
+
 // Low-rank adapters beside a shared projection (cubic_adapters.hip)
 constexpr int kAdapterDownK = 1024;  // columns of x per K partition
 constexpr int kAdapterUpTurn = 128;  // columns of y per wave and turn

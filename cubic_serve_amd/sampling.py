@@ -8,6 +8,8 @@ Host mirror of the reference's sampling API (paths under src/cubic_serve/):
   RootTopKTopPSamplingPrimitive ops/cuda/sampling/topk_topp.py:124-278
   MTPVerifyPlan                the finish_review composition,
                                executor/draft_graph.py:1034-1067
+  VocabSamplingPlan            sampling from the whole vocabulary (no
+                               counterpart in the reference)
 
 Candidate selection orders ties by ascending token id (torch.topk leaves the
 order of equal scores at the cutoff unspecified).  All arithmetic runs in the
@@ -403,3 +405,82 @@ class MTPVerifyPlan:
                          self.decisions.data_ptr(), self.merged.data_ptr(), self.emitted.data_ptr(),
                          self.workspace.data_ptr(), self.workspace.numel(),
                          _native.stream_of(self.logits.device))
+
+
+_MAX_SAMPLE_WIDTH = 1 << 20  # kMaxSampleWidth of the C ABI
+
+
+class VocabSamplingPlan:
+    """One token per row from logits over the whole vocabulary, in one launch.
+
+    Columns are ordered by logit, ties by ascending token id.  Of that order a
+    row keeps the first ``top_ks`` (<= 0: all), of these each whose preceding
+    probability mass is below ``top_ps``, and of these each with at least
+    ``min_ps`` times the largest probability, at its temperature; the token is the
+    first one kept whose inclusive mass exceeds ``uniforms`` times the kept mass.
+    Temperature 0 takes the largest logit.  Unlike RootTopKTopPSamplingPrimitive
+    there is no bound on top-k, and the random numbers are given.
+
+    ``logits`` [rows, V] bf16, fp16 or fp32 may have padded rows; -inf masks a
+    token.  Parameters are read when the launch runs: temperatures, top_ps in
+    (0, 1], min_ps in [0, 1] and uniforms in [0, 1) float32 [rows], top_ks int64
+    [rows].  Outputs: ``tokens`` int64, ``valid`` bool and ``logprobs`` float32
+    [rows], the log-probability of the token among those kept.  A row with NaN,
+    +inf or no finite logit, or with a parameter out of range, publishes
+    (-1, False, NaN).  The plan owns its outputs and its workspace: launches of
+    one plan must not overlap.
+    """
+
+    def __init__(self, *, logits: Tensor, temperatures: Tensor, top_ks: Tensor, top_ps: Tensor,
+                 min_ps: Tensor, uniforms: Tensor, visible_width: int | None = None):
+        operands = (logits, temperatures, top_ks, top_ps, min_ps, uniforms)
+        if any(not isinstance(t, Tensor) for t in operands):
+            raise TypeError("vocabulary sampling operands must be tensors")
+        if (logits.dtype not in _CANDIDATE_DTYPES or logits.ndim != 2 or min(logits.shape) < 1
+                or logits.device.type != "cuda" or (logits.stride(1) != 1 and logits.shape[1] > 1)
+                or (logits.stride(0) < logits.shape[1] and logits.shape[0] > 1)):
+            raise ValueError("vocabulary logits must be row-major CUDA bf16, fp16 or fp32 [rows, V]")
+        rows = logits.shape[0]
+        self.width = logits.shape[1] if visible_width is None else visible_width
+        if type(self.width) is not int or not 1 <= self.width <= min(logits.shape[1], _MAX_SAMPLE_WIDTH):
+            raise ValueError(f"visible width must be in 1..V and at most {_MAX_SAMPLE_WIDTH}")
+        for t, dt in ((temperatures, torch.float32), (top_ks, torch.int64), (top_ps, torch.float32),
+                      (min_ps, torch.float32), (uniforms, torch.float32)):
+            if t.shape != (rows,) or t.dtype is not dt or t.device != logits.device or not t.is_contiguous():
+                raise ValueError("sampling parameters must be contiguous float32 (top_ks int64) [rows] "
+                                 "on the logits' device")
+        nbytes = _native.lib().cubic_vocab_sample_workspace_bytes(rows, self.width,
+                                                                  _CANDIDATE_DTYPES[logits.dtype])
+        if nbytes < 0:
+            raise ValueError("vocabulary sampling geometry not admitted")
+        dev = logits.device
+        self.rows, self.logits, self.parameters = rows, logits, operands[1:]
+        self.tokens = torch.empty(rows, dtype=torch.int64, device=dev)
+        self.valid = torch.empty(rows, dtype=torch.bool, device=dev)
+        self.logprobs = torch.empty(rows, dtype=torch.float32, device=dev)
+        self.workspace = torch.zeros(nbytes, dtype=torch.uint8, device=dev)
+        self._fixed = tuple(_fingerprint(t) for t in operands)
+        self._index = dev.index
+        self._head = (_CANDIDATE_DTYPES[logits.dtype], max(logits.stride(0), logits.shape[1]), rows, self.width)
+
+    def launch(self, live_rows: int | Tensor | None = None) -> None:
+        """Enqueue on the current stream.  Rows at or past ``live_rows`` (a host
+        int, or a device int32 tensor whose first element is read when the
+        launch runs) keep their outputs."""
+        live, live_ptr = self.rows, None
+        if isinstance(live_rows, Tensor):
+            if (live_rows.dtype != torch.int32 or live_rows.device != self.logits.device
+                    or live_rows.numel() < 1 or not live_rows.is_contiguous()):
+                raise ValueError("live row count must be a device int32 tensor")
+            live_ptr = live_rows.data_ptr()
+        elif live_rows is not None:
+            if type(live_rows) is not int or not 0 <= live_rows <= self.rows:
+                raise ValueError(f"live row count must be an int in 0..{self.rows} or a device int32 tensor")
+            live = live_rows
+        if tuple(_fingerprint(t) for t in (self.logits, *self.parameters)) != self._fixed:
+            raise ValueError("sampling operands changed after binding")
+        with torch.cuda.device(self._index):
+            _native.call("cubic_vocab_sample", self.logits.data_ptr(), *self._head, live, live_ptr,
+                         *(t.data_ptr() for t in self.parameters), self.tokens.data_ptr(),
+                         self.valid.data_ptr(), self.logprobs.data_ptr(), self.workspace.data_ptr(),
+                         self.workspace.numel(), _native.stream_of(self._index))

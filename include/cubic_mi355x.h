@@ -248,6 +248,38 @@ CUBIC_API int cubic_root_sample(const void* scores, int scores_fp16, const int64
                                 int64_t* output_tokens, uint8_t* output_valid, void* stream);
 
 /* ---------------------------------------------------------------------------
+ * Sampling from the whole vocabulary (no reference counterpart): per row the
+ * token that temperature, top-k, top-p and min-p admit, from a given uniform
+ * number.  cubic_root_sample's order and filters over all of a row's logits, not
+ * over at most 20 gathered candidates, with min-p and given draws.
+ *   logits        dtype CUBIC_DTYPE_BF16, _F16 or _F32 [rows, row_stride], aligned to
+ *                 its element; -inf is a masked column
+ *   temperatures  f32 [rows], finite >= 0; 0 takes the largest logit
+ *   top_ks        int64 [rows]; <= 0 or >= width keeps every column
+ *   top_ps        f32 [rows] in (0, 1]; min_ps f32 [rows] in [0, 1]
+ *   uniforms      f32 [rows] in [0, 1)
+ * Columns are ordered by logit descending, column ascending on ties (-0 == +0).
+ * With p = softmax(logits / temperature): the first top_k columns; of these, in
+ * order, each whose preceding mass is below top_p of theirs; of these each with p
+ * >= min_p times the largest.  The token is the first kept column whose inclusive
+ * mass exceeds uniform times the kept mass.  Masses are 64-bit integers in units of
+ * 2^-43 of the largest, whatever the order of summation.
+ *   tokens int64 [rows], valid bool [rows], logprobs f32 [rows] or NULL (the log of
+ *   the probability with which the kept columns give the token; 0 at temperature 0)
+ * A row that holds NaN or +inf or no finite logit, or whose parameters are outside
+ * the ranges above, publishes -1, 0, NaN.  Rows at or past live_rows (live_count[0],
+ * a device int32 read when the launch runs, if given) are left as they are.
+ *   1 <= rows < 2^24, 1 <= width <= 2^20, width <= row_stride
+ * ------------------------------------------------------------------------- */
+CUBIC_API int64_t cubic_vocab_sample_workspace_bytes(int rows, int width, int dtype);
+CUBIC_API int cubic_vocab_sample(const void* logits, int dtype, int64_t row_stride, int rows, int width,
+                                 int live_rows, const int32_t* live_count, const float* temperatures,
+                                 const int64_t* top_ks, const float* top_ps, const float* min_ps,
+                                 const float* uniforms, int64_t* tokens, uint8_t* valid,
+                                 float* logprobs, void* workspace, int64_t workspace_bytes,
+                                 void* stream);
+
+/* ---------------------------------------------------------------------------
  * Greedy sampling for non-speculative decode (CapturedGreedySampler,
  * ops/cuda/sampling/greedy.py:41-420).  metadata is the sampler's device
  * int32 [2] = (active rows, cancel flag), read when the launch runs.
