@@ -703,10 +703,34 @@ int cubic_embedding(const void* ids, int id_bytes, int64_t tokens, int fmt, cons
 // ---------------------------------------------------------------------------
 // Sampling from the whole vocabulary
 // ---------------------------------------------------------------------------
+namespace {
+struct SamplePlan {
+    int chunks, chunk, list_words;
+    int64_t counters, heads, bytes;  // bytes of the counters, of the heads, of all
+};
+// Chunks of a row of 16-bit logits: as many as fill the chip with all rows'
+// (256 workgroups, one per CU: their counters take most of its LDS), of 4096
+// columns or more.
+SamplePlan plan_sample(int rows, int width, int dtype) {
+    SamplePlan p = {1, width, 0, 0, 0, 0};
+    if (dtype == CUBIC_DTYPE_F32) return p;
+    const int64_t least = ceil_div(width, cubic::kSampleChunk);
+    const int64_t want = std::min<int64_t>({256 / rows, width / 4096, cubic::kMaxSampleChunks});
+    p.chunks = (int)std::max(least, std::max<int64_t>(want, 1));
+    p.chunk = (int)ceil_div(ceil_div(width, p.chunks), 8) * 8;
+    p.chunks = (int)ceil_div(width, p.chunk);
+    p.list_words = std::min(p.chunk, cubic::kSampleList);
+    p.counters = align256((int64_t)rows * 4);
+    p.heads = align256((int64_t)rows * p.chunks * 16);
+    p.bytes = p.counters + p.heads + (int64_t)rows * p.chunks * p.list_words * 4;
+    return p;
+}
+}  // namespace
+
 int64_t cubic_vocab_sample_workspace_bytes(int rows, int width, int dtype) {
     if (rows < 1 || rows >= (1 << 24) || width < 1 || width > cubic::kMaxSampleWidth || dtype < 0 || dtype > 2)
         return -1;
-    return 0;
+    return plan_sample(rows, width, dtype).bytes;
 }
 
 int cubic_vocab_sample(const void* logits, int dtype, int64_t row_stride, int rows, int width, int live_rows,
@@ -724,12 +748,20 @@ int cubic_vocab_sample(const void* logits, int dtype, int64_t row_stride, int ro
     if ((uintptr_t)logits % (dtype == CUBIC_DTYPE_F32 ? 4 : 2))
         return fail(CUBIC_EINVAL, "vocabulary sampling: logits are not aligned to their element");
     if (live_rows < 0 || live_rows > rows) return fail(CUBIC_EINVAL, "live_rows outside 0..rows");
-    const int64_t need = cubic_vocab_sample_workspace_bytes(rows, width, dtype);
+    const SamplePlan p = plan_sample(rows, width, dtype);
+    const int64_t need = p.bytes;
     if (workspace_bytes < need)
         return fail(CUBIC_EWORKSPACE, "vocabulary sampling workspace %lld < %lld", (long long)workspace_bytes,
                     (long long)need);
-    if (need && !workspace) return fail(CUBIC_EINVAL, "null workspace");
+    if (need && (!workspace || !aligned16(workspace))) return fail(CUBIC_EINVAL, "workspace must be 16-byte aligned");
+    if ((int64_t)rows * p.chunks >= INT_MAX) return fail(CUBIC_ENOTSUP, "vocabulary sampling: too many rows");
     cubic::VocabSampleArgs a = {};
+    a.chunks = p.chunks;
+    a.chunk = p.chunk;
+    a.list_words = p.list_words;
+    a.counters = (uint32_t*)workspace;
+    a.heads = (uint32_t*)((uint8_t*)workspace + p.counters);
+    a.lists = (uint32_t*)((uint8_t*)workspace + p.counters + p.heads);
     a.logits = logits;
     a.row_stride = row_stride;
     a.dtype = dtype;

@@ -252,6 +252,9 @@ struct GuardArgs {
 
 // Sampling from the whole vocabulary (cubic_sample.hip)
 constexpr int kMaxSampleWidth = 1 << 20;
+constexpr int kMaxSampleChunks = 64;
+constexpr int kSampleChunk = 65504;    // columns per chunk at most (16-bit counters)
+constexpr int kSampleList = 16384;     // distinct keys per chunk that its list holds
 struct VocabSampleArgs {
     const void* logits;           // [rows, row_stride] bf16, fp16 or fp32 (dtype)
     int64_t row_stride;           // elements
@@ -266,6 +269,11 @@ struct VocabSampleArgs {
     int64_t* tokens;              // [rows]
     uint8_t* valid;               // [rows]
     float* logprobs;              // [rows] or null
+    // 16-bit logits: chunks of `chunk` columns (a multiple of 8), a workgroup each:
+    // counters [rows], zero between launches, heads [rows, chunks, 4],
+    // lists [rows, chunks, list_words]
+    int chunks, chunk, list_words;
+    uint32_t *counters, *heads, *lists;
 };
 hipError_t launch_vocab_sample(const VocabSampleArgs& a, hipStream_t s);
 

@@ -22,7 +22,7 @@ namespace {
 
 constexpr int kThreads = 1024;
 constexpr int kWaves = kThreads / 64;
-constexpr int kBins = 4096;
+constexpr int kBins = 2048;        // first digit of a search: 11 bits of the key
 constexpr double kOne = 8796093022208.0;  // 2^43
 
 // Keys order as the logits do: larger logit, larger key; NaN keys lie past
@@ -61,272 +61,725 @@ struct Limits {  // keys of +inf and -inf
                                                                            : ~0xfc000000u & 0xffff0000u;
 };
 
-// 2^t for t <= 0 in fixed point (2^43 at t = 0): 2^t = 2^n 2^f, |f| <= 1/2, the
-// second factor by the Taylor polynomial of e^(f ln 2) of degree 11 (off by
-// less than 1e-14).
-__device__ __forceinline__ uint64_t fixed_weight(double t) {
-    if (!(t > -46.0)) return 0;
-    const double n = __builtin_rint(t);
-    const double x = (t - n) * 0.69314718055994530942;
-    double p = 1.0 / 39916800.0;
-    p = __builtin_fma(p, x, 1.0 / 3628800.0);
-    p = __builtin_fma(p, x, 1.0 / 362880.0);
-    p = __builtin_fma(p, x, 1.0 / 40320.0);
-    p = __builtin_fma(p, x, 1.0 / 5040.0);
-    p = __builtin_fma(p, x, 1.0 / 720.0);
-    p = __builtin_fma(p, x, 1.0 / 120.0);
-    p = __builtin_fma(p, x, 1.0 / 24.0);
-    p = __builtin_fma(p, x, 1.0 / 6.0);
-    p = __builtin_fma(p, x, 0.5);
-    p = __builtin_fma(p, x, 1.0);
-    p = __builtin_fma(p, x, 1.0);
-    return (uint64_t)__builtin_rint(__builtin_ldexp(p, (int)n + 43));
+// Inclusive scan over the 64 lanes (the exchanges of wave_row_scan).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t dpp_u64(uint64_t v) {
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xF, false);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, ROWS, 0xF, false);
+    return (uint64_t)hi << 32 | lo;
 }
-
-__device__ __forceinline__ uint64_t wave_scan_u64(uint64_t v, int lane) {  // inclusive
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const uint64_t o = __shfl_up(v, d, 64);
-        if (lane >= d) v += o;
-    }
+__device__ __forceinline__ uint64_t wave_scan_u64(uint64_t v) {
+    v += dpp_u64<0x111, 0xF>(v);
+    v += dpp_u64<0x112, 0xF>(v);
+    v += dpp_u64<0x114, 0xF>(v);
+    v += dpp_u64<0x118, 0xF>(v);
+    v += dpp_u64<0x142, 0xA>(v);
+    v += dpp_u64<0x143, 0xC>(v);
     return v;
 }
+__device__ __forceinline__ uint64_t lane_u64(uint64_t v, int l) {  // wave-uniform l
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), l) << 32 |
+           (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, l);
+}
+// Sums of the waves' values before this wave, and of all; lds: one per wave.
+// A barrier lies between the values and the sums, none behind.
+__device__ __forceinline__ uint64_t before_wave(uint64_t value, uint64_t* lds, int lane, int wave, uint64_t& all) {
+    if (lane == 0) lds[wave] = value;
+    __syncthreads();
+    const uint64_t upto = wave_scan_u64(lane < kWaves ? lds[lane] : 0);
+    all = lane_u64(upto, 63);
+    return wave ? lane_u64(upto, wave - 1) : 0;
+}
 
-// Calls f(column, key) for this wave's columns [begin, end) of the row, in
-// ascending order per lane; whole 16-byte words where the row holds them.
-template <int TYPE, typename F>
-__device__ __forceinline__ void each_column(const void* row, int begin, int end, int lane, F&& f) {
+// Columns [c0, c0 + 8) (four of 32 bits) of a row of `width` columns as their
+// bits, c0 a multiple of as many; columns past the row read as -inf.  One load at
+// any alignment, without a branch before it, so that loads of several words go
+// out together: the row's last word is read where it ends and moved into place.
+struct __attribute__((packed, aligned(2))) AnyWord { uint32_t w[4]; };
+template <int TYPE>
+__device__ __forceinline__ uint4 load_word(const uint8_t* row, int c0, int width) {
     constexpr int kBytes = TYPE == 2 ? 4 : 2, kPer = 16 / kBytes;
-    const uint8_t* base = (const uint8_t*)row;
-    // first column of the 16-byte word that holds `begin`
-    const int head = (int)((((uintptr_t)base + (uintptr_t)begin * kBytes) & 15) / kBytes);
-    for (int c0 = begin - head + lane * kPer; c0 < end; c0 += 64 * kPer) {
-        uint32_t bits[kPer];
-        if (c0 >= begin && c0 + kPer <= end) {
-            const uint4 v = *(const uint4*)(base + (int64_t)c0 * kBytes);
-            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    if (width < kPer) {  // a row shorter than a word, element by element
+        uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
-            for (int i = 0; i < kPer; ++i)
-                bits[i] = TYPE == 2 ? w[i & 3] : (i & 1 ? w[i / 2 & 3] >> 16 : w[i / 2 & 3] & 0xffffu);
+        for (int i = 0; i < kPer; ++i) {
+            const uint32_t e = i >= width ? (TYPE == 2 ? 0xff800000u : TYPE == 1 ? 0xfc00u : 0xff80u)
+                               : TYPE == 2 ? ((const uint32_t*)row)[i] : ((const uint16_t*)row)[i];
+            if constexpr (TYPE == 2) w[i] = e;
+            else w[i / 2] |= e << (16 * (i & 1));
+        }
+        return uint4{w[0], w[1], w[2], w[3]};
+    }
+    const AnyWord v = *(const AnyWord*)(row + (int64_t)min(c0, width - kPer) * kBytes);
+    return uint4{v.w[0], v.w[1], v.w[2], v.w[3]};
+}
+template <int TYPE>
+__device__ __forceinline__ uint4 place_word(uint4 v, int c0, int width) {
+    constexpr int kBytes = TYPE == 2 ? 4 : 2, kPer = 16 / kBytes;
+    constexpr uint32_t kFill = TYPE == 2 ? 0xff800000u : TYPE == 1 ? 0xfc00fc00u : 0xff80ff80u;
+    const int past = width < kPer ? c0 : c0 - (width - kPer);  // columns to move by
+    if (past <= 0) return v;
+    if (past >= kPer) return uint4{kFill, kFill, kFill, kFill};
+    typedef unsigned __int128 u128;
+    const u128 fill = ((u128)((uint64_t)kFill << 32 | kFill) << 64) | ((uint64_t)kFill << 32 | kFill);
+    const u128 x = ((u128)((uint64_t)v.w << 32 | v.z) << 64) | ((uint64_t)v.y << 32 | v.x);
+    const u128 y = x >> (past * kBytes * 8) | fill << (128 - past * kBytes * 8);
+    return uint4{(uint32_t)y, (uint32_t)(y >> 32), (uint32_t)(y >> 64), (uint32_t)(y >> 96)};
+}
+template <int TYPE>
+__device__ __forceinline__ uint32_t word_key(const uint4& v, int i) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    if constexpr (TYPE == 2) return key_of<2>(w[i]);
+    else return key_of<TYPE>(i & 1 ? w[i / 2] >> 16 : w[i / 2] & 0xffffu);
+}
+// Calls f(key) for every column of the row (and for -infs past it), the
+// workgroup's threads taking words in turn, four in flight each.
+template <int TYPE, typename F>
+__device__ __forceinline__ void each_column(const uint8_t* row, int width, F&& f) {
+    constexpr int kEach = TYPE == 2 ? 4 : 8, kAhead = TYPE == 2 ? 8 : 4;
+    for (int c0 = (int)threadIdx.x * kEach; c0 < width; c0 += kAhead * kThreads * kEach) {
+        uint4 word[kAhead];
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) f(c0 + i, key_of<TYPE>(bits[i]));
-        } else {
-            for (int i = 0; i < kPer; ++i) {
-                const int c = c0 + i;
-                if (c < begin || c >= end) continue;
-                f(c, key_of<TYPE>(TYPE == 2 ? ((const uint32_t*)row)[c] : ((const uint16_t*)row)[c]));
-            }
+        for (int i = 0; i < kAhead; ++i) word[i] = load_word<TYPE>(row, c0 + i * kThreads * kEach, width);
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const uint4 v = place_word<TYPE>(word[i], c0 + i * kThreads * kEach, width);
+#pragma unroll
+            for (int j = 0; j < kEach; ++j) f(word_key<TYPE>(v, j));
         }
     }
 }
 
-struct Shared {
-    uint32_t count[2][kBins];   // [0]: the first digit's, kept for every search; [1]: deeper digits'
-    unsigned long long mass[2][kBins];
-    uint64_t wave_sum[kWaves];
-    uint32_t wave_key[kWaves];
-    uint32_t wave_flag[kWaves];
-    uint64_t totals[2][kWaves];
+// ---------------------------------------------------------------------------
+// The searches, by one workgroup, over items (key, number of columns with it):
+// the columns themselves, or the distinct keys of a row's chunks.
+// ---------------------------------------------------------------------------
+constexpr int kPer = kBins / kThreads;  // bins per thread
+constexpr int kTable = 128;             // 2^(i / 128)
+
+template <int TYPE>
+struct Search {
+    static constexpr int kDeepBins = TYPE == 2 ? kBins : 32;
+    static constexpr int kCached = TYPE == 2 ? 1 : 30720;  // items held in LDS
+    double table[kTable];
+    uint32_t count[kBins], deep_count[kDeepBins];
+    unsigned long long mass[kBins], deep_mass[kDeepBins];
+    uint32_t items[kCached];    // key's upper half | number
+    int starts[kMaxSampleChunks + 1], held[kMaxSampleChunks];
+    uint64_t sums[4][kWaves];   // before_wave's
     // a search's answer: the bin, and the sums above it
     uint32_t digit;
     uint64_t before_count, before_mass;
 };
 
-// First bin in descending order whose inclusive sum (counts, or masses) plus
-// `before` reaches x; the sums before it, in both measures.  Called by all.
-__device__ __forceinline__ void descend(Shared& sh, int set, bool by_mass, uint64_t x, uint64_t before_count,
-                                        uint64_t before_mass) {
-    constexpr int kPer = kBins / kThreads;
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    // thread t owns bins kBins - 1 - t kPer - i
-    uint64_t c[kPer], m[kPer], cs = 0, ms = 0;
+// A row's parameters, read by one thread (waves that read them by themselves
+// could take different ways through the barriers if a caller rewrites them).
+struct Row {
+    float temperature, top_p, min_p, u;
+    int64_t top_k;
+    __device__ __forceinline__ void read(const VocabSampleArgs& a, int row) {
+        temperature = a.temperatures[row];
+        top_p = a.top_ps[row];
+        min_p = a.min_ps[row];
+        u = a.uniforms[row];
+        top_k = a.top_ks[row];
+    }
+    __device__ __forceinline__ bool admitted() const {
+        return temperature >= 0.f && __builtin_isfinite(temperature) && top_p > 0.f && top_p <= 1.f &&
+               min_p >= 0.f && min_p <= 1.f && u >= 0.f && u < 1.f;
+    }
+};
+
+struct Choice {
+    uint32_t key;   // the token is the nth column (from 1) of this key
+    uint64_t nth;
+    uint64_t kept;  // mass of the kept columns
+};
+
+// Weight of a key in fixed point: with t = 128 log2(e) (l - max) / T and n = rint(t),
+// 2^(t / 128) = 2^(n / 128 rounded down) * table[n mod 128] * e^((t - n) ln 2 / 128), the
+// last by its Taylor polynomial of degree 4 (off by less than 2e-15), rounded to an
+// integer by adding 2^52.
+template <int TYPE>
+struct Weights {
+    double largest, scale, least;
+    const double* table;
+    __device__ __forceinline__ Weights(const double* lds, uint32_t top, const Row& r)
+        : largest(value_of<TYPE>(top)), scale(128.0 * 1.4426950408889634074 / (double)r.temperature),
+          least(r.min_p > 0.f ? 128.0 * log2((double)r.min_p) : -__builtin_inf()), table(lds) {}
+    __device__ __forceinline__ double exponent(uint32_t key) const { return (value_of<TYPE>(key) - largest) * scale; }
+    __device__ __forceinline__ uint64_t at(double t) const {
+        const double n = __builtin_rint(fmax(t, -46.0 * 128.0));
+        const int k = (int)n;
+        const double x = (t - n) * (0.69314718055994530942 / 128.0);
+        const double f = table[k & (kTable - 1)];
+        const double p = x * __builtin_fma(x, __builtin_fma(x, __builtin_fma(x, 1.0 / 24.0, 1.0 / 6.0), 0.5), 1.0);
+        const double w = __builtin_ldexp(__builtin_fma(f, p, f), (k >> 7) + 43) + 4503599627370496.0;
+        return t > -46.0 * 128.0 ? __builtin_bit_cast(uint64_t, w) & 0xfffffffffffffull : 0;
+    }
+    __device__ __forceinline__ uint64_t of(uint32_t key) const { return at(exponent(key)); }
+};
+
+// Sums of this thread's items.
+struct Tally {
+    uint64_t total = 0, likely = 0;  // mass; mass of the weights of at least min_p
+};
+
+// Called by the whole workgroup; a barrier has to follow.
+template <int TYPE>
+__device__ __forceinline__ void clear(Search<TYPE>& sh) {
+    const int t = threadIdx.x;
+    if (t < kTable) sh.table[t] = exp2((double)t / kTable);
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-        c[i] = sh.count[set][kBins - 1 - t * kPer - i];
-        m[i] = sh.mass[set][kBins - 1 - t * kPer - i];
-        cs += c[i];
-        ms += m[i];
+        sh.count[t + i * kThreads] = 0;
+        sh.mass[t + i * kThreads] = 0;
     }
-    const uint64_t ci = wave_scan_u64(cs, lane), mi = wave_scan_u64(ms, lane);
-    if (lane == 63) {
-        sh.totals[0][wave] = ci;
-        sh.totals[1][wave] = mi;
-    }
-    __syncthreads();
-    uint64_t cb = before_count + ci - cs, mb = before_mass + mi - ms;
-    for (int w = 0; w < wave; ++w) {
-        cb += sh.totals[0][w];
-        mb += sh.totals[1][w];
-    }
+}
+template <int TYPE>
+__device__ __forceinline__ void add(Search<TYPE>& sh, const Weights<TYPE>& weights, Tally& tally, uint32_t key,
+                                    uint32_t number) {
+    const double t = weights.exponent(key);
+    const uint64_t w = weights.at(t) * number;
+    if (!w) return;
+    atomicAdd(&sh.count[key >> 21], number);
+    atomicAdd(&sh.mass[key >> 21], (unsigned long long)w);
+    tally.total += w;
+    if (t >= weights.least) tally.likely += w;
+}
+
+// First of the bins in descending order whose inclusive sum (of counts, or of
+// masses) reaches x, with the sums before it; none: the digit is kNoDigit.
+// Thread t owns bins kBins - 1 - t kPer - i with c, m in them; cb, mb lie before.
+constexpr uint32_t kNoDigit = ~0u;
+template <int TYPE>
+__device__ __forceinline__ void pick(Search<TYPE>& sh, const uint32_t (&c)[kPer], const uint64_t (&m)[kPer],
+                                     uint64_t cb, uint64_t mb, bool by_mass, uint64_t x) {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
         const uint64_t lo = by_mass ? mb : cb, add = by_mass ? m[i] : c[i];
         if (lo < x && lo + add >= x) {  // one bin at most
-            sh.digit = kBins - 1 - t * kPer - i;
+            sh.digit = kBins - 1 - threadIdx.x * kPer - i;
             sh.before_count = cb;
             sh.before_mass = mb;
         }
         cb += c[i];
         mb += m[i];
     }
-    __syncthreads();
+}
+template <int TYPE>
+__device__ __forceinline__ void bins_before(Search<TYPE>& sh, const uint32_t* count, const unsigned long long* mass,
+                                            uint32_t (&c)[kPer], uint64_t (&m)[kPer], uint64_t& cb, uint64_t& mb) {
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    uint64_t cs = 0, ms = 0, all;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        c[i] = count[kBins - 1 - t * kPer - i];
+        m[i] = mass[kBins - 1 - t * kPer - i];
+        cs += c[i];
+        ms += m[i];
+    }
+    const uint64_t ci = wave_scan_u64(cs), mi = wave_scan_u64(ms);
+    if (lane == 0) sh.sums[1][wave] = lane_u64(ci, 63);
+    mb = before_wave(lane_u64(mi, 63), sh.sums[0], lane, wave, all) + mi - ms;
+    const uint64_t upto = wave_scan_u64(lane < kWaves ? sh.sums[1][lane] : 0);
+    cb = (wave ? lane_u64(upto, wave - 1) : 0) + ci - cs;
+}
+
+// Called by the whole workgroup once the items are added, after a barrier.
+// items(f) calls f(key, number) for this thread's share of them; columns whose
+// weight is 0 may be left out.
+template <int TYPE, typename Items>
+__device__ __forceinline__ Choice choose(Search<TYPE>& sh, const Weights<TYPE>& weights, const Tally& tally,
+                                         const Row& r, int width, Items&& items) {
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    uint32_t c[kPer];
+    uint64_t m[kPer], cb, mb, head, kept;
+    bins_before<TYPE>(sh, sh.count, sh.mass, c, m, cb, mb);
+    before_wave(lane_u64(wave_scan_u64(tally.total), 63), sh.sums[2], lane, wave, head);
+    before_wave(lane_u64(wave_scan_u64(tally.likely), 63), sh.sums[3], lane, wave, kept);
+    Choice out = {0, 1, 0};
+    for (int stage = 0; stage < 3; ++stage) {  // top-k, top-p, the token; head: mass of what they keep so far
+        uint64_t x;
+        if (stage == 0) {
+            if (r.top_k <= 0 || r.top_k >= width) continue;
+            x = (uint64_t)r.top_k;
+        } else if (stage == 1) {
+            if (r.top_p >= 1.f) continue;
+            x = max((uint64_t)1, min(head, (uint64_t)__builtin_ceil((double)r.top_p * (double)head)));
+        } else {
+            kept = min(kept, head);
+            x = min(kept, (uint64_t)((double)r.u * (double)kept) + 1);
+        }
+        // the key at which the inclusive count or mass reaches x
+        if (t == 0) sh.digit = kNoDigit;
+        if (t < Search<TYPE>::kDeepBins) sh.deep_count[t] = 0, sh.deep_mass[t] = 0;
+        __syncthreads();
+        pick<TYPE>(sh, c, m, cb, mb, stage > 0, x);
+        __syncthreads();
+        uint32_t prefix = sh.digit;
+        if (prefix == kNoDigit) {  // fewer than top_k columns weigh anything
+            __syncthreads();
+            continue;
+        }
+        if constexpr (TYPE != 2) {
+            // the other five bits of a 16-bit key, by one wave
+            items([&](uint32_t k, uint32_t number) {
+                if (k >> 21 != prefix) return;
+                atomicAdd(&sh.deep_count[k >> 16 & 31], number);
+                atomicAdd(&sh.deep_mass[k >> 16 & 31], (unsigned long long)(weights.of(k) * number));
+            });
+            __syncthreads();
+            if (wave == 0) {
+                const uint64_t dc = lane < 32 ? sh.deep_count[31 - lane] : 0, dm = lane < 32 ? sh.deep_mass[31 - lane] : 0;
+                const uint64_t lc = sh.before_count + wave_scan_u64(dc) - dc, lm = sh.before_mass + wave_scan_u64(dm) - dm;
+                const uint64_t lo = stage ? lm : lc, more = stage ? dm : dc;
+                if (lo < x && lo + more >= x) {
+                    sh.digit = 31 - lane;
+                    sh.before_count = lc;
+                    sh.before_mass = lm;
+                }
+            }
+            __syncthreads();
+            out.key = (prefix << 5 | sh.digit) << 16;
+        } else {
+            for (int shift = 21; shift > 0; shift -= shift == 21 ? 11 : 10) {
+                const int bits = shift == 21 ? 11 : 10;
+                const uint64_t bc = sh.before_count, bm = sh.before_mass;
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) {
+                    sh.deep_count[t + i * kThreads] = 0;
+                    sh.deep_mass[t + i * kThreads] = 0;
+                }
+                __syncthreads();
+                items([&](uint32_t k, uint32_t number) {
+                    if (k >> shift != prefix) return;
+                    const uint64_t w = weights.of(k) * number;
+                    const uint32_t d = k >> (shift - bits) & ((1u << bits) - 1);
+                    atomicAdd(&sh.deep_count[d], number);
+                    atomicAdd(&sh.deep_mass[d], (unsigned long long)w);
+                });
+                __syncthreads();
+                uint32_t dc[kPer];
+                uint64_t dm[kPer], dcb, dmb;
+                bins_before<TYPE>(sh, sh.deep_count, sh.deep_mass, dc, dm, dcb, dmb);
+                pick<TYPE>(sh, dc, dm, bc + dcb, bm + dmb, stage > 0, x);
+                __syncthreads();
+                prefix = prefix << bits | sh.digit;
+            }
+            out.key = prefix;
+        }
+        const uint64_t w = weights.of(out.key), above = sh.before_mass;
+        if (stage == 0) head = above + (x - sh.before_count) * w;
+        else out.nth = (x - above + w - 1) / w;
+        if (stage == 1) head = min(head, above + out.nth * w);
+        __syncthreads();
+    }
+    out.kept = kept;
+    return out;
+}
+
+__device__ __forceinline__ void refuse(const VocabSampleArgs& a, int row) {
+    if (threadIdx.x == 0) {
+        a.tokens[row] = -1;
+        a.valid[row] = 0;
+        if (a.logprobs) a.logprobs[row] = __builtin_nanf("");
+    }
+}
+
+// By the thread that holds the token.
+template <int TYPE>
+__device__ __forceinline__ void publish(const VocabSampleArgs& a, int row, const Row& r, uint32_t top,
+                                        const Choice& choice, int column) {
+    a.tokens[row] = column;
+    a.valid[row] = 1;
+    if (!a.logprobs) return;
+    double logprob = 0.0;
+    if (r.temperature > 0.f)
+        logprob = (value_of<TYPE>(choice.key) - value_of<TYPE>(top)) / (double)r.temperature -
+                  log((double)choice.kept / kOne);
+    a.logprobs[row] = (float)logprob;
+}
+
+// The bit pattern of a key's logit (+0 for zero).
+template <int TYPE>
+__device__ __forceinline__ uint32_t pattern_of(uint32_t key) {
+    if constexpr (TYPE == 2) return unordered(key);
+    else return (key & 0x80000000u ? key & 0x7fff0000u : ~key & 0xffff0000u) >> 16;
+}
+
+// Bit j: element j of the word has the pattern (its sign aside where that is 0).
+template <int TYPE>
+__device__ __forceinline__ uint32_t word_hits(const uint4& v, uint32_t pattern) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    uint32_t hits = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if constexpr (TYPE == 2) {
+            hits |= (uint32_t)((pattern ? w[j] : w[j] & 0x7fffffffu) == pattern) << j;
+        } else {
+            const uint32_t x = pattern ? w[j] : w[j] & 0x7fff7fffu;
+            hits |= (uint32_t)((x & 0xffffu) == pattern) << (2 * j) | (uint32_t)(x >> 16 == pattern) << (2 * j + 1);
+        }
+    }
+    return hits;
+}
+
+// The nth column of the key among [begin, end) is the token: WORDS words per
+// thread at a time, each wave a run of them, in order.
+template <int TYPE, int WORDS>
+__device__ __forceinline__ void locate(Search<TYPE>& sh, const VocabSampleArgs& a, int row, const uint8_t* logits,
+                                       int begin, int end, const Row& r, uint32_t top, const Choice& choice) {
+    constexpr int kEach = TYPE == 2 ? 4 : 8;  // columns per word
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const uint32_t pattern = pattern_of<TYPE>(choice.key);
+    uint64_t past = 0;  // columns of the key so far
+    for (int c0 = begin; c0 < end; c0 += kThreads * WORDS * kEach) {
+        // the words of a pass, evenly over the waves
+        const int each = min(WORDS, ((end - c0 + kEach - 1) / kEach + kThreads - 1) / kThreads);
+        const int first = c0 + (wave * each * 64 + lane) * kEach;
+        uint4 word[WORDS];
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i)
+            if (i < each) word[i] = load_word<TYPE>(logits, first + i * 64 * kEach, a.width);
+        uint32_t hits[WORDS];
+        uint32_t mine = 0;
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) {
+            hits[i] = 0;
+            const int c = first + i * 64 * kEach;
+            if (i < each && c < end) hits[i] = word_hits<TYPE>(place_word<TYPE>(word[i], c, a.width), pattern);
+            mine += __builtin_popcount(hits[i]);
+        }
+        const uint64_t upto = wave_scan_u64((uint64_t)mine);
+        uint64_t all;
+        const uint64_t rank = past + before_wave(lane_u64(upto, 63), sh.sums[0], lane, wave, all);
+        if (rank < choice.nth && rank + lane_u64(upto, 63) >= choice.nth) {  // this wave holds it
+            uint64_t from = rank;
+#pragma unroll
+            for (int i = 0; i < WORDS; ++i) {
+                const int here = __builtin_popcount(hits[i]);
+                const uint64_t sum = wave_scan_u64((uint64_t)here), before = from + sum - here;
+                if (before < choice.nth && before + here >= choice.nth) {
+                    uint32_t left = hits[i];
+                    for (uint64_t k = before + 1; k < choice.nth; ++k) left &= left - 1;
+                    publish<TYPE>(a, row, r, top, choice, first + i * 64 * kEach + __builtin_ctz(left));
+                }
+                from += lane_u64(sum, 63);
+            }
+        }
+        past += all;
+        if (past >= choice.nth) return;
+        __syncthreads();  // the sums are free again
+    }
+}
+
+template <int TYPE>
+__device__ __forceinline__ const uint8_t* row_of(const VocabSampleArgs& a, int row) {
+    return (const uint8_t*)a.logits + (int64_t)row * a.row_stride * (TYPE == 2 ? 4 : 2);
+}
+
+// ---------------------------------------------------------------------------
+// 16-bit logits.  A row is cut into chunks, a workgroup each, which reads its
+// chunk once and counts every bit pattern in LDS (65536 16-bit counters: a chunk
+// holds at most 65504 columns).  What is then worth searching of a row is its
+// distinct logits, some thousands for any number of columns: exponentials are
+// taken, and keys formed, per distinct logit and not per column.  The row's last
+// workgroup to arrive searches.
+// ---------------------------------------------------------------------------
+// The largest key below which weights beside a largest logit `top` are 0 (below
+// 2^-44: more than 30.5 T away; 32 T here, rounded down).
+template <int TYPE>
+__device__ __forceinline__ uint32_t least_key(uint32_t top, float temperature) {
+    const double d = value_of<TYPE>(top) - 32.0 * (double)temperature;
+    const float f = __double2float_rd(d);
+    if constexpr (TYPE == 1) return key_of<1>(__half_as_ushort(__float2half_rd(f)));
+    else return key_of<0>(__float_as_uint(f) >> 16) - (f < 0.f && (__float_as_uint(f) & 0xffffu) ? 0x10000u : 0u);
 }
 
 template <int TYPE>
 __global__ __launch_bounds__(kThreads) void vocab_sample_kernel(VocabSampleArgs a) {
-    __shared__ Shared sh;
-    const int row = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    constexpr int kWords = 8;  // 16-byte words per thread: 65504 / 8 / 1024, rounded up
+    constexpr uint32_t kInfBits = TYPE == 1 ? 0x7c00u : 0x7f80u, kNegInfBits = kInfBits | 0x8000u;
+    __shared__ union {
+        uint32_t counts[32768];  // bit pattern k: half k & 1 of word k / 2
+        Search<TYPE> search;
+    } sh;
+    __shared__ uint32_t wave_top[kWaves], wave_bad[kWaves], listed, last;
+    __shared__ Row r;
+    const int row = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     if (row >= (a.live_count ? *a.live_count : a.live_rows)) return;
-    const uint8_t* logits = (const uint8_t*)a.logits + (int64_t)row * a.row_stride * (TYPE == 2 ? 4 : 2);
-    const float temperature = a.temperatures[row], top_p = a.top_ps[row], min_p = a.min_ps[row], u = a.uniforms[row];
-    const int64_t top_k = a.top_ks[row];
-    const int seg = ((a.width + kWaves - 1) / kWaves + 7) / 8 * 8;
-    const int begin = min(a.width, wave * seg), end = min(a.width, begin + seg);
-
-    // the largest finite key, and whether a NaN or +inf is there
+    const uint8_t* logits = row_of<TYPE>(a, row);
+    {
+        const int begin = chunk * a.chunk, end = min(a.width, begin + a.chunk);
+        const int first = begin + t * 8;
+        uint4 word[kWords];
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) word[i] = load_word<TYPE>(logits, first + i * kThreads * 8, a.width);
+        if (t == 0) r.read(a, row);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ((uint4*)sh.counts)[t + i * kThreads] = uint4{0, 0, 0, 0};
+        if (t == 0) listed = 0;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) {
+            if (first + i * kThreads * 8 >= end) break;
+            const uint4 v = place_word<TYPE>(word[i], first + i * kThreads * 8, a.width);
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t lo = w[j] & 0xffffu, hi = w[j] >> 16;
+                // -inf weighs nothing, and a mask makes it most of a row
+                if (lo != kNegInfBits) atomicAdd(&sh.counts[lo >> 1], 1u << (lo << 4 & 16));
+                if (hi != kNegInfBits) atomicAdd(&sh.counts[hi >> 1], 1u << (hi << 4 & 16));
+            }
+        }
+    }
+    __syncthreads();
+    // this thread's patterns that occur: bit 8 i + 2 j + b stands for pattern
+    // 2 (4 (t + 1024 i) + j) + b, so that bits ascend with patterns; the lower
+    // half of the bits are positive numbers, the upper half negative ones
+    uint64_t there = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const uint4 v = ((const uint4*)sh.counts)[t + i * kThreads];
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        uint32_t bits = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            bits |= (uint32_t)((w[j] & 0xffffu) != 0) << (2 * j) | (uint32_t)(w[j] > 0xffffu) << (2 * j + 1);
+        there |= (uint64_t)bits << (8 * i);
+    }
+    auto pattern = [&](int bit) { return (uint32_t)(8 * (t + (bit >> 3) * kThreads) + (bit & 7)); };
+    const uint32_t plus = (uint32_t)there, minus = (uint32_t)(there >> 32);
     uint32_t top = 0, bad = 0;
-    each_column<TYPE>(logits, begin, end, lane, [&](int, uint32_t key) {
-        bad |= key >= Limits<TYPE>::kInf || key < Limits<TYPE>::kNegInf;
+    if (plus) {
+        const uint32_t p = pattern(31 - __builtin_clz(plus));
+        bad = p >= kInfBits;
+        top = key_of<TYPE>(p);
+    } else if (minus) {
+        top = key_of<TYPE>(pattern(32 + __builtin_ctz(minus)));
+    }
+    if (minus) bad |= pattern(63 - __builtin_clz(minus)) > kNegInfBits;
+    top = wave_max_u32(top);
+    bad = __ballot(bad) != 0;
+    if (lane == 0) {
+        wave_top[wave] = top;
+        wave_bad[wave] = bad;
+    }
+    __syncthreads();
+    top = wave_max_u32(lane < kWaves ? wave_top[lane] : 0);
+    bad = __ballot(lane < kWaves && wave_bad[lane]) != 0;
+    // list those that can weigh anything beside the chunk's largest (at
+    // temperature 0 the largest itself): patterns from `low` on among the
+    // positive, up to `high` among the negative ones
+    const uint32_t least = r.temperature > 0.f ? least_key<TYPE>(top, r.temperature) : top;
+    const bool signs = least < 0x80000000u;  // negative ones too
+    const int low = signs ? 0 : (int)pattern_of<TYPE>(least), high = signs ? (int)(pattern_of<TYPE>(least)) : 0;
+    uint32_t* const lists = a.lists + (int64_t)row * a.chunks * a.list_words;
+    uint32_t* const heads = a.heads + (int64_t)row * a.chunks * 4;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int first = 8 * (t + i * kThreads);
+        uint32_t in;
+        if (i < 4) in = 0xffu << min(max(low - first, 0), 8) & 0xffu;
+        else in = signs ? (1u << min(max(high + 1 - first, 0), 8)) - 1 : first == 0x8000 && low == 0 ? 1u : 0u;  // -0
+        there &= ~((uint64_t)(~in & 0xffu) << (8 * i));
+    }
+    const uint32_t mine = (uint32_t)__builtin_popcountll(there);
+    const uint32_t wave_mine = (uint32_t)lane_u64(wave_scan_u64((uint64_t)mine), 63);
+    int base = 0;
+    if (lane == 0 && wave_mine) base = (int)atomicAdd(&listed, wave_mine);
+    base = __builtin_amdgcn_readfirstlane(base);
+    uint32_t* const list = lists + (int64_t)chunk * a.list_words;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const uint32_t bits = (uint32_t)(there >> (8 * i)) & 0xffu;
+        if (__ballot(bits) == 0) continue;
+        const uint4 v = ((const uint4*)sh.counts)[t + i * kThreads];
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const bool in = bits >> j & 1;
+            const uint64_t who = __ballot(in);
+            const int at = base + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
+            if (in && at < a.list_words)
+                store_device(list + at, key_of<TYPE>((uint32_t)(8 * (t + i * kThreads) + j)) |
+                                            (j & 1 ? w[j / 2] >> 16 : w[j / 2] & 0xffffu));
+            base += __builtin_popcountll(who);
+        }
+    }
+    __syncthreads();
+    if (t == 0) {
+        store_device(heads + chunk * 4, listed);
+        store_device(heads + chunk * 4 + 1, top);
+        store_device(heads + chunk * 4 + 2, bad);
+    }
+    if (!arrive_last(a.counters + row, a.chunks, &last)) return;
+    // this workgroup searches the row (the counters' place is free)
+    Search<TYPE>& s = sh.search;
+    if (t == 0) store_device(a.counters + row, 0u);
+    if (wave == 0) {
+        uint32_t number = 0, key = 0, flag = 0;
+        if (lane < a.chunks) {
+            number = load_device(heads + lane * 4);
+            key = load_device(heads + lane * 4 + 1);
+            flag = load_device(heads + lane * 4 + 2);
+        }
+        const uint64_t sum = wave_scan_u64((uint64_t)number);
+        if (lane < a.chunks) {
+            s.starts[lane + 1] = (int)sum;
+            s.held[lane] = 0;
+        }
+        if (lane == 0) s.starts[0] = 0;
+        key = wave_max_u32(key);
+        const uint32_t over = __ballot(number > (uint32_t)a.list_words) != 0 ? 2u : 0u;
+        flag = __ballot(flag != 0) != 0 ? 1u : 0u;
+        if (lane == 0) {
+            wave_top[0] = key;
+            wave_bad[0] = flag | over;
+        }
+    }
+    __syncthreads();
+    top = wave_top[0];
+    const bool whole = !(wave_bad[0] & 2);  // no list overflowed
+    if ((wave_bad[0] & 1) || top <= Limits<TYPE>::kNegInf || !r.admitted()) {
+        refuse(a, row);
+        return;
+    }
+    const int items = s.starts[a.chunks];
+    constexpr int kCached = Search<TYPE>::kCached;
+    auto item_chunk = [&](int i) {  // the chunk whose list holds item i of all
+        int lo = 0, hi = a.chunks;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if (s.starts[mid] <= i) lo = mid;
+            else hi = mid;
+        }
+        return lo;
+    };
+    // f(item's number of all, key | number); the first kCached lie in LDS
+    auto each_item = [&](auto&& f) {
+        for (int i = t; i < min(items, kCached); i += kThreads) f(i, s.items[i]);
+        for (int i = kCached + t; i < items; i += kThreads) {
+            const int c = item_chunk(i);
+            f(i, load_device(lists + (int64_t)c * a.list_words + i - s.starts[c]));
+        }
+    };
+    Choice choice = {top, 1, 0};
+    if (r.temperature > 0.f) {
+        clear<TYPE>(s);
+        __syncthreads();
+        const Weights<TYPE> weights(s.table, top, r);
+        Tally tally;
+        if (whole) {
+            // every list once, four chunks' words in flight
+            constexpr int kAhead = 4;
+            for (int c0 = 0; c0 < a.chunks; c0 += kAhead) {
+                int longest = 0;
+#pragma unroll
+                for (int j = 0; j < kAhead; ++j)
+                    if (c0 + j < a.chunks) longest = max(longest, s.starts[c0 + j + 1] - s.starts[c0 + j]);
+                for (int i = t; i < longest; i += kThreads) {
+                    uint32_t v[kAhead];
+#pragma unroll
+                    for (int j = 0; j < kAhead; ++j) {
+                        const int c = min(c0 + j, a.chunks - 1);
+                        v[j] = c0 + j < a.chunks && i < s.starts[c + 1] - s.starts[c]
+                                   ? load_device(lists + (int64_t)c * a.list_words + i) : 0;
+                    }
+#pragma unroll
+                    for (int j = 0; j < kAhead; ++j) {
+                        if (!v[j]) continue;  // a number is never 0
+                        const int at = s.starts[c0 + j] + i;
+                        if (at < kCached) s.items[at] = v[j];
+                        add<TYPE>(s, weights, tally, v[j] & 0xffff0000u, v[j] & 0xffffu);
+                    }
+                }
+            }
+        } else {
+            each_column<TYPE>(logits, a.width, [&](uint32_t key) { add<TYPE>(s, weights, tally, key, 1u); });
+        }
+        __syncthreads();
+        choice = choose<TYPE>(s, weights, tally, r, a.width, [&](auto&& f) {
+            if (whole) each_item([&](int, uint32_t v) { f(v & 0xffff0000u, v & 0xffffu); });
+            else each_column<TYPE>(logits, a.width, [&](uint32_t key) { f(key, 1u); });
+        });
+    } else if (whole) {
+        // one item per chunk: its largest (two for +0 and -0)
+        for (int i = t; i < items; i += kThreads) {
+            const int c = item_chunk(i);
+            s.items[i] = load_device(lists + (int64_t)c * a.list_words + i - s.starts[c]);
+        }
+        __syncthreads();
+    }
+    // the chunk that holds the nth column of the key
+    int b = 0, e = a.width;
+    if (whole && a.chunks > 1) {
+        each_item([&](int i, uint32_t v) {
+            if ((v & 0xffff0000u) == choice.key) atomicAdd(&s.held[item_chunk(i)], (int)(v & 0xffffu));
+        });
+        __syncthreads();
+        int c = 0;
+        while (c + 1 < a.chunks && choice.nth > (uint64_t)s.held[c]) choice.nth -= s.held[c++];
+        b = c * a.chunk;
+        e = min(a.width, b + a.chunk);
+    }
+    locate<TYPE, kWords>(s, a, row, logits, b, e, r, top, choice);
+}
+
+// ---------------------------------------------------------------------------
+// 32-bit logits: a workgroup per row, the searches over the columns.
+// ---------------------------------------------------------------------------
+__global__ __launch_bounds__(kThreads) void vocab_sample_f32_kernel(VocabSampleArgs a) {
+    __shared__ Search<2> s;
+    __shared__ uint32_t wave_top[kWaves], wave_bad[kWaves];
+    __shared__ Row r;
+    const int row = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    if (row >= (a.live_count ? *a.live_count : a.live_rows)) return;
+    const uint8_t* logits = row_of<2>(a, row);
+    if (t == 0) r.read(a, row);
+    uint32_t top = 0, bad = 0;
+    each_column<2>(logits, a.width, [&](uint32_t key) {
+        bad |= key >= Limits<2>::kInf || key < Limits<2>::kNegInf;
         top = max(top, key);
     });
     top = wave_max_u32(top);
     bad = __ballot(bad) != 0;
     if (lane == 0) {
-        sh.wave_key[wave] = top;
-        sh.wave_flag[wave] = bad;
-    }
-    for (int i = t; i < kBins; i += kThreads) {
-        sh.count[0][i] = 0;
-        sh.mass[0][i] = 0;
+        wave_top[wave] = top;
+        wave_bad[wave] = bad;
     }
     __syncthreads();
-    for (int w = 0; w < kWaves; ++w) {
-        top = max(top, sh.wave_key[w]);
-        bad |= sh.wave_flag[w];
-    }
-    const bool valid = !bad && top > Limits<TYPE>::kNegInf && temperature >= 0.f &&
-                       __builtin_isfinite(temperature) && top_p > 0.f && top_p <= 1.f && min_p >= 0.f &&
-                       min_p <= 1.f && u >= 0.f && u < 1.f;
-    if (!valid) {
-        if (t == 0) {
-            a.tokens[row] = -1;
-            a.valid[row] = 0;
-            if (a.logprobs) a.logprobs[row] = __builtin_nanf("");
-        }
+    top = wave_max_u32(lane < kWaves ? wave_top[lane] : 0);
+    bad = __ballot(lane < kWaves && wave_bad[lane]) != 0;
+    if (bad || top <= Limits<2>::kNegInf || !r.admitted()) {
+        refuse(a, row);
         return;
     }
-    uint32_t key = top;
-    uint64_t nth = 1;  // the token is the nth column of that key
-    double logprob = 0.0;
-    if (temperature > 0.f) {
-        const double largest = value_of<TYPE>(top), scale = 1.4426950408889634074 / (double)temperature;
-        auto power = [&](uint32_t k) { return (value_of<TYPE>(k) - largest) * scale; };
-        const double least = min_p > 0.f ? log2((double)min_p) : -__builtin_inf();
-        uint64_t likely = 0;
-        each_column<TYPE>(logits, begin, end, lane, [&](int, uint32_t k) {
-            const double p = power(k);
-            const uint64_t w = fixed_weight(p);
-            atomicAdd(&sh.count[0][k >> 20], 1u);
-            if (w) atomicAdd(&sh.mass[0][k >> 20], (unsigned long long)w);
-            if (p >= least) likely += w;
-        });
-        likely = wave_scan_u64(likely, lane);
-        if (lane == 63) sh.wave_sum[wave] = likely;
+    Choice choice = {top, 1, 0};
+    if (r.temperature > 0.f) {
+        clear<2>(s);
         __syncthreads();
-        uint64_t kept = 0;
-        for (int w = 0; w < kWaves; ++w) kept += sh.wave_sum[w];
-        uint64_t head = ~0ull;  // mass of what the stages so far keep; all of it at first
-        for (int stage = 0; stage < 3; ++stage) {  // top-k, top-p, the token
-            uint64_t x;
-            if (stage == 0) {
-                if (top_k <= 0 || top_k >= a.width) continue;
-                x = (uint64_t)top_k;
-            } else if (stage == 1) {
-                if (top_p >= 1.f) continue;
-                if (head == ~0ull) {
-                    uint64_t total = 0;
-                    for (int i = lane; i < kBins; i += 64) total += sh.mass[0][i];
-                    head = __shfl(wave_scan_u64(total, lane), 63, 64);
-                }
-                x = max((uint64_t)1, min(head, (uint64_t)__builtin_ceil((double)top_p * (double)head)));
-            } else {
-                kept = min(kept, head);
-                x = min(kept, (uint64_t)((double)u * (double)kept) + 1);
-            }
-            // the key at which the inclusive count or mass reaches x
-            descend(sh, 0, stage > 0, x, 0, 0);
-            uint32_t prefix = sh.digit;
-            int shift = 20;
-            while (shift > (TYPE == 2 ? 0 : 16)) {
-                const int bits = shift == 20 ? 12 : 8;
-                const uint64_t bc = sh.before_count, bm = sh.before_mass;
-                for (int i = t; i < kBins; i += kThreads) {
-                    sh.count[1][i] = 0;
-                    sh.mass[1][i] = 0;
-                }
-                __syncthreads();
-                each_column<TYPE>(logits, begin, end, lane, [&](int, uint32_t k) {
-                    if (k >> shift != prefix) return;
-                    const uint32_t d = (k >> (shift - bits)) & ((1u << bits) - 1);
-                    atomicAdd(&sh.count[1][d], 1u);
-                    atomicAdd(&sh.mass[1][d], (unsigned long long)fixed_weight(power(k)));
-                });
-                __syncthreads();
-                descend(sh, 1, stage > 0, x, bc, bm);
-                prefix = prefix << bits | sh.digit;
-                shift -= bits;
-            }
-            key = prefix << shift;
-            const uint64_t w = fixed_weight(power(key)), above = sh.before_mass;
-            if (stage == 0) head = above + (x - sh.before_count) * w;
-            else nth = (x - above + w - 1) / w;
-            if (stage == 1) head = min(head, above + nth * w);
-            __syncthreads();
-        }
-        logprob = power(key) * 0.69314718055994530942 - log((double)kept / kOne);
+        const Weights<2> weights(s.table, top, r);
+        Tally tally;
+        each_column<2>(logits, a.width, [&](uint32_t key) { add<2>(s, weights, tally, key, 1u); });
+        __syncthreads();
+        choice = choose<2>(s, weights, tally, r, a.width, [&](auto&& f) {
+            each_column<2>(logits, a.width, [&](uint32_t key) { f(key, 1u); });
+        });
     }
-    // the nth column of that key, in ascending order
-    uint64_t found = 0;
-    each_column<TYPE>(logits, begin, end, lane, [&](int, uint32_t k) { found += k == key; });
-    found = wave_scan_u64(found, lane);
-    __syncthreads();
-    if (lane == 63) sh.wave_sum[wave] = found;
-    __syncthreads();
-    uint64_t before = 0;
-    for (int w = 0; w < wave; ++w) before += sh.wave_sum[w];
-    if (before < nth && before + sh.wave_sum[wave] >= nth) {
-        // this wave holds it: 64 columns at a time
-        for (int c0 = begin; c0 < end; c0 += 64) {
-            const int c = c0 + lane;
-            bool hit = false;
-            if (c < end)
-                hit = key_of<TYPE>(TYPE == 2 ? ((const uint32_t*)logits)[c] : ((const uint16_t*)logits)[c]) == key;
-            const uint64_t mask = __ballot(hit);
-            const int here = __builtin_popcountll(mask);
-            if (before + here >= nth) {
-                const int below = __builtin_popcountll(mask & ((1ull << lane) - 1));
-                if (hit && before + below + 1 == nth) {
-                    a.tokens[row] = c;
-                    a.valid[row] = 1;
-                    if (a.logprobs) a.logprobs[row] = (float)logprob;
-                }
-                break;
-            }
-            before += here;
-        }
-    }
-}
-
-template <int TYPE>
-hipError_t start(const VocabSampleArgs& a, hipStream_t s) {
-    vocab_sample_kernel<TYPE><<<a.rows, kThreads, 0, s>>>(a);
-    return hipGetLastError();
+    locate<2, 8>(s, a, row, logits, 0, a.width, r, top, choice);
 }
 
 }  // namespace
 
 hipError_t launch_vocab_sample(const VocabSampleArgs& a, hipStream_t s) {
-    return a.dtype == 2 ? start<2>(a, s) : a.dtype == 1 ? start<1>(a, s) : start<0>(a, s);
+    if (a.dtype == 2) vocab_sample_f32_kernel<<<a.rows, kThreads, 0, s>>>(a);
+    else if (a.dtype == 1) vocab_sample_kernel<1><<<a.rows * a.chunks, kThreads, 0, s>>>(a);
+    else vocab_sample_kernel<0><<<a.rows * a.chunks, kThreads, 0, s>>>(a);
+    return hipGetLastError();
 }
 
 }  // namespace cubic

@@ -179,6 +179,30 @@ def test_refused_rows(dtype):
     assert [r for r in range(16) if plan.tokens[r] >= 0] == [4, 15]
 
 
+@pytest.mark.parametrize("rows,width,spread", [(70, 120000, None), (260, 60001, None), (64, 151936, 3.0)])
+def test_many_distinct_logits(rows, width, spread):
+    """fp16 logits of more distinct values than a chunk's list, or than the
+    search's LDS, holds: all finite bit patterns, or N(0, 3)."""
+    print(f"sample distinct rows={rows} width={width} {spread}", flush=True)
+    gen = torch.Generator().manual_seed(width)
+    if spread:
+        logits = (torch.randn((rows, width), generator=gen) * spread).half()
+        temperature = 1.0
+    else:
+        logits = torch.randint(-32768, 32768, (rows, width), generator=gen, dtype=torch.int32).to(torch.int16)
+        logits = logits.view(torch.float16)
+        logits = torch.where(torch.isfinite(logits), logits, torch.zeros((), dtype=FP16))
+        temperature = 2e4
+    few = torch.arange(0, rows, max(1, rows // 12))
+    _, top_k, top_p, min_p, u = settings(rows, gen)
+    plan = run(logits.to(DEV), temperature, top_k, top_p, min_p, u)
+    part = sampling.VocabSamplingPlan.__new__(sampling.VocabSamplingPlan)
+    part.logits, part.width = plan.logits[few.to(DEV)], plan.width
+    part.parameters = [p[few.to(DEV)] for p in plan.parameters]
+    part.tokens, part.valid, part.logprobs = (t[few.to(DEV)] for t in (plan.tokens, plan.valid, plan.logprobs))
+    check(part)
+
+
 def test_rows_with_strides_and_a_visible_width():
     print("sample strided rows, visible width", flush=True)
     gen = torch.Generator().manual_seed(7)
