@@ -709,14 +709,12 @@ struct SamplePlan {
     int64_t counters, heads, bytes;  // bytes of the counters, of the heads, of all
 };
 // Chunks of a row of 16-bit logits: as many as fill the chip with all rows'
-// (256 workgroups, one per CU: their counters take most of its LDS), of 4096
+// (256 workgroups, one per CU: their counters take most of its LDS), of 8192
 // columns or more.
 SamplePlan plan_sample(int rows, int width, int dtype) {
     SamplePlan p = {1, width, 0, 0, 0, 0};
     if (dtype == CUBIC_DTYPE_F32) return p;
-    const int64_t least = ceil_div(width, cubic::kSampleChunk);
-    const int64_t want = std::min<int64_t>({256 / rows, width / 4096, cubic::kMaxSampleChunks});
-    p.chunks = (int)std::max(least, std::max<int64_t>(want, 1));
+    p.chunks = std::max(1, std::min({256 / rows, width / 8192, cubic::kMaxSampleChunks}));
     p.chunk = (int)ceil_div(ceil_div(width, p.chunks), 8) * 8;
     p.chunks = (int)ceil_div(width, p.chunk);
     p.list_words = std::min(p.chunk, cubic::kSampleList);

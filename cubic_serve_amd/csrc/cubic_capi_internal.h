@@ -253,8 +253,7 @@ struct GuardArgs {
 // Sampling from the whole vocabulary (cubic_sample.hip)
 constexpr int kMaxSampleWidth = 1 << 20;
 constexpr int kMaxSampleChunks = 64;
-constexpr int kSampleChunk = 65504;    // columns per chunk at most (16-bit counters)
-constexpr int kSampleList = 16384;     // distinct keys per chunk that its list holds
+constexpr int kSampleList = 32768;     // distinct logits that a chunk's list holds
 struct VocabSampleArgs {
     const void* logits;           // [rows, row_stride] bf16, fp16 or fp32 (dtype)
     int64_t row_stride;           // elements

@@ -77,6 +77,15 @@ __device__ __forceinline__ uint64_t wave_scan_u64(uint64_t v) {
     v += dpp_u64<0x143, 0xC>(v);
     return v;
 }
+__device__ __forceinline__ uint32_t wave_scan_u32(uint32_t v) {
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xF, 0xF, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xF, 0xF, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xF, 0xF, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xF, 0xF, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xA, 0xF, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xC, 0xF, false);
+    return v;
+}
 __device__ __forceinline__ uint64_t lane_u64(uint64_t v, int l) {  // wave-uniform l
     return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), l) << 32 |
            (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, l);
@@ -160,16 +169,18 @@ constexpr int kTable = 128;             // 2^(i / 128)
 template <int TYPE>
 struct Search {
     static constexpr int kDeepBins = TYPE == 2 ? kBins : 32;
-    static constexpr int kCached = TYPE == 2 ? 1 : 30720;  // items held in LDS
+    static constexpr int kCached = TYPE == 2 ? 4 : kSampleList;  // items held in LDS
+    uint32_t items[kCached];    // key's upper half | number
     double table[kTable];
     uint32_t count[kBins], deep_count[kDeepBins];
     unsigned long long mass[kBins], deep_mass[kDeepBins];
-    uint32_t items[kCached];    // key's upper half | number
     int starts[kMaxSampleChunks + 1], held[kMaxSampleChunks];
     uint64_t sums[4][kWaves];   // before_wave's
-    // a search's answer: the bin, and the sums above it
+    uint32_t count_sums[kWaves];
+    // a search's answer: the digit, the sums above it; of the whole key: its
+    // rank among the key's columns, the mass through it
     uint32_t digit;
-    uint64_t before_count, before_mass;
+    uint64_t before_count, before_mass, nth, through;
 };
 
 // A row's parameters, read by one thread (waves that read them by themselves
@@ -222,7 +233,7 @@ struct Weights {
 
 // Sums of this thread's items.
 struct Tally {
-    uint64_t total = 0, likely = 0;  // mass; mass of the weights of at least min_p
+    uint64_t likely = 0;  // mass of the weights of at least min_p
 };
 
 // Called by the whole workgroup; a barrier has to follow.
@@ -244,7 +255,6 @@ __device__ __forceinline__ void add(Search<TYPE>& sh, const Weights<TYPE>& weigh
     if (!w) return;
     atomicAdd(&sh.count[key >> 21], number);
     atomicAdd(&sh.mass[key >> 21], (unsigned long long)w);
-    tally.total += w;
     if (t >= weights.least) tally.likely += w;
 }
 
@@ -267,11 +277,14 @@ __device__ __forceinline__ void pick(Search<TYPE>& sh, const uint32_t (&c)[kPer]
         mb += m[i];
     }
 }
+// The thread's bins, the sums before them and the mass of all.
 template <int TYPE>
 __device__ __forceinline__ void bins_before(Search<TYPE>& sh, const uint32_t* count, const unsigned long long* mass,
-                                            uint32_t (&c)[kPer], uint64_t (&m)[kPer], uint64_t& cb, uint64_t& mb) {
+                                            uint32_t (&c)[kPer], uint64_t (&m)[kPer], uint64_t& cb, uint64_t& mb,
+                                            uint64_t& all) {
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
-    uint64_t cs = 0, ms = 0, all;
+    uint32_t cs = 0;
+    uint64_t ms = 0;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
         c[i] = count[kBins - 1 - t * kPer - i];
@@ -279,11 +292,32 @@ __device__ __forceinline__ void bins_before(Search<TYPE>& sh, const uint32_t* co
         cs += c[i];
         ms += m[i];
     }
-    const uint64_t ci = wave_scan_u64(cs), mi = wave_scan_u64(ms);
-    if (lane == 0) sh.sums[1][wave] = lane_u64(ci, 63);
+    const uint32_t ci = wave_scan_u32(cs);
+    const uint64_t mi = wave_scan_u64(ms);
+    if (lane == 63) sh.count_sums[wave] = ci;
     mb = before_wave(lane_u64(mi, 63), sh.sums[0], lane, wave, all) + mi - ms;
-    const uint64_t upto = wave_scan_u64(lane < kWaves ? sh.sums[1][lane] : 0);
-    cb = (wave ? lane_u64(upto, wave - 1) : 0) + ci - cs;
+    const uint32_t upto = wave_scan_u32(lane < kWaves ? sh.count_sums[lane] : 0);
+    cb = (wave ? (uint32_t)__builtin_amdgcn_readlane((int)upto, wave - 1) : 0) + ci - cs;
+}
+
+// With the sums before a whole key (weight w): the rank of the position at which
+// the inclusive count or mass reaches x among the key's columns, and the mass
+// through it.  By the thread that found the key.
+template <int TYPE>
+__device__ __forceinline__ void settle(Search<TYPE>& sh, bool by_mass, uint64_t x, uint64_t w) {
+    uint64_t nth;
+    if (by_mass) {
+        // ceil((x - before) / w), a column number (below 2^21), by a quotient
+        // in binary64 that is off by less than one
+        const uint64_t want = x - sh.before_mass;
+        nth = (uint64_t)((double)want / (double)w);
+        while (nth * w < want) ++nth;
+        while (nth > 1 && (nth - 1) * w >= want) --nth;
+    } else {
+        nth = x - sh.before_count;
+    }
+    sh.nth = nth;
+    sh.through = sh.before_mass + nth * w;
 }
 
 // Called by the whole workgroup once the items are added, after a barrier.
@@ -295,9 +329,9 @@ __device__ __forceinline__ Choice choose(Search<TYPE>& sh, const Weights<TYPE>& 
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     uint32_t c[kPer];
     uint64_t m[kPer], cb, mb, head, kept;
-    bins_before<TYPE>(sh, sh.count, sh.mass, c, m, cb, mb);
-    before_wave(lane_u64(wave_scan_u64(tally.total), 63), sh.sums[2], lane, wave, head);
-    before_wave(lane_u64(wave_scan_u64(tally.likely), 63), sh.sums[3], lane, wave, kept);
+    bins_before<TYPE>(sh, sh.count, sh.mass, c, m, cb, mb, head);
+    kept = head;
+    if (r.min_p > 0.f) before_wave(lane_u64(wave_scan_u64(tally.likely), 63), sh.sums[2], lane, wave, kept);
     Choice out = {0, 1, 0};
     for (int stage = 0; stage < 3; ++stage) {  // top-k, top-p, the token; head: mass of what they keep so far
         uint64_t x;
@@ -313,7 +347,8 @@ __device__ __forceinline__ Choice choose(Search<TYPE>& sh, const Weights<TYPE>& 
         }
         // the key at which the inclusive count or mass reaches x
         if (t == 0) sh.digit = kNoDigit;
-        if (t < Search<TYPE>::kDeepBins) sh.deep_count[t] = 0, sh.deep_mass[t] = 0;
+        if constexpr (TYPE != 2)
+            if (t < 32) sh.deep_count[t] = 0, sh.deep_mass[t] = 0;
         __syncthreads();
         pick<TYPE>(sh, c, m, cb, mb, stage > 0, x);
         __syncthreads();
@@ -335,13 +370,15 @@ __device__ __forceinline__ Choice choose(Search<TYPE>& sh, const Weights<TYPE>& 
                 const uint64_t lc = sh.before_count + wave_scan_u64(dc) - dc, lm = sh.before_mass + wave_scan_u64(dm) - dm;
                 const uint64_t lo = stage ? lm : lc, more = stage ? dm : dc;
                 if (lo < x && lo + more >= x) {
-                    sh.digit = 31 - lane;
+                    const uint32_t key = (prefix << 5 | (31 - lane)) << 16;
+                    sh.digit = key;
                     sh.before_count = lc;
                     sh.before_mass = lm;
+                    settle<TYPE>(sh, stage > 0, x, weights.of(key));
                 }
             }
             __syncthreads();
-            out.key = (prefix << 5 | sh.digit) << 16;
+            out.key = sh.digit;
         } else {
             for (int shift = 21; shift > 0; shift -= shift == 21 ? 11 : 10) {
                 const int bits = shift == 21 ? 11 : 10;
@@ -361,18 +398,18 @@ __device__ __forceinline__ Choice choose(Search<TYPE>& sh, const Weights<TYPE>& 
                 });
                 __syncthreads();
                 uint32_t dc[kPer];
-                uint64_t dm[kPer], dcb, dmb;
-                bins_before<TYPE>(sh, sh.deep_count, sh.deep_mass, dc, dm, dcb, dmb);
+                uint64_t dm[kPer], dcb, dmb, all;
+                bins_before<TYPE>(sh, sh.deep_count, sh.deep_mass, dc, dm, dcb, dmb, all);
                 pick<TYPE>(sh, dc, dm, bc + dcb, bm + dmb, stage > 0, x);
                 __syncthreads();
                 prefix = prefix << bits | sh.digit;
             }
+            if (t == 0) settle<TYPE>(sh, stage > 0, x, weights.of(prefix));
+            __syncthreads();
             out.key = prefix;
         }
-        const uint64_t w = weights.of(out.key), above = sh.before_mass;
-        if (stage == 0) head = above + (x - sh.before_count) * w;
-        else out.nth = (x - above + w - 1) / w;
-        if (stage == 1) head = min(head, above + out.nth * w);
+        out.nth = sh.nth;
+        if (stage < 2) head = min(head, sh.through);
         __syncthreads();
     }
     out.kept = kept;
@@ -433,6 +470,7 @@ __device__ __forceinline__ void locate(Search<TYPE>& sh, const VocabSampleArgs& 
     constexpr int kEach = TYPE == 2 ? 4 : 8;  // columns per word
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const uint32_t pattern = pattern_of<TYPE>(choice.key);
+    const bool ragged = end == a.width && a.width % kEach != 0;  // a word reaches past the row
     uint64_t past = 0;  // columns of the key so far
     for (int c0 = begin; c0 < end; c0 += kThreads * WORDS * kEach) {
         // the words of a pass, evenly over the waves
@@ -448,24 +486,26 @@ __device__ __forceinline__ void locate(Search<TYPE>& sh, const VocabSampleArgs& 
         for (int i = 0; i < WORDS; ++i) {
             hits[i] = 0;
             const int c = first + i * 64 * kEach;
-            if (i < each && c < end) hits[i] = word_hits<TYPE>(place_word<TYPE>(word[i], c, a.width), pattern);
+            if (i >= each) continue;
+            if (ragged) word[i] = place_word<TYPE>(word[i], c, a.width);
+            if (c < end) hits[i] = word_hits<TYPE>(word[i], pattern);
             mine += __builtin_popcount(hits[i]);
         }
-        const uint64_t upto = wave_scan_u64((uint64_t)mine);
+        const uint32_t here = (uint32_t)__builtin_amdgcn_readlane((int)wave_scan_u32(mine), 63);
         uint64_t all;
-        const uint64_t rank = past + before_wave(lane_u64(upto, 63), sh.sums[0], lane, wave, all);
-        if (rank < choice.nth && rank + lane_u64(upto, 63) >= choice.nth) {  // this wave holds it
-            uint64_t from = rank;
+        uint64_t from = past + before_wave(here, sh.sums[0], lane, wave, all);
+        if (from < choice.nth && from + here >= choice.nth) {  // this wave holds it
 #pragma unroll
             for (int i = 0; i < WORDS; ++i) {
-                const int here = __builtin_popcount(hits[i]);
-                const uint64_t sum = wave_scan_u64((uint64_t)here), before = from + sum - here;
-                if (before < choice.nth && before + here >= choice.nth) {
+                if (__ballot(hits[i] != 0) == 0) continue;
+                const uint32_t number = __builtin_popcount(hits[i]), sum = wave_scan_u32(number);
+                const uint64_t before = from + sum - number;
+                if (before < choice.nth && before + number >= choice.nth) {
                     uint32_t left = hits[i];
                     for (uint64_t k = before + 1; k < choice.nth; ++k) left &= left - 1;
                     publish<TYPE>(a, row, r, top, choice, first + i * 64 * kEach + __builtin_ctz(left));
                 }
-                from += lane_u64(sum, 63);
+                from += (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
             }
         }
         past += all;
@@ -481,8 +521,7 @@ __device__ __forceinline__ const uint8_t* row_of(const VocabSampleArgs& a, int r
 
 // ---------------------------------------------------------------------------
 // 16-bit logits.  A row is cut into chunks, a workgroup each, which reads its
-// chunk once and counts every bit pattern in LDS (65536 16-bit counters: a chunk
-// holds at most 65504 columns).  What is then worth searching of a row is its
+// chunk once and counts every bit pattern in LDS (65536 counters of 16 bits).  What is then worth searching of a row is its
 // distinct logits, some thousands for any number of columns: exponentials are
 // taken, and keys formed, per distinct logit and not per column.  The row's last
 // workgroup to arrive searches.
@@ -499,41 +538,50 @@ __device__ __forceinline__ uint32_t least_key(uint32_t top, float temperature) {
 
 template <int TYPE>
 __global__ __launch_bounds__(kThreads) void vocab_sample_kernel(VocabSampleArgs a) {
-    constexpr int kWords = 8;  // 16-byte words per thread: 65504 / 8 / 1024, rounded up
+    constexpr int kWords = 8;  // 16-byte words per thread in flight
     constexpr uint32_t kInfBits = TYPE == 1 ? 0x7c00u : 0x7f80u, kNegInfBits = kInfBits | 0x8000u;
     __shared__ union {
         uint32_t counts[32768];  // bit pattern k: half k & 1 of word k / 2
         Search<TYPE> search;
     } sh;
-    __shared__ uint32_t wave_top[kWaves], wave_bad[kWaves], listed, last;
+    __shared__ uint32_t wave_top[kWaves], wave_bad[kWaves], wave_lost[kWaves], listed, last;
     __shared__ Row r;
     const int row = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     if (row >= (a.live_count ? *a.live_count : a.live_rows)) return;
     const uint8_t* logits = row_of<TYPE>(a, row);
+    uint32_t counted = 0;  // this thread's columns, -inf left out
     {
         const int begin = chunk * a.chunk, end = min(a.width, begin + a.chunk);
-        const int first = begin + t * 8;
-        uint4 word[kWords];
+        const bool ragged = end == a.width && a.width % 8 != 0;
+        for (int first = begin + t * 8;; first += kWords * kThreads * 8) {
+            uint4 word[kWords];
 #pragma unroll
-        for (int i = 0; i < kWords; ++i) word[i] = load_word<TYPE>(logits, first + i * kThreads * 8, a.width);
-        if (t == 0) r.read(a, row);
+            for (int i = 0; i < kWords; ++i) word[i] = load_word<TYPE>(logits, first + i * kThreads * 8, a.width);
+            if (first - t * 8 == begin) {
+                if (t == 0) {
+                    r.read(a, row);
+                    listed = 0;
+                }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) ((uint4*)sh.counts)[t + i * kThreads] = uint4{0, 0, 0, 0};
-        if (t == 0) listed = 0;
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < kWords; ++i) {
-            if (first + i * kThreads * 8 >= end) break;
-            const uint4 v = place_word<TYPE>(word[i], first + i * kThreads * 8, a.width);
-            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t lo = w[j] & 0xffffu, hi = w[j] >> 16;
-                // -inf weighs nothing, and a mask makes it most of a row
-                if (lo != kNegInfBits) atomicAdd(&sh.counts[lo >> 1], 1u << (lo << 4 & 16));
-                if (hi != kNegInfBits) atomicAdd(&sh.counts[hi >> 1], 1u << (hi << 4 & 16));
+                for (int i = 0; i < 8; ++i) ((uint4*)sh.counts)[t + i * kThreads] = uint4{0, 0, 0, 0};
+                __syncthreads();
             }
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) {
+                const int c0 = first + i * kThreads * 8;
+                if (c0 >= end) break;
+                const uint4 v = ragged ? place_word<TYPE>(word[i], c0, a.width) : word[i];
+                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t lo = w[j] & 0xffffu, hi = w[j] >> 16;
+                    // -inf weighs nothing, and a mask makes it most of a row
+                    if (lo != kNegInfBits) atomicAdd(&sh.counts[lo >> 1], 1u << (lo << 4 & 16)), ++counted;
+                    if (hi != kNegInfBits) atomicAdd(&sh.counts[hi >> 1], 1u << (hi << 4 & 16)), ++counted;
+                }
+            }
+            if (first - t * 8 + kWords * kThreads * 8 >= end) break;
         }
     }
     __syncthreads();
@@ -541,15 +589,19 @@ __global__ __launch_bounds__(kThreads) void vocab_sample_kernel(VocabSampleArgs 
     // 2 (4 (t + 1024 i) + j) + b, so that bits ascend with patterns; the lower
     // half of the bits are positive numbers, the upper half negative ones
     uint64_t there = 0;
+    uint32_t found = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const uint4 v = ((const uint4*)sh.counts)[t + i * kThreads];
         const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        if (__ballot((v.x | v.y | v.z | v.w) != 0) == 0) continue;
         uint32_t bits = 0;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
             bits |= (uint32_t)((w[j] & 0xffffu) != 0) << (2 * j) | (uint32_t)(w[j] > 0xffffu) << (2 * j + 1);
         there |= (uint64_t)bits << (8 * i);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) found += (w[j] & 0xffffu) + (w[j] >> 16);
     }
     auto pattern = [&](int bit) { return (uint32_t)(8 * (t + (bit >> 3) * kThreads) + (bit & 7)); };
     const uint32_t plus = (uint32_t)there, minus = (uint32_t)(there >> 32);
@@ -562,15 +614,20 @@ __global__ __launch_bounds__(kThreads) void vocab_sample_kernel(VocabSampleArgs 
         top = key_of<TYPE>(pattern(32 + __builtin_ctz(minus)));
     }
     if (minus) bad |= pattern(63 - __builtin_clz(minus)) > kNegInfBits;
+    // a counter that overflows (more than 65535 columns of one logit, in a chunk
+    // that long) takes 65535 or 65536 off the counters' sum
     top = wave_max_u32(top);
     bad = __ballot(bad) != 0;
-    if (lane == 0) {
+    const uint32_t lost = wave_scan_u32(counted - found);
+    if (lane == 63) {
         wave_top[wave] = top;
         wave_bad[wave] = bad;
+        wave_lost[wave] = lost;
     }
     __syncthreads();
     top = wave_max_u32(lane < kWaves ? wave_top[lane] : 0);
     bad = __ballot(lane < kWaves && wave_bad[lane]) != 0;
+    const bool overflow = __builtin_amdgcn_readlane((int)wave_scan_u32(lane < kWaves ? wave_lost[lane] : 0), 63) != 0;
     // list those that can weigh anything beside the chunk's largest (at
     // temperature 0 the largest itself): patterns from `low` on among the
     // positive, up to `high` among the negative ones
@@ -612,7 +669,7 @@ __global__ __launch_bounds__(kThreads) void vocab_sample_kernel(VocabSampleArgs 
     }
     __syncthreads();
     if (t == 0) {
-        store_device(heads + chunk * 4, listed);
+        store_device(heads + chunk * 4, overflow ? ~0u : listed);  // (~0: no list holds it)
         store_device(heads + chunk * 4 + 1, top);
         store_device(heads + chunk * 4 + 2, bad);
     }
@@ -627,7 +684,7 @@ __global__ __launch_bounds__(kThreads) void vocab_sample_kernel(VocabSampleArgs 
             key = load_device(heads + lane * 4 + 1);
             flag = load_device(heads + lane * 4 + 2);
         }
-        const uint64_t sum = wave_scan_u64((uint64_t)number);
+        const uint64_t sum = wave_scan_u64((uint64_t)min(number, (uint32_t)a.list_words));
         if (lane < a.chunks) {
             s.starts[lane + 1] = (int)sum;
             s.held[lane] = 0;
@@ -650,22 +707,34 @@ __global__ __launch_bounds__(kThreads) void vocab_sample_kernel(VocabSampleArgs 
     }
     const int items = s.starts[a.chunks];
     constexpr int kCached = Search<TYPE>::kCached;
-    auto item_chunk = [&](int i) {  // the chunk whose list holds item i of all
-        int lo = 0, hi = a.chunks;
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) / 2;
-            if (s.starts[mid] <= i) lo = mid;
-            else hi = mid;
+    // f(c, i, v): word i of chunk c's list, four in flight, for the words whose
+    // number of all is at least `from`
+    auto each_listed = [&](int from, auto&& f) {
+        constexpr int kAhead = 4;
+        for (int c = 0; c < a.chunks; ++c) {
+            const int n = s.starts[c + 1] - s.starts[c];
+            for (int i = max(0, from - s.starts[c]) + t; i < n; i += kAhead * kThreads) {
+                uint32_t v[kAhead];
+#pragma unroll
+                for (int j = 0; j < kAhead; ++j)
+                    v[j] = i + j * kThreads < n ? load_device(lists + (int64_t)c * a.list_words + i + j * kThreads) : 0;
+#pragma unroll
+                for (int j = 0; j < kAhead; ++j)
+                    if (v[j]) f(c, i + j * kThreads, v[j]);  // (a number is never 0)
+            }
         }
-        return lo;
     };
-    // f(item's number of all, key | number); the first kCached lie in LDS
+    // f(i, v): item i of all; the first kCached lie in LDS, four to a read
     auto each_item = [&](auto&& f) {
-        for (int i = t; i < min(items, kCached); i += kThreads) f(i, s.items[i]);
-        for (int i = kCached + t; i < items; i += kThreads) {
-            const int c = item_chunk(i);
-            f(i, load_device(lists + (int64_t)c * a.list_words + i - s.starts[c]));
+        const int cached = min(items, kCached);
+        for (int i = 4 * t; i < cached; i += 4 * kThreads) {
+            const uint4 v = *(const uint4*)&s.items[i];
+            f(i, v.x);
+            if (i + 1 < cached) f(i + 1, v.y);
+            if (i + 2 < cached) f(i + 2, v.z);
+            if (i + 3 < cached) f(i + 3, v.w);
         }
+        if (items > kCached) each_listed(kCached, [&](int c, int i, uint32_t v) { f(s.starts[c] + i, v); });
     };
     Choice choice = {top, 1, 0};
     if (r.temperature > 0.f) {
@@ -681,19 +750,21 @@ __global__ __launch_bounds__(kThreads) void vocab_sample_kernel(VocabSampleArgs 
 #pragma unroll
                 for (int j = 0; j < kAhead; ++j)
                     if (c0 + j < a.chunks) longest = max(longest, s.starts[c0 + j + 1] - s.starts[c0 + j]);
-                for (int i = t; i < longest; i += kThreads) {
+                const int step = a.chunks == 1 ? kAhead * kThreads : kThreads;  // (one chunk: four of its words)
+                for (int i = t; i < longest; i += step) {
                     uint32_t v[kAhead];
+                    int at[kAhead];
 #pragma unroll
                     for (int j = 0; j < kAhead; ++j) {
-                        const int c = min(c0 + j, a.chunks - 1);
-                        v[j] = c0 + j < a.chunks && i < s.starts[c + 1] - s.starts[c]
-                                   ? load_device(lists + (int64_t)c * a.list_words + i) : 0;
+                        const int c = a.chunks == 1 ? 0 : min(c0 + j, a.chunks - 1), k = a.chunks == 1 ? i + j * kThreads : i;
+                        at[j] = s.starts[c] + k;
+                        v[j] = (a.chunks == 1 || c0 + j < a.chunks) && at[j] < s.starts[c + 1]
+                                   ? load_device(lists + (int64_t)c * a.list_words + k) : 0;
                     }
 #pragma unroll
                     for (int j = 0; j < kAhead; ++j) {
-                        if (!v[j]) continue;  // a number is never 0
-                        const int at = s.starts[c0 + j] + i;
-                        if (at < kCached) s.items[at] = v[j];
+                        if (!v[j]) continue;
+                        if (at[j] < kCached) s.items[at[j]] = v[j];
                         add<TYPE>(s, weights, tally, v[j] & 0xffff0000u, v[j] & 0xffffu);
                     }
                 }
@@ -708,17 +779,17 @@ __global__ __launch_bounds__(kThreads) void vocab_sample_kernel(VocabSampleArgs 
         });
     } else if (whole) {
         // one item per chunk: its largest (two for +0 and -0)
-        for (int i = t; i < items; i += kThreads) {
-            const int c = item_chunk(i);
-            s.items[i] = load_device(lists + (int64_t)c * a.list_words + i - s.starts[c]);
-        }
+        each_listed(0, [&](int c, int i, uint32_t v) { s.items[s.starts[c] + i] = v; });
         __syncthreads();
     }
     // the chunk that holds the nth column of the key
     int b = 0, e = a.width;
     if (whole && a.chunks > 1) {
         each_item([&](int i, uint32_t v) {
-            if ((v & 0xffff0000u) == choice.key) atomicAdd(&s.held[item_chunk(i)], (int)(v & 0xffffu));
+            if ((v & 0xffff0000u) != choice.key) return;
+            int c = 0;
+            while (s.starts[c + 1] <= i) ++c;
+            atomicAdd(&s.held[c], (int)(v & 0xffffu));
         });
         __syncthreads();
         int c = 0;
