@@ -708,18 +708,18 @@ struct SamplePlan {
     int chunks, chunk, list_words;
     int64_t counters, heads, bytes;  // bytes of the counters, of the heads, of all
 };
-// Chunks of a row of 16-bit logits: as many as fill the chip with all rows'
-// (256 workgroups, one per CU: their counters take most of its LDS), of 8192
-// columns or more.
+// Chunks of a row: as many as fill the chip with all rows' (256 workgroups, one
+// per CU: what they count takes most of its LDS), of 8192 columns or more.
 SamplePlan plan_sample(int rows, int width, int dtype) {
-    SamplePlan p = {1, width, 0, 0, 0, 0};
-    if (dtype == CUBIC_DTYPE_F32) return p;
+    SamplePlan p = {};
     p.chunks = std::max(1, std::min({256 / rows, width / 8192, cubic::kMaxSampleChunks}));
     p.chunk = (int)ceil_div(ceil_div(width, p.chunks), 8) * 8;
     p.chunks = (int)ceil_div(width, p.chunk);
-    p.list_words = std::min(p.chunk, cubic::kSampleList);
+    p.list_words = dtype != CUBIC_DTYPE_F32 ? std::min(p.chunk, cubic::kSampleList)
+                   : p.chunks == 1          ? 0
+                                            : 4 * std::min(p.chunk, cubic::kSampleBins);
     p.counters = align256((int64_t)rows * 4);
-    p.heads = align256((int64_t)rows * p.chunks * 16);
+    p.heads = align256((int64_t)rows * p.chunks * cubic::kSampleHead * 4);
     p.bytes = p.counters + p.heads + (int64_t)rows * p.chunks * p.list_words * 4;
     return p;
 }

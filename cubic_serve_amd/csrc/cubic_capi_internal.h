@@ -253,7 +253,9 @@ struct GuardArgs {
 // Sampling from the whole vocabulary (cubic_sample.hip)
 constexpr int kMaxSampleWidth = 1 << 20;
 constexpr int kMaxSampleChunks = 64;
-constexpr int kSampleList = 32768;     // distinct logits that a chunk's list holds
+constexpr int kSampleList = 32768;     // distinct 16-bit logits that a chunk's list holds
+constexpr int kSampleBins = 4096;      // bins of a chunk's list of 32-bit logits, four words each
+constexpr int kSampleHead = 8;         // words of a chunk's head
 struct VocabSampleArgs {
     const void* logits;           // [rows, row_stride] bf16, fp16 or fp32 (dtype)
     int64_t row_stride;           // elements
@@ -268,9 +270,8 @@ struct VocabSampleArgs {
     int64_t* tokens;              // [rows]
     uint8_t* valid;               // [rows]
     float* logprobs;              // [rows] or null
-    // 16-bit logits: chunks of `chunk` columns (a multiple of 8), a workgroup each:
-    // counters [rows], zero between launches, heads [rows, chunks, 4],
-    // lists [rows, chunks, list_words]
+    // chunks of `chunk` columns (a multiple of 8), a workgroup each: counters [rows],
+    // zero between launches, heads [rows, chunks, kSampleHead], lists [rows, chunks, list_words]
     int chunks, chunk, list_words;
     uint32_t *counters, *heads, *lists;
 };

@@ -22,7 +22,6 @@ namespace {
 
 constexpr int kThreads = 1024;
 constexpr int kWaves = kThreads / 64;
-constexpr int kBins = 2048;        // first digit of a search: 11 bits of the key
 constexpr double kOne = 8796093022208.0;  // 2^43
 
 // Keys order as the logits do: larger logit, larger key; NaN keys lie past
@@ -141,20 +140,23 @@ __device__ __forceinline__ uint32_t word_key(const uint4& v, int i) {
     if constexpr (TYPE == 2) return key_of<2>(w[i]);
     else return key_of<TYPE>(i & 1 ? w[i / 2] >> 16 : w[i / 2] & 0xffffu);
 }
-// Calls f(key) for every column of the row (and for -infs past it), the
-// workgroup's threads taking words in turn, four in flight each.
+// Calls f(column, key) for columns [begin, end) of the row, begin a multiple of 8
+// (and for -infs past its end), the workgroup's threads taking words in turn,
+// several in flight each.
 template <int TYPE, typename F>
-__device__ __forceinline__ void each_column(const uint8_t* row, int width, F&& f) {
-    constexpr int kEach = TYPE == 2 ? 4 : 8, kAhead = TYPE == 2 ? 8 : 4;
-    for (int c0 = (int)threadIdx.x * kEach; c0 < width; c0 += kAhead * kThreads * kEach) {
+__device__ __forceinline__ void each_column(const uint8_t* row, int begin, int end, int width, F&& f) {
+    constexpr int kEach = TYPE == 2 ? 4 : 8, kAhead = 4;
+    for (int c0 = begin + (int)threadIdx.x * kEach; c0 < end; c0 += kAhead * kThreads * kEach) {
         uint4 word[kAhead];
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) word[i] = load_word<TYPE>(row, c0 + i * kThreads * kEach, width);
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
-            const uint4 v = place_word<TYPE>(word[i], c0 + i * kThreads * kEach, width);
+            const int c = c0 + i * kThreads * kEach;
+            if (c >= end) break;
+            const uint4 v = place_word<TYPE>(word[i], c, width);
 #pragma unroll
-            for (int j = 0; j < kEach; ++j) f(word_key<TYPE>(v, j));
+            for (int j = 0; j < kEach; ++j) f(c + j, word_key<TYPE>(v, j));
         }
     }
 }
@@ -163,17 +165,23 @@ __device__ __forceinline__ void each_column(const uint8_t* row, int width, F&& f
 // The searches, by one workgroup, over items (key, number of columns with it):
 // the columns themselves, or the distinct keys of a row's chunks.
 // ---------------------------------------------------------------------------
-constexpr int kPer = kBins / kThreads;  // bins per thread
-constexpr int kTable = 128;             // 2^(i / 128)
+constexpr int kTable = 128;  // 2^(i / 128)
 
 template <int TYPE>
 struct Search {
-    static constexpr int kDeepBins = TYPE == 2 ? kBins : 32;
-    static constexpr int kCached = TYPE == 2 ? 4 : kSampleList;  // items held in LDS
-    uint32_t items[kCached];    // key's upper half | number
+    // bins: the first digit, 11 of a 16-bit key's bits or 12 of 32; then the
+    // other 5, or twice 10
+    static constexpr int kBins = TYPE == 2 ? 4096 : 2048, kShift = TYPE == 2 ? 20 : 21;
+    static constexpr int kPer = kBins / kThreads;  // bins per thread
+    static constexpr int kDeepBins = TYPE == 2 ? 1024 : 32;
+    // items held in LDS: key's upper half | number; or (32 bits) the columns of
+    // one first digit, key and column
+    static constexpr int kCached = TYPE == 2 ? 8192 : kSampleList;
+    uint32_t items[TYPE == 2 ? 2 * kCached : kCached];
     double table[kTable];
     uint32_t count[kBins], deep_count[kDeepBins];
     unsigned long long mass[kBins], deep_mass[kDeepBins];
+    uint32_t gathered;          // columns of the first digit (32 bits)
     int starts[kMaxSampleChunks + 1], held[kMaxSampleChunks];
     uint64_t sums[4][kWaves];   // before_wave's
     uint32_t count_sums[kWaves];
@@ -242,7 +250,7 @@ __device__ __forceinline__ void clear(Search<TYPE>& sh) {
     const int t = threadIdx.x;
     if (t < kTable) sh.table[t] = exp2((double)t / kTable);
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
+    for (int i = 0; i < Search<TYPE>::kPer; ++i) {
         sh.count[t + i * kThreads] = 0;
         sh.mass[t + i * kThreads] = 0;
     }
@@ -253,23 +261,23 @@ __device__ __forceinline__ void add(Search<TYPE>& sh, const Weights<TYPE>& weigh
     const double t = weights.exponent(key);
     const uint64_t w = weights.at(t) * number;
     if (!w) return;
-    atomicAdd(&sh.count[key >> 21], number);
-    atomicAdd(&sh.mass[key >> 21], (unsigned long long)w);
+    atomicAdd(&sh.count[key >> Search<TYPE>::kShift], number);
+    atomicAdd(&sh.mass[key >> Search<TYPE>::kShift], (unsigned long long)w);
     if (t >= weights.least) tally.likely += w;
 }
 
 // First of the bins in descending order whose inclusive sum (of counts, or of
 // masses) reaches x, with the sums before it; none: the digit is kNoDigit.
-// Thread t owns bins kBins - 1 - t kPer - i with c, m in them; cb, mb lie before.
+// Thread t owns bins BINS - 1 - t PER - i with c, m in them; cb, mb lie before.
 constexpr uint32_t kNoDigit = ~0u;
-template <int TYPE>
-__device__ __forceinline__ void pick(Search<TYPE>& sh, const uint32_t (&c)[kPer], const uint64_t (&m)[kPer],
+template <int TYPE, int PER>
+__device__ __forceinline__ void pick(Search<TYPE>& sh, const uint32_t (&c)[PER], const uint64_t (&m)[PER],
                                      uint64_t cb, uint64_t mb, bool by_mass, uint64_t x) {
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
+    for (int i = 0; i < PER; ++i) {
         const uint64_t lo = by_mass ? mb : cb, add = by_mass ? m[i] : c[i];
         if (lo < x && lo + add >= x) {  // one bin at most
-            sh.digit = kBins - 1 - threadIdx.x * kPer - i;
+            sh.digit = PER * kThreads - 1 - threadIdx.x * PER - i;
             sh.before_count = cb;
             sh.before_mass = mb;
         }
@@ -278,17 +286,17 @@ __device__ __forceinline__ void pick(Search<TYPE>& sh, const uint32_t (&c)[kPer]
     }
 }
 // The thread's bins, the sums before them and the mass of all.
-template <int TYPE>
+template <int TYPE, int PER>
 __device__ __forceinline__ void bins_before(Search<TYPE>& sh, const uint32_t* count, const unsigned long long* mass,
-                                            uint32_t (&c)[kPer], uint64_t (&m)[kPer], uint64_t& cb, uint64_t& mb,
+                                            uint32_t (&c)[PER], uint64_t (&m)[PER], uint64_t& cb, uint64_t& mb,
                                             uint64_t& all) {
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     uint32_t cs = 0;
     uint64_t ms = 0;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-        c[i] = count[kBins - 1 - t * kPer - i];
-        m[i] = mass[kBins - 1 - t * kPer - i];
+    for (int i = 0; i < PER; ++i) {
+        c[i] = count[PER * kThreads - 1 - t * PER - i];
+        m[i] = mass[PER * kThreads - 1 - t * PER - i];
         cs += c[i];
         ms += m[i];
     }
@@ -321,15 +329,20 @@ __device__ __forceinline__ void settle(Search<TYPE>& sh, bool by_mass, uint64_t 
 }
 
 // Called by the whole workgroup once the items are added, after a barrier.
-// items(f) calls f(key, number) for this thread's share of them; columns whose
-// weight is 0 may be left out.
-template <int TYPE, typename Items>
+// 16 bits: items(f) calls f(key, number) for this thread's share of them;
+// columns whose weight is 0 may be left out.  32 bits: items(digit) gathers the
+// columns of a first digit (key and column in sh.items, their number in
+// sh.gathered, past kCached only that), barriers before and behind included;
+// columns(f) calls f(key) for this thread's share of the row's columns.
+template <int TYPE, typename Items, typename Columns>
 __device__ __forceinline__ Choice choose(Search<TYPE>& sh, const Weights<TYPE>& weights, const Tally& tally,
-                                         const Row& r, int width, Items&& items) {
+                                         const Row& r, int width, Items&& items, Columns&& columns) {
+    constexpr int kPer = Search<TYPE>::kPer;
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    [[maybe_unused]] uint32_t held = kNoDigit;  // the digit whose columns are gathered (32 bits)
     uint32_t c[kPer];
     uint64_t m[kPer], cb, mb, head, kept;
-    bins_before<TYPE>(sh, sh.count, sh.mass, c, m, cb, mb, head);
+    bins_before<TYPE, kPer>(sh, sh.count, sh.mass, c, m, cb, mb, head);
     kept = head;
     if (r.min_p > 0.f) before_wave(lane_u64(wave_scan_u64(tally.likely), 63), sh.sums[2], lane, wave, kept);
     Choice out = {0, 1, 0};
@@ -350,7 +363,7 @@ __device__ __forceinline__ Choice choose(Search<TYPE>& sh, const Weights<TYPE>& 
         if constexpr (TYPE != 2)
             if (t < 32) sh.deep_count[t] = 0, sh.deep_mass[t] = 0;
         __syncthreads();
-        pick<TYPE>(sh, c, m, cb, mb, stage > 0, x);
+        pick<TYPE, kPer>(sh, c, m, cb, mb, stage > 0, x);
         __syncthreads();
         uint32_t prefix = sh.digit;
         if (prefix == kNoDigit) {  // fewer than top_k columns weigh anything
@@ -380,29 +393,33 @@ __device__ __forceinline__ Choice choose(Search<TYPE>& sh, const Weights<TYPE>& 
             __syncthreads();
             out.key = sh.digit;
         } else {
-            for (int shift = 21; shift > 0; shift -= shift == 21 ? 11 : 10) {
-                const int bits = shift == 21 ? 11 : 10;
+            if (prefix != held) items(prefix);
+            held = prefix;
+            const int gathered = (int)sh.gathered;
+            for (int shift = 20; shift > 0; shift -= 10) {
                 const uint64_t bc = sh.before_count, bm = sh.before_mass;
-#pragma unroll
-                for (int i = 0; i < kPer; ++i) {
-                    sh.deep_count[t + i * kThreads] = 0;
-                    sh.deep_mass[t + i * kThreads] = 0;
-                }
+                sh.deep_count[t] = 0;
+                sh.deep_mass[t] = 0;
                 __syncthreads();
-                items([&](uint32_t k, uint32_t number) {
+                auto deepen = [&](uint32_t k) {
                     if (k >> shift != prefix) return;
-                    const uint64_t w = weights.of(k) * number;
-                    const uint32_t d = k >> (shift - bits) & ((1u << bits) - 1);
-                    atomicAdd(&sh.deep_count[d], number);
+                    const uint64_t w = weights.of(k);
+                    if (!w) return;
+                    const uint32_t d = k >> (shift - 10) & 1023u;
+                    atomicAdd(&sh.deep_count[d], 1u);
                     atomicAdd(&sh.deep_mass[d], (unsigned long long)w);
-                });
+                };
+                if (gathered <= Search<TYPE>::kCached)
+                    for (int i = t; i < gathered; i += kThreads) deepen(sh.items[2 * i]);
+                else
+                    columns(deepen);
                 __syncthreads();
-                uint32_t dc[kPer];
-                uint64_t dm[kPer], dcb, dmb, all;
-                bins_before<TYPE>(sh, sh.deep_count, sh.deep_mass, dc, dm, dcb, dmb, all);
-                pick<TYPE>(sh, dc, dm, bc + dcb, bm + dmb, stage > 0, x);
+                uint32_t dc[1];
+                uint64_t dm[1], dcb, dmb, all;
+                bins_before<TYPE, 1>(sh, sh.deep_count, sh.deep_mass, dc, dm, dcb, dmb, all);
+                pick<TYPE, 1>(sh, dc, dm, bc + dcb, bm + dmb, stage > 0, x);
                 __syncthreads();
-                prefix = prefix << bits | sh.digit;
+                prefix = prefix << 10 | sh.digit;
             }
             if (t == 0) settle<TYPE>(sh, stage > 0, x, weights.of(prefix));
             __syncthreads();
@@ -554,13 +571,15 @@ __global__ __launch_bounds__(kThreads) void vocab_sample_kernel(VocabSampleArgs 
     {
         const int begin = chunk * a.chunk, end = min(a.width, begin + a.chunk);
         const bool ragged = end == a.width && a.width % 8 != 0;
+        Row params;  // (ahead of the words: what waits for it would wait for them)
+        params.read(a, row);
         for (int first = begin + t * 8;; first += kWords * kThreads * 8) {
             uint4 word[kWords];
 #pragma unroll
             for (int i = 0; i < kWords; ++i) word[i] = load_word<TYPE>(logits, first + i * kThreads * 8, a.width);
             if (first - t * 8 == begin) {
                 if (t == 0) {
-                    r.read(a, row);
+                    r = params;
                     listed = 0;
                 }
 #pragma unroll
@@ -635,7 +654,7 @@ __global__ __launch_bounds__(kThreads) void vocab_sample_kernel(VocabSampleArgs 
     const bool signs = least < 0x80000000u;  // negative ones too
     const int low = signs ? 0 : (int)pattern_of<TYPE>(least), high = signs ? (int)(pattern_of<TYPE>(least)) : 0;
     uint32_t* const lists = a.lists + (int64_t)row * a.chunks * a.list_words;
-    uint32_t* const heads = a.heads + (int64_t)row * a.chunks * 4;
+    uint32_t* const heads = a.heads + (int64_t)row * a.chunks * kSampleHead;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const int first = 8 * (t + i * kThreads);
@@ -669,9 +688,9 @@ __global__ __launch_bounds__(kThreads) void vocab_sample_kernel(VocabSampleArgs 
     }
     __syncthreads();
     if (t == 0) {
-        store_device(heads + chunk * 4, overflow ? ~0u : listed);  // (~0: no list holds it)
-        store_device(heads + chunk * 4 + 1, top);
-        store_device(heads + chunk * 4 + 2, bad);
+        store_device(heads + chunk * kSampleHead, overflow ? ~0u : listed);  // (~0: no list holds it)
+        store_device(heads + chunk * kSampleHead + 1, top);
+        store_device(heads + chunk * kSampleHead + 2, bad);
     }
     if (!arrive_last(a.counters + row, a.chunks, &last)) return;
     // this workgroup searches the row (the counters' place is free)
@@ -680,9 +699,9 @@ __global__ __launch_bounds__(kThreads) void vocab_sample_kernel(VocabSampleArgs 
     if (wave == 0) {
         uint32_t number = 0, key = 0, flag = 0;
         if (lane < a.chunks) {
-            number = load_device(heads + lane * 4);
-            key = load_device(heads + lane * 4 + 1);
-            flag = load_device(heads + lane * 4 + 2);
+            number = load_device(heads + lane * kSampleHead);
+            key = load_device(heads + lane * kSampleHead + 1);
+            flag = load_device(heads + lane * kSampleHead + 2);
         }
         const uint64_t sum = wave_scan_u64((uint64_t)min(number, (uint32_t)a.list_words));
         if (lane < a.chunks) {
@@ -770,13 +789,13 @@ __global__ __launch_bounds__(kThreads) void vocab_sample_kernel(VocabSampleArgs 
                 }
             }
         } else {
-            each_column<TYPE>(logits, a.width, [&](uint32_t key) { add<TYPE>(s, weights, tally, key, 1u); });
+            each_column<TYPE>(logits, 0, a.width, a.width, [&](int, uint32_t key) { add<TYPE>(s, weights, tally, key, 1u); });
         }
         __syncthreads();
         choice = choose<TYPE>(s, weights, tally, r, a.width, [&](auto&& f) {
             if (whole) each_item([&](int, uint32_t v) { f(v & 0xffff0000u, v & 0xffffu); });
-            else each_column<TYPE>(logits, a.width, [&](uint32_t key) { f(key, 1u); });
-        });
+            else each_column<TYPE>(logits, 0, a.width, a.width, [&](int, uint32_t key) { f(key, 1u); });
+        }, 0);
     } else if (whole) {
         // one item per chunk: its largest (two for +0 and -0)
         each_listed(0, [&](int c, int i, uint32_t v) { s.items[s.starts[c] + i] = v; });
@@ -801,18 +820,20 @@ __global__ __launch_bounds__(kThreads) void vocab_sample_kernel(VocabSampleArgs 
 }
 
 // ---------------------------------------------------------------------------
-// 32-bit logits: a workgroup per row, the searches over the columns.
+// 32-bit logits: nearly every column a logit of its own.  A first launch takes
+// the chunks' largest, so that the second can weigh its columns against the
+// row's: each chunk's masses by the keys' first 12 bits, joined by the row's last
+// workgroup to arrive, which gathers the columns of the bin in which a search
+// ends (a scan of the row) and finishes the search among those.
 // ---------------------------------------------------------------------------
-__global__ __launch_bounds__(kThreads) void vocab_sample_f32_kernel(VocabSampleArgs a) {
-    __shared__ Search<2> s;
+__global__ __launch_bounds__(kThreads) void vocab_top_f32_kernel(VocabSampleArgs a) {
     __shared__ uint32_t wave_top[kWaves], wave_bad[kWaves];
-    __shared__ Row r;
-    const int row = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const int row = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     if (row >= (a.live_count ? *a.live_count : a.live_rows)) return;
-    const uint8_t* logits = row_of<2>(a, row);
-    if (t == 0) r.read(a, row);
+    const int begin = chunk * a.chunk, end = min(a.width, begin + a.chunk);
     uint32_t top = 0, bad = 0;
-    each_column<2>(logits, a.width, [&](uint32_t key) {
+    each_column<2>(row_of<2>(a, row), begin, end, a.width, [&](int, uint32_t key) {
         bad |= key >= Limits<2>::kInf || key < Limits<2>::kNegInf;
         top = max(top, key);
     });
@@ -823,33 +844,153 @@ __global__ __launch_bounds__(kThreads) void vocab_sample_f32_kernel(VocabSampleA
         wave_bad[wave] = bad;
     }
     __syncthreads();
+    if (t >= 64) return;
     top = wave_max_u32(lane < kWaves ? wave_top[lane] : 0);
     bad = __ballot(lane < kWaves && wave_bad[lane]) != 0;
-    if (bad || top <= Limits<2>::kNegInf || !r.admitted()) {
-        refuse(a, row);
+    if (t == 0) {
+        uint32_t* head = a.heads + ((int64_t)row * a.chunks + chunk) * kSampleHead;
+        head[0] = top;
+        head[1] = bad;
+    }
+}
+
+__global__ __launch_bounds__(kThreads) void vocab_sample_f32_kernel(VocabSampleArgs a) {
+    __shared__ Search<2> s;
+    __shared__ uint32_t row_top, row_bad, listed, last;
+    __shared__ Row r;
+    constexpr int kPer = Search<2>::kPer;
+    const int row = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    if (row >= (a.live_count ? *a.live_count : a.live_rows)) return;
+    const uint8_t* logits = row_of<2>(a, row);
+    uint32_t* const heads = a.heads + (int64_t)row * a.chunks * kSampleHead;
+    if (wave == 0) {
+        if (t == 0) {
+            r.read(a, row);
+            listed = 0;
+        }
+        const uint32_t key = lane < a.chunks ? heads[lane * kSampleHead] : 0;
+        const uint32_t bad = lane < a.chunks ? heads[lane * kSampleHead + 1] : 0;
+        const uint32_t top = wave_max_u32(key);
+        const bool any = __ballot(bad != 0) != 0;
+        if (t == 0) {
+            row_top = top;
+            row_bad = any;
+        }
+    }
+    clear<2>(s);
+    __syncthreads();
+    const uint32_t top = row_top;
+    if (row_bad || top <= Limits<2>::kNegInf || !r.admitted()) {
+        if (chunk == 0) refuse(a, row);
         return;
     }
     Choice choice = {top, 1, 0};
-    if (r.temperature > 0.f) {
-        clear<2>(s);
-        __syncthreads();
-        const Weights<2> weights(s.table, top, r);
-        Tally tally;
-        each_column<2>(logits, a.width, [&](uint32_t key) { add<2>(s, weights, tally, key, 1u); });
-        __syncthreads();
-        choice = choose<2>(s, weights, tally, r, a.width, [&](auto&& f) {
-            each_column<2>(logits, a.width, [&](uint32_t key) { f(key, 1u); });
-        });
+    if (!(r.temperature > 0.f)) {
+        if (chunk == 0) locate<2, 4>(s, a, row, logits, 0, a.width, r, top, choice);
+        return;
     }
-    locate<2, 8>(s, a, row, logits, 0, a.width, r, top, choice);
+    const Weights<2> weights(s.table, top, r);
+    Tally tally;
+    const int begin = chunk * a.chunk, end = min(a.width, begin + a.chunk);
+    each_column<2>(logits, begin, end, a.width, [&](int, uint32_t key) { add<2>(s, weights, tally, key, 1u); });
+    __syncthreads();
+    if (a.chunks > 1) {
+        // the chunk's bins that hold anything: bin, columns, mass
+        uint32_t* const list = a.lists + ((int64_t)row * a.chunks + chunk) * a.list_words;
+        uint64_t likely;
+        before_wave(lane_u64(wave_scan_u64(tally.likely), 63), s.sums[2], lane, wave, likely);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const int b = t + i * kThreads;
+            const uint32_t number = s.count[b];
+            const uint64_t m = s.mass[b];
+            if (!number) continue;
+            const uint32_t at = atomicAdd(&listed, 1u) * 4;
+            store_device(list + at, (uint32_t)b);
+            store_device(list + at + 1, number);
+            store_device(list + at + 2, (uint32_t)m);
+            store_device(list + at + 3, (uint32_t)(m >> 32));
+        }
+        __syncthreads();
+        if (t == 0) {
+            store_device(heads + chunk * kSampleHead + 2, listed);
+            store_device(heads + chunk * kSampleHead + 3, (uint32_t)likely);
+            store_device(heads + chunk * kSampleHead + 4, (uint32_t)(likely >> 32));
+        }
+        if (!arrive_last(a.counters + row, a.chunks, &last)) return;
+        if (t == 0) store_device(a.counters + row, 0u);
+        // this workgroup searches the row: the others' bins on top of its own
+        if (wave == 0) {
+            if (lane < a.chunks) {
+                const uint32_t* h = heads + lane * kSampleHead;
+                s.held[lane] = lane == chunk ? 0 : (int)load_device(h + 2);
+                tally.likely = (uint64_t)load_device(h + 4) << 32 | load_device(h + 3);
+            } else {
+                tally.likely = 0;
+            }
+        } else {
+            tally.likely = 0;
+        }
+        __syncthreads();
+        for (int c = 0; c < a.chunks; ++c) {
+            const uint32_t* from = a.lists + ((int64_t)row * a.chunks + c) * a.list_words;
+            for (int i = t; i < s.held[c]; i += kThreads) {
+                const uint32_t b = load_device(from + 4 * i), number = load_device(from + 4 * i + 1);
+                const uint64_t m = (uint64_t)load_device(from + 4 * i + 3) << 32 | load_device(from + 4 * i + 2);
+                atomicAdd(&s.count[b], number);
+                atomicAdd(&s.mass[b], (unsigned long long)m);
+            }
+        }
+        __syncthreads();
+    }
+    choice = choose<2>(s, weights, tally, r, a.width, [&](uint32_t digit) {
+        __syncthreads();
+        if (t == 0) s.gathered = 0;
+        __syncthreads();
+        each_column<2>(logits, 0, a.width, a.width, [&](int c, uint32_t key) {
+            if (key >> Search<2>::kShift != digit) return;
+            const uint32_t at = atomicAdd(&s.gathered, 1u);
+            if (at >= Search<2>::kCached) return;
+            s.items[2 * at] = key;
+            s.items[2 * at + 1] = (uint32_t)c;
+        });
+        __syncthreads();
+    }, [&](auto&& f) { each_column<2>(logits, 0, a.width, a.width, [&](int, uint32_t key) { f(key); }); });
+    // the last search's columns are gathered: where the key is one of them
+    // only, that is the token
+    const int gathered = (int)s.gathered;
+    if (t == 0) listed = 0;
+    __syncthreads();
+    if (gathered <= Search<2>::kCached) {
+        for (int i = t; i < gathered; i += kThreads)
+            if (s.items[2 * i] == choice.key) {
+                const uint32_t at = atomicAdd(&listed, 1u);
+                if (at == 0) s.starts[0] = (int)s.items[2 * i + 1];
+            }
+        __syncthreads();
+        if (listed == 1) {
+            if (t == 0) publish<2>(a, row, r, top, choice, s.starts[0]);
+            return;
+        }
+    }
+    locate<2, 4>(s, a, row, logits, 0, a.width, r, top, choice);
 }
 
 }  // namespace
 
 hipError_t launch_vocab_sample(const VocabSampleArgs& a, hipStream_t s) {
-    if (a.dtype == 2) vocab_sample_f32_kernel<<<a.rows, kThreads, 0, s>>>(a);
-    else if (a.dtype == 1) vocab_sample_kernel<1><<<a.rows * a.chunks, kThreads, 0, s>>>(a);
-    else vocab_sample_kernel<0><<<a.rows * a.chunks, kThreads, 0, s>>>(a);
+    const int grid = a.rows * a.chunks;
+    if (a.dtype == 2) {
+        vocab_top_f32_kernel<<<grid, kThreads, 0, s>>>(a);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+        vocab_sample_f32_kernel<<<grid, kThreads, 0, s>>>(a);
+    } else if (a.dtype == 1) {
+        vocab_sample_kernel<1><<<grid, kThreads, 0, s>>>(a);
+    } else {
+        vocab_sample_kernel<0><<<grid, kThreads, 0, s>>>(a);
+    }
     return hipGetLastError();
 }
 
