@@ -115,6 +115,33 @@ def ptr(tensor) -> int | None:
 
 
 def stream_of(device) -> int:
+    """The current stream's handle on a device (an index is taken fastest:
+    1.4 us of the host's time through a stream object, 0.2 by the raw handle)."""
     import torch
 
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    if raw is not None and isinstance(device, int):
+        return raw(device)
     return int(torch.cuda.current_stream(device).cuda_stream)
+
+
+class on_device:
+    """Like torch.cuda.device(index), but nothing where that device is current
+    already (1.5 us of the host's time per launch)."""
+
+    __slots__ = ("index", "guard")
+
+    def __init__(self, index: int):
+        self.index, self.guard = index, None
+
+    def __enter__(self):
+        import torch
+
+        if torch.cuda.current_device() != self.index:
+            self.guard = torch.cuda.device(self.index)
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+        return False

@@ -854,6 +854,38 @@ __global__ __launch_bounds__(kThreads) void vocab_top_f32_kernel(VocabSampleArgs
     }
 }
 
+// The columns whose keys begin with the digit, into s.items.  The logits' own
+// first bits are compared, a word's four at a time: forming every column's key
+// cost the scan a sixth more (it is bound by what one CU reads).
+__device__ __forceinline__ void gather(Search<2>& s, const uint8_t* logits, int width, uint32_t digit) {
+    constexpr int kShift = Search<2>::kShift, kAhead = 4;
+    const uint32_t first = digit >> 11 ? digit ^ 0x800u : ~digit & 0xfffu;
+    for (int c0 = (int)threadIdx.x * 4; c0 < width; c0 += kAhead * kThreads * 4) {
+        uint4 word[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) word[i] = load_word<2>(logits, c0 + i * kThreads * 4, width);
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const int c = c0 + i * kThreads * 4;
+            if (c >= width) break;
+            const uint4 v = place_word<2>(word[i], c, width);
+            bool any = v.x >> kShift == first || v.y >> kShift == first || v.z >> kShift == first || v.w >> kShift == first;
+            // -0 begins as the negative numbers do and has +0's key
+            if (first == 0) any |= v.x == 0x80000000u || v.y == 0x80000000u || v.z == 0x80000000u || v.w == 0x80000000u;
+            if (!any) continue;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t key = word_key<2>(v, j);
+                if (key >> kShift != digit) continue;
+                const uint32_t at = atomicAdd(&s.gathered, 1u);
+                if (at >= Search<2>::kCached) continue;
+                s.items[2 * at] = key;
+                s.items[2 * at + 1] = (uint32_t)(c + j);
+            }
+        }
+    }
+}
+
 __global__ __launch_bounds__(kThreads) void vocab_sample_f32_kernel(VocabSampleArgs a) {
     __shared__ Search<2> s;
     __shared__ uint32_t row_top, row_bad, listed, last;
@@ -948,13 +980,7 @@ __global__ __launch_bounds__(kThreads) void vocab_sample_f32_kernel(VocabSampleA
         __syncthreads();
         if (t == 0) s.gathered = 0;
         __syncthreads();
-        each_column<2>(logits, 0, a.width, a.width, [&](int c, uint32_t key) {
-            if (key >> Search<2>::kShift != digit) return;
-            const uint32_t at = atomicAdd(&s.gathered, 1u);
-            if (at >= Search<2>::kCached) return;
-            s.items[2 * at] = key;
-            s.items[2 * at + 1] = (uint32_t)c;
-        });
+        gather(s, logits, a.width, digit);
         __syncthreads();
     }, [&](auto&& f) { each_column<2>(logits, 0, a.width, a.width, [&](int, uint32_t key) { f(key); }); });
     // the last search's columns are gathered: where the key is one of them

@@ -196,8 +196,9 @@ class PackedOperatorBinding:
         self.validate_operands()
         self._ordinal += 1
         first = self.output[0] if isinstance(self.output, tuple) else self.output
-        with torch.cuda.device(first.device):
-            stream = _native.stream_of(first.device)
+        index = first.device.index
+        with _native.on_device(index):
+            stream = _native.stream_of(index)
             for item in self._launches:
                 item(stream)
         return self._ordinal

@@ -459,7 +459,7 @@ class VocabSamplingPlan:
         self.valid = torch.empty(rows, dtype=torch.bool, device=dev)
         self.logprobs = torch.empty(rows, dtype=torch.float32, device=dev)
         self.workspace = torch.zeros(nbytes, dtype=torch.uint8, device=dev)
-        self._fixed = tuple(_fingerprint(t) for t in operands)
+        self._fixed = tuple((t.shape, t.stride(), t.dtype) for t in operands)
         self._index = dev.index
         self._head = (_CANDIDATE_DTYPES[logits.dtype], max(logits.stride(0), logits.shape[1]), rows, self.width)
 
@@ -477,9 +477,10 @@ class VocabSamplingPlan:
             if type(live_rows) is not int or not 0 <= live_rows <= self.rows:
                 raise ValueError(f"live row count must be an int in 0..{self.rows} or a device int32 tensor")
             live = live_rows
-        if tuple(_fingerprint(t) for t in (self.logits, *self.parameters)) != self._fixed:
-            raise ValueError("sampling operands changed after binding")
-        with torch.cuda.device(self._index):
+        for t, (shape, stride, dtype) in zip((self.logits, *self.parameters), self._fixed):
+            if t.shape != shape or t.stride() != stride or t.dtype is not dtype:
+                raise ValueError("sampling operands changed after binding")
+        with _native.on_device(self._index):
             _native.call("cubic_vocab_sample", self.logits.data_ptr(), *self._head, live, live_ptr,
                          *(t.data_ptr() for t in self.parameters), self.tokens.data_ptr(),
                          self.valid.data_ptr(), self.logprobs.data_ptr(), self.workspace.data_ptr(),
