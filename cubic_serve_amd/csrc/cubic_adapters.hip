@@ -3,9 +3,9 @@
 //   t[i, :]   = A_e x[i, :]                         e = row_slots[i], rank r_e
 //   y[i, :]   = round16(base[i, :] + s_e B_e t[i, :])
 //
-// for up to kMaxGemmMembers projections that share x, in two launches: the
-// down kernel writes t as binary32 partial sums over K partitions, the up
-// kernel adds the partitions and finishes the rows.
+// for up to kMaxGemmMembers projections that share x.  Few rows: one launch
+// (adapter_row_kernel).  Else two: a down kernel writes t as binary32 partial
+// sums over K partitions, an up kernel adds the partitions and finishes the rows.
 //
 // Rows come in any order.  A tile of consecutive rows is walked once per
 // distinct adapter in it (a ballot over the tile's slots finds the rows of
@@ -16,7 +16,8 @@
 //
 // Arithmetic order: K partitions of kDownK columns, each a sum of four quarters
 // (0 + 1) + (2 + 3), partitions added in ascending order; then the rank in steps
-// of 32.  Nothing of it depends on m, on the tile or on the other rows, so a row's result is the same bit for bit whichever batch it is in.
+// of 32.  Nothing of it depends on m, on the kernel, on the tile or on the
+// other rows, so a row's result is the same bit for bit whichever batch it is in.
 #include "cubic_gemm_common.h"
 
 namespace cubic {
@@ -59,10 +60,11 @@ __device__ __forceinline__ int tile_slots(const AdapterArgs& a, int row0, int ro
 // once.  MFMA operands straight from memory: the first is A (its rows are the
 // ranks), the second x, so a lane ends with four consecutive ranks of one row.
 // x goes out ahead of A in runs of four steps (256 bytes of every row).
-template <bool F16, int MT, int RT>
+// behind() runs once they have, before any is waited for.
+template <bool F16, int MT, int RT, typename Behind>
 __device__ __forceinline__ void quarter_product(__amdgpu_buffer_rsrc_t x, const uint32_t (&xoff)[MT],
                                                 __amdgpu_buffer_rsrc_t d, const uint32_t (&doff)[RT], int k0,
-                                                int k, floatx4_t (&acc)[MT][RT]) {
+                                                int k, floatx4_t (&acc)[MT][RT], Behind&& behind) {
     uint4 xf[kSteps][MT], df[kSteps][RT];
 #pragma unroll
     for (int h = 0; h < kSteps; h += 4) {
@@ -81,6 +83,8 @@ __device__ __forceinline__ void quarter_product(__amdgpu_buffer_rsrc_t x, const 
                 df[s][t] = load16(d, kk < k && doff[t] != kOutside ? doff[t] + (uint32_t)kk * 2 : kOutside);
             }
     }
+    __builtin_amdgcn_sched_barrier(0);
+    behind();
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int i = 0; i < MT; ++i)
@@ -141,7 +145,7 @@ __global__ __launch_bounds__(kThreads) void adapter_down_kernel(AdapterArgs a) {
         }
         const auto d = buffer(mb.down + (int64_t)e * mb.max_rank * a.k, (int64_t)mb.max_rank * a.k * 2);
         floatx4_t acc[MT][RT];
-        quarter_product<F16, MT, RT>(x, xoff, d, doff, k0, a.k, acc);
+        quarter_product<F16, MT, RT>(x, xoff, d, doff, k0, a.k, acc, [] {});
         // (0 + 1) + (2 + 3); the walk's next turn writes red only after the
         // last barrier, which follows every read of it
         if (wave & 1)
@@ -414,6 +418,120 @@ __global__ __launch_bounds__(kThreads) void adapter_up_kernel(AdapterArgs a) {
     }
 }
 
+// ---------------------------------------------------------------------------
+// Few rows, ranks of at most 16: both products in one launch.  Workgroup: one adapter's rows of a
+// 16-row tile x a column chunk; its sixteen waves make t, a quarter of a K
+// partition each, in LDS, then 64 columns of y per turn, whose B and base
+// (TURNS turns of them) are on the way since A is.  Every column chunk reads A
+// again.  What bounds it is the chain of dependent loads (slot, A and rank) and
+// what one CU takes in (30 - 60 GB/s); two launches have that chain twice: q k v
+// of 64 rows, each its own adapter, rank 16: 15.9 us in two, 12.5 in one.  B's
+// rows are permuted so that a lane ends with eight consecutive columns of one
+// row: of two 16-row tiles, row 4 p + s of tile u stands for column 8 p + 4 u + s.
+// ---------------------------------------------------------------------------
+template <bool F16, int TURNS, bool VEC>
+__global__ __launch_bounds__(kAdapterRowWaves * 64) void adapter_row_kernel(AdapterArgs a) {
+    constexpr int kW = kAdapterRowWaves, kTurn = kAdapterRowTurn;
+    __shared__ int slots_lds[64];
+    __shared__ floatx4_t quarters[kW][64];
+    const AdapterMember& mb = a.member[blockIdx.z];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 15, q = lane >> 4;
+    const int n = mb.n, max_rank = mb.max_rank;
+    const int row0 = (int)(blockIdx.x / a.down_groups) * 16;
+    const int c_begin = blockIdx.y * a.chunk_cols + wave * kTurn, c_end = min(n, (int)(blockIdx.y + 1) * a.chunk_cols);
+    if ((int)blockIdx.y * a.chunk_cols >= n) return;
+    const int slot = tile_slots(a, row0, 16, slots_lds);
+    // this workgroup's adapter: number blockIdx.x % groups of the tile's
+    uint64_t left = __ballot(slot != -1), mine = 0;
+    int lead = 0, e = 0;
+    for (int order = (int)(blockIdx.x % a.down_groups); order >= 0; --order) {
+        if (!left) return;
+        lead = __builtin_ctzll(left);
+        e = __builtin_amdgcn_readlane(slot, lead);
+        mine = __ballot(slot == e);
+        left &= ~mine;
+    }
+    const bool in_place = mb.base == mb.y;
+    if (e < 0 && in_place) return;
+    const int rank = e >= 0 ? min(mb.ranks[e], max_rank) : 0;
+    const float scale = e >= 0 ? mb.scales[e] : 0.f;
+    const int es = max(e, 0), parts = 4 * a.split;
+    const uint32_t ldbase = (uint32_t)mb.ldbase * 2, ldy = (uint32_t)mb.ldy * 2;  // bytes
+    const auto base = buffer(mb.base + (int64_t)row0 * mb.ldbase, 15 * (int64_t)ldbase + 2 * n);
+    const auto y = buffer(mb.y + (int64_t)row0 * mb.ldy, 15 * (int64_t)ldy + 2 * n);
+    const auto up = buffer(mb.up + (int64_t)es * n * max_rank, (int64_t)n * max_rank * 2);
+    const bool own = (mine >> col) & 1;
+    uint4 b[TURNS][kTurn / 16], in[TURNS][kTurn / 32];
+    auto fetch = [&](int c0) {
+#pragma unroll
+        for (int v = 0; v < TURNS; ++v)
+#pragma unroll
+            for (int g = 0; g < kTurn / 32; ++g) {
+                const int first = c0 + v * kW * kTurn + 32 * g;
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const int c = first + 8 * (col >> 2) + 4 * u + (col & 3);
+                    b[v][2 * g + u] = load16(up, q * 8 < rank && c < c_end ? (uint32_t)(c * max_rank + q * 8) * 2 : kOutside);
+                }
+                const int cy = first + 8 * q;
+                in[v][g] = load8<VEC>(base, own && cy < c_end ? col * ldbase : kOutside, cy, n);
+            }
+    };
+    {
+        const int rows = min(16, a.m - row0);
+        const auto x = buffer(a.x + (int64_t)row0 * a.ldx, ((int64_t)(rows - 1) * a.ldx + a.k) * 2);
+        const auto d = buffer(mb.down + (int64_t)es * max_rank * a.k, e >= 0 ? (int64_t)max_rank * a.k * 2 : 0);
+        const uint32_t xoff[1] = {(uint32_t)(own ? col : lead) * (uint32_t)(a.ldx * 2)};
+        // (not waiting for the rank: what lies past it split_row leaves out)
+        const uint32_t doff[1] = {col < max_rank ? (uint32_t)col * (uint32_t)(a.k * 2) : kOutside};
+        floatx4_t acc[1][1];
+        if (wave < parts) {
+            quarter_product<F16, 1, 1>(x, xoff, d, doff, wave * kQuarter + q * 8, a.k, acc, [&] { fetch(c_begin); });
+            quarters[wave][lane] = acc[0][0];
+        } else {
+            fetch(c_begin);
+        }
+    }
+    __syncthreads();
+    // t of row col, ranks 8 q .. 8 q + 7 (q < 2): lane 16 (rank / 4) + col holds
+    // four ranks; quarters and partitions in order
+    uint4 hi[1], lo[1];
+    floatx4_t t8[1][2];
+    t8[0][0] = t8[0][1] = floatx4_t{0.f, 0.f, 0.f, 0.f};
+    if (q < 2)
+        for (int j = 0; j < parts; j += 4)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const int at = 16 * (2 * q + c) + col;
+                t8[0][c] += (quarters[j][at] + quarters[j + 1][at]) + (quarters[j + 2][at] + quarters[j + 3][at]);
+            }
+    const float back = split_row<F16, 1>(t8, rank, scale, q, hi, lo);
+    if (rank <= 0 && in_place) return;
+    for (int c0 = c_begin; c0 < c_end; c0 += TURNS * kW * kTurn) {
+        if (c0 != c_begin) fetch(c0);
+#pragma unroll
+        for (int v = 0; v < TURNS; ++v)
+#pragma unroll
+            for (int g = 0; g < kTurn / 32; ++g) {
+                if (rank > 0) {
+                    floatx4_t acc[2];
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        acc[u] = mfma16<F16>(b[v][2 * g + u], lo[0], floatx4_t{0.f, 0.f, 0.f, 0.f});
+                        acc[u] = mfma16<F16>(b[v][2 * g + u], hi[0], acc[u]) * back;
+                    }
+                    in[v][g].x = add_pair<F16>(in[v][g].x, acc[0][0], acc[0][1]);
+                    in[v][g].y = add_pair<F16>(in[v][g].y, acc[0][2], acc[0][3]);
+                    in[v][g].z = add_pair<F16>(in[v][g].z, acc[1][0], acc[1][1]);
+                    in[v][g].w = add_pair<F16>(in[v][g].w, acc[1][2], acc[1][3]);
+                }
+                const int cy = c0 + v * kW * kTurn + 32 * g + 8 * q;
+                store8<VEC>(y, own && cy < c_end ? col * ldy : kOutside, cy, n, in[v][g]);
+            }
+    }
+}
+
 template <bool F16, int MT, int RT>
 void start_down(const AdapterArgs& a, hipStream_t s) {
     const dim3 grid((a.m + 16 * MT - 1) / (16 * MT) * a.down_groups * a.split,
@@ -441,8 +559,20 @@ void start_up_rows(const AdapterArgs& a, hipStream_t s) {
     else start_up<F16, KS, 4>(a, s);
 }
 
+template <bool F16, int TURNS, bool VEC>
+void start_row(const AdapterArgs& a, hipStream_t s) {
+    const dim3 grid((a.m + 15) / 16 * a.down_groups, a.chunks, a.members);
+    adapter_row_kernel<F16, TURNS, VEC><<<grid, kAdapterRowWaves * 64, 0, s>>>(a);
+}
+
 template <bool F16>
 hipError_t start(const AdapterArgs& a, hipStream_t s) {
+    if (a.fused) {
+        if (!a.vectors) start_row<F16, 1, false>(a, s);
+        else if (a.chunk_cols <= kAdapterRowWaves * kAdapterRowTurn) start_row<F16, 1, true>(a, s);
+        else start_row<F16, 2, true>(a, s);
+        return hipGetLastError();
+    }
     if (a.down_rows == 1) start_down_tiles<F16, 1>(a, s);
     else start_down_tiles<F16, 2>(a, s);
     const hipError_t e = hipGetLastError();

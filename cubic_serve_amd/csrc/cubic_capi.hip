@@ -863,6 +863,28 @@ int cubic_adapters(const void* x, int64_t ldx, const int32_t* row_slots, int64_t
         a.chunk_end[j] = (int)chunks;
     }
     a.chunks = (int)chunks;
+    // One launch where ranks are at most 16, K at most four partitions (a quarter
+    // per wave) and every row's column chunks together at most one workgroup per
+    // CU, the rows all with adapters of their own.  In a replayed graph, one
+    // launch and two: q k v (K = 4096) m = 1 8.7 and 7.9 us (a launch of the host's
+    // less: 11.4 -> 9.1 eagerly), 16 10.0 and 11.8, 64 12.5 and 15.9 (all with one of
+    // four adapters: 10.9 and 9.1); 2 x 12288 columns m = 32 14.5 and 18.6.  With
+    // more workgroups than CUs, 2 x 12288 m = 64 at 2048 columns: 31.0 and 28.8; with
+    // more K, 12288 -> 4096 m = 64: 22 and 16.
+    if (a.rank_tiles == 1 && a.split <= cubic::kAdapterRowWaves / 4) {
+        for (int cols = 512; cols <= 4096 && !a.fused; cols *= 2) {
+            int64_t all = 0, most = 0;
+            for (int j = 0; j < members; ++j) {
+                all += ceil_div(ns[j], cols);
+                most = std::max(most, ceil_div(ns[j], cols));
+            }
+            if (m * all > 256) continue;
+            a.fused = 1;
+            a.chunk_cols = cols;
+            a.chunks = (int)most;
+            a.down_groups = (int)std::min<int64_t>(16, m);
+        }
+    }
     if (items * chunks >= INT_MAX) return fail(CUBIC_ENOTSUP, "adapter extents too large");
     return hip_status(cubic::launch_adapters(a, (hipStream_t)stream), "cubic_adapters launch");
 }

@@ -281,6 +281,9 @@ hipError_t launch_vocab_sample(const VocabSampleArgs& a, hipStream_t s);
 constexpr int kAdapterDownK = 1024;  // columns of x per K partition
 constexpr int kAdapterUpTurn = 128;  // columns of y per wave and turn
 constexpr int kMaxAdapterRank = 256;
+// one-launch kernel: waves (a quarter of a K partition each) and columns of y
+// per wave and turn
+constexpr int kAdapterRowWaves = 16, kAdapterRowTurn = 64;
 struct AdapterMember {
     const uint16_t* down;         // [slots, max_rank, k]
     const uint16_t* up;           // [slots, n, max_rank]
@@ -302,6 +305,7 @@ struct AdapterArgs {
     int split, width;             // K partitions; ranks of all members, each rounded up to 16
     int rank_tiles;               // ceil(largest max_rank / 16)
     int vectors;                  // every member: 16-byte base and output accesses
+    int fused;                    // one launch (few rows); chunks: the widest member's
     int down_rows, up_rows;       // 16-row tiles per workgroup: 1 or 2; 1 or 4
     int down_groups, up_groups;   // workgroups that share a tile's distinct adapters
     int chunks, chunk_cols;       // column chunks of all members; columns per chunk
