@@ -41,6 +41,11 @@ __device__ __forceinline__ uint4 load16(__amdgpu_buffer_rsrc_t r, uint32_t byte_
     return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)byte_offset, 0, 0));
 }
 
+typedef __attribute__((address_space(3))) void lds_void_t;
+// s_waitcnt immediate: at most n vector-memory accesses in flight, no LDS access.
+constexpr int vmcnt_and_lds(int n) { return (n & 0xF) | (0x7 << 4) | ((n >> 4) << 14); }
+constexpr int kDownTileRanks = 8;  // 16-rank blocks of the prompts' down kernel
+
 // The tile's adapter slots, one per lane (-1: past the batch, kNone: no
 // adapter), the same in every wave: one wave reads them, so that waves cannot
 // disagree on the walk (and its barriers) if the caller rewrites them meanwhile.
@@ -182,6 +187,156 @@ __global__ __launch_bounds__(kThreads) void adapter_down_kernel(AdapterArgs a) {
 }
 
 // ---------------------------------------------------------------------------
+// t = A x for prompts: the same sums over tiles of 64 rows and 128 ranks, x and A
+// staged through LDS by direct loads, blocks of 64 columns, three deep (72 KB:
+// two workgroups per CU).  The kernel above has each wave read A from the caches for
+// its own 32 rows: at K = 8192, rank 128, 4096 rows that is 0.4 GB into the CUs
+// beside 0.07 from memory.  Here waves share the ranks in halves and the rows in
+// halves, and A is read once per 64 rows: 54 -> 27.5 us with one adapter, 57 -> 52
+// with 24 requests (a tile on a boundary is done once per adapter).  Four blocks
+// make a quarter; quarters add as above, bit for bit.  LDS image of a 16-row block:
+// 16-byte chunk c of row r in slot 8 r + (c ^ (r / 2) mod 8), so that the 16 rows of
+// a fragment read lie in distinct banks.
+// ---------------------------------------------------------------------------
+template <bool F16>
+__global__ __launch_bounds__(kThreads) void adapter_down_tile_kernel(AdapterArgs a) {
+    constexpr int RT = kDownTileRanks, S = 3;  // two blocks in flight; 72 KB: two workgroups per CU
+    constexpr int kBlock = 64, kBlocks = kDownK / kBlock, kBytes = 16 * kBlock * 2;
+    constexpr int kStage = (4 + RT) * kBytes;  // four row blocks, RT rank blocks
+    constexpr int kDown = RT / 2;              // 1 KB loads of A per wave and stage; two of x
+    constexpr int RW = RT / 2;                 // rank blocks per wave; two row blocks
+    __shared__ int slots_lds[64];
+    __shared__ __attribute__((aligned(16))) uint8_t stage[S * kStage];
+    const AdapterMember& mb = a.member[blockIdx.z];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 15, q = lane >> 4;
+    const int wr = wave >> 1, wc = wave & 1;
+    const int part = blockIdx.x % a.split, row0 = (int)(blockIdx.x / a.split) * 64;
+    const int rank0 = blockIdx.y * RT * 16;
+    if (rank0 >= mb.max_rank) return;
+    const int slot = tile_slots(a, row0, 64, slots_lds);
+
+    const int rows = min(64, a.m - row0);
+    const __amdgpu_buffer_rsrc_t x = buffer(a.x + (int64_t)row0 * a.ldx, ((int64_t)(rows - 1) * a.ldx + a.k) * 2);
+    // this lane's place in a 1 KB load: rows 8 i + lane / 8 of a block
+    const int dr = lane >> 3;
+    auto chunk_of = [&](int r) { return (lane & 7) ^ (r >> 1 & 7); };
+
+    uint64_t left = __ballot(slot >= 0);
+    while (left) {
+        const int e = __builtin_amdgcn_readlane(slot, __builtin_ctzll(left));
+        const uint64_t mine = __ballot(slot == e);
+        left &= ~mine;
+        const int rank = min(mb.ranks[e], mb.max_rank);
+        const __amdgpu_buffer_rsrc_t d = buffer(mb.down + (int64_t)e * mb.max_rank * a.k, (int64_t)mb.max_rank * a.k * 2);
+        // x: wave w's loads are the two halves of row block w; a block without a
+        // row of this adapter is not read
+        const bool need = (mine >> (16 * wave) & 0xffff) != 0;
+        uint32_t xoff[2], doff[kDown];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) xoff[i] = need ? (uint32_t)(16 * wave + 8 * i + dr) * (uint32_t)(a.ldx * 2) : kOutside;
+#pragma unroll
+        for (int i = 0; i < kDown; ++i) {
+            const int r = rank0 + 8 * (wave * kDown + i) + dr;
+            doff[i] = r < rank ? (uint32_t)r * (uint32_t)(a.k * 2) : kOutside;
+        }
+        // K block b into stage b % S; past the partition: reads nothing, writes 0
+        auto issue = [&](int b) {
+            auto* to = (__attribute__((address_space(3))) uint8_t*)(void*)(stage + b % S * kStage);
+            // (named operands: the host pass drops a kernel that passes array elements here)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int kk = part * kDownK + b * kBlock + chunk_of(8 * i + dr) * 8;
+                const uint32_t off = b < kBlocks && kk < a.k && xoff[i] != kOutside ? xoff[i] + (uint32_t)kk * 2 : kOutside;
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(x, (lds_void_t*)(to + (2 * wave + i) * 1024), 16, off, 0, 0, 0);
+            }
+#pragma unroll
+            for (int i = 0; i < kDown; ++i) {
+                const int at = wave * kDown + i;  // half block of A
+                const int kk = part * kDownK + b * kBlock + chunk_of(8 * (at & 1) + dr) * 8;
+                const uint32_t off = b < kBlocks && kk < a.k && doff[i] != kOutside ? doff[i] + (uint32_t)kk * 2 : kOutside;
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(d, (lds_void_t*)(to + 4 * kBytes + at * 1024), 16, off, 0, 0, 0);
+            }
+        };
+        floatx4_t sum[2][RW], even[2][RW], acc[2][RW];
+#pragma unroll
+        for (int b = 0; b < S - 1; ++b) issue(b);
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b) {
+            // this wave's loads of block b have landed (S - 2 younger blocks may
+            // be in flight); after the barrier every wave's have, and every wave
+            // is done with the stage that block b + S - 1 takes
+            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_waitcnt(vmcnt_and_lds((S - 2) * (2 + kDown)));
+            __builtin_amdgcn_s_barrier();
+            __builtin_amdgcn_sched_barrier(0);
+            issue(b + S - 1);
+            __builtin_amdgcn_sched_barrier(0);
+            const uint8_t* from = stage + b % S * kStage + col * 128;
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                const int at = ((4 * s + q) ^ (col >> 1)) * 16;
+                uint4 xf[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) xf[i] = *(const uint4*)(from + (2 * wr + i) * kBytes + at);
+#pragma unroll
+                for (int t = 0; t < RW; ++t) {
+                    const uint4 df = *(const uint4*)(from + (4 + wc * RW + t) * kBytes + at);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        if (b % 4 == 0 && s == 0) acc[i][t] = floatx4_t{0.f, 0.f, 0.f, 0.f};
+                        acc[i][t] = mfma16<F16>(df, xf[i], acc[i][t]);
+                    }
+                }
+            }
+            if (b % 4 == 3)  // a quarter is whole
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int t = 0; t < RW; ++t) {
+                        if (b % 8 == 3) even[i][t] = acc[i][t];
+                        else if (b == 7) sum[i][t] = even[i][t] + acc[i][t];
+                        else sum[i][t] += even[i][t] + acc[i][t];
+                    }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int r = 16 * (2 * wr + i) + col;
+            if (!((mine >> r) & 1)) continue;
+            float* out = a.partial + ((int64_t)part * a.m + row0 + r) * a.width + mb.rank0 + rank0 + 4 * q;
+#pragma unroll
+            for (int t = 0; t < RW; ++t) {
+                const int f = 16 * (wc * RW + t);
+                if (rank0 + f < mb.max_rank) *(floatx4_t*)(out + f) = sum[i][t];
+            }
+        }
+        // no load into LDS is left when the next adapter's, or the kernel's end, comes
+        __builtin_amdgcn_s_waitcnt(vmcnt_and_lds(0));
+        __syncthreads();
+    }
+}
+
+// t itself, the partitions added in ascending order, in place of the first: every
+// column chunk of the up kernel would read them all (8192 columns, 8 partitions:
+// 0.16 GB of partitions beside the 0.13 of base and y).
+__global__ __launch_bounds__(kThreads) void adapter_join_kernel(AdapterArgs a) {
+    const int64_t words = (int64_t)a.m * a.width;
+    const int64_t at = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * 4;
+    if (at >= words) return;
+    constexpr int kAhead = 8;
+    floatx4_t v = *(const floatx4_t*)(a.partial + at);
+    for (int part = 1; part < a.split; part += kAhead) {
+        floatx4_t in[kAhead];
+#pragma unroll
+        for (int p = 0; p < kAhead; ++p) in[p] = *(const floatx4_t*)(a.partial + at + min(part + p, a.split - 1) * words);
+#pragma unroll
+        for (int p = 0; p < kAhead; ++p)
+            if (part + p < a.split) v += in[p];
+    }
+    *(floatx4_t*)(a.partial + at) = v;
+}
+
+// ---------------------------------------------------------------------------
 // y = base + s B t.  A wave takes 16 rows x kTurn columns per turn; the four
 // waves of a workgroup stand side by side over columns (WR = 1: few rows) or
 // one below the other (WR = 4: they read the same B, which their CU's cache
@@ -251,6 +406,44 @@ __device__ __forceinline__ float split_row(const floatx4_t (&v)[KS][2], int rank
 #pragma unroll
     for (int s = 0; s < KS; ++s) split_parts<F16>(t[s], hi[s], lo[s]);
     return back;
+}
+
+// The parts of t of rows row0 .. row0 + 15 (this lane's: row0 + col, if own): the
+// partitions in ascending order, kParts requested together; what is not there
+// (another row, past the rank) reads as 0.
+template <bool F16, int KS>
+__device__ __forceinline__ float row_parts(const AdapterArgs& a, const AdapterMember& mb, int row0, bool own,
+                                           int rank, float scale, int col, int q, uint4 (&hi)[KS], uint4 (&lo)[KS]) {
+    constexpr int kParts = KS < 8 ? 8 / KS : 1;
+    uint32_t off[KS][2];
+    floatx4_t v[KS][2];
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const int f = s * 32 + q * 8 + 4 * c;
+            off[s][c] = own && f < rank ? (uint32_t)(col * a.width + mb.rank0 + f) * 4 : kOutside;
+            v[s][c] = floatx4_t{0.f, 0.f, 0.f, 0.f};
+        }
+    for (int part = 0; part < a.split; part += kParts) {
+        floatx4_t in[kParts][KS][2];
+#pragma unroll
+        for (int p = 0; p < kParts; ++p) {
+            const int64_t at = ((int64_t)min(part + p, a.split - 1) * a.m + row0) * a.width;
+            const auto buf = buffer(a.partial + at, part + p < a.split ? 16 * a.width * 4 : 0);
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) in[p][s][c] = __builtin_bit_cast(floatx4_t, load16(buf, off[s][c]));
+        }
+#pragma unroll
+        for (int p = 0; p < kParts; ++p)
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) v[s][c] += in[p][s][c];
+    }
+    return split_row<F16, KS>(v, rank, scale, q, hi, lo);
 }
 
 // Eight 16-bit values of a row at column c: one access, or (rows that are not
@@ -325,42 +518,7 @@ __global__ __launch_bounds__(kThreads) void adapter_up_kernel(AdapterArgs a) {
         if (rank <= 0 && in_place) continue;
         const float scale = e >= 0 ? mb.scales[e] : 0.f;
         uint4 hi[KS], lo[KS];
-        float back = 1.f;
-        {
-            // the partitions in ascending order, kParts requested together;
-            // what is not there (another row, past the rank) reads as 0
-            constexpr int kParts = KS < 8 ? 8 / KS : 1;
-            const bool own = (mine >> col) & 1;
-            uint32_t off[KS][2];
-            floatx4_t v[KS][2];
-#pragma unroll
-            for (int s = 0; s < KS; ++s)
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const int f = s * 32 + q * 8 + 4 * c;
-                    off[s][c] = own && f < rank ? (uint32_t)(col * a.width + mb.rank0 + f) * 4 : kOutside;
-                    v[s][c] = floatx4_t{0.f, 0.f, 0.f, 0.f};
-                }
-            for (int part = 0; part < a.split; part += kParts) {
-                floatx4_t in[kParts][KS][2];
-#pragma unroll
-                for (int p = 0; p < kParts; ++p) {
-                    const int64_t at = ((int64_t)min(part + p, a.split - 1) * a.m + row0) * a.width;
-                    const auto buf = buffer(a.partial + at, part + p < a.split ? 16 * a.width * 4 : 0);
-#pragma unroll
-                    for (int s = 0; s < KS; ++s)
-#pragma unroll
-                        for (int c = 0; c < 2; ++c) in[p][s][c] = __builtin_bit_cast(floatx4_t, load16(buf, off[s][c]));
-                }
-#pragma unroll
-                for (int p = 0; p < kParts; ++p)
-#pragma unroll
-                    for (int s = 0; s < KS; ++s)
-#pragma unroll
-                        for (int c = 0; c < 2; ++c) v[s][c] += in[p][s][c];
-            }
-            back = split_row<F16, KS>(v, rank, scale, q, hi, lo);
-        }
+        const float back = row_parts<F16, KS>(a, mb, row0, (mine >> col) & 1, rank, scale, col, q, hi, lo);
         const auto up = buffer(mb.up + (e >= 0 ? (int64_t)e * n * max_rank : 0), (int64_t)n * max_rank * 2);
         for (int c0 = c_begin; c0 < c_end; c0 += kColWaves * kTurn) {
             // base and y: rows q, q + 4, ..., eight columns per lane; what is
@@ -415,6 +573,124 @@ __global__ __launch_bounds__(kThreads) void adapter_up_kernel(AdapterArgs a) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) store8<VEC>(y, at[i] == kOutside ? kOutside : at[i] * ldy, cy, n, in[i]);
         }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// y = base + s B t for prompts.  Workgroup: 64 rows, 16 per wave, x a column
+// chunk, kTurn columns per turn.  The turn's B lies in LDS for all four waves
+// (direct loads, the next turn's under way): what bounds the kernel above at many
+// rows is what its waves read of B, each for its 16 rows (8192 columns, rank
+// 128, 4096 rows: 0.31 GB beside the 0.13 of base and y, 88 us).  LDS image of
+// 32 ranks of B: 16-byte chunk q of column c in slot 4 c + (q ^ (c / 4) mod 4), so that
+// the 16 columns of a fragment read lie in distinct banks.
+// ---------------------------------------------------------------------------
+template <bool F16, int KS, int kTurn>
+__global__ __launch_bounds__(kThreads) void adapter_up_tile_kernel(AdapterArgs a) {
+    constexpr int kPitch = kTurn + 4, kTiles = kTurn / 16;
+    constexpr int kRowsAt = 512 / kTurn, kPieces = 16 / kRowsAt;  // rows per access of base and y, accesses per turn
+    constexpr int kDma = kTurn / 64;                              // 1 KB pieces of a slab per wave
+    const int rr = (threadIdx.x & 63) / (kTurn / 8), rc = 8 * ((threadIdx.x & 63) % (kTurn / 8));  // row, column of an access
+    constexpr int kSlab = kTurn * 64;  // bytes of 32 ranks of a turn's columns
+    __shared__ int slots_lds[64];
+    __shared__ __attribute__((aligned(16))) uint8_t stage[2 * KS * kSlab];
+    __shared__ __attribute__((aligned(16))) float product[kWaves][16][kPitch];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 15, q = lane >> 4;
+    const int chunk = blockIdx.x % a.chunks, tile0 = (int)(blockIdx.x / a.chunks) * 64;
+    const int row0 = tile0 + 16 * wave;
+    int j = 0;
+#pragma unroll
+    for (int i = 0; i < kMaxGemmMembers; ++i) j += chunk >= a.chunk_end[i];
+    const AdapterMember& mb = a.member[j];
+    const int n = mb.n, max_rank = mb.max_rank;
+    const int c_begin = (chunk - mb.chunk0) * a.chunk_cols, c_end = min(n, c_begin + a.chunk_cols);
+    const uint32_t ldbase = (uint32_t)mb.ldbase * 2, ldy = (uint32_t)mb.ldy * 2;  // bytes
+    const auto base = buffer(mb.base + (int64_t)row0 * mb.ldbase, 15 * (int64_t)ldbase + 2 * n);
+    const auto y = buffer(mb.y + (int64_t)row0 * mb.ldy, 15 * (int64_t)ldy + 2 * n);
+    const bool in_place = mb.base == mb.y;
+    const int slot = tile_slots(a, tile0, 64, slots_lds);
+    // this lane's part of a slab's 1 KB pieces (two per wave): column, chunk
+    const int dc = lane >> 2, dq = (lane & 3) ^ (dc >> 2 & 3);
+    uint64_t left = __ballot(slot != -1);
+    while (left) {
+        const int e = __builtin_amdgcn_readlane(slot, __builtin_ctzll(left));
+        const uint64_t all = __ballot(slot == e);
+        left &= ~all;
+        if (e < 0 && in_place) continue;
+        const uint32_t mine = (uint32_t)(all >> (16 * wave)) & 0xffffu;
+        const int rank = e >= 0 ? min(mb.ranks[e], max_rank) : 0;
+        const float scale = e >= 0 ? mb.scales[e] : 0.f;
+        const __amdgpu_buffer_rsrc_t up = buffer(mb.up + (e >= 0 ? (int64_t)e * n * max_rank : 0), (int64_t)n * max_rank * 2);
+        // B of the turn at c0 into stage half h, and the turn's base
+        auto issue = [&](int c0, int h) {
+            auto* to = (__attribute__((address_space(3))) uint8_t*)(void*)(stage + h * KS * kSlab + wave * kDma * 1024);
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
+#pragma unroll
+                for (int p = 0; p < kDma; ++p) {
+                    const int c = c0 + 16 * (kDma * wave + p) + dc, r = s * 32 + dq * 8;
+                    const uint32_t off = r < rank && c < n ? (uint32_t)(c * max_rank + r) * 2 : kOutside;
+                    __builtin_amdgcn_raw_ptr_buffer_load_lds(up, (lds_void_t*)(to + s * kSlab + p * 1024), 16, off, 0, 0, 0);
+                }
+        };
+        auto row_at = [&](int i, int c0, uint32_t ld) {  // row kRowsAt i + rr, eight columns per lane
+            return (mine >> (kRowsAt * i + rr)) & 1 && c0 + rc < c_end ? (uint32_t)(kRowsAt * i + rr) * ld : kOutside;
+        };
+        uint4 next[kPieces];
+        issue(c_begin, 0);
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) next[i] = load16(base, row_at(i, c_begin, ldbase) + 2 * (c_begin + rc));
+        uint4 hi[KS], lo[KS];
+        const float back = row_parts<F16, KS>(a, mb, row0, (mine >> col) & 1, rank, scale, col, q, hi, lo);
+        int h = 0;
+        for (int c0 = c_begin; c0 < c_end; c0 += kTurn, h ^= 1) {
+            // this wave's loads of the turn have landed (the last turn's
+            // stores may be under way); after the barrier every wave's have, and
+            // every wave is done with the other half
+            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_waitcnt(vmcnt_and_lds(kPieces));
+            if (c0 == c_begin) __builtin_amdgcn_s_waitcnt(vmcnt_and_lds(0));
+            __builtin_amdgcn_s_barrier();
+            __builtin_amdgcn_sched_barrier(0);
+            uint4 in[kPieces];
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) in[i] = next[i];
+            if (c0 + kTurn < c_end) {
+                issue(c0 + kTurn, h ^ 1);
+#pragma unroll
+                for (int i = 0; i < kPieces; ++i) next[i] = load16(base, row_at(i, c0 + kTurn, ldbase) + 2 * (c0 + kTurn + rc));
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            const uint8_t* from = stage + h * KS * kSlab + col * 64 + ((q ^ (col >> 2)) & 3) * 16;
+#pragma unroll
+            for (int u = 0; u < kTiles; ++u) {
+                floatx4_t acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int s = 0; s < KS; ++s) {
+                    const uint4 b = *(const uint4*)(from + s * kSlab + u * 1024);
+                    acc = mfma16<F16>(b, lo[s], acc);
+                    acc = mfma16<F16>(b, hi[s], acc);
+                }
+                *(floatx4_t*)&product[wave][col][16 * u + 4 * q] = acc * back;
+            }
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) {
+                const floatx4_t d0 = *(const floatx4_t*)&product[wave][kRowsAt * i + rr][rc];
+                const floatx4_t d1 = *(const floatx4_t*)&product[wave][kRowsAt * i + rr][rc + 4];
+                if (rank > 0) {
+                    in[i].x = add_pair<F16>(in[i].x, d0[0], d0[1]);
+                    in[i].y = add_pair<F16>(in[i].y, d0[2], d0[3]);
+                    in[i].z = add_pair<F16>(in[i].z, d1[0], d1[1]);
+                    in[i].w = add_pair<F16>(in[i].w, d1[2], d1[3]);
+                }
+                store8<true>(y, row_at(i, c0, ldy), c0 + rc, n, in[i]);
+            }
+            __builtin_amdgcn_wave_barrier();
+        }
+        // the next adapter's first loads go into a half that may still be read
+        __syncthreads();
     }
 }
 
@@ -555,6 +831,11 @@ void start_up(const AdapterArgs& a, hipStream_t s) {
 
 template <bool F16, int KS>
 void start_up_rows(const AdapterArgs& a, hipStream_t s) {
+    if constexpr (KS <= 4)
+        if (a.up_tile) {
+            adapter_up_tile_kernel<F16, KS, KS == 4 ? 64 : kAdapterUpTurn><<<(a.m + 63) / 64 * a.chunks, kThreads, 0, s>>>(a);
+            return;
+        }
     if (a.up_rows == 1) start_up<F16, KS, 1>(a, s);
     else start_up<F16, KS, 4>(a, s);
 }
@@ -573,15 +854,23 @@ hipError_t start(const AdapterArgs& a, hipStream_t s) {
         else start_row<F16, 2, true>(a, s);
         return hipGetLastError();
     }
-    if (a.down_rows == 1) start_down_tiles<F16, 1>(a, s);
+    if (a.down_rows == 4) {
+        const dim3 grid((a.m + 63) / 64 * a.split, (a.rank_tiles + kDownTileRanks - 1) / kDownTileRanks, a.members);
+        adapter_down_tile_kernel<F16><<<grid, kThreads, 0, s>>>(a);
+    } else if (a.down_rows == 1) start_down_tiles<F16, 1>(a, s);
     else start_down_tiles<F16, 2>(a, s);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
+    AdapterArgs u = a;
+    if (a.join) {
+        adapter_join_kernel<<<(unsigned)(((int64_t)a.m * a.width / 4 + kThreads - 1) / kThreads), kThreads, 0, s>>>(a);
+        u.split = 1;
+    }
     const int steps = (a.rank_tiles + 1) / 2;
-    if (steps == 1) start_up_rows<F16, 1>(a, s);
-    else if (steps == 2) start_up_rows<F16, 2>(a, s);
-    else if (steps <= 4) start_up_rows<F16, 4>(a, s);
-    else start_up_rows<F16, 8>(a, s);
+    if (steps == 1) start_up_rows<F16, 1>(u, s);
+    else if (steps == 2) start_up_rows<F16, 2>(u, s);
+    else if (steps <= 4) start_up_rows<F16, 4>(u, s);
+    else start_up_rows<F16, 8>(u, s);
     return hipGetLastError();
 }
 

@@ -849,12 +849,24 @@ int cubic_adapters(const void* x, int64_t ldx, const int32_t* row_slots, int64_t
         return fail(CUBIC_EWORKSPACE, "adapter workspace %lld < %lld bytes", (long long)workspace_bytes, (long long)need);
     if (!workspace || !aligned16(workspace)) return fail(CUBIC_EINVAL, "adapter workspace must be 16-byte aligned");
     a.partial = (float*)workspace;
-    a.down_rows = m <= 1024 ? 1 : 2;
+    // 16-row blocks of a wave, or 4: the 64-row tiles.  Tiles where ranks are above 64 and
+    // two workgroups per CU are there: rank 128 m = 4096 K = 8192 (512 of them) 48.5
+    // and 43 us, with one adapter 54 and 27.5; half as many 35 and 36-37; rank 64 at
+    // K = 8192 34 and 34, fewer rows 14 and 22.
+    a.down_rows = m <= 1024 ? 1 : a.rank_tiles > 4 && ceil_div(m, 64) * a.split >= 512 ? 4 : 2;
     a.up_rows = m <= 128 ? 1 : 4;
     a.down_groups = m <= 128 ? (int)std::min<int64_t>(16, m) : m <= 1024 ? 4 : 1;
     a.up_groups = m <= 128 ? (int)std::min<int64_t>(16, m) : m <= 1024 ? 4 : 1;
     const int64_t items = ceil_div(m, 16 * a.up_rows) * a.up_groups;
-    a.chunk_cols = 4 * cubic::kAdapterUpTurn;
+    // The partitions added once where many column chunks would add them again:
+    // 8 of them, 4096 rows, rank 128: 77 -> 58.5 us of up kernel for 4.3 of joining;
+    // at 1024 rows and fewer the launch costs what it saves.  B in LDS for 64 rows
+    // against each wave's own reads: rank 32 51.6 -> 46.5 us, rank 128 67.8 -> 53.
+    a.join = m > 1024 && a.split > 1;
+    a.up_tile = m > 1024 && a.vectors && a.rank_tiles <= 8;
+    // columns of a workgroup: 256 and 512 at rank 128 (4096 rows) 53 and 58.5 us, at
+    // rank 32 (2048 rows, 2 x 12288 columns) 48 and 46.5
+    a.chunk_cols = (a.up_tile && a.rank_tiles > 4 ? 2 : 4) * cubic::kAdapterUpTurn;
     while (a.chunk_cols > cubic::kAdapterUpTurn && items * ceil_div(columns, a.chunk_cols) < 512) a.chunk_cols /= 2;
     int64_t chunks = 0;
     for (int j = 0; j < cubic::kMaxGemmMembers; ++j) {
