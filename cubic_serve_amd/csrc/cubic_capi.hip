@@ -705,7 +705,7 @@ int cubic_embedding(const void* ids, int id_bytes, int64_t tokens, int fmt, cons
 // ---------------------------------------------------------------------------
 namespace {
 struct SamplePlan {
-    int chunks, chunk, list_words;
+    int chunks, chunk, list_words, sorted;
     int64_t counters, heads, bytes;  // bytes of the counters, of the heads, of all
 };
 // Chunks of a row: as many as fill the chip with all rows' (256 workgroups, one
@@ -718,6 +718,9 @@ SamplePlan plan_sample(int rows, int width, int dtype) {
     p.list_words = dtype != CUBIC_DTYPE_F32 ? std::min(p.chunk, cubic::kSampleList)
                    : p.chunks == 1          ? 0
                                             : 4 * std::min(p.chunk, cubic::kSampleBins);
+    // column numbers of 16 bits, as many as LDS holds
+    p.sorted = dtype == CUBIC_DTYPE_F32 && p.chunks > 1 && p.chunk <= cubic::kSampleList;
+    if (p.sorted) p.list_words += cubic::kSampleBins / 2 + p.chunk / 2;
     p.counters = align256((int64_t)rows * 4);
     p.heads = align256((int64_t)rows * p.chunks * cubic::kSampleHead * 4);
     p.bytes = p.counters + p.heads + (int64_t)rows * p.chunks * p.list_words * 4;
@@ -757,6 +760,7 @@ int cubic_vocab_sample(const void* logits, int dtype, int64_t row_stride, int ro
     a.chunks = p.chunks;
     a.chunk = p.chunk;
     a.list_words = p.list_words;
+    a.sorted = p.sorted;
     a.counters = (uint32_t*)workspace;
     a.heads = (uint32_t*)((uint8_t*)workspace + p.counters);
     a.lists = (uint32_t*)((uint8_t*)workspace + p.counters + p.heads);

@@ -177,10 +177,11 @@ struct Search {
     // items held in LDS: key's upper half | number; or (32 bits) the columns of
     // one first digit, key and column
     static constexpr int kCached = TYPE == 2 ? 8192 : kSampleList;
-    uint32_t items[TYPE == 2 ? 2 * kCached : kCached];
+    alignas(16) uint32_t items[TYPE == 2 ? 2 * kCached : kCached];
     double table[kTable];
     uint32_t count[kBins], deep_count[kDeepBins];
     unsigned long long mass[kBins], deep_mass[kDeepBins];
+    uint32_t cursor[TYPE == 2 ? kBins : 1];  // where a bin's next column goes (32 bits)
     uint32_t gathered;          // columns of the first digit (32 bits)
     int starts[kMaxSampleChunks + 1], held[kMaxSampleChunks];
     uint64_t sums[4][kWaves];   // before_wave's
@@ -403,11 +404,9 @@ __device__ __forceinline__ Choice choose(Search<TYPE>& sh, const Weights<TYPE>& 
                 __syncthreads();
                 auto deepen = [&](uint32_t k) {
                     if (k >> shift != prefix) return;
-                    const uint64_t w = weights.of(k);
-                    if (!w) return;
                     const uint32_t d = k >> (shift - 10) & 1023u;
                     atomicAdd(&sh.deep_count[d], 1u);
-                    atomicAdd(&sh.deep_mass[d], (unsigned long long)w);
+                    atomicAdd(&sh.deep_mass[d], (unsigned long long)weights.of(k));
                 };
                 if (gathered <= Search<TYPE>::kCached)
                     for (int i = t; i < gathered; i += kThreads) deepen(sh.items[2 * i]);
@@ -549,7 +548,8 @@ template <int TYPE>
 __device__ __forceinline__ uint32_t least_key(uint32_t top, float temperature) {
     const double d = value_of<TYPE>(top) - 32.0 * (double)temperature;
     const float f = __double2float_rd(d);
-    if constexpr (TYPE == 1) return key_of<1>(__half_as_ushort(__float2half_rd(f)));
+    if constexpr (TYPE == 2) return max(key_of<2>(__float_as_uint(f)), Limits<2>::kNegInf + 1);
+    else if constexpr (TYPE == 1) return key_of<1>(__half_as_ushort(__float2half_rd(f)));
     else return key_of<0>(__float_as_uint(f) >> 16) - (f < 0.f && (__float_as_uint(f) & 0xffffu) ? 0x10000u : 0u);
 }
 
@@ -824,7 +824,11 @@ __global__ __launch_bounds__(kThreads) void vocab_sample_kernel(VocabSampleArgs 
 // the chunks' largest, so that the second can weigh its columns against the
 // row's: each chunk's masses by the keys' first 12 bits, joined by the row's last
 // workgroup to arrive, which gathers the columns of the bin in which a search
-// ends (a scan of the row) and finishes the search among those.
+// ends and finishes the search among those.  Where a row has several chunks of at
+// most 32768 columns, each leaves its columns' numbers in order of bins, so that
+// a bin is a run of each chunk's: 128001 columns, 48 rows, three searches, 78 -> 50 us
+// against scans of the row by the one workgroup (17 us each, what one CU reads).
+// With a chunk per row there is nothing to share out, and the scans stay.
 // ---------------------------------------------------------------------------
 __global__ __launch_bounds__(kThreads) void vocab_top_f32_kernel(VocabSampleArgs a) {
     __shared__ uint32_t wave_top[kWaves], wave_bad[kWaves];
@@ -925,24 +929,59 @@ __global__ __launch_bounds__(kThreads) void vocab_sample_f32_kernel(VocabSampleA
     const Weights<2> weights(s.table, top, r);
     Tally tally;
     const int begin = chunk * a.chunk, end = min(a.width, begin + a.chunk);
-    each_column<2>(logits, begin, end, a.width, [&](int, uint32_t key) { add<2>(s, weights, tally, key, 1u); });
+    const uint32_t least = least_key<2>(top, r.temperature);
+    each_column<2>(logits, begin, end, a.width, [&](int, uint32_t key) {
+        if (key < least) return;
+        const double e = weights.exponent(key);
+        const uint64_t w = weights.at(e);
+        atomicAdd(&s.count[key >> Search<2>::kShift], 1u);
+        atomicAdd(&s.mass[key >> Search<2>::kShift], (unsigned long long)w);
+        if (e >= weights.least) tally.likely += w;
+    });
     __syncthreads();
+    uint32_t* const lists = a.lists + (int64_t)row * a.chunks * a.list_words;
+    const __amdgpu_buffer_rsrc_t shared = device_rsrc(lists);
+    const int runs = 4 * min(a.chunk, kSampleBins), columns = runs + kSampleBins / 2;  // words into a chunk's list
     if (a.chunks > 1) {
         // the chunk's bins that hold anything: bin, columns, mass
-        uint32_t* const list = a.lists + ((int64_t)row * a.chunks + chunk) * a.list_words;
+        const int list = chunk * a.list_words;
         uint64_t likely;
         before_wave(lane_u64(wave_scan_u64(tally.likely), 63), s.sums[2], lane, wave, likely);
+        uint32_t number[kPer], before = 0;
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
-            const int b = t + i * kThreads;
-            const uint32_t number = s.count[b];
+            const int b = t * kPer + i;
+            number[i] = s.count[b];
+            before += number[i];
+            if (!number[i]) continue;
             const uint64_t m = s.mass[b];
-            if (!number) continue;
             const uint32_t at = atomicAdd(&listed, 1u) * 4;
-            store_device(list + at, (uint32_t)b);
-            store_device(list + at + 1, number);
-            store_device(list + at + 2, (uint32_t)m);
-            store_device(list + at + 3, (uint32_t)(m >> 32));
+            store_device4(shared, (list + (int)at) * 4, __builtin_bit_cast(floatx4_dev_t, uint4{(uint32_t)b, number[i], (uint32_t)m, (uint32_t)(m >> 32)}));
+        }
+        if (a.sorted) {
+            // where each bin's columns begin, and the columns, in order of bins
+            const uint32_t scan = wave_scan_u32(before);
+            if (lane == 63) s.count_sums[wave] = scan;
+            __syncthreads();
+            const uint32_t upto = wave_scan_u32(lane < kWaves ? s.count_sums[lane] : 0);
+            before = (wave ? (uint32_t)__builtin_amdgcn_readlane((int)upto, wave - 1) : 0) + scan - before;
+            const int held = __builtin_amdgcn_readlane((int)upto, kWaves - 1);
+            uint64_t begins = 0;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                s.cursor[t * kPer + i] = before;
+                begins |= (uint64_t)before << (16 * i);
+                before += number[i];
+            }
+            store_device((uint64_t*)(lists + list + runs) + t, begins);
+            __syncthreads();
+            uint16_t* const order = (uint16_t*)s.items;
+            each_column<2>(logits, begin, end, a.width, [&](int c, uint32_t key) {
+                if (key >= least) order[atomicAdd(&s.cursor[key >> Search<2>::kShift], 1u)] = (uint16_t)(c - begin);
+            });
+            __syncthreads();
+            for (int i = t; i < (held + 7) / 8; i += kThreads)
+                store_device4(shared, (list + columns) * 4 + 16 * i, ((const floatx4_dev_t*)order)[i]);
         }
         __syncthreads();
         if (t == 0) {
@@ -953,50 +992,114 @@ __global__ __launch_bounds__(kThreads) void vocab_sample_f32_kernel(VocabSampleA
         if (!arrive_last(a.counters + row, a.chunks, &last)) return;
         if (t == 0) store_device(a.counters + row, 0u);
         // this workgroup searches the row: the others' bins on top of its own
+        tally.likely = 0;
         if (wave == 0) {
+            uint32_t items = 0;
             if (lane < a.chunks) {
                 const uint32_t* h = heads + lane * kSampleHead;
-                s.held[lane] = lane == chunk ? 0 : (int)load_device(h + 2);
+                items = lane == chunk ? 0 : load_device(h + 2);
                 tally.likely = (uint64_t)load_device(h + 4) << 32 | load_device(h + 3);
-            } else {
-                tally.likely = 0;
             }
-        } else {
-            tally.likely = 0;
+            const uint32_t scan = wave_scan_u32(items);
+            s.starts[lane + 1] = (int)scan;
+            if (lane == 0) s.starts[0] = 0;
         }
         __syncthreads();
-        for (int c = 0; c < a.chunks; ++c) {
-            const uint32_t* from = a.lists + ((int64_t)row * a.chunks + c) * a.list_words;
-            for (int i = t; i < s.held[c]; i += kThreads) {
-                const uint32_t b = load_device(from + 4 * i), number = load_device(from + 4 * i + 1);
-                const uint64_t m = (uint64_t)load_device(from + 4 * i + 3) << 32 | load_device(from + 4 * i + 2);
-                atomicAdd(&s.count[b], number);
-                atomicAdd(&s.mass[b], (unsigned long long)m);
+        constexpr int kAhead = 4;
+        const int all = s.starts[kMaxSampleChunks];
+        for (int i0 = t; i0 < all; i0 += kAhead * kThreads) {
+            uint4 v[kAhead];
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                const int at = min(i0 + i * kThreads, all - 1);
+                int c = 0;
+                while (s.starts[c + 1] <= at) ++c;
+                v[i] = __builtin_bit_cast(uint4, load_device4(shared, (c * a.list_words + 4 * (at - s.starts[c])) * 4));
+            }
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                if (i0 + i * kThreads >= all) break;
+                atomicAdd(&s.count[v[i].x], v[i].y);
+                atomicAdd(&s.mass[v[i].x], (unsigned long long)((uint64_t)v[i].w << 32 | v[i].z));
             }
         }
         __syncthreads();
     }
+    // f(key, column) for this thread's share of the runs that s.starts and s.held tell
+    auto each_run = [&](int number, auto&& f) {
+        constexpr int kAhead = 4;
+        for (int i0 = t; i0 < number; i0 += kAhead * kThreads) {
+            int c[kAhead];
+            uint32_t bits[kAhead];
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                const int at = min(i0 + i * kThreads, number - 1);
+                int h = 0;
+                while (s.starts[h + 1] <= at) ++h;
+                const uint16_t* from = (const uint16_t*)(lists + (int64_t)h * a.list_words + columns);
+                c[i] = h * a.chunk + (int)load_device(from + s.held[h] + at - s.starts[h]);
+            }
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) bits[i] = ((const uint32_t*)logits)[c[i]];
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i)
+                if (i0 + i * kThreads < number) f(i0 + i * kThreads, key_of<2>(bits[i]), c[i]);
+        }
+    };
     choice = choose<2>(s, weights, tally, r, a.width, [&](uint32_t digit) {
         __syncthreads();
-        if (t == 0) s.gathered = 0;
+        if (!a.sorted) {
+            if (t == 0) s.gathered = 0;
+            __syncthreads();
+            gather(s, logits, a.width, digit);
+            __syncthreads();
+            return;
+        }
+        if (wave == 0) {
+            uint32_t number = 0;
+            if (lane < a.chunks) {
+                // (no finite number's digit is the last)
+                const uint16_t* from = (const uint16_t*)(lists + (int64_t)lane * a.list_words + runs) + digit;
+                const uint32_t run = load_device(from);
+                number = load_device(from + 1) - run;
+                s.held[lane] = (int)run;
+            }
+            const uint32_t scan = wave_scan_u32(number);
+            s.starts[lane + 1] = (int)scan;
+            if (lane == 0) s.starts[0] = 0;
+            if (lane == 63) s.gathered = scan;
+        }
         __syncthreads();
-        gather(s, logits, a.width, digit);
+        if (s.gathered <= Search<2>::kCached)
+            each_run((int)s.gathered, [&](int i, uint32_t key, int c) {
+                s.items[2 * i] = key;
+                s.items[2 * i + 1] = (uint32_t)c;
+            });
         __syncthreads();
-    }, [&](auto&& f) { each_column<2>(logits, 0, a.width, a.width, [&](int, uint32_t key) { f(key); }); });
-    // the last search's columns are gathered: where the key is one of them
-    // only, that is the token
+    }, [&](auto&& f) {
+        if (a.sorted) each_run((int)s.gathered, [&](int, uint32_t key, int) { f(key); });
+        else each_column<2>(logits, 0, a.width, a.width, [&](int, uint32_t key) { f(key); });
+    });
+    // the last search's columns are gathered: where few have the key, the token
+    // is that of them which as many precede as it takes
     const int gathered = (int)s.gathered;
     if (t == 0) listed = 0;
     __syncthreads();
     if (gathered <= Search<2>::kCached) {
+        constexpr uint32_t kFew = 256;
         for (int i = t; i < gathered; i += kThreads)
             if (s.items[2 * i] == choice.key) {
                 const uint32_t at = atomicAdd(&listed, 1u);
-                if (at == 0) s.starts[0] = (int)s.items[2 * i + 1];
+                if (at < kFew) s.deep_count[at] = s.items[2 * i + 1];
             }
         __syncthreads();
-        if (listed == 1) {
-            if (t == 0) publish<2>(a, row, r, top, choice, s.starts[0]);
+        if (listed <= kFew) {
+            if (t < (int)listed) {
+                const uint32_t mine = s.deep_count[t];
+                uint32_t before = 0;
+                for (uint32_t i = 0; i < listed; ++i) before += s.deep_count[i] < mine;
+                if (before + 1 == choice.nth) publish<2>(a, row, r, top, choice, (int)mine);
+            }
             return;
         }
     }
