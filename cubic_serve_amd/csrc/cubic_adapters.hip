@@ -7,12 +7,13 @@
 // (adapter_row_kernel).  Else two: a down kernel writes t as binary32 partial
 // sums over K partitions, an up kernel adds the partitions and finishes the rows.
 //
-// Rows come in any order.  A tile of consecutive rows is walked once per
-// distinct adapter in it (a ballot over the tile's slots finds the rows of
-// each), so a prompt's rows, which share an adapter, are one matrix product and
-// a decode batch whose rows all differ reads each adapter once, without a
-// grouping launch or any host knowledge of the slots.  `groups` workgroups may
-// share a tile's adapters: number j takes those at j, j + groups, ...
+// Rows come in any order, without a grouping launch or any host knowledge of
+// the slots.  Batches of some size are tiled in order of adapters, each
+// workgroup finding its tile's rows by itself (slot_rows): an adapter is then
+// read once per 16 of its rows, wherever they lie.  Else a tile of consecutive
+// rows is walked once per distinct adapter in it (a ballot over the tile's slots
+// finds the rows of each); a prompt's rows share one.  `groups` workgroups may
+// share such a tile's adapters: number j takes those at j, j + groups, ...
 //
 // Arithmetic order: K partitions of kDownK columns, each a sum of four quarters
 // (0 + 1) + (2 + 3), partitions added in ascending order; then the rank in steps
@@ -59,6 +60,66 @@ __device__ __forceinline__ int tile_slots(const AdapterArgs& a, int row0, int ro
     if (threadIdx.x < 64) lds[threadIdx.x] = row_slot(a, row0, rows, threadIdx.x);
     __syncthreads();
     return lds[threadIdx.x & 63];
+}
+
+// Rows in order of adapters (at most 1024 rows, 255 adapters, those without one
+// last): item w is the wth tile of up to 16 rows that share an adapter.  Returns
+// it (-1: no such item) and leaves the tile's rows in lds.rows, -1 behind them.
+// Ranks within an adapter are the rows' order, so that every workgroup finds the
+// same tiles.  A barrier has to precede another call.
+struct SlotRows { int count[kThreads], sums[kWaves], slot, tile, rows[16]; };
+__device__ __forceinline__ int slot_rows(const AdapterArgs& a, int w, SlotRows& lds) {
+    constexpr int kRows = 4;  // rows per thread
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    int slot[kRows];
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+        const int row = wave * 64 * kRows + i * 64 + lane;
+        slot[i] = row < a.m ? a.row_slots[row] : -1;
+        if (row < a.m && (slot[i] < 0 || slot[i] >= a.slots)) slot[i] = a.slots;
+    }
+    lds.count[t] = 0;
+    if (t < 16) lds.rows[t] = -1;
+    if (t == 0) lds.slot = -1;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kRows; ++i)
+        if (slot[i] >= 0) atomicAdd(&lds.count[slot[i]], 1);
+    __syncthreads();
+    const int tiles = (lds.count[t] + 15) / 16;
+    int before = (int)wave_scan_u32((uint32_t)tiles);
+    if (lane == 63) lds.sums[wave] = before;
+    before -= tiles;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) before += i < wave ? lds.sums[i] : 0;
+    if (before <= w && w < before + tiles) {
+        lds.slot = t;
+        lds.tile = w - before;
+    }
+    __syncthreads();
+    const int e = lds.slot;
+    if (e < 0) return -1;
+    uint64_t hits[kRows];
+    int held = 0;
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+        hits[i] = __ballot(slot[i] == e);
+        held += __popcll(hits[i]);
+    }
+    if (lane == 0) lds.sums[wave] = held;
+    __syncthreads();
+    int at = -16 * lds.tile;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) at += i < wave ? lds.sums[i] : 0;
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+        const int mine = at + __popcll(hits[i] & ((1ull << lane) - 1));
+        if (slot[i] == e && mine >= 0 && mine < 16) lds.rows[mine] = wave * 64 * kRows + i * 64 + lane;
+        at += __popcll(hits[i]);
+    }
+    __syncthreads();
+    return e == a.slots ? kNone : e;
 }
 
 // One quarter of t for 16 * MT rows x RT 16-rank tiles, every load in flight at
@@ -110,7 +171,10 @@ __device__ __forceinline__ void quarter_product(__amdgpu_buffer_rsrc_t x, const 
 template <bool F16, int MT, int RT>
 __global__ __launch_bounds__(kThreads) void adapter_down_kernel(AdapterArgs a) {
     constexpr int kRows = 16 * MT;
-    __shared__ int slots_lds[64];
+    __shared__ union {
+        int slots[64];
+        SlotRows rows;
+    } walk;
     __shared__ floatx4_t red[2][MT * RT][64];
     const AdapterMember& mb = a.member[blockIdx.z];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -120,11 +184,22 @@ __global__ __launch_bounds__(kThreads) void adapter_down_kernel(AdapterArgs a) {
     // range: 4096 x 8192 at rank 128, 76 -> 57 us)
     const int part = blockIdx.x % a.split, item = blockIdx.x / a.split;
     const int tile = item / a.down_groups, group = item % a.down_groups;
-    const int row0 = tile * kRows, rank0 = blockIdx.y * RT * 16;
+    const int rank0 = blockIdx.y * RT * 16;
     if (rank0 >= mb.max_rank) return;
-    const int slot = tile_slots(a, row0, kRows, slots_lds);
-
-    const int rows = min(kRows, a.m - row0);
+    // this lane's row, 16 i + col of the tile, from row0 on
+    int row0 = tile * kRows, rows = min(kRows, a.m - row0), slot, row[MT];
+    if (MT == 1 && a.items) {
+        const int e = slot_rows(a, item, walk.rows);
+        if (e < 0) return;  // no such tile, or one without an adapter
+        row0 = 0;
+        rows = a.m;
+        slot = lane < 16 && walk.rows.rows[lane] >= 0 ? e : -1;
+        row[0] = walk.rows.rows[col];
+    } else {
+        slot = tile_slots(a, row0, kRows, walk.slots);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) row[i] = 16 * i + col;
+    }
     const auto x = buffer(a.x + (int64_t)row0 * a.ldx, ((int64_t)(rows - 1) * a.ldx + a.k) * 2);
     const int k0 = part * kDownK + wave * kQuarter + q * 8;
     uint64_t left = __ballot(slot >= 0);
@@ -134,12 +209,13 @@ __global__ __launch_bounds__(kThreads) void adapter_down_kernel(AdapterArgs a) {
         const uint64_t mine = __ballot(slot == e);
         left &= ~mine;
         if (order % a.down_groups != group) continue;
+        const int first = MT == 1 ? __builtin_amdgcn_readlane(row[0], lead) : lead;
         // rows of other adapters repeat the first row: their columns of the
         // product are not stored
         uint32_t xoff[MT], doff[RT];
 #pragma unroll
         for (int i = 0; i < MT; ++i)
-            xoff[i] = (uint32_t)((mine >> (16 * i + col)) & 1 ? 16 * i + col : lead) * (uint32_t)(a.ldx * 2);
+            xoff[i] = (uint32_t)((mine >> (16 * i + col)) & 1 ? row[i] : first) * (uint32_t)(a.ldx * 2);
         // the first tile does not wait for the slot's rank (what lies past it
         // the up kernel leaves out); the others are read only below it
         const int rank = RT > 1 || rank0 ? min(mb.ranks[e], mb.max_rank) : mb.max_rank;
@@ -175,8 +251,7 @@ __global__ __launch_bounds__(kThreads) void adapter_down_kernel(AdapterArgs a) {
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
                 if (!((mine >> (16 * i + col)) & 1)) continue;
-                float* out = a.partial + ((int64_t)part * a.m + row0 + 16 * i + col) * a.width + mb.rank0 +
-                             rank0 + 4 * q;
+                float* out = a.partial + ((int64_t)part * a.m + row0 + row[i]) * a.width + mb.rank0 + rank0 + 4 * q;
 #pragma unroll
                 for (int t = 0; t < RT; ++t)
                     if (rank0 + 16 * t < mb.max_rank)
@@ -408,12 +483,12 @@ __device__ __forceinline__ float split_row(const floatx4_t (&v)[KS][2], int rank
     return back;
 }
 
-// The parts of t of rows row0 .. row0 + 15 (this lane's: row0 + col, if own): the
-// partitions in ascending order, kParts requested together; what is not there
+// The parts of t of this lane's row (row0 + row, if own; rows of them from row0 on
+// are there): the partitions in ascending order, kParts requested together; what is not there
 // (another row, past the rank) reads as 0.
 template <bool F16, int KS>
-__device__ __forceinline__ float row_parts(const AdapterArgs& a, const AdapterMember& mb, int row0, bool own,
-                                           int rank, float scale, int col, int q, uint4 (&hi)[KS], uint4 (&lo)[KS]) {
+__device__ __forceinline__ float row_parts(const AdapterArgs& a, const AdapterMember& mb, int row0, int rows, int row,
+                                           bool own, int rank, float scale, int q, uint4 (&hi)[KS], uint4 (&lo)[KS]) {
     constexpr int kParts = KS < 8 ? 8 / KS : 1;
     uint32_t off[KS][2];
     floatx4_t v[KS][2];
@@ -422,7 +497,7 @@ __device__ __forceinline__ float row_parts(const AdapterArgs& a, const AdapterMe
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
             const int f = s * 32 + q * 8 + 4 * c;
-            off[s][c] = own && f < rank ? (uint32_t)(col * a.width + mb.rank0 + f) * 4 : kOutside;
+            off[s][c] = own && f < rank ? (uint32_t)(row * a.width + mb.rank0 + f) * 4 : kOutside;
             v[s][c] = floatx4_t{0.f, 0.f, 0.f, 0.f};
         }
     for (int part = 0; part < a.split; part += kParts) {
@@ -430,7 +505,7 @@ __device__ __forceinline__ float row_parts(const AdapterArgs& a, const AdapterMe
 #pragma unroll
         for (int p = 0; p < kParts; ++p) {
             const int64_t at = ((int64_t)min(part + p, a.split - 1) * a.m + row0) * a.width;
-            const auto buf = buffer(a.partial + at, part + p < a.split ? 16 * a.width * 4 : 0);
+            const auto buf = buffer(a.partial + at, part + p < a.split ? (int64_t)rows * a.width * 4 : 0);
 #pragma unroll
             for (int s = 0; s < KS; ++s)
 #pragma unroll
@@ -490,9 +565,19 @@ __global__ __launch_bounds__(kThreads) void adapter_up_kernel(AdapterArgs a) {
     const int col = lane & 15, q = lane >> 4;
     const int chunk = blockIdx.x % a.chunks, item = blockIdx.x / a.chunks;
     const int tile = item / a.up_groups, group = item % a.up_groups;
-    const int row0 = (tile * WR + wave / kColWaves) * 16;
-    // every wave walks its own rows
-    const int slot = row_slot(a, row0, 16, lane);
+    // every wave walks its own rows, or all the item's: row0 + row_of(0 .. 15)
+    int row0 = (tile * WR + wave / kColWaves) * 16, rows = 16, slot;
+    __shared__ SlotRows walk;
+    if (WR == 1 && a.items) {
+        const int e = slot_rows(a, item, walk);
+        if (e == -1) return;
+        row0 = 0;
+        rows = a.m;
+        slot = lane < 16 && walk.rows[lane] >= 0 ? e : -1;
+    } else {
+        slot = row_slot(a, row0, 16, lane);
+    }
+    auto row_of = [&](int r) { return WR == 1 && a.items ? max(walk.rows[r], 0) : r; };
     // the member of this column chunk (a grid of members x the widest one's
     // chunks leaves workgroups that only end: m = 64, q k v: 7.4 -> 13 us)
     int j = 0;
@@ -503,8 +588,8 @@ __global__ __launch_bounds__(kThreads) void adapter_up_kernel(AdapterArgs a) {
     const int c_begin = (chunk - mb.chunk0) * a.chunk_cols + wave % kColWaves * kTurn;
     const int c_end = min(n, (chunk - mb.chunk0 + 1) * a.chunk_cols);
     const uint32_t ldbase = (uint32_t)mb.ldbase * 2, ldy = (uint32_t)mb.ldy * 2;  // bytes
-    const auto base = buffer(mb.base + (int64_t)row0 * mb.ldbase, 15 * (int64_t)ldbase + 2 * n);
-    const auto y = buffer(mb.y + (int64_t)row0 * mb.ldy, 15 * (int64_t)ldy + 2 * n);
+    const auto base = buffer(mb.base + (int64_t)row0 * mb.ldbase, (int64_t)(rows - 1) * ldbase + 2 * n);
+    const auto y = buffer(mb.y + (int64_t)row0 * mb.ldy, (int64_t)(rows - 1) * ldy + 2 * n);
     const bool in_place = mb.base == mb.y;
 
     uint64_t left = __ballot(slot != -1);
@@ -518,7 +603,7 @@ __global__ __launch_bounds__(kThreads) void adapter_up_kernel(AdapterArgs a) {
         if (rank <= 0 && in_place) continue;
         const float scale = e >= 0 ? mb.scales[e] : 0.f;
         uint4 hi[KS], lo[KS];
-        const float back = row_parts<F16, KS>(a, mb, row0, (mine >> col) & 1, rank, scale, col, q, hi, lo);
+        const float back = row_parts<F16, KS>(a, mb, row0, rows, row_of(col), (mine >> col) & 1, rank, scale, q, hi, lo);
         const auto up = buffer(mb.up + (e >= 0 ? (int64_t)e * n * max_rank : 0), (int64_t)n * max_rank * 2);
         for (int c0 = c_begin; c0 < c_end; c0 += kColWaves * kTurn) {
             // base and y: rows q, q + 4, ..., eight columns per lane; what is
@@ -529,8 +614,8 @@ __global__ __launch_bounds__(kThreads) void adapter_up_kernel(AdapterArgs a) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const bool own = ((mine >> (4 * i + q)) & 1) && cy < n;
-                at[i] = own ? (uint32_t)(4 * i + q) : kOutside;
-                in[i] = load8<VEC>(base, own ? (4 * i + q) * ldbase : kOutside, cy, n);
+                at[i] = own ? (uint32_t)row_of(4 * i + q) : kOutside;
+                in[i] = load8<VEC>(base, own ? at[i] * ldbase : kOutside, cy, n);
             }
             if (rank > 0) {
                 constexpr int kTiles = kTurn / 16, kHalf = kTiles / 2;
@@ -642,7 +727,7 @@ __global__ __launch_bounds__(kThreads) void adapter_up_tile_kernel(AdapterArgs a
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) next[i] = load16(base, row_at(i, c_begin, ldbase) + 2 * (c_begin + rc));
         uint4 hi[KS], lo[KS];
-        const float back = row_parts<F16, KS>(a, mb, row0, (mine >> col) & 1, rank, scale, col, q, hi, lo);
+        const float back = row_parts<F16, KS>(a, mb, row0, 16, col, (mine >> col) & 1, rank, scale, q, hi, lo);
         int h = 0;
         for (int c0 = c_begin; c0 < c_end; c0 += kTurn, h ^= 1) {
             // this wave's loads of the turn have landed (the last turn's
@@ -810,7 +895,7 @@ __global__ __launch_bounds__(kAdapterRowWaves * 64) void adapter_row_kernel(Adap
 
 template <bool F16, int MT, int RT>
 void start_down(const AdapterArgs& a, hipStream_t s) {
-    const dim3 grid((a.m + 16 * MT - 1) / (16 * MT) * a.down_groups * a.split,
+    const dim3 grid((a.items ? a.items : (a.m + 16 * MT - 1) / (16 * MT) * a.down_groups) * a.split,
                     (a.rank_tiles + RT - 1) / RT, a.members);
     adapter_down_kernel<F16, MT, RT><<<grid, kThreads, 0, s>>>(a);
 }
@@ -824,7 +909,7 @@ void start_down_tiles(const AdapterArgs& a, hipStream_t s) {
 
 template <bool F16, int KS, int WR>
 void start_up(const AdapterArgs& a, hipStream_t s) {
-    const dim3 grid((a.m + 16 * WR - 1) / (16 * WR) * a.up_groups * a.chunks);
+    const dim3 grid((a.items ? a.items : (a.m + 16 * WR - 1) / (16 * WR) * a.up_groups) * a.chunks);
     if (a.vectors) adapter_up_kernel<F16, KS, WR, true><<<grid, kThreads, 0, s>>>(a);
     else adapter_up_kernel<F16, KS, WR, false><<<grid, kThreads, 0, s>>>(a);
 }

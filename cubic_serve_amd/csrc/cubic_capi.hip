@@ -822,7 +822,7 @@ int cubic_adapters(const void* x, int64_t ldx, const int32_t* row_slots, int64_t
     a.f16 = dtype == CUBIC_DTYPE_F16;
     a.split = (int)ceil_div(k, cubic::kAdapterDownK);
     a.vectors = 1;
-    int64_t columns = 0;
+    int64_t columns = 0, widest = 0;
     int largest = 0;
     for (int j = 0; j < members; ++j) {
         if (!downs[j] || !ups[j] || !scales[j] || !ranks[j] || !bases[j] || !ys[j])
@@ -844,6 +844,7 @@ int cubic_adapters(const void* x, int64_t ldx, const int32_t* row_slots, int64_t
         a.vectors &= ns[j] % 8 == 0 && ldbases[j] % 8 == 0 && ldys[j] % 8 == 0 && aligned16(bases[j]) &&
                      aligned16(ys[j]);
         columns += ns[j];
+        widest = std::max({widest, ldbases[j], ldys[j]});
         largest = std::max(largest, max_ranks[j]);
     }
     a.members = members;
@@ -858,19 +859,31 @@ int cubic_adapters(const void* x, int64_t ldx, const int32_t* row_slots, int64_t
     // and 43 us, with one adapter 54 and 27.5; half as many 35 and 36-37; rank 64 at
     // K = 8192 34 and 34, fewer rows 14 and 22.
     a.down_rows = m <= 1024 ? 1 : a.rank_tiles > 4 && ceil_div(m, 64) * a.split >= 512 ? 4 : 2;
-    a.up_rows = m <= 128 ? 1 : 4;
+    // Batches of 17 to 1024 rows are tiled in order of adapters, the others as the
+    // rows stand, a tile's adapters shared by up to 16 workgroups.  In order and as
+    // they stand: 256 rows of 64 requests with 16 adapters, K = 12288 -> 4096, 26.3 and
+    // 36.0 us; 512 rows, 128 requests, 2 x 12288 columns 29.9 and 52.5; 1024 rows of 8
+    // requests, 2 x 12288 49 and 61; 64 rows, 64 adapters 21 and 28.5; 24 rows, 24
+    // adapters 16.5 and 15.5.  At 16 rows the search for a tile's rows costs more than it
+    // saves, 10.2 and 8.5.  (Its rows lie anywhere in the batch: 32-bit offsets from the
+    // first.)
+    const bool by_slot = m > 16 && m <= 1024 && slots < 256 && m * ldx < (1 << 30) && m * widest < (1 << 30) && 1;
+    a.items = by_slot ? (int)(std::min<int64_t>(slots + 1, m) + m / 16) : 0;
+    a.up_rows = m <= 128 || by_slot ? 1 : 4;
     a.down_groups = m <= 128 ? (int)std::min<int64_t>(16, m) : m <= 1024 ? 4 : 1;
     a.up_groups = m <= 128 ? (int)std::min<int64_t>(16, m) : m <= 1024 ? 4 : 1;
-    const int64_t items = ceil_div(m, 16 * a.up_rows) * a.up_groups;
+    if (by_slot) a.down_groups = a.up_groups = 1;
+    const int64_t items = by_slot ? a.items : ceil_div(m, 16 * a.up_rows) * a.up_groups;
     // The partitions added once where many column chunks would add them again:
     // 8 of them, 4096 rows, rank 128: 77 -> 58.5 us of up kernel for 4.3 of joining;
     // at 1024 rows and fewer the launch costs what it saves.  B in LDS for 64 rows
     // against each wave's own reads: rank 32 51.6 -> 46.5 us, rank 128 67.8 -> 53.
     a.join = m > 1024 && a.split > 1;
     a.up_tile = m > 1024 && a.vectors && a.rank_tiles <= 8;
-    // columns of a workgroup: 256 and 512 at rank 128 (4096 rows) 53 and 58.5 us, at
-    // rank 32 (2048 rows, 2 x 12288 columns) 48 and 46.5
-    a.chunk_cols = (a.up_tile && a.rank_tiles > 4 ? 2 : 4) * cubic::kAdapterUpTurn;
+    // Columns of a workgroup, while 512 workgroups are left.  Prompts: 256 and 512 at
+    // rank 128 (4096 rows) 53 and 58.5 us, at rank 32 (2048 rows, 2 x 12288 columns) 48
+    // and 46.5.  In order of adapters: 2048 and 512, 1024 rows x 2 x 12288 columns 49 and 64.
+    a.chunk_cols = (by_slot ? 16 : a.up_tile && a.rank_tiles > 4 ? 2 : 4) * cubic::kAdapterUpTurn;
     while (a.chunk_cols > cubic::kAdapterUpTurn && items * ceil_div(columns, a.chunk_cols) < 512) a.chunk_cols /= 2;
     int64_t chunks = 0;
     for (int j = 0; j < cubic::kMaxGemmMembers; ++j) {
@@ -883,10 +896,10 @@ int cubic_adapters(const void* x, int64_t ldx, const int32_t* row_slots, int64_t
     // per wave) and every row's column chunks together at most one workgroup per
     // CU, the rows all with adapters of their own.  In a replayed graph, one
     // launch and two: q k v (K = 4096) m = 1 8.7 and 7.9 us (a launch of the host's
-    // less: 11.4 -> 9.1 eagerly), 16 10.0 and 11.8, 64 12.5 and 15.9 (all with one of
-    // four adapters: 10.9 and 9.1); 2 x 12288 columns m = 32 14.5 and 18.6.  With
-    // more workgroups than CUs, 2 x 12288 m = 64 at 2048 columns: 31.0 and 28.8; with
-    // more K, 12288 -> 4096 m = 64: 22 and 16.
+    // less: 11.4 -> 9.1 eagerly), 16 10.1 and 12.2, 64 12.8 and 16.3 (eight adapters
+    // 11.3 and 11.4, four 11.5 and 11.0); 2 x 12288 columns m = 32 14.7 and 15.9.  With more
+    // workgroups than CUs, 2 x 12288 m = 64 at 2048 columns: 31.0 and 21.0; with more K,
+    // 12288 -> 4096 m = 64: 22 and 16.
     if (a.rank_tiles == 1 && a.split <= cubic::kAdapterRowWaves / 4) {
         for (int cols = 512; cols <= 4096 && !a.fused; cols *= 2) {
             int64_t all = 0, most = 0;
@@ -896,6 +909,7 @@ int cubic_adapters(const void* x, int64_t ldx, const int32_t* row_slots, int64_t
             }
             if (m * all > 256) continue;
             a.fused = 1;
+            a.items = 0;
             a.chunk_cols = cols;
             a.chunks = (int)most;
             a.down_groups = (int)std::min<int64_t>(16, m);

@@ -308,6 +308,7 @@ struct AdapterArgs {
     int vectors;                  // every member: 16-byte base and output accesses
     int fused;                    // one launch (few rows); chunks: the widest member's
     int down_rows, up_rows;       // 16-row tiles per workgroup: 1 or 2; 1 or 4
+    int items;                    // tiles of rows in order of adapters (0: tiles of the rows as they are)
     int join;                     // add the partitions in a launch of their own
     int up_tile;                  // 64-row tiles with B in LDS (prompts)
     int down_groups, up_groups;   // workgroups that share a tile's distinct adapters

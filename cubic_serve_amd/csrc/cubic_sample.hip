@@ -60,7 +60,7 @@ struct Limits {  // keys of +inf and -inf
                                                                            : ~0xfc000000u & 0xffff0000u;
 };
 
-// Inclusive scan over the 64 lanes (the exchanges of wave_row_scan).
+// Inclusive scan over the 64 lanes (as wave_scan_u32).
 template <int CTRL, int ROWS>
 __device__ __forceinline__ uint64_t dpp_u64(uint64_t v) {
     const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xF, false);
@@ -74,15 +74,6 @@ __device__ __forceinline__ uint64_t wave_scan_u64(uint64_t v) {
     v += dpp_u64<0x118, 0xF>(v);
     v += dpp_u64<0x142, 0xA>(v);
     v += dpp_u64<0x143, 0xC>(v);
-    return v;
-}
-__device__ __forceinline__ uint32_t wave_scan_u32(uint32_t v) {
-    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xF, 0xF, false);
-    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xF, 0xF, false);
-    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xF, 0xF, false);
-    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xF, 0xF, false);
-    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xA, 0xF, false);
-    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xC, 0xF, false);
     return v;
 }
 __device__ __forceinline__ uint64_t lane_u64(uint64_t v, int l) {  // wave-uniform l
