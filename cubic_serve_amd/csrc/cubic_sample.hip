@@ -157,30 +157,39 @@ __device__ __forceinline__ void each_column(const uint8_t* row, int begin, int e
 // the columns themselves, or the distinct keys of a row's chunks.
 // ---------------------------------------------------------------------------
 constexpr int kTable = 128;  // 2^(i / 128)
+constexpr uint32_t kNoDigit = ~0u;
+
+struct Choice {
+    uint32_t key;   // the token is the nth column (from 1) of this key
+    uint64_t nth;
+    uint64_t kept;  // mass of the kept columns
+};
 
 template <int TYPE>
 struct Search {
-    // bins: the first digit, 11 of a 16-bit key's bits or 12 of 32; then the
-    // other 5, or twice 10
+    // bins: the first digit, 11 of a 16-bit key's bits or 12 of 32; then (32 bits)
+    // twice 10
     static constexpr int kBins = TYPE == 2 ? 4096 : 2048, kShift = TYPE == 2 ? 20 : 21;
     static constexpr int kPer = kBins / kThreads;  // bins per thread
-    static constexpr int kDeepBins = TYPE == 2 ? 1024 : 32;
+    static constexpr int kDeepBins = TYPE == 2 ? 1024 : 1;
     // items held in LDS: key's upper half | number; or (32 bits) the columns of
     // one first digit, key and column
     static constexpr int kCached = TYPE == 2 ? 8192 : kSampleList;
     alignas(16) uint32_t items[TYPE == 2 ? 2 * kCached : kCached];
-    double table[kTable];
     uint32_t count[kBins], deep_count[kDeepBins];
     unsigned long long mass[kBins], deep_mass[kDeepBins];
     uint32_t cursor[TYPE == 2 ? kBins : 1];  // where a bin's next column goes (32 bits)
     uint32_t gathered;          // columns of the first digit (32 bits)
-    int starts[kMaxSampleChunks + 1], held[kMaxSampleChunks];
+    int starts[kMaxSampleChunks + 1], held[kMaxSampleChunks], number[kMaxSampleChunks];
     uint64_t sums[4][kWaves];   // before_wave's
     uint32_t count_sums[kWaves];
-    // a search's answer: the digit, the sums above it; of the whole key: its
-    // rank among the key's columns, the mass through it
+    // 32 bits: a search's digit and the sums before it
     uint32_t digit;
-    uint64_t before_count, before_mass, nth, through;
+    uint64_t before_count, before_mass;
+    // 16 bits: each search's digit, the counts of that digit's keys
+    uint32_t digits[3], keys[3][32], columns;
+    Choice choice;
+    float logprob;
 };
 
 // A row's parameters, read by one thread (waves that read them by themselves
@@ -188,6 +197,7 @@ struct Search {
 struct Row {
     float temperature, top_p, min_p, u;
     int64_t top_k;
+    double scale, least;  // of Weights; by the one thread
     __device__ __forceinline__ void read(const VocabSampleArgs& a, int row) {
         temperature = a.temperatures[row];
         top_p = a.top_ps[row];
@@ -195,16 +205,14 @@ struct Row {
         u = a.uniforms[row];
         top_k = a.top_ks[row];
     }
+    __device__ __forceinline__ void prepare() {
+        scale = 128.0 * 1.4426950408889634074 / (double)temperature;
+        least = min_p > 0.f ? 128.0 * log2((double)min_p) : -__builtin_inf();
+    }
     __device__ __forceinline__ bool admitted() const {
         return temperature >= 0.f && __builtin_isfinite(temperature) && top_p > 0.f && top_p <= 1.f &&
                min_p >= 0.f && min_p <= 1.f && u >= 0.f && u < 1.f;
     }
-};
-
-struct Choice {
-    uint32_t key;   // the token is the nth column (from 1) of this key
-    uint64_t nth;
-    uint64_t kept;  // mass of the kept columns
 };
 
 // Weight of a key in fixed point: with t = 128 log2(e) (l - max) / T and n = rint(t),
@@ -216,8 +224,7 @@ struct Weights {
     double largest, scale, least;
     const double* table;
     __device__ __forceinline__ Weights(const double* lds, uint32_t top, const Row& r)
-        : largest(value_of<TYPE>(top)), scale(128.0 * 1.4426950408889634074 / (double)r.temperature),
-          least(r.min_p > 0.f ? 128.0 * log2((double)r.min_p) : -__builtin_inf()), table(lds) {}
+        : largest(value_of<TYPE>(top)), scale(r.scale), least(r.least), table(lds) {}
     __device__ __forceinline__ double exponent(uint32_t key) const { return (value_of<TYPE>(key) - largest) * scale; }
     __device__ __forceinline__ uint64_t at(double t) const {
         const double n = __builtin_rint(fmax(t, -46.0 * 128.0));
@@ -236,15 +243,21 @@ struct Tally {
     uint64_t likely = 0;  // mass of the weights of at least min_p
 };
 
+__device__ __forceinline__ void fill_table(double* table) {
+    if (threadIdx.x < kTable) table[threadIdx.x] = exp2((double)threadIdx.x / kTable);
+}
+
 // Called by the whole workgroup; a barrier has to follow.
 template <int TYPE>
 __device__ __forceinline__ void clear(Search<TYPE>& sh) {
     const int t = threadIdx.x;
-    if (t < kTable) sh.table[t] = exp2((double)t / kTable);
 #pragma unroll
     for (int i = 0; i < Search<TYPE>::kPer; ++i) {
         sh.count[t + i * kThreads] = 0;
         sh.mass[t + i * kThreads] = 0;
+    }
+    if constexpr (TYPE != 2) {
+        if (t < 96) (&sh.keys[0][0])[t] = 0;
     }
 }
 template <int TYPE>
@@ -258,21 +271,25 @@ __device__ __forceinline__ void add(Search<TYPE>& sh, const Weights<TYPE>& weigh
     if (t >= weights.least) tally.likely += w;
 }
 
+// The chunk c whose part [starts[c], starts[c + 1]) holds i.
+template <int TYPE>
+__device__ __forceinline__ int chunk_of(const Search<TYPE>& sh, int chunks, int i) {
+    int c = 0;
+    for (int step = 1 << (31 - __builtin_clz(chunks)); step; step >>= 1)
+        if (c + step < chunks && sh.starts[c + step] <= i) c += step;
+    return c;
+}
+
 // First of the bins in descending order whose inclusive sum (of counts, or of
-// masses) reaches x, with the sums before it; none: the digit is kNoDigit.
+// masses) reaches x: its thread calls found(digit, count before, mass before).
 // Thread t owns bins BINS - 1 - t PER - i with c, m in them; cb, mb lie before.
-constexpr uint32_t kNoDigit = ~0u;
-template <int TYPE, int PER>
-__device__ __forceinline__ void pick(Search<TYPE>& sh, const uint32_t (&c)[PER], const uint64_t (&m)[PER],
-                                     uint64_t cb, uint64_t mb, bool by_mass, uint64_t x) {
+template <int PER, typename Found>
+__device__ __forceinline__ void pick(const uint32_t (&c)[PER], const uint64_t (&m)[PER], uint64_t cb, uint64_t mb,
+                                     bool by_mass, uint64_t x, Found&& found) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
         const uint64_t lo = by_mass ? mb : cb, add = by_mass ? m[i] : c[i];
-        if (lo < x && lo + add >= x) {  // one bin at most
-            sh.digit = PER * kThreads - 1 - threadIdx.x * PER - i;
-            sh.before_count = cb;
-            sh.before_mass = mb;
-        }
+        if (lo < x && lo + add >= x) found(PER * kThreads - 1 - threadIdx.x * PER - i, cb, mb);  // one bin at most
         cb += c[i];
         mb += m[i];
     }
@@ -300,123 +317,165 @@ __device__ __forceinline__ void bins_before(Search<TYPE>& sh, const uint32_t* co
     cb = (wave ? (uint32_t)__builtin_amdgcn_readlane((int)upto, wave - 1) : 0) + ci - cs;
 }
 
-// With the sums before a whole key (weight w): the rank of the position at which
-// the inclusive count or mass reaches x among the key's columns, and the mass
-// through it.  By the thread that found the key.
-template <int TYPE>
-__device__ __forceinline__ void settle(Search<TYPE>& sh, bool by_mass, uint64_t x, uint64_t w) {
-    uint64_t nth;
-    if (by_mass) {
-        // ceil((x - before) / w), a column number (below 2^21), by a quotient
-        // in binary64 that is off by less than one
-        const uint64_t want = x - sh.before_mass;
-        nth = (uint64_t)((double)want / (double)w);
-        while (nth * w < want) ++nth;
-        while (nth > 1 && (nth - 1) * w >= want) --nth;
-    } else {
-        nth = x - sh.before_count;
-    }
-    sh.nth = nth;
-    sh.through = sh.before_mass + nth * w;
+// ceil(want / w), a number of columns (at most 2^20): by a reciprocal, off by
+// less than a half, which rounding down leaves at most two short.
+__device__ __forceinline__ uint64_t columns_to(uint64_t want, uint64_t w) {
+    uint64_t n = (uint32_t)((double)want * __builtin_amdgcn_rcp((double)max(w, (uint64_t)1)));
+    if (n * w < want) ++n;
+    if (n * w < want) ++n;
+    return n;
 }
 
-// Called by the whole workgroup once the items are added, after a barrier.
-// 16 bits: items(f) calls f(key, number) for this thread's share of them;
-// columns whose weight is 0 may be left out.  32 bits: items(digit) gathers the
-// columns of a first digit (key and column in sh.items, their number in
-// sh.gathered, past kCached only that), barriers before and behind included;
-// columns(f) calls f(key) for this thread's share of the row's columns.
-template <int TYPE, typename Items, typename Columns>
-__device__ __forceinline__ Choice choose(Search<TYPE>& sh, const Weights<TYPE>& weights, const Tally& tally,
-                                         const Row& r, int width, Items&& items, Columns&& columns) {
-    constexpr int kPer = Search<TYPE>::kPer;
+// What the searches look for, in turn: x for top-k (a count), top-p and the token
+// (masses); head: mass of what they keep so far, kept: of min-p.  False: the
+// search leaves nothing out.
+__device__ __forceinline__ bool wanted(int stage, const Row& r, int width, uint64_t head, uint64_t& kept, uint64_t& x) {
+    if (stage == 0) {
+        x = (uint64_t)r.top_k;
+        return r.top_k > 0 && r.top_k < width;
+    }
+    if (stage == 1) {
+        x = max((uint64_t)1, min(head, (uint64_t)__builtin_ceil((double)r.top_p * (double)head)));
+        return r.top_p < 1.f;
+    }
+    kept = min(kept, head);
+    x = min(kept, (uint64_t)((double)r.u * (double)kept) + 1);
+    return true;
+}
+
+// The searches of a row of 16-bit logits.  Called by the whole workgroup once
+// the items are added, after a barrier; items(f) calls f(key, number) for this
+// thread's share of them; columns whose weight is 0 may be left out.  What is
+// serial is done by one wave: sixteen that do it side by side share four issue
+// ports (a search 4700 cycles, 3000 to 4300 so).
+template <int TYPE, typename Items>
+__device__ __forceinline__ Choice choose_narrow(Search<TYPE>& sh, const Weights<TYPE>& weights, const Tally& tally,
+                                                const Row& r, int width, Items&& items) {
+    constexpr int kPer = Search<TYPE>::kPer, kBins = Search<TYPE>::kBins, kRun = kBins / 64;
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
-    [[maybe_unused]] uint32_t held = kNoDigit;  // the digit whose columns are gathered (32 bits)
+    uint64_t head, kept;
+    {
+        // the bins' sums become the sums before them
+        uint32_t c[kPer];
+        uint64_t m[kPer], cb, mb;
+        bins_before<TYPE, kPer>(sh, sh.count, sh.mass, c, m, cb, mb, head);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            sh.count[kBins - 1 - t * kPer - i] = (uint32_t)cb;
+            sh.mass[kBins - 1 - t * kPer - i] = mb;
+            cb += c[i];
+            mb += m[i];
+        }
+        if (t == kThreads - 1) sh.columns = (uint32_t)cb;
+    }
+    kept = head;
+    if (r.min_p > 0.f) before_wave(lane_u64(wave_scan_u64(tally.likely), 63), sh.sums[2], lane, wave, kept);
+    __syncthreads();
+    uint32_t key = 0;
+    uint64_t nth = 1;
+    for (int stage = 0; stage < 3; ++stage) {
+        uint64_t x = 0;
+        if (!wanted(stage, r, width, head, kept, x)) continue;  // (the same in every wave)
+        uint64_t count = 0, mass = 0;
+        if (wave == 0) {
+            // the last bin in descending order before which the sum is below x
+            auto before = [&](int d) { return stage ? (uint64_t)sh.mass[kBins - 1 - d] : (uint64_t)sh.count[kBins - 1 - d]; };
+            const int run = max(__popcll(__ballot(before(lane * kRun) < x)) - 1, 0);
+            const int d = run * kRun + max(__popcll(__ballot(lane < kRun && before(run * kRun + min(lane, kRun - 1)) < x)) - 1, 0);
+            count = sh.count[kBins - 1 - d];
+            mass = sh.mass[kBins - 1 - d];
+            // (fewer than top_k columns may weigh anything)
+            if (lane == 0) sh.digits[stage] = stage == 0 && sh.columns < x ? kNoDigit : (uint32_t)(kBins - 1 - d);
+        }
+        __syncthreads();
+        const uint32_t digit = sh.digits[stage];
+        if (digit == kNoDigit) continue;
+        items([&](uint32_t k, uint32_t number) {
+            if (k >> 21 == digit) atomicAdd(&sh.keys[stage][k >> 16 & 31], number);
+        });
+        __syncthreads();
+        if (wave != 0) continue;
+        const uint32_t mine = (digit << 5 | (31 - (lane & 31))) << 16;
+        const uint32_t number = lane < 32 ? sh.keys[stage][31 - lane] : 0;
+        const uint64_t w = weights.of(mine), all = w * number;
+        count += wave_scan_u32(number) - number;
+        mass += wave_scan_u64(all) - all;
+        const uint64_t lo = stage ? mass : count, more = stage ? all : number;
+        const uint64_t hit = __ballot(lo < x && lo + more >= x);
+        const int at = hit ? __builtin_ctzll(hit) : 0;
+        const uint64_t weight = lane_u64(w, at);
+        key = (uint32_t)__builtin_amdgcn_readlane((int)mine, at);
+        x -= lane_u64(lo, at);
+        nth = stage ? columns_to(x, weight) : x;
+        head = min(head, lane_u64(mass, at) + nth * weight);  // (of the token's own search: not used)
+    }
+    if (t == 0) sh.choice = {key, nth, kept};
+    __syncthreads();
+    return sh.choice;
+}
+
+// The searches of a row of 32-bit logits: gather(digit) leaves the columns of a
+// first digit in sh.items (key and column) and their number in sh.gathered (past
+// kCached only that), barriers before and behind included; columns(f) calls f(key)
+// for this thread's share of them (and of any other columns).
+template <typename Gather, typename Columns>
+__device__ __forceinline__ Choice choose_wide(Search<2>& sh, const Weights<2>& weights, const Tally& tally,
+                                              const Row& r, int width, Gather&& gather, Columns&& columns) {
+    constexpr int kPer = Search<2>::kPer;
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    uint32_t held = kNoDigit;  // the digit whose columns are gathered
     uint32_t c[kPer];
-    uint64_t m[kPer], cb, mb, head, kept;
-    bins_before<TYPE, kPer>(sh, sh.count, sh.mass, c, m, cb, mb, head);
+    uint64_t m[kPer], cb, mb, head, kept, x;
+    bins_before<2, kPer>(sh, sh.count, sh.mass, c, m, cb, mb, head);
     kept = head;
     if (r.min_p > 0.f) before_wave(lane_u64(wave_scan_u64(tally.likely), 63), sh.sums[2], lane, wave, kept);
     Choice out = {0, 1, 0};
-    for (int stage = 0; stage < 3; ++stage) {  // top-k, top-p, the token; head: mass of what they keep so far
-        uint64_t x;
-        if (stage == 0) {
-            if (r.top_k <= 0 || r.top_k >= width) continue;
-            x = (uint64_t)r.top_k;
-        } else if (stage == 1) {
-            if (r.top_p >= 1.f) continue;
-            x = max((uint64_t)1, min(head, (uint64_t)__builtin_ceil((double)r.top_p * (double)head)));
-        } else {
-            kept = min(kept, head);
-            x = min(kept, (uint64_t)((double)r.u * (double)kept) + 1);
-        }
-        // the key at which the inclusive count or mass reaches x
+    auto found = [&](uint32_t digit, uint64_t count, uint64_t mass) {
+        sh.digit = digit;
+        sh.before_count = count;
+        sh.before_mass = mass;
+    };
+    for (int stage = 0; stage < 3; ++stage) {
+        if (!wanted(stage, r, width, head, kept, x)) continue;
         if (t == 0) sh.digit = kNoDigit;
-        if constexpr (TYPE != 2)
-            if (t < 32) sh.deep_count[t] = 0, sh.deep_mass[t] = 0;
         __syncthreads();
-        pick<TYPE, kPer>(sh, c, m, cb, mb, stage > 0, x);
+        pick<kPer>(c, m, cb, mb, stage > 0, x, found);
         __syncthreads();
         uint32_t prefix = sh.digit;
         if (prefix == kNoDigit) {  // fewer than top_k columns weigh anything
             __syncthreads();
             continue;
         }
-        if constexpr (TYPE != 2) {
-            // the other five bits of a 16-bit key, by one wave
-            items([&](uint32_t k, uint32_t number) {
-                if (k >> 21 != prefix) return;
-                atomicAdd(&sh.deep_count[k >> 16 & 31], number);
-                atomicAdd(&sh.deep_mass[k >> 16 & 31], (unsigned long long)(weights.of(k) * number));
-            });
+        if (prefix != held) gather(prefix);
+        held = prefix;
+        const int gathered = (int)sh.gathered;
+        for (int shift = 20; shift > 0; shift -= 10) {
+            const uint64_t bc = sh.before_count, bm = sh.before_mass;
+            sh.deep_count[t] = 0;
+            sh.deep_mass[t] = 0;
             __syncthreads();
-            if (wave == 0) {
-                const uint64_t dc = lane < 32 ? sh.deep_count[31 - lane] : 0, dm = lane < 32 ? sh.deep_mass[31 - lane] : 0;
-                const uint64_t lc = sh.before_count + wave_scan_u64(dc) - dc, lm = sh.before_mass + wave_scan_u64(dm) - dm;
-                const uint64_t lo = stage ? lm : lc, more = stage ? dm : dc;
-                if (lo < x && lo + more >= x) {
-                    const uint32_t key = (prefix << 5 | (31 - lane)) << 16;
-                    sh.digit = key;
-                    sh.before_count = lc;
-                    sh.before_mass = lm;
-                    settle<TYPE>(sh, stage > 0, x, weights.of(key));
-                }
-            }
+            auto deepen = [&](uint32_t k) {
+                if (k >> shift != prefix) return;
+                const uint32_t d = k >> (shift - 10) & 1023u;
+                atomicAdd(&sh.deep_count[d], 1u);
+                atomicAdd(&sh.deep_mass[d], (unsigned long long)weights.of(k));
+            };
+            if (gathered <= Search<2>::kCached)
+                for (int i = t; i < gathered; i += kThreads) deepen(sh.items[2 * i]);
+            else
+                columns(deepen);
             __syncthreads();
-            out.key = sh.digit;
-        } else {
-            if (prefix != held) items(prefix);
-            held = prefix;
-            const int gathered = (int)sh.gathered;
-            for (int shift = 20; shift > 0; shift -= 10) {
-                const uint64_t bc = sh.before_count, bm = sh.before_mass;
-                sh.deep_count[t] = 0;
-                sh.deep_mass[t] = 0;
-                __syncthreads();
-                auto deepen = [&](uint32_t k) {
-                    if (k >> shift != prefix) return;
-                    const uint32_t d = k >> (shift - 10) & 1023u;
-                    atomicAdd(&sh.deep_count[d], 1u);
-                    atomicAdd(&sh.deep_mass[d], (unsigned long long)weights.of(k));
-                };
-                if (gathered <= Search<TYPE>::kCached)
-                    for (int i = t; i < gathered; i += kThreads) deepen(sh.items[2 * i]);
-                else
-                    columns(deepen);
-                __syncthreads();
-                uint32_t dc[1];
-                uint64_t dm[1], dcb, dmb, all;
-                bins_before<TYPE, 1>(sh, sh.deep_count, sh.deep_mass, dc, dm, dcb, dmb, all);
-                pick<TYPE, 1>(sh, dc, dm, bc + dcb, bm + dmb, stage > 0, x);
-                __syncthreads();
-                prefix = prefix << 10 | sh.digit;
-            }
-            if (t == 0) settle<TYPE>(sh, stage > 0, x, weights.of(prefix));
+            uint32_t dc[1];
+            uint64_t dm[1], dcb, dmb, all;
+            bins_before<2, 1>(sh, sh.deep_count, sh.deep_mass, dc, dm, dcb, dmb, all);
+            pick<1>(dc, dm, bc + dcb, bm + dmb, stage > 0, x, found);
             __syncthreads();
-            out.key = prefix;
+            prefix = prefix << 10 | (sh.digit & 1023u);
         }
-        out.nth = sh.nth;
-        if (stage < 2) head = min(head, sh.through);
+        const uint64_t w = weights.of(prefix);
+        out.key = prefix;
+        out.nth = stage ? columns_to(x - sh.before_mass, w) : x - sh.before_count;
+        head = min(head, sh.before_mass + out.nth * w);  // (of the token's own search: not used)
         __syncthreads();
     }
     out.kept = kept;
@@ -431,18 +490,18 @@ __device__ __forceinline__ void refuse(const VocabSampleArgs& a, int row) {
     }
 }
 
-// By the thread that holds the token.
 template <int TYPE>
-__device__ __forceinline__ void publish(const VocabSampleArgs& a, int row, const Row& r, uint32_t top,
-                                        const Choice& choice, int column) {
+__device__ __forceinline__ float logprob_of(const Row& r, uint32_t top, const Choice& choice) {
+    if (!(r.temperature > 0.f)) return 0.f;
+    return (float)((value_of<TYPE>(choice.key) - value_of<TYPE>(top)) / (double)r.temperature -
+                   log((double)choice.kept / kOne));
+}
+
+// By the thread that holds the token.
+__device__ __forceinline__ void publish(const VocabSampleArgs& a, int row, int column, float logprob) {
     a.tokens[row] = column;
     a.valid[row] = 1;
-    if (!a.logprobs) return;
-    double logprob = 0.0;
-    if (r.temperature > 0.f)
-        logprob = (value_of<TYPE>(choice.key) - value_of<TYPE>(top)) / (double)r.temperature -
-                  log((double)choice.kept / kOne);
-    a.logprobs[row] = (float)logprob;
+    if (a.logprobs) a.logprobs[row] = logprob;
 }
 
 // The bit pattern of a key's logit (+0 for zero).
@@ -487,6 +546,10 @@ __device__ __forceinline__ void locate(Search<TYPE>& sh, const VocabSampleArgs& 
 #pragma unroll
         for (int i = 0; i < WORDS; ++i)
             if (i < each) word[i] = load_word<TYPE>(logits, first + i * 64 * kEach, a.width);
+        if (c0 == begin && t == kThreads - 1) {  // while they come (a barrier follows)
+            __builtin_amdgcn_sched_barrier(0);
+            sh.logprob = logprob_of<TYPE>(r, top, choice);
+        }
         uint32_t hits[WORDS];
         uint32_t mine = 0;
 #pragma unroll
@@ -510,7 +573,7 @@ __device__ __forceinline__ void locate(Search<TYPE>& sh, const VocabSampleArgs& 
                 if (before < choice.nth && before + number >= choice.nth) {
                     uint32_t left = hits[i];
                     for (uint64_t k = before + 1; k < choice.nth; ++k) left &= left - 1;
-                    publish<TYPE>(a, row, r, top, choice, first + i * 64 * kEach + __builtin_ctz(left));
+                    publish(a, row, first + i * 64 * kEach + __builtin_ctz(left), sh.logprob);
                 }
                 from += (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
             }
@@ -553,6 +616,7 @@ __global__ __launch_bounds__(kThreads) void vocab_sample_kernel(VocabSampleArgs 
         Search<TYPE> search;
     } sh;
     __shared__ uint32_t wave_top[kWaves], wave_bad[kWaves], wave_lost[kWaves], listed, last;
+    __shared__ double table[kTable];
     __shared__ Row r;
     const int row = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -571,8 +635,10 @@ __global__ __launch_bounds__(kThreads) void vocab_sample_kernel(VocabSampleArgs 
             if (first - t * 8 == begin) {
                 if (t == 0) {
                     r = params;
+                    r.prepare();
                     listed = 0;
                 }
+                fill_table(table);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) ((uint4*)sh.counts)[t + i * kThreads] = uint4{0, 0, 0, 0};
                 __syncthreads();
@@ -646,6 +712,7 @@ __global__ __launch_bounds__(kThreads) void vocab_sample_kernel(VocabSampleArgs 
     const int low = signs ? 0 : (int)pattern_of<TYPE>(least), high = signs ? (int)(pattern_of<TYPE>(least)) : 0;
     uint32_t* const lists = a.lists + (int64_t)row * a.chunks * a.list_words;
     uint32_t* const heads = a.heads + (int64_t)row * a.chunks * kSampleHead;
+    const __amdgpu_buffer_rsrc_t shared = device_rsrc(lists);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const int first = 8 * (t + i * kThreads);
@@ -687,6 +754,7 @@ __global__ __launch_bounds__(kThreads) void vocab_sample_kernel(VocabSampleArgs 
     // this workgroup searches the row (the counters' place is free)
     Search<TYPE>& s = sh.search;
     if (t == 0) store_device(a.counters + row, 0u);
+    clear<TYPE>(s);
     if (wave == 0) {
         uint32_t number = 0, key = 0, flag = 0;
         if (lane < a.chunks) {
@@ -694,10 +762,12 @@ __global__ __launch_bounds__(kThreads) void vocab_sample_kernel(VocabSampleArgs 
             key = load_device(heads + lane * kSampleHead + 1);
             flag = load_device(heads + lane * kSampleHead + 2);
         }
-        const uint64_t sum = wave_scan_u64((uint64_t)min(number, (uint32_t)a.list_words));
+        // (lists begin at multiples of four items)
+        const uint32_t words = min(number, (uint32_t)a.list_words), sum = wave_scan_u32((words + 3) & ~3u);
         if (lane < a.chunks) {
             s.starts[lane + 1] = (int)sum;
             s.held[lane] = 0;
+            s.number[lane] = (int)words;
         }
         if (lane == 0) s.starts[0] = 0;
         key = wave_max_u32(key);
@@ -717,79 +787,59 @@ __global__ __launch_bounds__(kThreads) void vocab_sample_kernel(VocabSampleArgs 
     }
     const int items = s.starts[a.chunks];
     constexpr int kCached = Search<TYPE>::kCached;
-    // f(c, i, v): word i of chunk c's list, four in flight, for the words whose
-    // number of all is at least `from`
+    // f(i, v): the items from i on, four at a time (0: there is none), for the
+    // fours from number `from` on; a load of four words each, four in flight
     auto each_listed = [&](int from, auto&& f) {
         constexpr int kAhead = 4;
-        for (int c = 0; c < a.chunks; ++c) {
-            const int n = s.starts[c + 1] - s.starts[c];
-            for (int i = max(0, from - s.starts[c]) + t; i < n; i += kAhead * kThreads) {
-                uint32_t v[kAhead];
+        for (int q0 = from / 4 + t; 4 * q0 < items; q0 += kAhead * kThreads) {
+            uint4 v[kAhead];
+            int rest[kAhead];
 #pragma unroll
-                for (int j = 0; j < kAhead; ++j)
-                    v[j] = i + j * kThreads < n ? load_device(lists + (int64_t)c * a.list_words + i + j * kThreads) : 0;
+            for (int j = 0; j < kAhead; ++j) {
+                const int i = 4 * (q0 + j * kThreads), c = chunk_of<TYPE>(s, a.chunks, i), k = i - s.starts[c];
+                rest[j] = i < items ? s.number[c] - k : 0;
+                // (past the end: an offset that reads nothing)
+                v[j] = __builtin_bit_cast(uint4, load_device4(shared, rest[j] > 0 ? (c * a.list_words + k) * 4 : -16));
+            }
 #pragma unroll
-                for (int j = 0; j < kAhead; ++j)
-                    if (v[j]) f(c, i + j * kThreads, v[j]);  // (a number is never 0)
+            for (int j = 0; j < kAhead; ++j) {
+                if (rest[j] <= 0) continue;
+                if (rest[j] < 4) v[j].w = 0;
+                if (rest[j] < 3) v[j].z = 0;
+                if (rest[j] < 2) v[j].y = 0;
+                f(4 * (q0 + j * kThreads), v[j]);
             }
         }
     };
-    // f(i, v): item i of all; the first kCached lie in LDS, four to a read
+    // f(i, v): item i of all (v = 0: none); the first kCached lie in LDS, four to a read
     auto each_item = [&](auto&& f) {
-        const int cached = min(items, kCached);
-        for (int i = 4 * t; i < cached; i += 4 * kThreads) {
-            const uint4 v = *(const uint4*)&s.items[i];
-            f(i, v.x);
-            if (i + 1 < cached) f(i + 1, v.y);
-            if (i + 2 < cached) f(i + 2, v.z);
-            if (i + 3 < cached) f(i + 3, v.w);
-        }
-        if (items > kCached) each_listed(kCached, [&](int c, int i, uint32_t v) { f(s.starts[c] + i, v); });
+        auto four = [&](int i, const uint4& v) { f(i, v.x), f(i + 1, v.y), f(i + 2, v.z), f(i + 3, v.w); };
+        for (int i = 4 * t; i < min(items, kCached); i += 4 * kThreads) four(i, *(const uint4*)&s.items[i]);
+        if (items > kCached) each_listed(kCached, four);
     };
     Choice choice = {top, 1, 0};
     if (r.temperature > 0.f) {
-        clear<TYPE>(s);
-        __syncthreads();
-        const Weights<TYPE> weights(s.table, top, r);
+        const Weights<TYPE> weights(table, top, r);
         Tally tally;
         if (whole) {
-            // every list once, four chunks' words in flight
-            constexpr int kAhead = 4;
-            for (int c0 = 0; c0 < a.chunks; c0 += kAhead) {
-                int longest = 0;
+            each_listed(0, [&](int i, const uint4& v) {
+                if (i < kCached) *(uint4*)&s.items[i] = v;
+                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-                for (int j = 0; j < kAhead; ++j)
-                    if (c0 + j < a.chunks) longest = max(longest, s.starts[c0 + j + 1] - s.starts[c0 + j]);
-                const int step = a.chunks == 1 ? kAhead * kThreads : kThreads;  // (one chunk: four of its words)
-                for (int i = t; i < longest; i += step) {
-                    uint32_t v[kAhead];
-                    int at[kAhead];
-#pragma unroll
-                    for (int j = 0; j < kAhead; ++j) {
-                        const int c = a.chunks == 1 ? 0 : min(c0 + j, a.chunks - 1), k = a.chunks == 1 ? i + j * kThreads : i;
-                        at[j] = s.starts[c] + k;
-                        v[j] = (a.chunks == 1 || c0 + j < a.chunks) && at[j] < s.starts[c + 1]
-                                   ? load_device(lists + (int64_t)c * a.list_words + k) : 0;
-                    }
-#pragma unroll
-                    for (int j = 0; j < kAhead; ++j) {
-                        if (!v[j]) continue;
-                        if (at[j] < kCached) s.items[at[j]] = v[j];
-                        add<TYPE>(s, weights, tally, v[j] & 0xffff0000u, v[j] & 0xffffu);
-                    }
-                }
-            }
+                for (int k = 0; k < 4; ++k)
+                    if (w[k]) add<TYPE>(s, weights, tally, w[k] & 0xffff0000u, w[k] & 0xffffu);
+            });
         } else {
             each_column<TYPE>(logits, 0, a.width, a.width, [&](int, uint32_t key) { add<TYPE>(s, weights, tally, key, 1u); });
         }
         __syncthreads();
-        choice = choose<TYPE>(s, weights, tally, r, a.width, [&](auto&& f) {
+        choice = choose_narrow<TYPE>(s, weights, tally, r, a.width, [&](auto&& f) {
             if (whole) each_item([&](int, uint32_t v) { f(v & 0xffff0000u, v & 0xffffu); });
             else each_column<TYPE>(logits, 0, a.width, a.width, [&](int, uint32_t key) { f(key, 1u); });
-        }, 0);
+        });
     } else if (whole) {
         // one item per chunk: its largest (two for +0 and -0)
-        each_listed(0, [&](int c, int i, uint32_t v) { s.items[s.starts[c] + i] = v; });
+        each_listed(0, [&](int i, const uint4& v) { *(uint4*)&s.items[i] = v; });
         __syncthreads();
     }
     // the chunk that holds the nth column of the key
@@ -797,9 +847,7 @@ __global__ __launch_bounds__(kThreads) void vocab_sample_kernel(VocabSampleArgs 
     if (whole && a.chunks > 1) {
         each_item([&](int i, uint32_t v) {
             if ((v & 0xffff0000u) != choice.key) return;
-            int c = 0;
-            while (s.starts[c + 1] <= i) ++c;
-            atomicAdd(&s.held[c], (int)(v & 0xffffu));
+            atomicAdd(&s.held[chunk_of<TYPE>(s, a.chunks, i)], (int)(v & 0xffffu));
         });
         __syncthreads();
         int c = 0;
@@ -884,6 +932,7 @@ __device__ __forceinline__ void gather(Search<2>& s, const uint8_t* logits, int 
 __global__ __launch_bounds__(kThreads) void vocab_sample_f32_kernel(VocabSampleArgs a) {
     __shared__ Search<2> s;
     __shared__ uint32_t row_top, row_bad, listed, last;
+    __shared__ double table[kTable];
     __shared__ Row r;
     constexpr int kPer = Search<2>::kPer;
     const int row = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
@@ -894,6 +943,7 @@ __global__ __launch_bounds__(kThreads) void vocab_sample_f32_kernel(VocabSampleA
     if (wave == 0) {
         if (t == 0) {
             r.read(a, row);
+            r.prepare();
             listed = 0;
         }
         const uint32_t key = lane < a.chunks ? heads[lane * kSampleHead] : 0;
@@ -906,6 +956,7 @@ __global__ __launch_bounds__(kThreads) void vocab_sample_f32_kernel(VocabSampleA
         }
     }
     clear<2>(s);
+    fill_table(table);
     __syncthreads();
     const uint32_t top = row_top;
     if (row_bad || top <= Limits<2>::kNegInf || !r.admitted()) {
@@ -917,7 +968,7 @@ __global__ __launch_bounds__(kThreads) void vocab_sample_f32_kernel(VocabSampleA
         if (chunk == 0) locate<2, 4>(s, a, row, logits, 0, a.width, r, top, choice);
         return;
     }
-    const Weights<2> weights(s.table, top, r);
+    const Weights<2> weights(table, top, r);
     Tally tally;
     const int begin = chunk * a.chunk, end = min(a.width, begin + a.chunk);
     const uint32_t least = least_key<2>(top, r.temperature);
@@ -1002,10 +1053,8 @@ __global__ __launch_bounds__(kThreads) void vocab_sample_f32_kernel(VocabSampleA
             uint4 v[kAhead];
 #pragma unroll
             for (int i = 0; i < kAhead; ++i) {
-                const int at = min(i0 + i * kThreads, all - 1);
-                int c = 0;
-                while (s.starts[c + 1] <= at) ++c;
-                v[i] = __builtin_bit_cast(uint4, load_device4(shared, (c * a.list_words + 4 * (at - s.starts[c])) * 4));
+                const int at = i0 + i * kThreads, c = chunk_of<2>(s, a.chunks, at);
+                v[i] = __builtin_bit_cast(uint4, load_device4(shared, at < all ? (c * a.list_words + 4 * (at - s.starts[c])) * 4 : -16));
             }
 #pragma unroll
             for (int i = 0; i < kAhead; ++i) {
@@ -1025,8 +1074,7 @@ __global__ __launch_bounds__(kThreads) void vocab_sample_f32_kernel(VocabSampleA
 #pragma unroll
             for (int i = 0; i < kAhead; ++i) {
                 const int at = min(i0 + i * kThreads, number - 1);
-                int h = 0;
-                while (s.starts[h + 1] <= at) ++h;
+                const int h = chunk_of<2>(s, a.chunks, at);
                 const uint16_t* from = (const uint16_t*)(lists + (int64_t)h * a.list_words + columns);
                 c[i] = h * a.chunk + (int)load_device(from + s.held[h] + at - s.starts[h]);
             }
@@ -1037,7 +1085,7 @@ __global__ __launch_bounds__(kThreads) void vocab_sample_f32_kernel(VocabSampleA
                 if (i0 + i * kThreads < number) f(i0 + i * kThreads, key_of<2>(bits[i]), c[i]);
         }
     };
-    choice = choose<2>(s, weights, tally, r, a.width, [&](uint32_t digit) {
+    choice = choose_wide(s, weights, tally, r, a.width, [&](uint32_t digit) {
         __syncthreads();
         if (!a.sorted) {
             if (t == 0) s.gathered = 0;
@@ -1077,6 +1125,7 @@ __global__ __launch_bounds__(kThreads) void vocab_sample_f32_kernel(VocabSampleA
     if (t == 0) listed = 0;
     __syncthreads();
     if (gathered <= Search<2>::kCached) {
+        if (t == kThreads - 1) s.logprob = logprob_of<2>(r, top, choice);
         constexpr uint32_t kFew = 256;
         for (int i = t; i < gathered; i += kThreads)
             if (s.items[2 * i] == choice.key) {
@@ -1089,7 +1138,7 @@ __global__ __launch_bounds__(kThreads) void vocab_sample_f32_kernel(VocabSampleA
                 const uint32_t mine = s.deep_count[t];
                 uint32_t before = 0;
                 for (uint32_t i = 0; i < listed; ++i) before += s.deep_count[i] < mine;
-                if (before + 1 == choice.nth) publish<2>(a, row, r, top, choice, (int)mine);
+                if (before + 1 == choice.nth) publish(a, row, (int)mine, s.logprob);
             }
             return;
         }
