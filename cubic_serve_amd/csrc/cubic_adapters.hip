@@ -484,12 +484,13 @@ __device__ __forceinline__ float split_row(const floatx4_t (&v)[KS][2], int rank
 }
 
 // The parts of t of this lane's row (row0 + row, if own; rows of them from row0 on
-// are there): the partitions in ascending order, kParts requested together; what is not there
-// (another row, past the rank) reads as 0.
-template <bool F16, int KS>
+// are there): the partitions in ascending order, kParts requested together (four
+// of 32 ranks: 26.0 us of 256 rows, rank 64, K = 12288, with eight 26.3, sixteen 27.5; what
+// the registers cost is more than the wait); what is not there (another row, past
+// the rank) reads as 0.
+template <bool F16, int KS, int kParts>
 __device__ __forceinline__ float row_parts(const AdapterArgs& a, const AdapterMember& mb, int row0, int rows, int row,
                                            bool own, int rank, float scale, int q, uint4 (&hi)[KS], uint4 (&lo)[KS]) {
-    constexpr int kParts = KS < 8 ? 8 / KS : 1;
     uint32_t off[KS][2];
     floatx4_t v[KS][2];
 #pragma unroll
@@ -603,7 +604,7 @@ __global__ __launch_bounds__(kThreads) void adapter_up_kernel(AdapterArgs a) {
         if (rank <= 0 && in_place) continue;
         const float scale = e >= 0 ? mb.scales[e] : 0.f;
         uint4 hi[KS], lo[KS];
-        const float back = row_parts<F16, KS>(a, mb, row0, rows, row_of(col), (mine >> col) & 1, rank, scale, q, hi, lo);
+        const float back = row_parts<F16, KS, KS < 4 ? 4 / KS : 1>(a, mb, row0, rows, row_of(col), (mine >> col) & 1, rank, scale, q, hi, lo);
         const auto up = buffer(mb.up + (e >= 0 ? (int64_t)e * n * max_rank : 0), (int64_t)n * max_rank * 2);
         for (int c0 = c_begin; c0 < c_end; c0 += kColWaves * kTurn) {
             // base and y: rows q, q + 4, ..., eight columns per lane; what is
@@ -727,7 +728,7 @@ __global__ __launch_bounds__(kThreads) void adapter_up_tile_kernel(AdapterArgs a
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) next[i] = load16(base, row_at(i, c_begin, ldbase) + 2 * (c_begin + rc));
         uint4 hi[KS], lo[KS];
-        const float back = row_parts<F16, KS>(a, mb, row0, 16, col, (mine >> col) & 1, rank, scale, q, hi, lo);
+        const float back = row_parts<F16, KS, 1>(a, mb, row0, 16, col, (mine >> col) & 1, rank, scale, q, hi, lo);
         int h = 0;
         for (int c0 = c_begin; c0 < c_end; c0 += kTurn, h ^= 1) {
             // this wave's loads of the turn have landed (the last turn's
