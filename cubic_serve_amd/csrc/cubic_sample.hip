@@ -174,7 +174,7 @@ struct Search {
     static constexpr int kDeepBins = TYPE == 2 ? 1024 : 1;
     // items held in LDS: key's upper half | number; or (32 bits) the columns of
     // one first digit, key and column
-    static constexpr int kCached = TYPE == 2 ? 8192 : kSampleList;
+    static constexpr int kCached = TYPE == 2 ? 8192 : 28672;
     alignas(16) uint32_t items[TYPE == 2 ? 2 * kCached : kCached];
     uint32_t count[kBins], deep_count[kDeepBins];
     unsigned long long mass[kBins], deep_mass[kDeepBins];
@@ -188,6 +188,7 @@ struct Search {
     uint64_t before_count, before_mass;
     // 16 bits: each search's digit, the counts of that digit's keys
     uint32_t digits[3], keys[3][32], columns;
+    uint32_t split[TYPE == 2 ? 1 : 32][kMaxSampleChunks];  // the token's digit's by chunk
     Choice choice;
     float logprob;
 };
@@ -258,6 +259,7 @@ __device__ __forceinline__ void clear(Search<TYPE>& sh) {
     }
     if constexpr (TYPE != 2) {
         if (t < 96) (&sh.keys[0][0])[t] = 0;
+        for (int i = t; i < 32 * kMaxSampleChunks; i += kThreads) (&sh.split[0][0])[i] = 0;
     }
 }
 template <int TYPE>
@@ -344,8 +346,8 @@ __device__ __forceinline__ bool wanted(int stage, const Row& r, int width, uint6
 }
 
 // The searches of a row of 16-bit logits.  Called by the whole workgroup once
-// the items are added, after a barrier; items(f) calls f(key, number) for this
-// thread's share of them; columns whose weight is 0 may be left out.  What is
+// the items are added, after a barrier; items(f) calls f(key, number, chunk()) for
+// this thread's share of them; columns whose weight is 0 may be left out.  What is
 // serial is done by one wave: sixteen that do it side by side share four issue
 // ports (a search 4700 cycles, 3000 to 4300 so).
 template <int TYPE, typename Items>
@@ -390,8 +392,10 @@ __device__ __forceinline__ Choice choose_narrow(Search<TYPE>& sh, const Weights<
         __syncthreads();
         const uint32_t digit = sh.digits[stage];
         if (digit == kNoDigit) continue;
-        items([&](uint32_t k, uint32_t number) {
-            if (k >> 21 == digit) atomicAdd(&sh.keys[stage][k >> 16 & 31], number);
+        items([&](uint32_t k, uint32_t number, auto&& chunk) {
+            if (k >> 21 != digit) return;
+            atomicAdd(&sh.keys[stage][k >> 16 & 31], number);
+            if (stage == 2) atomicAdd(&sh.split[k >> 16 & 31][chunk()], number);
         });
         __syncthreads();
         if (wave != 0) continue;
@@ -709,20 +713,21 @@ __global__ __launch_bounds__(kThreads) void vocab_sample_kernel(VocabSampleArgs 
     // positive, up to `high` among the negative ones
     const uint32_t least = r.temperature > 0.f ? least_key<TYPE>(top, r.temperature) : top;
     const bool signs = least < 0x80000000u;  // negative ones too
-    const int low = signs ? 0 : (int)pattern_of<TYPE>(least), high = signs ? (int)(pattern_of<TYPE>(least)) : 0;
+    const int low = signs ? 0 : (int)pattern_of<TYPE>(least);
+    const int high = signs ? (int)pattern_of<TYPE>(least) : low == 0 ? 0x8000 : 0;  // (-0)
     uint32_t* const lists = a.lists + (int64_t)row * a.chunks * a.list_words;
     uint32_t* const heads = a.heads + (int64_t)row * a.chunks * kSampleHead;
     const __amdgpu_buffer_rsrc_t shared = device_rsrc(lists);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int first = 8 * (t + i * kThreads);
-        uint32_t in;
-        if (i < 4) in = 0xffu << min(max(low - first, 0), 8) & 0xffu;
-        else in = signs ? (1u << min(max(high + 1 - first, 0), 8)) - 1 : first == 0x8000 && low == 0 ? 1u : 0u;  // -0
-        there &= ~((uint64_t)(~in & 0xffu) << (8 * i));
-    }
+    // how many of this thread's patterns of one sign lie below p
+    auto below = [&](int p) {
+        const int x = max(p - 8 * t, 0);
+        return min(8 * (x >> 13) + min(x & 8191, 8), 32);
+    };
+    const uint64_t keep_plus = 0xffffffffull << below(low) & 0xffffffffull;
+    const uint64_t keep_minus = (1ull << below(high + 1 - 0x8000)) - 1;
+    there &= keep_minus << 32 | keep_plus;
     const uint32_t mine = (uint32_t)__builtin_popcountll(there);
-    const uint32_t wave_mine = (uint32_t)lane_u64(wave_scan_u64((uint64_t)mine), 63);
+    const uint32_t wave_mine = (uint32_t)__builtin_amdgcn_readlane((int)wave_scan_u32(mine), 63);
     int base = 0;
     if (lane == 0 && wave_mine) base = (int)atomicAdd(&listed, wave_mine);
     base = __builtin_amdgcn_readfirstlane(base);
@@ -766,7 +771,6 @@ __global__ __launch_bounds__(kThreads) void vocab_sample_kernel(VocabSampleArgs 
         const uint32_t words = min(number, (uint32_t)a.list_words), sum = wave_scan_u32((words + 3) & ~3u);
         if (lane < a.chunks) {
             s.starts[lane + 1] = (int)sum;
-            s.held[lane] = 0;
             s.number[lane] = (int)words;
         }
         if (lane == 0) s.starts[0] = 0;
@@ -834,24 +838,26 @@ __global__ __launch_bounds__(kThreads) void vocab_sample_kernel(VocabSampleArgs 
         }
         __syncthreads();
         choice = choose_narrow<TYPE>(s, weights, tally, r, a.width, [&](auto&& f) {
-            if (whole) each_item([&](int, uint32_t v) { f(v & 0xffff0000u, v & 0xffffu); });
-            else each_column<TYPE>(logits, 0, a.width, a.width, [&](int, uint32_t key) { f(key, 1u); });
+            if (whole) each_item([&](int i, uint32_t v) { f(v & 0xffff0000u, v & 0xffffu, [&] { return chunk_of<TYPE>(s, a.chunks, i); }); });
+            else each_column<TYPE>(logits, 0, a.width, a.width, [&](int c, uint32_t key) { f(key, 1u, [&] { return min(c / a.chunk, a.chunks - 1); }); });
         });
     } else if (whole) {
         // one item per chunk: its largest (two for +0 and -0)
-        each_listed(0, [&](int i, const uint4& v) { *(uint4*)&s.items[i] = v; });
+        each_listed(0, [&](int i, const uint4& v) {
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if ((w[k] & 0xffff0000u) == top) atomicAdd(&s.split[top >> 16 & 31][chunk_of<TYPE>(s, a.chunks, i)], w[k] & 0xffffu);
+        });
         __syncthreads();
     }
     // the chunk that holds the nth column of the key
     int b = 0, e = a.width;
-    if (whole && a.chunks > 1) {
-        each_item([&](int i, uint32_t v) {
-            if ((v & 0xffff0000u) != choice.key) return;
-            atomicAdd(&s.held[chunk_of<TYPE>(s, a.chunks, i)], (int)(v & 0xffffu));
-        });
-        __syncthreads();
-        int c = 0;
-        while (c + 1 < a.chunks && choice.nth > (uint64_t)s.held[c]) choice.nth -= s.held[c++];
+    if (a.chunks > 1 && (whole || r.temperature > 0.f)) {
+        const uint32_t number = lane < a.chunks ? s.split[choice.key >> 16 & 31][lane] : 0, upto = wave_scan_u32(number);
+        const uint64_t hit = __ballot(upto >= choice.nth);
+        const int c = hit ? __builtin_ctzll(hit) : a.chunks - 1;
+        choice.nth -= (uint32_t)__builtin_amdgcn_readlane((int)(upto - number), c);
         b = c * a.chunk;
         e = min(a.width, b + a.chunk);
     }
