@@ -267,8 +267,10 @@ __global__ __launch_bounds__(kThreads) void adapter_down_kernel(AdapterArgs a) {
 // two workgroups per CU).  The kernel above has each wave read A from the caches for
 // its own 32 rows: at K = 8192, rank 128, 4096 rows that is 0.4 GB into the CUs
 // beside 0.07 from memory.  Here waves share the ranks in halves and the rows in
-// halves, and A is read once per 64 rows: 54 -> 27.5 us with one adapter, 57 -> 52
-// with 24 requests (a tile on a boundary is done once per adapter).  Four blocks
+// halves, and A is read once per 64 rows: 54 -> 27.5 us with one adapter.  A tile on a
+// boundary is done once per adapter, at the end alone on its CU: with two requests
+// and up 39 to 52 (workgroups of their own for the second adapter wait for a place
+// until the others end: 44 and 41 with three requests).  Four blocks
 // make a quarter; quarters add as above, bit for bit.  LDS image of a 16-row block:
 // 16-byte chunk c of row r in slot 8 r + (c ^ (r / 2) mod 8), so that the 16 rows of
 // a fragment read lie in distinct banks.
@@ -550,6 +552,15 @@ __device__ __forceinline__ void store8(__amdgpu_buffer_rsrc_t r, uint32_t row, i
     }
 }
 
+// Eight values of LDS at column c = 0, 8, ...: every other four lanes take their
+// second half first, so that the eight lanes of a pass lie in distinct banks.
+__device__ __forceinline__ void eight_of(const float* from, int c, floatx4_t& d0, floatx4_t& d1) {
+    const int first = c >> 3 & 4;
+    const floatx4_t a = *(const floatx4_t*)(from + first), b = *(const floatx4_t*)(from + (first ^ 4));
+    d0 = first ? b : a;
+    d1 = first ? a : b;
+}
+
 // Two 16-bit values plus two binary32 ones, each sum rounded once.
 template <bool F16>
 __device__ __forceinline__ uint32_t add_pair(uint32_t in, float lo, float hi) {
@@ -647,8 +658,8 @@ __global__ __launch_bounds__(kThreads) void adapter_up_kernel(AdapterArgs a) {
                 __builtin_amdgcn_wave_barrier();
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const floatx4_t d0 = *(const floatx4_t*)&product[wave][4 * i + q][8 * col];
-                    const floatx4_t d1 = *(const floatx4_t*)&product[wave][4 * i + q][8 * col + 4];
+                    floatx4_t d0, d1;
+                    eight_of(&product[wave][4 * i + q][8 * col], 8 * col, d0, d1);
                     in[i].x = add_pair<F16>(in[i].x, d0[0], d0[1]);
                     in[i].y = add_pair<F16>(in[i].y, d0[2], d0[3]);
                     in[i].z = add_pair<F16>(in[i].z, d1[0], d1[1]);
@@ -668,8 +679,8 @@ __global__ __launch_bounds__(kThreads) void adapter_up_kernel(AdapterArgs a) {
 // (direct loads, the next turn's under way): what bounds the kernel above at many
 // rows is what its waves read of B, each for its 16 rows (8192 columns, rank
 // 128, 4096 rows: 0.31 GB beside the 0.13 of base and y, 88 us).  LDS image of
-// 32 ranks of B: 16-byte chunk q of column c in slot 4 c + (q ^ (c / 4) mod 4), so that
-// the 16 columns of a fragment read lie in distinct banks.
+// 32 ranks of B: 16-byte chunk q of column c in slot 4 c + (q ^ (c / 2) mod 4), so that
+// eight columns of a fragment read, what one pass takes, lie in distinct banks.
 // ---------------------------------------------------------------------------
 template <bool F16, int KS, int kTurn>
 __global__ __launch_bounds__(kThreads) void adapter_up_tile_kernel(AdapterArgs a) {
@@ -697,7 +708,7 @@ __global__ __launch_bounds__(kThreads) void adapter_up_tile_kernel(AdapterArgs a
     const bool in_place = mb.base == mb.y;
     const int slot = tile_slots(a, tile0, 64, slots_lds);
     // this lane's part of a slab's 1 KB pieces (two per wave): column, chunk
-    const int dc = lane >> 2, dq = (lane & 3) ^ (dc >> 2 & 3);
+    const int dc = lane >> 2, dq = (lane & 3) ^ (dc >> 1 & 3);
     uint64_t left = __ballot(slot != -1);
     while (left) {
         const int e = __builtin_amdgcn_readlane(slot, __builtin_ctzll(left));
@@ -748,7 +759,7 @@ __global__ __launch_bounds__(kThreads) void adapter_up_tile_kernel(AdapterArgs a
                 for (int i = 0; i < kPieces; ++i) next[i] = load16(base, row_at(i, c0 + kTurn, ldbase) + 2 * (c0 + kTurn + rc));
             }
             __builtin_amdgcn_sched_barrier(0);
-            const uint8_t* from = stage + h * KS * kSlab + col * 64 + ((q ^ (col >> 2)) & 3) * 16;
+            const uint8_t* from = stage + h * KS * kSlab + col * 64 + ((q ^ (col >> 1)) & 3) * 16;
 #pragma unroll
             for (int u = 0; u < kTiles; ++u) {
                 floatx4_t acc = {0.f, 0.f, 0.f, 0.f};
@@ -763,8 +774,8 @@ __global__ __launch_bounds__(kThreads) void adapter_up_tile_kernel(AdapterArgs a
             __builtin_amdgcn_wave_barrier();
 #pragma unroll
             for (int i = 0; i < kPieces; ++i) {
-                const floatx4_t d0 = *(const floatx4_t*)&product[wave][kRowsAt * i + rr][rc];
-                const floatx4_t d1 = *(const floatx4_t*)&product[wave][kRowsAt * i + rr][rc + 4];
+                floatx4_t d0, d1;
+                eight_of(&product[wave][kRowsAt * i + rr][rc], rc, d0, d1);
                 if (rank > 0) {
                     in[i].x = add_pair<F16>(in[i].x, d0[0], d0[1]);
                     in[i].y = add_pair<F16>(in[i].y, d0[2], d0[3]);

@@ -880,10 +880,11 @@ int cubic_adapters(const void* x, int64_t ldx, const int32_t* row_slots, int64_t
     // against each wave's own reads: rank 32 51.6 -> 46.5 us, rank 128 67.8 -> 53.
     a.join = m > 1024 && a.split > 1;
     a.up_tile = m > 1024 && a.vectors && a.rank_tiles <= 8;
-    // Columns of a workgroup, while 512 workgroups are left.  Prompts: 256 and 512 at
-    // rank 128 (4096 rows) 53 and 58.5 us, at rank 32 (2048 rows, 2 x 12288 columns) 48
-    // and 46.5.  In order of adapters: 2048 and 512, 1024 rows x 2 x 12288 columns 49 and 64.
-    a.chunk_cols = (by_slot ? 16 : a.up_tile && a.rank_tiles > 4 ? 2 : 4) * cubic::kAdapterUpTurn;
+    // Columns of a workgroup, while 512 workgroups are left.  Prompts, in all: 256 and
+    // 512 at rank 128 (4096 rows) 103 and 110 us, at rank 32 (2048 rows, 2 x 12288
+    // columns) 64.4 and 67.4.  In order of adapters: 2048 and 512, 1024 rows x 2 x 12288
+    // columns 49 and 64.
+    a.chunk_cols = (by_slot ? 16 : a.up_tile ? 2 : 4) * cubic::kAdapterUpTurn;
     while (a.chunk_cols > cubic::kAdapterUpTurn && items * ceil_div(columns, a.chunk_cols) < 512) a.chunk_cols /= 2;
     int64_t chunks = 0;
     for (int j = 0; j < cubic::kMaxGemmMembers; ++j) {
