@@ -8,6 +8,11 @@ Two halves, both hand-written HIP for gfx950 behind a C ABI
   bind_linear_group, the Cubic extension hooks).
 * ``sampling`` -- acceptance: candidate preparation, K1 p/q verification,
   accepted-prefix merge, and the fused single-pass verify-from-logits plan.
+
+For batches whose requests differ: ``adapters`` -- a low-rank adapter per
+request beside a shared projection (PackedLinearOperators.bind_adapters,
+bind_adapted_linear), and ``sampling.VocabSamplingPlan`` -- a token per row from
+the whole vocabulary under each request's own settings.
 """
 from .quantization import (  # noqa: F401
     CUBIC_FORMAT,

@@ -411,7 +411,8 @@ _MAX_SAMPLE_WIDTH = 1 << 20  # kMaxSampleWidth of the C ABI
 
 
 class VocabSamplingPlan:
-    """One token per row from logits over the whole vocabulary, in one launch.
+    """One token per row from logits over the whole vocabulary, in one launch
+    (two for 32-bit logits).
 
     Columns are ordered by logit, ties by ascending token id.  Of that order a
     row keeps the first ``top_ks`` (<= 0: all), of these each whose preceding

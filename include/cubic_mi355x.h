@@ -166,7 +166,8 @@ CUBIC_API int cubic_gemm_grouped(const void* x, int64_t ldx, const uint32_t* cod
  * 17 bits or more).  A slot outside [0, slots) or of rank 0 leaves y = base.
  *   x          dtype [m, ldx], 16-byte aligned, k % 8 == 0, ldx % 8 == 0
  *   row_slots  int32 [m], any order
- *   downs[j]   dtype [slots, max_ranks[j], k], 16-byte aligned
+ *   downs[j]   dtype [slots, max_ranks[j], k], 16-byte aligned; rows at or past a
+ *              slot's rank may hold anything
  *   ups[j]     dtype [slots, ns[j], max_ranks[j]], 16-byte aligned; entries at or
  *              past a slot's rank, up to the next multiple of 8, must be zero
  *   scales[j]  f32 [slots]; ranks[j] int32 [slots], 0 = empty slot; a rank past
@@ -270,6 +271,10 @@ CUBIC_API int cubic_root_sample(const void* scores, int scores_fp16, const int64
  * the ranges above, publishes -1, 0, NaN.  Rows at or past live_rows (live_count[0],
  * a device int32 read when the launch runs, if given) are left as they are.
  *   1 <= rows < 2^24, 1 <= width <= 2^20, width <= row_stride
+ * Workspace: cubic_vocab_sample_workspace_bytes(rows, width, dtype) bytes (-1:
+ * outside the ranges above), 16-byte aligned, zero-filled before the first launch; a
+ * completed launch leaves the counters in it zero again.  One per launch that may
+ * run at the same time, one geometry (rows, width, dtype).
  * ------------------------------------------------------------------------- */
 CUBIC_API int64_t cubic_vocab_sample_workspace_bytes(int rows, int width, int dtype);
 CUBIC_API int cubic_vocab_sample(const void* logits, int dtype, int64_t row_stride, int rows, int width,
