@@ -705,22 +705,33 @@ int cubic_embedding(const void* ids, int id_bytes, int64_t tokens, int fmt, cons
 // ---------------------------------------------------------------------------
 namespace {
 struct SamplePlan {
-    int chunks, chunk, list_words, sorted;
+    int chunks, chunk, list_words;
     int64_t counters, heads, bytes;  // bytes of the counters, of the heads, of all
 };
 // Chunks of a row: as many as fill the chip with all rows' (256 workgroups, one
-// per CU: what they count takes most of its LDS), of 8192 columns or more.
+// per CU: what they count takes most of its LDS), but not many more than pay: the
+// row's last workgroup goes through every chunk's distinct logits, which for 16 bits
+// grow slowly with the chunk.  Columns per chunk, one row of 151936 (us): bf16 8192
+// 41.8, 16384 29.7, 32768 26.0, 65536 26.9, all 30.8; fp16 106, 78, 54, 40, 39; 64
+// rows fp16 59 down to 45.  32-bit logits, which are hardly ever equal: 35.0, 38.5, 56.8,
+// 70.9, 97.9; past 32768 columns a chunk cannot leave its columns in order: 64 rows of
+// 151936 in five chunks and in four 78 and 110, 128 rows in five and in two 114 and
+// 132 (but 180 rows of 40000 in two and in one 78 and 61).
 SamplePlan plan_sample(int rows, int width, int dtype) {
     SamplePlan p = {};
-    p.chunks = std::max(1, std::min({256 / rows, width / 8192, cubic::kMaxSampleChunks}));
+    const int most = dtype == CUBIC_DTYPE_F32    ? width / 8192
+                     : dtype == CUBIC_DTYPE_BF16 ? (width + 16384) / 32768
+                                                 : width / 65536;
+    p.chunks = std::max(1, std::min({256 / rows, most, cubic::kMaxSampleChunks}));
+    if (dtype == CUBIC_DTYPE_F32 && p.chunks > 1)
+        p.chunks = std::max(p.chunks, (int)ceil_div(width, cubic::kSampleList));
     p.chunk = (int)ceil_div(ceil_div(width, p.chunks), 8) * 8;
     p.chunks = (int)ceil_div(width, p.chunk);
+    // 32 bits: bins of four words, where each bin's columns begin, column numbers
+    // of 16 bits; a row of one chunk leaves nothing
     p.list_words = dtype != CUBIC_DTYPE_F32 ? std::min(p.chunk, cubic::kSampleList)
                    : p.chunks == 1          ? 0
-                                            : 4 * std::min(p.chunk, cubic::kSampleBins);
-    // column numbers of 16 bits, as many as LDS holds
-    p.sorted = dtype == CUBIC_DTYPE_F32 && p.chunks > 1 && p.chunk <= cubic::kSampleList;
-    if (p.sorted) p.list_words += cubic::kSampleBins / 2 + p.chunk / 2;
+                                            : 4 * std::min(p.chunk, cubic::kSampleBins) + cubic::kSampleBins / 2 + p.chunk / 2;
     p.counters = align256((int64_t)rows * 4);
     p.heads = align256((int64_t)rows * p.chunks * cubic::kSampleHead * 4);
     p.bytes = p.counters + p.heads + (int64_t)rows * p.chunks * p.list_words * 4;
@@ -760,7 +771,6 @@ int cubic_vocab_sample(const void* logits, int dtype, int64_t row_stride, int ro
     a.chunks = p.chunks;
     a.chunk = p.chunk;
     a.list_words = p.list_words;
-    a.sorted = p.sorted;
     a.counters = (uint32_t*)workspace;
     a.heads = (uint32_t*)((uint8_t*)workspace + p.counters);
     a.lists = (uint32_t*)((uint8_t*)workspace + p.counters + p.heads);

@@ -253,7 +253,7 @@ struct GuardArgs {
 // Sampling from the whole vocabulary (cubic_sample.hip)
 constexpr int kMaxSampleWidth = 1 << 20;
 constexpr int kMaxSampleChunks = 64;
-constexpr int kSampleList = 32768;     // distinct 16-bit logits that a chunk's list holds
+constexpr int kSampleList = 32768;     // distinct 16-bit logits, or 32-bit ones' columns, that a chunk's list holds
 constexpr int kSampleBins = 4096;      // bins of a chunk's list of 32-bit logits, four words each
 constexpr int kSampleHead = 8;         // words of a chunk's head
 struct VocabSampleArgs {
@@ -273,7 +273,6 @@ struct VocabSampleArgs {
     // chunks of `chunk` columns (a multiple of 8), a workgroup each: counters [rows],
     // zero between launches, heads [rows, chunks, kSampleHead], lists [rows, chunks, list_words]
     int chunks, chunk, list_words;
-    int sorted;                   // 32-bit logits: the lists hold the chunks' columns in order of bins
     uint32_t *counters, *heads, *lists;
 };
 hipError_t launch_vocab_sample(const VocabSampleArgs& a, hipStream_t s);

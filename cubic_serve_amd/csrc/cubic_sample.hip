@@ -869,8 +869,8 @@ __global__ __launch_bounds__(kThreads) void vocab_sample_kernel(VocabSampleArgs 
 // the chunks' largest, so that the second can weigh its columns against the
 // row's: each chunk's masses by the keys' first 12 bits, joined by the row's last
 // workgroup to arrive, which gathers the columns of the bin in which a search
-// ends and finishes the search among those.  Where a row has several chunks of at
-// most 32768 columns, each leaves its columns' numbers in order of bins, so that
+// ends and finishes the search among those.  Where a row has several chunks (of at
+// most 32768 columns then), each leaves its columns' numbers in order of bins, so that
 // a bin is a run of each chunk's: 128001 columns, 48 rows, three searches, 78 -> 50 us
 // against scans of the row by the one workgroup (17 us each, what one CU reads).
 // With a chunk per row there is nothing to share out, and the scans stay.
@@ -1006,31 +1006,32 @@ __global__ __launch_bounds__(kThreads) void vocab_sample_f32_kernel(VocabSampleA
             const uint32_t at = atomicAdd(&listed, 1u) * 4;
             store_device4(shared, (list + (int)at) * 4, __builtin_bit_cast(floatx4_dev_t, uint4{(uint32_t)b, number[i], (uint32_t)m, (uint32_t)(m >> 32)}));
         }
-        if (a.sorted) {
-            // where each bin's columns begin, and the columns, in order of bins
-            const uint32_t scan = wave_scan_u32(before);
-            if (lane == 63) s.count_sums[wave] = scan;
-            __syncthreads();
-            const uint32_t upto = wave_scan_u32(lane < kWaves ? s.count_sums[lane] : 0);
-            before = (wave ? (uint32_t)__builtin_amdgcn_readlane((int)upto, wave - 1) : 0) + scan - before;
-            const int held = __builtin_amdgcn_readlane((int)upto, kWaves - 1);
-            uint64_t begins = 0;
+        // where each bin's columns begin, and the columns, in order of bins
+        const uint32_t scan = wave_scan_u32(before);
+        if (lane == 63) s.count_sums[wave] = scan;
+        __syncthreads();
+        const uint32_t upto = wave_scan_u32(lane < kWaves ? s.count_sums[lane] : 0);
+        before = (wave ? (uint32_t)__builtin_amdgcn_readlane((int)upto, wave - 1) : 0) + scan - before;
+        const int held = __builtin_amdgcn_readlane((int)upto, kWaves - 1);
+        uint64_t begins = 0;
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) {
-                s.cursor[t * kPer + i] = before;
-                begins |= (uint64_t)before << (16 * i);
-                before += number[i];
-            }
-            store_device((uint64_t*)(lists + list + runs) + t, begins);
-            __syncthreads();
-            uint16_t* const order = (uint16_t*)s.items;
-            each_column<2>(logits, begin, end, a.width, [&](int c, uint32_t key) {
-                if (key >= least) order[atomicAdd(&s.cursor[key >> Search<2>::kShift], 1u)] = (uint16_t)(c - begin);
-            });
-            __syncthreads();
-            for (int i = t; i < (held + 7) / 8; i += kThreads)
-                store_device4(shared, (list + columns) * 4 + 16 * i, ((const floatx4_dev_t*)order)[i]);
+        for (int i = 0; i < kPer; ++i) {
+            s.cursor[t * kPer + i] = before;
+            begins |= (uint64_t)before << (16 * i);
+            before += number[i];
         }
+        store_device((uint64_t*)(lists + list + runs) + t, begins);
+        __syncthreads();
+        uint16_t* const order = (uint16_t*)s.items;
+        each_column<2>(logits, begin, end, a.width, [&](int c, uint32_t key) {
+            if (key < least) return;
+            // (within the list also if the caller rewrites the logits meanwhile)
+            const uint32_t at = atomicAdd(&s.cursor[key >> Search<2>::kShift], 1u);
+            if (at < (uint32_t)held) order[at] = (uint16_t)(c - begin);
+        });
+        __syncthreads();
+        for (int i = t; i < (held + 7) / 8; i += kThreads)
+            store_device4(shared, (list + columns) * 4 + 16 * i, ((const floatx4_dev_t*)order)[i]);
         __syncthreads();
         if (t == 0) {
             store_device(heads + chunk * kSampleHead + 2, listed);
@@ -1082,7 +1083,7 @@ __global__ __launch_bounds__(kThreads) void vocab_sample_f32_kernel(VocabSampleA
                 const int at = min(i0 + i * kThreads, number - 1);
                 const int h = chunk_of<2>(s, a.chunks, at);
                 const uint16_t* from = (const uint16_t*)(lists + (int64_t)h * a.list_words + columns);
-                c[i] = h * a.chunk + (int)load_device(from + s.held[h] + at - s.starts[h]);
+                c[i] = min(h * a.chunk + (int)load_device(from + s.held[h] + at - s.starts[h]), a.width - 1);
             }
 #pragma unroll
             for (int i = 0; i < kAhead; ++i) bits[i] = ((const uint32_t*)logits)[c[i]];
@@ -1093,7 +1094,7 @@ __global__ __launch_bounds__(kThreads) void vocab_sample_f32_kernel(VocabSampleA
     };
     choice = choose_wide(s, weights, tally, r, a.width, [&](uint32_t digit) {
         __syncthreads();
-        if (!a.sorted) {
+        if (a.chunks == 1) {
             if (t == 0) s.gathered = 0;
             __syncthreads();
             gather(s, logits, a.width, digit);
@@ -1122,7 +1123,7 @@ __global__ __launch_bounds__(kThreads) void vocab_sample_f32_kernel(VocabSampleA
             });
         __syncthreads();
     }, [&](auto&& f) {
-        if (a.sorted) each_run((int)s.gathered, [&](int, uint32_t key, int) { f(key); });
+        if (a.chunks > 1) each_run((int)s.gathered, [&](int, uint32_t key, int) { f(key); });
         else each_column<2>(logits, 0, a.width, a.width, [&](int, uint32_t key) { f(key); });
     });
     // the last search's columns are gathered: where few have the key, the token

@@ -29,7 +29,7 @@ def test_more_columns_of_a_logit_than_a_counter_holds(dtype):
         check(run(logits, 1.0, top_k, top_p, 0.0, u), rows=6)
 
 
-# chunks of at most 32768 columns, of more, and one per row
+# few chunks, many, and one per row
 @pytest.mark.parametrize("rows,width", [(8, 60001), (100, 140003), (140, 50002)])
 def test_wide_bins_of_32_bit_logits(rows, width):
     """More distinct columns in a bin of the first digit than are gathered, a key
