@@ -337,7 +337,10 @@ __global__ __launch_bounds__(kThreads) void adapter_down_tile_kernel(AdapterArgs
         };
         floatx4_t sum[2][RW], even[2][RW], acc[2][RW];
 #pragma unroll
-        for (int b = 0; b < S - 1; ++b) issue(b);
+        for (int b = 0; b < S - 1; ++b) {
+            issue(b);
+            __builtin_amdgcn_sched_barrier(0);  // in the order in which they are waited for
+        }
 #pragma unroll
         for (int b = 0; b < kBlocks; ++b) {
             // this wave's loads of block b have landed (S - 2 younger blocks may
@@ -524,31 +527,55 @@ __device__ __forceinline__ float row_parts(const AdapterArgs& a, const AdapterMe
     return split_row<F16, KS>(v, rank, scale, q, hi, lo);
 }
 
-// Eight 16-bit values of a row at column c: one access, or (rows that are not
-// 16-byte aligned) eight, those past column n left out.
+// Rows of base or y from the tile's first on, and eight 16-bit values of one (its
+// byte offset, or kOutside: reads what is not used, writes nothing) at column c.
+// VEC: rows and columns in 16-byte words, past the row reads 0 and is not written.  Else
+// the words lie anywhere: one access all the same, a row's last word read where
+// it ends and moved into place; element by element (1218 rows x 27723 columns 117 us
+// against 66) only to write that and where a row is shorter than a word.
+struct __attribute__((packed, aligned(2))) AnyWord { uint32_t w[4]; };
 template <bool VEC>
-__device__ __forceinline__ uint4 load8(__amdgpu_buffer_rsrc_t r, uint32_t row, int c, int n) {
+struct Rows {
+    __amdgpu_buffer_rsrc_t r;
+    uint8_t* p;
+    __device__ __forceinline__ Rows(const uint16_t* first, int64_t bytes) : r(buffer(first, bytes)), p((uint8_t*)first) {}
+};
+template <bool VEC>
+__device__ __forceinline__ uint4 load8(const Rows<VEC>& rows, uint32_t row, int c, int n) {
     if constexpr (VEC) {
-        return load16(r, row + 2 * c);
+        return load16(rows.r, row + 2 * c);
     } else {
-        uint32_t v[8];
+        const uint8_t* from = rows.p + (row == kOutside ? 0 : row);
+        if (n < 8) {
+            uint32_t v[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            v[i] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(r, (int)(c + i < n ? row + 2 * (c + i) : kOutside), 0, 0);
-        return uint4{v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16};
+            for (int i = 0; i < 8; ++i) v[i] = c + i < n ? ((const uint16_t*)from)[c + i] : 0;
+            return uint4{v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16};
+        }
+        const int past = max(c - (n - 8), 0);
+        const AnyWord w = *(const AnyWord*)(from + 2 * (c - past));
+        if (past <= 0 || past >= 8) return uint4{w.w[0], w.w[1], w.w[2], w.w[3]};
+        unsigned __int128 x = ((unsigned __int128)((uint64_t)w.w[3] << 32 | w.w[2]) << 64) | ((uint64_t)w.w[1] << 32 | w.w[0]);
+        x >>= 16 * past;
+        return uint4{(uint32_t)x, (uint32_t)(x >> 32), (uint32_t)(x >> 64), (uint32_t)(x >> 96)};
     }
 }
 
 template <bool VEC>
-__device__ __forceinline__ void store8(__amdgpu_buffer_rsrc_t r, uint32_t row, int c, int n, uint4 v) {
+__device__ __forceinline__ void store8(const Rows<VEC>& rows, uint32_t row, int c, int n, uint4 v) {
     if constexpr (VEC) {
-        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_dev_t, v), r, (int)(row + 2 * c), 0, 0);
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_dev_t, v), rows.r, (int)(row + 2 * c), 0, 0);
     } else {
+        if (row == kOutside) return;
+        uint8_t* to = rows.p + row;
+        if (c + 8 <= n) {
+            *(AnyWord*)(to + 2 * c) = AnyWord{{v.x, v.y, v.z, v.w}};
+            return;
+        }
         const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            __builtin_amdgcn_raw_buffer_store_b16((short)(w[i / 2] >> (16 * (i & 1))), r,
-                                                  (int)(c + i < n ? row + 2 * (c + i) : kOutside), 0, 0);
+            if (c + i < n) ((uint16_t*)to)[c + i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
     }
 }
 
@@ -600,8 +627,8 @@ __global__ __launch_bounds__(kThreads) void adapter_up_kernel(AdapterArgs a) {
     const int c_begin = (chunk - mb.chunk0) * a.chunk_cols + wave % kColWaves * kTurn;
     const int c_end = min(n, (chunk - mb.chunk0 + 1) * a.chunk_cols);
     const uint32_t ldbase = (uint32_t)mb.ldbase * 2, ldy = (uint32_t)mb.ldy * 2;  // bytes
-    const auto base = buffer(mb.base + (int64_t)row0 * mb.ldbase, (int64_t)(rows - 1) * ldbase + 2 * n);
-    const auto y = buffer(mb.y + (int64_t)row0 * mb.ldy, (int64_t)(rows - 1) * ldy + 2 * n);
+    const Rows<VEC> base(mb.base + (int64_t)row0 * mb.ldbase, (int64_t)(rows - 1) * ldbase + 2 * n);
+    const Rows<VEC> y(mb.y + (int64_t)row0 * mb.ldy, (int64_t)(rows - 1) * ldy + 2 * n);
     const bool in_place = mb.base == mb.y;
 
     uint64_t left = __ballot(slot != -1);
@@ -682,7 +709,7 @@ __global__ __launch_bounds__(kThreads) void adapter_up_kernel(AdapterArgs a) {
 // 32 ranks of B: 16-byte chunk q of column c in slot 4 c + (q ^ (c / 2) mod 4), so that
 // eight columns of a fragment read, what one pass takes, lie in distinct banks.
 // ---------------------------------------------------------------------------
-template <bool F16, int KS, int kTurn>
+template <bool F16, int KS, int kTurn, bool VEC>
 __global__ __launch_bounds__(kThreads) void adapter_up_tile_kernel(AdapterArgs a) {
     constexpr int kPitch = kTurn + 4, kTiles = kTurn / 16;
     constexpr int kRowsAt = 512 / kTurn, kPieces = 16 / kRowsAt;  // rows per access of base and y, accesses per turn
@@ -703,8 +730,10 @@ __global__ __launch_bounds__(kThreads) void adapter_up_tile_kernel(AdapterArgs a
     const int n = mb.n, max_rank = mb.max_rank;
     const int c_begin = (chunk - mb.chunk0) * a.chunk_cols, c_end = min(n, c_begin + a.chunk_cols);
     const uint32_t ldbase = (uint32_t)mb.ldbase * 2, ldy = (uint32_t)mb.ldy * 2;  // bytes
-    const auto base = buffer(mb.base + (int64_t)row0 * mb.ldbase, 15 * (int64_t)ldbase + 2 * n);
-    const auto y = buffer(mb.y + (int64_t)row0 * mb.ldy, 15 * (int64_t)ldy + 2 * n);
+    // (a wave past the last row reads none of its own)
+    const int64_t first = min(row0, a.m - 1);
+    const Rows<VEC> base(mb.base + first * mb.ldbase, 15 * (int64_t)ldbase + 2 * n);
+    const Rows<VEC> y(mb.y + first * mb.ldy, 15 * (int64_t)ldy + 2 * n);
     const bool in_place = mb.base == mb.y;
     const int slot = tile_slots(a, tile0, 64, slots_lds);
     // this lane's part of a slab's 1 KB pieces (two per wave): column, chunk
@@ -737,7 +766,7 @@ __global__ __launch_bounds__(kThreads) void adapter_up_tile_kernel(AdapterArgs a
         uint4 next[kPieces];
         issue(c_begin, 0);
 #pragma unroll
-        for (int i = 0; i < kPieces; ++i) next[i] = load16(base, row_at(i, c_begin, ldbase) + 2 * (c_begin + rc));
+        for (int i = 0; i < kPieces; ++i) next[i] = load8<VEC>(base, row_at(i, c_begin, ldbase), c_begin + rc, n);
         uint4 hi[KS], lo[KS];
         const float back = row_parts<F16, KS, 1>(a, mb, row0, 16, col, (mine >> col) & 1, rank, scale, q, hi, lo);
         int h = 0;
@@ -755,8 +784,9 @@ __global__ __launch_bounds__(kThreads) void adapter_up_tile_kernel(AdapterArgs a
             for (int i = 0; i < kPieces; ++i) in[i] = next[i];
             if (c0 + kTurn < c_end) {
                 issue(c0 + kTurn, h ^ 1);
+                __builtin_amdgcn_sched_barrier(0);  // what is waited for with kPieces left goes out first
 #pragma unroll
-                for (int i = 0; i < kPieces; ++i) next[i] = load16(base, row_at(i, c0 + kTurn, ldbase) + 2 * (c0 + kTurn + rc));
+                for (int i = 0; i < kPieces; ++i) next[i] = load8<VEC>(base, row_at(i, c0 + kTurn, ldbase), c0 + kTurn + rc, n);
             }
             __builtin_amdgcn_sched_barrier(0);
             const uint8_t* from = stage + h * KS * kSlab + col * 64 + ((q ^ (col >> 1)) & 3) * 16;
@@ -782,7 +812,7 @@ __global__ __launch_bounds__(kThreads) void adapter_up_tile_kernel(AdapterArgs a
                     in[i].z = add_pair<F16>(in[i].z, d1[0], d1[1]);
                     in[i].w = add_pair<F16>(in[i].w, d1[2], d1[3]);
                 }
-                store8<true>(y, row_at(i, c0, ldy), c0 + rc, n, in[i]);
+                store8<VEC>(y, row_at(i, c0, ldy), c0 + rc, n, in[i]);
             }
             __builtin_amdgcn_wave_barrier();
         }
@@ -831,8 +861,8 @@ __global__ __launch_bounds__(kAdapterRowWaves * 64) void adapter_row_kernel(Adap
     const float scale = e >= 0 ? mb.scales[e] : 0.f;
     const int es = max(e, 0), parts = 4 * a.split;
     const uint32_t ldbase = (uint32_t)mb.ldbase * 2, ldy = (uint32_t)mb.ldy * 2;  // bytes
-    const auto base = buffer(mb.base + (int64_t)row0 * mb.ldbase, 15 * (int64_t)ldbase + 2 * n);
-    const auto y = buffer(mb.y + (int64_t)row0 * mb.ldy, 15 * (int64_t)ldy + 2 * n);
+    const Rows<VEC> base(mb.base + (int64_t)row0 * mb.ldbase, 15 * (int64_t)ldbase + 2 * n);
+    const Rows<VEC> y(mb.y + (int64_t)row0 * mb.ldy, 15 * (int64_t)ldy + 2 * n);
     const auto up = buffer(mb.up + (int64_t)es * n * max_rank, (int64_t)n * max_rank * 2);
     const bool own = (mine >> col) & 1;
     uint4 b[TURNS][kTurn / 16], in[TURNS][kTurn / 32];
@@ -930,7 +960,10 @@ template <bool F16, int KS>
 void start_up_rows(const AdapterArgs& a, hipStream_t s) {
     if constexpr (KS <= 4)
         if (a.up_tile) {
-            adapter_up_tile_kernel<F16, KS, KS == 4 ? 64 : kAdapterUpTurn><<<(a.m + 63) / 64 * a.chunks, kThreads, 0, s>>>(a);
+            constexpr int kTurn = KS == 4 ? 64 : kAdapterUpTurn;
+            const int grid = (a.m + 63) / 64 * a.chunks;
+            if (a.vectors) adapter_up_tile_kernel<F16, KS, kTurn, true><<<grid, kThreads, 0, s>>>(a);
+            else adapter_up_tile_kernel<F16, KS, kTurn, false><<<grid, kThreads, 0, s>>>(a);
             return;
         }
     if (a.up_rows == 1) start_up<F16, KS, 1>(a, s);

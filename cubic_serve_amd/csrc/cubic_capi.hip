@@ -889,7 +889,7 @@ int cubic_adapters(const void* x, int64_t ldx, const int32_t* row_slots, int64_t
     // at 1024 rows and fewer the launch costs what it saves.  B in LDS for 64 rows
     // against each wave's own reads: rank 32 51.6 -> 46.5 us, rank 128 67.8 -> 53.
     a.join = m > 1024 && a.split > 1;
-    a.up_tile = m > 1024 && a.vectors && a.rank_tiles <= 8;
+    a.up_tile = m > 1024 && a.rank_tiles <= 8;
     // Columns of a workgroup, while 512 workgroups are left.  Prompts, in all: 256 and
     // 512 at rank 128 (4096 rows) 103 and 110 us, at rank 32 (2048 rows, 2 x 12288
     // columns) 64.4 and 67.4.  In order of adapters: 2048 and 512, 1024 rows x 2 x 12288
