@@ -99,6 +99,7 @@ class _AdapterLaunch:
         c = _native.ctypes
         self.x, self.banks, self.row_slots = x, banks, row_slots
         self.bases, self.outputs, self.workspace = bases, outputs, workspace
+        self._held = tuple(t for b in banks for t in (b.down, b.up, b.scales, b.ranks))
         self.identity = self._identity()
         ptrs = lambda ts: _table(c.c_void_p, [t.data_ptr() for t in ts])
         # (the row stride of a single row means nothing: at least a row then)
@@ -115,7 +116,9 @@ class _AdapterLaunch:
                      for t in (self.x, self.row_slots, *self.bases, *self.outputs))
 
     def validate(self) -> None:
-        if self._identity() != self.identity:
+        held = iter(self._held)
+        if self._identity() != self.identity or any(
+                t is not next(held) for b in self.banks for t in (b.down, b.up, b.scales, b.ranks)):
             raise ValueError("adapter launch operands changed after binding")
 
     def __call__(self, stream: int) -> None:

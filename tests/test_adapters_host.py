@@ -126,3 +126,17 @@ def test_entry_refuses_null_and_misaligned_operands():
     t[2][0] = 4104
     with pytest.raises(ValueError, match="16-byte"):
         _native.call("cubic_adapters", 4096, 64, 4096, 4, 64, 2, 1, *t, 0, 4096, 1 << 20, None)
+
+
+def test_binding_notices_a_bank_given_other_tensors():
+    """The launch holds the bank's addresses: a bank whose tensors are replaced,
+    not written, is refused."""
+    b = bank()
+    x, slots, y = torch.zeros((2, 64)).bfloat16(), torch.zeros(2, dtype=torch.int32), torch.zeros((2, 24)).bfloat16()
+    launch = adapters._AdapterLaunch(x, (b,), slots, (y,), (y,), torch.empty(16, dtype=torch.uint8))
+    launch.validate()
+    b.load(1, torch.ones((5, 64)).bfloat16(), torch.ones((24, 5)).bfloat16())
+    launch.validate()
+    b.down = b.down.clone()
+    with pytest.raises(ValueError, match="changed after binding"):
+        launch.validate()

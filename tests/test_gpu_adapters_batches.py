@@ -178,3 +178,24 @@ def test_decode_step_adapters_then_a_token():
         torch.cuda.synchronize()
         assert torch.equal(logits, seen[0]) and torch.equal(plan.tokens, seen[1])
         assert torch.equal(plan.logprobs[:count], seen[2][:count])
+
+
+@pytest.mark.parametrize("m,k,n", [(1, 1024, 40), (12, 6000, 40), (40, 520, 72), (300, 520, 72), (1100, 520, 72),
+                                   (2101, 16384, 24)])
+def test_what_lies_past_a_rank_is_not_used(m, k, n):
+    """A's rows past a slot's rank hold NaN and infinities, and another row of x
+    does: neither reaches a row that has no part in them."""
+    print(f"adapters: past the rank m={m}", flush=True)
+    ranks = (5, 17, 66, 1)
+    x, bases, banks, held, slots = case(m, k, (n,), ranks, 72, torch.bfloat16, "mixed", seed=17)
+    for s, r in enumerate(ranks):
+        banks[0].down[s, r:] = float("nan")
+        banks[0].down[s, (r + 72) // 2:] = float("inf")
+    got, = launch(x, banks, slots, bases)
+    check(got, x, bases[0], held[0], slots)
+    if m > 1:
+        spoilt = x.clone()
+        spoilt[m // 2] = float("nan")
+        other, = launch(spoilt, banks, slots, bases)
+        rest = torch.arange(m, device=DEV) != m // 2
+        assert torch.equal(other[rest], got[rest])
