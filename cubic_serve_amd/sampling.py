@@ -450,6 +450,8 @@ class VocabSamplingPlan:
             if t.shape != (rows,) or t.dtype is not dt or t.device != logits.device or not t.is_contiguous():
                 raise ValueError("sampling parameters must be contiguous float32 (top_ks int64) [rows] "
                                  "on the logits' device")
+        if torch.cuda.is_current_stream_capturing():  # the workspace has to be zero outside the graph
+            raise RuntimeError("vocabulary sampling must be planned before graph capture")
         nbytes = _native.lib().cubic_vocab_sample_workspace_bytes(rows, self.width,
                                                                   _CANDIDATE_DTYPES[logits.dtype])
         if nbytes < 0:

@@ -127,3 +127,19 @@ def test_plan_refusals():
     good["uniforms"].set_(full(0.5, n=6))
     with pytest.raises(ValueError, match="changed after binding"):
         plan.launch()
+
+
+def test_plan_is_not_made_under_capture():
+    print("sample plan under capture", flush=True)
+    full = lambda v, dt=FP32: torch.full((4,), v, dtype=dt, device=DEV)
+    good = dict(logits=torch.zeros((4, 64), device=DEV), temperatures=full(1.0), top_ks=full(0, torch.int64),
+                top_ps=full(1.0), min_ps=full(0.0), uniforms=full(0.5))
+    plan = sampling.VocabSamplingPlan(**good)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="before graph capture"):
+            sampling.VocabSamplingPlan(**good)
+        plan.launch()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert plan.tokens.tolist() == [32] * 4
