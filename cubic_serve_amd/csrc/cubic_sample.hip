@@ -183,10 +183,10 @@ struct Search {
     int starts[kMaxSampleChunks + 1], held[kMaxSampleChunks], number[kMaxSampleChunks];
     uint64_t sums[4][kWaves];   // before_wave's
     uint32_t count_sums[kWaves];
-    // 32 bits: a search's digit and the sums before it
+    // 32 bits: a search's digit, the sums before it, what it looks for
     uint32_t digit;
-    uint64_t before_count, before_mass;
-    // 16 bits: each search's digit, the counts of that digit's keys
+    uint64_t before_count, before_mass, want;
+    // each search's digit; 16 bits: the counts of that digit's keys
     uint32_t digits[3], keys[3][32], columns;
     uint32_t split[TYPE == 2 ? 1 : 32][kMaxSampleChunks];  // the token's digit's by chunk
     Choice choice;
@@ -345,6 +345,42 @@ __device__ __forceinline__ bool wanted(int stage, const Row& r, int width, uint6
     return true;
 }
 
+// The bins' sums become the sums before them, sh.columns all columns; head: all
+// mass, kept: that of min-p.  By the whole workgroup, a barrier before and behind.
+template <int TYPE>
+__device__ __forceinline__ void sums_before(Search<TYPE>& sh, const Tally& tally, const Row& r, uint64_t& head, uint64_t& kept) {
+    constexpr int kPer = Search<TYPE>::kPer, kBins = Search<TYPE>::kBins;
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    uint32_t c[kPer];
+    uint64_t m[kPer], cb, mb;
+    bins_before<TYPE, kPer>(sh, sh.count, sh.mass, c, m, cb, mb, head);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        sh.count[kBins - 1 - t * kPer - i] = (uint32_t)cb;
+        sh.mass[kBins - 1 - t * kPer - i] = mb;
+        cb += c[i];
+        mb += m[i];
+    }
+    if (t == kThreads - 1) sh.columns = (uint32_t)cb;
+    kept = head;
+    if (r.min_p > 0.f) before_wave(lane_u64(wave_scan_u64(tally.likely), 63), sh.sums[2], lane, wave, kept);
+    __syncthreads();
+}
+
+// The last bin in descending order before which the sum (of masses, of counts) is
+// below x, and the sums before it.  By one wave.
+template <int TYPE>
+__device__ __forceinline__ int bin_of(const Search<TYPE>& sh, bool by_mass, uint64_t x, uint64_t& count, uint64_t& mass) {
+    constexpr int kBins = Search<TYPE>::kBins, kRun = kBins / 64;
+    const int lane = threadIdx.x & 63;
+    auto before = [&](int d) { return by_mass ? (uint64_t)sh.mass[kBins - 1 - d] : (uint64_t)sh.count[kBins - 1 - d]; };
+    const int run = max(__popcll(__ballot(before(lane * kRun) < x)) - 1, 0);
+    const int d = run * kRun + max(__popcll(__ballot(lane < kRun && before(run * kRun + min(lane, kRun - 1)) < x)) - 1, 0);
+    count = sh.count[kBins - 1 - d];
+    mass = sh.mass[kBins - 1 - d];
+    return kBins - 1 - d;
+}
+
 // The searches of a row of 16-bit logits.  Called by the whole workgroup once
 // the items are added, after a barrier; items(f) calls f(key, number, chunk()) for
 // this thread's share of them; columns whose weight is 0 may be left out.  What is
@@ -353,26 +389,9 @@ __device__ __forceinline__ bool wanted(int stage, const Row& r, int width, uint6
 template <int TYPE, typename Items>
 __device__ __forceinline__ Choice choose_narrow(Search<TYPE>& sh, const Weights<TYPE>& weights, const Tally& tally,
                                                 const Row& r, int width, Items&& items) {
-    constexpr int kPer = Search<TYPE>::kPer, kBins = Search<TYPE>::kBins, kRun = kBins / 64;
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     uint64_t head, kept;
-    {
-        // the bins' sums become the sums before them
-        uint32_t c[kPer];
-        uint64_t m[kPer], cb, mb;
-        bins_before<TYPE, kPer>(sh, sh.count, sh.mass, c, m, cb, mb, head);
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            sh.count[kBins - 1 - t * kPer - i] = (uint32_t)cb;
-            sh.mass[kBins - 1 - t * kPer - i] = mb;
-            cb += c[i];
-            mb += m[i];
-        }
-        if (t == kThreads - 1) sh.columns = (uint32_t)cb;
-    }
-    kept = head;
-    if (r.min_p > 0.f) before_wave(lane_u64(wave_scan_u64(tally.likely), 63), sh.sums[2], lane, wave, kept);
-    __syncthreads();
+    sums_before(sh, tally, r, head, kept);
     uint32_t key = 0;
     uint64_t nth = 1;
     for (int stage = 0; stage < 3; ++stage) {
@@ -380,14 +399,9 @@ __device__ __forceinline__ Choice choose_narrow(Search<TYPE>& sh, const Weights<
         if (!wanted(stage, r, width, head, kept, x)) continue;  // (the same in every wave)
         uint64_t count = 0, mass = 0;
         if (wave == 0) {
-            // the last bin in descending order before which the sum is below x
-            auto before = [&](int d) { return stage ? (uint64_t)sh.mass[kBins - 1 - d] : (uint64_t)sh.count[kBins - 1 - d]; };
-            const int run = max(__popcll(__ballot(before(lane * kRun) < x)) - 1, 0);
-            const int d = run * kRun + max(__popcll(__ballot(lane < kRun && before(run * kRun + min(lane, kRun - 1)) < x)) - 1, 0);
-            count = sh.count[kBins - 1 - d];
-            mass = sh.mass[kBins - 1 - d];
+            const int d = bin_of(sh, stage > 0, x, count, mass);
             // (fewer than top_k columns may weigh anything)
-            if (lane == 0) sh.digits[stage] = stage == 0 && sh.columns < x ? kNoDigit : (uint32_t)(kBins - 1 - d);
+            if (lane == 0) sh.digits[stage] = stage == 0 && sh.columns < x ? kNoDigit : (uint32_t)d;
         }
         __syncthreads();
         const uint32_t digit = sh.digits[stage];
@@ -425,65 +439,109 @@ __device__ __forceinline__ Choice choose_narrow(Search<TYPE>& sh, const Weights<
 template <typename Gather, typename Columns>
 __device__ __forceinline__ Choice choose_wide(Search<2>& sh, const Weights<2>& weights, const Tally& tally,
                                               const Row& r, int width, Gather&& gather, Columns&& columns) {
-    constexpr int kPer = Search<2>::kPer;
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
-    uint32_t held = kNoDigit;  // the digit whose columns are gathered
-    uint32_t c[kPer];
-    uint64_t m[kPer], cb, mb, head, kept, x;
-    bins_before<2, kPer>(sh, sh.count, sh.mass, c, m, cb, mb, head);
-    kept = head;
-    if (r.min_p > 0.f) before_wave(lane_u64(wave_scan_u64(tally.likely), 63), sh.sums[2], lane, wave, kept);
-    Choice out = {0, 1, 0};
-    auto found = [&](uint32_t digit, uint64_t count, uint64_t mass) {
-        sh.digit = digit;
-        sh.before_count = count;
-        sh.before_mass = mass;
-    };
+    constexpr int kFew = 128;
+    uint32_t held = kNoDigit, key = 0;  // held: the digit whose columns are gathered
+    uint64_t head, kept, nth = 1;
+    sums_before(sh, tally, r, head, kept);
     for (int stage = 0; stage < 3; ++stage) {
-        if (!wanted(stage, r, width, head, kept, x)) continue;
-        if (t == 0) sh.digit = kNoDigit;
-        __syncthreads();
-        pick<kPer>(c, m, cb, mb, stage > 0, x, found);
-        __syncthreads();
-        uint32_t prefix = sh.digit;
-        if (prefix == kNoDigit) {  // fewer than top_k columns weigh anything
-            __syncthreads();
-            continue;
+        uint64_t x = 0;
+        if (!wanted(stage, r, width, head, kept, x)) continue;  // (the same in every wave)
+        uint64_t count = 0, mass = 0;
+        if (wave == 0) {
+            const int d = bin_of(sh, stage > 0, x, count, mass);
+            if (lane == 0) {
+                // (fewer than top_k columns may weigh anything)
+                sh.digits[stage] = stage == 0 && sh.columns < x ? kNoDigit : (uint32_t)d;
+                sh.want = x;
+                sh.before_count = count;
+                sh.before_mass = mass;
+            }
         }
+        __syncthreads();
+        uint32_t prefix = sh.digits[stage];
+        if (prefix == kNoDigit) continue;
         if (prefix != held) gather(prefix);
         held = prefix;
         const int gathered = (int)sh.gathered;
-        for (int shift = 20; shift > 0; shift -= 10) {
-            const uint64_t bc = sh.before_count, bm = sh.before_mass;
-            sh.deep_count[t] = 0;
-            sh.deep_mass[t] = 0;
+        uint64_t weight = 0;
+        if (gathered <= kFew) {
+            // every column against every other: the sums over larger keys (from 0
+            // on) and over equal ones (from kFew on).  31 columns: 2400 cycles, by bins
+            // 7100; 119: 6100 and 7700.
+            const int lanes = gathered <= 64 ? 64 : kFew, i = t & (lanes - 1);
+            const uint32_t mine = i < gathered ? sh.items[2 * i] : 0;
+            if (t < 2 * kFew) sh.deep_count[t] = 0, sh.deep_mass[t] = 0;
+            if (t >= kThreads - lanes) sh.deep_mass[2 * kFew + i] = i < gathered ? weights.of(mine) : 0;
             __syncthreads();
-            auto deepen = [&](uint32_t k) {
-                if (k >> shift != prefix) return;
-                const uint32_t d = k >> (shift - 10) & 1023u;
-                atomicAdd(&sh.deep_count[d], 1u);
-                atomicAdd(&sh.deep_mass[d], (unsigned long long)weights.of(k));
-            };
-            if (gathered <= Search<2>::kCached)
-                for (int i = t; i < gathered; i += kThreads) deepen(sh.items[2 * i]);
-            else
-                columns(deepen);
+            uint32_t over = 0, equal = 0;
+            uint64_t overs = 0, equals = 0;
+            for (int j = t / lanes; j < gathered; j += kThreads / lanes) {
+                const uint32_t other = sh.items[2 * j];
+                const uint64_t w = sh.deep_mass[2 * kFew + j];
+                over += other > mine;
+                overs += other > mine ? w : 0;
+                equal += other == mine;
+                equals += other == mine ? w : 0;
+            }
+            if (over) atomicAdd(&sh.deep_count[i], over), atomicAdd(&sh.deep_mass[i], (unsigned long long)overs);
+            if (equal) atomicAdd(&sh.deep_count[kFew + i], equal), atomicAdd(&sh.deep_mass[kFew + i], (unsigned long long)equals);
             __syncthreads();
-            uint32_t dc[1];
-            uint64_t dm[1], dcb, dmb, all;
-            bins_before<2, 1>(sh, sh.deep_count, sh.deep_mass, dc, dm, dcb, dmb, all);
-            pick<1>(dc, dm, bc + dcb, bm + dmb, stage > 0, x, found);
-            __syncthreads();
-            prefix = prefix << 10 | (sh.digit & 1023u);
+            if (wave != 0) continue;
+            for (int from = 0; from < gathered; from += 64) {
+                const int k = from + lane;
+                const uint64_t c = count + sh.deep_count[k], m = mass + sh.deep_mass[k];
+                const uint64_t lo = stage ? m : c, more = stage ? sh.deep_mass[kFew + k] : sh.deep_count[kFew + k];
+                const uint64_t hit = __ballot(k < gathered && lo < x && lo + more >= x);
+                if (!hit && from + 64 < gathered) continue;
+                const int at = hit ? __builtin_ctzll(hit) : 0;
+                key = sh.items[2 * (from + at)];
+                weight = sh.deep_mass[2 * kFew + from + at];
+                mass = lane_u64(m, at);
+                count = lane_u64(c, at);
+                break;
+            }
+        } else {
+            x = sh.want;
+            for (int shift = 20; shift > 0; shift -= 10) {
+                const uint64_t bc = sh.before_count, bm = sh.before_mass;
+                sh.deep_count[t] = 0;
+                sh.deep_mass[t] = 0;
+                __syncthreads();
+                auto deepen = [&](uint32_t k) {
+                    if (k >> shift != prefix) return;
+                    const uint32_t d = k >> (shift - 10) & 1023u;
+                    atomicAdd(&sh.deep_count[d], 1u);
+                    atomicAdd(&sh.deep_mass[d], (unsigned long long)weights.of(k));
+                };
+                if (gathered <= Search<2>::kCached)
+                    for (int i = t; i < gathered; i += kThreads) deepen(sh.items[2 * i]);
+                else
+                    columns(deepen);
+                __syncthreads();
+                uint32_t dc[1];
+                uint64_t dm[1], dcb, dmb, all;
+                bins_before<2, 1>(sh, sh.deep_count, sh.deep_mass, dc, dm, dcb, dmb, all);
+                pick<1>(dc, dm, bc + dcb, bm + dmb, stage > 0, x, [&](uint32_t digit, uint64_t c, uint64_t m) {
+                    sh.digit = digit;
+                    sh.before_count = c;
+                    sh.before_mass = m;
+                });
+                __syncthreads();
+                prefix = prefix << 10 | (sh.digit & 1023u);
+            }
+            key = prefix;
+            weight = weights.of(prefix);
+            count = sh.before_count;
+            mass = sh.before_mass;
+            __syncthreads();  // (the next search's sums before its bin)
         }
-        const uint64_t w = weights.of(prefix);
-        out.key = prefix;
-        out.nth = stage ? columns_to(x - sh.before_mass, w) : x - sh.before_count;
-        head = min(head, sh.before_mass + out.nth * w);  // (of the token's own search: not used)
-        __syncthreads();
+        nth = stage ? columns_to(x - mass, weight) : x - count;
+        head = min(head, mass + nth * weight);  // (of the token's own search: not used)
     }
-    out.kept = kept;
-    return out;
+    if (t == 0) sh.choice = {key, nth, kept};
+    __syncthreads();
+    return sh.choice;
 }
 
 __device__ __forceinline__ void refuse(const VocabSampleArgs& a, int row) {
