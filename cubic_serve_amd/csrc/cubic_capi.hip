@@ -872,7 +872,7 @@ int cubic_adapters(const void* x, int64_t ldx, const int32_t* row_slots, int64_t
     // Batches of 17 to 1024 rows are tiled in order of adapters, the others as the
     // rows stand, a tile's adapters shared by up to 16 workgroups.  In order and as
     // they stand: 256 rows of 64 requests with 16 adapters, K = 12288 -> 4096, 26.3 and
-    // 36.0 us; 512 rows, 128 requests, 2 x 12288 columns 29.9 and 52.5; 1024 rows of 8
+    // 36.0 us (partitions not joined); 512 rows, 128 requests, 2 x 12288 columns 29.9 and 52.5; 1024 rows of 8
     // requests, 2 x 12288 49 and 61; 64 rows, 64 adapters 21 and 28.5; 24 rows, 24
     // adapters 16.5 and 15.5.  At 16 rows the search for a tile's rows costs more than it
     // saves, 10.2 and 8.5.  (Its rows lie anywhere in the batch: 32-bit offsets from the
@@ -884,11 +884,14 @@ int cubic_adapters(const void* x, int64_t ldx, const int32_t* row_slots, int64_t
     a.up_groups = m <= 128 ? (int)std::min<int64_t>(16, m) : m <= 1024 ? 4 : 1;
     if (by_slot) a.down_groups = a.up_groups = 1;
     const int64_t items = by_slot ? a.items : ceil_div(m, 16 * a.up_rows) * a.up_groups;
-    // The partitions added once where many column chunks would add them again:
-    // 8 of them, 4096 rows, rank 128: 77 -> 58.5 us of up kernel for 4.3 of joining;
-    // at 1024 rows and fewer the launch costs what it saves.  B in LDS for 64 rows
-    // against each wave's own reads: rank 32 51.6 -> 46.5 us, rank 128 67.8 -> 53.
-    a.join = m > 1024 && a.split > 1;
+    // The partitions added once, in a launch of their own, where the column chunks
+    // would otherwise add much again.  Added again and once: 4096 rows, rank 128, K =
+    // 8192 (8 partitions) 150 and 135 us; 512 rows, rank 64, K = 12288 39.6 and 28.7, 256 rows
+    // 26.1 and 21.8, 24 rows 20.4 and 19.0 (but 64 rows with 64 adapters 36.3 and 37.5);
+    // 128 rows, rank 64, K = 8192 29.2 and 26.6, rank 16 16.2 and 17.2; 512 rows, rank 32, K =
+    // 4096 30.9 and 33.0.  B in LDS for 64 rows against each wave's own reads: rank 32
+    // 51.6 -> 46.5 us, rank 128 67.8 -> 53.
+    a.join = a.split > 1 && (m > 1024 || (m > 64 && a.rank_tiles * a.split >= 24));
     a.up_tile = m > 1024 && a.rank_tiles <= 8;
     // Columns of a workgroup, while 512 workgroups are left.  Prompts, in all: 256 and
     // 512 at rank 128 (4096 rows) 103 and 110 us, at rank 32 (2048 rows, 2 x 12288

@@ -199,3 +199,17 @@ def test_what_lies_past_a_rank_is_not_used(m, k, n):
         other, = launch(spoilt, banks, slots, bases)
         rest = torch.arange(m, device=DEV) != m // 2
         assert torch.equal(other[rest], got[rest])
+
+
+def test_joined_partitions_agree_with_added_ones():
+    """Many partitions of K: joined in a launch of their own in batches of some
+    size, added by the up kernel in smaller ones, with the same bits."""
+    for dtype in DTYPES:
+        print(f"adapters: joined partitions {dtype}", flush=True)
+        x, bases, banks, held, slots = case(300, 8200, (264, 41), (48, 20, 7), 48, dtype, "mixed", seed=18)
+        whole = launch(x, banks, slots, bases)
+        for y, base, h in zip(whole, bases, held):
+            check(y, x, base, h, slots)
+        for rows in (65, 64, 17, 9, 1):
+            part = launch(x[:rows], banks, slots[:rows], [b[:rows] for b in bases])
+            assert all(torch.equal(p, w[:rows]) for p, w in zip(part, whole))
