@@ -270,10 +270,10 @@ __global__ __launch_bounds__(kThreads) void adapter_down_kernel(AdapterArgs a) {
 // halves, and A is read once per 64 rows: 54 -> 27.5 us with one adapter.  A tile on a
 // boundary is done once per adapter, at the end alone on its CU: with two requests
 // and up 39 to 52 (workgroups of their own for the second adapter wait for a place
-// until the others end: 44 and 41 with three requests).  Four blocks
-// make a quarter; quarters add as above, bit for bit.  LDS image of a 16-row block:
-// 16-byte chunk c of row r in slot 8 r + (c ^ (r / 2) mod 8), so that the 16 rows of
-// a fragment read lie in distinct banks.
+// until the others end: 44 and 41 with three requests).  Four blocks make a
+// quarter; quarters add as above, bit for bit.  LDS image of a 16-row block: 16-byte
+// chunk c of row r in slot 8 r + (c ^ (r / 2) mod 8), so that the 16 rows of a
+// fragment read lie in distinct banks.
 // ---------------------------------------------------------------------------
 template <bool F16>
 __global__ __launch_bounds__(kThreads) void adapter_down_tile_kernel(AdapterArgs a) {

@@ -872,12 +872,12 @@ int cubic_adapters(const void* x, int64_t ldx, const int32_t* row_slots, int64_t
     // Batches of 17 to 1024 rows are tiled in order of adapters, the others as the
     // rows stand, a tile's adapters shared by up to 16 workgroups.  In order and as
     // they stand: 256 rows of 64 requests with 16 adapters, K = 12288 -> 4096, 26.3 and
-    // 36.0 us (partitions not joined); 512 rows, 128 requests, 2 x 12288 columns 29.9 and 52.5; 1024 rows of 8
-    // requests, 2 x 12288 49 and 61; 64 rows, 64 adapters 21 and 28.5; 24 rows, 24
-    // adapters 16.5 and 15.5.  At 16 rows the search for a tile's rows costs more than it
-    // saves, 10.2 and 8.5.  (Its rows lie anywhere in the batch: 32-bit offsets from the
-    // first.)
-    const bool by_slot = m > 16 && m <= 1024 && slots < 256 && m * ldx < (1 << 30) && m * widest < (1 << 30) && 1;
+    // 36.0 us (partitions not joined); 512 rows, 128 requests, 2 x 12288 columns 29.9
+    // and 52.5; 1024 rows of 8 requests, 2 x 12288 49 and 61; 64 rows, 64 adapters 21 and
+    // 28.5; 24 rows, 24 adapters 16.5 and 15.5.  At 16 rows the search for a tile's rows
+    // costs more than it saves, 10.2 and 8.5.  (Its rows lie anywhere in the batch:
+    // 32-bit offsets from the first.)
+    const bool by_slot = m > 16 && m <= 1024 && slots < 256 && m * ldx < (1 << 30) && m * widest < (1 << 30);
     a.items = by_slot ? (int)(std::min<int64_t>(slots + 1, m) + m / 16) : 0;
     a.up_rows = m <= 128 || by_slot ? 1 : 4;
     a.down_groups = m <= 128 ? (int)std::min<int64_t>(16, m) : m <= 1024 ? 4 : 1;
