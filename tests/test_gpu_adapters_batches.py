@@ -213,3 +213,18 @@ def test_joined_partitions_agree_with_added_ones():
         for rows in (65, 64, 17, 9, 1):
             part = launch(x[:rows], banks, slots[:rows], [b[:rows] for b in bases])
             assert all(torch.equal(p, w[:rows]) for p, w in zip(part, whole))
+
+
+@pytest.mark.parametrize("m,ld", [(600, 1 << 21), (1100, 1 << 21), (40, 1 << 23)])
+def test_rows_that_lie_far_apart(m, ld):
+    """Row strides whose last rows start past 2^31 bytes, or past 2^30 elements in
+    all, in batches that are otherwise tiled in order of adapters."""
+    print(f"adapters: rows {ld} elements apart, m={m}", flush=True)
+    x, bases, banks, held, slots = case(m, 264, (41,), (16, 7, 12), 16, torch.bfloat16, "mixed", seed=19)
+    far = lambda t: torch.empty((m, ld), dtype=t.dtype, device=DEV)[:, :t.shape[1]].copy_(t)
+    got = far(bases[0])
+    linear.PackedLinearOperators().bind_adapters(far(x), banks, slots, got).launch()
+    torch.cuda.synchronize()
+    check(got, x, bases[0], held[0], slots)
+    near, = launch(x, banks, slots, bases)
+    assert torch.equal(got, near)

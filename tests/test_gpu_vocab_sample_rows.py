@@ -143,3 +143,18 @@ def test_plan_is_not_made_under_capture():
     graph.replay()
     torch.cuda.synchronize()
     assert plan.tokens.tolist() == [32] * 4
+
+
+def test_rows_that_lie_far_apart():
+    """Rows that start past 2^32 bytes."""
+    for dtype, stride in ((BF16, 1 << 30), (FP32, 1 << 29)):
+        print(f"sample rows {stride} elements apart", flush=True)
+        gen = torch.Generator().manual_seed(24)
+        near = (torch.randn((4, 20001), generator=gen) * 3).to(dtype).to(DEV)
+        far = torch.empty(3 * stride + 20001, dtype=dtype, device=DEV).as_strided((4, 20001), (stride, 1))
+        far.copy_(near)
+        params = settings(4, gen)
+        plan = run(far, *params)
+        check(plan)
+        assert torch.equal(plan.tokens, run(near, *params).tokens)
+        del far, plan
