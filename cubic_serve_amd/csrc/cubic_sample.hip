@@ -766,6 +766,27 @@ __global__ __launch_bounds__(kThreads) void vocab_sample_kernel(VocabSampleArgs 
     top = wave_max_u32(lane < kWaves ? wave_top[lane] : 0);
     bad = __ballot(lane < kWaves && wave_bad[lane]) != 0;
     const bool overflow = __builtin_amdgcn_readlane((int)wave_scan_u32(lane < kWaves ? wave_lost[lane] : 0), 63) != 0;
+    if (overflow) {
+        // the counters tell neither the largest nor whether there is a NaN: a lower
+        // half has carried into its neighbour's, an upper one lost 65536
+        const int begin = chunk * a.chunk, end = min(a.width, begin + a.chunk);
+        top = 0;
+        bad = 0;
+        each_column<TYPE>(logits, begin, end, a.width, [&](int, uint32_t key) {
+            bad |= key >= Limits<TYPE>::kInf || key < Limits<TYPE>::kNegInf;
+            top = max(top, key);
+        });
+        top = wave_max_u32(top);
+        bad = __ballot(bad) != 0;
+        __syncthreads();  // (the waves' first values are read)
+        if (lane == 63) {
+            wave_top[wave] = top;
+            wave_bad[wave] = bad;
+        }
+        __syncthreads();
+        top = wave_max_u32(lane < kWaves ? wave_top[lane] : 0);
+        bad = __ballot(lane < kWaves && wave_bad[lane]) != 0;
+    }
     // list those that can weigh anything beside the chunk's largest (at
     // temperature 0 the largest itself): patterns from `low` on among the
     // positive, up to `high` among the negative ones
