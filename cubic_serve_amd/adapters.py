@@ -64,6 +64,7 @@ class AdapterBank:
             raise ValueError(f"adapter slot must be an int in 0..{self.slots - 1}")
         return slot
 
+    @torch.no_grad()  # of trained parameters too: no history in the bank
     def load(self, slot: int, down: Tensor, up: Tensor, scale: float = 1.0) -> None:
         """Put an adapter (down [rank, k], up [n, rank]) into a slot, on the
         device's current stream: order it against launches on other streams."""

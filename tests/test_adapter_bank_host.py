@@ -1,0 +1,28 @@
+"""Adapter banks (no GPU): what loading leaves behind, and what a binding notices."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from cubic_serve_amd import adapters
+
+
+def bank(**changes):
+    args = dict(n=24, k=64, slots=3, max_rank=12, device="cpu")
+    args.update(changes)
+    return adapters.AdapterBank(args.pop("n"), args.pop("k"), **args)
+
+
+def adapter(rank, seed=0):
+    gen = torch.Generator().manual_seed(seed)
+    return torch.randn((rank, 64), generator=gen).bfloat16(), torch.randn((24, rank), generator=gen).bfloat16()
+
+
+def test_loading_parameters_records_no_history():
+    b = bank()
+    for turn in range(3):
+        down, up = (torch.nn.Parameter(t) for t in adapter(5, turn))
+        b.load(1, down, up, torch.nn.Parameter(torch.tensor(0.5)))
+    for t in (b.down, b.up, b.scales, b.ranks):
+        assert not t.requires_grad and t.grad_fn is None
+    assert torch.equal(b.down[1, :5], down.detach()) and torch.equal(b.up[1, :, :5], up.detach())
