@@ -76,11 +76,12 @@ class AdapterBank:
             raise ValueError(f"adapter rank {rank} outside 1..{self.max_rank}")
         if down.dtype != self.dtype or up.dtype != self.dtype:
             raise ValueError("adapter matrices differ from the bank's dtype")
+        scale = float(scale)  # before anything of the slot changes
         self.down[slot, :rank].copy_(down)
         self.down[slot, rank:].zero_()
         self.up[slot, :, :rank].copy_(up)
         self.up[slot, :, rank:].zero_()  # the kernel multiplies whole groups of 8 ranks
-        self.scales[slot].fill_(float(scale))
+        self.scales[slot].fill_(scale)
         self.ranks[slot].fill_(rank)
 
     def clear(self, slot: int) -> None:

@@ -26,3 +26,14 @@ def test_loading_parameters_records_no_history():
     for t in (b.down, b.up, b.scales, b.ranks):
         assert not t.requires_grad and t.grad_fn is None
     assert torch.equal(b.down[1, :5], down.detach()) and torch.equal(b.up[1, :, :5], up.detach())
+
+
+def test_a_refused_load_leaves_the_slot_as_it_was():
+    b = bank()
+    held = adapter(5)
+    b.load(1, *held, 0.5)
+    before = [t.clone() for t in (b.down, b.up, b.scales, b.ranks)]
+    for scale in ("large", None, torch.ones(2), 1j):
+        with pytest.raises((TypeError, ValueError, RuntimeError)):
+            b.load(1, *adapter(7, 1), scale)
+        assert all(torch.equal(t, u) for t, u in zip((b.down, b.up, b.scales, b.ranks), before))
