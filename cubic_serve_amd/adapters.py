@@ -101,8 +101,10 @@ class _AdapterLaunch:
         c = _native.ctypes
         self.x, self.banks, self.row_slots = x, banks, row_slots
         self.bases, self.outputs, self.workspace = bases, outputs, workspace
-        self._held = tuple(t for b in banks for t in (b.down, b.up, b.scales, b.ranks))
-        self.identity = self._identity()
+        self._operands = (x, row_slots, *bases, *outputs)
+        # the banks' memory is held, so that no other tensor can come to its addresses
+        self._held = tuple(t.untyped_storage() for b in banks for t in (b.down, b.up, b.scales, b.ranks))
+        self.identity, self._addresses = self._identity(), self._bank_addresses()
         ptrs = lambda ts: _table(c.c_void_p, [t.data_ptr() for t in ts])
         # (the row stride of a single row means nothing: at least a row then)
         self._args = (
@@ -114,13 +116,13 @@ class _AdapterLaunch:
             workspace.data_ptr(), workspace.numel())
 
     def _identity(self):
-        return tuple((t.data_ptr(), t.shape, t.stride(), t.dtype)
-                     for t in (self.x, self.row_slots, *self.bases, *self.outputs))
+        return [(t.data_ptr(), t.shape, t.stride(), t.dtype) for t in self._operands]
+
+    def _bank_addresses(self):
+        return [(b.down.data_ptr(), b.up.data_ptr(), b.scales.data_ptr(), b.ranks.data_ptr()) for b in self.banks]
 
     def validate(self) -> None:
-        held = iter(self._held)
-        if self._identity() != self.identity or any(
-                t is not next(held) for b in self.banks for t in (b.down, b.up, b.scales, b.ranks)):
+        if self._identity() != self.identity or self._bank_addresses() != self._addresses:
             raise ValueError("adapter launch operands changed after binding")
 
     def __call__(self, stream: int) -> None:

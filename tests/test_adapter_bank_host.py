@@ -37,3 +37,26 @@ def test_a_refused_load_leaves_the_slot_as_it_was():
         with pytest.raises((TypeError, ValueError, RuntimeError)):
             b.load(1, *adapter(7, 1), scale)
         assert all(torch.equal(t, u) for t, u in zip((b.down, b.up, b.scales, b.ranks), before))
+
+
+CHANGES = {
+    "other storage": lambda b: b.ranks.set_(torch.zeros(3, dtype=torch.int32)),
+    "other data": lambda b: setattr(b.down, "data", torch.zeros_like(b.down)),
+    "freed": lambda b: b.up.untyped_storage().resize_(0),
+    "grown": lambda b: b.scales.resize_(1 << 12),
+    "moved": lambda b: b.ranks.set_(torch.zeros(9, dtype=torch.int32)[3:6]),
+    "replaced": lambda b: setattr(b, "up", b.up.clone()),
+}
+
+
+@pytest.mark.parametrize("change", CHANGES)
+def test_a_binding_notices_a_bank_whose_memory_is_another(change):
+    """The launch holds the bank's addresses; writing to the bank keeps them."""
+    b = bank()
+    x, slots, y = torch.zeros((2, 64)).bfloat16(), torch.zeros(2, dtype=torch.int32), torch.zeros((2, 24)).bfloat16()
+    launch = adapters._AdapterLaunch(x, (b,), slots, (y,), (y,), torch.empty(16, dtype=torch.uint8))
+    b.load(2, *adapter(5))
+    launch.validate()
+    CHANGES[change](b)
+    with pytest.raises(ValueError, match="changed after binding"):
+        launch.validate()
