@@ -59,6 +59,15 @@ class AdapterBank:
         self.scales = torch.zeros(slots, dtype=torch.float32, device=self.device)
         self.ranks = torch.zeros(slots, dtype=torch.int32, device=self.device)
 
+    def check(self) -> None:
+        """Whether the tensors are as the bank was made: a launch reads those extents."""
+        for name, shape, dtype in (("down", (self.slots, self.capacity, self.k), self.dtype),
+                                   ("up", (self.slots, self.n, self.capacity), self.dtype),
+                                   ("scales", (self.slots,), torch.float32), ("ranks", (self.slots,), torch.int32)):
+            t = getattr(self, name)
+            if t.shape != shape or t.dtype is not dtype or not t.is_contiguous() or t.device != self.down.device:
+                raise ValueError(f"adapter bank's {name} must be contiguous {dtype} {list(shape)} on one device")
+
     def _slot(self, slot: int) -> int:
         if type(slot) is not int or not 0 <= slot < self.slots:
             raise ValueError(f"adapter slot must be an int in 0..{self.slots - 1}")
@@ -162,6 +171,8 @@ def bind_adapters(x: Tensor, banks: Sequence[AdapterBank] | AdapterBank, row_slo
         raise ValueError(f"adapters need 1..{MAX_GROUP_MEMBERS} banks with one base and one output each")
     if any(not isinstance(b, AdapterBank) for b in banks):
         raise TypeError("adapters must be AdapterBank objects")
+    for bank in banks:
+        bank.check()
     tensors = (x, row_slots, *bases, *outputs)
     if any(not isinstance(t, Tensor) for t in tensors):
         raise TypeError("adapter operands must be tensors")

@@ -60,3 +60,30 @@ def test_a_binding_notices_a_bank_whose_memory_is_another(change):
     CHANGES[change](b)
     with pytest.raises(ValueError, match="changed after binding"):
         launch.validate()
+
+
+@pytest.mark.parametrize("name,shape,dtype", [
+    ("down", (3, 8, 64), torch.bfloat16), ("down", (2, 16, 64), torch.bfloat16), ("down", (3, 16, 64), torch.float16),
+    ("up", (3, 24, 8), torch.bfloat16), ("up", (3, 23, 16), torch.bfloat16), ("up", (3, 24, 16), torch.float32),
+    ("scales", (2,), torch.float32), ("scales", (3,), torch.float64), ("ranks", (2,), torch.int32),
+    ("ranks", (3,), torch.int64)])
+def test_a_bank_whose_tensors_do_not_fit_it_is_not_bound(name, shape, dtype):
+    """The launch reads the extents that the bank was made with."""
+    b = bank()
+    x, slots, y = torch.zeros((2, 64)).bfloat16(), torch.zeros(2, dtype=torch.int32), torch.zeros((2, 24)).bfloat16()
+    setattr(b, name, torch.zeros(shape, dtype=dtype))
+    with pytest.raises(ValueError, match=f"adapter bank's {name}"):
+        adapters.bind_adapters(x, b, slots, y)
+
+
+def test_a_bank_whose_matrices_lie_in_another_order_is_not_bound():
+    x, slots, y = torch.zeros((2, 64)).bfloat16(), torch.zeros(2, dtype=torch.int32), torch.zeros((2, 24)).bfloat16()
+    for name in ("down", "up"):
+        b = bank()
+        setattr(b, name, getattr(b, name).transpose(1, 2).contiguous().transpose(1, 2))
+        with pytest.raises(ValueError, match=f"adapter bank's {name}"):
+            adapters.bind_adapters(x, b, slots, y)
+    b = bank()
+    b.scales = torch.zeros(6)[::2]
+    with pytest.raises(ValueError, match="adapter bank's scales"):
+        adapters.bind_adapters(x, b, slots, y)
