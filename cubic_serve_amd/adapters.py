@@ -115,9 +115,9 @@ class _AdapterLaunch:
         self._held = tuple(t.untyped_storage() for b in banks for t in (b.down, b.up, b.scales, b.ranks))
         self.identity, self._addresses = self._identity(), self._bank_addresses()
         ptrs = lambda ts: _table(c.c_void_p, [t.data_ptr() for t in ts])
-        # (the row stride of a single row means nothing: at least a row then)
+        # (the row stride of a single row means nothing: a row, or at least that, then)
         self._args = (
-            x.data_ptr(), x.stride(0), row_slots.data_ptr(), x.shape[0], x.shape[1], banks[0].slots,
+            x.data_ptr(), x.stride(0) if x.shape[0] > 1 else x.shape[1], row_slots.data_ptr(), x.shape[0], x.shape[1], banks[0].slots,
             len(banks), _table(c.c_int64, [b.n for b in banks]), _table(c.c_int, [b.capacity for b in banks]),
             ptrs([b.down for b in banks]), ptrs([b.up for b in banks]), ptrs([b.scales for b in banks]),
             ptrs([b.ranks for b in banks]), ptrs(bases), _table(c.c_int64, [max(b.stride(0), b.shape[1]) for b in bases]),
@@ -182,8 +182,8 @@ def bind_adapters(x: Tensor, banks: Sequence[AdapterBank] | AdapterBank, row_slo
         raise RuntimeError("adapters must be bound before graph capture")
     if any(t.device != x.device for t in tensors) or any(b.down.device != x.device for b in banks):
         raise ValueError("adapter operands must be on one CUDA device")
-    if x.ndim != 2 or min(x.shape) < 1 or x.stride(1) != 1 or x.stride(0) < x.shape[1] or \
-            x.stride(0) % 8 or x.data_ptr() % 16:
+    if x.ndim != 2 or min(x.shape) < 1 or x.stride(1) != 1 or x.data_ptr() % 16 or \
+            (x.shape[0] > 1 and (x.stride(0) < x.shape[1] or x.stride(0) % 8)):
         raise ValueError("adapters require positive 16-byte aligned [M,K] activations")
     m, k = x.shape
     if row_slots.dtype != torch.int32 or row_slots.shape != (m,) or not row_slots.is_contiguous():
