@@ -766,7 +766,6 @@ int cubic_vocab_sample(const void* logits, int dtype, int64_t row_stride, int ro
         return fail(CUBIC_EWORKSPACE, "vocabulary sampling workspace %lld < %lld", (long long)workspace_bytes,
                     (long long)need);
     if (need && (!workspace || !aligned16(workspace))) return fail(CUBIC_EINVAL, "workspace must be 16-byte aligned");
-    if ((int64_t)rows * p.chunks >= INT_MAX) return fail(CUBIC_ENOTSUP, "vocabulary sampling: too many rows");
     cubic::VocabSampleArgs a = {};
     a.chunks = p.chunks;
     a.chunk = p.chunk;

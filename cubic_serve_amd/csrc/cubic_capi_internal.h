@@ -273,6 +273,7 @@ struct VocabSampleArgs {
     // chunks of `chunk` columns (a multiple of 8), a workgroup each: counters [rows],
     // zero between launches, heads [rows, chunks, kSampleHead], lists [rows, chunks, list_words]
     int chunks, chunk, list_words;
+    int row0;                     // the grid's first row
     uint32_t *counters, *heads, *lists;
 };
 hipError_t launch_vocab_sample(const VocabSampleArgs& a, hipStream_t s);

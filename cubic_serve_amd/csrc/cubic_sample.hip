@@ -14,6 +14,8 @@
 //   exceeds u S; its log-probability ln(w / S).
 // So a row takes at most three searches "first position whose inclusive count or
 // mass reaches X", each a descent over the bits of the logits' ordered keys.
+#include <algorithm>
+
 #include "cubic_device.h"
 #include "cubic_capi_internal.h"
 
@@ -680,7 +682,7 @@ __global__ __launch_bounds__(kThreads) void vocab_sample_kernel(VocabSampleArgs 
     __shared__ uint32_t wave_top[kWaves], wave_bad[kWaves], wave_lost[kWaves], listed, last;
     __shared__ double table[kTable];
     __shared__ Row r;
-    const int row = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
+    const int row = a.row0 + blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     if (row >= (a.live_count ? *a.live_count : a.live_rows)) return;
     const uint8_t* logits = row_of<TYPE>(a, row);
@@ -956,7 +958,7 @@ __global__ __launch_bounds__(kThreads) void vocab_sample_kernel(VocabSampleArgs 
 // ---------------------------------------------------------------------------
 __global__ __launch_bounds__(kThreads) void vocab_top_f32_kernel(VocabSampleArgs a) {
     __shared__ uint32_t wave_top[kWaves], wave_bad[kWaves];
-    const int row = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
+    const int row = a.row0 + blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     if (row >= (a.live_count ? *a.live_count : a.live_rows)) return;
     const int begin = chunk * a.chunk, end = min(a.width, begin + a.chunk);
@@ -1020,7 +1022,7 @@ __global__ __launch_bounds__(kThreads) void vocab_sample_f32_kernel(VocabSampleA
     __shared__ double table[kTable];
     __shared__ Row r;
     constexpr int kPer = Search<2>::kPer;
-    const int row = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
+    const int row = a.row0 + blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     if (row >= (a.live_count ? *a.live_count : a.live_rows)) return;
     const uint8_t* logits = row_of<2>(a, row);
@@ -1234,19 +1236,26 @@ __global__ __launch_bounds__(kThreads) void vocab_sample_f32_kernel(VocabSampleA
 
 }  // namespace
 
-hipError_t launch_vocab_sample(const VocabSampleArgs& a, hipStream_t s) {
-    const int grid = a.rows * a.chunks;
-    if (a.dtype == 2) {
-        vocab_top_f32_kernel<<<grid, kThreads, 0, s>>>(a);
+// In runs of rows whose workgroups fit a grid (fewer than 2^32 threads).
+hipError_t launch_vocab_sample(const VocabSampleArgs& args, hipStream_t s) {
+    VocabSampleArgs a = args;
+    const int most = (int)(((1ull << 32) / kThreads - 1) / a.chunks);
+    for (; a.row0 < a.rows; a.row0 += most) {
+        const int grid = std::min(a.rows - a.row0, most) * a.chunks;
+        if (a.dtype == 2) {
+            vocab_top_f32_kernel<<<grid, kThreads, 0, s>>>(a);
+            const hipError_t e = hipGetLastError();
+            if (e != hipSuccess) return e;
+            vocab_sample_f32_kernel<<<grid, kThreads, 0, s>>>(a);
+        } else if (a.dtype == 1) {
+            vocab_sample_kernel<1><<<grid, kThreads, 0, s>>>(a);
+        } else {
+            vocab_sample_kernel<0><<<grid, kThreads, 0, s>>>(a);
+        }
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
-        vocab_sample_f32_kernel<<<grid, kThreads, 0, s>>>(a);
-    } else if (a.dtype == 1) {
-        vocab_sample_kernel<1><<<grid, kThreads, 0, s>>>(a);
-    } else {
-        vocab_sample_kernel<0><<<grid, kThreads, 0, s>>>(a);
     }
-    return hipGetLastError();
+    return hipSuccess;
 }
 
 }  // namespace cubic

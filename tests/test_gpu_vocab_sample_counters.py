@@ -86,3 +86,31 @@ def test_the_largest_logit_fills_a_counter(dtype, rows, width):
             plan.launch()
             torch.cuda.synchronize()
             check(plan, rows=12)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_more_rows_than_a_grid_holds(dtype):
+    """4194304 workgroups of 1024 threads are more than one launch takes."""
+    rows, width = (1 << 22) + 37, 4
+    print(f"sample rows={rows} {dtype}", flush=True)
+    gen = torch.Generator(device=DEV).manual_seed(25)
+    logits = torch.randn((rows, width), generator=gen, device=DEV).to(dtype)
+    logits[5, 2] = float("nan")
+    column = lambda v, dt=FP32: torch.full((rows,), v, dtype=dt, device=DEV)
+    params = dict(temperatures=column(0.0), top_ks=column(0, torch.int64), top_ps=column(1.0), min_ps=column(0.0),
+                  uniforms=torch.rand(rows, generator=gen, device=DEV))
+    params["temperatures"][-50:] = 1.0
+    plan = sampling.VocabSamplingPlan(logits=logits, **params)
+    plan.tokens.fill_(-9)
+    live = torch.tensor([rows - 3], dtype=torch.int32, device=DEV)
+    plan.launch(live)
+    torch.cuda.synchronize()
+    first = (logits == logits.amax(1, keepdim=True)).int().argmax(1)
+    first[5] = -1
+    assert torch.equal(plan.tokens[:-50], first[:-50]) and not plan.valid[5] and plan.valid[6]
+    last = sampling.VocabSamplingPlan(logits=logits[-50:], **{k: v[-50:] for k, v in params.items()})
+    last.launch()
+    torch.cuda.synchronize()
+    check(last)
+    assert torch.equal(plan.tokens[-50:-3], last.tokens[:-3]) and torch.equal(plan.logprobs[-50:-3], last.logprobs[:-3])
+    assert (plan.tokens[-3:] == -9).all()
