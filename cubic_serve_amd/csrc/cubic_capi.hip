@@ -7,7 +7,6 @@
 #include <cstdlib>
 #include <mutex>
 #include <algorithm>
-#include <climits>
 
 #include "cubic_mi355x.h"
 #include "cubic_capi_internal.h"
@@ -928,7 +927,12 @@ int cubic_adapters(const void* x, int64_t ldx, const int32_t* row_slots, int64_t
             a.down_groups = (int)std::min<int64_t>(16, m);
         }
     }
-    if (items * chunks >= INT_MAX) return fail(CUBIC_ENOTSUP, "adapter extents too large");
+    // a grid of 256-thread workgroups holds fewer than 2^24 of them
+    const int64_t down = (by_slot ? a.items : ceil_div(m, 16 * a.down_rows) * a.down_groups) * a.split;
+    const int64_t join = a.join ? ceil_div(m * a.width, 1024) : 0;
+    if (!a.fused && std::max({items * chunks, down, join}) >= (1 << 24))
+        return fail(CUBIC_ENOTSUP, "adapter extents past a launch: m=%lld k=%lld columns=%lld ranks=%d", (long long)m,
+                    (long long)k, (long long)columns, a.width);
     return hip_status(cubic::launch_adapters(a, (hipStream_t)stream), "cubic_adapters launch");
 }
 

@@ -178,7 +178,8 @@ CUBIC_API int cubic_gemm_grouped(const void* x, int64_t ldx, const uint32_t* cod
  * result does not depend on m or on the other rows, bit for bit.  No output may
  * overlap x, another member's output or base, or the adapters.  1 <= m < 2^24,
  * slots < 2^20, k <= 2^20, ldx <= 2^23, ldbases and ldys <= 2^25, ns[j] *
- * max_ranks[j] < 2^30.
+ * max_ranks[j] < 2^30.  Extents whose launches would pass a grid are refused (from
+ * m times the members' ranks of 2^34 on, or 2^24 tiles of rows by columns or by K).
  * Workspace: cubic_adapters_workspace_bytes(m, k, members, max_ranks) bytes, not
  * initialised, 16-byte aligned; one per concurrently running launch.  It covers
  * every smaller m.

@@ -140,3 +140,13 @@ def test_binding_notices_a_bank_given_other_tensors():
     b.down = b.down.clone()
     with pytest.raises(ValueError, match="changed after binding"):
         launch.validate()
+
+
+@pytest.mark.parametrize("m,k,ns,caps", [
+    ((1 << 23) + 64, 1032, (8,) * 8, (256,) * 8),  # partitions to be joined
+    ((1 << 24) - 1, 64, (1 << 16,), (8,)),         # rows by columns
+    (1 << 23, 1 << 20, (8,), (8,)),                # rows by partitions of K
+])
+def test_entry_refuses_extents_past_a_grid(m, k, ns, caps):
+    with pytest.raises(ValueError, match="past a launch"):
+        _native.call("cubic_adapters", 4096, k, 4096, m, k, 2, len(ns), *tables(ns, caps), 0, 4096, 1 << 50, None)
