@@ -45,6 +45,7 @@ __device__ __forceinline__ uint4 load16(__amdgpu_buffer_rsrc_t r, uint32_t byte_
 typedef __attribute__((address_space(3))) void lds_void_t;
 // s_waitcnt immediate: at most n vector-memory accesses in flight, no LDS access.
 constexpr int vmcnt_and_lds(int n) { return (n & 0xF) | (0x7 << 4) | ((n >> 4) << 14); }
+constexpr int kParts = 3;          // 16-bit parts of t in the second product
 constexpr int kDownTileRanks = 8;  // 16-rank blocks of the prompts' down kernel
 
 // The tile's adapter slots, one per lane (-1: past the batch, kNone: no
@@ -426,33 +427,52 @@ __global__ __launch_bounds__(kThreads) void adapter_join_kernel(AdapterArgs a) {
 // that pattern runs at 4.6 - 4.8 TB/s where 64-byte pieces of 16 rows, which
 // the product's own layout gives, run at 3.1 - 3.7 (2048 x 24576 and 4096 x 8192).
 //
-// t is split into two 16-bit parts, t = hi + lo with an error below 2^-17
-// (bf16) or 2^-22 of the row's largest (fp16) of t, so that the only rounding
-// to 16 bits that counts is y's; the operator is bound by y's bytes, and the
-// second product costs matrix time that is idle.  fp16 parts are taken of t
-// scaled by a power of two to at most 1, which fp16's range needs and which
-// changes no digit of the product.
+// t is split into three 16-bit parts whose sum is all its 24 bits, so that the only
+// rounding to 16 bits is y's: with two, 2^-17 of t, what is left where the base
+// cancels the adapter is off by up to eleven times what binary32 allows.  The third
+// product and the longer split cost 0 to 2 %, at rank 128 6 to 8 % (4096 rows x 8192
+// columns, K = 8192, 103 -> 112 us; 2048 rows, K = 4096 39.5 -> 42.0).  All parts of a
+// value have its sign and none is 0 unless it is, so that a product with an
+// infinity of B is that infinity in each, as in the formula.  fp16 parts are taken of
+// t scaled by a power of two, its row's largest into [2^14, 2^15), which fp16's range
+// needs and which changes no digit of the product.
 // ---------------------------------------------------------------------------
+// Eight values t into their parts: each is what is left of t, cut to 16 bits
+// towards 0, so that all have t's sign, and at least a trifle (2^-30 of t, fp16:
+// 2^-24), so that none is 0 unless t is.
 template <bool F16>
-__device__ __forceinline__ void split_parts(const float* t, uint4& hi, uint4& lo) {
-    uint32_t h[4], l[4];
+__device__ __forceinline__ void split_parts(const float* t, uint4 (&part)[kParts]) {
+    uint32_t h[kParts][4];
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
-        const float a = t[2 * p], b = t[2 * p + 1];
-        h[p] = gemm::pack_level2<F16>(a, b);
-        float ha, hb;
-        if constexpr (F16) {
-            ha = half_bits_to_float(h[p] & 0xffffu);
-            hb = half_bits_to_float(h[p] >> 16);
-        } else {
-            ha = bf16_bits_to_float(h[p] & 0xffffu);
-            hb = bf16_bits_to_float(h[p] >> 16);
+        float rest[2], least[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const float x = t[2 * p + c];
+            least[c] = F16 ? __builtin_amdgcn_fmed3f(x * 0x1p60f, -0x1p-24f, 0x1p-24f) : x * 0x1p-30f;
+            rest[c] = F16 ? x + least[c] : x;
         }
-        // an infinity or NaN is whole in its first part
-        l[p] = gemm::pack_level2<F16>(__builtin_isfinite(ha) ? a - ha : 0.f, __builtin_isfinite(hb) ? b - hb : 0.f);
+#pragma unroll
+        for (int i = 0; i < kParts; ++i) {
+            float cut[2];
+            if constexpr (F16) {
+                h[i][p] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(rest[0], rest[1]));
+                cut[0] = half_bits_to_float(h[i][p] & 0xffffu);
+                cut[1] = half_bits_to_float(h[i][p] >> 16);
+            } else {
+                cut[0] = __uint_as_float(__float_as_uint(rest[0]) & 0xffff0000u);
+                cut[1] = __uint_as_float(__float_as_uint(rest[1]) & 0xffff0000u);
+                h[i][p] = __builtin_amdgcn_perm(__float_as_uint(rest[1]), __float_as_uint(rest[0]), 0x07060302u);
+            }
+            if (i == kParts - 1) break;
+            // the middle one: least <= rest - cut <= t in size; of an infinity the
+            // difference is NaN, and the result the smaller of the other two, itself
+#pragma unroll
+            for (int c = 0; c < 2; ++c) rest[c] = __builtin_amdgcn_fmed3f(rest[c] - cut[c], least[c], t[2 * p + c]);
+        }
     }
-    hi = uint4{h[0], h[1], h[2], h[3]};
-    lo = uint4{l[0], l[1], l[2], l[3]};
+#pragma unroll
+    for (int i = 0; i < kParts; ++i) part[i] = uint4{h[i][0], h[i][1], h[i][2], h[i][3]};
 }
 
 // The parts of a row of t (this lane's eight ranks of every step; lanes of one
@@ -460,7 +480,7 @@ __device__ __forceinline__ void split_parts(const float* t, uint4& hi, uint4& lo
 // to be multiplied by.
 template <bool F16, int KS>
 __device__ __forceinline__ float split_row(const floatx4_t (&v)[KS][2], int rank, float scale, int q,
-                                           uint4 (&hi)[KS], uint4 (&lo)[KS]) {
+                                           uint4 (&t16)[KS][kParts]) {
     float t[KS][8];
     float top = 0.f, back = 1.f;
 #pragma unroll
@@ -473,29 +493,29 @@ __device__ __forceinline__ float split_row(const floatx4_t (&v)[KS][2], int rank
     if constexpr (F16) {
         top = fmaxf(top, __uint_as_float(xor16_u32(__float_as_uint(top))));
         top = fmaxf(top, __uint_as_float(xor32_u32(__float_as_uint(top))));
-        // 2^-(exponent + 1) of the row's largest, kept within normal numbers
+        // the row's largest into [2^14, 2^15), the scale kept within normal numbers
         int ex = (int)(__float_as_uint(top) >> 23) - 126;
-        ex = top == 0.f || !__builtin_isfinite(top) ? 0 : min(max(ex, -120), 120);
-        const float down = __uint_as_float((uint32_t)(127 - ex) << 23);
-        back = __uint_as_float((uint32_t)(127 + ex) << 23);
+        ex = top == 0.f || !__builtin_isfinite(top) ? 15 : max(ex, -105);
+        const float down = __uint_as_float((uint32_t)(127 + 15 - ex) << 23);
+        back = __uint_as_float((uint32_t)(127 - 15 + ex) << 23);
 #pragma unroll
         for (int s = 0; s < KS; ++s)
 #pragma unroll
             for (int c = 0; c < 8; ++c) t[s][c] *= down;
     }
 #pragma unroll
-    for (int s = 0; s < KS; ++s) split_parts<F16>(t[s], hi[s], lo[s]);
+    for (int s = 0; s < KS; ++s) split_parts<F16>(t[s], t16[s]);
     return back;
 }
 
 // The parts of t of this lane's row (row0 + row, if own; rows of them from row0 on
-// are there): the partitions in ascending order, kParts requested together (four
+// are there): the partitions in ascending order, kAhead requested together (four
 // of 32 ranks: 26.0 us of 256 rows, rank 64, K = 12288, with eight 26.3, sixteen 27.5; what
 // the registers cost is more than the wait); what is not there (another row, past
 // the rank) reads as 0.
-template <bool F16, int KS, int kParts>
+template <bool F16, int KS, int kAhead>
 __device__ __forceinline__ float row_parts(const AdapterArgs& a, const AdapterMember& mb, int row0, int rows, int row,
-                                           bool own, int rank, float scale, int q, uint4 (&hi)[KS], uint4 (&lo)[KS]) {
+                                           bool own, int rank, float scale, int q, uint4 (&t16)[KS][kParts]) {
     uint32_t off[KS][2];
     floatx4_t v[KS][2];
 #pragma unroll
@@ -506,10 +526,10 @@ __device__ __forceinline__ float row_parts(const AdapterArgs& a, const AdapterMe
             off[s][c] = own && f < rank ? (uint32_t)(row * a.width + mb.rank0 + f) * 4 : kOutside;
             v[s][c] = floatx4_t{0.f, 0.f, 0.f, 0.f};
         }
-    for (int part = 0; part < a.split; part += kParts) {
-        floatx4_t in[kParts][KS][2];
+    for (int part = 0; part < a.split; part += kAhead) {
+        floatx4_t in[kAhead][KS][2];
 #pragma unroll
-        for (int p = 0; p < kParts; ++p) {
+        for (int p = 0; p < kAhead; ++p) {
             const int64_t at = ((int64_t)min(part + p, a.split - 1) * a.m + row0) * a.width;
             const auto buf = buffer(a.partial + at, part + p < a.split ? (int64_t)rows * a.width * 4 : 0);
 #pragma unroll
@@ -518,13 +538,13 @@ __device__ __forceinline__ float row_parts(const AdapterArgs& a, const AdapterMe
                 for (int c = 0; c < 2; ++c) in[p][s][c] = __builtin_bit_cast(floatx4_t, load16(buf, off[s][c]));
         }
 #pragma unroll
-        for (int p = 0; p < kParts; ++p)
+        for (int p = 0; p < kAhead; ++p)
 #pragma unroll
             for (int s = 0; s < KS; ++s)
 #pragma unroll
                 for (int c = 0; c < 2; ++c) v[s][c] += in[p][s][c];
     }
-    return split_row<F16, KS>(v, rank, scale, q, hi, lo);
+    return split_row<F16, KS>(v, rank, scale, q, t16);
 }
 
 // Rows of base or y from the tile's first on, and eight 16-bit values of one (its
@@ -596,7 +616,8 @@ __device__ __forceinline__ uint32_t add_pair(uint32_t in, float lo, float hi) {
 }
 
 template <bool F16, int KS, int WR, bool VEC>
-__global__ __launch_bounds__(kThreads) void adapter_up_kernel(AdapterArgs a) {
+// (two waves per SIMD, 256 registers; fp16 prompts of more than 128 ranks do not fit them)
+__global__ __launch_bounds__(kThreads, F16 && KS == 8 && WR == 4 ? 1 : 2) void adapter_up_kernel(AdapterArgs a) {
     constexpr int kColWaves = kWaves / WR;  // waves side by side
     constexpr int kTurn = kAdapterUpTurn, kPitch = kTurn + 4;
     __shared__ __attribute__((aligned(16))) float product[kWaves][16][kPitch];
@@ -641,8 +662,8 @@ __global__ __launch_bounds__(kThreads) void adapter_up_kernel(AdapterArgs a) {
         const int rank = e >= 0 ? min(mb.ranks[e], max_rank) : 0;
         if (rank <= 0 && in_place) continue;
         const float scale = e >= 0 ? mb.scales[e] : 0.f;
-        uint4 hi[KS], lo[KS];
-        const float back = row_parts<F16, KS, KS < 4 ? 4 / KS : 1>(a, mb, row0, rows, row_of(col), (mine >> col) & 1, rank, scale, q, hi, lo);
+        uint4 t16[KS][kParts];
+        const float back = row_parts<F16, KS, KS < 4 ? 4 / KS : 1>(a, mb, row0, rows, row_of(col), (mine >> col) & 1, rank, scale, q, t16);
         const auto up = buffer(mb.up + (e >= 0 ? (int64_t)e * n * max_rank : 0), (int64_t)n * max_rank * 2);
         for (int c0 = c_begin; c0 < c_end; c0 += kColWaves * kTurn) {
             // base and y: rows q, q + 4, ..., eight columns per lane; what is
@@ -676,8 +697,8 @@ __global__ __launch_bounds__(kThreads) void adapter_up_kernel(AdapterArgs a) {
 #pragma unroll
                     for (int u = 0; u < kHalf; ++u) {
                         if (s == 0) acc[u] = floatx4_t{0.f, 0.f, 0.f, 0.f};
-                        acc[u] = mfma16<F16>(b[v & 1][u], lo[s], acc[u]);
-                        acc[u] = mfma16<F16>(b[v & 1][u], hi[s], acc[u]);
+#pragma unroll
+                        for (int i = 0; i < kParts; ++i) acc[u] = mfma16<F16>(b[v & 1][u], t16[s][i], acc[u]);
                         if (s == KS - 1)
                             *(floatx4_t*)&product[wave][col][16 * (v / KS * kHalf + u) + 4 * q] = acc[u] * back;
                     }
@@ -767,8 +788,8 @@ __global__ __launch_bounds__(kThreads) void adapter_up_tile_kernel(AdapterArgs a
         issue(c_begin, 0);
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) next[i] = load8<VEC>(base, row_at(i, c_begin, ldbase), c_begin + rc, n);
-        uint4 hi[KS], lo[KS];
-        const float back = row_parts<F16, KS, 1>(a, mb, row0, 16, col, (mine >> col) & 1, rank, scale, q, hi, lo);
+        uint4 t16[KS][kParts];
+        const float back = row_parts<F16, KS, 1>(a, mb, row0, 16, col, (mine >> col) & 1, rank, scale, q, t16);
         int h = 0;
         for (int c0 = c_begin; c0 < c_end; c0 += kTurn, h ^= 1) {
             // this wave's loads of the turn have landed (the last turn's
@@ -796,8 +817,8 @@ __global__ __launch_bounds__(kThreads) void adapter_up_tile_kernel(AdapterArgs a
 #pragma unroll
                 for (int s = 0; s < KS; ++s) {
                     const uint4 b = *(const uint4*)(from + s * kSlab + u * 1024);
-                    acc = mfma16<F16>(b, lo[s], acc);
-                    acc = mfma16<F16>(b, hi[s], acc);
+#pragma unroll
+                    for (int i = 0; i < kParts; ++i) acc = mfma16<F16>(b, t16[s][i], acc);
                 }
                 *(floatx4_t*)&product[wave][col][16 * u + 4 * q] = acc * back;
             }
@@ -899,7 +920,7 @@ __global__ __launch_bounds__(kAdapterRowWaves * 64) void adapter_row_kernel(Adap
     __syncthreads();
     // t of row col, ranks 8 q .. 8 q + 7 (q < 2): lane 16 (rank / 4) + col holds
     // four ranks; quarters and partitions in order
-    uint4 hi[1], lo[1];
+    uint4 t16[1][kParts];
     floatx4_t t8[1][2];
     t8[0][0] = t8[0][1] = floatx4_t{0.f, 0.f, 0.f, 0.f};
     if (q < 2)
@@ -909,7 +930,7 @@ __global__ __launch_bounds__(kAdapterRowWaves * 64) void adapter_row_kernel(Adap
                 const int at = 16 * (2 * q + c) + col;
                 t8[0][c] += (quarters[j][at] + quarters[j + 1][at]) + (quarters[j + 2][at] + quarters[j + 3][at]);
             }
-    const float back = split_row<F16, 1>(t8, rank, scale, q, hi, lo);
+    const float back = split_row<F16, 1>(t8, rank, scale, q, t16);
     if (rank <= 0 && in_place) return;
     for (int c0 = c_begin; c0 < c_end; c0 += TURNS * kW * kTurn) {
         if (c0 != c_begin) fetch(c0);
@@ -921,8 +942,10 @@ __global__ __launch_bounds__(kAdapterRowWaves * 64) void adapter_row_kernel(Adap
                     floatx4_t acc[2];
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
-                        acc[u] = mfma16<F16>(b[v][2 * g + u], lo[0], floatx4_t{0.f, 0.f, 0.f, 0.f});
-                        acc[u] = mfma16<F16>(b[v][2 * g + u], hi[0], acc[u]) * back;
+                        acc[u] = floatx4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                        for (int i = 0; i < kParts; ++i) acc[u] = mfma16<F16>(b[v][2 * g + u], t16[0][i], acc[u]);
+                        acc[u] *= back;
                     }
                     in[v][g].x = add_pair<F16>(in[v][g].x, acc[0][0], acc[0][1]);
                     in[v][g].y = add_pair<F16>(in[v][g].y, acc[0][2], acc[0][3]);

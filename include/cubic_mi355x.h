@@ -162,8 +162,8 @@ CUBIC_API int cubic_gemm_grouped(const void* x, int64_t ldx, const uint32_t* cod
  * j of up to 8 projections that share x,
  *   y_j[i, :] = base_j[i, :] + scales_j[e] * up_j[e] . (down_j[e] . x[i, :])
  * rounded once to dtype; everything before is held in 32 bits (the rank-wide
- * intermediate enters the second product as two 16-bit parts whose sum is it to
- * 17 bits or more).  A slot outside [0, slots) or of rank 0 leaves y = base.
+ * intermediate enters the second product as three 16-bit parts that are all of
+ * it). A slot outside [0, slots) or of rank 0 leaves y = base.
  *   x          dtype [m, ldx], 16-byte aligned, k % 8 == 0, ldx % 8 == 0
  *   row_slots  int32 [m], any order
  *   downs[j]   dtype [slots, max_ranks[j], k], 16-byte aligned; rows at or past a
