@@ -593,7 +593,8 @@ __device__ __forceinline__ uint32_t word_hits(const uint4& v, uint32_t pattern) 
 }
 
 // The nth column of the key among [begin, end) is the token: WORDS words per
-// thread at a time, each wave a run of them, in order.
+// thread at a time, each wave a run of them, in order.  There is one, unless the
+// caller has rewritten the logits meanwhile: the row is refused then.
 template <int TYPE, int WORDS>
 __device__ __forceinline__ void locate(Search<TYPE>& sh, const VocabSampleArgs& a, int row, const uint8_t* logits,
                                        int begin, int end, const Row& r, uint32_t top, const Choice& choice) {
@@ -601,6 +602,7 @@ __device__ __forceinline__ void locate(Search<TYPE>& sh, const VocabSampleArgs& 
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const uint32_t pattern = pattern_of<TYPE>(choice.key);
     const bool ragged = end == a.width && a.width % kEach != 0;  // a word reaches past the row
+    const uint64_t nth = max(choice.nth, (uint64_t)1);
     uint64_t past = 0;  // columns of the key so far
     for (int c0 = begin; c0 < end; c0 += kThreads * WORDS * kEach) {
         // the words of a pass, evenly over the waves
@@ -628,29 +630,38 @@ __device__ __forceinline__ void locate(Search<TYPE>& sh, const VocabSampleArgs& 
         const uint32_t here = (uint32_t)__builtin_amdgcn_readlane((int)wave_scan_u32(mine), 63);
         uint64_t all;
         uint64_t from = past + before_wave(here, sh.sums[0], lane, wave, all);
-        if (from < choice.nth && from + here >= choice.nth) {  // this wave holds it
+        if (from < nth && from + here >= nth) {  // this wave holds it
 #pragma unroll
             for (int i = 0; i < WORDS; ++i) {
                 if (__ballot(hits[i] != 0) == 0) continue;
                 const uint32_t number = __builtin_popcount(hits[i]), sum = wave_scan_u32(number);
                 const uint64_t before = from + sum - number;
-                if (before < choice.nth && before + number >= choice.nth) {
+                if (before < nth && before + number >= nth) {
                     uint32_t left = hits[i];
-                    for (uint64_t k = before + 1; k < choice.nth; ++k) left &= left - 1;
+                    for (uint64_t k = before + 1; k < nth; ++k) left &= left - 1;
                     publish(a, row, first + i * 64 * kEach + __builtin_ctz(left), sh.logprob);
                 }
                 from += (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
             }
         }
         past += all;
-        if (past >= choice.nth) return;
+        if (past >= nth) return;
         __syncthreads();  // the sums are free again
     }
+    refuse(a, row);
 }
 
 template <int TYPE>
 __device__ __forceinline__ const uint8_t* row_of(const VocabSampleArgs& a, int row) {
     return (const uint8_t*)a.logits + (int64_t)row * a.row_stride * (TYPE == 2 ? 4 : 2);
+}
+
+// Whether the row is sampled, read once for the workgroup (as Row is).
+__device__ __forceinline__ bool row_lives(const VocabSampleArgs& a, int row, uint32_t* lds) {
+    if (!a.live_count) return row < a.live_rows;
+    if (threadIdx.x == 0) *lds = row < *a.live_count;
+    __syncthreads();
+    return *lds != 0;
 }
 
 // ---------------------------------------------------------------------------
@@ -684,7 +695,12 @@ __global__ __launch_bounds__(kThreads) void vocab_sample_kernel(VocabSampleArgs 
     __shared__ Row r;
     const int row = a.row0 + blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
-    if (row >= (a.live_count ? *a.live_count : a.live_rows)) return;
+    if (!row_lives(a, row, &last)) {
+        // (all of a row's workgroups arrive or none: a count rewritten meanwhile would
+        // leave the row's counter between its ends)
+        if (a.live_count && arrive_last(a.counters + row, a.chunks, &last) && t == 0) store_device(a.counters + row, 0u);
+        return;
+    }
     const uint8_t* logits = row_of<TYPE>(a, row);
     uint32_t counted = 0;  // this thread's columns, -inf left out
     {
@@ -957,10 +973,13 @@ __global__ __launch_bounds__(kThreads) void vocab_sample_kernel(VocabSampleArgs 
 // With a chunk per row there is nothing to share out, and the scans stay.
 // ---------------------------------------------------------------------------
 __global__ __launch_bounds__(kThreads) void vocab_top_f32_kernel(VocabSampleArgs a) {
-    __shared__ uint32_t wave_top[kWaves], wave_bad[kWaves];
+    __shared__ uint32_t wave_top[kWaves], wave_bad[kWaves], live;
     const int row = a.row0 + blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    if (row >= (a.live_count ? *a.live_count : a.live_rows)) return;
+    // the sampling launch finds the row's counter at 0, whatever became of the last
+    // one's arrivals (its workgroups read the row's parameters each for itself)
+    if (a.chunks > 1 && chunk == 0 && t == 0) store_device(a.counters + row, 0u);
+    if (!row_lives(a, row, &live)) return;
     const int begin = chunk * a.chunk, end = min(a.width, begin + a.chunk);
     uint32_t top = 0, bad = 0;
     each_column<2>(row_of<2>(a, row), begin, end, a.width, [&](int, uint32_t key) {
@@ -1024,7 +1043,7 @@ __global__ __launch_bounds__(kThreads) void vocab_sample_f32_kernel(VocabSampleA
     constexpr int kPer = Search<2>::kPer;
     const int row = a.row0 + blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
-    if (row >= (a.live_count ? *a.live_count : a.live_rows)) return;
+    if (!row_lives(a, row, &last)) return;
     const uint8_t* logits = row_of<2>(a, row);
     uint32_t* const heads = a.heads + (int64_t)row * a.chunks * kSampleHead;
     if (wave == 0) {
@@ -1185,10 +1204,12 @@ __global__ __launch_bounds__(kThreads) void vocab_sample_f32_kernel(VocabSampleA
         if (wave == 0) {
             uint32_t number = 0;
             if (lane < a.chunks) {
-                // (no finite number's digit is the last)
+                // (no finite number's digit is the last; within the list also if the
+                // caller rewrites the logits meanwhile)
                 const uint16_t* from = (const uint16_t*)(lists + (int64_t)lane * a.list_words + runs) + digit;
-                const uint32_t run = load_device(from);
-                number = load_device(from + 1) - run;
+                const uint32_t run = min((uint32_t)load_device(from), (uint32_t)a.chunk);
+                const uint32_t next = digit + 1 < kSampleBins ? min((uint32_t)load_device(from + 1), (uint32_t)a.chunk) : run;
+                number = next > run ? next - run : 0;
                 s.held[lane] = (int)run;
             }
             const uint32_t scan = wave_scan_u32(number);
@@ -1228,6 +1249,7 @@ __global__ __launch_bounds__(kThreads) void vocab_sample_f32_kernel(VocabSampleA
                 for (uint32_t i = 0; i < listed; ++i) before += s.deep_count[i] < mine;
                 if (before + 1 == choice.nth) publish(a, row, (int)mine, s.logprob);
             }
+            if (choice.nth < 1 || choice.nth > listed) refuse(a, row);  // (as in locate)
             return;
         }
     }
