@@ -10,8 +10,9 @@ launch follows later changes of both.
 
 ``PackedLinearOperators.bind_adapters`` adds to given projection outputs and
 ``bind_adapted_linear`` binds the shared projection with it.  No counterpart in
-the reference.  The kernels are cubic_adapters (one down and one up launch);
-there is no eager fallback.
+the reference.  The kernels are cubic_adapters (one launch for few rows, else
+a down and an up launch, with one between them that joins partial sums of
+long K); there is no eager fallback.
 """
 from __future__ import annotations
 

@@ -4,8 +4,9 @@
 //   y[i, :]   = round16(base[i, :] + s_e B_e t[i, :])
 //
 // for up to kMaxGemmMembers projections that share x.  Few rows: one launch
-// (adapter_row_kernel).  Else two: a down kernel writes t as binary32 partial
-// sums over K partitions, an up kernel adds the partitions and finishes the rows.
+// (adapter_row_kernel).  Else a down kernel writes t as binary32 partial sums over K
+// partitions and an up kernel adds them and finishes the rows; where column chunks
+// would add them much again, a launch between the two does (adapter_join_kernel).
 //
 // Rows come in any order, without a grouping launch or any host knowledge of
 // the slots.  Batches of some size are tiled in order of adapters, each

@@ -307,7 +307,7 @@ struct AdapterArgs {
     int rank_tiles;               // ceil(largest max_rank / 16)
     int vectors;                  // every member: 16-byte base and output accesses
     int fused;                    // one launch (few rows); chunks: the widest member's
-    int down_rows, up_rows;       // 16-row tiles per workgroup: 1 or 2; 1 or 4
+    int down_rows, up_rows;       // 16-row tiles per workgroup: 1, 2 or 4 (A in LDS); 1 or 4
     int items;                    // tiles of rows in order of adapters (0: tiles of the rows as they are)
     int join;                     // add the partitions in a launch of their own
     int up_tile;                  // 64-row tiles with B in LDS (prompts)

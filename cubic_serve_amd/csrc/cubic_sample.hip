@@ -4,7 +4,8 @@
 // Order of a row: logit descending, column ascending on ties (-0 == +0).  Weight
 // of a column: w = 2^((l - max) log2(e) / T), in 64-bit fixed point with 2^43 for
 // the maximum (so up to 2^20 columns sum below 2^63 and sums do not depend on
-// their order; a weight is off by at most half a unit, 2^-44 of the maximum's).
+// their order; a weight is off by at most half a unit, 2^-44 of the maximum's, and a
+// sum over 151936 columns by 2^-26 of it, below the 2^-24 steps of u).
 // What top-k, top-p and min-p keep is a prefix of the order each, and a prefix is
 // as good as its mass:
 //   S_k  mass of the first k

@@ -428,8 +428,10 @@ class VocabSamplingPlan:
     [rows].  Outputs: ``tokens`` int64, ``valid`` bool and ``logprobs`` float32
     [rows], the log-probability of the token among those kept.  A row with NaN,
     +inf or no finite logit, or with a parameter out of range, publishes
-    (-1, False, NaN).  The plan owns its outputs and its workspace: launches of
-    one plan must not overlap.
+    (-1, False, NaN).  The plan owns its outputs and its workspace, which is
+    cleared on the current stream: a launch on another one has to follow it, and
+    launches of one plan must not overlap.  Logits must not change while a launch
+    runs; settings that do leave that launch's tokens unspecified.
     """
 
     def __init__(self, *, logits: Tensor, temperatures: Tensor, top_ks: Tensor, top_ps: Tensor,

@@ -272,6 +272,8 @@ CUBIC_API int cubic_root_sample(const void* scores, int scores_fp16, const int64
  * the ranges above, publishes -1, 0, NaN.  Rows at or past live_rows (live_count[0],
  * a device int32 read when the launch runs, if given) are left as they are.
  *   1 <= rows < 2^24, 1 <= width <= 2^20, width <= row_stride
+ * Settings or live_count rewritten while a launch runs leave its rows' tokens
+ * unspecified, and nothing else.  Logits must not change while a launch runs.
  * Workspace: cubic_vocab_sample_workspace_bytes(rows, width, dtype) bytes (-1:
  * outside the ranges above), 16-byte aligned, zero-filled before the first launch; a
  * completed launch leaves the counters in it zero again.  One per launch that may
