@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from cubic_serve_amd import adapters, linear
-from test_gpu_adapters import DEV, case, check
+from test_gpu_adapters import DEV, case, check, reference
 
 pytestmark = pytest.mark.gpu
 DTYPES = [torch.bfloat16, torch.float16]
@@ -77,8 +77,6 @@ def test_infinities_in_the_second_matrix(m, k, ranks, capacity, dtype):
     assert torch.equal(torch.sign(got)[torch.isinf(want)], torch.sign(want)[torch.isinf(want)])
     # every other element is what it is without them
     clean = [(d, torch.where(torch.isinf(u), torch.zeros_like(u), u), s) for d, u, s in held]
-    from test_gpu_adapters import reference
-
     value, bound = reference(x, base, clean, slots)
     finite = want == 0
     assert ((got - value).abs() <= bound)[finite].all()
