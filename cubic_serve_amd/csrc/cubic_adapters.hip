@@ -431,8 +431,8 @@ __global__ __launch_bounds__(kThreads) void adapter_join_kernel(AdapterArgs a) {
 // t is split into three 16-bit parts whose sum is all its 24 bits, so that the only
 // rounding to 16 bits is y's: with two, 2^-17 of t, what is left where the base
 // cancels the adapter is off by up to eleven times what binary32 allows.  The third
-// product and the longer split cost 0 to 2 %, at rank 128 6 to 8 % (4096 rows x 8192
-// columns, K = 8192, 103 -> 112 us; 2048 rows, K = 4096 39.5 -> 42.0).  All parts of a
+// product and the longer split cost 0 to 2 %, at rank 128 1 to 4 % (4096 rows x 8192
+// columns, K = 8192, 104 -> 108 us; 2048 rows, K = 4096 39.9 -> 40.3).  All parts of a
 // value have its sign and none is 0 unless it is, so that a product with an
 // infinity of B is that infinity in each, as in the formula.  fp16 parts are taken of
 // t scaled by a power of two, its row's largest into [2^14, 2^15), which fp16's range
@@ -813,15 +813,25 @@ __global__ __launch_bounds__(kThreads) void adapter_up_tile_kernel(AdapterArgs a
             __builtin_amdgcn_sched_barrier(0);
             const uint8_t* from = stage + h * KS * kSlab + col * 64 + ((q ^ (col >> 1)) & 3) * 16;
 #pragma unroll
-            for (int u = 0; u < kTiles; ++u) {
-                floatx4_t acc = {0.f, 0.f, 0.f, 0.f};
+            for (int u0 = 0; u0 < kTiles; u0 += 4) {
+                // four column tiles side by side: one's products wait for each other
+                // (4096 rows x 8192 columns, rank 128: one by one 61 us, so 56)
+                floatx4_t acc[4];
 #pragma unroll
                 for (int s = 0; s < KS; ++s) {
-                    const uint4 b = *(const uint4*)(from + s * kSlab + u * 1024);
+                    uint4 b[4];
 #pragma unroll
-                    for (int i = 0; i < kParts; ++i) acc = mfma16<F16>(b, t16[s][i], acc);
+                    for (int u = 0; u < 4; ++u) b[u] = *(const uint4*)(from + s * kSlab + (u0 + u) * 1024);
+#pragma unroll
+                    for (int i = 0; i < kParts; ++i)
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) {
+                            if (s == 0 && i == 0) acc[u] = floatx4_t{0.f, 0.f, 0.f, 0.f};
+                            acc[u] = mfma16<F16>(b[u], t16[s][i], acc[u]);
+                        }
                 }
-                *(floatx4_t*)&product[wave][col][16 * u + 4 * q] = acc * back;
+#pragma unroll
+                for (int u = 0; u < 4; ++u) *(floatx4_t*)&product[wave][col][16 * (u0 + u) + 4 * q] = acc[u] * back;
             }
             __builtin_amdgcn_wave_barrier();
 #pragma unroll
