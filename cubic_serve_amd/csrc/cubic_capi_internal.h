@@ -255,7 +255,7 @@ constexpr int kMaxSampleWidth = 1 << 20;
 constexpr int kMaxSampleChunks = 64;
 constexpr int kSampleList = 32768;     // distinct 16-bit logits, or 32-bit ones' columns, that a chunk's list holds
 constexpr int kSampleBins = 4096;      // bins of a chunk's list of 32-bit logits, four words each
-constexpr int kSampleHead = 8;         // words of a chunk's head
+constexpr int kSampleHead = 16;        // words of a chunk's head
 struct VocabSampleArgs {
     const void* logits;           // [rows, row_stride] bf16, fp16 or fp32 (dtype)
     int64_t row_stride;           // elements

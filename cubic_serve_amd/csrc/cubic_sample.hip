@@ -209,6 +209,22 @@ struct Row {
         u = a.uniforms[row];
         top_k = a.top_ks[row];
     }
+    // As words of a chunk's head, for a launch that follows.
+    __device__ __forceinline__ void put(uint32_t* head) const {
+        head[0] = __float_as_uint(temperature);
+        head[1] = __float_as_uint(top_p);
+        head[2] = __float_as_uint(min_p);
+        head[3] = __float_as_uint(u);
+        head[4] = (uint32_t)top_k;
+        head[5] = (uint32_t)((uint64_t)top_k >> 32);
+    }
+    __device__ __forceinline__ void get(const uint32_t* head) {
+        temperature = __uint_as_float(head[0]);
+        top_p = __uint_as_float(head[1]);
+        min_p = __uint_as_float(head[2]);
+        u = __uint_as_float(head[3]);
+        top_k = (int64_t)((uint64_t)head[5] << 32 | head[4]);
+    }
     __device__ __forceinline__ void prepare() {
         scale = 128.0 * 1.4426950408889634074 / (double)temperature;
         least = min_p > 0.f ? 128.0 * log2((double)min_p) : -__builtin_inf();
@@ -972,15 +988,27 @@ __global__ __launch_bounds__(kThreads) void vocab_sample_kernel(VocabSampleArgs 
 // a bin is a run of each chunk's: 128001 columns, 48 rows, three searches, 78 -> 50 us
 // against scans of the row by the one workgroup (17 us each, what one CU reads).
 // With a chunk per row there is nothing to share out, and the scans stay.
+// The first launch also reads a row's settings and whether it lives, into the first
+// chunk's head: the second one's workgroups, which meet at the row's counter, all
+// go by that, whatever a caller rewrites meanwhile.
 // ---------------------------------------------------------------------------
+constexpr int kHeadLives = 8, kHeadRow = 9;  // words of the first chunk's head
 __global__ __launch_bounds__(kThreads) void vocab_top_f32_kernel(VocabSampleArgs a) {
     __shared__ uint32_t wave_top[kWaves], wave_bad[kWaves], live;
     const int row = a.row0 + blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    // the sampling launch finds the row's counter at 0, whatever became of the last
-    // one's arrivals (its workgroups read the row's parameters each for itself)
-    if (a.chunks > 1 && chunk == 0 && t == 0) store_device(a.counters + row, 0u);
-    if (!row_lives(a, row, &live)) return;
+    uint32_t* const head = a.heads + ((int64_t)row * a.chunks + chunk) * kSampleHead;
+    const bool lives = row_lives(a, row, &live);
+    if (chunk == 0 && t == 0) {
+        head[kHeadLives] = lives;
+        Row r;
+        r.read(a, row);
+        r.put(head + kHeadRow);
+    }
+    if (!lives) {
+        if (t == 0) head[1] = 1;  // (where only some of its workgroups saw it live)
+        return;
+    }
     const int begin = chunk * a.chunk, end = min(a.width, begin + a.chunk);
     uint32_t top = 0, bad = 0;
     each_column<2>(row_of<2>(a, row), begin, end, a.width, [&](int, uint32_t key) {
@@ -998,7 +1026,6 @@ __global__ __launch_bounds__(kThreads) void vocab_top_f32_kernel(VocabSampleArgs
     top = wave_max_u32(lane < kWaves ? wave_top[lane] : 0);
     bad = __ballot(lane < kWaves && wave_bad[lane]) != 0;
     if (t == 0) {
-        uint32_t* head = a.heads + ((int64_t)row * a.chunks + chunk) * kSampleHead;
         head[0] = top;
         head[1] = bad;
     }
@@ -1044,12 +1071,12 @@ __global__ __launch_bounds__(kThreads) void vocab_sample_f32_kernel(VocabSampleA
     constexpr int kPer = Search<2>::kPer;
     const int row = a.row0 + blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
-    if (!row_lives(a, row, &last)) return;
     const uint8_t* logits = row_of<2>(a, row);
     uint32_t* const heads = a.heads + (int64_t)row * a.chunks * kSampleHead;
+    if (!heads[kHeadLives]) return;
     if (wave == 0) {
         if (t == 0) {
-            r.read(a, row);
+            r.get(heads + kHeadRow);
             r.prepare();
             listed = 0;
         }
