@@ -15,6 +15,7 @@ _lib: ctypes.CDLL | None = None
 P = ctypes.c_void_p
 I32 = ctypes.c_int
 I64 = ctypes.c_int64
+F32 = ctypes.c_float
 
 ABI_VERSION = 6  # cubic_abi_version() of the library these signatures describe
 
@@ -38,6 +39,11 @@ SIGNATURES: dict[str, tuple] = {
     "cubic_vocab_sample": (I32, [P, I32, I64, I32, I32, I32, P, P, P, P, P, P, P, P, P, P, I64, P]),
     "cubic_adapters_workspace_bytes": (I64, [I64, I64, I32, P]),
     "cubic_adapters": (I32, [P, I64, P, I64, I64, I32, I32, P, P, P, P, P, P, P, P, P, P, I32, P, I64, P]),
+    "cubic_row_norm": (I32, [P, I64, P, I64, P, I64, I64, I32, F32, F32, P, I64, P, I64, P, I64, P, I64, I64, P]),
+    "cubic_quantize_rows": (I32, [P, I64, P, I64, I64, I64, I32, P, I64, P, I64, I64, P]),
+    "cubic_block_prepared_bytes": (I64, [I64, I64]),
+    "cubic_block_prepare": (I32, [P, I64, I64, I64, P, P]),
+    "cubic_block_gemm": (I32, [P, I64, P, I64, I64, I64, I64, I32, P, P, P, P, P, I32, P]),
     "cubic_moe_pad_routes": (I32, [P, P, P, P, P, I32, I32, I32, P, P, P, P]),
     "cubic_moe_max_blocks": (I64, [I64, I32, I32]),
     "cubic_moe_gemm": (I32, [P, I64, P, P, I64, I64, P, P, P, I64, I32, I32, I32, I64, I64, I32, I32, I32,

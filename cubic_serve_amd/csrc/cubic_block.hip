@@ -1,0 +1,237 @@
+// Block-scaled 8-bit products for gfx950:
+//
+//   y[m, n] = sum_b sx[m, b] sw[n / 128, b] sum_{k in block b} xq[m, k] wq[n, k]
+//
+// over e4m3 values and blocks of 128 columns.  One v_mfma_f32_16x16x128_f8f6f4
+// (unscaled form: the plain products of its 8-bit operands, at twice the rate of
+// the K = 32 ones) is one block of a 16 x 16 tile, so each block's product
+// starts from zero and is added to the 32-bit accumulator under its scale.
+// The instruction adds eight neighbouring products at 14 bits below the largest's
+// exponent, and those sums in 32 bits.  That is the one rounding below 32 bits here,
+// taken for its rate: of N(0, 1) operands it leaves y 1.5e-5 off (root mean
+// square), a hundredth of bf16's rounding and a fourteenth of fp16's.
+// Weights are its first operand: a lane then holds four columns n of one row m, the
+// scale is one number per lane, and outputs leave four columns at a time.
+//
+// Any order of k inside a block serves as long as both operands have it.  Here
+// lane l of an operand has row l % 16 and the 16 bytes at 16 (l / 16) of each half
+// block: loads of 64 contiguous bytes per row of x.  Weights are laid out once as
+// [tile of 16 rows][block][half][lane][16 bytes], 2 KB per tile and block.
+#include "cubic_capi_internal.h"
+#include "cubic_device.h"
+
+namespace cubic {
+namespace {
+
+typedef int v8i __attribute__((ext_vector_type(8)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+constexpr int kBlockBytes = 2048;              // one tile and block
+constexpr uint32_t kPastEnd = 0x80000000u;     // a buffer offset past every extent
+
+__device__ __forceinline__ v8i join(u32x4_dev_t a, u32x4_dev_t b) {
+    return v8i{(int)a.x, (int)a.y, (int)a.z, (int)a.w, (int)b.x, (int)b.y, (int)b.z, (int)b.w};
+}
+
+// 16 x 16 products over one block from zero: rows of w by rows of x.
+__device__ __forceinline__ v4f block_product(v8i w, v8i x) {
+    const v4f zero = {0.f, 0.f, 0.f, 0.f};
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, zero, 0, 0, 0, 0, 0, 0);
+}
+
+// Four columns of one row of y.
+__device__ __forceinline__ void store4(const BlockGemmArgs& a, const BlockMember& w, int64_t m, int n, v4f v) {
+    if (n >= w.n) return;
+    if (a.out == 2) {
+        float* y = static_cast<float*>(w.y) + m * w.ldy + n;
+        if (w.vec && n + 4 <= w.n) {
+            *reinterpret_cast<v4f*>(y) = v;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (n + i < w.n) y[i] = v[i];
+        }
+        return;
+    }
+    uint32_t lo, hi;
+    if (a.out == 1) {
+        lo = float_to_f16_bits(v[0]) | float_to_f16_bits(v[1]) << 16;
+        hi = float_to_f16_bits(v[2]) | float_to_f16_bits(v[3]) << 16;
+    } else {
+        lo = pack_bf16x2(v[0], v[1]);
+        hi = pack_bf16x2(v[2], v[3]);
+    }
+    uint16_t* y = static_cast<uint16_t*>(w.y) + m * w.ldy + n;
+    if (w.vec && n + 4 <= w.n) {
+        *reinterpret_cast<uint2*>(y) = make_uint2(lo, hi);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (n + i < w.n) y[i] = (uint16_t)((i < 2 ? lo : hi) >> (16 * (i & 1)));
+    }
+}
+
+// The member and its first tile of a column group.
+__device__ __forceinline__ int find_member(const BlockGemmArgs& a, int group) {
+    int j = 0;
+    for (int i = 0; i + 1 < a.members; ++i) j += group >= a.group_end[i];
+    return j;
+}
+
+// ---------------------------------------------------------------------------
+// Few rows: the weight stream bounds it.  A workgroup has NT tiles of columns and
+// 16 MT rows; its waves take the blocks of K in turn, each block's weights and
+// activations straight into registers, DEPTH blocks ahead, no barrier until
+// the waves' sums are added through LDS, in the order of the waves.
+// ---------------------------------------------------------------------------
+template <int NT, int MT, int DEPTH>
+__global__ __launch_bounds__(512) void block_stream_kernel(BlockGemmArgs a) {
+    extern __shared__ __attribute__((aligned(16))) float sums[];  // [waves][NT * MT][64] of four
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int waves = blockDim.x >> 6;
+    const int quarter = lane >> 4, row = lane & 15;
+    const int j = find_member(a, blockIdx.x);
+    const BlockMember& w = a.member[j];
+    const int tile0 = (blockIdx.x - (j ? a.group_end[j - 1] : 0)) * NT;
+    const int m0 = blockIdx.y * (16 * MT);
+    const int rows = min(16 * MT, a.m - m0);
+
+    const uint8_t* x = a.x + (int64_t)m0 * a.ldx;
+    const __amdgpu_buffer_rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint8_t*>(x), 0, (int)((rows - 1) * a.ldx) + a.k, 0x00020000);
+    uint32_t x_at[MT];
+    const float* sx[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        x_at[i] = (uint32_t)((16 * i + row) * a.ldx) + 16u * quarter;
+        sx[i] = a.x_scales + (int64_t)min(m0 + 16 * i + row, a.m - 1) * a.scale_row;
+    }
+    // a buffer per workgroup: tiles and blocks past the last read nothing
+    const int tile_bytes = a.blocks * kBlockBytes;
+    const __amdgpu_buffer_rsrc_t wr = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint8_t*>(w.codes + (int64_t)tile0 * tile_bytes), 0, min(NT, w.tiles - tile0) * tile_bytes, 0x00020000);
+    const uint32_t w_at = lane * 16;
+    const float* sw = w.scales + (int64_t)(tile0 >> 3) * a.blocks;
+
+    struct Stage {
+        u32x4_dev_t w[NT][2], x[MT][2];
+        float sx[MT], sw;
+    };
+    Stage st[DEPTH];
+    auto load = [&](Stage& s, int b) {
+        const bool some = b < a.blocks;
+        const uint32_t from = some ? (uint32_t)b * kBlockBytes : kPastEnd;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                s.w[t][h] = __builtin_amdgcn_raw_buffer_load_b128(wr, from + w_at + (uint32_t)(t * tile_bytes) + h * 1024, 0, 2);  // nt
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int k = b * kScaleBlock + h * 64;
+            const bool in = some && k + 16 * quarter < a.k;
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+                s.x[i][h] = __builtin_amdgcn_raw_buffer_load_b128(xr, in ? x_at[i] + (uint32_t)k : kPastEnd, 0, 0);
+        }
+        const int at = min(b, a.blocks - 1);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) s.sx[i] = sx[i][(int64_t)at * a.scale_group];
+        s.sw = sw[at];
+    };
+    v4f acc[NT][MT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) acc[t][i] = v4f{0.f, 0.f, 0.f, 0.f};
+
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) load(st[d], wave + d * waves);
+    for (int b = wave; b < a.blocks; b += DEPTH * waves) {
+#pragma unroll
+        for (int d = 0; d < DEPTH; ++d) {
+            if (b + d * waves < a.blocks) {
+                Stage& s = st[d];
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                    const float scale = s.sx[i] * s.sw;
+                    const v8i xv = join(s.x[i][0], s.x[i][1]);
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) {
+                        const v4f p = block_product(join(s.w[t][0], s.w[t][1]), xv);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[t][i][e] = fmaf(scale, p[e], acc[t][i][e]);
+                    }
+                }
+                load(s, b + (d + DEPTH) * waves);
+            }
+        }
+    }
+
+    v4f* mine = reinterpret_cast<v4f*>(sums) + lane;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) mine[(wave * NT * MT + t * MT + i) * 64] = acc[t][i];
+    __syncthreads();
+    for (int p = wave; p < NT * MT; p += waves) {
+        v4f v = mine[p * 64];
+        for (int o = 1; o < waves; ++o) v += mine[(o * NT * MT + p) * 64];
+        const int t = p / MT, i = p % MT, m = m0 + 16 * i + row;
+        if (tile0 + t < w.tiles && m < a.m) store4(a, w, m, (tile0 + t) * 16 + quarter * 4, v);
+    }
+}
+
+// Values [n, k] of any row stride to tiles; rows past n and columns past k are 0.
+__global__ __launch_bounds__(256) void block_prepare_kernel(const uint8_t* values, int64_t ld, int64_t n, int k,
+                                                            int blocks, int64_t chunks, uint8_t* out) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < chunks; i += (int64_t)gridDim.x * 256) {
+        const int lane = i & 63, half = (i >> 6) & 1;
+        const int64_t at = i >> 7, tile = at / blocks;
+        const int64_t r = tile * 16 + (lane & 15);
+        const int c = (int)(at - tile * blocks) * kScaleBlock + half * 64 + (lane >> 4) * 16;
+        uint8_t v[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[e] = r < n && c + e < k ? values[r * ld + c + e] : 0;
+        uint32_t u[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            u[e] = v[4 * e] | (uint32_t)v[4 * e + 1] << 8 | (uint32_t)v[4 * e + 2] << 16 | (uint32_t)v[4 * e + 3] << 24;
+        *reinterpret_cast<uint4*>(out + i * 16) = make_uint4(u[0], u[1], u[2], u[3]);
+    }
+}
+
+template <int NT, int MT, int DEPTH>
+hipError_t launch_stream(const BlockGemmArgs& a, hipStream_t s) {
+    const dim3 grid(a.group_end[a.members - 1], (a.m + 16 * MT - 1) / (16 * MT));
+    block_stream_kernel<NT, MT, DEPTH><<<grid, a.waves * 64, a.waves * NT * MT * 1024, s>>>(a);
+    return hipGetLastError();
+}
+
+template <int NT>
+hipError_t launch_stream_rows(const BlockGemmArgs& a, hipStream_t s) {
+    switch (a.row_tiles) {
+        case 1: return launch_stream<NT, 1, 4>(a, s);
+        case 2: return launch_stream<NT, 2, 2>(a, s);
+        default: return launch_stream<NT, 4, 2>(a, s);
+    }
+}
+
+}  // namespace
+
+hipError_t launch_block_gemm(const BlockGemmArgs& a, hipStream_t s) {
+    switch (a.col_tiles) {
+        case 1: return launch_stream_rows<1>(a, s);
+        case 2: return launch_stream_rows<2>(a, s);
+        default: return launch_stream_rows<4>(a, s);
+    }
+}
+
+hipError_t launch_block_prepare(const uint8_t* values, int64_t ld, int64_t n, int64_t k, uint8_t* out, hipStream_t s) {
+    const int blocks = (int)((k + kScaleBlock - 1) / kScaleBlock);
+    const int64_t chunks = (n + 15) / 16 * blocks * 128, groups = (chunks + 255) / 256;
+    block_prepare_kernel<<<(unsigned)(groups < (1 << 20) ? groups : (1 << 20)), 256, 0, s>>>(values, ld, n, (int)k, blocks,
+                                                                                           chunks, out);
+    return hipGetLastError();
+}
+
+}  // namespace cubic

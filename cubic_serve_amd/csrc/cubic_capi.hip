@@ -791,6 +791,166 @@ int cubic_vocab_sample(const void* logits, int dtype, int64_t row_stride, int ro
 }
 
 // ---------------------------------------------------------------------------
+// Row norms and 8-bit activations
+// ---------------------------------------------------------------------------
+namespace {
+bool vectors(const void* p, int64_t ld, int64_t m, int element) {
+    return ((uintptr_t)p & (8 * element - 1)) == 0 && (m == 1 || ld % 8 == 0);
+}
+
+// Whether no two (row, group) scales lie at one place.
+bool scales_apart(int64_t m, int64_t groups, int64_t row, int64_t group) {
+    return (m == 1 || row >= 1) && (groups == 1 || group >= 1) && row <= ((int64_t)1 << 40) && group <= ((int64_t)1 << 40) &&
+           (m == 1 || groups == 1 || row > (groups - 1) * group || group / row >= m || group > (m - 1) * row);
+}
+
+int rows_common(cubic::RowArgs& a, int dtype, void* stream, const char* what) {
+    if (dtype != CUBIC_DTYPE_BF16 && dtype != CUBIC_DTYPE_F16) return fail(CUBIC_ENOTSUP, "%s: dtype=%d", what, dtype);
+    if (a.m < 1 || a.m > 0x7fffffff) return fail(CUBIC_EINVAL, "%s: m=%lld", what, (long long)a.m);
+    a.f16 = dtype == CUBIC_DTYPE_F16;
+    const int64_t least = a.k, most = (int64_t)1 << 40;
+    const void* base[] = {a.x, a.other, a.y, a.sum, a.q};
+    const int64_t ld[] = {a.ldx, a.ldother, a.ldy, a.ldsum, a.ldq};
+    int* const vec[] = {&a.vec_x, &a.vec_other, &a.vec_y, &a.vec_sum, &a.vec_q};
+    for (int i = 0; i < 5; ++i) {
+        if (!base[i]) continue;
+        const int element = i == 4 ? 1 : 2;
+        if (a.m > 1 && (ld[i] < least || ld[i] > most))
+            return fail(CUBIC_EINVAL, "%s: row stride %lld of %lld columns", what, (long long)ld[i], (long long)least);
+        if ((uintptr_t)base[i] % element) return fail(CUBIC_EINVAL, "%s: operand is not aligned to its element", what);
+        *vec[i] = vectors(base[i], ld[i], a.m, element);
+    }
+    if (a.q) {
+        if (!a.scales || (uintptr_t)a.scales % 4) return fail(CUBIC_EINVAL, "%s: 8-bit rows need aligned scales", what);
+        if (!scales_apart(a.m, ceil_div(a.k, cubic::kScaleBlock), a.scale_row, a.scale_group))
+            return fail(CUBIC_EINVAL, "%s: scale strides %lld, %lld overlap", what, (long long)a.scale_row, (long long)a.scale_group);
+    }
+    return hip_status(cubic::launch_rows(a, (hipStream_t)stream), what);
+}
+}  // namespace
+
+int cubic_row_norm(const void* x, int64_t ldx, const void* residual, int64_t ldresidual, const void* weight,
+                   int64_t m, int64_t k, int dtype, float epsilon, float weight_offset, void* y, int64_t ldy,
+                   void* sum, int64_t ldsum, void* q, int64_t ldq, float* scales, int64_t scale_row,
+                   int64_t scale_group, void* stream) {
+    if (!x || !weight || (!y && !q)) return fail(CUBIC_EINVAL, "row norm: null operand");
+    if (k < 1 || k > cubic::kMaxRowColumns) return fail(CUBIC_EINVAL, "row norm: k=%lld", (long long)k);
+    if (!(epsilon >= 0.0f && epsilon <= 1e30f) || !(weight_offset >= -1e30f && weight_offset <= 1e30f))
+        return fail(CUBIC_EINVAL, "row norm: epsilon must be finite and >= 0, the weights' offset finite");
+    if ((uintptr_t)weight % 2) return fail(CUBIC_EINVAL, "row norm: weights are not aligned to their element");
+    cubic::RowArgs a = {};
+    a.x = x;
+    a.other = residual;
+    a.weight = weight;
+    a.ldx = ldx;
+    a.ldother = ldresidual;
+    a.m = m;
+    a.k = (int)k;
+    a.norm = 1;
+    a.epsilon = epsilon;
+    a.offset = weight_offset;
+    a.y = y;
+    a.ldy = ldy;
+    a.sum = sum;
+    a.ldsum = ldsum;
+    a.q = (uint8_t*)q;
+    a.ldq = ldq;
+    a.scales = scales;
+    a.scale_row = scale_row;
+    a.scale_group = scale_group;
+    a.vec_weight = ((uintptr_t)weight & 15) == 0;
+    return rows_common(a, dtype, stream, "row norm");
+}
+
+int cubic_quantize_rows(const void* x, int64_t ldx, const void* gate, int64_t ldgate, int64_t m, int64_t k,
+                        int dtype, void* q, int64_t ldq, float* scales, int64_t scale_row, int64_t scale_group,
+                        void* stream) {
+    if (!x || !q) return fail(CUBIC_EINVAL, "quantize rows: null operand");
+    if (k < 1 || k > cubic::kMaxRowColumns) return fail(CUBIC_EINVAL, "quantize rows: k=%lld", (long long)k);
+    cubic::RowArgs a = {};
+    a.x = x;
+    a.other = gate;
+    a.ldx = ldx;
+    a.ldother = ldgate;
+    a.m = m;
+    a.k = (int)k;
+    a.q = (uint8_t*)q;
+    a.ldq = ldq;
+    a.scales = scales;
+    a.scale_row = scale_row;
+    a.scale_group = scale_group;
+    return rows_common(a, dtype, stream, "quantize rows");
+}
+
+// ---------------------------------------------------------------------------
+// Block-scaled 8-bit products
+// ---------------------------------------------------------------------------
+int64_t cubic_block_prepared_bytes(int64_t n, int64_t k) {
+    if (n < 1 || n > (1 << 24) || k < 1 || k > (1 << 20)) return -1;
+    return ceil_div(n, 16) * 16 * ceil_div(k, cubic::kScaleBlock) * cubic::kScaleBlock;
+}
+
+int cubic_block_prepare(const void* values, int64_t ld, int64_t n, int64_t k, void* prepared, void* stream) {
+    if (!values || !prepared) return fail(CUBIC_EINVAL, "block prepare: null operand");
+    if (cubic_block_prepared_bytes(n, k) < 0 || (n > 1 && ld < k) || ld > ((int64_t)1 << 40))
+        return fail(CUBIC_EINVAL, "block prepare: n=%lld k=%lld row stride %lld", (long long)n, (long long)k, (long long)ld);
+    if (!aligned16(prepared)) return fail(CUBIC_EINVAL, "block prepare: the layout needs 16-byte alignment");
+    return hip_status(cubic::launch_block_prepare((const uint8_t*)values, ld, n, k, (uint8_t*)prepared, (hipStream_t)stream),
+                      "block prepare");
+}
+
+int cubic_block_gemm(const void* x, int64_t ldx, const float* x_scales, int64_t scale_row, int64_t scale_group,
+                     int64_t m, int64_t k, int members, const int64_t* ns, const void* const* prepared,
+                     const float* const* scales, void* const* ys, const int64_t* ldys, int out_dtype, void* stream) {
+    if (!x || !x_scales || !ns || !prepared || !scales || !ys || !ldys) return fail(CUBIC_EINVAL, "block gemm: null operand");
+    if (members < 1 || members > cubic::kMaxGemmMembers)
+        return fail(CUBIC_EINVAL, "members=%d outside 1..%d", members, cubic::kMaxGemmMembers);
+    if (out_dtype != CUBIC_DTYPE_BF16 && out_dtype != CUBIC_DTYPE_F16 && out_dtype != CUBIC_DTYPE_F32)
+        return fail(CUBIC_ENOTSUP, "block gemm: dtype=%d", out_dtype);
+    if (m < 1 || m >= (1 << 21) || k < 1 || k > (1 << 20))
+        return fail(CUBIC_EINVAL, "block gemm extents: m=%lld k=%lld", (long long)m, (long long)k);
+    if (m == 1) ldx = k;
+    if (k % 16 || ldx % 16 || ldx < k || ldx > (1 << 23) || !aligned16(x))
+        return fail(CUBIC_ENOTSUP, "8-bit activations need k %% 16 == 0, a row stride of whole 16 bytes in k..2^23 and 16-byte alignment");
+    if ((uintptr_t)x_scales % 4 || (m > 1 && (scale_row < 1 || scale_row > ((int64_t)1 << 40))) ||
+        (k > cubic::kScaleBlock && (scale_group < 1 || scale_group > ((int64_t)1 << 40))))
+        return fail(CUBIC_EINVAL, "block gemm: scale strides %lld, %lld", (long long)scale_row, (long long)scale_group);
+    cubic::BlockGemmArgs a = {};
+    a.x = (const uint8_t*)x;
+    a.x_scales = x_scales;
+    a.ldx = ldx;
+    a.scale_row = scale_row;
+    a.scale_group = scale_group;
+    a.m = (int)m;
+    a.k = (int)k;
+    a.blocks = (int)ceil_div(k, cubic::kScaleBlock);
+    a.members = members;
+    a.out = out_dtype;
+    const int element = out_dtype == CUBIC_DTYPE_F32 ? 4 : 2;
+    int64_t tiles = 0;
+    for (int j = 0; j < members; ++j) {
+        if (!prepared[j] || !scales[j] || !ys[j]) return fail(CUBIC_EINVAL, "block gemm: null operand of member %d", j);
+        if (ns[j] < 1 || ns[j] > (1 << 24)) return fail(CUBIC_EINVAL, "block gemm: width %lld of member %d", (long long)ns[j], j);
+        if (m > 1 && (ldys[j] < ns[j] || ldys[j] > ((int64_t)1 << 40)))
+            return fail(CUBIC_EINVAL, "output leading dimension too small");
+        if (!aligned16(prepared[j]) || (uintptr_t)scales[j] % 4 || (uintptr_t)ys[j] % element)
+            return fail(CUBIC_EINVAL, "block gemm: misaligned operand of member %d", j);
+        a.member[j] = {(const uint8_t*)prepared[j], scales[j], ys[j], ldys[j], (int)ns[j], (int)ceil_div(ns[j], 16),
+                       ((uintptr_t)ys[j] & (4 * element - 1)) == 0 && (m == 1 || ldys[j] % 4 == 0)};
+        tiles += a.member[j].tiles;
+    }
+    a.row_tiles = m <= 16 ? 1 : m <= 32 ? 2 : 4;
+    a.col_tiles = tiles >= 2048 ? 4 : tiles >= 1024 ? 2 : 1;
+    a.waves = a.col_tiles * a.row_tiles >= 16 ? 4 : 8;
+    int64_t groups = 0;
+    for (int j = 0; j < cubic::kMaxGemmMembers; ++j) {
+        if (j < members) groups += ceil_div(a.member[j].tiles, a.col_tiles);
+        a.group_end[j] = (int)groups;
+    }
+    return hip_status(cubic::launch_block_gemm(a, (hipStream_t)stream), "block gemm launch");
+}
+
+// ---------------------------------------------------------------------------
 // Low-rank adapters
 // ---------------------------------------------------------------------------
 int64_t cubic_adapters_workspace_bytes(int64_t m, int64_t k, int members, const int* max_ranks) {

@@ -317,6 +317,47 @@ struct AdapterArgs {
     AdapterMember member[kMaxGemmMembers];
 };
 
+// Row norms and 8-bit activations (cubic_rows.hip)
+constexpr int kScaleBlock = 128;      // columns (and rows of a weight) that share a scale
+constexpr int kMaxRowColumns = 1 << 24;
+struct RowArgs {
+    const void* x;                // [m, k] bf16 or fp16 (f16)
+    const void* other;            // norm: added to x; quantise: its gate; or null
+    const void* weight;           // norm: [k]
+    int64_t ldx, ldother;
+    int64_t m;
+    int k, f16, norm;
+    float epsilon, offset;
+    void* y;                      // [m, k] in 16 bits, or null
+    void* sum;                    // norm: x + other in 16 bits, or null
+    uint8_t* q;                   // [m, k] e4m3, or null
+    float* scales;                // of group g of row r at r * scale_row + g * scale_group
+    int64_t ldy, ldsum, ldq, scale_row, scale_group;
+    int vec_x, vec_other, vec_weight, vec_y, vec_sum, vec_q;  // whole vectors of eight may be accessed at once
+};
+hipError_t launch_rows(const RowArgs& a, hipStream_t s);
+
+// Block-scaled 8-bit products (cubic_block.hip)
+struct BlockMember {
+    const uint8_t* codes;         // tiles of 16 rows, laid out by launch_block_prepare
+    const float* scales;          // [ceil(n / 128), blocks]
+    void* y;                      // [m, n], row stride ldy
+    int64_t ldy;
+    int n, tiles;
+    int vec;                      // four columns may be stored at once
+};
+struct BlockGemmArgs {
+    const uint8_t* x;             // [m, k] e4m3, row stride ldx
+    const float* x_scales;        // of block b of row r at r * scale_row + b * scale_group
+    int64_t ldx, scale_row, scale_group;
+    int m, k, blocks, members;
+    int out;                      // CUBIC_DTYPE_* of y
+    int col_tiles, row_tiles, waves;  // per workgroup
+    int group_end[kMaxGemmMembers];   // ends of the members' column groups
+    BlockMember member[kMaxGemmMembers];
+};
+hipError_t launch_block_gemm(const BlockGemmArgs& a, hipStream_t s);
+hipError_t launch_block_prepare(const uint8_t* values, int64_t ld, int64_t n, int64_t k, uint8_t* out, hipStream_t s);
 hipError_t launch_adapters(const AdapterArgs& a, hipStream_t s);
 hipError_t launch_accept(const AcceptArgs& a, bool fused, hipStream_t s);
 hipError_t launch_greedy(const GreedyArgs& a, hipStream_t s);

@@ -1,0 +1,240 @@
+// Row norms and 8-bit activations for gfx950.
+//
+//   norm      h = x + r,  y = h * (offset + w) / sqrt(mean(h^2) + eps)
+//   quantise  y = x,  or  y = silu(g) x = g x / (1 + exp(-g))
+//
+// y leaves in 16 bits, and / or per group of 128 columns as a 32-bit scale
+// s = max(max |y|, 2^-96) / 448 and values q = e4m3(y * (448 / max(max |y|, 2^-96))),
+// so that q s stands for y (448: the largest e4m3 value; below 2^-96 the scale's
+// reciprocal would leave the normal numbers).  h leaves in 16 bits too.  All is
+// held in 32 bits and each output rounded once: y is computed from h as added, not
+// from the rounded one.  A NaN or an infinity makes all of its group NaN.
+//
+// What bounds it: the bytes of the rows.  A row is read once, its columns stay in
+// registers, eight to a vector, between the sum of squares and the outputs.  A
+// group of 128 columns is the vectors of 16 lanes, one DPP row: its maximum
+// takes four lane exchanges and no LDS.
+#include "cubic_capi_internal.h"
+#include "cubic_device.h"
+
+namespace cubic {
+namespace {
+
+constexpr int kVec = 8;          // columns of a thread's vector
+constexpr float kTop = 448.0f;   // largest e4m3 value
+constexpr float kSmallest = 0x1p-96f;
+
+template <bool F16>
+__device__ __forceinline__ float from_bits(uint32_t b) {
+    return F16 ? half_bits_to_float(b) : bf16_bits_to_float(b);
+}
+template <bool F16>
+__device__ __forceinline__ uint32_t to_bits(float f) {
+    return F16 ? float_to_f16_bits(f) : float_to_bf16_bits(f);
+}
+
+// Columns c..c+7 of a row; the ones past k read as zero.
+template <bool F16>
+__device__ __forceinline__ void load8(const uint16_t* row, int c, int k, bool vec, float (&v)[kVec]) {
+    if (vec && c + kVec <= k) {
+        const uint4 w = *reinterpret_cast<const uint4*>(row + c);
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] = from_bits<F16>(u[i] & 0xFFFFu);
+            v[2 * i + 1] = from_bits<F16>(u[i] >> 16);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) v[i] = c + i < k ? from_bits<F16>(row[c + i]) : 0.0f;
+    }
+}
+
+template <bool F16>
+__device__ __forceinline__ void store8(uint16_t* row, int c, int k, bool vec, const float (&v)[kVec]) {
+    if (vec && c + kVec <= k) {
+        uint32_t u[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            u[i] = F16 ? to_bits<F16>(v[2 * i]) | to_bits<F16>(v[2 * i + 1]) << 16 : pack_bf16x2(v[2 * i], v[2 * i + 1]);
+        *reinterpret_cast<uint4*>(row + c) = make_uint4(u[0], u[1], u[2], u[3]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < kVec; ++i)
+            if (c + i < k) row[c + i] = (uint16_t)to_bits<F16>(v[i]);
+    }
+}
+
+// exp(-g) in binary32: 2^t with t = -g log2(e) in two parts, so that the error does
+// not grow with |g|.
+__device__ __forceinline__ float exp_minus(float g) {
+    constexpr float kHi = 1.44269502162933349609375f, kLo = 1.92596299112661746887e-8f;  // log2(e)
+    const float t = -g * kHi;
+    const float rest = fmaf(-g, kHi, -t) + -g * kLo;
+    const float e = __builtin_amdgcn_exp2f(t);
+    const float whole = fmaf(e, rest * 0.693147182464599609375f, e);
+    return e < __builtin_huge_valf() ? whole : e;
+}
+
+__device__ __forceinline__ float silu(float g) { return g * __builtin_amdgcn_rcpf(1.0f + exp_minus(g)); }
+
+// Quantises the eight columns of every lane; the 16 lanes of a DPP row hold a
+// group.  Every lane of the wave calls it.
+__device__ __forceinline__ void quantise8(const RowArgs& a, int64_t row, int c, const float (&y)[kVec]) {
+    uint32_t most = 0;  // of the magnitudes' bits: a NaN is above an infinity
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) most = max(most, __float_as_uint(y[i]) & 0x7FFFFFFFu);
+    most = max(most, dpp_u32<0xB1>(most));
+    most = max(most, dpp_u32<0x4E>(most));
+    most = max(most, dpp_u32<0x141>(most));
+    most = max(most, dpp_u32<0x140>(most));
+    if (c >= a.k) return;
+    const float top = __uint_as_float(max(most, __float_as_uint(kSmallest)));
+    const float inverse = kTop / top;
+    if ((threadIdx.x & 15) == 0) a.scales[row * a.scale_row + (int64_t)(c >> 7) * a.scale_group] = top / kTop;
+    uint32_t lo = 0, hi = 0;
+    lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[0] * inverse, y[1] * inverse, lo, false);
+    lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[2] * inverse, y[3] * inverse, lo, true);
+    hi = __builtin_amdgcn_cvt_pk_fp8_f32(y[4] * inverse, y[5] * inverse, hi, false);
+    hi = __builtin_amdgcn_cvt_pk_fp8_f32(y[6] * inverse, y[7] * inverse, hi, true);
+    uint8_t* q = a.q + row * a.ldq + c;
+    if (a.vec_q && c + kVec <= a.k) {
+        *reinterpret_cast<uint2*>(q) = make_uint2(lo, hi);
+    } else {
+#pragma unroll
+        for (int i = 0; i < kVec; ++i)
+            if (c + i < a.k) q[i] = (uint8_t)((i < 4 ? lo : hi) >> (8 * (i & 3)));
+    }
+}
+
+// The sum over a workgroup's threads, in a fixed order; `sums` is reused by the
+// next row after a barrier.
+template <bool WAVE>
+__device__ __forceinline__ float row_sum(float part, float* sums) {
+    part = wave_butterfly_sum(part, 64);
+    if constexpr (WAVE) return part;
+    const int waves = blockDim.x >> 6;
+    if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = part;
+    __syncthreads();
+    const int of = threadIdx.x & 15;  // every 16 lanes add all waves' sums
+    return wave_butterfly_sum(of < waves ? sums[of] : 0.0f, 16);
+}
+
+// One row per workgroup, or per wave (WAVE: blockDim.x == 64, four rows to a
+// workgroup); NV vectors per thread cover it.  NV = 0: any length, the row is read
+// again (from the caches) for the outputs.
+template <bool F16, int NV, bool WAVE>
+__global__ __launch_bounds__(1024) void row_norm_kernel(RowArgs a) {
+    __shared__ float sums[16];
+    constexpr int N = NV ? NV : 1;
+    const int turns = (a.k + blockDim.x * kVec - 1) / (blockDim.x * kVec);
+    const uint16_t* x = static_cast<const uint16_t*>(a.x);
+    const uint16_t* other = static_cast<const uint16_t*>(a.other);
+    const uint16_t* weight = static_cast<const uint16_t*>(a.weight);
+    for (int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y; row < a.m; row += (int64_t)gridDim.x * blockDim.y) {
+        float v[N][kVec];
+        auto read = [&](int i, float (&h)[kVec]) {
+            const int c = (i * blockDim.x + threadIdx.x) * kVec;
+            load8<F16>(x + row * a.ldx, c, a.k, a.vec_x, h);
+            if (other) {
+                float o[kVec];
+                load8<F16>(other + row * a.ldother, c, a.k, a.vec_other, o);
+#pragma unroll
+                for (int e = 0; e < kVec; ++e) h[e] += o[e];
+            }
+        };
+        auto write = [&](int i, float factor, float (&h)[kVec]) {
+            const int c = (i * blockDim.x + threadIdx.x) * kVec;
+            if (a.sum) store8<F16>(static_cast<uint16_t*>(a.sum) + row * a.ldsum, c, a.k, a.vec_sum, h);
+            float w[kVec];
+            load8<F16>(weight, c, a.k, a.vec_weight, w);
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) h[e] = h[e] * factor * (a.offset + w[e]);
+            if (a.y) store8<F16>(static_cast<uint16_t*>(a.y) + row * a.ldy, c, a.k, a.vec_y, h);
+            if (a.q) quantise8(a, row, c, h);
+        };
+        float part = 0.0f;
+        for (int i = 0; i < (NV ? 0 : turns); ++i) {
+            read(i, v[0]);
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) part = fmaf(v[0][e], v[0][e], part);
+        }
+        if constexpr (NV != 0) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) read(i, v[i]);
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+#pragma unroll
+                for (int e = 0; e < kVec; ++e) part = fmaf(v[i][e], v[i][e], part);
+        }
+        const float sum = row_sum<WAVE>(part, sums);
+        const float factor = 1.0f / sqrtf(sum / (float)a.k + a.epsilon);
+        if constexpr (NV != 0) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) write(i, factor, v[i]);
+        } else {
+            for (int i = 0; i < turns; ++i) {
+                read(i, v[0]);
+                write(i, factor, v[0]);
+            }
+        }
+        if constexpr (!WAVE) __syncthreads();  // the sums are read
+    }
+}
+
+// 2048 columns per workgroup and turn: blockDim.x vectors of blockDim.y rows.
+// blockDim.x is a multiple of 16, so a group's lanes are one DPP row.
+template <bool F16, bool GATED>
+__global__ __launch_bounds__(256) void quantize_kernel(RowArgs a) {
+    const int c = (blockIdx.y * blockDim.x + threadIdx.x) * kVec;
+    for (int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y; row < a.m; row += (int64_t)gridDim.x * blockDim.y) {
+        float y[kVec];
+        load8<F16>(static_cast<const uint16_t*>(a.x) + row * a.ldx, c, a.k, a.vec_x, y);
+        if constexpr (GATED) {
+            float g[kVec];
+            load8<F16>(static_cast<const uint16_t*>(a.other) + row * a.ldother, c, a.k, a.vec_other, g);
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) y[e] = silu(g[e]) * y[e];
+        }
+        quantise8(a, row, c, y);
+    }
+}
+
+template <bool F16>
+hipError_t launch_norm(const RowArgs& a, hipStream_t s) {
+    const int vectors = (a.k + kVec - 1) / kVec;
+    const int64_t most = 1 << 18;  // workgroups; the rest of the rows in turns
+    if (vectors <= 128) {
+        const dim3 block(64, 4), grid((unsigned)((a.m + 3) / 4 < most ? (a.m + 3) / 4 : most));
+        if (vectors <= 64) row_norm_kernel<F16, 1, true><<<grid, block, 0, s>>>(a);
+        else row_norm_kernel<F16, 2, true><<<grid, block, 0, s>>>(a);
+        return hipGetLastError();
+    }
+    const dim3 grid((unsigned)(a.m < most ? a.m : most));
+    auto threads = [&](int nv) { return (unsigned)((vectors + nv * 64 - 1) / (nv * 64) * 64); };
+    if (vectors <= 512 || (vectors <= 1024 && a.m <= 512)) row_norm_kernel<F16, 1, false><<<grid, threads(1), 0, s>>>(a);
+    else if (vectors <= 2048) row_norm_kernel<F16, 2, false><<<grid, threads(2), 0, s>>>(a);
+    else if (vectors <= 4096) row_norm_kernel<F16, 4, false><<<grid, threads(4), 0, s>>>(a);
+    else row_norm_kernel<F16, 0, false><<<grid, 1024, 0, s>>>(a);
+    return hipGetLastError();
+}
+
+template <bool F16>
+hipError_t launch_quantize(const RowArgs& a, hipStream_t s) {
+    const int vectors = (a.k + kVec - 1) / kVec, wide = (vectors + 15) / 16 * 16;
+    const unsigned across = wide < 256 ? wide : 256, down = 256 / across;
+    const int64_t rows = (a.m + down - 1) / down, most = 1 << 16;
+    const dim3 block(across, down), grid((unsigned)(rows < most ? rows : most), (vectors + across - 1) / across);
+    if (a.other) quantize_kernel<F16, true><<<grid, block, 0, s>>>(a);
+    else quantize_kernel<F16, false><<<grid, block, 0, s>>>(a);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_rows(const RowArgs& a, hipStream_t s) {
+    if (a.norm) return a.f16 ? launch_norm<true>(a, s) : launch_norm<false>(a, s);
+    return a.f16 ? launch_quantize<true>(a, s) : launch_quantize<false>(a, s);
+}
+
+}  // namespace cubic

@@ -62,8 +62,12 @@ DTYPE_IDS = {torch.bfloat16: 0, torch.float16: 1}  # CUBIC_DTYPE_BF16 / CUBIC_DT
 
 
 def _versions(matrix: QuantizedMatrix) -> tuple:
+    return tensor_versions(matrix.payload.values())
+
+
+def tensor_versions(tensors) -> tuple:
     versions = []
-    for tensor in matrix.payload.values():
+    for tensor in tensors:
         try:
             versions.append(tensor._version)
         except RuntimeError:  # inference-mode tensors
@@ -178,12 +182,14 @@ class PackedOperatorBinding:
     """Startup-bound native launches with owned scratch (binding.py:134-265)."""
 
     def __init__(self, output: Tensor | tuple[Tensor, ...], launches: tuple, *,
-                 scratch: tuple[Tensor, ...] = (), row_tile_count: int | None = None):
+                 scratch: tuple[Tensor, ...] = (), row_tile_count: int | None = None,
+                 device: torch.device | None = None):
         if row_tile_count is not None and (type(row_tile_count) is not int or row_tile_count < 1):
             raise ValueError("row tile count must be a positive integer")
         self.output = output
         self.scratch = scratch
         self.row_tile_count = row_tile_count
+        self._device = device  # of the launches; None: the first output's
         self._launches = launches
         self._ordinal = 0
 
@@ -196,7 +202,7 @@ class PackedOperatorBinding:
         self.validate_operands()
         self._ordinal += 1
         first = self.output[0] if isinstance(self.output, tuple) else self.output
-        index = first.device.index
+        index = (self._device or first.device).index
         with _native.on_device(index):
             stream = _native.stream_of(index)
             for item in self._launches:
@@ -349,6 +355,16 @@ class PackedLinearOperators:
         self.prepared_weights[key] = (weights, prepared)
         return prepared
 
+    def prepared_block(self, weight, device: torch.device) -> tuple[Tensor, Tensor]:
+        """A BlockScaledMatrix as its products read it: (values laid out, scales)."""
+        from . import blockscale
+
+        key = ("block.mi355x.v1", id(weight), tensor_versions((weight.values, weight.scales)), str(device))
+        cached = self.prepared_weights.get(key)
+        if cached is None:  # the weight is kept, so its id cannot be reused while cached
+            cached = self.prepared_weights[key] = (weight, blockscale.prepare_block_matrix(weight, device))
+        return cached[1]
+
     # -- validation (quantized.py:348-405) ------------------------------------
     @staticmethod
     def _validate(x: Tensor, weight: QuantizedMatrix, output: Tensor) -> None:
@@ -424,6 +440,32 @@ class PackedLinearOperators:
         added = self.bind_adapters(x, banks, row_slots, outputs)
         return PackedOperatorBinding(shared.output, (*shared._launches, *added._launches),
                                      scratch=(*shared.scratch, *added.scratch))
+
+    def bind_norm(self, x: Tensor, weight: Tensor, *, epsilon: float, weight_offset: float = 0.0,
+                  residual: Tensor | None = None, residual_output: Tensor | None = None,
+                  output: Tensor | None = None, quantized=None) -> PackedOperatorBinding:
+        """Root-mean-square norm of rows, with the residual's addition, to 16 and /
+        or 8 bits (blockscale.bind_norm)."""
+        from . import blockscale
+
+        return blockscale.bind_norm(x, weight, epsilon=epsilon, weight_offset=weight_offset, residual=residual,
+                                    residual_output=residual_output, output=output, quantized=quantized)
+
+    def bind_quantize(self, x: Tensor, quantized, *, gate: Tensor | None = None) -> PackedOperatorBinding:
+        """Activations, or silu(gate) * x, to 8 bits (blockscale.bind_quantize)."""
+        from . import blockscale
+
+        return blockscale.bind_quantize(x, quantized, gate=gate)
+
+    def bind_block_linear(self, x, weight, output: Tensor) -> PackedOperatorBinding:
+        """Product of 8-bit activations and a block-scaled weight (blockscale)."""
+        return self.bind_block_linear_group(x, (weight,), (output,))
+
+    def bind_block_linear_group(self, x, weights, outputs: Sequence[Tensor]) -> PackedOperatorBinding:
+        """The same for weights that share x, in one launch."""
+        from . import blockscale
+
+        return blockscale.bind_block_linear_group(self, x, weights, outputs)
 
     def embedding(self, input_ids: Tensor, weight: QuantizedMatrix, *, dtype: torch.dtype) -> Tensor:
         """Eager lookup (quantized.py:776-784)."""

@@ -392,6 +392,60 @@ CUBIC_API int cubic_embedding(const void* ids, int id_bytes, int64_t tokens, int
                               int group_in, int group_out, void* out, int out_dtype, void* stream);
 
 /* ---------------------------------------------------------------------------
+ * Row norms and 8-bit activations.  No counterpart in the reference's subset
+ * that this library replaces.
+ *
+ * cubic_row_norm: h = x + residual (residual NULL: h = x), per row
+ *   y = h * (weight_offset + weight) / sqrt(mean(h^2) + epsilon)
+ *   y     NULL or [m, k] in the inputs' 16-bit dtype
+ *   sum   NULL or h in that dtype; may be the residual or x itself (same
+ *         address and row stride), as y may be x or the residual
+ *   q     NULL or [m, k] e4m3 with `scales`; y or q is given
+ * cubic_quantize_rows: y = x, or silu(gate) * x, to q and scales.
+ * Per group of 128 columns (the last one may be shorter), in 32 bits:
+ *   top = max(max |y|, 2^-96), scale = top / 448, q = e4m3(y * (448 / top))
+ * The scale of group g of row r is at scales[r * scale_row + g * scale_group].
+ * y is computed from h before its rounding.  A group that holds a NaN or an
+ * infinity stands for NaNs.  Row strides in elements, at least k (any, for a
+ * single row); every alignment to an element is taken, whole 16-byte (q: 8-byte)
+ * rows are faster.  1 <= k <= 2^24; no workspace.
+ * ------------------------------------------------------------------------- */
+CUBIC_API int cubic_row_norm(const void* x, int64_t ldx, const void* residual, int64_t ldresidual,
+                             const void* weight, int64_t m, int64_t k, int dtype, float epsilon,
+                             float weight_offset, void* y, int64_t ldy, void* sum, int64_t ldsum,
+                             void* q, int64_t ldq, float* scales, int64_t scale_row,
+                             int64_t scale_group, void* stream);
+CUBIC_API int cubic_quantize_rows(const void* x, int64_t ldx, const void* gate, int64_t ldgate,
+                                  int64_t m, int64_t k, int dtype, void* q, int64_t ldq,
+                                  float* scales, int64_t scale_row, int64_t scale_group,
+                                  void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Block-scaled 8-bit products.  No counterpart in the reference's subset that
+ * this library replaces.
+ *   y_j[m, n] = sum_b sx[m, b] sw_j[n / 128, b] sum_{k in block b} x[m, k] w_j[n, k]
+ * for up to 8 members that share x, b over blocks of 128 columns (the last one
+ * may be shorter).
+ *   x        e4m3 [m, k], its scales at x_scales[r * scale_row + b * scale_group]
+ *   prepared w_j's e4m3 values [n_j, k] as cubic_block_prepare lays them out, once
+ *            (cubic_block_prepared_bytes(n_j, k) bytes, 16-byte aligned)
+ *   scales   f32 [ceil(n_j / 128), ceil(k / 128)] contiguous
+ *   ys       [m, n_j] of out_dtype CUBIC_DTYPE_BF16, _F16 or _F32, rounded once
+ * Host arrays ns, prepared, scales, ys, ldys have one entry per member and are
+ * read during the call.  k % 16 == 0, x 16-byte aligned with a row stride of whole
+ * 16 bytes up to 2^23, m < 2^21.  NaN values and scales propagate.  Sums are in 32
+ * bits; their order depends on the sizes only, no workspace.
+ * ------------------------------------------------------------------------- */
+CUBIC_API int64_t cubic_block_prepared_bytes(int64_t n, int64_t k);
+CUBIC_API int cubic_block_prepare(const void* values, int64_t ld, int64_t n, int64_t k,
+                                  void* prepared, void* stream);
+CUBIC_API int cubic_block_gemm(const void* x, int64_t ldx, const float* x_scales, int64_t scale_row,
+                               int64_t scale_group, int64_t m, int64_t k, int members,
+                               const int64_t* ns, const void* const* prepared,
+                               const float* const* scales, void* const* ys, const int64_t* ldys,
+                               int out_dtype, void* stream);
+
+/* ---------------------------------------------------------------------------
  * MoE router: per row, the top_k experts by (logit desc, expert id asc), then
  * a softmax over the selected logits, re-ordered by ascending expert id.
  * Replaces the routing launches of PackedRoutedExpertsPrimitive

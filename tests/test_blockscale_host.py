@@ -1,0 +1,124 @@
+"""CPU: block-scaled types, quantisation of weights, and what the C entries refuse
+before anything is launched."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from cubic_serve_amd import _native, blockscale, linear
+
+E4M3 = blockscale.E4M3
+
+
+@pytest.mark.parametrize("n,k", [(1, 1), (128, 128), (130, 257), (4100, 300)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_quantized_matrix_is_within_half_a_step(n, k, dtype):
+    w = (torch.randn((n, k), generator=torch.Generator().manual_seed(1)) * 0.1).to(dtype)
+    w[:, 0] = 0
+    m = blockscale.quantize_block_scaled(w)
+    assert m.shape == (n, k) and m.scales.shape == ((n + 127) // 128, (k + 127) // 128)
+    scale = m.scales.double().repeat_interleave(128, 0)[:n].repeat_interleave(128, 1)[:, :k]
+    v = w.double() / scale
+    # half a step of e4m3, and three roundings in 32 bits (top / 448, 448 / top, their product)
+    bound = torch.maximum(v.abs() * 2.0 ** -4, torch.full_like(v, 2.0 ** -10)) + v.abs() * 2.0 ** -21
+    assert ((m.values.double() - v).abs() <= bound).all()
+    assert torch.equal(m.dequantize(), m.values.float() * scale.float())
+
+
+def test_quantized_matrix_of_zeros():
+    m = blockscale.quantize_block_scaled(torch.zeros((130, 130)))
+    assert not m.values.float().any() and torch.isfinite(m.scales).all() and (m.scales > 0).all()
+
+
+def test_types_check_their_tensors():
+    v, s = torch.zeros((4, 256), dtype=E4M3), torch.ones((4, 2))
+    q = blockscale.BlockScaledActivations(v, s)
+    assert torch.equal(q.dequantize(), torch.zeros((4, 256)))
+    blockscale.BlockScaledActivations(v, torch.ones((2, 4)).t())
+    for values, scales in ((v.float(), s), (v, s.double()), (v, s[:, :1]), (v, s[:1].expand(4, 2)), (v.t(), s), (v[0], s)):
+        with pytest.raises(ValueError):
+            blockscale.BlockScaledActivations(values, scales)
+    blockscale.BlockScaledMatrix(v, torch.ones((1, 2)))
+    for values, scales in ((v, s), (v, torch.ones((1, 2)).double()), (v.float(), torch.ones((1, 2))),
+                           (v, torch.ones((2, 1)).expand(2, 2)[:1].t())):
+        with pytest.raises(ValueError):
+            blockscale.BlockScaledMatrix(values, scales)
+    with pytest.raises(TypeError):
+        blockscale.BlockScaledActivations(v, None)
+    for m, k in ((0, 4), (4, 0), (2.0, 4)):
+        with pytest.raises(ValueError):
+            blockscale.BlockScaledActivations.empty(m, k, "cpu")
+    e = blockscale.BlockScaledActivations.empty(3, 130, "cpu")
+    assert e.values.shape == (3, 130) and e.values.stride(0) == 144 and e.scales.stride() == (1, 3)
+    for bad in (torch.zeros(4), torch.zeros((0, 4)), torch.zeros((2, 2), dtype=torch.int32)):
+        with pytest.raises(ValueError):
+            blockscale.quantize_block_scaled(bad)
+
+
+def test_bindings_need_a_gpu():
+    ops = linear.PackedLinearOperators()
+    x, w = torch.zeros((2, 64), dtype=torch.bfloat16), torch.ones(64, dtype=torch.bfloat16)
+    q = blockscale.BlockScaledActivations.empty(2, 64, "cpu")
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.bind_norm(x, w, epsilon=1e-6, output=x)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.bind_quantize(x, q)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.bind_block_linear(q, blockscale.BlockScaledMatrix(torch.zeros((4, 64), dtype=E4M3), torch.ones((1, 1))), x)
+
+
+def norm(**change):
+    a = dict(x=16, ldx=64, r=None, ldr=0, w=16, m=2, k=64, dtype=0, eps=1e-6, off=0.0, y=16, ldy=64, s=None, lds=0,
+             q=None, ldq=0, sc=None, row=0, group=0, stream=None) | change
+    return _native.call("cubic_row_norm", *a.values())
+
+
+@pytest.mark.parametrize("change,match", [
+    (dict(x=None), "null"), (dict(w=None), "null"), (dict(y=None), "null"), (dict(k=0), "k="), (dict(k=(1 << 24) + 1), "k="),
+    (dict(m=0), "m="), (dict(m=1 << 31), "m="), (dict(dtype=2), "dtype"), (dict(ldx=63), "row stride"), (dict(ldy=63), "row stride"),
+    (dict(r=16, ldr=63), "row stride"), (dict(eps=-1.0), "epsilon"), (dict(eps=float("nan")), "epsilon"),
+    (dict(off=float("inf")), "epsilon"), (dict(x=17), "aligned"), (dict(w=17), "aligned"), (dict(q=16, ldq=64), "scales"),
+    (dict(q=16, ldq=64, sc=18, row=1, group=2), "scales"), (dict(q=16, ldq=64, sc=16, row=0, group=1), "overlap"),
+    (dict(q=16, ldq=256, sc=16, row=1, group=1, k=256, ldx=256, ldy=256), "overlap")])
+def test_norm_entry_refuses(change, match):
+    with pytest.raises(ValueError, match=match):
+        norm(**change)
+
+
+@pytest.mark.parametrize("change,match", [
+    (dict(q=None), "null"), (dict(x=None), "null"), (dict(k=0), "k="), (dict(m=0), "m="), (dict(ldg=3, g=16), "row stride"),
+    (dict(ldq=63), "row stride"), (dict(dtype=7), "dtype"), (dict(sc=None), "scales")])
+def test_quantize_entry_refuses(change, match):
+    a = dict(x=16, ldx=64, g=None, ldg=0, m=2, k=64, dtype=0, q=16, ldq=64, sc=16, row=1, group=2, stream=None) | change
+    with pytest.raises(ValueError, match=match):
+        _native.call("cubic_quantize_rows", *a.values())
+
+
+@pytest.mark.parametrize("change,match", [
+    (dict(x=None), "null"), (dict(sx=None), "null"), (dict(members=0), "members"), (dict(members=9), "members"), (dict(out=3), "dtype"),
+    (dict(m=0), "extents"), (dict(m=1 << 21), "extents"), (dict(k=0), "extents"), (dict(k=1 << 21), "extents"),
+    (dict(k=72), "k % 16"), (dict(ldx=120), "row stride"), (dict(ldx=1 << 24), "row stride"), (dict(x=24), "alignment"),
+    (dict(row=0), "scale strides"), (dict(k=256, ldx=256, group=0), "scale strides"), (dict(n=0), "width"), (dict(n=(1 << 24) + 1), "width"),
+    (dict(w=24), "misaligned"), (dict(w=None), "null operand of"), (dict(y=None), "null operand of"), (dict(y=17), "misaligned"),
+    (dict(ldy=63), "leading dimension")])
+def test_block_gemm_entry_refuses(change, match):
+    a = dict(x=16, ldx=128, sx=16, row=1, group=2, m=2, k=128, members=1, n=64, w=16, sw=16, y=16, ldy=64, out=0) | change
+    c = _native.ctypes
+    one = lambda ctype, v: (ctype * 1)(v)
+    with pytest.raises(ValueError, match=match):
+        _native.call("cubic_block_gemm", a["x"], a["ldx"], a["sx"], a["row"], a["group"], a["m"], a["k"], a["members"],
+                     one(c.c_int64, a["n"]), one(c.c_void_p, a["w"]), one(c.c_void_p, a["sw"]), one(c.c_void_p, a["y"]),
+                     one(c.c_int64, a["ldy"]), a["out"], None)
+
+
+def test_block_prepare_entry():
+    lib = _native.lib()
+    assert lib.cubic_block_prepared_bytes(16, 128) == 2048
+    assert lib.cubic_block_prepared_bytes(17, 129) == 4 * 2048
+    for n, k in ((0, 1), (1, 0), ((1 << 24) + 1, 1), (1, (1 << 20) + 1)):
+        assert lib.cubic_block_prepared_bytes(n, k) == -1
+        with pytest.raises(ValueError):
+            _native.call("cubic_block_prepare", 16, 1 << 21, n, k, 16, None)
+    for args in ((None, 128, 4, 128, 16), (16, 127, 4, 128, 16), (16, 128, 4, 128, 24), (16, 128, 4, 128, None)):
+        with pytest.raises(ValueError):
+            _native.call("cubic_block_prepare", *args, None)

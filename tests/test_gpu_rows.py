@@ -1,0 +1,241 @@
+"""GPU: row norms and 8-bit activations against their formulas in 64 bits.
+
+Tolerances.  h = x + r is rounded once (2^-24), the mean of squares is summed by
+at most 32 additions per thread, 6 in the wave and 4 over the waves, its root halves
+that, and three products and the weights' offset follow: at most 2^-18 of y in all
+(u(y)); y in 16 bits adds half a step of its type, a 16-bit sum too.  A scale is off by u(y)
+and its division, 2^-17 in all.  An e4m3 value is off by half a step, 2^-4 of it
+(2^-10 below 2^-6), from a value that is off by 2^-16.  silu(g): the exponent t is off
+by 2^-24 of 1 (its rest is added), exp2 and the reciprocal by 2^-22 each: within
+u(y); where exp(-g) overflows it is 0, off by less than 2^-110.
+"""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from cubic_serve_amd import blockscale, linear
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+BF16, FP16 = torch.bfloat16, torch.float16
+HALF_STEP = {BF16: 2.0 ** -8, FP16: 2.0 ** -11}
+LEAST = {BF16: 2.0 ** -134, FP16: 2.0 ** -25}  # half a step below the normal numbers
+U = 2.0 ** -18
+OPS = linear.PackedLinearOperators()
+
+
+def rows(m, k, dtype, seed, scale=1.0, pad=0):
+    """[m, k] of N(0, scale) in rows of k + pad."""
+    gen = torch.Generator().manual_seed(seed)
+    whole = (torch.randn((m, k + pad), generator=gen) * scale).to(dtype).to(DEV)
+    return whole[:, :k]
+
+
+def norm_exact(x, r, w, eps, offset):
+    h = x.double() + (r.double() if r is not None else 0)
+    return h, h / torch.sqrt((h * h).mean(1, keepdim=True) + eps) * (offset + w.double())
+
+
+def near16(got, want, what=""):
+    bound = want.abs() * (HALF_STEP[got.dtype] + U) + LEAST[got.dtype]
+    off = (got.double() - want).abs()
+    assert (off <= bound).all(), (what, (off / bound).max().item())
+
+
+def near8(q, want):
+    """Values and scales against the exact y."""
+    values, scales = q.values.double(), q.scales.double()
+    m, k = want.shape
+    blocks = (k + 127) // 128
+    padded = torch.nn.functional.pad(want, (0, blocks * 128 - k)).view(m, blocks, 128)
+    top = padded.abs().amax(2).clamp_min(2.0 ** -96)
+    assert ((scales - top / 448).abs() <= top / 448 * 2.0 ** -17).all()
+    v = want * (448 / top).repeat_interleave(128, 1)[:, :k]
+    bound = torch.maximum(v.abs() * 2.0 ** -4, torch.full_like(v, 2.0 ** -10)) + v.abs() * 2.0 ** -16
+    off = (values - v).abs()
+    assert (off <= bound).all(), (off / bound).max().item()
+
+
+SHAPES = [(1, 1), (3, 7), (5, 8), (2, 127), (4, 128), (3, 129), (7, 520), (2, 1024), (5, 1025), (1, 4096),
+          (33, 2056), (2, 8192), (600, 8200), (3, 16384), (2, 20003), (2, 32768), (2, 32769), (1, 70000)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("m,k", SHAPES)
+def test_norm(m, k, dtype):
+    print(f"norm m={m} k={k} {dtype}", flush=True)
+    x, r, w = rows(m, k, dtype, 1), rows(m, k, dtype, 2, 3.0), rows(1, k, dtype, 3)[0].contiguous()
+    y, s = torch.empty((m, k), dtype=dtype, device=DEV), torch.empty((m, k), dtype=dtype, device=DEV)
+    q = blockscale.BlockScaledActivations.empty(m, k, DEV)
+    for residual in (r, None):
+        OPS.bind_norm(x, w, epsilon=1e-5, residual=residual, residual_output=s, output=y, quantized=q).launch()
+        h, want = norm_exact(x, residual, w, 1e-5, 0.0)
+        near16(s, h, "sum")
+        near16(y, want, "y")
+        near8(q, want)
+
+
+@pytest.mark.parametrize("m,k", [(3, 100), (2, 1024), (9, 2056), (3, 40000)])
+def test_norm_in_place_padded_offset(m, k):
+    """Rows at strides that no vector fits, columns of one matrix, outputs over their inputs."""
+    print(f"norm in place m={m} k={k}", flush=True)
+    whole = rows(m, 2 * k + 3, BF16, 4, pad=2)
+    x, r = whole[:, 1:1 + k], whole[:, k + 2:2 * k + 2]
+    w = rows(1, k + 1, BF16, 5)[0][1:]
+    h, want = norm_exact(x, r, w, 1e-6, 1.0)
+    around = whole.clone()
+    q = blockscale.BlockScaledActivations(torch.zeros((m, k + 5), dtype=blockscale.E4M3, device=DEV)[:, 3:3 + k],
+                                          torch.zeros((m, (k + 127) // 128 + 1), device=DEV)[:, 1:])
+    OPS.bind_norm(x, w, epsilon=1e-6, weight_offset=1.0, residual=r, residual_output=r, output=x, quantized=q).launch()
+    near16(x, want)
+    near16(r, h)
+    near8(q, want)
+    for c in (0, k + 1, 2 * k + 2):  # what lies between the columns
+        assert torch.equal(whole[:, c], around[:, c])
+
+
+def test_norm_values_at_the_edges():
+    k = 384
+    x = rows(6, k, FP16, 6)
+    x[0] = 0
+    x[1, :128] = 0                      # a group of zeros beside others
+    x[2, 5] = float("nan")
+    x[3, 7] = float("inf")
+    x[4] = 2.0 ** -24                   # the least numbers
+    w = torch.ones(k, dtype=FP16, device=DEV)
+    q, y = blockscale.BlockScaledActivations.empty(6, k, DEV), torch.empty_like(x)
+    OPS.bind_norm(x, w, epsilon=1e-6, output=y, quantized=q).launch()
+    _, want = norm_exact(x, None, w, 1e-6, 0.0)
+    assert not y[0].any() and not q.values[0].float().any() and torch.isfinite(q.scales[:2]).all()
+    assert not q.values[1, :128].float().any()
+    assert torch.isnan(y[2]).all() and torch.isnan(q.dequantize()[2]).all()
+    assert torch.isnan(y[3, 7]) and not y[3, :7].any()  # inf / inf, and finite / inf
+    for r in (1, 4, 5):
+        near16(y[r:r + 1], want[r:r + 1])
+    near8(blockscale.BlockScaledActivations(q.values[4:], q.scales[4:]), want[4:])
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("m,k", [(1, 1), (3, 7), (5, 120), (4, 128), (9, 136), (2, 777), (70, 2048), (3, 2056), (129, 4104), (2, 20001)])
+def test_quantize(m, k, dtype):
+    print(f"quantize m={m} k={k} {dtype}", flush=True)
+    both = rows(m, 2 * k, dtype, 7, 3.0)
+    gate, up = both[:, :k], both[:, k:]
+    q = blockscale.BlockScaledActivations.empty(m, k, DEV)
+    OPS.bind_quantize(up, q).launch()
+    near8(q, up.double())
+    OPS.bind_quantize(up, q, gate=gate).launch()
+    g = gate.double()
+    near8(q, g / (1 + torch.exp(-g)) * up.double())
+
+
+def test_quantize_values_at_the_edges():
+    k = 256
+    up, gate = torch.ones((5, k), dtype=BF16, device=DEV), torch.ones((5, k), dtype=BF16, device=DEV)
+    gate[0] = torch.linspace(-200, 200, k)      # exp(-g) overflows on one side and vanishes on the other
+    up[1, 3] = float("nan")                     # its group, not the next
+    up[2, 130] = float("-inf")
+    up[3] = torch.finfo(BF16).max
+    up[4] = torch.finfo(BF16).tiny
+    q = blockscale.BlockScaledActivations.empty(5, k, DEV)
+    OPS.bind_quantize(up, q, gate=gate).launch()
+    g = gate.double()
+    near8(blockscale.BlockScaledActivations(q.values[:1], q.scales[:1]), (g / (1 + torch.exp(-g)) * up.double())[:1])
+    got = q.dequantize()
+    assert torch.isnan(got[1, :128]).all() and torch.isfinite(got[1, 128:]).all()
+    assert torch.isnan(got[2, 128:]).all() and torch.isfinite(got[2, :128]).all()
+    assert torch.isfinite(got[3]).all() and (got[3] > 0).all()
+    assert torch.isfinite(got[4]).all() and (q.scales[4].double() == 2.0 ** -96 / 448).logical_or(
+        (q.scales[4].double() - 2.0 ** -96 / 448).abs() <= 2.0 ** -96 / 448 * 2.0 ** -23).all()
+
+
+def test_rows_that_lie_far_apart():
+    """The second row starts past 2^31 elements of the first."""
+    k, stride = 200, (1 << 31) + 16
+    whole = torch.empty(stride + k, dtype=BF16, device=DEV)
+    x = whole.as_strided((2, k), (stride, 1))
+    x.copy_(rows(2, k, BF16, 8))
+    y, q = torch.empty((2, k), dtype=BF16, device=DEV), blockscale.BlockScaledActivations.empty(2, k, DEV)
+    w = torch.ones(k, dtype=BF16, device=DEV)
+    _, want = norm_exact(x, None, w, 1e-6, 0.0)
+    OPS.bind_norm(x, w, epsilon=1e-6, output=y, quantized=q).launch()
+    near16(y, want)
+    near8(q, want)
+    OPS.bind_quantize(x, q).launch()
+    near8(q, x.double())
+
+
+def test_many_short_rows():
+    """More rows than workgroups of one launch: a head's norm over many tokens."""
+    m, k = (1 << 20) + 5, 64
+    gen = torch.Generator(device=DEV).manual_seed(9)
+    x = torch.randn((m, k), generator=gen, device=DEV).to(BF16)
+    y, q, w = torch.empty_like(x), blockscale.BlockScaledActivations.empty(m, k, DEV), torch.ones(k, dtype=BF16, device=DEV)
+    OPS.bind_norm(x, w, epsilon=1e-6, output=y, quantized=q).launch()
+    _, want = norm_exact(x, None, w, 1e-6, 0.0)
+    near16(y, want)
+    near8(q, want)
+    OPS.bind_quantize(x, q).launch()
+    near8(q, x.double())
+
+
+def test_captured_and_replayed_on_another_stream():
+    m, k = 40, 2056
+    x, r, w = rows(m, k, BF16, 10), rows(m, k, BF16, 11), rows(1, k, BF16, 12)[0].contiguous()
+    y, s = torch.empty((m, k), dtype=BF16, device=DEV), torch.empty((m, k), dtype=BF16, device=DEV)
+    q = blockscale.BlockScaledActivations.empty(m, k, DEV)
+    norm = OPS.bind_norm(x, w, epsilon=1e-6, residual=r, residual_output=s, output=y)
+    quantize = OPS.bind_quantize(y, q)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        norm.launch(), quantize.launch()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        norm.launch(), quantize.launch()
+    for turn in range(3):
+        x.copy_(rows(m, k, BF16, 20 + turn))
+        y.zero_(), s.zero_(), q.scales.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = y.clone(), s.clone(), q.values.float(), q.scales.clone()
+        norm.launch(), quantize.launch()
+        torch.cuda.synchronize()
+        for a, b in zip(got, (y, s, q.values.float(), q.scales)):
+            assert torch.equal(a, b)
+        near16(y, norm_exact(x, r, w, 1e-6, 0.0)[1])
+        near8(q, y.double())
+
+
+def test_operands_changed_after_binding():
+    x, w = rows(2, 64, BF16, 13), torch.ones(64, dtype=BF16, device=DEV)
+    y = torch.empty_like(x)
+    binding = OPS.bind_norm(x, w, epsilon=1e-6, output=y)
+    y.resize_((2, 32))
+    with pytest.raises(ValueError, match="changed after binding"):
+        binding.launch()
+
+
+def test_refusals():
+    x, w = rows(4, 64, BF16, 14), torch.ones(64, dtype=BF16, device=DEV)
+    y, q = torch.empty_like(x), blockscale.BlockScaledActivations.empty(4, 64, DEV)
+    bad = [(dict(x=x.float()), "FP16/BF16"), (dict(x=x.t()), "row-major"), (dict(weight=w.half()), "weight"),
+           (dict(weight=w[:63]), "weight"), (dict(output=None), "output"), (dict(output=y.half()), "output"),
+           (dict(residual=x[:3]), "residual"), (dict(residual_output=y), "alias"), (dict(output=x[:, :1].expand(4, 64)), "output"),
+           (dict(quantized=blockscale.BlockScaledActivations.empty(4, 65, DEV)), "8-bit"), (dict(epsilon=float("nan")), "epsilon"),
+           (dict(epsilon=-1.0), "epsilon"), (dict(weight_offset=float("inf")), "epsilon|offset")]
+    for change, match in bad:
+        args = dict(x=x, weight=w, output=y, epsilon=1e-6) | change
+        with pytest.raises(ValueError, match=match):
+            OPS.bind_norm(args.pop("x"), args.pop("weight"), **args).launch()
+    big = torch.empty((5, 64), dtype=BF16, device=DEV)
+    with pytest.raises(ValueError, match="alias"):  # a row below its input
+        OPS.bind_norm(big[:4], w, epsilon=1e-6, output=big[1:])
+    with pytest.raises(ValueError, match="alias"):
+        OPS.bind_quantize(x, blockscale.BlockScaledActivations(x.view(torch.uint8).view(blockscale.E4M3)[:, :64], q.scales))
+    with pytest.raises(TypeError):
+        OPS.bind_quantize(x, y)
+    with pytest.raises(ValueError, match="gate"):
+        OPS.bind_quantize(x, q, gate=x[:, :63])
