@@ -39,6 +39,11 @@ SIGNATURES: dict[str, tuple] = {
     "cubic_vocab_sample": (I32, [P, I32, I64, I32, I32, I32, P, P, P, P, P, P, P, P, P, P, I64, P]),
     "cubic_adapters_workspace_bytes": (I64, [I64, I64, I32, P]),
     "cubic_adapters": (I32, [P, I64, P, I64, I64, I32, I32, P, P, P, P, P, P, P, P, P, P, I32, P, I64, P]),
+    "cubic_history_append": (I32, [P, P, P, P, I32, I32, P, P, I32, I64, I32, I32, I32, I32, P, P]),
+    "cubic_history_clear": (I32, [P, P, P, P, I32, I32, P, I32, I32, I32, P]),
+    "cubic_history_bias": (I32, [P, P, P, P, I32, I32, I32, P, P, I32, P]),
+    "cubic_logit_penalties": (I32, [P, I32, I64, I32, I32, I32, I32, P, P, P, P, P, I32, I32, P, P, P, P, P, P, I64,
+                                    P, I32, I64, P]),
     "cubic_row_norm": (I32, [P, I64, P, I64, P, I64, I64, I32, F32, F32, P, I64, P, I64, P, I64, P, I64, I64, P]),
     "cubic_quantize_rows": (I32, [P, I64, P, I64, I64, I64, I32, P, I64, P, I64, I64, P]),
     "cubic_block_prepared_bytes": (I64, [I64, I64]),

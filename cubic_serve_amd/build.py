@@ -21,7 +21,7 @@ LIB_DIR = PACKAGE / "_lib"
 LIB = LIB_DIR / "libcubic_mi355x.so"
 SOURCES = ("cubic_capi.hip", "cubic_gemm.hip", "cubic_panel.hip", "cubic_wide.hip", "cubic_accept.hip", "cubic_embed.hip", "cubic_moe.hip",
            "cubic_greedy.hip", "cubic_adapters.hip", "cubic_sample.hip", "cubic_rows.hip",
-           "cubic_block.hip")
+           "cubic_block.hip", "cubic_penalty.hip")
 ARCH = "gfx950"
 # Per-source flags.  The acceptance kernel sizes its LDS for three workgroups
 # per CU (three waves per SIMD at its register count); LLVM's promotion of

@@ -791,6 +791,111 @@ int cubic_vocab_sample(const void* logits, int dtype, int64_t row_stride, int ro
 }
 
 // ---------------------------------------------------------------------------
+// Token histories and penalties on logits
+// ---------------------------------------------------------------------------
+namespace {
+int check_history(const cubic::HistoryArgs& h, const char* what) {
+    if (!h.marks || !h.biases || !h.listed || !h.sizes) return fail(CUBIC_EINVAL, "%s: null history", what);
+    if (h.slots < 1 || h.slots >= (1 << 20) || h.vocab < 1 || h.vocab > cubic::kMaxHistoryVocab)
+        return fail(CUBIC_EINVAL, "%s: history of %d slots, %d tokens", what, h.slots, h.vocab);
+    if (((uintptr_t)h.marks | (uintptr_t)h.biases | (uintptr_t)h.listed | (uintptr_t)h.sizes) % 4)
+        return fail(CUBIC_EINVAL, "%s: misaligned history", what);
+    return CUBIC_OK;
+}
+}  // namespace
+
+int cubic_history_append(uint32_t* marks, float* biases, int32_t* listed, int32_t* sizes, int slots, int vocab,
+                         const int32_t* row_slots, const void* tokens, int token_bytes, int64_t ld, int rows,
+                         int length, int prompt, int live_rows, const int32_t* live_count, void* stream) {
+    const cubic::HistoryArgs h = {marks, biases, listed, sizes, slots, vocab};
+    if (const int status = check_history(h, "history append")) return status;
+    if (!row_slots || !tokens) return fail(CUBIC_EINVAL, "history append: null operand");
+    if (token_bytes != 4 && token_bytes != 8) return fail(CUBIC_EINVAL, "history tokens must be int32 or int64");
+    if (rows < 1 || rows >= (1 << 24) || length < 1 || (rows > 1 && (ld < length || ld > ((int64_t)1 << 40))))
+        return fail(CUBIC_EINVAL, "history append: rows=%d length=%d row stride %lld", rows, length, (long long)ld);
+    if (live_rows < 0 || live_rows > rows) return fail(CUBIC_EINVAL, "live_rows outside 0..rows");
+    if ((uintptr_t)tokens % token_bytes || (uintptr_t)row_slots % 4 || (uintptr_t)live_count % 4)
+        return fail(CUBIC_EINVAL, "history append: misaligned operand");
+    const cubic::HistoryTokens a = {row_slots, tokens, ld, token_bytes, length, prompt != 0, live_rows, live_count};
+    return hip_status(cubic::launch_history_append(h, a, (hipStream_t)stream), "history append launch");
+}
+
+int cubic_history_clear(uint32_t* marks, float* biases, int32_t* listed, int32_t* sizes, int slots, int vocab,
+                        const int32_t* row_slots, int rows, int slot, int biases_only, void* stream) {
+    const cubic::HistoryArgs h = {marks, biases, listed, sizes, slots, vocab};
+    if (const int status = check_history(h, "history clear")) return status;
+    if (!row_slots && (slot < 0 || slot >= slots)) return fail(CUBIC_EINVAL, "history slot %d outside 0..%d", slot, slots - 1);
+    if (rows < 1 || rows >= (1 << 24)) return fail(CUBIC_EINVAL, "history clear: rows=%d", rows);
+    return hip_status(cubic::launch_history_clear(h, row_slots, row_slots ? rows : 1, slot, biases_only != 0, (hipStream_t)stream),
+                      "history clear launch");
+}
+
+int cubic_history_bias(uint32_t* marks, float* biases, int32_t* listed, int32_t* sizes, int slots, int vocab,
+                       int slot, const int32_t* ids, const float* values, int count, void* stream) {
+    const cubic::HistoryArgs h = {marks, biases, listed, sizes, slots, vocab};
+    if (const int status = check_history(h, "history bias")) return status;
+    if (!ids || !values) return fail(CUBIC_EINVAL, "history bias: null operand");
+    if (slot < 0 || slot >= slots) return fail(CUBIC_EINVAL, "history slot %d outside 0..%d", slot, slots - 1);
+    if (count < 1 || count > vocab) return fail(CUBIC_EINVAL, "history bias: %d biases", count);
+    return hip_status(cubic::launch_history_bias(h, slot, ids, values, count, (hipStream_t)stream), "history bias launch");
+}
+
+int cubic_logit_penalties(const void* logits, int dtype, int64_t row_stride, int sequences, int depth, int width,
+                          int live_sequences, const int32_t* live_count, uint32_t* marks, float* biases,
+                          int32_t* listed, int32_t* sizes, int slots, int vocab, const int32_t* row_slots,
+                          const float* repetition, const float* presence, const float* frequency,
+                          const int64_t* drafts, const int32_t* mask, int64_t mask_words, void* out, int out_dtype,
+                          int64_t out_stride, void* stream) {
+    const cubic::HistoryArgs h = {marks, biases, listed, sizes, slots, vocab};
+    if (const int status = check_history(h, "logit penalties")) return status;
+    if (!logits || !row_slots || !out) return fail(CUBIC_EINVAL, "logit penalties: null operand");
+    if (dtype != CUBIC_DTYPE_BF16 && dtype != CUBIC_DTYPE_F16 && dtype != CUBIC_DTYPE_F32)
+        return fail(CUBIC_EINVAL, "logit penalties: dtype must be CUBIC_DTYPE_BF16, _F16 or _F32");
+    if (out_dtype != dtype && out_dtype != CUBIC_DTYPE_F32)
+        return fail(CUBIC_EINVAL, "logit penalties: outputs have the logits' type or 32 bits");
+    if (sequences < 1 || depth < 0 || depth > cubic::kMaxPenaltyDepth || (int64_t)sequences * (depth + 1) >= (1 << 24))
+        return fail(CUBIC_EINVAL, "logit penalties: sequences=%d depth=%d", sequences, depth);
+    if (width < 1 || width > vocab) return fail(CUBIC_EINVAL, "logit penalties: width %d outside the history's 1..%d", width, vocab);
+    const int64_t rows = (int64_t)sequences * (depth + 1), most = (int64_t)1 << 40;
+    if (rows > 1 && (row_stride < width || out_stride < width || row_stride > most || out_stride > most))
+        return fail(CUBIC_EINVAL, "logit penalties: row strides %lld, %lld", (long long)row_stride, (long long)out_stride);
+    if (depth > 0 && !drafts) return fail(CUBIC_EINVAL, "logit penalties: null drafts");
+    if (mask && mask_words < ceil_div(width, 32))
+        return fail(CUBIC_EINVAL, "grammar mask of %lld words for %d columns", (long long)mask_words, width);
+    if (live_sequences < 0 || live_sequences > sequences) return fail(CUBIC_EINVAL, "live_sequences outside 0..sequences");
+    const int size = dtype == CUBIC_DTYPE_F32 ? 4 : 2, out_size = out_dtype == CUBIC_DTYPE_F32 ? 4 : 2;
+    if ((uintptr_t)logits % size || (uintptr_t)out % out_size || (uintptr_t)drafts % 8 ||
+        ((uintptr_t)row_slots | (uintptr_t)repetition | (uintptr_t)presence | (uintptr_t)frequency | (uintptr_t)mask |
+         (uintptr_t)live_count) % 4)
+        return fail(CUBIC_EINVAL, "logit penalties: misaligned operand");
+    cubic::PenaltyArgs a = {};
+    a.inplace = out == logits;
+    if (a.inplace && (out_dtype != dtype || (rows > 1 && out_stride != row_stride)))
+        return fail(CUBIC_EINVAL, "logit penalties: in place the outputs have the logits' type and row stride");
+    a.logits = logits;
+    a.out = out;
+    a.ld = row_stride;
+    a.ldout = out_stride;
+    a.in = dtype;
+    a.out_type = out_dtype;
+    a.sequences = sequences;
+    a.depth = depth;
+    a.width = width;
+    a.chunks = (int)ceil_div(width, cubic::kPenaltyChunk);
+    a.live_sequences = live_sequences;
+    a.live_count = live_count;
+    a.history = h;
+    a.row_slots = row_slots;
+    a.repetition = repetition;
+    a.presence = presence;
+    a.frequency = frequency;
+    a.drafts = drafts;
+    a.mask = (const uint32_t*)mask;
+    a.mask_words = mask_words;
+    return hip_status(cubic::launch_penalties(a, (hipStream_t)stream), "logit penalties launch");
+}
+
+// ---------------------------------------------------------------------------
 // Row norms and 8-bit activations
 // ---------------------------------------------------------------------------
 namespace {

@@ -337,6 +337,45 @@ struct RowArgs {
 };
 hipError_t launch_rows(const RowArgs& a, hipStream_t s);
 
+// Penalties on logits and the history of tokens they read (cubic_penalty.hip)
+constexpr int kMaxPenaltyDepth = 8;
+constexpr int kPenaltyChunk = 8192;   // columns per workgroup
+constexpr int kMaxHistoryVocab = 1 << 24;
+struct HistoryArgs {
+    uint32_t* marks;              // [slots, vocab]: outputs counted | 2^30 listed | 2^31 in the prompt
+    float* biases;                // [slots, vocab], 0 unless listed
+    int32_t* listed;              // [slots, vocab]: the first sizes[slot] are the listed tokens
+    int32_t* sizes;               // [slots]
+    int slots, vocab;
+};
+struct HistoryTokens {
+    const int32_t* row_slots;     // [rows]; outside [0, slots): skipped
+    const void* tokens;           // [rows, length] int32 or int64 (token_bytes), row stride ld; outside [0, vocab): skipped
+    int64_t ld;
+    int token_bytes, length, prompt;
+    int live_rows;                // rows below it are taken
+    const int32_t* live_count;    // device int32 that may lower it, or null
+};
+struct PenaltyArgs {
+    const void* logits;           // [sequences * (depth + 1), ld] of type `in` (CUBIC_DTYPE_*)
+    void* out;                    // row stride ldout, type out_type; the logits themselves if inplace
+    int64_t ld, ldout;
+    int in, out_type, inplace;
+    int sequences, depth, width, chunks;
+    int live_sequences;           // sequences below it are changed, the others' rows left as they are
+    const int32_t* live_count;    // device int32 that may lower it, or null
+    HistoryArgs history;
+    const int32_t* row_slots;     // [sequences]; outside [0, slots): mask only
+    const float *repetition, *presence, *frequency;  // [sequences] or null
+    const int64_t* drafts;        // [depth, sequences]
+    const uint32_t* mask;         // [rows, mask_words] or null
+    int64_t mask_words;
+};
+hipError_t launch_penalties(const PenaltyArgs& a, hipStream_t s);
+hipError_t launch_history_append(const HistoryArgs& h, const HistoryTokens& a, hipStream_t s);
+hipError_t launch_history_clear(const HistoryArgs& h, const int32_t* row_slots, int rows, int only_slot, int biases_only, hipStream_t s);
+hipError_t launch_history_bias(const HistoryArgs& h, int slot, const int32_t* ids, const float* values, int n, hipStream_t s);
+
 // Block-scaled 8-bit products (cubic_block.hip)
 struct BlockMember {
     const uint8_t* codes;         // tiles of 16 rows, laid out by launch_block_prepare

@@ -392,6 +392,56 @@ CUBIC_API int cubic_embedding(const void* ids, int id_bytes, int64_t tokens, int
                               int group_in, int group_out, void* out, int out_dtype, void* stream);
 
 /* ---------------------------------------------------------------------------
+ * Penalties, biases and grammar masks on logits.  No counterpart in the
+ * reference's subset that this library replaces.
+ *
+ * A history of `slots` requests over `vocab` tokens is four arrays of the
+ * caller's, zero on first use: marks u32, biases f32 and listed i32
+ * [slots, vocab], sizes i32 [slots].  Per slot: how often each token was put out,
+ * whether the prompt has it, its bias, and the list of tokens that have any.
+ *
+ * cubic_history_append: tokens [rows, length] (int32 or int64: token_bytes; row
+ *   stride ld) of row r go to slot row_slots[r], as outputs or (prompt != 0) as
+ *   prompt.  Tokens outside [0, vocab) (-1 pads) and slots outside the history are
+ *   skipped; a slot or a token may come more than once.  Rows at or past live_rows,
+ *   or past live_count[0] where that is less, are not taken.
+ * cubic_history_clear: empties the slots of row_slots [rows] (or, where that is
+ *   NULL, `slot`), or only their biases.
+ * cubic_history_bias: sets biases of `slot` (distinct ids).
+ * cubic_logit_penalties: sequence s has rows s * (depth + 1) + d; with c the
+ *   outputs of token t in slot row_slots[s], and of the first d drafts of it
+ *   (drafts i64 [depth, sequences]):
+ *     l > 0 ? l / repetition : l * repetition   where the prompt has t or c > 0
+ *     l - frequency * c - (c > 0 ? presence : 0);  l + bias;  -inf where bit t of
+ *     the row's mask words is 0 (mask NULL: all admitted)
+ *   in 32 bits, rounded once to out_dtype (the logits' or _F32).  out may be the
+ *   logits themselves.  A slot outside the history: the mask only.  Settings f32
+ *   [sequences] or NULL (none); a repetition that is not positive and finite, or a
+ *   penalty that is not finite, makes all of the sequence's columns NaN, which
+ *   the samplers refuse.  Columns at or past width, and the rows of sequences at or
+ *   past live_sequences (live_count[0], where that is less), are left as they are.
+ *   0 <= depth <= 8, width <= vocab.  No workspace.
+ * ------------------------------------------------------------------------- */
+CUBIC_API int cubic_history_append(uint32_t* marks, float* biases, int32_t* listed, int32_t* sizes,
+                                   int slots, int vocab, const int32_t* row_slots, const void* tokens,
+                                   int token_bytes, int64_t ld, int rows, int length, int prompt,
+                                   int live_rows, const int32_t* live_count, void* stream);
+CUBIC_API int cubic_history_clear(uint32_t* marks, float* biases, int32_t* listed, int32_t* sizes,
+                                  int slots, int vocab, const int32_t* row_slots, int rows, int slot,
+                                  int biases_only, void* stream);
+CUBIC_API int cubic_history_bias(uint32_t* marks, float* biases, int32_t* listed, int32_t* sizes,
+                                 int slots, int vocab, int slot, const int32_t* ids,
+                                 const float* values, int count, void* stream);
+CUBIC_API int cubic_logit_penalties(const void* logits, int dtype, int64_t row_stride, int sequences,
+                                    int depth, int width, int live_sequences,
+                                    const int32_t* live_count, uint32_t* marks, float* biases,
+                                    int32_t* listed, int32_t* sizes, int slots, int vocab,
+                                    const int32_t* row_slots, const float* repetition,
+                                    const float* presence, const float* frequency,
+                                    const int64_t* drafts, const int32_t* mask, int64_t mask_words,
+                                    void* out, int out_dtype, int64_t out_stride, void* stream);
+
+/* ---------------------------------------------------------------------------
  * Row norms and 8-bit activations.  No counterpart in the reference's subset
  * that this library replaces.
  *
