@@ -181,6 +181,176 @@ __global__ __launch_bounds__(512) void block_stream_kernel(BlockGemmArgs a) {
     }
 }
 
+// ---------------------------------------------------------------------------
+// Many rows: the matrix cores bound it.  A workgroup has a tile of 16 NTW WN columns
+// by 16 MTW WM rows, WN x WM waves of 16 NTW x 16 MTW.  Both operands of a
+// block, and its row scales, go straight to LDS (buffer and global loads to LDS)
+// while the block before is multiplied.
+//
+// LDS order: weights as they were laid out, 16 bytes per lane in lane order.  x: of
+// a tile of 16 rows and half block 64 slots of 16 bytes, row r's chunk q at slot
+// 4 r + (q ^ turn(r)); four neighbouring lanes of the load then take one 64-byte
+// segment of a row, and the lanes that read a fragment together lie on different banks.
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ int turn(int r) { return (r >> 2 & 1) * 2 + (r >> 3); }
+
+typedef __attribute__((address_space(3))) void lds_void_t;
+typedef const __attribute__((address_space(1))) void global_void_t;
+
+template <int NTW, int MTW, int WN, int WM>
+__global__ __launch_bounds__(WN * WM * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
+void block_tile_kernel(BlockGemmArgs a) {
+    constexpr int W = WN * WM, N = NTW * WN, M = MTW * WM;  // tiles of 16
+    static_assert(8 % NTW == 0, "a wave's columns share a scale");
+    static_assert(2 * M % W == 0 && 2 * N % W == 0 && 16 * M % 64 == 0, "loads are shared out evenly");
+    // stages as objects of their own: a load into one does not wait for reads of the other
+    __shared__ __attribute__((aligned(1024))) uint8_t x0[M * kBlockBytes], x1[M * kBlockBytes];
+    __shared__ __attribute__((aligned(1024))) uint8_t w0[N * kBlockBytes], w1[N * kBlockBytes];
+    __shared__ __attribute__((aligned(256))) float s0[M * 16], s1[M * 16];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int quarter = lane >> 4, row = lane & 15;
+    const int wn = wave % WN, wm = wave / WN;
+
+    // Workgroups go round robin over the eight XCDs; an XCD takes consecutive items of an
+    // order that goes through 8 column groups for a row group, then the next
+    // rows, so that those it has at one time share operands in its L2.
+    const int cols = a.group_end[a.members - 1], row_groups = (a.m + 16 * M - 1) / (16 * M);
+    int id = blockIdx.x;
+    {
+        const int total = cols * row_groups, per = total >> 3, rest = total & 7, xcd = id & 7;
+        id = xcd * per + min(xcd, rest) + (id >> 3);
+    }
+    const int band = id / (8 * row_groups), wide = min(8, cols - 8 * band);
+    id -= band * 8 * row_groups;
+    const int m0 = id / wide * (16 * M);
+    const int group = 8 * band + id % wide;
+    const int j = find_member(a, group);
+    const BlockMember& w = a.member[j];
+    const int tile0 = (group - (j ? a.group_end[j - 1] : 0)) * N;
+
+    // --- loads to LDS: of a wave's 2 M / W half tiles of x and 2 N / W of w -----------
+    // Every tile of rows has a buffer of its own, moved on by the block: what a lane
+    // adds to it is one number.  Rows past the last, columns past K and blocks past
+    // the last read as zero.
+    const int load_row = lane >> 2, load_chunk = (lane & 3) ^ turn(load_row);
+    const uint32_t x_at = (uint32_t)(load_row * a.ldx) + 16u * load_chunk, w_at = lane * 16;
+    const int x_columns = a.k - 16 * load_chunk;
+    const int scale_part = wave % (M / 4);
+    const float* sx = a.x_scales + (int64_t)min(m0 + scale_part * 64 + lane, a.m - 1) * a.scale_row;
+    const int tile_bytes = a.blocks * kBlockBytes;
+    auto dma = [&](int b, uint8_t* xs, uint8_t* ws, float* ss) {
+        __attribute__((address_space(3))) uint8_t* xl = (__attribute__((address_space(3))) uint8_t*)(void*)xs;
+        __attribute__((address_space(3))) uint8_t* wl = (__attribute__((address_space(3))) uint8_t*)(void*)ws;
+        const int k = b * kScaleBlock;
+        const uint32_t off[2] = {k < x_columns ? x_at : kPastEnd, k + 64 < x_columns ? x_at + 64 : kPastEnd};
+#pragma unroll
+        for (int p = 0; p < M / W; ++p) {
+            const int tile = wave * (M / W) + p, first = m0 + 16 * tile, left = min(a.m - first, 16);
+            const __amdgpu_buffer_rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc(
+                const_cast<uint8_t*>(a.x + (int64_t)first * a.ldx + k), 0,
+                left <= 0 || k >= a.k ? 0 : (int)((left - 1) * a.ldx) + a.k - k, 0x00020000);
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(xr, (lds_void_t*)(xl + tile * kBlockBytes + h * 1024), 16, off[h], 0, 0, 0);
+        }
+#pragma unroll
+        for (int p = 0; p < N / W; ++p) {
+            const int tile = wave * (N / W) + p;
+            const __amdgpu_buffer_rsrc_t wr = __builtin_amdgcn_make_buffer_rsrc(
+                const_cast<uint8_t*>(w.codes + (int64_t)(tile0 + tile) * tile_bytes + (int64_t)b * kBlockBytes), 0,
+                tile0 + tile < w.tiles && b < a.blocks ? kBlockBytes : 0, 0x00020000);
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(wr, (lds_void_t*)(wl + tile * kBlockBytes + h * 1024), 16, w_at + h * 1024, 0, 0, 0);
+        }
+        // 64 rows' scales per wave; waves past the rows repeat (a branch would split the
+        // loop's body, and the compiler then moves sums across the parts)
+        __builtin_amdgcn_global_load_lds((global_void_t*)(sx + (int64_t)min(b, a.blocks - 1) * a.scale_group),
+                                         (lds_void_t*)((__attribute__((address_space(3))) float*)(void*)ss + scale_part * 64), 4, 0, 0);
+    };
+
+    v4f acc[NTW][MTW];
+#pragma unroll
+    for (int t = 0; t < NTW; ++t)
+#pragma unroll
+        for (int i = 0; i < MTW; ++i) acc[t][i] = v4f{0.f, 0.f, 0.f, 0.f};
+    // (the constant address space: one scalar load per wave)
+    const __attribute__((address_space(4))) float* sw = (const __attribute__((address_space(4))) float*)(
+        w.scales + (int64_t)(min(tile0 + wn * NTW, w.tiles - 1) >> 3) * a.blocks);
+    const uint32_t x_slot = (uint32_t)(wm * MTW * kBlockBytes) + (uint32_t)(4 * row + (quarter ^ turn(row))) * 16;
+    const uint32_t w_slot = (uint32_t)(wn * NTW * kBlockBytes) + lane * 16;
+    auto fragment = [](const uint8_t* at) {
+        return join(*reinterpret_cast<const u32x4_dev_t*>(at), *reinterpret_cast<const u32x4_dev_t*>(at + 1024));
+    };
+
+    // A product is added to its sum kLag products later, in the shadow of theirs.
+    constexpr int kLag = 2;
+    auto step = [&](int b, uint8_t* xs, uint8_t* ws, float* ss, uint8_t* xn, uint8_t* wnext, float* sn) {
+        float scale[MTW];
+        v8i xv[MTW], wv[2];
+        v4f p[kLag + 1];
+        const float block_scale = sw[min(b, a.blocks - 1)];
+#pragma unroll
+        for (int i = 0; i < MTW; ++i) xv[i] = fragment(xs + x_slot + i * kBlockBytes);
+        wv[0] = fragment(ws + w_slot);
+#pragma unroll
+        for (int i = 0; i < MTW; ++i) {
+            scale[i] = ss[(wm * MTW + i) * 16 + row] * block_scale;
+            asm("" : "+v"(scale[i]));  // (read always: no branch around it)
+            scale[i] = b < a.blocks ? scale[i] : 0.0f;
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        dma(b + 1, xn, wnext, sn);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int q = 0; q < NTW * MTW + kLag; ++q) {
+            const int t = q / MTW, i = q % MTW;
+            if (i == 0 && t + 1 < NTW) wv[(t + 1) & 1] = fragment(ws + w_slot + (t + 1) * kBlockBytes);
+            if (t < NTW) p[q % (kLag + 1)] = block_product(wv[t & 1], xv[i]);
+            if (q >= kLag) {
+                const int of = q - kLag;
+                v4f& sum = acc[of / MTW][of % MTW];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum[e] = fmaf(scale[of % MTW], p[of % (kLag + 1)][e], sum[e]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        __syncthreads();  // the next stage has landed, this one is read
+    };
+    dma(0, x0, w0, s0);
+    __syncthreads();
+    // (where the number of blocks is odd, the last step is one of zeros under scale 0)
+#pragma unroll 1
+    for (int b = 0; b < a.blocks; b += 2) {
+        step(b, x0, w0, s0, x1, w1, s1);
+        step(b + 1, x1, w1, s1, x0, w0, s0);
+    }
+
+    // 16 rows at a time through a wave-private run of LDS, to leave in whole lines
+    constexpr int kPitch = 16 * NTW + 4;  // of 32-bit sums
+    constexpr int kShare = W / 4;         // waves per stage object
+    static_assert(W % 4 == 0 && kShare * 16 * kPitch * 4 <= (M < N ? M : N) * kBlockBytes, "");
+    const int object = wave / kShare;
+    float* out = reinterpret_cast<float*>(object == 0 ? x0 : object == 1 ? x1 : object == 2 ? w0 : w1) + wave % kShare * 16 * kPitch;
+    const int n0 = (tile0 + wn * NTW) * 16;
+#pragma unroll
+    for (int i = 0; i < MTW; ++i) {
+#pragma unroll
+        for (int t = 0; t < NTW; ++t) *reinterpret_cast<v4f*>(out + row * kPitch + t * 16 + quarter * 4) = acc[t][i];
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll 1
+        for (int at = lane; at < 64 * NTW; at += 64) {
+            const int r = at / (4 * NTW), c = at % (4 * NTW) * 4, m = m0 + (wm * MTW + i) * 16 + r;
+            if (m < a.m) store4(a, w, m, n0 + c, *reinterpret_cast<const v4f*>(out + r * kPitch + c));
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
+}
+
 // Values [n, k] of any row stride to tiles; rows past n and columns past k are 0.
 __global__ __launch_bounds__(256) void block_prepare_kernel(const uint8_t* values, int64_t ld, int64_t n, int k,
                                                             int blocks, int64_t chunks, uint8_t* out) {
@@ -219,6 +389,12 @@ hipError_t launch_stream_rows(const BlockGemmArgs& a, hipStream_t s) {
 }  // namespace
 
 hipError_t launch_block_gemm(const BlockGemmArgs& a, hipStream_t s) {
+    if (a.tile) {
+        const unsigned rows = a.tile == 2 ? 256 : 128, grid = a.group_end[a.members - 1] * ((a.m + rows - 1) / rows);
+        if (a.tile == 2) block_tile_kernel<8, 4, 2, 4><<<grid, 512, 0, s>>>(a);
+        else block_tile_kernel<4, 4, 2, 2><<<grid, 256, 0, s>>>(a);
+        return hipGetLastError();
+    }
     switch (a.col_tiles) {
         case 1: return launch_stream_rows<1>(a, s);
         case 2: return launch_stream_rows<2>(a, s);

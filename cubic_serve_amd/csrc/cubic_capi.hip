@@ -1047,11 +1047,15 @@ int cubic_block_gemm(const void* x, int64_t ldx, const float* x_scales, int64_t 
     a.row_tiles = m <= 16 ? 1 : m <= 32 ? 2 : 4;
     a.col_tiles = tiles >= 2048 ? 4 : tiles >= 1024 ? 2 : 1;
     a.waves = a.col_tiles * a.row_tiles >= 16 ? 4 : 8;
+    a.tile = m > 64 ? (ceil_div(tiles, 16) * ceil_div(m, 256) >= 256 ? 2 : 1) : 0;
+    if (a.tile) a.col_tiles = a.tile * 8;
     int64_t groups = 0;
     for (int j = 0; j < cubic::kMaxGemmMembers; ++j) {
         if (j < members) groups += ceil_div(a.member[j].tiles, a.col_tiles);
         a.group_end[j] = (int)groups;
     }
+    if (a.tile && groups * ceil_div(m, 128) >= (1 << 22))
+        return fail(CUBIC_ENOTSUP, "block gemm: more tiles than one launch holds");
     return hip_status(cubic::launch_block_gemm(a, (hipStream_t)stream), "block gemm launch");
 }
 

@@ -391,6 +391,7 @@ struct BlockGemmArgs {
     int64_t ldx, scale_row, scale_group;
     int m, k, blocks, members;
     int out;                      // CUBIC_DTYPE_* of y
+    int tile;                     // 0: the stream kernel; 1: 128 x 128 tiles, 2: 256 x 256
     int col_tiles, row_tiles, waves;  // per workgroup
     int group_end[kMaxGemmMembers];   // ends of the members' column groups
     BlockMember member[kMaxGemmMembers];
