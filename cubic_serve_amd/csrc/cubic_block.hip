@@ -16,7 +16,10 @@
 // Any order of k inside a block serves as long as both operands have it.  Here
 // lane l of an operand has row l % 16 and the 16 bytes at 16 (l / 16) of each half
 // block: loads of 64 contiguous bytes per row of x.  Weights are laid out once as
-// [tile of 16 rows][block][half][lane][16 bytes], 2 KB per tile and block.
+// [128 rows][block][tile of 16 rows][half][lane][16 bytes]: 2 KB per tile and block, 16 KB
+// in one piece for all columns that share a scale.
+#include <type_traits>
+
 #include "cubic_capi_internal.h"
 #include "cubic_device.h"
 
@@ -26,6 +29,7 @@ namespace {
 typedef int v8i __attribute__((ext_vector_type(8)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 constexpr int kBlockBytes = 2048;              // one tile and block
+constexpr int kGroupBytes = 8 * kBlockBytes;   // 128 rows of one block
 constexpr uint32_t kPastEnd = 0x80000000u;     // a buffer offset past every extent
 
 __device__ __forceinline__ v8i join(u32x4_dev_t a, u32x4_dev_t b) {
@@ -105,11 +109,10 @@ __global__ __launch_bounds__(512) void block_stream_kernel(BlockGemmArgs a) {
         x_at[i] = (uint32_t)((16 * i + row) * a.ldx) + 16u * quarter;
         sx[i] = a.x_scales + (int64_t)min(m0 + 16 * i + row, a.m - 1) * a.scale_row;
     }
-    // a buffer per workgroup: tiles and blocks past the last read nothing
-    const int tile_bytes = a.blocks * kBlockBytes;
+    // a buffer of the workgroup's 128 rows: blocks past the last read nothing
     const __amdgpu_buffer_rsrc_t wr = __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<uint8_t*>(w.codes + (int64_t)tile0 * tile_bytes), 0, min(NT, w.tiles - tile0) * tile_bytes, 0x00020000);
-    const uint32_t w_at = lane * 16;
+        const_cast<uint8_t*>(w.codes + (int64_t)(tile0 >> 3) * a.blocks * kGroupBytes), 0, a.blocks * kGroupBytes, 0x00020000);
+    const uint32_t w_at = (tile0 & 7) * kBlockBytes + lane * 16;
     const float* sw = w.scales + (int64_t)(tile0 >> 3) * a.blocks;
 
     struct Stage {
@@ -119,12 +122,12 @@ __global__ __launch_bounds__(512) void block_stream_kernel(BlockGemmArgs a) {
     Stage st[DEPTH];
     auto load = [&](Stage& s, int b) {
         const bool some = b < a.blocks;
-        const uint32_t from = some ? (uint32_t)b * kBlockBytes : kPastEnd;
+        const uint32_t from = some ? (uint32_t)b * kGroupBytes : kPastEnd;
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int h = 0; h < 2; ++h)
-                s.w[t][h] = __builtin_amdgcn_raw_buffer_load_b128(wr, from + w_at + (uint32_t)(t * tile_bytes) + h * 1024, 0, 2);  // nt
+                s.w[t][h] = __builtin_amdgcn_raw_buffer_load_b128(wr, from + w_at + t * kBlockBytes + h * 1024, 0, 2);  // nt
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int k = b * kScaleBlock + h * 64;
@@ -197,16 +200,24 @@ __device__ __forceinline__ int turn(int r) { return (r >> 2 & 1) * 2 + (r >> 3);
 typedef __attribute__((address_space(3))) void lds_void_t;
 typedef const __attribute__((address_space(1))) void global_void_t;
 
-template <int NTW, int MTW, int WN, int WM>
-__global__ __launch_bounds__(WN * WM * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
+// s_waitcnt vmcnt(n), the other counters left alone
+constexpr int vm_waits(int n) { return (n & 0xF) | (0x7 << 4) | (0xF << 8) | ((n >> 4) << 14); }
+
+template <int NTW, int MTW, int WN, int WM, int S, int EU>
+__global__ __launch_bounds__(WN * WM * 64) __attribute__((amdgpu_waves_per_eu(EU, EU)))
 void block_tile_kernel(BlockGemmArgs a) {
     constexpr int W = WN * WM, N = NTW * WN, M = MTW * WM;  // tiles of 16
     static_assert(8 % NTW == 0, "a wave's columns share a scale");
-    static_assert(2 * M % W == 0 && 2 * N % W == 0 && 16 * M % 64 == 0, "loads are shared out evenly");
-    // stages as objects of their own: a load into one does not wait for reads of the other
-    __shared__ __attribute__((aligned(1024))) uint8_t x0[M * kBlockBytes], x1[M * kBlockBytes];
-    __shared__ __attribute__((aligned(1024))) uint8_t w0[N * kBlockBytes], w1[N * kBlockBytes];
-    __shared__ __attribute__((aligned(256))) float s0[M * 16], s1[M * 16];
+    static_assert(2 * M % W == 0 && 2 * N % W == 0 && M % 4 == 0 && S >= 2 && S <= 4, "loads are shared out evenly");
+    // A stage is x, w and the rows' scales.  Each is an object of its own: a load into one
+    // then does not wait for reads of another.
+    constexpr int kW = M * kBlockBytes, kScales = kW + N * kBlockBytes, kStage = kScales + M * 64;
+    __shared__ __attribute__((aligned(1024))) uint8_t stage0[kStage], stage1[kStage], stage2[kStage], stage3[kStage];
+    auto stage_of = [&](auto stage) -> uint8_t* {
+        constexpr int P = decltype(stage)::value;
+        if constexpr (P == 0) return stage0; else if constexpr (P == 1) return stage1; else if constexpr (P == 2) return stage2; else return stage3;
+    };
+    constexpr int kLoads = 2 * M / W + 2 * N / W + 1;  // to LDS, per wave and block
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int quarter = lane >> 4, row = lane & 15;
     const int wn = wave % WN, wm = wave / WN;
@@ -237,36 +248,58 @@ void block_tile_kernel(BlockGemmArgs a) {
     const int x_columns = a.k - 16 * load_chunk;
     const int scale_part = wave % (M / 4);
     const float* sx = a.x_scales + (int64_t)min(m0 + scale_part * 64 + lane, a.m - 1) * a.scale_row;
-    const int tile_bytes = a.blocks * kBlockBytes;
-    auto dma = [&](int b, uint8_t* xs, uint8_t* ws, float* ss) {
-        __attribute__((address_space(3))) uint8_t* xl = (__attribute__((address_space(3))) uint8_t*)(void*)xs;
-        __attribute__((address_space(3))) uint8_t* wl = (__attribute__((address_space(3))) uint8_t*)(void*)ws;
+    // per load of a wave: its tile's start, and its extent
+    constexpr int kX = M % W == 0 ? M / W : 1, kWt = N % W == 0 ? N / W : 1;  // tiles a wave loads (or half of)
+    const uint8_t *x_from[kX], *w_from[kWt];
+    int x_bytes[kX], w_bytes[kWt];
+#pragma unroll
+    for (int p = 0; p < kX; ++p) {
+        const int first = m0 + 16 * (M % W == 0 ? wave * kX + p : wave >> 1), left = min(a.m - first, 16);
+        x_from[p] = a.x + (int64_t)first * a.ldx;
+        x_bytes[p] = left <= 0 ? 0 : (int)((left - 1) * a.ldx) + a.k;
+    }
+#pragma unroll
+    for (int p = 0; p < kWt; ++p) {
+        const int tile = tile0 + (N % W == 0 ? wave * kWt + p : wave >> 1);
+        w_from[p] = w.codes + (int64_t)(tile >> 3) * a.blocks * kGroupBytes + (tile & 7) * kBlockBytes;
+        w_bytes[p] = tile < w.tiles ? kBlockBytes : 0;
+    }
+    const int blocks = a.blocks;
+    const int64_t scale_group = a.scale_group;
+    auto dma = [&](int b, auto stage) {
+        uint8_t* to = stage_of(stage);
+        __attribute__((address_space(3))) uint8_t* xl = (__attribute__((address_space(3))) uint8_t*)(void*)to;
+        __attribute__((address_space(3))) uint8_t* wl = xl + kW;
         const int k = b * kScaleBlock;
         const uint32_t off[2] = {k < x_columns ? x_at : kPastEnd, k + 64 < x_columns ? x_at + 64 : kPastEnd};
 #pragma unroll
-        for (int p = 0; p < M / W; ++p) {
-            const int tile = wave * (M / W) + p, first = m0 + 16 * tile, left = min(a.m - first, 16);
+        for (int p = 0; p < kX; ++p) {
             const __amdgpu_buffer_rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc(
-                const_cast<uint8_t*>(a.x + (int64_t)first * a.ldx + k), 0,
-                left <= 0 || k >= a.k ? 0 : (int)((left - 1) * a.ldx) + a.k - k, 0x00020000);
+                const_cast<uint8_t*>(x_from[p] + k), 0, max(x_bytes[p] - k, 0), 0x00020000);
+            if constexpr (M % W == 0) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(xr, (lds_void_t*)(xl + tile * kBlockBytes + h * 1024), 16, off[h], 0, 0, 0);
+                for (int h = 0; h < 2; ++h)
+                    __builtin_amdgcn_raw_ptr_buffer_load_lds(xr, (lds_void_t*)(xl + (wave * kX + p) * kBlockBytes + h * 1024), 16, off[h], 0, 0, 0);
+            } else {  // half a tile per wave
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(xr, (lds_void_t*)(xl + wave * 1024), 16, wave & 1 ? off[1] : off[0], 0, 0, 0);
+            }
         }
 #pragma unroll
-        for (int p = 0; p < N / W; ++p) {
-            const int tile = wave * (N / W) + p;
+        for (int p = 0; p < kWt; ++p) {
             const __amdgpu_buffer_rsrc_t wr = __builtin_amdgcn_make_buffer_rsrc(
-                const_cast<uint8_t*>(w.codes + (int64_t)(tile0 + tile) * tile_bytes + (int64_t)b * kBlockBytes), 0,
-                tile0 + tile < w.tiles && b < a.blocks ? kBlockBytes : 0, 0x00020000);
+                const_cast<uint8_t*>(w_from[p] + (int64_t)b * kGroupBytes), 0, b < blocks ? w_bytes[p] : 0, 0x00020000);
+            if constexpr (N % W == 0) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(wr, (lds_void_t*)(wl + tile * kBlockBytes + h * 1024), 16, w_at + h * 1024, 0, 0, 0);
+                for (int h = 0; h < 2; ++h)
+                    __builtin_amdgcn_raw_ptr_buffer_load_lds(wr, (lds_void_t*)(wl + (wave * kWt + p) * kBlockBytes + h * 1024), 16, w_at + h * 1024, 0, 0, 0);
+            } else {
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(wr, (lds_void_t*)(wl + wave * 1024), 16, w_at + (wave & 1) * 1024, 0, 0, 0);
+            }
         }
         // 64 rows' scales per wave; waves past the rows repeat (a branch would split the
         // loop's body, and the compiler then moves sums across the parts)
-        __builtin_amdgcn_global_load_lds((global_void_t*)(sx + (int64_t)min(b, a.blocks - 1) * a.scale_group),
-                                         (lds_void_t*)((__attribute__((address_space(3))) float*)(void*)ss + scale_part * 64), 4, 0, 0);
+        __builtin_amdgcn_global_load_lds((global_void_t*)(sx + (int64_t)min(b, blocks - 1) * scale_group),
+                                         (lds_void_t*)(xl + kScales + scale_part * 256), 4, 0, 0);
     };
 
     v4f acc[NTW][MTW];
@@ -285,22 +318,26 @@ void block_tile_kernel(BlockGemmArgs a) {
 
     // A product is added to its sum kLag products later, in the shadow of theirs.
     constexpr int kLag = 2;
-    auto step = [&](int b, uint8_t* xs, uint8_t* ws, float* ss, uint8_t* xn, uint8_t* wnext, float* sn) {
+    // S - 1 blocks are on their way.  A step begins where its block has landed and
+    // every wave is done with the block before, into whose place the next load goes.
+    auto step = [&](int b, auto stage) {
+        constexpr int P = decltype(stage)::value;
+        const uint8_t *xs = stage_of(stage), *ws = xs + kW;
+        const float* ss = reinterpret_cast<const float*>(xs + kScales);
         float scale[MTW];
         v8i xv[MTW], wv[2];
         v4f p[kLag + 1];
-        const float block_scale = sw[min(b, a.blocks - 1)];
+        __builtin_amdgcn_s_waitcnt(vm_waits((S - 2) * kLoads));
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        const float block_scale = sw[b];
 #pragma unroll
         for (int i = 0; i < MTW; ++i) xv[i] = fragment(xs + x_slot + i * kBlockBytes);
         wv[0] = fragment(ws + w_slot);
 #pragma unroll
-        for (int i = 0; i < MTW; ++i) {
-            scale[i] = ss[(wm * MTW + i) * 16 + row] * block_scale;
-            asm("" : "+v"(scale[i]));  // (read always: no branch around it)
-            scale[i] = b < a.blocks ? scale[i] : 0.0f;
-        }
+        for (int i = 0; i < MTW; ++i) scale[i] = ss[(wm * MTW + i) * 16 + row] * block_scale;
         __builtin_amdgcn_sched_barrier(0);
-        dma(b + 1, xn, wnext, sn);
+        dma(b + S - 1, std::integral_constant<int, (P + S - 1) % S>{});
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int q = 0; q < NTW * MTW + kLag; ++q) {
@@ -315,23 +352,42 @@ void block_tile_kernel(BlockGemmArgs a) {
             }
             __builtin_amdgcn_sched_barrier(0);
         }
-        __syncthreads();  // the next stage has landed, this one is read
+        // the sums stay in this step (the compiler would move additions to the next one)
+#pragma unroll
+        for (int t = 0; t < NTW; ++t)
+#pragma unroll
+            for (int i = 0; i < MTW; ++i) asm volatile("" : "+v"(acc[t][i]));
     };
-    dma(0, x0, w0, s0);
-    __syncthreads();
-    // (where the number of blocks is odd, the last step is one of zeros under scale 0)
-#pragma unroll 1
-    for (int b = 0; b < a.blocks; b += 2) {
-        step(b, x0, w0, s0, x1, w1, s1);
-        step(b + 1, x1, w1, s1, x0, w0, s0);
+    auto first = [&](auto... stages) { (dma(decltype(stages)::value, stages), ...); };
+    typedef std::integral_constant<int, 0> I0;
+    typedef std::integral_constant<int, 1> I1;
+    typedef std::integral_constant<int, 2> I2;
+    typedef std::integral_constant<int, 3> I3;
+    if constexpr (S == 2) first(I0{});
+    else if constexpr (S == 3) first(I0{}, I1{});
+    else first(I0{}, I1{}, I2{});
+    // Whole rounds of the stages, then the rest: a loop of one exit, through which the
+    // compiler follows which loads are on their way (with more it waits for all).
+    int b = 0;
+    for (; b + S <= blocks; b += S) {
+        step(b, I0{});
+        step(b + 1, I1{});
+        if constexpr (S > 2) step(b + 2, I2{});
+        if constexpr (S > 3) step(b + 3, I3{});
     }
+    if (b < blocks) step(b, I0{});
+    if constexpr (S > 2) {
+        if (b + 1 < blocks) step(b + 1, I1{});
+    }
+    if constexpr (S > 3) {
+        if (b + 2 < blocks) step(b + 2, I2{});
+    }
+    __syncthreads();  // the last loads (of nothing) have landed, all is read
 
     // 16 rows at a time through a wave-private run of LDS, to leave in whole lines
     constexpr int kPitch = 16 * NTW + 4;  // of 32-bit sums
-    constexpr int kShare = W / 4;         // waves per stage object
-    static_assert(W % 4 == 0 && kShare * 16 * kPitch * 4 <= (M < N ? M : N) * kBlockBytes, "");
-    const int object = wave / kShare;
-    float* out = reinterpret_cast<float*>(object == 0 ? x0 : object == 1 ? x1 : object == 2 ? w0 : w1) + wave % kShare * 16 * kPitch;
+    static_assert((W / 2) * 16 * kPitch * 4 <= kStage, "half of the waves per stage");
+    float* out = reinterpret_cast<float*>(wave & 1 ? stage1 : stage0) + (wave >> 1) * 16 * kPitch;
     const int n0 = (tile0 + wn * NTW) * 16;
 #pragma unroll
     for (int i = 0; i < MTW; ++i) {
@@ -356,9 +412,9 @@ __global__ __launch_bounds__(256) void block_prepare_kernel(const uint8_t* value
                                                             int blocks, int64_t chunks, uint8_t* out) {
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < chunks; i += (int64_t)gridDim.x * 256) {
         const int lane = i & 63, half = (i >> 6) & 1;
-        const int64_t at = i >> 7, tile = at / blocks;
-        const int64_t r = tile * 16 + (lane & 15);
-        const int c = (int)(at - tile * blocks) * kScaleBlock + half * 64 + (lane >> 4) * 16;
+        const int64_t at = i >> 10, group = at / blocks;
+        const int64_t r = group * kScaleBlock + (i >> 7 & 7) * 16 + (lane & 15);
+        const int c = (int)(at - group * blocks) * kScaleBlock + half * 64 + (lane >> 4) * 16;
         uint8_t v[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) v[e] = r < n && c + e < k ? values[r * ld + c + e] : 0;
@@ -386,14 +442,27 @@ hipError_t launch_stream_rows(const BlockGemmArgs& a, hipStream_t s) {
     }
 }
 
+template <int NTW, int MTW, int WN, int WM, int S, int EU>
+hipError_t launch_tile(const BlockGemmArgs& given, hipStream_t s) {
+    BlockGemmArgs a = given;
+    int64_t groups = 0;
+    for (int j = 0; j < kMaxGemmMembers; ++j) {
+        if (j < a.members) groups += (a.member[j].tiles + NTW * WN - 1) / (NTW * WN);
+        a.group_end[j] = (int)groups;
+    }
+    const unsigned grid = (unsigned)(groups * ((a.m + 16 * MTW * WM - 1) / (16 * MTW * WM)));
+    block_tile_kernel<NTW, MTW, WN, WM, S, EU><<<grid, WN * WM * 64, 0, s>>>(a);
+    return hipGetLastError();
+}
+
 }  // namespace
 
 hipError_t launch_block_gemm(const BlockGemmArgs& a, hipStream_t s) {
-    if (a.tile) {
-        const unsigned rows = a.tile == 2 ? 256 : 128, grid = a.group_end[a.members - 1] * ((a.m + rows - 1) / rows);
-        if (a.tile == 2) block_tile_kernel<8, 4, 2, 4><<<grid, 512, 0, s>>>(a);
-        else block_tile_kernel<4, 4, 2, 2><<<grid, 256, 0, s>>>(a);
-        return hipGetLastError();
+    switch (a.tile) {
+        case 1: return launch_tile<2, 2, 2, 2, 3, 3>(a, s);
+        case 2: return launch_tile<4, 2, 2, 2, 3, 2>(a, s);
+        case 3: return launch_tile<8, 4, 2, 4, 2, 2>(a, s);
+        default: break;
     }
     switch (a.col_tiles) {
         case 1: return launch_stream_rows<1>(a, s);
@@ -404,7 +473,7 @@ hipError_t launch_block_gemm(const BlockGemmArgs& a, hipStream_t s) {
 
 hipError_t launch_block_prepare(const uint8_t* values, int64_t ld, int64_t n, int64_t k, uint8_t* out, hipStream_t s) {
     const int blocks = (int)((k + kScaleBlock - 1) / kScaleBlock);
-    const int64_t chunks = (n + 15) / 16 * blocks * 128, groups = (chunks + 255) / 256;
+    const int64_t chunks = (n + kScaleBlock - 1) / kScaleBlock * blocks * 1024, groups = (chunks + 255) / 256;
     block_prepare_kernel<<<(unsigned)(groups < (1 << 20) ? groups : (1 << 20)), 256, 0, s>>>(values, ld, n, (int)k, blocks,
                                                                                            chunks, out);
     return hipGetLastError();

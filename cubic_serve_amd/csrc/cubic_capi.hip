@@ -881,7 +881,7 @@ int cubic_logit_penalties(const void* logits, int dtype, int64_t row_stride, int
     a.sequences = sequences;
     a.depth = depth;
     a.width = width;
-    a.chunks = (int)ceil_div(width, cubic::kPenaltyChunk);
+    a.chunks = (int)ceil_div(width, cubic::kPenaltyBytes / out_size);
     a.live_sequences = live_sequences;
     a.live_count = live_count;
     a.history = h;
@@ -992,7 +992,7 @@ int cubic_quantize_rows(const void* x, int64_t ldx, const void* gate, int64_t ld
 // ---------------------------------------------------------------------------
 int64_t cubic_block_prepared_bytes(int64_t n, int64_t k) {
     if (n < 1 || n > (1 << 24) || k < 1 || k > (1 << 20)) return -1;
-    return ceil_div(n, 16) * 16 * ceil_div(k, cubic::kScaleBlock) * cubic::kScaleBlock;
+    return ceil_div(n, cubic::kScaleBlock) * ceil_div(k, cubic::kScaleBlock) * cubic::kScaleBlock * cubic::kScaleBlock;
 }
 
 int cubic_block_prepare(const void* values, int64_t ld, int64_t n, int64_t k, void* prepared, void* stream) {
@@ -1047,14 +1047,18 @@ int cubic_block_gemm(const void* x, int64_t ldx, const float* x_scales, int64_t 
     a.row_tiles = m <= 16 ? 1 : m <= 32 ? 2 : 4;
     a.col_tiles = tiles >= 2048 ? 4 : tiles >= 1024 ? 2 : 1;
     a.waves = a.col_tiles * a.row_tiles >= 16 ? 4 : 8;
-    a.tile = m > 64 ? (ceil_div(tiles, 16) * ceil_div(m, 256) >= 256 ? 2 : 1) : 0;
-    if (a.tile) a.col_tiles = a.tile * 8;
+    // Tiles (columns x rows) of 256 x 256 where they fill the chip, else 128 x 64 where
+    // those do, else 64 x 64.  4096 x 8192 x 8192 258, 393 and 562 us; 1024 rows of it at K = 4096
+    // 65, 55 and 73; 512 x 4096 x 4096 61, 18.9 and 21.8; 256 x 4096 x 12288 171, 44 and 34.
+    // The stream kernel up to 16 rows: 16 x 6144 x 4096 12.4 and 11.2 in tiles, 1 row 6.5.
+    a.tile = m <= 16 ? 0 : m > 128 && ceil_div(tiles, 16) * ceil_div(m, 256) >= 256 ? 3 : ceil_div(tiles, 8) * ceil_div(m, 64) >= 256 ? 2 : 1;
+
     int64_t groups = 0;
     for (int j = 0; j < cubic::kMaxGemmMembers; ++j) {
         if (j < members) groups += ceil_div(a.member[j].tiles, a.col_tiles);
         a.group_end[j] = (int)groups;
     }
-    if (a.tile && groups * ceil_div(m, 128) >= (1 << 22))
+    if (a.tile && ceil_div(tiles, 4) * ceil_div(m, 64) >= (1 << 22))
         return fail(CUBIC_ENOTSUP, "block gemm: more tiles than one launch holds");
     return hip_status(cubic::launch_block_gemm(a, (hipStream_t)stream), "block gemm launch");
 }

@@ -339,13 +339,15 @@ hipError_t launch_rows(const RowArgs& a, hipStream_t s);
 
 // Penalties on logits and the history of tokens they read (cubic_penalty.hip)
 constexpr int kMaxPenaltyDepth = 8;
-constexpr int kPenaltyChunk = 8192;   // columns per workgroup
+constexpr int kPenaltyBytes = 16384;  // of outputs per workgroup
 constexpr int kMaxHistoryVocab = 1 << 24;
+constexpr int kHistoryBucket = 4096;  // tokens of the vocabulary that share a list
+constexpr int history_buckets(int vocab) { return (vocab + kHistoryBucket - 1) / kHistoryBucket; }
 struct HistoryArgs {
     uint32_t* marks;              // [slots, vocab]: outputs counted | 2^30 listed | 2^31 in the prompt
     float* biases;                // [slots, vocab], 0 unless listed
-    int32_t* listed;              // [slots, vocab]: the first sizes[slot] are the listed tokens
-    int32_t* sizes;               // [slots]
+    int32_t* listed;              // [slots, vocab]: of bucket b from b * kHistoryBucket on the listed tokens
+    int32_t* sizes;               // [slots, buckets]: how many
     int slots, vocab;
 };
 struct HistoryTokens {

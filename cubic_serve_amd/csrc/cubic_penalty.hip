@@ -10,12 +10,14 @@
 // bits), and once to the output's type.
 //
 // A history keeps per slot a table of marks (outputs counted, in the prompt,
-// listed), a table of biases, and the list of the tokens that have either, in
-// the order of their arrival.  The list's order is that of atomics; nothing depends on
+// listed), a table of biases, and for every kHistoryBucket tokens of the vocabulary a list
+// of those that have either.  A list's order is that of atomics; nothing depends on
 // it, since each listed token is taken by itself.
 //
 // What bounds the penalties: reading and writing the logits.  Listed tokens are a few
-// thousand of 10^5 columns, so each is looked up by itself.
+// thousand of 10^5 columns, so each is looked up by itself, by the workgroup that has
+// its column: it reads the lists of its own columns only (one list per slot, which every
+// workgroup of a row has to search, took 95 us where this takes 50: 256 rows of 151936).
 #include <type_traits>
 
 #include "cubic_capi_internal.h"
@@ -27,11 +29,13 @@ namespace {
 constexpr uint32_t kListed = 1u << 30, kPrompt = 1u << 31, kCount = kListed - 1;
 constexpr int kThreads = 256;
 
-// Puts a token on its slot's list unless it is there.
+// Puts a token on its bucket's list unless it is there.
 __device__ __forceinline__ void list_token(const HistoryArgs& h, int64_t slot, int t, uint32_t mark) {
     if (mark & kListed) return;
     if (atomicOr(&h.marks[slot * h.vocab + t], kListed) & kListed) return;
-    h.listed[slot * h.vocab + atomicAdd(&h.sizes[slot], 1)] = t;
+    const int bucket = t / kHistoryBucket;
+    const int at = atomicAdd(&h.sizes[slot * history_buckets(h.vocab) + bucket], 1);
+    h.listed[slot * h.vocab + bucket * kHistoryBucket + at] = t;
 }
 
 __global__ __launch_bounds__(kThreads) void history_append_kernel(HistoryArgs h, HistoryTokens a) {
@@ -48,22 +52,25 @@ __global__ __launch_bounds__(kThreads) void history_append_kernel(HistoryArgs h,
     }
 }
 
-// One workgroup per row: the tables' listed places back to zero (biases_only:
-// those of the biases), then the list.
+// One workgroup per row, a wave per bucket: the tables' listed places back to zero
+// (biases_only: those of the biases), then the list.
 __global__ __launch_bounds__(1024) void history_clear_kernel(HistoryArgs h, const int32_t* row_slots, int rows, int only_slot,
                                                              int biases_only) {
+    const int lane = threadIdx.x & 63, buckets = history_buckets(h.vocab);
     for (int row = blockIdx.x; row < rows; row += gridDim.x) {
         const int slot = row_slots ? row_slots[row] : only_slot;
         if (slot < 0 || slot >= h.slots) continue;
         const int64_t base = (int64_t)slot * h.vocab;
-        const int n = min(h.sizes[slot], h.vocab);
-        for (int i = threadIdx.x; i < n; i += blockDim.x) {
-            const int t = h.listed[base + i];
-            h.biases[base + t] = 0.0f;
-            if (!biases_only) h.marks[base + t] = 0;
+        for (int b = threadIdx.x >> 6; b < buckets; b += 16) {
+            int32_t* size = &h.sizes[(int64_t)slot * buckets + b];
+            const int n = min(*size, min(kHistoryBucket, h.vocab - b * kHistoryBucket));
+            for (int i = lane; i < n; i += 64) {
+                const int t = h.listed[base + b * kHistoryBucket + i];
+                h.biases[base + t] = 0.0f;
+                if (!biases_only) h.marks[base + t] = 0;
+            }
+            if (!biases_only && lane == 0 && n) *size = 0;
         }
-        __syncthreads();
-        if (!biases_only && threadIdx.x == 0) h.sizes[slot] = 0;
     }
 }
 
@@ -117,83 +124,152 @@ __device__ __forceinline__ bool admitted(const uint32_t* mask, int column) {
     return !mask || (mask[column >> 5] >> (column & 31) & 1);
 }
 
-// A (row, chunk of kPenaltyChunk columns) per workgroup and turn.
-// Out of place: the chunk is staged in LDS in the output's type, the listed tokens
-// in it are changed there, and it leaves with the mask applied: every output line is
-// written once.  In place (INPLACE): listed tokens, shared out over the
-// row's workgroups, and masked columns are written by themselves; a token
-// whose bit is 0 is left to the mask, so no two threads write one column.
+// Eight columns from any element on, as the words they lie in: global memory takes 16
+// bytes at any element's address.
+template <int TYPE>
+struct Eight {
+    uint32_t u[TYPE == 2 ? 8 : 4];
+};
+template <int TYPE>
+__device__ __forceinline__ Eight<TYPE> load8(const void* p, int64_t i) {
+    Eight<TYPE> v;
+    __builtin_memcpy(&v, static_cast<const uint8_t*>(p) + i * (TYPE == 2 ? 4 : 2), sizeof v);
+    return v;
+}
+template <int TYPE>
+__device__ __forceinline__ void store8(void* p, int64_t i, const Eight<TYPE>& v) {
+    __builtin_memcpy(static_cast<uint8_t*>(p) + i * (TYPE == 2 ? 4 : 2), &v, sizeof v);
+}
+// The same in another type (16 bits to 32).
+template <int IN, int OUT>
+__device__ __forceinline__ Eight<OUT> to_type(const Eight<IN>& v) {
+    if constexpr (IN == OUT) return v;
+    else {
+        Eight<OUT> w;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const uint32_t b = v.u[e >> 1] >> (16 * (e & 1)) & 0xFFFFu;
+            w.u[e] = __float_as_uint(IN == 1 ? half_bits_to_float(b) : bf16_bits_to_float(b));
+        }
+        return w;
+    }
+}
+// Columns whose bit is 0 become `other` (a 16-bit value in both halves).
+template <int TYPE>
+__device__ __forceinline__ void keep8(Eight<TYPE>& v, uint32_t bits, uint32_t other) {
+#pragma unroll
+    for (int w = 0; w < (int)(sizeof v / 4); ++w) {
+        uint32_t keep;
+        if constexpr (TYPE == 2) keep = 0u - (bits >> w & 1);
+        else keep = ((0u - (bits >> (2 * w) & 1)) & 0xFFFFu) | (0u - (bits >> (2 * w + 1) & 1)) << 16;
+        v.u[w] = (v.u[w] & keep) | (other & ~keep);
+    }
+}
+template <int TYPE>
+__device__ __forceinline__ Eight<TYPE> load_some(const void* p, int64_t i, uint32_t some) {
+    Eight<TYPE> v = {};
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if (some >> e & 1) {
+            if constexpr (TYPE == 2) v.u[e] = static_cast<const uint32_t*>(p)[i + e];
+            else v.u[e >> 1] |= (uint32_t)static_cast<const uint16_t*>(p)[i + e] << (16 * (e & 1));
+        }
+    return v;
+}
+template <int TYPE>
+__device__ __forceinline__ void store_some(void* p, int64_t i, const Eight<TYPE>& v, uint32_t some) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if (some >> e & 1) {
+            if constexpr (TYPE == 2) static_cast<uint32_t*>(p)[i + e] = v.u[e];
+            else static_cast<uint16_t*>(p)[i + e] = (uint16_t)(v.u[e >> 1] >> (16 * (e & 1)));
+        }
+}
+template <int TYPE>
+constexpr uint32_t minus_infinity() { return TYPE == 2 ? 0xFF800000u : TYPE == 1 ? 0xFC00FC00u : 0xFF80FF80u; }
+template <int TYPE>
+constexpr uint32_t not_a_number() { return TYPE == 2 ? 0x7FC00000u : TYPE == 1 ? 0x7E007E00u : 0x7FC07FC0u; }
+
+// A (row, chunk of columns) per workgroup and turn: the chunk goes from logits to outputs
+// with the mask applied, eight columns per thread and access (in place: masked columns
+// are written, no other); then, those stores done, listed tokens are written one by
+// one from the logits.  A token whose bit is 0 is left to the mask.
 template <int IN, int OUT, bool INPLACE>
 __global__ __launch_bounds__(kThreads) void penalty_kernel(PenaltyArgs a) {
-    typedef typename std::conditional<OUT == 2, float, uint16_t>::type out_t;
-    __shared__ __attribute__((aligned(16))) out_t staged[INPLACE ? 8 : kPenaltyChunk];
-    __shared__ int drafts[kMaxPenaltyDepth];
+    constexpr int kChunk = kPenaltyBytes / (OUT == 2 ? 4 : 2), kTurns = kChunk / (8 * kThreads), kLists = kChunk / kHistoryBucket;
+    static_assert(kChunk % kHistoryBucket == 0, "a list is one workgroup's");
     const int live = a.live_count ? min(max(*a.live_count, 0), a.live_sequences) : a.live_sequences;
     const int64_t items = (int64_t)live * (a.depth + 1) * a.chunks;
+    const int buckets = history_buckets(a.history.vocab);
     for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
         const int row = (int)(item / a.chunks), chunk = (int)(item - (int64_t)row * a.chunks);
         const int sequence = row / (a.depth + 1), ahead = row - sequence * (a.depth + 1);
-        const int c0 = chunk * kPenaltyChunk, columns = min(kPenaltyChunk, a.width - c0);
+        const int c0 = chunk * kChunk, columns = min(kChunk, a.width - c0);
         const uint32_t* mask = a.mask ? a.mask + (int64_t)row * a.mask_words : nullptr;
         const int64_t in_row = (int64_t)row * a.ld, out_row = (int64_t)row * a.ldout;
         const int slot = a.row_slots[sequence];
         const Settings s = settings_of(a, sequence);
-        const bool known = slot >= 0 && slot < a.history.slots;
+        const bool known = s.valid && slot >= 0 && slot < a.history.slots;
         const int64_t base = known ? (int64_t)slot * a.history.vocab : 0;
-        if ((int)threadIdx.x < ahead) {
-            const int64_t t = a.drafts[(int64_t)threadIdx.x * a.sequences + sequence];
-            drafts[threadIdx.x] = t >= 0 && t < a.width ? (int)t : -1;
+        int sizes[kLists];
+#pragma unroll
+        for (int l = 0; l < kLists; ++l) {
+            const int bucket = c0 / kHistoryBucket + l;
+            sizes[l] = known && bucket < buckets ? a.history.sizes[(int64_t)slot * buckets + bucket] : 0;
         }
-        if constexpr (!INPLACE) {
-            for (int c = threadIdx.x; c < columns; c += kThreads) set_value<OUT>(staged, c, value_of<IN>(a.logits, in_row + c0 + c));
-        }
-        __syncthreads();
-        // a token of this chunk (in place: of this workgroup's share)
-        auto change = [&](int t, uint32_t mark, float bias) {
-            if constexpr (INPLACE) {
-                if (!admitted(mask, t)) return;
+
+        if (!INPLACE || mask || !s.valid) {
+            const uint32_t other = s.valid ? minus_infinity<OUT>() : not_a_number<OUT>();
+#pragma unroll
+            for (int i = 0; i < kTurns; ++i) {
+                const int c = (i * kThreads + (int)threadIdx.x) * 8;
+                if (c >= columns) break;
+                const uint32_t bits = !s.valid ? 0u : mask ? reinterpret_cast<const uint8_t*>(mask)[(c0 + c) >> 3] : 0xFFu;
+                const uint32_t all = columns - c >= 8 ? 0xFFu : (1u << (columns - c)) - 1;
+                Eight<OUT> out = {};
+                if constexpr (INPLACE) {
+                    keep8<OUT>(out, 0u, other);
+                    if ((all & ~bits) == 0xFFu) store8<OUT>(a.out, out_row + c0 + c, out);
+                    else store_some<OUT>(a.out, out_row + c0 + c, out, all & ~bits);
+                } else if (all == 0xFFu) {
+                    out = to_type<IN, OUT>(load8<IN>(a.logits, in_row + c0 + c));
+                    keep8<OUT>(out, bits, other);
+                    store8<OUT>(a.out, out_row + c0 + c, out);
+                } else {
+                    out = to_type<IN, OUT>(load_some<IN>(a.logits, in_row + c0 + c, all));
+                    keep8<OUT>(out, bits, other);
+                    store_some<OUT>(a.out, out_row + c0 + c, out, all);
+                }
             }
+        }
+        if (!known) continue;
+        if constexpr (!INPLACE) {  // two stores to one column follow each other
+            __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+            __syncthreads();
+        }
+        const uint32_t* marks = a.history.marks + base;
+        const int64_t* drafts = a.drafts + sequence;
+        auto change = [&](int t, float l, uint32_t mark, float bias) {
             int more = 0;
-            for (int j = 0; j < ahead; ++j) more += drafts[j] == t;
-            const float v = penalised(value_of<IN>(a.logits, in_row + t), mark, more, bias, s);
-            if constexpr (INPLACE) set_value<OUT>(a.out, out_row + t, v);
-            else set_value<OUT>(staged, t - c0, v);
+            for (int j = 0; j < ahead; ++j) more += drafts[(int64_t)j * a.sequences] == t;
+            set_value<OUT>(a.out, out_row + t, penalised(l, mark, more, bias, s));
         };
-        if (known && s.valid) {
-            const uint32_t* marks = a.history.marks + base;
-            const int n = min(a.history.sizes[slot], a.history.vocab);
-            if constexpr (INPLACE) {
-                for (int i = chunk * kThreads + threadIdx.x; i < n; i += a.chunks * kThreads) {
-                    const int t = a.history.listed[base + i];
-                    if (t < a.width) change(t, marks[t], a.history.biases[base + t]);
-                }
-            } else {
-                for (int i = threadIdx.x; i < n; i += kThreads) {
-                    const int t = a.history.listed[base + i];
-                    if (t >= c0 && t < c0 + columns) change(t, marks[t], a.history.biases[base + t]);
-                }
-            }
-            if ((int)threadIdx.x < ahead) {  // drafts that are new to the request
-                const int t = drafts[threadIdx.x];
-                bool first = t >= 0;
-                for (int j = 0; j < (int)threadIdx.x; ++j) first = first && drafts[j] != t;
-                if (first && (INPLACE ? chunk == 0 : t >= c0 && t < c0 + columns) && !(marks[t] & kListed)) change(t, 0, 0.0f);
+#pragma unroll
+        for (int l = 0; l < kLists; ++l) {
+            const int first = c0 + l * kHistoryBucket, n = min(sizes[l], kHistoryBucket);
+            for (int i = threadIdx.x; i < n; i += kThreads) {
+                const int t = a.history.listed[base + first + i];
+                if (t < a.width && admitted(mask, t))
+                    change(t, value_of<IN>(a.logits, in_row + t), marks[t], a.history.biases[base + t]);
             }
         }
-        __syncthreads();
-        if constexpr (INPLACE) {
-            if (mask || !s.valid)
-                for (int c = c0 + threadIdx.x; c < c0 + columns; c += kThreads) {
-                    if (!s.valid) set_value<OUT>(a.out, out_row + c, __builtin_nanf(""));
-                    else if (!admitted(mask, c)) set_value<OUT>(a.out, out_row + c, -__builtin_huge_valf());
-                }
-        } else {
-            for (int c = threadIdx.x; c < columns; c += kThreads) {
-                const float v = !s.valid ? __builtin_nanf("") : !admitted(mask, c0 + c) ? -__builtin_huge_valf() : value_of<OUT>(staged, c);
-                set_value<OUT>(a.out, out_row + c0 + c, v);
-            }
+        if ((int)threadIdx.x < ahead) {  // drafts that are new to the request
+            const int64_t t = drafts[(int64_t)threadIdx.x * a.sequences];
+            bool mine = t >= c0 && t < c0 + columns;
+            for (int j = 0; j < (int)threadIdx.x; ++j) mine = mine && drafts[(int64_t)j * a.sequences] != t;
+            if (mine && admitted(mask, (int)t) && !(marks[t] & kListed))
+                change((int)t, value_of<IN>(a.logits, in_row + t), 0, 0.0f);
         }
-        __syncthreads();  // the staged chunk and the drafts are read
     }
 }
 

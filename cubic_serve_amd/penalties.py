@@ -22,6 +22,7 @@ from . import _native
 from .sampling import _CANDIDATE_DTYPES
 
 MAX_DEPTH = 8  # kMaxPenaltyDepth of the C ABI
+BUCKET = 4096  # kHistoryBucket: tokens of the vocabulary that share a list
 
 
 def _live(live, most: int, device: torch.device, what: str) -> tuple[int, int | None]:
@@ -40,8 +41,8 @@ def _live(live, most: int, device: torch.device, what: str) -> tuple[int, int | 
 class TokenHistory:
     """Tokens and biases of ``slots`` requests over ``vocab`` tokens.
 
-    ``marks`` int32, ``biases`` float32 and ``listed`` int32 [slots, vocab], ``sizes``
-    int32 [slots]: 12 bytes per slot and token.  Its methods enqueue on the
+    ``marks`` int32, ``biases`` float32 and ``listed`` int32 [slots, vocab]: 12 bytes per
+    slot and token, and ``sizes`` int32 [slots, ceil(vocab / 4096)].  Its methods enqueue on the
     current stream and order nothing against other streams; but for ``set_bias``
     they may be captured, and read their tensors when they run.
     """
@@ -55,7 +56,7 @@ class TokenHistory:
         self.marks = torch.zeros((slots, vocab), dtype=torch.int32, device=device)
         self.biases = torch.zeros((slots, vocab), dtype=torch.float32, device=device)
         self.listed = torch.zeros((slots, vocab), dtype=torch.int32, device=device)
-        self.sizes = torch.zeros(slots, dtype=torch.int32, device=device)
+        self.sizes = torch.zeros((slots, (vocab + BUCKET - 1) // BUCKET), dtype=torch.int32, device=device)
         self.device = self.marks.device
         self._held = (self.marks, self.biases, self.listed, self.sizes)  # whose addresses bindings copy
         self._args = (*(t.data_ptr() for t in self._held), slots, vocab)

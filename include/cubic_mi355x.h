@@ -397,8 +397,9 @@ CUBIC_API int cubic_embedding(const void* ids, int id_bytes, int64_t tokens, int
  *
  * A history of `slots` requests over `vocab` tokens is four arrays of the
  * caller's, zero on first use: marks u32, biases f32 and listed i32
- * [slots, vocab], sizes i32 [slots].  Per slot: how often each token was put out,
- * whether the prompt has it, its bias, and the list of tokens that have any.
+ * [slots, vocab], sizes i32 [slots, ceil(vocab / 4096)].  Per slot: how often each
+ * token was put out, whether the prompt has it, its bias, and per 4096 tokens a
+ * list of those that have any.
  *
  * cubic_history_append: tokens [rows, length] (int32 or int64: token_bytes; row
  *   stride ld) of row r go to slot row_slots[r], as outputs or (prompt != 0) as

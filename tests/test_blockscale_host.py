@@ -113,8 +113,8 @@ def test_block_gemm_entry_refuses(change, match):
 
 def test_block_prepare_entry():
     lib = _native.lib()
-    assert lib.cubic_block_prepared_bytes(16, 128) == 2048
-    assert lib.cubic_block_prepared_bytes(17, 129) == 4 * 2048
+    assert lib.cubic_block_prepared_bytes(16, 128) == 128 * 128
+    assert lib.cubic_block_prepared_bytes(129, 129) == 4 * 128 * 128
     for n, k in ((0, 1), (1, 0), ((1 << 24) + 1, 1), (1, (1 << 20) + 1)):
         assert lib.cubic_block_prepared_bytes(n, k) == -1
         with pytest.raises(ValueError):
