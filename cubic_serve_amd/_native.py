@@ -39,10 +39,10 @@ SIGNATURES: dict[str, tuple] = {
     "cubic_vocab_sample": (I32, [P, I32, I64, I32, I32, I32, P, P, P, P, P, P, P, P, P, P, I64, P]),
     "cubic_adapters_workspace_bytes": (I64, [I64, I64, I32, P]),
     "cubic_adapters": (I32, [P, I64, P, I64, I64, I32, I32, P, P, P, P, P, P, P, P, P, P, I32, P, I64, P]),
-    "cubic_history_append": (I32, [P, P, P, P, I32, I32, P, P, I32, I64, I32, I32, I32, I32, P, P]),
-    "cubic_history_clear": (I32, [P, P, P, P, I32, I32, P, I32, I32, I32, P]),
-    "cubic_history_bias": (I32, [P, P, P, P, I32, I32, I32, P, P, I32, P]),
-    "cubic_logit_penalties": (I32, [P, I32, I64, I32, I32, I32, I32, P, P, P, P, P, I32, I32, P, P, P, P, P, P, I64,
+    "cubic_history_append": (I32, [P, P, P, I32, I32, P, P, I32, I64, I32, I32, I32, I32, P, P]),
+    "cubic_history_clear": (I32, [P, P, P, I32, I32, P, I32, I32, I32, P]),
+    "cubic_history_bias": (I32, [P, P, P, I32, I32, I32, P, P, I32, P]),
+    "cubic_logit_penalties": (I32, [P, I32, I64, I32, I32, I32, I32, P, P, P, P, I32, I32, P, P, P, P, P, P, I64,
                                     P, I32, I64, P]),
     "cubic_row_norm": (I32, [P, I64, P, I64, P, I64, I64, I32, F32, F32, P, I64, P, I64, P, I64, P, I64, I64, P]),
     "cubic_quantize_rows": (I32, [P, I64, P, I64, I64, I64, I32, P, I64, P, I64, I64, P]),
@@ -109,9 +109,8 @@ def lib() -> ctypes.CDLL:
     return _lib
 
 
-def call(name: str, *args) -> int:
-    """Call an int-status entry point; raise ValueError/RuntimeError on failure."""
-    status = getattr(lib(), name)(*args)
+def check(name: str, status: int) -> int:
+    """The status of an entry point; ValueError/RuntimeError where it failed."""
     if status < 0:
         message = (lib().cubic_last_error() or b"").decode(errors="replace")
         if status in (-1, -2, -4):
@@ -120,19 +119,44 @@ def call(name: str, *args) -> int:
     return status
 
 
+def call(name: str, *args) -> int:
+    """Call an int-status entry point; raise ValueError/RuntimeError on failure."""
+    return check(name, getattr(lib(), name)(*args))
+
+
+def converted(name: str, args) -> tuple:
+    """Leading arguments of an entry point as ctypes objects, for a call made often
+    (20 arguments: 1.8 us of the host's time, 2.5 from Python numbers)."""
+    return tuple(None if v is None else v if hasattr(v, "_length_") else kind(v)
+                 for kind, v in zip(SIGNATURES[name][1], args))
+
+
 def ptr(tensor) -> int | None:
     """Device address of a tensor (None for a missing optional operand)."""
     return None if tensor is None else tensor.data_ptr()
 
 
+_raw_stream = _get_device = None  # torch's own functions, once they have been looked up
+
+
+def _look_up() -> None:
+    import torch
+
+    global _raw_stream, _get_device
+    _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+        (lambda index: int(torch.cuda.current_stream(index).cuda_stream))
+    _get_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
 def stream_of(device) -> int:
     """The current stream's handle on a device (an index is taken fastest:
     1.4 us of the host's time through a stream object, 0.2 by the raw handle)."""
+    if isinstance(device, int):
+        if _raw_stream is None:
+            _look_up()
+        return _raw_stream(device)
     import torch
 
-    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-    if raw is not None and isinstance(device, int):
-        return raw(device)
     return int(torch.cuda.current_stream(device).cuda_stream)
 
 
@@ -146,9 +170,11 @@ class on_device:
         self.index, self.guard = index, None
 
     def __enter__(self):
-        import torch
+        if _get_device is None:
+            _look_up()
+        if _get_device() != self.index:
+            import torch
 
-        if torch.cuda.current_device() != self.index:
             self.guard = torch.cuda.device(self.index)
             self.guard.__enter__()
 

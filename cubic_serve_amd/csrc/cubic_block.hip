@@ -31,6 +31,7 @@ typedef float v4f __attribute__((ext_vector_type(4)));
 constexpr int kBlockBytes = 2048;              // one tile and block
 constexpr int kGroupBytes = 8 * kBlockBytes;   // 128 rows of one block
 constexpr uint32_t kPastEnd = 0x80000000u;     // a buffer offset past every extent
+constexpr int kStreamWaves = 8;
 
 __device__ __forceinline__ v8i join(u32x4_dev_t a, u32x4_dev_t b) {
     return v8i{(int)a.x, (int)a.y, (int)a.z, (int)a.w, (int)b.x, (int)b.y, (int)b.z, (int)b.w};
@@ -82,42 +83,33 @@ __device__ __forceinline__ int find_member(const BlockGemmArgs& a, int group) {
 }
 
 // ---------------------------------------------------------------------------
-// Few rows: the weight stream bounds it.  A workgroup has NT tiles of columns and
-// 16 MT rows; its waves take the blocks of K in turn, each block's weights and
-// activations straight into registers, DEPTH blocks ahead, no barrier until
-// the waves' sums are added through LDS, in the order of the waves.
+// Up to 8 rows: the weight stream bounds it.  A workgroup has NT tiles of columns; its
+// waves take the blocks of K in turn, each block's weights and activations straight
+// into registers, DEPTH blocks ahead, no barrier until the waves' sums are added
+// through LDS, in the order of the waves.  1 row, 151936 x 4096: 118 us, 5.3 TB/s.
 // ---------------------------------------------------------------------------
-template <int NT, int MT, int DEPTH>
-__global__ __launch_bounds__(512) void block_stream_kernel(BlockGemmArgs a) {
-    extern __shared__ __attribute__((aligned(16))) float sums[];  // [waves][NT * MT][64] of four
+template <int NT, int DEPTH>
+__global__ __launch_bounds__(kStreamWaves * 64) void block_stream_kernel(BlockGemmArgs a) {
+    __shared__ v4f sums[kStreamWaves][NT][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int waves = blockDim.x >> 6;
     const int quarter = lane >> 4, row = lane & 15;
     const int j = find_member(a, blockIdx.x);
     const BlockMember& w = a.member[j];
     const int tile0 = (blockIdx.x - (j ? a.group_end[j - 1] : 0)) * NT;
-    const int m0 = blockIdx.y * (16 * MT);
-    const int rows = min(16 * MT, a.m - m0);
 
-    const uint8_t* x = a.x + (int64_t)m0 * a.ldx;
+    // buffers of x and of the workgroup's 128 rows of w: what lies past them reads as zero
     const __amdgpu_buffer_rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<uint8_t*>(x), 0, (int)((rows - 1) * a.ldx) + a.k, 0x00020000);
-    uint32_t x_at[MT];
-    const float* sx[MT];
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-        x_at[i] = (uint32_t)((16 * i + row) * a.ldx) + 16u * quarter;
-        sx[i] = a.x_scales + (int64_t)min(m0 + 16 * i + row, a.m - 1) * a.scale_row;
-    }
-    // a buffer of the workgroup's 128 rows: blocks past the last read nothing
+        const_cast<uint8_t*>(a.x), 0, (int)((a.m - 1) * a.ldx) + a.k, 0x00020000);
+    const uint32_t x_at = (uint32_t)(row * a.ldx) + 16u * quarter;
+    const float* sx = a.x_scales + (int64_t)min(row, a.m - 1) * a.scale_row;
     const __amdgpu_buffer_rsrc_t wr = __builtin_amdgcn_make_buffer_rsrc(
         const_cast<uint8_t*>(w.codes + (int64_t)(tile0 >> 3) * a.blocks * kGroupBytes), 0, a.blocks * kGroupBytes, 0x00020000);
     const uint32_t w_at = (tile0 & 7) * kBlockBytes + lane * 16;
     const float* sw = w.scales + (int64_t)(tile0 >> 3) * a.blocks;
 
     struct Stage {
-        u32x4_dev_t w[NT][2], x[MT][2];
-        float sx[MT], sw;
+        u32x4_dev_t w[NT][2], x[2];
+        float sx, sw;
     };
     Stage st[DEPTH];
     auto load = [&](Stage& s, int b) {
@@ -131,56 +123,44 @@ __global__ __launch_bounds__(512) void block_stream_kernel(BlockGemmArgs a) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int k = b * kScaleBlock + h * 64;
-            const bool in = some && k + 16 * quarter < a.k;
-#pragma unroll
-            for (int i = 0; i < MT; ++i)
-                s.x[i][h] = __builtin_amdgcn_raw_buffer_load_b128(xr, in ? x_at[i] + (uint32_t)k : kPastEnd, 0, 0);
+            s.x[h] = __builtin_amdgcn_raw_buffer_load_b128(
+                xr, some && row < a.m && k + 16 * quarter < a.k ? x_at + (uint32_t)k : kPastEnd, 0, 0);
         }
         const int at = min(b, a.blocks - 1);
-#pragma unroll
-        for (int i = 0; i < MT; ++i) s.sx[i] = sx[i][(int64_t)at * a.scale_group];
+        s.sx = sx[(int64_t)at * a.scale_group];
         s.sw = sw[at];
     };
-    v4f acc[NT][MT];
+    v4f acc[NT];
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int i = 0; i < MT; ++i) acc[t][i] = v4f{0.f, 0.f, 0.f, 0.f};
+    for (int t = 0; t < NT; ++t) acc[t] = v4f{0.f, 0.f, 0.f, 0.f};
 
 #pragma unroll
-    for (int d = 0; d < DEPTH; ++d) load(st[d], wave + d * waves);
-    for (int b = wave; b < a.blocks; b += DEPTH * waves) {
+    for (int d = 0; d < DEPTH; ++d) load(st[d], wave + d * kStreamWaves);
+    for (int b = wave; b < a.blocks; b += DEPTH * kStreamWaves) {
 #pragma unroll
         for (int d = 0; d < DEPTH; ++d) {
-            if (b + d * waves < a.blocks) {
+            if (b + d * kStreamWaves < a.blocks) {
                 Stage& s = st[d];
+                const float scale = s.sx * s.sw;
+                const v8i xv = join(s.x[0], s.x[1]);
 #pragma unroll
-                for (int i = 0; i < MT; ++i) {
-                    const float scale = s.sx[i] * s.sw;
-                    const v8i xv = join(s.x[i][0], s.x[i][1]);
+                for (int t = 0; t < NT; ++t) {
+                    const v4f p = block_product(join(s.w[t][0], s.w[t][1]), xv);
 #pragma unroll
-                    for (int t = 0; t < NT; ++t) {
-                        const v4f p = block_product(join(s.w[t][0], s.w[t][1]), xv);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) acc[t][i][e] = fmaf(scale, p[e], acc[t][i][e]);
-                    }
+                    for (int e = 0; e < 4; ++e) acc[t][e] = fmaf(scale, p[e], acc[t][e]);
                 }
-                load(s, b + (d + DEPTH) * waves);
+                load(s, b + (d + DEPTH) * kStreamWaves);
             }
         }
     }
 
-    v4f* mine = reinterpret_cast<v4f*>(sums) + lane;
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int i = 0; i < MT; ++i) mine[(wave * NT * MT + t * MT + i) * 64] = acc[t][i];
+    for (int t = 0; t < NT; ++t) sums[wave][t][lane] = acc[t];
     __syncthreads();
-    for (int p = wave; p < NT * MT; p += waves) {
-        v4f v = mine[p * 64];
-        for (int o = 1; o < waves; ++o) v += mine[(o * NT * MT + p) * 64];
-        const int t = p / MT, i = p % MT, m = m0 + 16 * i + row;
-        if (tile0 + t < w.tiles && m < a.m) store4(a, w, m, (tile0 + t) * 16 + quarter * 4, v);
+    if (wave < NT && tile0 + wave < w.tiles && row < a.m) {
+        v4f v = sums[0][wave][lane];
+        for (int o = 1; o < kStreamWaves; ++o) v += sums[o][wave][lane];
+        store4(a, w, row, (tile0 + wave) * 16 + quarter * 4, v);
     }
 }
 
@@ -191,11 +171,11 @@ __global__ __launch_bounds__(512) void block_stream_kernel(BlockGemmArgs a) {
 // while the block before is multiplied.
 //
 // LDS order: weights as they were laid out, 16 bytes per lane in lane order.  x: of
-// a tile of 16 rows and half block 64 slots of 16 bytes, row r's chunk q at slot
-// 4 r + (q ^ turn(r)); four neighbouring lanes of the load then take one 64-byte
-// segment of a row, and the lanes that read a fragment together lie on different banks.
+// a tile of 16 rows 128 slots of 16 bytes, row r's chunk c at slot 8 r + (c ^ turn(r)):
+// eight neighbouring lanes of a load take one line of a row, and eight rows (in 128
+// bytes of banks) or sixteen (in 256) that read a chunk together lie on different banks.
 // ---------------------------------------------------------------------------
-__device__ __forceinline__ int turn(int r) { return (r >> 2 & 1) * 2 + (r >> 3); }
+__device__ __forceinline__ int turn(int r) { return (r >> 1 & 3) | ((r ^ r >> 3) & 1) << 2; }
 
 typedef __attribute__((address_space(3))) void lds_void_t;
 typedef const __attribute__((address_space(1))) void global_void_t;
@@ -203,22 +183,25 @@ typedef const __attribute__((address_space(1))) void global_void_t;
 // s_waitcnt vmcnt(n), the other counters left alone
 constexpr int vm_waits(int n) { return (n & 0xF) | (0x7 << 4) | (0xF << 8) | ((n >> 4) << 14); }
 
-template <int NTW, int MTW, int WN, int WM, int S, int EU>
-__global__ __launch_bounds__(WN * WM * 64) __attribute__((amdgpu_waves_per_eu(EU, EU)))
+template <int NTW, int MTW, int WN, int WM, int S, int G, int EU>
+__global__ __launch_bounds__(G * WN * WM * 64) __attribute__((amdgpu_waves_per_eu(EU, EU)))
 void block_tile_kernel(BlockGemmArgs a) {
-    constexpr int W = WN * WM, N = NTW * WN, M = MTW * WM;  // tiles of 16
+    constexpr int W = WN * WM, N = NTW * WN, M = MTW * WM;  // waves of a group; tiles of 16
     static_assert(8 % NTW == 0, "a wave's columns share a scale");
-    static_assert(2 * M % W == 0 && 2 * N % W == 0 && M % 4 == 0 && S >= 2 && S <= 4, "loads are shared out evenly");
-    // A stage is x, w and the rows' scales.  Each is an object of its own: a load into one
-    // then does not wait for reads of another.
-    constexpr int kW = M * kBlockBytes, kScales = kW + N * kBlockBytes, kStage = kScales + M * 64;
-    __shared__ __attribute__((aligned(1024))) uint8_t stage0[kStage], stage1[kStage], stage2[kStage], stage3[kStage];
+    static_assert(2 * M % W == 0 && 2 * N % W == 0 && S >= 2 && S <= 4, "loads are shared out evenly");
+    // A stage is x, w and the rows' scales of G blocks, one per group.  Each is an object of
+    // its own: a load into one then does not wait for reads of another.
+    constexpr int kW = M * kBlockBytes, kScales = kW + N * kBlockBytes, kStage = kScales + W * 256;
+    __shared__ __attribute__((aligned(1024))) uint8_t stage0[G * kStage], stage1[G * kStage], stage2[G * kStage], stage3[G * kStage];
     auto stage_of = [&](auto stage) -> uint8_t* {
         constexpr int P = decltype(stage)::value;
         if constexpr (P == 0) return stage0; else if constexpr (P == 1) return stage1; else if constexpr (P == 2) return stage2; else return stage3;
     };
     constexpr int kLoads = 2 * M / W + 2 * N / W + 1;  // to LDS, per wave and block
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    constexpr int kScaleRows = 16 * M / W, kScaleLanes = 64 / kScaleRows;  // whose scales a wave loads, lanes for each
+    static_assert(64 % kScaleRows == 0 && kScaleRows >= 16, "");
+    const int lane = threadIdx.x & 63, wave_of_all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wave = wave_of_all % W, k_group = wave_of_all / W;
     const int quarter = lane >> 4, row = lane & 15;
     const int wn = wave % WN, wm = wave / WN;
 
@@ -243,11 +226,12 @@ void block_tile_kernel(BlockGemmArgs a) {
     // Every tile of rows has a buffer of its own, moved on by the block: what a lane
     // adds to it is one number.  Rows past the last, columns past K and blocks past
     // the last read as zero.
-    const int load_row = lane >> 2, load_chunk = (lane & 3) ^ turn(load_row);
-    const uint32_t x_at = (uint32_t)(load_row * a.ldx) + 16u * load_chunk, w_at = lane * 16;
-    const int x_columns = a.k - 16 * load_chunk;
-    const int scale_part = wave % (M / 4);
-    const float* sx = a.x_scales + (int64_t)min(m0 + scale_part * 64 + lane, a.m - 1) * a.scale_row;
+    const int load_row = lane >> 3;  // of a tile's first half, or second
+    const int load_chunk[2] = {(lane & 7) ^ turn(load_row), (lane & 7) ^ turn(load_row + 8)};
+    const uint32_t w_at = lane * 16;
+    const uint32_t x_at[2] = {(uint32_t)(load_row * a.ldx) + 16u * load_chunk[0], (uint32_t)((load_row + 8) * a.ldx) + 16u * load_chunk[1]};
+    const int x_columns[2] = {a.k - 16 * load_chunk[0], a.k - 16 * load_chunk[1]};
+    const float* sx = a.x_scales + (int64_t)min(m0 + wave * kScaleRows + lane / kScaleLanes, a.m - 1) * a.scale_row;
     // per load of a wave: its tile's start, and its extent
     constexpr int kX = M % W == 0 ? M / W : 1, kWt = N % W == 0 ? N / W : 1;  // tiles a wave loads (or half of)
     const uint8_t *x_from[kX], *w_from[kWt];
@@ -267,11 +251,11 @@ void block_tile_kernel(BlockGemmArgs a) {
     const int blocks = a.blocks;
     const int64_t scale_group = a.scale_group;
     auto dma = [&](int b, auto stage) {
-        uint8_t* to = stage_of(stage);
+        uint8_t* to = stage_of(stage) + k_group * kStage;
         __attribute__((address_space(3))) uint8_t* xl = (__attribute__((address_space(3))) uint8_t*)(void*)to;
         __attribute__((address_space(3))) uint8_t* wl = xl + kW;
         const int k = b * kScaleBlock;
-        const uint32_t off[2] = {k < x_columns ? x_at : kPastEnd, k + 64 < x_columns ? x_at + 64 : kPastEnd};
+        const uint32_t off[2] = {k < x_columns[0] ? x_at[0] : kPastEnd, k < x_columns[1] ? x_at[1] : kPastEnd};
 #pragma unroll
         for (int p = 0; p < kX; ++p) {
             const __amdgpu_buffer_rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc(
@@ -296,10 +280,10 @@ void block_tile_kernel(BlockGemmArgs a) {
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(wr, (lds_void_t*)(wl + wave * 1024), 16, w_at + (wave & 1) * 1024, 0, 0, 0);
             }
         }
-        // 64 rows' scales per wave; waves past the rows repeat (a branch would split the
-        // loop's body, and the compiler then moves sums across the parts)
+        // (each scale by neighbouring lanes, one access where a row's scales lie together; by
+        // some of the lanes alone, under a branch, the 333 rows below take 11.2 us, not 9.7)
         __builtin_amdgcn_global_load_lds((global_void_t*)(sx + (int64_t)min(b, blocks - 1) * scale_group),
-                                         (lds_void_t*)(xl + kScales + scale_part * 256), 4, 0, 0);
+                                         (lds_void_t*)(xl + kScales + wave * 256), 4, 0, 0);
     };
 
     v4f acc[NTW][MTW];
@@ -310,19 +294,22 @@ void block_tile_kernel(BlockGemmArgs a) {
     // (the constant address space: one scalar load per wave)
     const __attribute__((address_space(4))) float* sw = (const __attribute__((address_space(4))) float*)(
         w.scales + (int64_t)(min(tile0 + wn * NTW, w.tiles - 1) >> 3) * a.blocks);
-    const uint32_t x_slot = (uint32_t)(wm * MTW * kBlockBytes) + (uint32_t)(4 * row + (quarter ^ turn(row))) * 16;
+    const uint32_t x_slot = (uint32_t)(wm * MTW * kBlockBytes) + (uint32_t)(8 * row + (quarter ^ turn(row))) * 16;
+    const uint32_t x_half = x_slot ^ 64;  // of its second half block
     const uint32_t w_slot = (uint32_t)(wn * NTW * kBlockBytes) + lane * 16;
+    const uint32_t s_slot = (uint32_t)(wm * MTW * 16 + row) * kScaleLanes;  // row r is lane r * kScaleLanes of all waves' loads
     auto fragment = [](const uint8_t* at) {
         return join(*reinterpret_cast<const u32x4_dev_t*>(at), *reinterpret_cast<const u32x4_dev_t*>(at + 1024));
     };
 
     // A product is added to its sum kLag products later, in the shadow of theirs.
     constexpr int kLag = 2;
-    // S - 1 blocks are on their way.  A step begins where its block has landed and
-    // every wave is done with the block before, into whose place the next load goes.
-    auto step = [&](int b, auto stage) {
+    // S - 1 steps' blocks are on their way.  A step begins where its blocks have landed and
+    // every wave is done with the step before, into whose place the next load goes.
+    auto step = [&](int at, auto stage) {
         constexpr int P = decltype(stage)::value;
-        const uint8_t *xs = stage_of(stage), *ws = xs + kW;
+        const int b = at * G + k_group;
+        const uint8_t *xs = stage_of(stage) + k_group * kStage, *ws = xs + kW;
         const float* ss = reinterpret_cast<const float*>(xs + kScales);
         float scale[MTW];
         v8i xv[MTW], wv[2];
@@ -330,14 +317,22 @@ void block_tile_kernel(BlockGemmArgs a) {
         __builtin_amdgcn_s_waitcnt(vm_waits((S - 2) * kLoads));
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
-        const float block_scale = sw[b];
+        const float block_scale = sw[G == 1 ? b : min(b, blocks - 1)];
 #pragma unroll
-        for (int i = 0; i < MTW; ++i) xv[i] = fragment(xs + x_slot + i * kBlockBytes);
+        for (int i = 0; i < MTW; ++i) 
+            xv[i] = join(*reinterpret_cast<const u32x4_dev_t*>(xs + x_slot + i * kBlockBytes),
+                         *reinterpret_cast<const u32x4_dev_t*>(xs + x_half + i * kBlockBytes));
         wv[0] = fragment(ws + w_slot);
 #pragma unroll
-        for (int i = 0; i < MTW; ++i) scale[i] = ss[(wm * MTW + i) * 16 + row] * block_scale;
+        for (int i = 0; i < MTW; ++i) {
+            scale[i] = ss[s_slot + i * 16 * kScaleLanes] * block_scale;
+            if constexpr (G > 1) {  // groups past the last block add products of zeros under scale 0
+                asm("" : "+v"(scale[i]));
+                scale[i] = b < blocks ? scale[i] : 0.0f;
+            }
+        }
         __builtin_amdgcn_sched_barrier(0);
-        dma(b + S - 1, std::integral_constant<int, (P + S - 1) % S>{});
+        dma(b + (S - 1) * G, std::integral_constant<int, (P + S - 1) % S>{});
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int q = 0; q < NTW * MTW + kLag; ++q) {
@@ -358,7 +353,7 @@ void block_tile_kernel(BlockGemmArgs a) {
 #pragma unroll
             for (int i = 0; i < MTW; ++i) asm volatile("" : "+v"(acc[t][i]));
     };
-    auto first = [&](auto... stages) { (dma(decltype(stages)::value, stages), ...); };
+    auto first = [&](auto... stages) { (dma(decltype(stages)::value * G + k_group, stages), ...); };
     typedef std::integral_constant<int, 0> I0;
     typedef std::integral_constant<int, 1> I1;
     typedef std::integral_constant<int, 2> I2;
@@ -368,26 +363,47 @@ void block_tile_kernel(BlockGemmArgs a) {
     else first(I0{}, I1{}, I2{});
     // Whole rounds of the stages, then the rest: a loop of one exit, through which the
     // compiler follows which loads are on their way (with more it waits for all).
-    int b = 0;
-    for (; b + S <= blocks; b += S) {
-        step(b, I0{});
-        step(b + 1, I1{});
-        if constexpr (S > 2) step(b + 2, I2{});
-        if constexpr (S > 3) step(b + 3, I3{});
+    const int steps = (blocks + G - 1) / G;
+    int at = 0;
+    for (; at + S <= steps; at += S) {
+        step(at, I0{});
+        step(at + 1, I1{});
+        if constexpr (S > 2) step(at + 2, I2{});
+        if constexpr (S > 3) step(at + 3, I3{});
     }
-    if (b < blocks) step(b, I0{});
+    if (at < steps) step(at, I0{});
     if constexpr (S > 2) {
-        if (b + 1 < blocks) step(b + 1, I1{});
+        if (at + 1 < steps) step(at + 1, I1{});
     }
     if constexpr (S > 3) {
-        if (b + 2 < blocks) step(b + 2, I2{});
+        if (at + 2 < steps) step(at + 2, I2{});
     }
     __syncthreads();  // the last loads (of nothing) have landed, all is read
+    if constexpr (G > 1) {  // the groups' sums, in order
+        static_assert((G - 1) * W * NTW * MTW * 1024 <= G * kStage, "the other groups' sums fit a stage");
+        v4f* sums = reinterpret_cast<v4f*>(stage0) + wave * NTW * MTW * 64 + lane;
+        constexpr int kGroup = W * NTW * MTW * 64;
+        if (k_group) {
+#pragma unroll
+            for (int t = 0; t < NTW; ++t)
+#pragma unroll
+                for (int i = 0; i < MTW; ++i) sums[(k_group - 1) * kGroup + (t * MTW + i) * 64] = acc[t][i];
+        }
+        __syncthreads();
+        if (k_group) return;
+#pragma unroll
+        for (int t = 0; t < NTW; ++t)
+#pragma unroll
+            for (int i = 0; i < MTW; ++i)
+#pragma unroll
+                for (int g = 0; g + 1 < G; ++g) acc[t][i] += sums[g * kGroup + (t * MTW + i) * 64];
+    }
 
     // 16 rows at a time through a wave-private run of LDS, to leave in whole lines
     constexpr int kPitch = 16 * NTW + 4;  // of 32-bit sums
-    static_assert((W / 2) * 16 * kPitch * 4 <= kStage, "half of the waves per stage");
-    float* out = reinterpret_cast<float*>(wave & 1 ? stage1 : stage0) + (wave >> 1) * 16 * kPitch;
+    static_assert((G > 1 ? W : W / 2) * 16 * kPitch * 4 <= G * kStage, "the waves' rows fit one stage, or two");
+    float* out = G > 1 ? reinterpret_cast<float*>(stage1) + wave * 16 * kPitch
+                       : reinterpret_cast<float*>(wave & 1 ? stage1 : stage0) + (wave >> 1) * 16 * kPitch;
     const int n0 = (tile0 + wn * NTW) * 16;
 #pragma unroll
     for (int i = 0; i < MTW; ++i) {
@@ -426,32 +442,26 @@ __global__ __launch_bounds__(256) void block_prepare_kernel(const uint8_t* value
     }
 }
 
-template <int NT, int MT, int DEPTH>
-hipError_t launch_stream(const BlockGemmArgs& a, hipStream_t s) {
-    const dim3 grid(a.group_end[a.members - 1], (a.m + 16 * MT - 1) / (16 * MT));
-    block_stream_kernel<NT, MT, DEPTH><<<grid, a.waves * 64, a.waves * NT * MT * 1024, s>>>(a);
-    return hipGetLastError();
+// The members' column groups of so many tiles.
+unsigned count_groups(BlockGemmArgs& a, int tiles) {
+    unsigned groups = 0;
+    for (int j = 0; j < kMaxGemmMembers; ++j) {
+        if (j < a.members) groups += (a.member[j].tiles + tiles - 1) / tiles;
+        a.group_end[j] = (int)groups;
+    }
+    return groups;
 }
 
 template <int NT>
-hipError_t launch_stream_rows(const BlockGemmArgs& a, hipStream_t s) {
-    switch (a.row_tiles) {
-        case 1: return launch_stream<NT, 1, 4>(a, s);
-        case 2: return launch_stream<NT, 2, 2>(a, s);
-        default: return launch_stream<NT, 4, 2>(a, s);
-    }
+hipError_t launch_stream(BlockGemmArgs a, hipStream_t s) {
+    block_stream_kernel<NT, 4><<<count_groups(a, NT), kStreamWaves * 64, 0, s>>>(a);
+    return hipGetLastError();
 }
 
-template <int NTW, int MTW, int WN, int WM, int S, int EU>
-hipError_t launch_tile(const BlockGemmArgs& given, hipStream_t s) {
-    BlockGemmArgs a = given;
-    int64_t groups = 0;
-    for (int j = 0; j < kMaxGemmMembers; ++j) {
-        if (j < a.members) groups += (a.member[j].tiles + NTW * WN - 1) / (NTW * WN);
-        a.group_end[j] = (int)groups;
-    }
-    const unsigned grid = (unsigned)(groups * ((a.m + 16 * MTW * WM - 1) / (16 * MTW * WM)));
-    block_tile_kernel<NTW, MTW, WN, WM, S, EU><<<grid, WN * WM * 64, 0, s>>>(a);
+template <int NTW, int MTW, int WN, int WM, int S, int G, int EU>
+hipError_t launch_tile(BlockGemmArgs a, hipStream_t s) {
+    const unsigned grid = count_groups(a, NTW * WN) * ((a.m + 16 * MTW * WM - 1) / (16 * MTW * WM));
+    block_tile_kernel<NTW, MTW, WN, WM, S, G, EU><<<grid, G * WN * WM * 64, 0, s>>>(a);
     return hipGetLastError();
 }
 
@@ -459,16 +469,18 @@ hipError_t launch_tile(const BlockGemmArgs& given, hipStream_t s) {
 
 hipError_t launch_block_gemm(const BlockGemmArgs& a, hipStream_t s) {
     switch (a.tile) {
-        case 1: return launch_tile<2, 2, 2, 2, 3, 3>(a, s);
-        case 2: return launch_tile<4, 2, 2, 2, 3, 2>(a, s);
-        case 3: return launch_tile<8, 4, 2, 4, 2, 2>(a, s);
+        case 1: return launch_tile<2, 2, 2, 2, 3, 1, 3>(a, s);
+        case 2: return launch_tile<4, 2, 2, 2, 3, 1, 2>(a, s);
+        case 3: return launch_tile<4, 4, 4, 2, 3, 1, 2>(a, s);
+        case 4: return launch_tile<8, 4, 2, 4, 2, 1, 2>(a, s);
+        case 5: return launch_tile<2, 2, 2, 2, 4, 2, 2>(a, s);
         default: break;
     }
-    switch (a.col_tiles) {
-        case 1: return launch_stream_rows<1>(a, s);
-        case 2: return launch_stream_rows<2>(a, s);
-        default: return launch_stream_rows<4>(a, s);
-    }
+    // the more columns there are, the fewer times x is read
+    int64_t tiles = 0;
+    for (int j = 0; j < a.members; ++j) tiles += a.member[j].tiles;
+    if (tiles >= 2048) return launch_stream<4>(a, s);
+    return tiles >= 1024 ? launch_stream<2>(a, s) : launch_stream<1>(a, s);
 }
 
 hipError_t launch_block_prepare(const uint8_t* values, int64_t ld, int64_t n, int64_t k, uint8_t* out, hipStream_t s) {

@@ -795,19 +795,19 @@ int cubic_vocab_sample(const void* logits, int dtype, int64_t row_stride, int ro
 // ---------------------------------------------------------------------------
 namespace {
 int check_history(const cubic::HistoryArgs& h, const char* what) {
-    if (!h.marks || !h.biases || !h.listed || !h.sizes) return fail(CUBIC_EINVAL, "%s: null history", what);
+    if (!h.state || !h.listed || !h.sizes) return fail(CUBIC_EINVAL, "%s: null history", what);
     if (h.slots < 1 || h.slots >= (1 << 20) || h.vocab < 1 || h.vocab > cubic::kMaxHistoryVocab)
         return fail(CUBIC_EINVAL, "%s: history of %d slots, %d tokens", what, h.slots, h.vocab);
-    if (((uintptr_t)h.marks | (uintptr_t)h.biases | (uintptr_t)h.listed | (uintptr_t)h.sizes) % 4)
+    if ((uintptr_t)h.state % 8 || ((uintptr_t)h.listed | (uintptr_t)h.sizes) % 4)
         return fail(CUBIC_EINVAL, "%s: misaligned history", what);
     return CUBIC_OK;
 }
 }  // namespace
 
-int cubic_history_append(uint32_t* marks, float* biases, int32_t* listed, int32_t* sizes, int slots, int vocab,
+int cubic_history_append(uint32_t* state, int32_t* listed, int32_t* sizes, int slots, int vocab,
                          const int32_t* row_slots, const void* tokens, int token_bytes, int64_t ld, int rows,
                          int length, int prompt, int live_rows, const int32_t* live_count, void* stream) {
-    const cubic::HistoryArgs h = {marks, biases, listed, sizes, slots, vocab};
+    const cubic::HistoryArgs h = {(uint2*)state, listed, sizes, slots, vocab};
     if (const int status = check_history(h, "history append")) return status;
     if (!row_slots || !tokens) return fail(CUBIC_EINVAL, "history append: null operand");
     if (token_bytes != 4 && token_bytes != 8) return fail(CUBIC_EINVAL, "history tokens must be int32 or int64");
@@ -820,9 +820,9 @@ int cubic_history_append(uint32_t* marks, float* biases, int32_t* listed, int32_
     return hip_status(cubic::launch_history_append(h, a, (hipStream_t)stream), "history append launch");
 }
 
-int cubic_history_clear(uint32_t* marks, float* biases, int32_t* listed, int32_t* sizes, int slots, int vocab,
+int cubic_history_clear(uint32_t* state, int32_t* listed, int32_t* sizes, int slots, int vocab,
                         const int32_t* row_slots, int rows, int slot, int biases_only, void* stream) {
-    const cubic::HistoryArgs h = {marks, biases, listed, sizes, slots, vocab};
+    const cubic::HistoryArgs h = {(uint2*)state, listed, sizes, slots, vocab};
     if (const int status = check_history(h, "history clear")) return status;
     if (!row_slots && (slot < 0 || slot >= slots)) return fail(CUBIC_EINVAL, "history slot %d outside 0..%d", slot, slots - 1);
     if (rows < 1 || rows >= (1 << 24)) return fail(CUBIC_EINVAL, "history clear: rows=%d", rows);
@@ -830,9 +830,9 @@ int cubic_history_clear(uint32_t* marks, float* biases, int32_t* listed, int32_t
                       "history clear launch");
 }
 
-int cubic_history_bias(uint32_t* marks, float* biases, int32_t* listed, int32_t* sizes, int slots, int vocab,
+int cubic_history_bias(uint32_t* state, int32_t* listed, int32_t* sizes, int slots, int vocab,
                        int slot, const int32_t* ids, const float* values, int count, void* stream) {
-    const cubic::HistoryArgs h = {marks, biases, listed, sizes, slots, vocab};
+    const cubic::HistoryArgs h = {(uint2*)state, listed, sizes, slots, vocab};
     if (const int status = check_history(h, "history bias")) return status;
     if (!ids || !values) return fail(CUBIC_EINVAL, "history bias: null operand");
     if (slot < 0 || slot >= slots) return fail(CUBIC_EINVAL, "history slot %d outside 0..%d", slot, slots - 1);
@@ -841,19 +841,19 @@ int cubic_history_bias(uint32_t* marks, float* biases, int32_t* listed, int32_t*
 }
 
 int cubic_logit_penalties(const void* logits, int dtype, int64_t row_stride, int sequences, int depth, int width,
-                          int live_sequences, const int32_t* live_count, uint32_t* marks, float* biases,
+                          int live_sequences, const int32_t* live_count, uint32_t* state,
                           int32_t* listed, int32_t* sizes, int slots, int vocab, const int32_t* row_slots,
                           const float* repetition, const float* presence, const float* frequency,
                           const int64_t* drafts, const int32_t* mask, int64_t mask_words, void* out, int out_dtype,
                           int64_t out_stride, void* stream) {
-    const cubic::HistoryArgs h = {marks, biases, listed, sizes, slots, vocab};
+    const cubic::HistoryArgs h = {(uint2*)state, listed, sizes, slots, vocab};
     if (const int status = check_history(h, "logit penalties")) return status;
     if (!logits || !row_slots || !out) return fail(CUBIC_EINVAL, "logit penalties: null operand");
     if (dtype != CUBIC_DTYPE_BF16 && dtype != CUBIC_DTYPE_F16 && dtype != CUBIC_DTYPE_F32)
         return fail(CUBIC_EINVAL, "logit penalties: dtype must be CUBIC_DTYPE_BF16, _F16 or _F32");
     if (out_dtype != dtype && out_dtype != CUBIC_DTYPE_F32)
         return fail(CUBIC_EINVAL, "logit penalties: outputs have the logits' type or 32 bits");
-    if (sequences < 1 || depth < 0 || depth > cubic::kMaxPenaltyDepth || (int64_t)sequences * (depth + 1) >= (1 << 24))
+    if (sequences < 1 || depth < 0 || depth > cubic::kMaxPenaltyDepth || (int64_t)sequences * (depth + 1) >= (1 << 22))
         return fail(CUBIC_EINVAL, "logit penalties: sequences=%d depth=%d", sequences, depth);
     if (width < 1 || width > vocab) return fail(CUBIC_EINVAL, "logit penalties: width %d outside the history's 1..%d", width, vocab);
     const int64_t rows = (int64_t)sequences * (depth + 1), most = (int64_t)1 << 40;
@@ -1044,19 +1044,24 @@ int cubic_block_gemm(const void* x, int64_t ldx, const float* x_scales, int64_t 
                        ((uintptr_t)ys[j] & (4 * element - 1)) == 0 && (m == 1 || ldys[j] % 4 == 0)};
         tiles += a.member[j].tiles;
     }
-    a.row_tiles = m <= 16 ? 1 : m <= 32 ? 2 : 4;
-    a.col_tiles = tiles >= 2048 ? 4 : tiles >= 1024 ? 2 : 1;
-    a.waves = a.col_tiles * a.row_tiles >= 16 ? 4 : 8;
-    // Tiles (columns x rows) of 256 x 256 where they fill the chip, else 128 x 64 where
-    // those do, else 64 x 64.  4096 x 8192 x 8192 258, 393 and 562 us; 1024 rows of it at K = 4096
-    // 65, 55 and 73; 512 x 4096 x 4096 61, 18.9 and 21.8; 256 x 4096 x 12288 171, 44 and 34.
-    // The stream kernel up to 16 rows: 16 x 6144 x 4096 12.4 and 11.2 in tiles, 1 row 6.5.
-    a.tile = m <= 16 ? 0 : m > 128 && ceil_div(tiles, 16) * ceil_div(m, 256) >= 256 ? 3 : ceil_div(tiles, 8) * ceil_div(m, 64) >= 256 ? 2 : 1;
-
-    int64_t groups = 0;
-    for (int j = 0; j < cubic::kMaxGemmMembers; ++j) {
-        if (j < members) groups += ceil_div(a.member[j].tiles, a.col_tiles);
-        a.group_end[j] = (int)groups;
+    // Up to 8 rows the stream kernel, else the tiles (columns x rows) whose rounds over 256
+    // CUs are expected to end first, by what a block of K takes a round, in hundredths of a us:
+    //   64 x 64 27, 128 x 64 36 and 10 more, 256 x 128 120, 256 x 256 200
+    // 4096 x 8192 x 8192: 548, 371, 292 and 249 us; 1024 rows x 8192 x 4096: 72, 53, 42 and 61; 512 x
+    // 4096 x 4096: 21, 18.6, - and 57; 256 x 4096 x 12288: 34, 43, - and 153.  64 x 64 tiles that one
+    // round holds have two groups of waves, each every other block of K: 256 x 4096 x 12288 30
+    // and 34 us, 64 x 6144 x 4096 11.2 and 11.7, 333 x 1024 x 2064 8.2 and 8.0.  Rows of 6144 x 4096,
+    // stream and tiles: 1 6.5 and 10.4, 8 10.3 and 10.4, 16 12.5 and 10.6.
+    auto rounds = [&](int columns, int rows) {
+        int64_t groups = 0;
+        for (int j = 0; j < members; ++j) groups += ceil_div(ns[j], columns);
+        return ceil_div(groups * ceil_div(m, rows), 256);
+    };
+    if (m > 8) {
+        const int64_t small = rounds(64, 64);
+        const int64_t cost[] = {27 * small, 10 + 36 * rounds(128, 64), 120 * rounds(256, 128), 200 * rounds(256, 256)};
+        a.tile = 1 + (int)(std::min_element(cost, cost + 4) - cost);
+        if (a.tile == 1 && small == 1 && a.blocks >= 24) a.tile = 5;
     }
     if (a.tile && ceil_div(tiles, 4) * ceil_div(m, 64) >= (1 << 22))
         return fail(CUBIC_ENOTSUP, "block gemm: more tiles than one launch holds");

@@ -344,8 +344,7 @@ constexpr int kMaxHistoryVocab = 1 << 24;
 constexpr int kHistoryBucket = 4096;  // tokens of the vocabulary that share a list
 constexpr int history_buckets(int vocab) { return (vocab + kHistoryBucket - 1) / kHistoryBucket; }
 struct HistoryArgs {
-    uint32_t* marks;              // [slots, vocab]: outputs counted | 2^30 listed | 2^31 in the prompt
-    float* biases;                // [slots, vocab], 0 unless listed
+    uint2* state;                 // [slots, vocab]: outputs counted | 2^30 listed | 2^31 in the prompt; the bias' bits
     int32_t* listed;              // [slots, vocab]: of bucket b from b * kHistoryBucket on the listed tokens
     int32_t* sizes;               // [slots, buckets]: how many
     int slots, vocab;
@@ -393,9 +392,9 @@ struct BlockGemmArgs {
     int64_t ldx, scale_row, scale_group;
     int m, k, blocks, members;
     int out;                      // CUBIC_DTYPE_* of y
-    int tile;                     // 0: the stream kernel; 1: 128 x 128 tiles, 2: 256 x 256
-    int col_tiles, row_tiles, waves;  // per workgroup
-    int group_end[kMaxGemmMembers];   // ends of the members' column groups
+    int tile;                     // 0: the stream kernel (up to 16 rows); tiles of 1: 64 x 64, 2: 128 x 64, 3: 256 x 128, 4: 256 x 256
+                                  // columns x rows, 5: 64 x 64 by two groups of waves
+    int group_end[kMaxGemmMembers];   // ends of the members' column groups (set at launch)
     BlockMember member[kMaxGemmMembers];
 };
 hipError_t launch_block_gemm(const BlockGemmArgs& a, hipStream_t s);

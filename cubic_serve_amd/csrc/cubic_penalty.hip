@@ -9,15 +9,20 @@
 // in 32 bits, in this order, each step rounded (an unfused plain form has the same
 // bits), and once to the output's type.
 //
-// A history keeps per slot a table of marks (outputs counted, in the prompt,
-// listed), a table of biases, and for every kHistoryBucket tokens of the vocabulary a list
+// A history keeps per slot a table of each token's mark (outputs counted, in the
+// prompt, listed) and bias, and for every kHistoryBucket tokens of the vocabulary a list
 // of those that have either.  A list's order is that of atomics; nothing depends on
 // it, since each listed token is taken by itself.
 //
 // What bounds the penalties: reading and writing the logits.  Listed tokens are a few
 // thousand of 10^5 columns, so each is looked up by itself, by the workgroup that has
-// its column: it reads the lists of its own columns only (one list per slot, which every
-// workgroup of a row has to search, took 95 us where this takes 50: 256 rows of 151936).
+// its column: it reads the lists of its own columns only, and changes their logits in
+// LDS on their way.  256 rows of 151936, 3700 tokens listed for each: 44 us (48 under a
+// grammar), where a copy takes 31 and a history of no tokens 36; with listed tokens
+// changed in memory after the rest 69 (a grammar admits 2 % of them: 50), with
+// one list per slot, which every workgroup of a row has to search, 95.  Four rows of
+// a sequence one after the other in a workgroup, for their common list: 81 (too few
+// loads on their way).
 #include <type_traits>
 
 #include "cubic_capi_internal.h"
@@ -32,7 +37,7 @@ constexpr int kThreads = 256;
 // Puts a token on its bucket's list unless it is there.
 __device__ __forceinline__ void list_token(const HistoryArgs& h, int64_t slot, int t, uint32_t mark) {
     if (mark & kListed) return;
-    if (atomicOr(&h.marks[slot * h.vocab + t], kListed) & kListed) return;
+    if (atomicOr(&h.state[slot * h.vocab + t].x, kListed) & kListed) return;
     const int bucket = t / kHistoryBucket;
     const int at = atomicAdd(&h.sizes[slot * history_buckets(h.vocab) + bucket], 1);
     h.listed[slot * h.vocab + bucket * kHistoryBucket + at] = t;
@@ -46,7 +51,7 @@ __global__ __launch_bounds__(kThreads) void history_append_kernel(HistoryArgs h,
         const int64_t t = a.token_bytes == 8 ? static_cast<const int64_t*>(a.tokens)[at] : static_cast<const int32_t*>(a.tokens)[at];
         const int slot = a.row_slots[row];
         if (slot < 0 || slot >= h.slots || t < 0 || t >= h.vocab) continue;
-        uint32_t* mark = &h.marks[(int64_t)slot * h.vocab + t];
+        uint32_t* mark = &h.state[(int64_t)slot * h.vocab + t].x;
         const uint32_t old = a.prompt ? atomicOr(mark, kPrompt) : atomicAdd(mark, 1u);
         list_token(h, slot, (int)t, old);
     }
@@ -66,8 +71,8 @@ __global__ __launch_bounds__(1024) void history_clear_kernel(HistoryArgs h, cons
             const int n = min(*size, min(kHistoryBucket, h.vocab - b * kHistoryBucket));
             for (int i = lane; i < n; i += 64) {
                 const int t = h.listed[base + b * kHistoryBucket + i];
-                h.biases[base + t] = 0.0f;
-                if (!biases_only) h.marks[base + t] = 0;
+                h.state[base + t].y = 0;
+                if (!biases_only) h.state[base + t].x = 0;
             }
             if (!biases_only && lane == 0 && n) *size = 0;
         }
@@ -79,7 +84,7 @@ __global__ __launch_bounds__(kThreads) void history_bias_kernel(HistoryArgs h, i
     if (i >= n) return;
     const int t = ids[i];
     if (t < 0 || t >= h.vocab) return;
-    h.biases[(int64_t)slot * h.vocab + t] = values[i];
+    h.state[(int64_t)slot * h.vocab + t].y = __float_as_uint(values[i]);
     list_token(h, slot, t, 0);
 }
 
@@ -166,17 +171,6 @@ __device__ __forceinline__ void keep8(Eight<TYPE>& v, uint32_t bits, uint32_t ot
     }
 }
 template <int TYPE>
-__device__ __forceinline__ Eight<TYPE> load_some(const void* p, int64_t i, uint32_t some) {
-    Eight<TYPE> v = {};
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-        if (some >> e & 1) {
-            if constexpr (TYPE == 2) v.u[e] = static_cast<const uint32_t*>(p)[i + e];
-            else v.u[e >> 1] |= (uint32_t)static_cast<const uint16_t*>(p)[i + e] << (16 * (e & 1));
-        }
-    return v;
-}
-template <int TYPE>
 __device__ __forceinline__ void store_some(void* p, int64_t i, const Eight<TYPE>& v, uint32_t some) {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
@@ -190,93 +184,150 @@ constexpr uint32_t minus_infinity() { return TYPE == 2 ? 0xFF800000u : TYPE == 1
 template <int TYPE>
 constexpr uint32_t not_a_number() { return TYPE == 2 ? 0x7FC00000u : TYPE == 1 ? 0x7E007E00u : 0x7FC07FC0u; }
 
-// A (row, chunk of columns) per workgroup and turn: the chunk goes from logits to outputs
-// with the mask applied, eight columns per thread and access (in place: masked columns
-// are written, no other); then, those stores done, listed tokens are written one by
-// one from the logits.  A token whose bit is 0 is left to the mask.
+// A (row, chunk of columns) per workgroup.
+// Out of place: the chunk goes from logits to outputs through registers, eight columns
+// per thread and access, and where its columns have listed tokens or drafts through
+// LDS, in the output's type (16 KB), where those are changed; then the mask is applied.
+// A last vector that the columns do not fill starts earlier, over columns that another
+// thread writes too, with the same values.
+// In place (INPLACE): listed tokens and masked columns are written by themselves. A
+// token whose bit is 0 is left to the mask, so no column is written with two values.
 template <int IN, int OUT, bool INPLACE>
-__global__ __launch_bounds__(kThreads) void penalty_kernel(PenaltyArgs a) {
+// (eight waves per SIMD: with four the copy alone takes 45 us)
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(8, 8))) void penalty_kernel(PenaltyArgs a) {
     constexpr int kChunk = kPenaltyBytes / (OUT == 2 ? 4 : 2), kTurns = kChunk / (8 * kThreads), kLists = kChunk / kHistoryBucket;
     static_assert(kChunk % kHistoryBucket == 0, "a list is one workgroup's");
+    __shared__ __attribute__((aligned(16))) uint8_t staged[INPLACE ? 16 : kPenaltyBytes];
+    __shared__ int drafts[kMaxPenaltyDepth];
+    // (all rows' first chunks first: vocabularies begin with the tokens that come often, so
+    // those have the long lists and should not come last)
+    const int row = blockIdx.x, chunk = blockIdx.y;
     const int live = a.live_count ? min(max(*a.live_count, 0), a.live_sequences) : a.live_sequences;
-    const int64_t items = (int64_t)live * (a.depth + 1) * a.chunks;
     const int buckets = history_buckets(a.history.vocab);
-    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-        const int row = (int)(item / a.chunks), chunk = (int)(item - (int64_t)row * a.chunks);
-        const int sequence = row / (a.depth + 1), ahead = row - sequence * (a.depth + 1);
-        const int c0 = chunk * kChunk, columns = min(kChunk, a.width - c0);
-        const uint32_t* mask = a.mask ? a.mask + (int64_t)row * a.mask_words : nullptr;
-        const int64_t in_row = (int64_t)row * a.ld, out_row = (int64_t)row * a.ldout;
-        const int slot = a.row_slots[sequence];
-        const Settings s = settings_of(a, sequence);
-        const bool known = s.valid && slot >= 0 && slot < a.history.slots;
-        const int64_t base = known ? (int64_t)slot * a.history.vocab : 0;
-        int sizes[kLists];
-#pragma unroll
-        for (int l = 0; l < kLists; ++l) {
-            const int bucket = c0 / kHistoryBucket + l;
-            sizes[l] = known && bucket < buckets ? a.history.sizes[(int64_t)slot * buckets + bucket] : 0;
-        }
+    const int sequence = row / (a.depth + 1), ahead = row - sequence * (a.depth + 1);
+    if (sequence >= live) return;
+    const int c0 = chunk * kChunk, columns = min(kChunk, a.width - c0);
+    const uint32_t* mask = a.mask ? a.mask + (int64_t)row * a.mask_words : nullptr;
+    const int64_t in_at = (int64_t)row * a.ld + c0, out_at = (int64_t)row * a.ldout + c0;
+    const bool whole = columns >= 8;  // else one column per thread
+    auto start = [&](int i) { return min((i * kThreads + (int)threadIdx.x) * 8, columns - 8); };
+    auto mine = [&](int i) { return whole && (i * kThreads + (int)threadIdx.x) * 8 < columns; };
+    auto bits_of = [&](int c) -> uint32_t {  // of eight columns, at any place of the mask's bytes
+        if (!mask) return 0xFFu;
+        const int first = c0 + c, byte = min(first >> 3, (int)min(a.mask_words, (int64_t)1 << 28) * 4 - 2);
+        uint16_t two;
+        __builtin_memcpy(&two, reinterpret_cast<const uint8_t*>(mask) + byte, 2);
+        return (uint32_t)two >> (first - 8 * byte) & 0xFFu;
+    };
 
-        if (!INPLACE || mask || !s.valid) {
-            const uint32_t other = s.valid ? minus_infinity<OUT>() : not_a_number<OUT>();
+    int64_t draft = -1;
+    if ((int)threadIdx.x < ahead) draft = a.drafts[(int64_t)threadIdx.x * a.sequences + sequence] - c0;
+    const int slot = a.row_slots[sequence];
+    const bool slotted = slot >= 0 && slot < a.history.slots;
+    const int64_t base = slotted ? (int64_t)slot * a.history.vocab : 0;
+    const uint2* state = a.history.state + base + c0;
+    const int32_t* listed = a.history.listed + base + c0;
+    // Each thread's first token of every list, and what is kept of it, before it is
+    // known how many there are: a place past a list's end holds an older token, or 0.
+    int early[kLists];
+    uint2 early_of[kLists];
 #pragma unroll
-            for (int i = 0; i < kTurns; ++i) {
-                const int c = (i * kThreads + (int)threadIdx.x) * 8;
-                if (c >= columns) break;
-                const uint32_t bits = !s.valid ? 0u : mask ? reinterpret_cast<const uint8_t*>(mask)[(c0 + c) >> 3] : 0xFFu;
-                const uint32_t all = columns - c >= 8 ? 0xFFu : (1u << (columns - c)) - 1;
-                Eight<OUT> out = {};
-                if constexpr (INPLACE) {
-                    keep8<OUT>(out, 0u, other);
-                    if ((all & ~bits) == 0xFFu) store8<OUT>(a.out, out_row + c0 + c, out);
-                    else store_some<OUT>(a.out, out_row + c0 + c, out, all & ~bits);
-                } else if (all == 0xFFu) {
-                    out = to_type<IN, OUT>(load8<IN>(a.logits, in_row + c0 + c));
-                    keep8<OUT>(out, bits, other);
-                    store8<OUT>(a.out, out_row + c0 + c, out);
-                } else {
-                    out = to_type<IN, OUT>(load_some<IN>(a.logits, in_row + c0 + c, all));
-                    keep8<OUT>(out, bits, other);
-                    store_some<OUT>(a.out, out_row + c0 + c, out, all);
-                }
-            }
+    for (int l = 0; l < kLists; ++l) {
+        const int at = l * kHistoryBucket + (int)threadIdx.x;
+        early[l] = slotted && c0 + at < a.history.vocab ? listed[at] - c0 : -1;
+    }
+    // all loads of the chunk before the first store: the compiler does not move a
+    // load up over a store that may be to its place
+    Eight<IN> in[kTurns] = {};
+    uint32_t bits[kTurns];
+#pragma unroll
+    for (int i = 0; i < kTurns; ++i) {
+        bits[i] = 0xFFu;
+        if (mine(i)) {
+            bits[i] = bits_of(start(i));
+            if constexpr (!INPLACE) in[i] = load8<IN>(a.logits, in_at + start(i));
         }
-        if (!known) continue;
-        if constexpr (!INPLACE) {  // two stores to one column follow each other
-            __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
-            __syncthreads();
+    }
+#pragma unroll
+    for (int l = 0; l < kLists; ++l) {
+        const bool in_chunk = early[l] >= 0 && early[l] < columns && admitted(mask, c0 + early[l]);
+        early[l] = in_chunk ? early[l] : -1;
+        early_of[l] = in_chunk ? state[early[l]] : make_uint2(0, 0);
+    }
+    const Settings s = settings_of(a, sequence);
+    const bool known = s.valid && slotted;
+    int sizes[kLists], some = known ? ahead : 0;
+#pragma unroll
+    for (int l = 0; l < kLists; ++l) {
+        const int bucket = c0 / kHistoryBucket + l;
+        sizes[l] = known && bucket < buckets ? min(a.history.sizes[(int64_t)slot * buckets + bucket], kHistoryBucket) : 0;
+        some += sizes[l];
+    }
+    if (some || !whole) {
+        if ((int)threadIdx.x < ahead) drafts[threadIdx.x] = draft >= 0 && draft < columns ? (int)draft : -1;  // columns of this chunk
+        if constexpr (!INPLACE) {
+#pragma unroll
+            for (int i = 0; i < kTurns; ++i)
+                if (mine(i)) store8<OUT>(staged, start(i), to_type<IN, OUT>(in[i]));
+            if (!whole && (int)threadIdx.x < columns)
+                set_value<OUT>(staged, threadIdx.x, value_of<IN>(a.logits, in_at + threadIdx.x));
         }
-        const uint32_t* marks = a.history.marks + base;
-        const int64_t* drafts = a.drafts + sequence;
-        auto change = [&](int t, float l, uint32_t mark, float bias) {
+        __syncthreads();
+        auto change = [&](int c, uint2 mark) {
             int more = 0;
-            for (int j = 0; j < ahead; ++j) more += drafts[(int64_t)j * a.sequences] == t;
-            set_value<OUT>(a.out, out_row + t, penalised(l, mark, more, bias, s));
+            for (int j = 0; j < ahead; ++j) more += drafts[j] == c;
+            const float l = INPLACE ? value_of<IN>(a.logits, in_at + c) : value_of<OUT>(staged, c);
+            const float to = penalised(l, mark.x, more, __uint_as_float(mark.y), s);
+            if constexpr (INPLACE) set_value<OUT>(a.out, out_at + c, to);
+            else set_value<OUT>(staged, c, to);
         };
 #pragma unroll
         for (int l = 0; l < kLists; ++l) {
-            const int first = c0 + l * kHistoryBucket, n = min(sizes[l], kHistoryBucket);
-            for (int i = threadIdx.x; i < n; i += kThreads) {
-                const int t = a.history.listed[base + first + i];
-                if (t < a.width && admitted(mask, t))
-                    change(t, value_of<IN>(a.logits, in_row + t), marks[t], a.history.biases[base + t]);
+            if ((int)threadIdx.x < sizes[l] && early[l] >= 0) change(early[l], early_of[l]);
+            // the others two at a time, whose loads are on their way together
+            for (int i = kThreads + threadIdx.x; i < sizes[l]; i += 2 * kThreads) {
+                const int j = i + kThreads;
+                int c = listed[l * kHistoryBucket + i] - c0, d = j < sizes[l] ? listed[l * kHistoryBucket + j] - c0 : -1;
+                if (c >= columns || !admitted(mask, c0 + c)) c = -1;
+                if (d >= columns || (d >= 0 && !admitted(mask, c0 + d))) d = -1;
+                const uint2 of_c = c >= 0 ? state[c] : make_uint2(0, 0), of_d = d >= 0 ? state[d] : make_uint2(0, 0);
+                if (c >= 0) change(c, of_c);
+                if (d >= 0) change(d, of_d);
             }
         }
-        if ((int)threadIdx.x < ahead) {  // drafts that are new to the request
-            const int64_t t = drafts[(int64_t)threadIdx.x * a.sequences];
-            bool mine = t >= c0 && t < c0 + columns;
-            for (int j = 0; j < (int)threadIdx.x; ++j) mine = mine && drafts[(int64_t)j * a.sequences] != t;
-            if (mine && admitted(mask, (int)t) && !(marks[t] & kListed))
-                change((int)t, value_of<IN>(a.logits, in_row + t), 0, 0.0f);
+        if (known && (int)threadIdx.x < ahead) {  // drafts that are new to the request
+            const int c = drafts[threadIdx.x];
+            bool first = c >= 0;
+            for (int j = 0; j < (int)threadIdx.x; ++j) first = first && drafts[j] != c;
+            if (first && admitted(mask, c0 + c) && !(state[c].x & kListed)) change(c, make_uint2(0, 0));
+        }
+        __syncthreads();
+    }
+    if (!INPLACE || mask || !s.valid) {
+        const uint32_t other = s.valid ? minus_infinity<OUT>() : not_a_number<OUT>();
+#pragma unroll
+        for (int i = 0; i < kTurns; ++i) {
+            if (!mine(i)) continue;
+            Eight<OUT> out = to_type<IN, OUT>(in[i]);
+            if constexpr (!INPLACE) {
+                if (some) out = load8<OUT>(staged, start(i));
+            }
+            const uint32_t keep = s.valid ? bits[i] : 0u;
+            keep8<OUT>(out, keep, other);
+            if (!INPLACE || keep == 0u) store8<OUT>(a.out, out_at + start(i), out);
+            else if (keep != 0xFFu) store_some<OUT>(a.out, out_at + start(i), out, ~keep);
+        }
+        if (!whole && (int)threadIdx.x < columns) {
+            const bool keep = s.valid && admitted(mask, c0 + threadIdx.x);
+            if (!keep) set_value<OUT>(a.out, out_at + threadIdx.x, s.valid ? -__builtin_huge_valf() : __builtin_nanf(""));
+            else if constexpr (!INPLACE) set_value<OUT>(a.out, out_at + threadIdx.x, value_of<OUT>(staged, threadIdx.x));
         }
     }
 }
 
 template <int IN, int OUT>
 hipError_t launch_typed(const PenaltyArgs& a, hipStream_t s) {
-    const int64_t items = (int64_t)a.live_sequences * (a.depth + 1) * a.chunks, most = 1 << 22;
-    const unsigned grid = (unsigned)(items < most ? items : most);
+    const dim3 grid((unsigned)(a.live_sequences * (a.depth + 1)), (unsigned)a.chunks);
     if (a.inplace) penalty_kernel<IN, IN, true><<<grid, kThreads, 0, s>>>(a);
     else penalty_kernel<IN, OUT, false><<<grid, kThreads, 0, s>>>(a);
     return hipGetLastError();

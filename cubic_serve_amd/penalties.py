@@ -41,8 +41,8 @@ def _live(live, most: int, device: torch.device, what: str) -> tuple[int, int | 
 class TokenHistory:
     """Tokens and biases of ``slots`` requests over ``vocab`` tokens.
 
-    ``marks`` int32, ``biases`` float32 and ``listed`` int32 [slots, vocab]: 12 bytes per
-    slot and token, and ``sizes`` int32 [slots, ceil(vocab / 4096)].  Its methods enqueue on the
+    ``state`` int32 [slots, vocab, 2] (a token's mark and its bias' bits) and ``listed``
+    int32 [slots, vocab]: 12 bytes per slot and token; ``sizes`` int32 [slots, ceil(vocab / 4096)].  Its methods enqueue on the
     current stream and order nothing against other streams; but for ``set_bias``
     they may be captured, and read their tensors when they run.
     """
@@ -53,12 +53,11 @@ class TokenHistory:
         if type(vocab) is not int or not 1 <= vocab <= 1 << 24:
             raise ValueError("history vocabulary must be an int in 1..2^24")
         self.slots, self.vocab = slots, vocab
-        self.marks = torch.zeros((slots, vocab), dtype=torch.int32, device=device)
-        self.biases = torch.zeros((slots, vocab), dtype=torch.float32, device=device)
+        self.state = torch.zeros((slots, vocab, 2), dtype=torch.int32, device=device)
         self.listed = torch.zeros((slots, vocab), dtype=torch.int32, device=device)
         self.sizes = torch.zeros((slots, (vocab + BUCKET - 1) // BUCKET), dtype=torch.int32, device=device)
-        self.device = self.marks.device
-        self._held = (self.marks, self.biases, self.listed, self.sizes)  # whose addresses bindings copy
+        self.device = self.state.device
+        self._held = (self.state, self.listed, self.sizes)  # whose addresses bindings copy
         self._args = (*(t.data_ptr() for t in self._held), slots, vocab)
 
     def _check_slots(self, row_slots: Tensor) -> None:
@@ -136,7 +135,11 @@ class TokenHistory:
 
     def counts(self, slot: int) -> Tensor:
         """How often each token was put out, int32 [vocab]."""
-        return self.marks[self._slot(slot)] & ((1 << 30) - 1)
+        return self.state[self._slot(slot), :, 0] & ((1 << 30) - 1)
+
+    def biases(self, slot: int) -> Tensor:
+        """Each token's bias, float32 [vocab]."""
+        return self.state[self._slot(slot), :, 1].contiguous().view(torch.float32)
 
 
 class LogitPenaltyPlan:
@@ -210,23 +213,28 @@ class LogitPenaltyPlan:
                  for t in (logits, slots, repetition, presence, frequency, draft_tokens, token_mask) if t is not None):
             raise ValueError("penalty outputs must not alias their operands")
         self.logits, self.history, self.outputs = logits, history, outputs
-        self._operands = tuple(t for t in (logits, outputs, slots, *optional[:5]) if t is not None)
+        operands = [t for t in (logits, outputs, slots, *optional[:5]) if t is not None]
         stride = lambda t: max(t.stride(0), t.shape[1])
-        self._head = (logits.data_ptr(), _CANDIDATE_DTYPES[logits.dtype], stride(logits), self.sequences, self.depth, self.width)
-        self._tail = (*history._args, slots.data_ptr(), *(_native.ptr(t) for t in optional[:5]), words, outputs.data_ptr(),
-                      _CANDIDATE_DTYPES[outputs.dtype], stride(outputs))
-        self._identity = self._identify()
-
-    def _identify(self):
-        return [(t.data_ptr(), t.shape, t.stride(), t.dtype) for t in self._operands]
+        head = (logits.data_ptr(), _CANDIDATE_DTYPES[logits.dtype], stride(logits), self.sequences, self.depth, self.width)
+        tail = (*history._args, slots.data_ptr(), *(_native.ptr(t) for t in optional[:5]), words, outputs.data_ptr(),
+                _CANDIDATE_DTYPES[outputs.dtype], stride(outputs))
+        converted = _native.converted("cubic_logit_penalties", (*head, 0, None, *tail))
+        self._head, self._tail = converted[:len(head)], converted[len(head) + 2:]
+        self._function = _native.lib().cubic_logit_penalties
+        # what a launch looks at: whether every operand still has its memory (which is held) and size
+        self._held = tuple(t.untyped_storage() for t in operands)
+        self._probes = tuple(f for t in operands for f in (t.data_ptr, t.numel))
+        self._identity = [f() for f in self._probes]
 
     def launch(self, live_sequences: int | Tensor | None = None) -> None:
         """Enqueue on the current stream.  The rows of sequences at or past
         ``live_sequences`` (a host int, or a device int32 tensor whose first element
         is read when the launch runs) keep their outputs."""
-        live = _live(live_sequences, self.sequences, self.logits.device, "sequence")
-        if self._identify() != self._identity:
+        live = _live(live_sequences, self.sequences, self.history.device, "sequence")
+        if [f() for f in self._probes] != self._identity:
             raise ValueError("penalty operands changed after binding")
-        index = self.logits.device.index
+        index = self.history.device.index
         with _native.on_device(index):
-            _native.call("cubic_logit_penalties", *self._head, *live, *self._tail, _native.stream_of(index))
+            status = self._function(*self._head, *live, *self._tail, _native.stream_of(index))
+        if status < 0:
+            _native.check("cubic_logit_penalties", status)

@@ -395,11 +395,11 @@ CUBIC_API int cubic_embedding(const void* ids, int id_bytes, int64_t tokens, int
  * Penalties, biases and grammar masks on logits.  No counterpart in the
  * reference's subset that this library replaces.
  *
- * A history of `slots` requests over `vocab` tokens is four arrays of the
- * caller's, zero on first use: marks u32, biases f32 and listed i32
- * [slots, vocab], sizes i32 [slots, ceil(vocab / 4096)].  Per slot: how often each
- * token was put out, whether the prompt has it, its bias, and per 4096 tokens a
- * list of those that have any.
+ * A history of `slots` requests over `vocab` tokens is three arrays of the
+ * caller's, zero on first use: state, two words [slots, vocab] (8-byte aligned),
+ * listed i32 [slots, vocab], sizes i32 [slots, ceil(vocab / 4096)].  Per slot: how often
+ * each token was put out, whether the prompt has it, its bias (f32), and per 4096
+ * tokens a list of those that have any.
  *
  * cubic_history_append: tokens [rows, length] (int32 or int64: token_bytes; row
  *   stride ld) of row r go to slot row_slots[r], as outputs or (prompt != 0) as
@@ -423,19 +423,19 @@ CUBIC_API int cubic_embedding(const void* ids, int id_bytes, int64_t tokens, int
  *   past live_sequences (live_count[0], where that is less), are left as they are.
  *   0 <= depth <= 8, width <= vocab.  No workspace.
  * ------------------------------------------------------------------------- */
-CUBIC_API int cubic_history_append(uint32_t* marks, float* biases, int32_t* listed, int32_t* sizes,
+CUBIC_API int cubic_history_append(uint32_t* state, int32_t* listed, int32_t* sizes,
                                    int slots, int vocab, const int32_t* row_slots, const void* tokens,
                                    int token_bytes, int64_t ld, int rows, int length, int prompt,
                                    int live_rows, const int32_t* live_count, void* stream);
-CUBIC_API int cubic_history_clear(uint32_t* marks, float* biases, int32_t* listed, int32_t* sizes,
+CUBIC_API int cubic_history_clear(uint32_t* state, int32_t* listed, int32_t* sizes,
                                   int slots, int vocab, const int32_t* row_slots, int rows, int slot,
                                   int biases_only, void* stream);
-CUBIC_API int cubic_history_bias(uint32_t* marks, float* biases, int32_t* listed, int32_t* sizes,
+CUBIC_API int cubic_history_bias(uint32_t* state, int32_t* listed, int32_t* sizes,
                                  int slots, int vocab, int slot, const int32_t* ids,
                                  const float* values, int count, void* stream);
 CUBIC_API int cubic_logit_penalties(const void* logits, int dtype, int64_t row_stride, int sequences,
                                     int depth, int width, int live_sequences,
-                                    const int32_t* live_count, uint32_t* marks, float* biases,
+                                    const int32_t* live_count, uint32_t* state,
                                     int32_t* listed, int32_t* sizes, int slots, int vocab,
                                     const int32_t* row_slots, const float* repetition,
                                     const float* presence, const float* frequency,

@@ -237,10 +237,10 @@ def test_history_appends_clears_and_biases():
     m.bias[2] = 0
 
     def check():
-        marks = h.marks.cpu().numpy().view(np.uint32)
+        marks = h.state[:, :, 0].contiguous().cpu().numpy().view(np.uint32)
         assert np.array_equal(marks & ((1 << 30) - 1), m.counts) and np.array_equal(marks >> 31 != 0, m.prompt)
-        assert np.array_equal(h.biases.cpu().numpy(), m.bias.astype(np.float32))
         for s in range(slots):  # every token that has anything is listed, once
+            assert np.array_equal(h.biases(s).cpu().numpy(), m.bias[s].astype(np.float32))
             listed = [t for b, n in enumerate(h.sizes[s].tolist()) for t in h.listed[s, 4096 * b:4096 * b + n].tolist()]
             assert len(set(listed)) == len(listed)
             assert set(np.flatnonzero((m.counts[s] > 0) | m.prompt[s] | (m.bias[s] != 0))) <= set(listed)
@@ -315,7 +315,7 @@ def test_rows_that_lie_far_apart():
     compare(out, *want)
     assert h.counts(slots - 1)[vocab - 1].item() == 1
     h.clear(slots - 1)
-    assert not h.marks[slots - 1].any() and not h.biases[slots - 1].any()
+    assert not h.state[slots - 1].any() and not h.sizes.any()
 
 
 def test_head_penalties_sampling_chain():

@@ -6,10 +6,10 @@ import torch
 
 from cubic_serve_amd import _native, penalties
 
-HISTORY = dict(marks=16, biases=16, listed=16, sizes=16, slots=4, vocab=100)
-BAD_HISTORY = [(dict(marks=None), "null history"), (dict(sizes=None), "null history"), (dict(slots=0), "history of"),
+HISTORY = dict(state=16, listed=16, sizes=16, slots=4, vocab=100)
+BAD_HISTORY = [(dict(state=None), "null history"), (dict(listed=None), "null history"), (dict(sizes=None), "null history"), (dict(slots=0), "history of"),
                (dict(slots=1 << 20), "history of"), (dict(vocab=0), "history of"), (dict(vocab=(1 << 24) + 1), "history of"),
-               (dict(biases=18), "misaligned history")]
+               (dict(state=20), "misaligned history"), (dict(sizes=18), "misaligned history")]
 APPEND = HISTORY | dict(rows_slots=16, tokens=16, bytes=8, ld=5, rows=2, length=5, prompt=0, live=2, count=None, stream=None)
 CLEAR = HISTORY | dict(row_slots=None, rows=1, slot=0, only=0, stream=None)
 BIAS = HISTORY | dict(slot=0, ids=16, values=16, count=3, stream=None)
