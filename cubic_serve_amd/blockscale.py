@@ -270,9 +270,9 @@ def bind_quantize(x: Tensor, quantized: BlockScaledActivations, *, gate: Tensor 
     return _binding((quantized,), _Launch("cubic_quantize_rows", (*inputs, *eight), args), device)
 
 
-def _binding(results: Sequence, launch: _Launch, device: torch.device) -> PackedOperatorBinding:
+def _binding(results: Sequence, launch: _Launch, device: torch.device, scratch: tuple = ()) -> PackedOperatorBinding:
     given = tuple(r for r in results if r is not None)
-    return PackedOperatorBinding(given[0] if len(given) == 1 else given, (launch,), device=device)
+    return PackedOperatorBinding(given[0] if len(given) == 1 else given, (launch,), scratch=scratch, device=device)
 
 
 def prepare_block_matrix(weight: BlockScaledMatrix, device: torch.device | None = None) -> tuple[Tensor, Tensor]:
@@ -301,6 +301,8 @@ def bind_block_linear_group(operators, x: BlockScaledActivations, weights: Seque
 
     Outputs are bf16, fp16 or fp32 (one type for all) and may have padded rows.
     K has to be a multiple of 16, x 16-byte aligned with rows of whole 16 bytes.
+    The binding owns its workspace, cleared on the current stream: a launch on
+    another one has to follow it, and launches of one binding must not overlap.
     """
     weights, outputs = tuple(weights), tuple(outputs)
     if not 1 <= len(weights) <= MAX_GROUP_MEMBERS or len(weights) != len(outputs):
@@ -329,9 +331,13 @@ def bind_block_linear_group(operators, x: BlockScaledActivations, weights: Seque
     _check_apart(outputs, [values, x.scales, *(t for pair in prepared for t in pair)])
     c = _native.ctypes
     table = lambda ctype, items: (ctype * len(items))(*items)
-    args = (values.data_ptr(), _stride(values), x.scales.data_ptr(), *x.scales.stride(), m, k, len(weights),
-            table(c.c_int64, [w.shape[0] for w in weights]), table(c.c_void_p, [p.data_ptr() for p, _ in prepared]),
+    widths = table(c.c_int64, [w.shape[0] for w in weights])
+    nbytes = _native.lib().cubic_block_gemm_workspace_bytes(m, k, len(weights), widths)
+    if nbytes < 0:
+        raise ValueError("block-scaled linear geometry not admitted")
+    workspace = torch.zeros(nbytes, dtype=torch.uint8, device=device)
+    args = (values.data_ptr(), _stride(values), x.scales.data_ptr(), *x.scales.stride(), m, k, len(weights), widths, table(c.c_void_p, [p.data_ptr() for p, _ in prepared]),
             table(c.c_void_p, [s.data_ptr() for _, s in prepared]), table(c.c_void_p, [y.data_ptr() for y in outputs]),
-            table(c.c_int64, [_stride(y) for y in outputs]), OUTPUT_IDS[outputs[0].dtype])
-    launch = _Launch("cubic_block_gemm", (values, x.scales, *outputs), args, held=(weights, prepared))
-    return _binding(outputs, launch, device)
+            table(c.c_int64, [_stride(y) for y in outputs]), OUTPUT_IDS[outputs[0].dtype], workspace.data_ptr(), nbytes)
+    launch = _Launch("cubic_block_gemm", (values, x.scales, *outputs), args, held=(weights, prepared, workspace))
+    return _binding(outputs, launch, device, scratch=(workspace,) if nbytes else ())

@@ -183,7 +183,7 @@ typedef const __attribute__((address_space(1))) void global_void_t;
 // s_waitcnt vmcnt(n), the other counters left alone
 constexpr int vm_waits(int n) { return (n & 0xF) | (0x7 << 4) | (0xF << 8) | ((n >> 4) << 14); }
 
-template <int NTW, int MTW, int WN, int WM, int S, int G, int EU>
+template <int NTW, int MTW, int WN, int WM, int S, int G, int EU, bool SPLIT>
 __global__ __launch_bounds__(G * WN * WM * 64) __attribute__((amdgpu_waves_per_eu(EU, EU)))
 void block_tile_kernel(BlockGemmArgs a) {
     constexpr int W = WN * WM, N = NTW * WN, M = MTW * WM;  // waves of a group; tiles of 16
@@ -209,11 +209,15 @@ void block_tile_kernel(BlockGemmArgs a) {
     // order that goes through 8 column groups for a row group, then the next
     // rows, so that those it has at one time share operands in its L2.
     const int cols = a.group_end[a.members - 1], row_groups = (a.m + 16 * M - 1) / (16 * M);
+    const int tiles = cols * row_groups;
     int id = blockIdx.x;
     {
-        const int total = cols * row_groups, per = total >> 3, rest = total & 7, xcd = id & 7;
+        const int total = SPLIT ? tiles * a.split : tiles, per = total >> 3, rest = total & 7, xcd = id & 7;
         id = xcd * per + min(xcd, rest) + (id >> 3);
     }
+    const int part = SPLIT ? id / tiles : 0;  // of K
+    if constexpr (SPLIT) id -= part * tiles;
+    const int tile_id = id;
     const int band = id / (8 * row_groups), wide = min(8, cols - 8 * band);
     id -= band * 8 * row_groups;
     const int m0 = id / wide * (16 * M);
@@ -248,14 +252,16 @@ void block_tile_kernel(BlockGemmArgs a) {
         w_from[p] = w.codes + (int64_t)(tile >> 3) * a.blocks * kGroupBytes + (tile & 7) * kBlockBytes;
         w_bytes[p] = tile < w.tiles ? kBlockBytes : 0;
     }
-    const int blocks = a.blocks;
+    const int b_first = SPLIT ? part * a.part_blocks : 0;
+    const int blocks = SPLIT ? min(a.blocks, b_first + a.part_blocks) : a.blocks;  // up to there
     const int64_t scale_group = a.scale_group;
     auto dma = [&](int b, auto stage) {
         uint8_t* to = stage_of(stage) + k_group * kStage;
         __attribute__((address_space(3))) uint8_t* xl = (__attribute__((address_space(3))) uint8_t*)(void*)to;
         __attribute__((address_space(3))) uint8_t* wl = xl + kW;
         const int k = b * kScaleBlock;
-        const uint32_t off[2] = {k < x_columns[0] ? x_at[0] : kPastEnd, k < x_columns[1] ? x_at[1] : kPastEnd};
+        const bool some = !SPLIT || b < blocks;
+        const uint32_t off[2] = {some && k < x_columns[0] ? x_at[0] : kPastEnd, some && k < x_columns[1] ? x_at[1] : kPastEnd};
 #pragma unroll
         for (int p = 0; p < kX; ++p) {
             const __amdgpu_buffer_rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc(
@@ -308,7 +314,7 @@ void block_tile_kernel(BlockGemmArgs a) {
     // every wave is done with the step before, into whose place the next load goes.
     auto step = [&](int at, auto stage) {
         constexpr int P = decltype(stage)::value;
-        const int b = at * G + k_group;
+        const int b = b_first + at * G + k_group;
         const uint8_t *xs = stage_of(stage) + k_group * kStage, *ws = xs + kW;
         const float* ss = reinterpret_cast<const float*>(xs + kScales);
         float scale[MTW];
@@ -353,7 +359,7 @@ void block_tile_kernel(BlockGemmArgs a) {
 #pragma unroll
             for (int i = 0; i < MTW; ++i) asm volatile("" : "+v"(acc[t][i]));
     };
-    auto first = [&](auto... stages) { (dma(decltype(stages)::value * G + k_group, stages), ...); };
+    auto first = [&](auto... stages) { (dma(b_first + decltype(stages)::value * G + k_group, stages), ...); };
     typedef std::integral_constant<int, 0> I0;
     typedef std::integral_constant<int, 1> I1;
     typedef std::integral_constant<int, 2> I2;
@@ -363,7 +369,7 @@ void block_tile_kernel(BlockGemmArgs a) {
     else first(I0{}, I1{}, I2{});
     // Whole rounds of the stages, then the rest: a loop of one exit, through which the
     // compiler follows which loads are on their way (with more it waits for all).
-    const int steps = (blocks + G - 1) / G;
+    const int steps = (blocks - b_first + G - 1) / G;
     int at = 0;
     for (; at + S <= steps; at += S) {
         step(at, I0{});
@@ -390,13 +396,41 @@ void block_tile_kernel(BlockGemmArgs a) {
                 for (int i = 0; i < MTW; ++i) sums[(k_group - 1) * kGroup + (t * MTW + i) * 64] = acc[t][i];
         }
         __syncthreads();
+        if (!SPLIT && k_group) return;
+        if (k_group == 0) {
+#pragma unroll
+            for (int t = 0; t < NTW; ++t)
+#pragma unroll
+                for (int i = 0; i < MTW; ++i)
+#pragma unroll
+                    for (int g = 0; g + 1 < G; ++g) acc[t][i] += sums[g * kGroup + (t * MTW + i) * 64];
+        }
+    }
+    if constexpr (SPLIT) {
+        // The parts' sums through memory; the workgroup that arrives last adds them, in
+        // the order of the parts.
+        __shared__ uint32_t last;
+        constexpr int kTileBytes = W * NTW * MTW * 1024;
+        const __amdgpu_buffer_rsrc_t r = device_rsrc(a.partial + (int64_t)tile_id * a.split * (kTileBytes / 4));
+        const int at = wave * NTW * MTW * 1024 + lane * 16;
+        if (k_group == 0) {
+#pragma unroll
+            for (int t = 0; t < NTW; ++t)
+#pragma unroll
+                for (int i = 0; i < MTW; ++i) store_device4(r, part * kTileBytes + at + (t * MTW + i) * 1024, acc[t][i]);
+        }
+        if (!arrive_last(&a.counters[tile_id], a.split, &last)) return;
+        if (threadIdx.x == 0) store_device(&a.counters[tile_id], 0u);
         if (k_group) return;
 #pragma unroll
         for (int t = 0; t < NTW; ++t)
 #pragma unroll
-            for (int i = 0; i < MTW; ++i)
+            for (int i = 0; i < MTW; ++i) acc[t][i] = load_device4(r, at + (t * MTW + i) * 1024);
+        for (int o = 1; o < a.split; ++o)
 #pragma unroll
-                for (int g = 0; g + 1 < G; ++g) acc[t][i] += sums[g * kGroup + (t * MTW + i) * 64];
+            for (int t = 0; t < NTW; ++t)
+#pragma unroll
+                for (int i = 0; i < MTW; ++i) acc[t][i] += load_device4(r, o * kTileBytes + at + (t * MTW + i) * 1024);
     }
 
     // 16 rows at a time through a wave-private run of LDS, to leave in whole lines
@@ -458,10 +492,10 @@ hipError_t launch_stream(BlockGemmArgs a, hipStream_t s) {
     return hipGetLastError();
 }
 
-template <int NTW, int MTW, int WN, int WM, int S, int G, int EU>
+template <int NTW, int MTW, int WN, int WM, int S, int G, int EU, bool SPLIT = false>
 hipError_t launch_tile(BlockGemmArgs a, hipStream_t s) {
-    const unsigned grid = count_groups(a, NTW * WN) * ((a.m + 16 * MTW * WM - 1) / (16 * MTW * WM));
-    block_tile_kernel<NTW, MTW, WN, WM, S, G, EU><<<grid, G * WN * WM * 64, 0, s>>>(a);
+    const unsigned tiles = count_groups(a, NTW * WN) * ((a.m + 16 * MTW * WM - 1) / (16 * MTW * WM));
+    block_tile_kernel<NTW, MTW, WN, WM, S, G, EU, SPLIT><<<SPLIT ? tiles * a.split : tiles, G * WN * WM * 64, 0, s>>>(a);
     return hipGetLastError();
 }
 
@@ -473,7 +507,7 @@ hipError_t launch_block_gemm(const BlockGemmArgs& a, hipStream_t s) {
         case 2: return launch_tile<4, 2, 2, 2, 3, 1, 2>(a, s);
         case 3: return launch_tile<4, 4, 4, 2, 3, 1, 2>(a, s);
         case 4: return launch_tile<8, 4, 2, 4, 2, 1, 2>(a, s);
-        case 5: return launch_tile<2, 2, 2, 2, 4, 2, 2>(a, s);
+        case 5: return a.split > 1 ? launch_tile<2, 2, 2, 2, 4, 2, 2, true>(a, s) : launch_tile<2, 2, 2, 2, 4, 2, 2>(a, s);
         default: break;
     }
     // the more columns there are, the fewer times x is read

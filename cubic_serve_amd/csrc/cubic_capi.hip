@@ -990,9 +990,59 @@ int cubic_quantize_rows(const void* x, int64_t ldx, const void* gate, int64_t ld
 // ---------------------------------------------------------------------------
 // Block-scaled 8-bit products
 // ---------------------------------------------------------------------------
+namespace {
+struct BlockPlan {
+    int tile, split, part_blocks;
+    int64_t counters, bytes;  // of the workspace
+};
+// Up to 8 rows the stream kernel, else the tiles (columns x rows) whose rounds over 256
+// CUs are expected to end first, by what a block of K takes a round, in hundredths of a us:
+//   64 x 64 27, 128 x 64 36 and 10 more, 256 x 128 120, 256 x 256 200
+// 4096 x 8192 x 8192: 548, 371, 292 and 249 us; 1024 rows x 8192 x 4096: 72, 53, 42 and 61; 512 x
+// 4096 x 4096: 21, 18.6, - and 57; 256 x 4096 x 12288: 34, 43, - and 153.  64 x 64 tiles that one
+// round holds have two groups of waves, each every other block of K: 256 x 4096 x 12288 30
+// and 34 us, 64 x 6144 x 4096 11.2 and 11.7, 333 x 1024 x 2064 8.2 and 8.0.  Rows of 6144 x 4096,
+// stream and tiles: 1 6.5 and 10.4, 8 10.3 and 10.4, 16 12.5 and 10.6.
+BlockPlan plan_block(int64_t m, int64_t k, int members, const int64_t* ns) {
+    BlockPlan p = {0, 1, 0, 0, 0};
+    if (m <= 8) return p;
+    auto tiles = [&](int columns, int rows) {
+        int64_t groups = 0;
+        for (int j = 0; j < members; ++j) groups += ceil_div(ns[j], columns);
+        return groups * ceil_div(m, rows);
+    };
+    const int64_t small = tiles(64, 64), blocks = ceil_div(k, cubic::kScaleBlock);
+    auto rounds = [&](int columns, int rows) { return ceil_div(tiles(columns, rows), 256); };
+    const int64_t cost[] = {27 * rounds(64, 64), 10 + 36 * rounds(128, 64), 120 * rounds(256, 128), 200 * rounds(256, 256)};
+    p.tile = 1 + (int)(std::min_element(cost, cost + 4) - cost);
+    if (p.tile != 1 || small > 256) return p;
+    // K in as many parts as leave one round, at most 4 of 8 blocks and more.  One part and
+    // this, weights in a cache and not: 64 rows x 4096 x 12288 28 and 15 us, 46 and 23; 64 x 1024 x 8192
+    // 17.6 and 10.4, 64 x 6144 x 4096 11.3 and 11.0, 16.7 and 13.6; 16 blocks 7.5 and 8.0.
+    const int64_t split = blocks < 32 ? 1 : std::min({256 / small, blocks / 8, (int64_t)4});
+    if (split > 1) {
+        p.part_blocks = (int)ceil_div(ceil_div(blocks, split), 2) * 2;
+        p.split = (int)ceil_div(blocks, p.part_blocks);
+    }
+    if (p.split > 1 || blocks >= 24) p.tile = 5;
+    if (p.split > 1) {
+        p.counters = align256(small * 4);
+        p.bytes = p.counters + small * p.split * 4096 * (int64_t)sizeof(float);
+    }
+    return p;
+}
+}  // namespace
+
 int64_t cubic_block_prepared_bytes(int64_t n, int64_t k) {
     if (n < 1 || n > (1 << 24) || k < 1 || k > (1 << 20)) return -1;
     return ceil_div(n, cubic::kScaleBlock) * ceil_div(k, cubic::kScaleBlock) * cubic::kScaleBlock * cubic::kScaleBlock;
+}
+
+int64_t cubic_block_gemm_workspace_bytes(int64_t m, int64_t k, int members, const int64_t* ns) {
+    if (m < 1 || m >= (1 << 21) || k < 1 || k > (1 << 20) || members < 1 || members > cubic::kMaxGemmMembers || !ns) return -1;
+    for (int j = 0; j < members; ++j)
+        if (ns[j] < 1 || ns[j] > (1 << 24)) return -1;
+    return plan_block(m, k, members, ns).bytes;
 }
 
 int cubic_block_prepare(const void* values, int64_t ld, int64_t n, int64_t k, void* prepared, void* stream) {
@@ -1006,7 +1056,8 @@ int cubic_block_prepare(const void* values, int64_t ld, int64_t n, int64_t k, vo
 
 int cubic_block_gemm(const void* x, int64_t ldx, const float* x_scales, int64_t scale_row, int64_t scale_group,
                      int64_t m, int64_t k, int members, const int64_t* ns, const void* const* prepared,
-                     const float* const* scales, void* const* ys, const int64_t* ldys, int out_dtype, void* stream) {
+                     const float* const* scales, void* const* ys, const int64_t* ldys, int out_dtype, void* workspace,
+                     int64_t workspace_bytes, void* stream) {
     if (!x || !x_scales || !ns || !prepared || !scales || !ys || !ldys) return fail(CUBIC_EINVAL, "block gemm: null operand");
     if (members < 1 || members > cubic::kMaxGemmMembers)
         return fail(CUBIC_EINVAL, "members=%d outside 1..%d", members, cubic::kMaxGemmMembers);
@@ -1044,27 +1095,17 @@ int cubic_block_gemm(const void* x, int64_t ldx, const float* x_scales, int64_t 
                        ((uintptr_t)ys[j] & (4 * element - 1)) == 0 && (m == 1 || ldys[j] % 4 == 0)};
         tiles += a.member[j].tiles;
     }
-    // Up to 8 rows the stream kernel, else the tiles (columns x rows) whose rounds over 256
-    // CUs are expected to end first, by what a block of K takes a round, in hundredths of a us:
-    //   64 x 64 27, 128 x 64 36 and 10 more, 256 x 128 120, 256 x 256 200
-    // 4096 x 8192 x 8192: 548, 371, 292 and 249 us; 1024 rows x 8192 x 4096: 72, 53, 42 and 61; 512 x
-    // 4096 x 4096: 21, 18.6, - and 57; 256 x 4096 x 12288: 34, 43, - and 153.  64 x 64 tiles that one
-    // round holds have two groups of waves, each every other block of K: 256 x 4096 x 12288 30
-    // and 34 us, 64 x 6144 x 4096 11.2 and 11.7, 333 x 1024 x 2064 8.2 and 8.0.  Rows of 6144 x 4096,
-    // stream and tiles: 1 6.5 and 10.4, 8 10.3 and 10.4, 16 12.5 and 10.6.
-    auto rounds = [&](int columns, int rows) {
-        int64_t groups = 0;
-        for (int j = 0; j < members; ++j) groups += ceil_div(ns[j], columns);
-        return ceil_div(groups * ceil_div(m, rows), 256);
-    };
-    if (m > 8) {
-        const int64_t small = rounds(64, 64);
-        const int64_t cost[] = {27 * small, 10 + 36 * rounds(128, 64), 120 * rounds(256, 128), 200 * rounds(256, 256)};
-        a.tile = 1 + (int)(std::min_element(cost, cost + 4) - cost);
-        if (a.tile == 1 && small == 1 && a.blocks >= 24) a.tile = 5;
-    }
-    if (a.tile && ceil_div(tiles, 4) * ceil_div(m, 64) >= (1 << 22))
+    if (m > 8 && ceil_div(tiles, 4) * ceil_div(m, 64) >= (1 << 22))
         return fail(CUBIC_ENOTSUP, "block gemm: more tiles than one launch holds");
+    const BlockPlan p = plan_block(m, k, members, ns);
+    if (workspace_bytes < p.bytes)
+        return fail(CUBIC_EWORKSPACE, "block gemm workspace %lld < %lld bytes", (long long)workspace_bytes, (long long)p.bytes);
+    if (p.bytes && (!workspace || !aligned16(workspace))) return fail(CUBIC_EINVAL, "workspace must be 16-byte aligned");
+    a.tile = p.tile;
+    a.split = p.split;
+    a.part_blocks = p.part_blocks;
+    a.counters = (uint32_t*)workspace;
+    a.partial = (float*)((uint8_t*)workspace + p.counters);
     return hip_status(cubic::launch_block_gemm(a, (hipStream_t)stream), "block gemm launch");
 }
 

@@ -394,6 +394,9 @@ struct BlockGemmArgs {
     int out;                      // CUBIC_DTYPE_* of y
     int tile;                     // 0: the stream kernel (up to 16 rows); tiles of 1: 64 x 64, 2: 128 x 64, 3: 256 x 128, 4: 256 x 256
                                   // columns x rows, 5: 64 x 64 by two groups of waves
+    int split, part_blocks;       // tile 5: parts of K and blocks in each, joined by the last to arrive
+    uint32_t* counters;           // [tiles], zero between launches
+    float* partial;               // [tiles, split, 4096]
     int group_end[kMaxGemmMembers];   // ends of the members' column groups (set at launch)
     BlockMember member[kMaxGemmMembers];
 };

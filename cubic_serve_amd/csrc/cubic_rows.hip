@@ -50,14 +50,17 @@ __device__ __forceinline__ void load8(const uint16_t* row, int c, int k, bool ve
     }
 }
 
-template <bool F16>
+// STREAM: past the caches.
+template <bool F16, bool STREAM = false>
 __device__ __forceinline__ void store8(uint16_t* row, int c, int k, bool vec, const float (&v)[kVec]) {
     if (vec && c + kVec <= k) {
         uint32_t u[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             u[i] = F16 ? to_bits<F16>(v[2 * i]) | to_bits<F16>(v[2 * i + 1]) << 16 : pack_bf16x2(v[2 * i], v[2 * i + 1]);
-        *reinterpret_cast<uint4*>(row + c) = make_uint4(u[0], u[1], u[2], u[3]);
+        const u32x4_dev_t w = {u[0], u[1], u[2], u[3]};
+        if constexpr (STREAM) __builtin_nontemporal_store(w, reinterpret_cast<u32x4_dev_t*>(row + c));
+        else *reinterpret_cast<u32x4_dev_t*>(row + c) = w;
     } else {
 #pragma unroll
         for (int i = 0; i < kVec; ++i)
@@ -145,7 +148,8 @@ __global__ __launch_bounds__(1024) void row_norm_kernel(RowArgs a) {
         };
         auto write = [&](int i, float factor, float (&h)[kVec]) {
             const int c = (i * blockDim.x + threadIdx.x) * kVec;
-            if (a.sum) store8<F16>(static_cast<uint16_t*>(a.sum) + row * a.ldsum, c, a.k, a.vec_sum, h);
+            // (the sum is read again a layer later: 4096 x 8192 in 55.9 and 52.1 us past the caches)
+            if (a.sum) store8<F16, true>(static_cast<uint16_t*>(a.sum) + row * a.ldsum, c, a.k, a.vec_sum, h);
             float w[kVec];
             load8<F16>(weight, c, a.k, a.vec_weight, w);
 #pragma unroll

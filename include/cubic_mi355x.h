@@ -485,8 +485,13 @@ CUBIC_API int cubic_quantize_rows(const void* x, int64_t ldx, const void* gate, 
  * Host arrays ns, prepared, scales, ys, ldys have one entry per member and are
  * read during the call.  k % 16 == 0, x 16-byte aligned with a row stride of whole
  * 16 bytes up to 2^23, m < 2^21.  NaN values and scales propagate.  Sums are in 32
- * bits; their order depends on the sizes only, no workspace.
+ * bits; their order depends on the sizes only.
+ *   workspace  cubic_block_gemm_workspace_bytes(m, k, members, ns) bytes, 16-byte
+ *            aligned, zero before the first launch; every launch leaves its
+ *            counters zero.  Launches that share one must not overlap.
  * ------------------------------------------------------------------------- */
+CUBIC_API int64_t cubic_block_gemm_workspace_bytes(int64_t m, int64_t k, int members,
+                                                   const int64_t* ns);
 CUBIC_API int64_t cubic_block_prepared_bytes(int64_t n, int64_t k);
 CUBIC_API int cubic_block_prepare(const void* values, int64_t ld, int64_t n, int64_t k,
                                   void* prepared, void* stream);
@@ -494,7 +499,8 @@ CUBIC_API int cubic_block_gemm(const void* x, int64_t ldx, const float* x_scales
                                int64_t scale_group, int64_t m, int64_t k, int members,
                                const int64_t* ns, const void* const* prepared,
                                const float* const* scales, void* const* ys, const int64_t* ldys,
-                               int out_dtype, void* stream);
+                               int out_dtype, void* workspace, int64_t workspace_bytes,
+                               void* stream);
 
 /* ---------------------------------------------------------------------------
  * MoE router: per row, the top_k experts by (logit desc, expert id asc), then

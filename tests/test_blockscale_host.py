@@ -108,7 +108,7 @@ def test_block_gemm_entry_refuses(change, match):
     with pytest.raises(ValueError, match=match):
         _native.call("cubic_block_gemm", a["x"], a["ldx"], a["sx"], a["row"], a["group"], a["m"], a["k"], a["members"],
                      one(c.c_int64, a["n"]), one(c.c_void_p, a["w"]), one(c.c_void_p, a["sw"]), one(c.c_void_p, a["y"]),
-                     one(c.c_int64, a["ldy"]), a["out"], None)
+                     one(c.c_int64, a["ldy"]), a["out"], 16, 1 << 30, None)
 
 
 def test_block_prepare_entry():
@@ -122,3 +122,17 @@ def test_block_prepare_entry():
     for args in ((None, 128, 4, 128, 16), (16, 127, 4, 128, 16), (16, 128, 4, 128, 24), (16, 128, 4, 128, None)):
         with pytest.raises(ValueError):
             _native.call("cubic_block_prepare", *args, None)
+
+
+def test_block_gemm_workspace():
+    c, lib = _native.ctypes, _native.lib()
+    need = lambda m, k, *ns: lib.cubic_block_gemm_workspace_bytes(m, k, len(ns), (c.c_int64 * len(ns))(*ns))
+    assert need(1, 12288, 4096) == 0 and need(4096, 8192, 8192) == 0 and need(64, 2048, 4096) == 0
+    # 64 tiles of 64 x 64 in four parts of K, and a counter each
+    assert need(64, 12288, 4096) == 256 + 64 * 4 * 64 * 64 * 4
+    assert need(0, 128, 64) == -1 and need(64, 0, 64) == -1 and need(64, 128, 0) == -1
+    one = lambda ctype, v: (ctype * 1)(v)
+    for workspace, nbytes, match in ((16, need(64, 12288, 4096) - 1, "workspace"), (None, 1 << 30, "aligned"), (24, 1 << 30, "aligned")):
+        with pytest.raises(ValueError, match=match):
+            _native.call("cubic_block_gemm", 16, 12288, 16, 96, 1, 64, 12288, 1, one(c.c_int64, 4096), one(c.c_void_p, 16),
+                         one(c.c_void_p, 16), one(c.c_void_p, 16), one(c.c_int64, 4096), 0, workspace, nbytes, None)

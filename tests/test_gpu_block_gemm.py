@@ -100,7 +100,8 @@ def test_group(m):
         check(x, w, y)
 
 
-@pytest.mark.parametrize("m,n,k", [(3, 5000, 4096), (64, 40000, 1024), (200, 33000, 512), (700, 2048, 8192), (1111, 3333, 1040), (2048, 1536, 2048)])
+@pytest.mark.parametrize("m,n,k", [(3, 5000, 4096), (64, 40000, 1024), (200, 33000, 512), (700, 2048, 8192), (1111, 3333, 1040), (2048, 1536, 2048),
+                                   (64, 1024, 8192), (20, 3000, 12272), (100, 500, 6000), (17, 130, 4224)])
 def test_larger(m, n, k):
     print(f"block gemm m={m} n={n} k={k}", flush=True)
     x, w = activations(m, k, 5), matrix(n, k, 6)
@@ -109,7 +110,7 @@ def test_larger(m, n, k):
 
 
 @pytest.mark.parametrize("m", [1, 9, 17, 48, 80, 200, 513])
-@pytest.mark.parametrize("n,k", [(1, 16), (17, 144), (300, 2096), (1000, 256), (2100, 1040)])
+@pytest.mark.parametrize("n,k", [(1, 16), (17, 144), (300, 2096), (1000, 256), (2100, 1040), (700, 4400)])
 def test_integers_are_exact(m, n, k):
     """Whole numbers and scales of powers of two: every sum is exact in 32 bits, no product cut."""
     gen = torch.Generator(device=DEV).manual_seed(7)
@@ -163,12 +164,12 @@ def test_rows_do_not_depend_on_their_neighbours(m):
 
 
 def test_captured_replayed_and_concurrent():
-    m, n, k = 30, 3000, 1040
+    m, n, k = 30, 3000, 4112  # K in parts that meet in the workspace
     x, w = activations(m, k, 14), matrix(n, k, 15)
     ops = linear.PackedLinearOperators()
     y, z = (torch.empty((m, n), dtype=BF16, device=DEV) for _ in range(2))
     one, two = ops.bind_block_linear(x, w, y), ops.bind_block_linear(x, w, z)
-    assert len(ops.prepared_weights) == 1
+    assert len(ops.prepared_weights) == 1 and one.scratch and one.scratch[0].data_ptr() != two.scratch[0].data_ptr()
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     for _ in range(5):  # two launches at once
@@ -191,6 +192,7 @@ def test_captured_replayed_and_concurrent():
         two.launch()
         torch.cuda.synchronize()
         assert torch.equal(y, z)
+    assert not one.scratch[0][:4 * ((n + 63) // 64)].any()  # the counters
 
 
 def test_weights_changed_later_are_prepared_again():
