@@ -142,7 +142,7 @@ def quantize_block_scaled(weight: Tensor) -> BlockScaledMatrix:
 # bindings
 # --------------------------------------------------------------------------- #
 class _Launch:
-    """One bound C entry: its arguments, converted once, and the operands they came from.
+    """One bound C call and the operands it came from.
 
     Addresses, extents and strides are those at bind time.  A launch looks whether
     every operand still has its memory and size (0.8 us of the host's time; shapes
@@ -150,9 +150,9 @@ class _Launch:
     """
 
     def __init__(self, name: str, operands: Sequence[Tensor], args: tuple, held: tuple = ()):
-        self.name, self.args = name, _native.converted(name, args)
-        self.held = (held, args, tuple(t.untyped_storage() for t in operands))
-        self._function = getattr(_native.lib(), name)
+        self.held = (held, tuple(t.untyped_storage() for t in operands))
+        with torch.cuda.device(operands[0].device):
+            self._call = _native.BoundCall(name, *args)
         self._probes = tuple(f for t in operands for f in (t.data_ptr, t.numel))
         self._identity = [f() for f in self._probes]
 
@@ -161,9 +161,7 @@ class _Launch:
             raise ValueError("packed launch operands changed after binding")
 
     def __call__(self, stream: int) -> None:
-        status = self._function(*self.args, stream)
-        if status < 0:
-            _native.check(self.name, status)
+        self._call.launch(stream)
 
 
 def _stride(t: Tensor) -> int:

@@ -791,6 +791,46 @@ int cubic_vocab_sample(const void* logits, int dtype, int64_t row_stride, int ro
 }
 
 // ---------------------------------------------------------------------------
+// Bound calls: a call's arguments as its kernels take them, checked once
+// ---------------------------------------------------------------------------
+namespace {
+struct BoundCall {
+    uint32_t magic;
+    enum Kind : uint32_t { kRows, kBlock, kPenalties } kind;
+    union {
+        cubic::RowArgs rows;
+        cubic::BlockGemmArgs block;
+        cubic::PenaltyArgs penalties;
+    };
+};
+constexpr uint32_t kBoundMagic = 0x43424c31;
+
+int launch_call(const BoundCall& c, void* stream) {
+    switch (c.kind) {
+        case BoundCall::kRows: return hip_status(cubic::launch_rows(c.rows, (hipStream_t)stream), "row launch");
+        case BoundCall::kBlock: return hip_status(cubic::launch_block_gemm(c.block, (hipStream_t)stream), "block gemm launch");
+        default: return hip_status(cubic::launch_penalties(c.penalties, (hipStream_t)stream), "logit penalties launch");
+    }
+}
+
+// Keeps a checked call in `bound`, or launches it.
+int bind_or_launch(const BoundCall& c, void* bound, void* stream) {
+    if (!bound) return launch_call(c, stream);
+    if ((uintptr_t)bound % alignof(BoundCall)) return fail(CUBIC_EINVAL, "bound call is not aligned to 8 bytes");
+    *(BoundCall*)bound = c;
+    return CUBIC_OK;
+}
+}  // namespace
+
+int64_t cubic_bound_bytes(void) { return sizeof(BoundCall); }
+
+int cubic_launch_bound(const void* bound, void* stream) {
+    const BoundCall* c = (const BoundCall*)bound;
+    if (!c || (uintptr_t)c % alignof(BoundCall) || c->magic != kBoundMagic) return fail(CUBIC_EINVAL, "not a bound call");
+    return launch_call(*c, stream);
+}
+
+// ---------------------------------------------------------------------------
 // Token histories and penalties on logits
 // ---------------------------------------------------------------------------
 namespace {
@@ -845,7 +885,7 @@ int cubic_logit_penalties(const void* logits, int dtype, int64_t row_stride, int
                           int32_t* listed, int32_t* sizes, int slots, int vocab, const int32_t* row_slots,
                           const float* repetition, const float* presence, const float* frequency,
                           const int64_t* drafts, const int32_t* mask, int64_t mask_words, void* out, int out_dtype,
-                          int64_t out_stride, void* stream) {
+                          int64_t out_stride, void* bound, void* stream) {
     const cubic::HistoryArgs h = {(uint2*)state, listed, sizes, slots, vocab};
     if (const int status = check_history(h, "logit penalties")) return status;
     if (!logits || !row_slots || !out) return fail(CUBIC_EINVAL, "logit penalties: null operand");
@@ -868,7 +908,9 @@ int cubic_logit_penalties(const void* logits, int dtype, int64_t row_stride, int
         ((uintptr_t)row_slots | (uintptr_t)repetition | (uintptr_t)presence | (uintptr_t)frequency | (uintptr_t)mask |
          (uintptr_t)live_count) % 4)
         return fail(CUBIC_EINVAL, "logit penalties: misaligned operand");
-    cubic::PenaltyArgs a = {};
+    BoundCall call = {kBoundMagic, BoundCall::kPenalties, {}};
+    cubic::PenaltyArgs& a = call.penalties;
+    a = {};
     a.inplace = out == logits;
     if (a.inplace && (out_dtype != dtype || (rows > 1 && out_stride != row_stride)))
         return fail(CUBIC_EINVAL, "logit penalties: in place the outputs have the logits' type and row stride");
@@ -892,7 +934,7 @@ int cubic_logit_penalties(const void* logits, int dtype, int64_t row_stride, int
     a.drafts = drafts;
     a.mask = (const uint32_t*)mask;
     a.mask_words = mask_words;
-    return hip_status(cubic::launch_penalties(a, (hipStream_t)stream), "logit penalties launch");
+    return bind_or_launch(call, bound, stream);
 }
 
 // ---------------------------------------------------------------------------
@@ -909,7 +951,8 @@ bool scales_apart(int64_t m, int64_t groups, int64_t row, int64_t group) {
            (m == 1 || groups == 1 || row > (groups - 1) * group || group / row >= m || group > (m - 1) * row);
 }
 
-int rows_common(cubic::RowArgs& a, int dtype, void* stream, const char* what) {
+int rows_common(BoundCall& call, int dtype, void* bound, void* stream, const char* what) {
+    cubic::RowArgs& a = call.rows;
     if (dtype != CUBIC_DTYPE_BF16 && dtype != CUBIC_DTYPE_F16) return fail(CUBIC_ENOTSUP, "%s: dtype=%d", what, dtype);
     if (a.m < 1 || a.m > 0x7fffffff) return fail(CUBIC_EINVAL, "%s: m=%lld", what, (long long)a.m);
     a.f16 = dtype == CUBIC_DTYPE_F16;
@@ -930,20 +973,22 @@ int rows_common(cubic::RowArgs& a, int dtype, void* stream, const char* what) {
         if (!scales_apart(a.m, ceil_div(a.k, cubic::kScaleBlock), a.scale_row, a.scale_group))
             return fail(CUBIC_EINVAL, "%s: scale strides %lld, %lld overlap", what, (long long)a.scale_row, (long long)a.scale_group);
     }
-    return hip_status(cubic::launch_rows(a, (hipStream_t)stream), what);
+    return bind_or_launch(call, bound, stream);
 }
 }  // namespace
 
 int cubic_row_norm(const void* x, int64_t ldx, const void* residual, int64_t ldresidual, const void* weight,
                    int64_t m, int64_t k, int dtype, float epsilon, float weight_offset, void* y, int64_t ldy,
                    void* sum, int64_t ldsum, void* q, int64_t ldq, float* scales, int64_t scale_row,
-                   int64_t scale_group, void* stream) {
+                   int64_t scale_group, void* bound, void* stream) {
     if (!x || !weight || (!y && !q)) return fail(CUBIC_EINVAL, "row norm: null operand");
     if (k < 1 || k > cubic::kMaxRowColumns) return fail(CUBIC_EINVAL, "row norm: k=%lld", (long long)k);
     if (!(epsilon >= 0.0f && epsilon <= 1e30f) || !(weight_offset >= -1e30f && weight_offset <= 1e30f))
         return fail(CUBIC_EINVAL, "row norm: epsilon must be finite and >= 0, the weights' offset finite");
     if ((uintptr_t)weight % 2) return fail(CUBIC_EINVAL, "row norm: weights are not aligned to their element");
-    cubic::RowArgs a = {};
+    BoundCall call = {kBoundMagic, BoundCall::kRows, {}};
+    cubic::RowArgs& a = call.rows;
+    a = {};
     a.x = x;
     a.other = residual;
     a.weight = weight;
@@ -964,15 +1009,17 @@ int cubic_row_norm(const void* x, int64_t ldx, const void* residual, int64_t ldr
     a.scale_row = scale_row;
     a.scale_group = scale_group;
     a.vec_weight = ((uintptr_t)weight & 15) == 0;
-    return rows_common(a, dtype, stream, "row norm");
+    return rows_common(call, dtype, bound, stream, "row norm");
 }
 
 int cubic_quantize_rows(const void* x, int64_t ldx, const void* gate, int64_t ldgate, int64_t m, int64_t k,
                         int dtype, void* q, int64_t ldq, float* scales, int64_t scale_row, int64_t scale_group,
-                        void* stream) {
+                        void* bound, void* stream) {
     if (!x || !q) return fail(CUBIC_EINVAL, "quantize rows: null operand");
     if (k < 1 || k > cubic::kMaxRowColumns) return fail(CUBIC_EINVAL, "quantize rows: k=%lld", (long long)k);
-    cubic::RowArgs a = {};
+    BoundCall call = {kBoundMagic, BoundCall::kRows, {}};
+    cubic::RowArgs& a = call.rows;
+    a = {};
     a.x = x;
     a.other = gate;
     a.ldx = ldx;
@@ -984,7 +1031,7 @@ int cubic_quantize_rows(const void* x, int64_t ldx, const void* gate, int64_t ld
     a.scales = scales;
     a.scale_row = scale_row;
     a.scale_group = scale_group;
-    return rows_common(a, dtype, stream, "quantize rows");
+    return rows_common(call, dtype, bound, stream, "quantize rows");
 }
 
 // ---------------------------------------------------------------------------
@@ -1057,7 +1104,7 @@ int cubic_block_prepare(const void* values, int64_t ld, int64_t n, int64_t k, vo
 int cubic_block_gemm(const void* x, int64_t ldx, const float* x_scales, int64_t scale_row, int64_t scale_group,
                      int64_t m, int64_t k, int members, const int64_t* ns, const void* const* prepared,
                      const float* const* scales, void* const* ys, const int64_t* ldys, int out_dtype, void* workspace,
-                     int64_t workspace_bytes, void* stream) {
+                     int64_t workspace_bytes, void* bound, void* stream) {
     if (!x || !x_scales || !ns || !prepared || !scales || !ys || !ldys) return fail(CUBIC_EINVAL, "block gemm: null operand");
     if (members < 1 || members > cubic::kMaxGemmMembers)
         return fail(CUBIC_EINVAL, "members=%d outside 1..%d", members, cubic::kMaxGemmMembers);
@@ -1071,7 +1118,9 @@ int cubic_block_gemm(const void* x, int64_t ldx, const float* x_scales, int64_t 
     if ((uintptr_t)x_scales % 4 || (m > 1 && (scale_row < 1 || scale_row > ((int64_t)1 << 40))) ||
         (k > cubic::kScaleBlock && (scale_group < 1 || scale_group > ((int64_t)1 << 40))))
         return fail(CUBIC_EINVAL, "block gemm: scale strides %lld, %lld", (long long)scale_row, (long long)scale_group);
-    cubic::BlockGemmArgs a = {};
+    BoundCall call = {kBoundMagic, BoundCall::kBlock, {}};
+    cubic::BlockGemmArgs& a = call.block;
+    a = {};
     a.x = (const uint8_t*)x;
     a.x_scales = x_scales;
     a.ldx = ldx;
@@ -1106,7 +1155,7 @@ int cubic_block_gemm(const void* x, int64_t ldx, const float* x_scales, int64_t 
     a.part_blocks = p.part_blocks;
     a.counters = (uint32_t*)workspace;
     a.partial = (float*)((uint8_t*)workspace + p.counters);
-    return hip_status(cubic::launch_block_gemm(a, (hipStream_t)stream), "block gemm launch");
+    return bind_or_launch(call, bound, stream);
 }
 
 // ---------------------------------------------------------------------------

@@ -201,13 +201,21 @@ class PackedOperatorBinding:
         """Enqueue every launch on the current stream; returns the launch ordinal."""
         self.validate_operands()
         self._ordinal += 1
-        first = self.output[0] if isinstance(self.output, tuple) else self.output
-        index = (self._device or first.device).index
-        with _native.on_device(index):
-            stream = _native.stream_of(index)
-            for item in self._launches:
-                item(stream)
+        device = self._device
+        if device is None:
+            device = (self.output[0] if isinstance(self.output, tuple) else self.output).device
+        index = device.index
+        if _native.current_device() == index:  # (no guard: half a us of the host's time)
+            self._enqueue(index)
+        else:
+            with _native.on_device(index):
+                self._enqueue(index)
         return self._ordinal
+
+    def _enqueue(self, index: int) -> None:
+        stream = _native.stream_of(index)
+        for item in self._launches:
+            item(stream)
 
 
 # --------------------------------------------------------------------------- #

@@ -215,26 +215,30 @@ class LogitPenaltyPlan:
         self.logits, self.history, self.outputs = logits, history, outputs
         operands = [t for t in (logits, outputs, slots, *optional[:5]) if t is not None]
         stride = lambda t: max(t.stride(0), t.shape[1])
-        head = (logits.data_ptr(), _CANDIDATE_DTYPES[logits.dtype], stride(logits), self.sequences, self.depth, self.width)
-        tail = (*history._args, slots.data_ptr(), *(_native.ptr(t) for t in optional[:5]), words, outputs.data_ptr(),
-                _CANDIDATE_DTYPES[outputs.dtype], stride(outputs))
-        converted = _native.converted("cubic_logit_penalties", (*head, 0, None, *tail))
-        self._head, self._tail = converted[:len(head)], converted[len(head) + 2:]
-        self._function = _native.lib().cubic_logit_penalties
+        self._head = (logits.data_ptr(), _CANDIDATE_DTYPES[logits.dtype], stride(logits), self.sequences, self.depth, self.width)
+        self._tail = (*history._args, slots.data_ptr(), *(_native.ptr(t) for t in optional[:5]), words, outputs.data_ptr(),
+                      _CANDIDATE_DTYPES[outputs.dtype], stride(outputs), None)
+        # the call with all sequences live
+        self._call = _native.BoundCall("cubic_logit_penalties", *self._head, self.sequences, None, *self._tail[:-1])
         # what a launch looks at: whether every operand still has its memory (which is held) and size
         self._held = tuple(t.untyped_storage() for t in operands)
         self._probes = tuple(f for t in operands for f in (t.data_ptr, t.numel))
         self._identity = [f() for f in self._probes]
+        self._index = device.index
 
     def launch(self, live_sequences: int | Tensor | None = None) -> None:
         """Enqueue on the current stream.  The rows of sequences at or past
         ``live_sequences`` (a host int, or a device int32 tensor whose first element
         is read when the launch runs) keep their outputs."""
-        live = _live(live_sequences, self.sequences, self.history.device, "sequence")
         if [f() for f in self._probes] != self._identity:
             raise ValueError("penalty operands changed after binding")
-        index = self.history.device.index
+        index = self._index
+        live = None if live_sequences is None else _live(live_sequences, self.sequences, self.history.device, "sequence")
+        if live is None and _native.current_device() == index:
+            self._call.launch(_native.stream_of(index))
+            return
         with _native.on_device(index):
-            status = self._function(*self._head, *live, *self._tail, _native.stream_of(index))
-        if status < 0:
-            _native.check("cubic_logit_penalties", status)
+            if live is None:
+                self._call.launch(_native.stream_of(index))
+            else:
+                _native.call("cubic_logit_penalties", *self._head, *live, *self._tail, _native.stream_of(index))

@@ -392,6 +392,16 @@ CUBIC_API int cubic_embedding(const void* ids, int id_bytes, int64_t tokens, int
                               int group_in, int group_out, void* out, int out_dtype, void* stream);
 
 /* ---------------------------------------------------------------------------
+ * Bound calls.  An entry with a `bound` argument launches where that is NULL; else it
+ * checks its arguments, writes the call into `bound` (cubic_bound_bytes() bytes of
+ * host memory, 8-byte aligned) and launches nothing.  cubic_launch_bound then
+ * launches it any number of times, on any stream, with the addresses and sizes it
+ * was given; nothing is checked again.
+ * ------------------------------------------------------------------------- */
+CUBIC_API int64_t cubic_bound_bytes(void);
+CUBIC_API int cubic_launch_bound(const void* bound, void* stream);
+
+/* ---------------------------------------------------------------------------
  * Penalties, biases and grammar masks on logits.  No counterpart in the
  * reference's subset that this library replaces.
  *
@@ -440,7 +450,8 @@ CUBIC_API int cubic_logit_penalties(const void* logits, int dtype, int64_t row_s
                                     const int32_t* row_slots, const float* repetition,
                                     const float* presence, const float* frequency,
                                     const int64_t* drafts, const int32_t* mask, int64_t mask_words,
-                                    void* out, int out_dtype, int64_t out_stride, void* stream);
+                                    void* out, int out_dtype, int64_t out_stride, void* bound,
+                                    void* stream);
 
 /* ---------------------------------------------------------------------------
  * Row norms and 8-bit activations.  No counterpart in the reference's subset
@@ -465,11 +476,11 @@ CUBIC_API int cubic_row_norm(const void* x, int64_t ldx, const void* residual, i
                              const void* weight, int64_t m, int64_t k, int dtype, float epsilon,
                              float weight_offset, void* y, int64_t ldy, void* sum, int64_t ldsum,
                              void* q, int64_t ldq, float* scales, int64_t scale_row,
-                             int64_t scale_group, void* stream);
+                             int64_t scale_group, void* bound, void* stream);
 CUBIC_API int cubic_quantize_rows(const void* x, int64_t ldx, const void* gate, int64_t ldgate,
                                   int64_t m, int64_t k, int dtype, void* q, int64_t ldq,
                                   float* scales, int64_t scale_row, int64_t scale_group,
-                                  void* stream);
+                                  void* bound, void* stream);
 
 /* ---------------------------------------------------------------------------
  * Block-scaled 8-bit products.  No counterpart in the reference's subset that
@@ -500,7 +511,7 @@ CUBIC_API int cubic_block_gemm(const void* x, int64_t ldx, const float* x_scales
                                const int64_t* ns, const void* const* prepared,
                                const float* const* scales, void* const* ys, const int64_t* ldys,
                                int out_dtype, void* workspace, int64_t workspace_bytes,
-                               void* stream);
+                               void* bound, void* stream);
 
 /* ---------------------------------------------------------------------------
  * MoE router: per row, the top_k experts by (logit desc, expert id asc), then

@@ -69,7 +69,7 @@ def test_bindings_need_a_gpu():
 
 def norm(**change):
     a = dict(x=16, ldx=64, r=None, ldr=0, w=16, m=2, k=64, dtype=0, eps=1e-6, off=0.0, y=16, ldy=64, s=None, lds=0,
-             q=None, ldq=0, sc=None, row=0, group=0, stream=None) | change
+             q=None, ldq=0, sc=None, row=0, group=0, bound=None, stream=None) | change
     return _native.call("cubic_row_norm", *a.values())
 
 
@@ -89,7 +89,7 @@ def test_norm_entry_refuses(change, match):
     (dict(q=None), "null"), (dict(x=None), "null"), (dict(k=0), "k="), (dict(m=0), "m="), (dict(ldg=3, g=16), "row stride"),
     (dict(ldq=63), "row stride"), (dict(dtype=7), "dtype"), (dict(sc=None), "scales")])
 def test_quantize_entry_refuses(change, match):
-    a = dict(x=16, ldx=64, g=None, ldg=0, m=2, k=64, dtype=0, q=16, ldq=64, sc=16, row=1, group=2, stream=None) | change
+    a = dict(x=16, ldx=64, g=None, ldg=0, m=2, k=64, dtype=0, q=16, ldq=64, sc=16, row=1, group=2, bound=None, stream=None) | change
     with pytest.raises(ValueError, match=match):
         _native.call("cubic_quantize_rows", *a.values())
 
@@ -108,7 +108,7 @@ def test_block_gemm_entry_refuses(change, match):
     with pytest.raises(ValueError, match=match):
         _native.call("cubic_block_gemm", a["x"], a["ldx"], a["sx"], a["row"], a["group"], a["m"], a["k"], a["members"],
                      one(c.c_int64, a["n"]), one(c.c_void_p, a["w"]), one(c.c_void_p, a["sw"]), one(c.c_void_p, a["y"]),
-                     one(c.c_int64, a["ldy"]), a["out"], 16, 1 << 30, None)
+                     one(c.c_int64, a["ldy"]), a["out"], 16, 1 << 30, None, None)
 
 
 def test_block_prepare_entry():
@@ -135,4 +135,22 @@ def test_block_gemm_workspace():
     for workspace, nbytes, match in ((16, need(64, 12288, 4096) - 1, "workspace"), (None, 1 << 30, "aligned"), (24, 1 << 30, "aligned")):
         with pytest.raises(ValueError, match=match):
             _native.call("cubic_block_gemm", 16, 12288, 16, 96, 1, 64, 12288, 1, one(c.c_int64, 4096), one(c.c_void_p, 16),
-                         one(c.c_void_p, 16), one(c.c_void_p, 16), one(c.c_int64, 4096), 0, workspace, nbytes, None)
+                         one(c.c_void_p, 16), one(c.c_void_p, 16), one(c.c_int64, 4096), 0, workspace, nbytes, None, None)
+
+
+def test_bound_calls():
+    """A checked call is kept, not launched; what is no bound call is refused."""
+    c, lib = _native.ctypes, _native.lib()
+    nbytes = lib.cubic_bound_bytes()
+    assert 0 < nbytes <= 4096
+    memory = c.create_string_buffer(nbytes + 8)
+    with pytest.raises(ValueError, match="not a bound call"):
+        _native.call("cubic_launch_bound", c.addressof(memory), None)
+    with pytest.raises(ValueError, match="not a bound call"):
+        _native.call("cubic_launch_bound", None, None)
+    assert norm(bound=c.addressof(memory)) == 0
+    assert any(memory.raw)
+    with pytest.raises(ValueError, match="aligned to 8"):
+        norm(bound=c.addressof(memory) + 4)
+    with pytest.raises(ValueError, match="epsilon"):
+        norm(eps=-1.0, bound=c.addressof(memory))

@@ -15,7 +15,7 @@ CLEAR = HISTORY | dict(row_slots=None, rows=1, slot=0, only=0, stream=None)
 BIAS = HISTORY | dict(slot=0, ids=16, values=16, count=3, stream=None)
 PENALTIES = (dict(logits=16, dtype=0, ld=100, sequences=2, depth=1, width=100, live=2, count=None) | HISTORY
              | dict(row_slots=16, rep=None, pres=None, freq=None, drafts=16, mask=None, words=0, out=32, out_dtype=0, ldo=100,
-                    stream=None))
+                    bound=None, stream=None))
 
 
 @pytest.mark.parametrize("change,match", BAD_HISTORY)
