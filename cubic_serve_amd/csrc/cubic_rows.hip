@@ -225,8 +225,10 @@ hipError_t launch_norm(const RowArgs& a, hipStream_t s) {
 
 template <bool F16>
 hipError_t launch_quantize(const RowArgs& a, hipStream_t s) {
-    const int vectors = (a.k + kVec - 1) / kVec, wide = (vectors + 15) / 16 * 16;
-    const unsigned across = wide < 256 ? wide : 256, down = 256 / across;
+    // a row's vectors evenly over as few workgroups as hold them (1999 x 4104: 6.6 us, and
+    // 7.7 with a second workgroup per row for what 256 threads leave)
+    const int vectors = (a.k + kVec - 1) / kVec, chunks = (vectors + 255) / 256;
+    const unsigned across = ((vectors + chunks - 1) / chunks + 15) / 16 * 16, down = 256 / across;
     const int64_t rows = (a.m + down - 1) / down, most = 1 << 16;
     const dim3 block(across, down), grid((unsigned)(rows < most ? rows : most), (vectors + across - 1) / across);
     if (a.other) quantize_kernel<F16, true><<<grid, block, 0, s>>>(a);
