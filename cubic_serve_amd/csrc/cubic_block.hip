@@ -28,6 +28,7 @@ namespace {
 
 typedef int v8i __attribute__((ext_vector_type(8)));
 typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v2f __attribute__((ext_vector_type(2)));
 constexpr int kBlockBytes = 2048;              // one tile and block
 constexpr int kGroupBytes = 8 * kBlockBytes;   // 128 rows of one block
 constexpr uint32_t kPastEnd = 0x80000000u;     // a buffer offset past every extent
@@ -180,51 +181,85 @@ __device__ __forceinline__ int turn(int r) { return (r >> 1 & 3) | ((r ^ r >> 3)
 typedef __attribute__((address_space(3))) void lds_void_t;
 typedef const __attribute__((address_space(1))) void global_void_t;
 
-// s_waitcnt vmcnt(n), the other counters left alone
+// s_waitcnt vmcnt(n) lgkmcnt(0), and vmcnt(n) alone
+constexpr int step_waits(int n) { return (n & 0xF) | (0x7 << 4) | ((n >> 4) << 14); }
 constexpr int vm_waits(int n) { return (n & 0xF) | (0x7 << 4) | (0xF << 8) | ((n >> 4) << 14); }
+
+constexpr int leave_pitch(int ntw) { return 16 * ntw + 4; }  // of 32-bit sums
+
+// Workgroups go round robin over the eight XCDs; an XCD takes consecutive items of an
+// order that goes through 8 column groups for a row group, then the next rows, so that
+// those it has at one time share operands in its L2.
+__device__ __forceinline__ int xcd_item(int id, int total) {
+    const int per = total >> 3, rest = total & 7, xcd = id & 7;
+    return xcd * per + min(xcd, rest) + (id >> 3);
+}
+
+struct TileAt {
+    int m0, tile0, member;  // first row, first tile of 16 columns of that member
+};
+
+__device__ __forceinline__ TileAt tile_at(const BlockGemmArgs& a, int id, int row_groups, int M, int N) {
+    const int cols = a.group_end[a.members - 1], band = id / (8 * row_groups), wide = min(8, cols - 8 * band);
+    id -= band * 8 * row_groups;
+    const int group = 8 * band + id % wide, j = find_member(a, group);
+    return {id / wide * (16 * M), (group - (j ? a.group_end[j - 1] : 0)) * N, j};
+}
+
+// A wave's sums, 16 rows at a time through a run of LDS of its own (`out`), to leave in whole lines.
+template <int NTW, int MTW>
+__device__ __forceinline__ void leave(const BlockGemmArgs& a, const BlockMember& w, int m_first, int n0, const v4f (&acc)[NTW][MTW], float* out) {
+    constexpr int kPitch = leave_pitch(NTW);
+    const int lane = threadIdx.x & 63, quarter = lane >> 4, row = lane & 15;
+#pragma unroll
+    for (int i = 0; i < MTW; ++i) {
+#pragma unroll
+        for (int t = 0; t < NTW; ++t) *reinterpret_cast<v4f*>(out + row * kPitch + t * 16 + quarter * 4) = acc[t][i];
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll 1
+        for (int at = lane; at < 64 * NTW; at += 64) {
+            const int r = at / (4 * NTW), c = at % (4 * NTW) * 4, m = m_first + i * 16 + r;
+            if (m < a.m) store4(a, w, m, n0 + c, *reinterpret_cast<const v4f*>(out + r * kPitch + c));
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
+}
 
 template <int NTW, int MTW, int WN, int WM, int S, int G, int EU, bool SPLIT>
 __global__ __launch_bounds__(G * WN * WM * 64) __attribute__((amdgpu_waves_per_eu(EU, EU)))
 void block_tile_kernel(BlockGemmArgs a) {
     constexpr int W = WN * WM, N = NTW * WN, M = MTW * WM;  // waves of a group; tiles of 16
     static_assert(8 % NTW == 0, "a wave's columns share a scale");
-    static_assert(2 * M % W == 0 && 2 * N % W == 0 && S >= 2 && S <= 4, "loads are shared out evenly");
-    // A stage is x, w and the rows' scales of G blocks, one per group.  Each is an object of
-    // its own: a load into one then does not wait for reads of another.
-    constexpr int kW = M * kBlockBytes, kScales = kW + N * kBlockBytes, kStage = kScales + W * 256;
+    static_assert(2 * M % W == 0 && 2 * N % W == 0 && (S == 3 || S == 4), "loads are shared out evenly");
+    // A stage is x and w of G blocks, one per group; the rows' scales are for S blocks of a
+    // group, four places a row.  Each is an object of its own: a load into one then does not wait
+    // for reads of another.
+    constexpr int kW = M * kBlockBytes, kStage = kW + N * kBlockBytes;
     __shared__ __attribute__((aligned(1024))) uint8_t stage0[G * kStage], stage1[G * kStage], stage2[G * kStage], stage3[G * kStage];
+    __shared__ __attribute__((aligned(1024))) uint8_t row_scales[G * W * 256];
     auto stage_of = [&](auto stage) -> uint8_t* {
         constexpr int P = decltype(stage)::value;
         if constexpr (P == 0) return stage0; else if constexpr (P == 1) return stage1; else if constexpr (P == 2) return stage2; else return stage3;
     };
-    constexpr int kLoads = 2 * M / W + 2 * N / W + 1;  // to LDS, per wave and block
-    constexpr int kScaleRows = 16 * M / W, kScaleLanes = 64 / kScaleRows;  // whose scales a wave loads, lanes for each
-    static_assert(64 % kScaleRows == 0 && kScaleRows >= 16, "");
+    constexpr int kLoads = 2 * M / W + 2 * N / W;  // to LDS, per wave and block
+    static_assert(M == W, "a wave loads the scales of 16 rows, four lanes each");
     const int lane = threadIdx.x & 63, wave_of_all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wave = wave_of_all % W, k_group = wave_of_all / W;
     const int quarter = lane >> 4, row = lane & 15;
     const int wn = wave % WN, wm = wave / WN;
 
-    // Workgroups go round robin over the eight XCDs; an XCD takes consecutive items of an
-    // order that goes through 8 column groups for a row group, then the next
-    // rows, so that those it has at one time share operands in its L2.
-    const int cols = a.group_end[a.members - 1], row_groups = (a.m + 16 * M - 1) / (16 * M);
-    const int tiles = cols * row_groups;
-    int id = blockIdx.x;
-    {
-        const int total = SPLIT ? tiles * a.split : tiles, per = total >> 3, rest = total & 7, xcd = id & 7;
-        id = xcd * per + min(xcd, rest) + (id >> 3);
-    }
+    const int row_groups = (a.m + 16 * M - 1) / (16 * M), tiles = a.group_end[a.members - 1] * row_groups;
+    int id = xcd_item(blockIdx.x, SPLIT ? tiles * a.split : tiles);
     const int part = SPLIT ? id / tiles : 0;  // of K
     if constexpr (SPLIT) id -= part * tiles;
     const int tile_id = id;
-    const int band = id / (8 * row_groups), wide = min(8, cols - 8 * band);
-    id -= band * 8 * row_groups;
-    const int m0 = id / wide * (16 * M);
-    const int group = 8 * band + id % wide;
-    const int j = find_member(a, group);
-    const BlockMember& w = a.member[j];
-    const int tile0 = (group - (j ? a.group_end[j - 1] : 0)) * N;
+    const TileAt at_tile = tile_at(a, id, row_groups, M, N);
+    const int m0 = at_tile.m0, tile0 = at_tile.tile0;
+    const BlockMember& w = a.member[at_tile.member];
 
     // --- loads to LDS: of a wave's 2 M / W half tiles of x and 2 N / W of w -----------
     // Every tile of rows has a buffer of its own, moved on by the block: what a lane
@@ -235,7 +270,7 @@ void block_tile_kernel(BlockGemmArgs a) {
     const uint32_t w_at = lane * 16;
     const uint32_t x_at[2] = {(uint32_t)(load_row * a.ldx) + 16u * load_chunk[0], (uint32_t)((load_row + 8) * a.ldx) + 16u * load_chunk[1]};
     const int x_columns[2] = {a.k - 16 * load_chunk[0], a.k - 16 * load_chunk[1]};
-    const float* sx = a.x_scales + (int64_t)min(m0 + wave * kScaleRows + lane / kScaleLanes, a.m - 1) * a.scale_row;
+    const float* sx = a.x_scales + (int64_t)min(m0 + wave * 16 + (lane >> 2), a.m - 1) * a.scale_row;
     // per load of a wave: its tile's start, and its extent
     constexpr int kX = M % W == 0 ? M / W : 1, kWt = N % W == 0 ? N / W : 1;  // tiles a wave loads (or half of)
     const uint8_t *x_from[kX], *w_from[kWt];
@@ -286,10 +321,12 @@ void block_tile_kernel(BlockGemmArgs a) {
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(wr, (lds_void_t*)(wl + wave * 1024), 16, w_at + (wave & 1) * 1024, 0, 0, 0);
             }
         }
-        // (each scale by neighbouring lanes, one access where a row's scales lie together; by
-        // some of the lanes alone, under a branch, the 333 rows below take 11.2 us, not 9.7)
-        __builtin_amdgcn_global_load_lds((global_void_t*)(sx + (int64_t)min(b, blocks - 1) * scale_group),
-                                         (lds_void_t*)(xl + kScales + wave * 256), 4, 0, 0);
+    };
+    // Those of a group's next S blocks at a time: where a row's lie together, four lanes
+    // are one access (a block at a time, 64 x 151936 x 4096 takes 134 us and not 129)
+    auto load_scales = [&](int b) {
+        __builtin_amdgcn_global_load_lds((global_void_t*)(sx + (int64_t)min(b + (lane & 3) * G, blocks - 1) * scale_group),
+                                         (lds_void_t*)((__attribute__((address_space(3))) uint8_t*)(void*)row_scales + (k_group * W + wave) * 256), 4, 0, 0);
     };
 
     v4f acc[NTW][MTW];
@@ -303,24 +340,26 @@ void block_tile_kernel(BlockGemmArgs a) {
     const uint32_t x_slot = (uint32_t)(wm * MTW * kBlockBytes) + (uint32_t)(8 * row + (quarter ^ turn(row))) * 16;
     const uint32_t x_half = x_slot ^ 64;  // of its second half block
     const uint32_t w_slot = (uint32_t)(wn * NTW * kBlockBytes) + lane * 16;
-    const uint32_t s_slot = (uint32_t)(wm * MTW * 16 + row) * kScaleLanes;  // row r is lane r * kScaleLanes of all waves' loads
+    const float* const row_scale = reinterpret_cast<const float*>(row_scales + k_group * W * 256) + (wm * MTW * 16 + row) * 4;
     auto fragment = [](const uint8_t* at) {
         return join(*reinterpret_cast<const u32x4_dev_t*>(at), *reinterpret_cast<const u32x4_dev_t*>(at + 1024));
     };
 
-    // A product is added to its sum kLag products later, in the shadow of theirs.
-    constexpr int kLag = 2;
+    // A product is added to its sum kLag products later, in the shadow of theirs (1024 x 8192 x 4096:
+    // 43.6 us for 2, 41.8 for 3).
+    constexpr int kLag = 3;
     // S - 1 steps' blocks are on their way.  A step begins where its blocks have landed and
     // every wave is done with the step before, into whose place the next load goes.
+    v4f scales[MTW];  // of a row's next S blocks
     auto step = [&](int at, auto stage) {
         constexpr int P = decltype(stage)::value;
         const int b = b_first + at * G + k_group;
         const uint8_t *xs = stage_of(stage) + k_group * kStage, *ws = xs + kW;
-        const float* ss = reinterpret_cast<const float*>(xs + kScales);
         float scale[MTW];
         v8i xv[MTW], wv[2];
         v4f p[kLag + 1];
-        __builtin_amdgcn_s_waitcnt(vm_waits((S - 2) * kLoads));
+        // (S - 2 steps' loads may be on their way, and the scales' that step 1 of S sends)
+        __builtin_amdgcn_s_waitcnt(vm_waits((S - 2) * kLoads + (P >= 2 ? 1 : 0)));
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
         const float block_scale = sw[G == 1 ? b : min(b, blocks - 1)];
@@ -331,7 +370,8 @@ void block_tile_kernel(BlockGemmArgs a) {
         wv[0] = fragment(ws + w_slot);
 #pragma unroll
         for (int i = 0; i < MTW; ++i) {
-            scale[i] = ss[s_slot + i * 16 * kScaleLanes] * block_scale;
+            if constexpr (P == 0) scales[i] = *reinterpret_cast<const v4f*>(row_scale + i * 64);
+            scale[i] = scales[i][P] * block_scale;
             if constexpr (G > 1) {  // groups past the last block add products of zeros under scale 0
                 asm("" : "+v"(scale[i]));
                 scale[i] = b < blocks ? scale[i] : 0.0f;
@@ -339,6 +379,7 @@ void block_tile_kernel(BlockGemmArgs a) {
         }
         __builtin_amdgcn_sched_barrier(0);
         dma(b + (S - 1) * G, std::integral_constant<int, (P + S - 1) % S>{});
+        if constexpr (P == 1) load_scales(b + (S - 1) * G);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int q = 0; q < NTW * MTW + kLag; ++q) {
@@ -359,6 +400,7 @@ void block_tile_kernel(BlockGemmArgs a) {
 #pragma unroll
             for (int i = 0; i < MTW; ++i) asm volatile("" : "+v"(acc[t][i]));
     };
+    load_scales(b_first + k_group);
     auto first = [&](auto... stages) { (dma(b_first + decltype(stages)::value * G + k_group, stages), ...); };
     typedef std::integral_constant<int, 0> I0;
     typedef std::integral_constant<int, 1> I1;
@@ -433,30 +475,196 @@ void block_tile_kernel(BlockGemmArgs a) {
                 for (int i = 0; i < MTW; ++i) acc[t][i] += load_device4(r, o * kTileBytes + at + (t * MTW + i) * 1024);
     }
 
-    // 16 rows at a time through a wave-private run of LDS, to leave in whole lines
-    constexpr int kPitch = 16 * NTW + 4;  // of 32-bit sums
-    static_assert((G > 1 ? W : W / 2) * 16 * kPitch * 4 <= G * kStage, "the waves' rows fit one stage, or two");
-    float* out = G > 1 ? reinterpret_cast<float*>(stage1) + wave * 16 * kPitch
-                       : reinterpret_cast<float*>(wave & 1 ? stage1 : stage0) + (wave >> 1) * 16 * kPitch;
-    const int n0 = (tile0 + wn * NTW) * 16;
-#pragma unroll
-    for (int i = 0; i < MTW; ++i) {
-#pragma unroll
-        for (int t = 0; t < NTW; ++t) *reinterpret_cast<v4f*>(out + row * kPitch + t * 16 + quarter * 4) = acc[t][i];
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-#pragma unroll 1
-        for (int at = lane; at < 64 * NTW; at += 64) {
-            const int r = at / (4 * NTW), c = at % (4 * NTW) * 4, m = m0 + (wm * MTW + i) * 16 + r;
-            if (m < a.m) store4(a, w, m, n0 + c, *reinterpret_cast<const v4f*>(out + r * kPitch + c));
-        }
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    }
+    constexpr int kRun = 16 * leave_pitch(NTW);
+    static_assert((G > 1 ? W : W / 2) * kRun * 4 <= G * kStage, "the waves' rows fit one stage, or two");
+    float* out = G > 1 ? reinterpret_cast<float*>(stage1) + wave * kRun
+                       : reinterpret_cast<float*>(wave & 1 ? stage1 : stage0) + (wave >> 1) * kRun;
+    leave(a, w, m0 + wm * MTW * 16, (tile0 + wn * NTW) * 16, acc, out);
 }
 
+// ---------------------------------------------------------------------------
+// The largest tile, 256 columns by 256 rows: eight waves of 128 x 64, K block by block.
+// 4096 x 8192 x 8192 in 230 us, 2.4 P operations a second; the matrix cores are busy for 56 % of
+// its cycles, and its loads bound it (262 us below are 180 without them, 255 without three
+// quarters of its additions).  160 KB hold two blocks of both operands, so a place is loaded
+// again as soon as it is read: a wave has all of x in registers at a block's start, and half of the
+// weights' columns at the half, where a second barrier lets the loads of the block after
+// next go; the other half's go at the next block's start.  Each is on its way for one and a half
+// blocks.  The rows' scales come four blocks at a time, 16 bytes of a row.  With one
+// barrier, loads a block ahead and scales by the block, which are then a third of the lines
+// asked for: 262 us (of column-major scales 240, and 233 with loads as here).  The two
+// waves of a SIMD half a block apart, one reading while the other multiplies: 240.
+// ---------------------------------------------------------------------------
+constexpr int kWideTiles = 16, kScaleBlocks = 4;  // of 16 rows, or columns; scales of a row at a time
+
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2)))
+void block_wide_kernel(BlockGemmArgs a) {
+    constexpr int NTW = 8, MTW = 4, WN = 2;
+    // objects of their own: a load into one does not wait for reads of another
+    __shared__ __attribute__((aligned(1024))) uint8_t x0[32768], x1[32768], lo0[16384], lo1[16384], hi0[16384], hi1[16384];
+    __shared__ __attribute__((aligned(1024))) uint8_t row_scales[256 * kScaleBlocks * 4];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int quarter = lane >> 4, row = lane & 15, wn = wave % WN, wm = wave / WN;
+    const int row_groups = (a.m + 255) / 256;
+    const TileAt at_tile = tile_at(a, xcd_item(blockIdx.x, a.group_end[a.members - 1] * row_groups), row_groups, kWideTiles, kWideTiles);
+    const int m0 = at_tile.m0, tile0 = at_tile.tile0;
+    const BlockMember& w = a.member[at_tile.member];
+    const int blocks = a.blocks;
+
+    // --- loads: two tiles of x per wave, a tile of each half of the columns, 32 rows' scales
+    // (extents and rows as in the kernel above)
+    const int load_row = lane >> 3;
+    const int load_chunk[2] = {(lane & 7) ^ turn(load_row), (lane & 7) ^ turn(load_row + 8)};
+    const uint32_t x_at[2] = {(uint32_t)(load_row * a.ldx) + 16u * load_chunk[0], (uint32_t)((load_row + 8) * a.ldx) + 16u * load_chunk[1]};
+    const int x_columns[2] = {a.k - 16 * load_chunk[0], a.k - 16 * load_chunk[1]};
+    const uint8_t *x_from[2], *w_from[2];
+    int x_bytes[2], w_bytes[2];
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+        const int first = m0 + 16 * (2 * wave + p), left = min(a.m - first, 16);
+        x_from[p] = a.x + (int64_t)first * a.ldx;
+        x_bytes[p] = left <= 0 ? 0 : (int)((left - 1) * a.ldx) + a.k;
+        const int tile = tile0 + (wave >> 2) * 8 + p * 4 + (wave & 3);
+        w_from[p] = w.codes + (int64_t)(tile >> 3) * blocks * kGroupBytes + (tile & 7) * kBlockBytes;
+        w_bytes[p] = tile < w.tiles ? kBlockBytes : 0;
+    }
+    const float* sx[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) sx[h] = a.x_scales + (int64_t)min(m0 + wave * 32 + h * 16 + (lane >> 2), a.m - 1) * a.scale_row;
+    typedef __attribute__((address_space(3))) uint8_t lds_t;
+    auto load_x = [&](int b, uint8_t* to, int p) {
+        const int k = b * kScaleBlock;
+        const uint32_t off[2] = {k < x_columns[0] ? x_at[0] : kPastEnd, k < x_columns[1] ? x_at[1] : kPastEnd};
+        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(x_from[p] + k), 0, max(x_bytes[p] - k, 0), 0x00020000);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void_t*)((lds_t*)(void*)to + (2 * wave + p) * kBlockBytes + h * 1024), 16, off[h], 0, 0, 0);
+    };
+    auto load_w = [&](int b, uint8_t* to, int half) {
+        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<uint8_t*>(w_from[half] + (int64_t)b * kGroupBytes), 0, b < blocks ? w_bytes[half] : 0, 0x00020000);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void_t*)((lds_t*)(void*)to + wave * kBlockBytes + h * 1024), 16, (uint32_t)lane * 16 + h * 1024, 0, 0, 0);
+    };
+    auto load_scales = [&](int b) {
+        const int64_t at = (int64_t)min(b + (lane & 3), blocks - 1) * a.scale_group;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            __builtin_amdgcn_global_load_lds((global_void_t*)(sx[h] + at), (lds_void_t*)((lds_t*)(void*)row_scales + wave * 512 + h * 256), 4, 0, 0);
+    };
+
+    // (w lies past the 64 KB that an LDS read's constant reaches: from a base beyond them all
+    // its places are constants, 30 registers fewer)
+    constexpr uint32_t kFar = 65536;
+    v4f acc[NTW][MTW];
+#pragma unroll
+    for (int t = 0; t < NTW; ++t)
+#pragma unroll
+        for (int i = 0; i < MTW; ++i) acc[t][i] = v4f{0.f, 0.f, 0.f, 0.f};
+    const __attribute__((address_space(4))) float* sw = (const __attribute__((address_space(4))) float*)(
+        w.scales + (int64_t)(min(tile0 + wn * NTW, w.tiles - 1) >> 3) * blocks);
+    const uint32_t x_slot = (uint32_t)(wm * MTW * kBlockBytes) + (uint32_t)(8 * row + (quarter ^ turn(row))) * 16;
+    uint32_t w_slot = kFar + (uint32_t)(wn * 4 * kBlockBytes) + lane * 16;
+    asm("" : "+v"(w_slot));
+    auto fragment = [&](const uint8_t* of, int t) {
+        return join(*reinterpret_cast<const u32x4_dev_t*>(of + (w_slot - kFar + t * kBlockBytes)), *reinterpret_cast<const u32x4_dev_t*>(of + (w_slot - kFar + t * kBlockBytes + 1024)));
+    };
+
+    // Per block b a wave loads, in this order: at its start hi(b + 1) (2 loads), at its half
+    // x(b + 2), lo(b + 2) (6) and, every fourth, the scales from b + 2 on (2).  The start needs the
+    // half's before last, the half the last start's: either way a start's and a half's may stay on their way.
+    constexpr int kLag = 3;  // (as above: 240 us for 2, 257 for 1)
+    float block_scale = sw[0];
+    v2f scales[MTW];  // of a block and the next
+    auto step = [&](int b, auto turn_of) {
+        constexpr int J = decltype(turn_of)::value, kAway = 8 + (J == 3 ? 2 : 0);
+        uint8_t *const xs = J & 1 ? x1 : x0, *const lo = J & 1 ? lo1 : lo0, *const hi = J & 1 ? hi1 : hi0;
+        float scale[MTW], next_scale = 0.0f;
+        v8i xv[MTW], wv[2];
+        v4f p[kLag + 1];
+        __builtin_amdgcn_s_waitcnt(step_waits(kAway));
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        wv[0] = fragment(lo, 0);
+#pragma unroll
+        for (int i = 0; i < MTW; ++i)
+            xv[i] = join(*reinterpret_cast<const u32x4_dev_t*>(xs + x_slot + i * kBlockBytes),
+                         *reinterpret_cast<const u32x4_dev_t*>(xs + (x_slot ^ 64) + i * kBlockBytes));
+        if constexpr (J % 2 == 0) {
+#pragma unroll
+            for (int i = 0; i < MTW; ++i) scales[i] = *reinterpret_cast<const v2f*>(row_scales + ((wm * MTW + i) * 16 + row) * 16 + J * 4);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int q = 0; q < NTW * MTW + kLag; ++q) {
+            const int t = q / MTW, i = q % MTW;
+            if (q == 3 * MTW) {
+                __builtin_amdgcn_s_waitcnt(step_waits(kAway));
+                __builtin_amdgcn_s_barrier();
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if (i == 0 && t + 1 < NTW) wv[(t + 1) & 1] = fragment(t + 1 < 4 ? lo : hi, (t + 1) % 4);
+            if (t < NTW) p[q % (kLag + 1)] = block_product(wv[t & 1], xv[i]);
+            if (q == kLag) {
+#pragma unroll
+                for (int j = 0; j < MTW; ++j) scale[j] = scales[j][J & 1] * block_scale;
+            }
+            if (q >= kLag) {
+                const int of = q - kLag;
+                v4f& sum = acc[of / MTW][of % MTW];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum[e] = fmaf(scale[of % MTW], p[of % (kLag + 1)][e], sum[e]);
+            }
+            // (here, so that no scalar load is on its way beside the LDS reads of a start:
+            // they share a counter, and it could only be waited to 0)
+            if (q == NTW * MTW - 1) next_scale = sw[min(b + 1, blocks - 1)];
+            if (q == 1) load_w(b + 1, J & 1 ? hi0 : hi1, 1);
+            if (q == 3 * MTW + 3) load_x(b + 2, xs, 0);
+            if (q == 4 * MTW+3) load_x(b + 2, xs, 1);
+            if (q == 5 * MTW + 3) load_w(b + 2, lo, 0);
+            if (J == 2 && q == 6 * MTW) load_scales(b + 2);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        block_scale = next_scale;
+        // the sums stay in this step (the compiler would move additions to the next one)
+#pragma unroll
+        for (int t = 0; t < NTW; ++t)
+#pragma unroll
+            for (int i = 0; i < MTW; ++i) asm volatile("" : "+v"(acc[t][i]));
+    };
+    load_scales(0);
+    load_x(0, x0, 0);
+    load_x(0, x0, 1);
+    load_w(0, lo0, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    load_w(0, hi0, 1);
+    __builtin_amdgcn_sched_barrier(0);
+    load_x(1, x1, 0);
+    load_x(1, x1, 1);
+    load_w(1, lo1, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    typedef std::integral_constant<int, 0> I0;
+    typedef std::integral_constant<int, 1> I1;
+    typedef std::integral_constant<int, 2> I2;
+    typedef std::integral_constant<int, 3> I3;
+    int b = 0;
+    for (; b + 4 <= blocks; b += 4) {
+        step(b, I0{});
+        step(b + 1, I1{});
+        step(b + 2, I2{});
+        step(b + 3, I3{});
+    }
+    if (b < blocks) step(b, I0{});
+    if (b + 1 < blocks) step(b + 1, I1{});
+    if (b + 2 < blocks) step(b + 2, I2{});
+    __builtin_amdgcn_s_waitcnt(0);  // the last loads (of nothing) have landed
+    __syncthreads();
+    constexpr int kRun = 16 * leave_pitch(NTW);
+    static_assert(3 * kRun * 4 <= 32768 && kRun * 4 <= 16384, "three waves' rows fit x0 or x1, one's the others");
+    uint8_t* const out = wave < 3 ? x0 + wave * kRun * 4 : wave < 6 ? x1 + (wave - 3) * kRun * 4 : wave < 7 ? lo0 : lo1;
+    leave(a, w, m0 + wm * MTW * 16, (tile0 + wn * NTW) * 16, acc, reinterpret_cast<float*>(out));
+}
 // Values [n, k] of any row stride to tiles; rows past n and columns past k are 0.
 __global__ __launch_bounds__(256) void block_prepare_kernel(const uint8_t* values, int64_t ld, int64_t n, int k,
                                                             int blocks, int64_t chunks, uint8_t* out) {
@@ -499,6 +707,11 @@ hipError_t launch_tile(BlockGemmArgs a, hipStream_t s) {
     return hipGetLastError();
 }
 
+hipError_t launch_wide(BlockGemmArgs a, hipStream_t s) {
+    block_wide_kernel<<<count_groups(a, kWideTiles) * ((a.m + 255) / 256), 512, 0, s>>>(a);
+    return hipGetLastError();
+}
+
 }  // namespace
 
 hipError_t launch_block_gemm(const BlockGemmArgs& a, hipStream_t s) {
@@ -506,7 +719,7 @@ hipError_t launch_block_gemm(const BlockGemmArgs& a, hipStream_t s) {
         case 1: return launch_tile<2, 2, 2, 2, 3, 1, 3>(a, s);
         case 2: return launch_tile<4, 2, 2, 2, 3, 1, 2>(a, s);
         case 3: return launch_tile<4, 4, 4, 2, 3, 1, 2>(a, s);
-        case 4: return launch_tile<8, 4, 2, 4, 2, 1, 2>(a, s);
+        case 4: return launch_wide(a, s);
         case 5: return a.split > 1 ? launch_tile<2, 2, 2, 2, 4, 2, 2, true>(a, s) : launch_tile<2, 2, 2, 2, 4, 2, 2>(a, s);
         default: break;
     }
