@@ -68,18 +68,19 @@ __device__ __forceinline__ void store8(uint16_t* row, int c, int k, bool vec, co
     }
 }
 
-// exp(-g) in binary32: 2^t with t = -g log2(e) in two parts, so that the error does
-// not grow with |g|.
-__device__ __forceinline__ float exp_minus(float g) {
+// silu(g) x, from exp(-|g|) = 2^t with t = -|g| log2(e) in two parts, so that the error
+// does not grow with |g|.  Past 64 below zero silu(g) = g exp(g), under 2^128, which x brings
+// back to the 32-bit numbers: half of those powers of two are taken off x, half off the product.
+__device__ __forceinline__ float gated(float g, float x) {
     constexpr float kHi = 1.44269502162933349609375f, kLo = 1.92596299112661746887e-8f;  // log2(e)
-    const float t = -g * kHi;
-    const float rest = fmaf(-g, kHi, -t) + -g * kLo;
-    const float e = __builtin_amdgcn_exp2f(t);
-    const float whole = fmaf(e, rest * 0.693147182464599609375f, e);
-    return e < __builtin_huge_valf() ? whole : e;
+    const float a = fabsf(g), t = -a * kHi;
+    const float rest = fmaf(-a, kHi, -t) + -a * kLo;
+    const bool far = a > 64.0f;
+    float e = __builtin_amdgcn_exp2f(far ? t + 128.0f : t);
+    e = e > 0.0f ? fmaf(e, rest * 0.693147182464599609375f, e) : e;  // (the rest of an infinite t is none)
+    const float down = far && g < 0.0f ? 0x1p-64f : 1.0f;
+    return (g < 0.0f ? g * e : g) * __builtin_amdgcn_rcpf(1.0f + (far ? 0.0f : e)) * (x * down) * down;
 }
-
-__device__ __forceinline__ float silu(float g) { return g * __builtin_amdgcn_rcpf(1.0f + exp_minus(g)); }
 
 // Quantises the eight columns of every lane; the 16 lanes of a DPP row hold a
 // group.  Every lane of the wave calls it.
@@ -198,7 +199,7 @@ __global__ __launch_bounds__(256) void quantize_kernel(RowArgs a) {
             float g[kVec];
             load8<F16>(static_cast<const uint16_t*>(a.other) + row * a.ldother, c, a.k, a.vec_other, g);
 #pragma unroll
-            for (int e = 0; e < kVec; ++e) y[e] = silu(g[e]) * y[e];
+            for (int e = 0; e < kVec; ++e) y[e] = gated(g[e], y[e]);
         }
         quantise8(a, row, c, y);
     }

@@ -7,7 +7,7 @@ that, and three products and the weights' offset follow: at most 2^-18 of y in a
 and its division, 2^-17 in all.  An e4m3 value is off by half a step, 2^-4 of it
 (2^-10 below 2^-6), from a value that is off by 2^-16.  silu(g): the exponent t is off
 by 2^-24 of 1 (its rest is added), exp2 and the reciprocal by 2^-22 each: within
-u(y); where exp(-g) overflows it is 0, off by less than 2^-110.
+u(y), also where exp(-g) is past the 32-bit numbers.
 """
 from __future__ import annotations
 
@@ -148,6 +148,21 @@ def test_quantize_values_at_the_edges():
     assert torch.isfinite(got[3]).all() and (got[3] > 0).all()
     assert torch.isfinite(got[4]).all() and (q.scales[4].double() == 2.0 ** -96 / 448).logical_or(
         (q.scales[4].double() - 2.0 ** -96 / 448).abs() <= 2.0 ** -96 / 448 * 2.0 ** -23).all()
+
+
+def test_gates_far_below_zero():
+    """silu(g) is below the 32-bit numbers, its product with x is not.  (Products by powers of two, exact, and
+    silu's error as above: u(y).)"""
+    gate = torch.linspace(-170, -60, 23)[:, None].repeat(1, 128).to(BF16).to(DEV)
+    gate[:, 1::2] += 3
+    gate[0, 0::2], gate[1] = 3.3e38, -3.3e38
+    for x in (2.0 ** 127, 2.0 ** 40, 1.0):
+        up = torch.full_like(gate, x)
+        up[0] = 1.0
+        q = blockscale.BlockScaledActivations.empty(*gate.shape, DEV)
+        OPS.bind_quantize(up, q, gate=gate).launch()
+        g = gate.double()
+        near8(q, g / (1 + torch.exp(-g)) * up.double())
 
 
 def test_rows_that_lie_far_apart():
