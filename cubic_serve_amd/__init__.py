@@ -13,6 +13,11 @@ For batches whose requests differ: ``adapters`` -- a low-rank adapter per
 request beside a shared projection (PackedLinearOperators.bind_adapters,
 bind_adapted_linear), and ``sampling.VocabSamplingPlan`` -- a token per row from
 the whole vocabulary under each request's own settings.
+
+Around them: ``blockscale`` -- row norms, 8-bit activations and block-scaled
+8-bit products (PackedLinearOperators.bind_norm, bind_quantize,
+bind_block_linear), and ``penalties`` -- penalties, biases and grammar masks on
+logits over histories of tokens.
 """
 from .quantization import (  # noqa: F401
     CUBIC_FORMAT,

@@ -1044,12 +1044,12 @@ struct BlockPlan {
 };
 // Up to 8 rows the stream kernel, else the tiles (columns x rows) whose rounds over 256
 // CUs are expected to end first, by what a block of K takes a round, in hundredths of a us:
-//   64 x 64 27, 128 x 64 36 and 10 more, 256 x 128 120, 256 x 256 200
-// 4096 x 8192 x 8192: 548, 371, 292 and 249 us; 1024 rows x 8192 x 4096: 72, 53, 42 and 61; 512 x
-// 4096 x 4096: 21, 18.6, - and 57; 256 x 4096 x 12288: 34, 43, - and 153.  64 x 64 tiles that one
-// round holds have two groups of waves, each every other block of K: 256 x 4096 x 12288 30
-// and 34 us, 64 x 6144 x 4096 11.2 and 11.7, 333 x 1024 x 2064 8.2 and 8.0.  Rows of 6144 x 4096,
-// stream and tiles: 1 6.5 and 10.4, 8 10.3 and 10.4, 16 12.5 and 10.6.
+//   64 x 64 24, 128 x 64 36 and 10 more, 256 x 128 112, 256 x 256 180
+// 4096 x 8192 x 8192: 432, 378, 283 and 229 us; 1024 rows x 8192 x 4096: 58, 50, 40 and 52; 512 x
+// 4096 x 4096: 17.7, 17.8, 33 and 50; 256 x 4096 x 12288: 32, 40, 82 and 126.  64 x 64 tiles that one
+// round holds have two groups of waves, each every other block of K: 256 x 4096 x 12288 32
+// and 26 us, 64 x 6144 x 4096 12.7 and 11.4, 333 x 1024 x 2064 7.9 and 7.7.  Rows of 6144 x 4096,
+// stream and tiles: 1 8.5 and 12.0, 8 10.8 and 10.7, 16 13.1 and 10.7.
 BlockPlan plan_block(int64_t m, int64_t k, int members, const int64_t* ns) {
     BlockPlan p = {0, 1, 0, 0, 0};
     if (m <= 8) return p;
@@ -1060,12 +1060,12 @@ BlockPlan plan_block(int64_t m, int64_t k, int members, const int64_t* ns) {
     };
     const int64_t small = tiles(64, 64), blocks = ceil_div(k, cubic::kScaleBlock);
     auto rounds = [&](int columns, int rows) { return ceil_div(tiles(columns, rows), 256); };
-    const int64_t cost[] = {27 * rounds(64, 64), 10 + 36 * rounds(128, 64), 120 * rounds(256, 128), 200 * rounds(256, 256)};
+    const int64_t cost[] = {24 * rounds(64, 64), 10 + 36 * rounds(128, 64), 112 * rounds(256, 128), 180 * rounds(256, 256)};
     p.tile = 1 + (int)(std::min_element(cost, cost + 4) - cost);
     if (p.tile != 1 || small > 256) return p;
     // K in as many parts as leave one round, at most 4 of 8 blocks and more.  One part and
-    // this, weights in a cache and not: 64 rows x 4096 x 12288 28 and 15 us, 46 and 23; 64 x 1024 x 8192
-    // 17.6 and 10.4, 64 x 6144 x 4096 11.3 and 11.0, 16.7 and 13.6; 16 blocks 7.5 and 8.0.
+    // this, weights in a cache and not: 64 rows x 4096 x 12288 25 and 15 us, 38 and 20; 64 x 1024 x 8192
+    // 16 and 10, 17.6 and 10.6; 64 x 6144 x 4096 11.6 and 10.7, 15.6 and 13.9; 16 blocks 7.1 and 8.1.
     const int64_t split = blocks < 32 ? 1 : std::min({256 / small, blocks / 8, (int64_t)4});
     if (split > 1) {
         p.part_blocks = (int)ceil_div(ceil_div(blocks, split), 2) * 2;

@@ -123,6 +123,16 @@ def test_integers_are_exact(m, n, k):
     assert torch.equal(y.double(), wide(x) @ wide(w).t())
 
 
+@pytest.mark.parametrize("m,ns", [(200, [8100]), (1000, [8100]), (2050, [4000, 2001])])
+@pytest.mark.parametrize("k", [16, 144, 272, 512, 528, 768, 784, 1168])
+def test_every_number_of_blocks(m, ns, k):
+    """Tiles of 128, 256 and 256 columns by 64, 128 and 256 rows go through K in rounds of three and four blocks."""
+    print(f"block gemm m={m} ns={ns} k={k}", flush=True)
+    x, ws = activations(m, k, 21, column_major=k % 32 == 0, pad=16 * (k % 3)), [matrix(n, k, 22 + n) for n in ns]
+    for w, y in zip(ws, product(x, ws, BF16, pad=k % 5)):
+        check(x, w, y)
+
+
 @pytest.mark.parametrize("m", [2, 70, 400])
 def test_values_at_the_edges(m):
     k, n = 272, 140
