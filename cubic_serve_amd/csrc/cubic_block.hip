@@ -169,7 +169,7 @@ __global__ __launch_bounds__(kStreamWaves * 64) void block_stream_kernel(BlockGe
 // Many rows: the matrix cores bound it.  A workgroup has a tile of 16 NTW WN columns
 // by 16 MTW WM rows, WN x WM waves of 16 NTW x 16 MTW.  Both operands of a
 // block, and its row scales, go straight to LDS (buffer and global loads to LDS)
-// while the block before is multiplied.
+// while the block before is multiplied (PAST: weights past the caches).
 //
 // LDS order: weights as they were laid out, 16 bytes per lane in lane order.  x: of
 // a tile of 16 rows 128 slots of 16 bytes, row r's chunk c at slot 8 r + (c ^ turn(r)):
@@ -229,7 +229,7 @@ __device__ __forceinline__ void leave(const BlockGemmArgs& a, const BlockMember&
     }
 }
 
-template <int NTW, int MTW, int WN, int WM, int S, int G, int EU, bool SPLIT>
+template <int NTW, int MTW, int WN, int WM, int S, int G, int EU, bool SPLIT, bool PAST>
 __global__ __launch_bounds__(G * WN * WM * 64) __attribute__((amdgpu_waves_per_eu(EU, EU)))
 void block_tile_kernel(BlockGemmArgs a) {
     constexpr int W = WN * WM, N = NTW * WN, M = MTW * WM;  // waves of a group; tiles of 16
@@ -316,14 +316,14 @@ void block_tile_kernel(BlockGemmArgs a) {
             if constexpr (N % W == 0) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
-                    __builtin_amdgcn_raw_ptr_buffer_load_lds(wr, (lds_void_t*)(wl + (wave * kWt + p) * kBlockBytes + h * 1024), 16, w_at + h * 1024, 0, 0, 0);
+                    __builtin_amdgcn_raw_ptr_buffer_load_lds(wr, (lds_void_t*)(wl + (wave * kWt + p) * kBlockBytes + h * 1024), 16, w_at + h * 1024, 0, 0, PAST ? 2 : 0);
             } else {
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(wr, (lds_void_t*)(wl + wave * 1024), 16, w_at + (wave & 1) * 1024, 0, 0, 0);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(wr, (lds_void_t*)(wl + wave * 1024), 16, w_at + (wave & 1) * 1024, 0, 0, PAST ? 2 : 0);
             }
         }
     };
     // Those of a group's next S blocks at a time: where a row's lie together, four lanes
-    // are one access (a block at a time, 64 x 151936 x 4096 takes 134 us and not 129)
+    // are one access (a block at a time, 64 x 151936 x 4096 takes 134 us and not 129; PAST 125)
     auto load_scales = [&](int b) {
         __builtin_amdgcn_global_load_lds((global_void_t*)(sx + (int64_t)min(b + (lane & 3) * G, blocks - 1) * scale_group),
                                          (lds_void_t*)((__attribute__((address_space(3))) uint8_t*)(void*)row_scales + (k_group * W + wave) * 256), 4, 0, 0);
@@ -700,10 +700,10 @@ hipError_t launch_stream(BlockGemmArgs a, hipStream_t s) {
     return hipGetLastError();
 }
 
-template <int NTW, int MTW, int WN, int WM, int S, int G, int EU, bool SPLIT = false>
+template <int NTW, int MTW, int WN, int WM, int S, int G, int EU, bool SPLIT = false, bool PAST = false>
 hipError_t launch_tile(BlockGemmArgs a, hipStream_t s) {
     const unsigned tiles = count_groups(a, NTW * WN) * ((a.m + 16 * MTW * WM - 1) / (16 * MTW * WM));
-    block_tile_kernel<NTW, MTW, WN, WM, S, G, EU, SPLIT><<<SPLIT ? tiles * a.split : tiles, G * WN * WM * 64, 0, s>>>(a);
+    block_tile_kernel<NTW, MTW, WN, WM, S, G, EU, SPLIT, PAST><<<SPLIT ? tiles * a.split : tiles, G * WN * WM * 64, 0, s>>>(a);
     return hipGetLastError();
 }
 
@@ -715,17 +715,23 @@ hipError_t launch_wide(BlockGemmArgs a, hipStream_t s) {
 }  // namespace
 
 hipError_t launch_block_gemm(const BlockGemmArgs& a, hipStream_t s) {
+    int64_t tiles = 0;
+    for (int j = 0; j < a.members; ++j) tiles += a.member[j].tiles;
+    // Weights that the 256 MB cache cannot hold, read by one workgroup each, are read past
+    // it: 64 rows of 151936 x 4096 131 and 125 us, 128 rows 156 and 147; 64 rows of 65536 x 4096, which
+    // it all but holds, 45 and 56; by two workgroups, 128 rows of 24576 x 4096 in 64-row tiles, 39 and 41.
+    const bool large = tiles * a.blocks * kBlockBytes > (int64_t)300 << 20;
     switch (a.tile) {
         case 1: return launch_tile<2, 2, 2, 2, 3, 1, 3>(a, s);
-        case 2: return launch_tile<4, 2, 2, 2, 3, 1, 2>(a, s);
-        case 3: return launch_tile<4, 4, 4, 2, 3, 1, 2>(a, s);
+        case 2:
+            return large && a.m <= 64 ? launch_tile<4, 2, 2, 2, 3, 1, 2, false, true>(a, s) : launch_tile<4, 2, 2, 2, 3, 1, 2>(a, s);
+        case 3:
+            return large && a.m <= 128 ? launch_tile<4, 4, 4, 2, 3, 1, 2, false, true>(a, s) : launch_tile<4, 4, 4, 2, 3, 1, 2>(a, s);
         case 4: return launch_wide(a, s);
         case 5: return a.split > 1 ? launch_tile<2, 2, 2, 2, 4, 2, 2, true>(a, s) : launch_tile<2, 2, 2, 2, 4, 2, 2>(a, s);
         default: break;
     }
     // the more columns there are, the fewer times x is read
-    int64_t tiles = 0;
-    for (int j = 0; j < a.members; ++j) tiles += a.member[j].tiles;
     if (tiles >= 2048) return launch_stream<4>(a, s);
     return tiles >= 1024 ? launch_stream<2>(a, s) : launch_stream<1>(a, s);
 }

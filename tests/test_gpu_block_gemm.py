@@ -123,6 +123,14 @@ def test_integers_are_exact(m, n, k):
     assert torch.equal(y.double(), wide(x) @ wide(w).t())
 
 
+@pytest.mark.parametrize("m", [50, 128])
+def test_weights_larger_than_the_cache(m):
+    print(f"block gemm m={m} n=65000 k=4864", flush=True)
+    x, w = activations(m, 4864, 31, column_major=m == 50), matrix(65000, 4864, 32)
+    y, = product(x, [w], BF16)
+    check(x, w, y)
+
+
 @pytest.mark.parametrize("m,ns", [(200, [8100]), (1000, [8100]), (2050, [4000, 2001])])
 @pytest.mark.parametrize("k", [16, 144, 272, 512, 528, 768, 784, 1168])
 def test_every_number_of_blocks(m, ns, k):
