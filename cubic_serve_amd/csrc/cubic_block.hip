@@ -44,13 +44,13 @@ __device__ __forceinline__ v4f block_product(v8i w, v8i x) {
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, zero, 0, 0, 0, 0, 0, 0);
 }
 
-// Four columns of one row of y.
+// Four columns of one row of y (global memory takes 8 or 16 bytes at any element's address).
 __device__ __forceinline__ void store4(const BlockGemmArgs& a, const BlockMember& w, int64_t m, int n, v4f v) {
     if (n >= w.n) return;
     if (a.out == 2) {
         float* y = static_cast<float*>(w.y) + m * w.ldy + n;
-        if (w.vec && n + 4 <= w.n) {
-            *reinterpret_cast<v4f*>(y) = v;
+        if (n + 4 <= w.n) {
+            __builtin_memcpy(y, &v, sizeof v);
         } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
@@ -67,8 +67,9 @@ __device__ __forceinline__ void store4(const BlockGemmArgs& a, const BlockMember
         hi = pack_bf16x2(v[2], v[3]);
     }
     uint16_t* y = static_cast<uint16_t*>(w.y) + m * w.ldy + n;
-    if (w.vec && n + 4 <= w.n) {
-        *reinterpret_cast<uint2*>(y) = make_uint2(lo, hi);
+    if (n + 4 <= w.n) {
+        const uint32_t u[2] = {lo, hi};
+        __builtin_memcpy(y, u, sizeof u);
     } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i)

@@ -941,10 +941,6 @@ int cubic_logit_penalties(const void* logits, int dtype, int64_t row_stride, int
 // Row norms and 8-bit activations
 // ---------------------------------------------------------------------------
 namespace {
-bool vectors(const void* p, int64_t ld, int64_t m, int element) {
-    return ((uintptr_t)p & (8 * element - 1)) == 0 && (m == 1 || ld % 8 == 0);
-}
-
 // Whether no two (row, group) scales lie at one place.
 bool scales_apart(int64_t m, int64_t groups, int64_t row, int64_t group) {
     return (m == 1 || row >= 1) && (groups == 1 || group >= 1) && row <= ((int64_t)1 << 40) && group <= ((int64_t)1 << 40) &&
@@ -959,14 +955,12 @@ int rows_common(BoundCall& call, int dtype, void* bound, void* stream, const cha
     const int64_t least = a.k, most = (int64_t)1 << 40;
     const void* base[] = {a.x, a.other, a.y, a.sum, a.q};
     const int64_t ld[] = {a.ldx, a.ldother, a.ldy, a.ldsum, a.ldq};
-    int* const vec[] = {&a.vec_x, &a.vec_other, &a.vec_y, &a.vec_sum, &a.vec_q};
     for (int i = 0; i < 5; ++i) {
         if (!base[i]) continue;
         const int element = i == 4 ? 1 : 2;
         if (a.m > 1 && (ld[i] < least || ld[i] > most))
             return fail(CUBIC_EINVAL, "%s: row stride %lld of %lld columns", what, (long long)ld[i], (long long)least);
         if ((uintptr_t)base[i] % element) return fail(CUBIC_EINVAL, "%s: operand is not aligned to its element", what);
-        *vec[i] = vectors(base[i], ld[i], a.m, element);
     }
     if (a.q) {
         if (!a.scales || (uintptr_t)a.scales % 4) return fail(CUBIC_EINVAL, "%s: 8-bit rows need aligned scales", what);
@@ -1008,7 +1002,6 @@ int cubic_row_norm(const void* x, int64_t ldx, const void* residual, int64_t ldr
     a.scales = scales;
     a.scale_row = scale_row;
     a.scale_group = scale_group;
-    a.vec_weight = ((uintptr_t)weight & 15) == 0;
     return rows_common(call, dtype, bound, stream, "row norm");
 }
 
@@ -1140,8 +1133,7 @@ int cubic_block_gemm(const void* x, int64_t ldx, const float* x_scales, int64_t 
             return fail(CUBIC_EINVAL, "output leading dimension too small");
         if (!aligned16(prepared[j]) || (uintptr_t)scales[j] % 4 || (uintptr_t)ys[j] % element)
             return fail(CUBIC_EINVAL, "block gemm: misaligned operand of member %d", j);
-        a.member[j] = {(const uint8_t*)prepared[j], scales[j], ys[j], ldys[j], (int)ns[j], (int)ceil_div(ns[j], 16),
-                       ((uintptr_t)ys[j] & (4 * element - 1)) == 0 && (m == 1 || ldys[j] % 4 == 0)};
+        a.member[j] = {(const uint8_t*)prepared[j], scales[j], ys[j], ldys[j], (int)ns[j], (int)ceil_div(ns[j], 16)};
         tiles += a.member[j].tiles;
     }
     if (m > 8 && ceil_div(tiles, 4) * ceil_div(m, 64) >= (1 << 22))

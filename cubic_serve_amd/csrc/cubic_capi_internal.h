@@ -333,7 +333,6 @@ struct RowArgs {
     uint8_t* q;                   // [m, k] e4m3, or null
     float* scales;                // of group g of row r at r * scale_row + g * scale_group
     int64_t ldy, ldsum, ldq, scale_row, scale_group;
-    int vec_x, vec_other, vec_weight, vec_y, vec_sum, vec_q;  // whole vectors of eight may be accessed at once
 };
 hipError_t launch_rows(const RowArgs& a, hipStream_t s);
 
@@ -384,7 +383,6 @@ struct BlockMember {
     void* y;                      // [m, n], row stride ldy
     int64_t ldy;
     int n, tiles;
-    int vec;                      // four columns may be stored at once
 };
 struct BlockGemmArgs {
     const uint8_t* x;             // [m, k] e4m3, row stride ldx

@@ -469,8 +469,7 @@ CUBIC_API int cubic_logit_penalties(const void* logits, int dtype, int64_t row_s
  * The scale of group g of row r is at scales[r * scale_row + g * scale_group].
  * y is computed from h before its rounding.  A group that holds a NaN or an
  * infinity stands for NaNs.  Row strides in elements, at least k (any, for a
- * single row); every alignment to an element is taken, whole 16-byte (q: 8-byte)
- * rows are faster.  1 <= k <= 2^24; no workspace.
+ * single row), of any alignment to an element.  1 <= k <= 2^24; no workspace.
  * ------------------------------------------------------------------------- */
 CUBIC_API int cubic_row_norm(const void* x, int64_t ldx, const void* residual, int64_t ldresidual,
                              const void* weight, int64_t m, int64_t k, int dtype, float epsilon,
