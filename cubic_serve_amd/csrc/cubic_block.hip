@@ -29,6 +29,7 @@ namespace {
 typedef int v8i __attribute__((ext_vector_type(8)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef float v2f __attribute__((ext_vector_type(2)));
+typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 constexpr int kBlockBytes = 2048;              // one tile and block
 constexpr int kGroupBytes = 8 * kBlockBytes;   // 128 rows of one block
 constexpr uint32_t kPastEnd = 0x80000000u;     // a buffer offset past every extent
@@ -45,11 +46,17 @@ __device__ __forceinline__ v4f block_product(v8i w, v8i x) {
 }
 
 // Four columns of one row of y (global memory takes 8 or 16 bytes at any element's address).
+// LINES: past the caches where rows of y are whole lines, which a wave then writes whole: 64 rows
+// of 151936 x 4096 in 124 and 117 us, 2048 x 24576 x 4096 185 and 179; rows that share lines
+// (333 of 1521 x 2064) lose by it, 9.1 and 9.5.
+template <bool LINES = false>
 __device__ __forceinline__ void store4(const BlockGemmArgs& a, const BlockMember& w, int64_t m, int n, v4f v) {
     if (n >= w.n) return;
     if (a.out == 2) {
         float* y = static_cast<float*>(w.y) + m * w.ldy + n;
-        if (n + 4 <= w.n) {
+        if (LINES && w.lines) {
+            __builtin_nontemporal_store(v, reinterpret_cast<v4f*>(y));
+        } else if (n + 4 <= w.n) {
             __builtin_memcpy(y, &v, sizeof v);
         } else {
 #pragma unroll
@@ -67,9 +74,11 @@ __device__ __forceinline__ void store4(const BlockGemmArgs& a, const BlockMember
         hi = pack_bf16x2(v[2], v[3]);
     }
     uint16_t* y = static_cast<uint16_t*>(w.y) + m * w.ldy + n;
-    if (n + 4 <= w.n) {
-        const uint32_t u[2] = {lo, hi};
-        __builtin_memcpy(y, u, sizeof u);
+    const v2u u = {lo, hi};
+    if (LINES && w.lines) {
+        __builtin_nontemporal_store(u, reinterpret_cast<v2u*>(y));
+    } else if (n + 4 <= w.n) {
+        __builtin_memcpy(y, &u, sizeof u);
     } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -222,7 +231,7 @@ __device__ __forceinline__ void leave(const BlockGemmArgs& a, const BlockMember&
 #pragma unroll 1
         for (int at = lane; at < 64 * NTW; at += 64) {
             const int r = at / (4 * NTW), c = at % (4 * NTW) * 4, m = m_first + i * 16 + r;
-            if (m < a.m) store4(a, w, m, n0 + c, *reinterpret_cast<const v4f*>(out + r * kPitch + c));
+            if (m < a.m) store4<true>(a, w, m, n0 + c, *reinterpret_cast<const v4f*>(out + r * kPitch + c));
         }
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();

@@ -1133,7 +1133,8 @@ int cubic_block_gemm(const void* x, int64_t ldx, const float* x_scales, int64_t 
             return fail(CUBIC_EINVAL, "output leading dimension too small");
         if (!aligned16(prepared[j]) || (uintptr_t)scales[j] % 4 || (uintptr_t)ys[j] % element)
             return fail(CUBIC_EINVAL, "block gemm: misaligned operand of member %d", j);
-        a.member[j] = {(const uint8_t*)prepared[j], scales[j], ys[j], ldys[j], (int)ns[j], (int)ceil_div(ns[j], 16)};
+        a.member[j] = {(const uint8_t*)prepared[j], scales[j], ys[j], ldys[j], (int)ns[j], (int)ceil_div(ns[j], 16),
+                       (((uintptr_t)ys[j] | (uintptr_t)((m > 1 ? ldys[j] : 0) * element) | (uintptr_t)(ns[j] * element)) & 127) == 0};
         tiles += a.member[j].tiles;
     }
     if (m > 8 && ceil_div(tiles, 4) * ceil_div(m, 64) >= (1 << 22))

@@ -383,6 +383,7 @@ struct BlockMember {
     void* y;                      // [m, n], row stride ldy
     int64_t ldy;
     int n, tiles;
+    int lines;                    // rows of y are whole lines of 128 bytes
 };
 struct BlockGemmArgs {
     const uint8_t* x;             // [m, k] e4m3, row stride ldx
