@@ -494,8 +494,8 @@ void block_tile_kernel(BlockGemmArgs a) {
 
 // ---------------------------------------------------------------------------
 // The largest tile, 256 columns by 256 rows: eight waves of 128 x 64, K block by block.
-// 4096 x 8192 x 8192 in 230 us, 2.4 P operations a second; the matrix cores are busy for 58 % of
-// its cycles, and its loads bound it (262 us below are 180 without them, 255 without three
+// 4096 x 8192 x 8192 in 218 to 227 us, 2.5 P operations a second; the matrix cores are busy for 58 % of
+// its cycles, and its loads bound it, then the stores of y (20 us) (262 us below are 180 without them, 255 without three
 // quarters of its additions).  160 KB hold two blocks of both operands, so a place is loaded
 // again as soon as it is read: a wave has all of x in registers at a block's start, and half of the
 // weights' columns at the half, where a second barrier lets the loads of the block after

@@ -1038,7 +1038,7 @@ struct BlockPlan {
 // Up to 8 rows the stream kernel, else the tiles (columns x rows) whose rounds over 256
 // CUs are expected to end first, by what a block of K takes a round, in hundredths of a us:
 //   64 x 64 24, 128 x 64 36 and 10 more, 256 x 128 112, 256 x 256 180
-// 4096 x 8192 x 8192: 432, 378, 283 and 229 us; 1024 rows x 8192 x 4096: 58, 50, 40 and 52; 512 x
+// (before outputs went past the caches) 4096 x 8192 x 8192: 432, 378, 283 and 229 us; 1024 rows x 8192 x 4096: 58, 50, 40 and 52; 512 x
 // 4096 x 4096: 17.7, 17.8, 33 and 50; 256 x 4096 x 12288: 32, 40, 82 and 126.  64 x 64 tiles that one
 // round holds have two groups of waves, each every other block of K: 256 x 4096 x 12288 32
 // and 26 us, 64 x 6144 x 4096 12.7 and 11.4, 333 x 1024 x 2064 7.9 and 7.7.  Rows of 6144 x 4096,

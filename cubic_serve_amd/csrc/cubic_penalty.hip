@@ -17,12 +17,12 @@
 // What bounds the penalties: reading and writing the logits.  Listed tokens are a few
 // thousand of 10^5 columns, so each is looked up by itself, by the workgroup that has
 // its column: it reads the lists of its own columns only, and changes their logits in
-// LDS on their way.  256 rows of 151936, 3700 tokens listed for each: 44 us (48 under a
-// grammar), where a copy takes 31 and a history of no tokens 36; with listed tokens
-// changed in memory after the rest 69 (a grammar admits 2 % of them: 50), with
-// one list per slot, which every workgroup of a row has to search, 95.  Four rows of
-// a sequence one after the other in a workgroup, for their common list: 81 (too few
-// loads on their way).
+// LDS on their way.  256 rows of 151936, 3700 tokens listed for each: 42 us (38 under a
+// grammar, which admits 2 % of them), where a copy takes 31 and a history of no tokens 27.
+// What else was built, when this took 44 (its outputs went through the caches): listed tokens
+// changed in memory after the rest 69, one list per slot, which every workgroup of a row
+// has to search, 95, four rows of a sequence one after the other in a workgroup, for their common
+// list, 81 (too few loads on their way).
 #include <type_traits>
 
 #include "cubic_capi_internal.h"
@@ -144,6 +144,15 @@ __device__ __forceinline__ Eight<TYPE> load8(const void* p, int64_t i) {
 template <int TYPE>
 __device__ __forceinline__ void store8(void* p, int64_t i, const Eight<TYPE>& v) {
     __builtin_memcpy(static_cast<uint8_t*>(p) + i * (TYPE == 2 ? 4 : 2), &v, sizeof v);
+}
+// Past the caches: 256 rows of 151936 in 48 and 38 us; with a sampler behind them the same, 81.
+template <int TYPE>
+__device__ __forceinline__ void store8_past(void* p, int64_t i, const Eight<TYPE>& v) {
+    typedef uint32_t any_u32x4_t __attribute__((ext_vector_type(4), aligned(2)));
+    any_u32x4_t* to = reinterpret_cast<any_u32x4_t*>(static_cast<uint8_t*>(p) + i * (TYPE == 2 ? 4 : 2));
+#pragma unroll
+    for (int w = 0; w < (int)(sizeof v / 16); ++w)
+        __builtin_nontemporal_store(any_u32x4_t{v.u[4 * w], v.u[4 * w + 1], v.u[4 * w + 2], v.u[4 * w + 3]}, to + w);
 }
 // The same in another type (16 bits to 32).
 template <int IN, int OUT>
@@ -314,7 +323,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(8, 8))
             }
             const uint32_t keep = s.valid ? bits[i] : 0u;
             keep8<OUT>(out, keep, other);
-            if (!INPLACE || keep == 0u) store8<OUT>(a.out, out_at + start(i), out);
+            if constexpr (!INPLACE) store8_past<OUT>(a.out, out_at + start(i), out);
+            else if (keep == 0u) store8<OUT>(a.out, out_at + start(i), out);
             else if (keep != 0xFFu) store_some<OUT>(a.out, out_at + start(i), out, ~keep);
         }
         if (!whole && (int)threadIdx.x < columns) {
