@@ -150,6 +150,52 @@ def test_quantize_values_at_the_edges():
         (q.scales[4].double() - 2.0 ** -96 / 448).abs() <= 2.0 ** -96 / 448 * 2.0 ** -23).all()
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("m,k", [(3, 5), (5, 8), (4, 135), (2, 1032), (6, 4104), (2, 9161), (2, 33000)])
+def test_any_alignment(m, k, dtype):
+    """Operands that begin at any element, in rows of odd strides, whose neighbours stay as they are."""
+    print(f"alignment m={m} k={k} {dtype}", flush=True)
+
+    def inside(offset, pad, kind=dtype):
+        whole = torch.full((m, k + pad), 7.0, device=DEV).to(kind)
+        return whole, whole[:, offset:offset + k]
+
+    x, r = rows(m, k, dtype, 41, pad=3), inside(1, 5)[1].copy_(rows(m, k, dtype, 42))
+    w = rows(1, k + 1, dtype, 43)[0, 1:]
+    (all_y, y), (all_s, s), (all_q, values) = inside(3, 4), inside(5, 7), inside(1, 2, blockscale.E4M3)
+    q = blockscale.BlockScaledActivations(values, torch.empty((m, (k + 127) // 128), device=DEV))
+    OPS.bind_norm(x, w, epsilon=1e-5, residual=r, residual_output=s, output=y, quantized=q).launch()
+    h, want = norm_exact(x, r, w, 1e-5, 0.0)
+    near16(s, h, "sum")
+    near16(y, want, "y")
+    near8(q, want)
+    for whole, part in ((all_y, 3), (all_s, 5), (all_q, 1)):
+        assert (whole[:, :part].float() == 7).all() and (whole[:, part + k:].float() == 7).all()
+    OPS.bind_quantize(x, q, gate=r).launch()
+    g = r.double()
+    near8(q, g / (1 + torch.exp(-g)) * x.double())
+    assert (all_q[:, :1].float() == 7).all() and (all_q[:, 1 + k:].float() == 7).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("m,k", [(131200, 128), (33000, 520), (16500, 1017), (4200, 4097), (2100, 8200), (520, 32768), (250, 70001)])
+def test_outputs_past_the_caches(m, k, dtype):
+    print(f"large m={m} k={k} {dtype}", flush=True)
+    gen = torch.Generator(device=DEV).manual_seed(51)
+    x, r = (torch.randn((m, k), generator=gen, device=DEV).to(dtype) for _ in range(2))
+    w = rows(1, k, dtype, 52)[0].contiguous()
+    y, s = torch.empty_like(x), torch.empty_like(x)
+    q = blockscale.BlockScaledActivations.empty(m, k, DEV)
+    OPS.bind_norm(x, w, epsilon=1e-5, residual=r, residual_output=s, output=y, quantized=q).launch()
+    h, want = norm_exact(x, r, w, 1e-5, 0.0)
+    near16(s, h, "sum")
+    near16(y, want, "y")
+    near8(q, want)
+    OPS.bind_quantize(x, q, gate=r).launch()
+    g = r.double()
+    near8(q, g / (1 + torch.exp(-g)) * x.double())
+
+
 def test_gates_far_below_zero():
     """silu(g) is below the 32-bit numbers, its product with x is not.  (Products by powers of two, exact, and
     silu's error as above: u(y).)"""
