@@ -17,7 +17,7 @@
 // What bounds the penalties: reading and writing the logits.  Listed tokens are a few
 // thousand of 10^5 columns, so each is looked up by itself, by the workgroup that has
 // its column: it reads the lists of its own columns only, and changes their logits in
-// LDS on their way.  256 rows of 151936, 3700 tokens listed for each: 42 us (38 under a
+// LDS on their way.  256 rows of 151936, 3700 tokens listed for each: 39 us (38 under a
 // grammar, which admits 2 % of them), where a copy takes 31 and a history of no tokens 27.
 // What else was built, when this took 44 (its outputs went through the caches): listed tokens
 // changed in memory after the rest 69, one list per slot, which every workgroup of a row
@@ -210,7 +210,11 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(8, 8))
     __shared__ int drafts[kMaxPenaltyDepth];
     // (all rows' first chunks first: vocabularies begin with the tokens that come often, so
     // those have the long lists and should not come last)
-    const int row = blockIdx.x, chunk = blockIdx.y;
+    // The rows of a sequence, eight sequences at a time, on one XCD (workgroups go round robin
+    // over the eight): its lists and marks come from one L2 (the 39 us were 42).
+    int row = blockIdx.x;
+    const int chunk = blockIdx.y, band = 8 * (a.depth + 1), within = row % band;
+    if (row - within + band <= (int)gridDim.x) row = row - within + (within & 7) * (a.depth + 1) + (within >> 3);
     const int live = a.live_count ? min(max(*a.live_count, 0), a.live_sequences) : a.live_sequences;
     const int buckets = history_buckets(a.history.vocab);
     const int sequence = row / (a.depth + 1), ahead = row - sequence * (a.depth + 1);
