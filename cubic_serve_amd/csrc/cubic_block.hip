@@ -244,7 +244,7 @@ __global__ __launch_bounds__(G * WN * WM * 64) __attribute__((amdgpu_waves_per_e
 void block_tile_kernel(BlockGemmArgs a) {
     constexpr int W = WN * WM, N = NTW * WN, M = MTW * WM;  // waves of a group; tiles of 16
     static_assert(8 % NTW == 0, "a wave's columns share a scale");
-    static_assert(2 * M % W == 0 && 2 * N % W == 0 && (S == 3 || S == 4), "loads are shared out evenly");
+    static_assert(M == W && N % W == 0 && (S == 3 || S == 4), "a wave loads a tile of x, the scales of its rows, whole tiles of w");
     // A stage is x and w of G blocks, one per group; the rows' scales are for S blocks of a
     // group, four places a row.  Each is an object of its own: a load into one then does not wait
     // for reads of another.
@@ -255,8 +255,7 @@ void block_tile_kernel(BlockGemmArgs a) {
         constexpr int P = decltype(stage)::value;
         if constexpr (P == 0) return stage0; else if constexpr (P == 1) return stage1; else if constexpr (P == 2) return stage2; else return stage3;
     };
-    constexpr int kLoads = 2 * M / W + 2 * N / W;  // to LDS, per wave and block
-    static_assert(M == W, "a wave loads the scales of 16 rows, four lanes each");
+    constexpr int kWt = N / W, kLoads = 2 + 2 * kWt;  // tiles of w, and loads to LDS, per wave and block
     const int lane = threadIdx.x & 63, wave_of_all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wave = wave_of_all % W, k_group = wave_of_all / W;
     const int quarter = lane >> 4, row = lane & 15;
@@ -271,7 +270,7 @@ void block_tile_kernel(BlockGemmArgs a) {
     const int m0 = at_tile.m0, tile0 = at_tile.tile0;
     const BlockMember& w = a.member[at_tile.member];
 
-    // --- loads to LDS: of a wave's 2 M / W half tiles of x and 2 N / W of w -----------
+    // --- loads to LDS -------------------------------------------------------------------
     // Every tile of rows has a buffer of its own, moved on by the block: what a lane
     // adds to it is one number.  Rows past the last, columns past K and blocks past
     // the last read as zero.
@@ -281,19 +280,14 @@ void block_tile_kernel(BlockGemmArgs a) {
     const uint32_t x_at[2] = {(uint32_t)(load_row * a.ldx) + 16u * load_chunk[0], (uint32_t)((load_row + 8) * a.ldx) + 16u * load_chunk[1]};
     const int x_columns[2] = {a.k - 16 * load_chunk[0], a.k - 16 * load_chunk[1]};
     const float* sx = a.x_scales + (int64_t)min(m0 + wave * 16 + (lane >> 2), a.m - 1) * a.scale_row;
-    // per load of a wave: its tile's start, and its extent
-    constexpr int kX = M % W == 0 ? M / W : 1, kWt = N % W == 0 ? N / W : 1;  // tiles a wave loads (or half of)
-    const uint8_t *x_from[kX], *w_from[kWt];
-    int x_bytes[kX], w_bytes[kWt];
-#pragma unroll
-    for (int p = 0; p < kX; ++p) {
-        const int first = m0 + 16 * (M % W == 0 ? wave * kX + p : wave >> 1), left = min(a.m - first, 16);
-        x_from[p] = a.x + (int64_t)first * a.ldx;
-        x_bytes[p] = left <= 0 ? 0 : (int)((left - 1) * a.ldx) + a.k;
-    }
+    // a wave's tiles' starts and extents
+    const int x_first = m0 + 16 * wave, x_left = min(a.m - x_first, 16);
+    const uint8_t *const x_from = a.x + (int64_t)x_first * a.ldx, *w_from[kWt];
+    const int x_bytes = x_left <= 0 ? 0 : (int)((x_left - 1) * a.ldx) + a.k;
+    int w_bytes[kWt];
 #pragma unroll
     for (int p = 0; p < kWt; ++p) {
-        const int tile = tile0 + (N % W == 0 ? wave * kWt + p : wave >> 1);
+        const int tile = tile0 + wave * kWt + p;
         w_from[p] = w.codes + (int64_t)(tile >> 3) * a.blocks * kGroupBytes + (tile & 7) * kBlockBytes;
         w_bytes[p] = tile < w.tiles ? kBlockBytes : 0;
     }
@@ -307,29 +301,17 @@ void block_tile_kernel(BlockGemmArgs a) {
         const int k = b * kScaleBlock;
         const bool some = !SPLIT || b < blocks;
         const uint32_t off[2] = {some && k < x_columns[0] ? x_at[0] : kPastEnd, some && k < x_columns[1] ? x_at[1] : kPastEnd};
+        const __amdgpu_buffer_rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(x_from + k), 0, max(x_bytes - k, 0), 0x00020000);
 #pragma unroll
-        for (int p = 0; p < kX; ++p) {
-            const __amdgpu_buffer_rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc(
-                const_cast<uint8_t*>(x_from[p] + k), 0, max(x_bytes[p] - k, 0), 0x00020000);
-            if constexpr (M % W == 0) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    __builtin_amdgcn_raw_ptr_buffer_load_lds(xr, (lds_void_t*)(xl + (wave * kX + p) * kBlockBytes + h * 1024), 16, off[h], 0, 0, 0);
-            } else {  // half a tile per wave
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(xr, (lds_void_t*)(xl + wave * 1024), 16, wave & 1 ? off[1] : off[0], 0, 0, 0);
-            }
-        }
+        for (int h = 0; h < 2; ++h)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(xr, (lds_void_t*)(xl + wave * kBlockBytes + h * 1024), 16, off[h], 0, 0, 0);
 #pragma unroll
         for (int p = 0; p < kWt; ++p) {
             const __amdgpu_buffer_rsrc_t wr = __builtin_amdgcn_make_buffer_rsrc(
                 const_cast<uint8_t*>(w_from[p] + (int64_t)b * kGroupBytes), 0, b < blocks ? w_bytes[p] : 0, 0x00020000);
-            if constexpr (N % W == 0) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    __builtin_amdgcn_raw_ptr_buffer_load_lds(wr, (lds_void_t*)(wl + (wave * kWt + p) * kBlockBytes + h * 1024), 16, w_at + h * 1024, 0, 0, PAST ? 2 : 0);
-            } else {
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(wr, (lds_void_t*)(wl + wave * 1024), 16, w_at + (wave & 1) * 1024, 0, 0, PAST ? 2 : 0);
-            }
+            for (int h = 0; h < 2; ++h)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(wr, (lds_void_t*)(wl + (wave * kWt + p) * kBlockBytes + h * 1024), 16, w_at + h * 1024, 0, 0, PAST ? 2 : 0);
         }
     };
     // Those of a group's next S blocks at a time: where a row's lie together, four lanes
@@ -416,8 +398,7 @@ void block_tile_kernel(BlockGemmArgs a) {
     typedef std::integral_constant<int, 1> I1;
     typedef std::integral_constant<int, 2> I2;
     typedef std::integral_constant<int, 3> I3;
-    if constexpr (S == 2) first(I0{});
-    else if constexpr (S == 3) first(I0{}, I1{});
+    if constexpr (S == 3) first(I0{}, I1{});
     else first(I0{}, I1{}, I2{});
     // Whole rounds of the stages, then the rest: a loop of one exit, through which the
     // compiler follows which loads are on their way (with more it waits for all).
@@ -426,13 +407,11 @@ void block_tile_kernel(BlockGemmArgs a) {
     for (; at + S <= steps; at += S) {
         step(at, I0{});
         step(at + 1, I1{});
-        if constexpr (S > 2) step(at + 2, I2{});
+        step(at + 2, I2{});
         if constexpr (S > 3) step(at + 3, I3{});
     }
     if (at < steps) step(at, I0{});
-    if constexpr (S > 2) {
-        if (at + 1 < steps) step(at + 1, I1{});
-    }
+    if (at + 1 < steps) step(at + 1, I1{});
     if constexpr (S > 3) {
         if (at + 2 < steps) step(at + 2, I2{});
     }
