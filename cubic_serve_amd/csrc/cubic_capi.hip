@@ -1040,8 +1040,9 @@ struct BlockPlan {
 //   64 x 64 24, 128 x 64 36 and 10 more, 256 x 128 112, 256 x 256 180
 // (before outputs went past the caches) 4096 x 8192 x 8192: 432, 378, 283 and 229 us; 1024 rows x 8192 x 4096: 58, 50, 40 and 52; 512 x
 // 4096 x 4096: 17.7, 17.8, 33 and 50; 256 x 4096 x 12288: 32, 40, 82 and 126.  64 x 64 tiles that one
-// round holds have two groups of waves, each every other block of K: 256 x 4096 x 12288 32
-// and 26 us, 64 x 6144 x 4096 12.7 and 11.4, 333 x 1024 x 2064 7.9 and 7.7.  Rows of 6144 x 4096,
+// round holds have two groups of waves from 14 blocks on, each every other block of K: 256 x 4096 x
+// 12288 32 and 26 us, 64 x 6144 x 4096 12.7 and 11.4, 333 x 1521 x 2048 8.8 and 8.4, x 1536 7.8
+// and 7.7, x 1024 6.4 and 6.5, x 512 4.9 and 5.3.  Rows of 6144 x 4096,
 // stream and tiles: 1 8.5 and 12.0, 8 10.8 and 10.7, 16 13.1 and 10.7.
 BlockPlan plan_block(int64_t m, int64_t k, int members, const int64_t* ns) {
     BlockPlan p = {0, 1, 0, 0, 0};
@@ -1064,7 +1065,7 @@ BlockPlan plan_block(int64_t m, int64_t k, int members, const int64_t* ns) {
         p.part_blocks = (int)ceil_div(ceil_div(blocks, split), 2) * 2;
         p.split = (int)ceil_div(blocks, p.part_blocks);
     }
-    if (p.split > 1 || blocks >= 24) p.tile = 5;
+    if (p.split > 1 || blocks >= 14) p.tile = 5;
     if (p.split > 1) {
         p.counters = align256(small * 4);
         p.bytes = p.counters + small * p.split * 4096 * (int64_t)sizeof(float);
