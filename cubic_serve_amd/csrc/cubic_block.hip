@@ -45,6 +45,13 @@ __device__ __forceinline__ v4f block_product(v8i w, v8i x) {
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, zero, 0, 0, 0, 0, 0, 0);
 }
 
+// Four outputs in 16 bits.
+__device__ __forceinline__ v2u pack4(const BlockGemmArgs& a, v4f v) {
+    if (a.out == 1)
+        return v2u{float_to_f16_bits(v[0]) | float_to_f16_bits(v[1]) << 16, float_to_f16_bits(v[2]) | float_to_f16_bits(v[3]) << 16};
+    return v2u{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+}
+
 // Four columns of one row of y (global memory takes 8 or 16 bytes at any element's address).
 // LINES: past the caches where rows of y are whole lines, which a wave then writes whole: 64 rows
 // of 151936 x 4096 in 124 and 117 us, 2048 x 24576 x 4096 185 and 179; rows that share lines
@@ -65,25 +72,29 @@ __device__ __forceinline__ void store4(const BlockGemmArgs& a, const BlockMember
         }
         return;
     }
-    uint32_t lo, hi;
-    if (a.out == 1) {
-        lo = float_to_f16_bits(v[0]) | float_to_f16_bits(v[1]) << 16;
-        hi = float_to_f16_bits(v[2]) | float_to_f16_bits(v[3]) << 16;
-    } else {
-        lo = pack_bf16x2(v[0], v[1]);
-        hi = pack_bf16x2(v[2], v[3]);
-    }
+    const v2u u = pack4(a, v);
     uint16_t* y = static_cast<uint16_t*>(w.y) + m * w.ldy + n;
-    const v2u u = {lo, hi};
-    if (LINES && w.lines) {
-        __builtin_nontemporal_store(u, reinterpret_cast<v2u*>(y));
-    } else if (n + 4 <= w.n) {
+    if (n + 4 <= w.n) {
         __builtin_memcpy(y, &u, sizeof u);
     } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            if (n + i < w.n) y[i] = (uint16_t)((i < 2 ? lo : hi) >> (16 * (i & 1)));
+            if (n + i < w.n) y[i] = (uint16_t)(u[i >> 1] >> (16 * (i & 1)));
     }
+}
+
+// Eight columns in 16 bits, past the caches as above.
+__device__ __forceinline__ void store8(const BlockGemmArgs& a, const BlockMember& w, int64_t m, int n, v4f lo, v4f hi) {
+    if (n + 8 > w.n) {
+        store4(a, w, m, n, lo);
+        store4(a, w, m, n + 4, hi);
+        return;
+    }
+    const v2u l = pack4(a, lo), h = pack4(a, hi);
+    const u32x4_dev_t u = {l[0], l[1], h[0], h[1]};
+    uint16_t* y = static_cast<uint16_t*>(w.y) + m * w.ldy + n;
+    if (w.lines) __builtin_nontemporal_store(u, reinterpret_cast<u32x4_dev_t*>(y));
+    else __builtin_memcpy(y, &u, sizeof u);
 }
 
 // The member and its first tile of a column group.
@@ -228,10 +239,19 @@ __device__ __forceinline__ void leave(const BlockGemmArgs& a, const BlockMember&
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        if (a.out != 2) {  // (eight columns a lane: 2048 x 24576 x 4096 in 174 us by four, and 166)
+#pragma unroll
+            for (int at = lane; at < 32 * NTW; at += 64) {
+                const int r = at / (2 * NTW), c = at % (2 * NTW) * 8, m = m_first + i * 16 + r;
+                const v4f lo = *reinterpret_cast<const v4f*>(out + r * kPitch + c), hi = *reinterpret_cast<const v4f*>(out + r * kPitch + c + 4);
+                if (m < a.m) store8(a, w, m, n0 + c, lo, hi);
+            }
+        } else {
 #pragma unroll 1
-        for (int at = lane; at < 64 * NTW; at += 64) {
-            const int r = at / (4 * NTW), c = at % (4 * NTW) * 4, m = m_first + i * 16 + r;
-            if (m < a.m) store4<true>(a, w, m, n0 + c, *reinterpret_cast<const v4f*>(out + r * kPitch + c));
+            for (int at = lane; at < 64 * NTW; at += 64) {
+                const int r = at / (4 * NTW), c = at % (4 * NTW) * 4, m = m_first + i * 16 + r;
+                if (m < a.m) store4<true>(a, w, m, n0 + c, *reinterpret_cast<const v4f*>(out + r * kPitch + c));
+            }
         }
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
@@ -473,9 +493,9 @@ void block_tile_kernel(BlockGemmArgs a) {
 
 // ---------------------------------------------------------------------------
 // The largest tile, 256 columns by 256 rows: eight waves of 128 x 64, K block by block.
-// 4096 x 8192 x 8192 in 218 to 227 us, 2.5 P operations a second; the matrix cores are busy for 58 % of
-// its cycles, and its loads bound it, then the stores of y (20 us) (262 us below are 180 without them, 255 without three
-// quarters of its additions).  160 KB hold two blocks of both operands, so a place is loaded
+// 4096 x 8192 x 8192 in 207 to 217 us, 2.6 P operations a second; the matrix cores are busy for 58 % of
+// its cycles, and its loads bound it (262 us below are 180 without them, 255 without three quarters of its
+// additions), then the stores of y, two bursts of all CUs.  160 KB hold two blocks of both operands, so a place is loaded
 // again as soon as it is read: a wave has all of x in registers at a block's start, and half of the
 // weights' columns at the half, where a second barrier lets the loads of the block after
 // next go; the other half's go at the next block's start.  Each is on its way for one and a half
