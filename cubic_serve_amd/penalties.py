@@ -58,7 +58,15 @@ class TokenHistory:
         self.sizes = torch.zeros((slots, (vocab + BUCKET - 1) // BUCKET), dtype=torch.int32, device=device)
         self.device = self.state.device
         self._held = (self.state, self.listed, self.sizes)  # whose addresses bindings copy
-        self._args = (*(t.data_ptr() for t in self._held), slots, vocab)
+        self._args = (*self._tables(), slots, vocab)
+        self._storages = tuple(t.untyped_storage() for t in self._held)
+
+    def _tables(self) -> tuple[int, int, int]:
+        return self.state.data_ptr(), self.listed.data_ptr(), self.sizes.data_ptr()
+
+    def _check_tables(self) -> None:
+        if self._tables() != self._args[:3]:
+            raise ValueError("a history's tensors were replaced")
 
     def _check_slots(self, row_slots: Tensor) -> None:
         if not isinstance(row_slots, Tensor):
@@ -73,6 +81,7 @@ class TokenHistory:
         return slot
 
     def _call(self, name: str, *args) -> None:
+        self._check_tables()
         if self.device.type != "cuda":
             raise ValueError("a token history must be on a CUDA device")
         with _native.on_device(self.device.index):
@@ -179,6 +188,7 @@ class LogitPenaltyPlan:
         if logits.dtype not in _CANDIDATE_DTYPES or logits.device.type != "cuda" or not row_major(logits):
             raise ValueError("penalised logits must be row-major CUDA bf16, fp16 or fp32 [rows, V]")
         device = logits.device
+        history._check_tables()
         history._check_slots(slots)
         if history.device != device:
             raise ValueError("logits and history must be on one CUDA device")
@@ -232,6 +242,7 @@ class LogitPenaltyPlan:
         is read when the launch runs) keep their outputs."""
         if [f() for f in self._probes] != self._identity:
             raise ValueError("penalty operands changed after binding")
+        self.history._check_tables()
         index = self._index
         live = None if live_sequences is None else _live(live_sequences, self.sequences, self.history.device, "sequence")
         if live is None and _native.current_device() == index:

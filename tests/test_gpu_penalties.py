@@ -381,6 +381,19 @@ def test_verify_step_with_penalties():
         assert h.counts(s)[drafts[0, s]].item() == (2 if s % 2 == 0 else 1)
 
 
+def test_a_plan_whose_history_was_given_other_memory():
+    h = penalties.TokenHistory(2, 100, DEV)
+    logits, slots = torch.zeros((2, 100), dtype=BF16, device=DEV), torch.arange(2, dtype=torch.int32, device=DEV)
+    plan = penalties.LogitPenaltyPlan(logits=logits, history=h, slots=slots)
+    plan.launch()
+    h.state.data = h.state.clone()
+    for refused in (plan.launch, lambda: plan.launch(1), lambda: h.append(slots, slots), lambda: h.set_bias(0, [1], [1.0]),
+                    lambda: penalties.LogitPenaltyPlan(logits=logits, history=h, slots=slots)):
+        with pytest.raises(ValueError, match="replaced"):
+            refused()
+    assert not logits.any()
+
+
 def test_refusals():
     h = penalties.TokenHistory(3, 100, DEV)
     logits, slots = torch.zeros((3, 90), dtype=BF16, device=DEV), torch.zeros(3, dtype=torch.int32, device=DEV)

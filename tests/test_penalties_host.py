@@ -61,3 +61,14 @@ def test_history_on_the_host_is_refused():
     for slots, vocab in ((0, 10), (1 << 20, 10), (2, 0), (2, (1 << 24) + 1), (2.0, 10)):
         with pytest.raises(ValueError):
             penalties.TokenHistory(slots, vocab, "cpu")
+
+
+@pytest.mark.parametrize("name", ["state", "listed", "sizes"])
+def test_a_history_whose_tensors_were_replaced(name):
+    """Launches copy their addresses."""
+    given, reassigned = penalties.TokenHistory(2, 100, device="cpu"), penalties.TokenHistory(2, 100, device="cpu")
+    getattr(given, name).data = getattr(given, name).clone()
+    setattr(reassigned, name, getattr(reassigned, name).clone())
+    for history in (given, reassigned):
+        with pytest.raises(ValueError, match="replaced"):
+            history.clear(0)
