@@ -108,7 +108,7 @@ __device__ __forceinline__ int find_member(const BlockGemmArgs& a, int group) {
 // Up to 8 rows: the weight stream bounds it.  A workgroup has NT tiles of columns; its
 // waves take the blocks of K in turn, each block's weights and activations straight
 // into registers, DEPTH blocks ahead, no barrier until the waves' sums are added
-// through LDS, in the order of the waves.  1 row, 151936 x 4096: 118 us, 5.3 TB/s.
+// through LDS, in the order of the waves.  1 row, 20000 x 16384: 61 us, 5.4 TB/s.
 // ---------------------------------------------------------------------------
 template <int NT, int DEPTH>
 __global__ __launch_bounds__(kStreamWaves * 64) void block_stream_kernel(BlockGemmArgs a) {
@@ -729,7 +729,7 @@ hipError_t launch_block_gemm(const BlockGemmArgs& a, hipStream_t s) {
     // Weights that the 256 MB cache cannot hold, read by one workgroup each, are read past
     // it: 64 rows of 151936 x 4096 131 and 125 us, 128 rows 156 and 147; 64 rows of 65536 x 4096, which
     // it all but holds, 45 and 56; by two workgroups, 128 rows of 24576 x 4096 in 64-row tiles, 39 and 41.
-    const bool large = tiles * a.blocks * kBlockBytes > (int64_t)300 << 20;
+    const bool large = tiles * a.blocks * kBlockBytes > kPastCacheBytes;
     switch (a.tile) {
         case 1: return launch_tile<2, 2, 2, 2, 3, 1, 3>(a, s);
         case 2:

@@ -1035,7 +1035,7 @@ struct BlockPlan {
     int tile, split, part_blocks;
     int64_t counters, bytes;  // of the workspace
 };
-// Up to 8 rows the stream kernel, else the tiles (columns x rows) whose rounds over 256
+// Up to 8 rows the stream kernel (mostly), else the tiles (columns x rows) whose rounds over 256
 // CUs are expected to end first, by what a block of K takes a round, in hundredths of a us:
 //   64 x 64 24, 128 x 64 36 and 10 more, 256 x 128 112, 256 x 256 180
 // (before outputs went past the caches) 4096 x 8192 x 8192: 432, 378, 283 and 229 us; 1024 rows x 8192 x 4096: 58, 50, 40 and 52; 512 x
@@ -1046,13 +1046,20 @@ struct BlockPlan {
 // stream and tiles: 1 8.5 and 12.0, 8 10.8 and 10.7, 16 13.1 and 10.7.
 BlockPlan plan_block(int64_t m, int64_t k, int members, const int64_t* ns) {
     BlockPlan p = {0, 1, 0, 0, 0};
-    if (m <= 8) return p;
+    const int64_t blocks = ceil_div(k, cubic::kScaleBlock);
     auto tiles = [&](int columns, int rows) {
         int64_t groups = 0;
         for (int j = 0; j < members; ++j) groups += ceil_div(ns[j], columns);
         return groups * ceil_div(m, rows);
     };
-    const int64_t small = tiles(64, 64), blocks = ceil_div(k, cubic::kScaleBlock);
+    if (m <= 8) {
+        // Large weights in tiles that read past the cache, where every CU has two: 1 row of 151936 x
+        // 4096 114 us by the stream kernel and 100, 8 rows 129 and 113, 1 row of 80000 x 4096 61 and 59; of
+        // 20000 x 16384, 157 tiles, 61 and 71.
+        if (tiles(16, 8) * blocks * 2048 > cubic::kPastCacheBytes && tiles(128, 64) >= 512) p.tile = 2;
+        return p;
+    }
+    const int64_t small = tiles(64, 64);
     auto rounds = [&](int columns, int rows) { return ceil_div(tiles(columns, rows), 256); };
     const int64_t cost[] = {24 * rounds(64, 64), 10 + 36 * rounds(128, 64), 112 * rounds(256, 128), 180 * rounds(256, 256)};
     p.tile = 1 + (int)(std::min_element(cost, cost + 4) - cost);

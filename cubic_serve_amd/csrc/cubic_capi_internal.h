@@ -377,6 +377,7 @@ hipError_t launch_history_clear(const HistoryArgs& h, const int32_t* row_slots, 
 hipError_t launch_history_bias(const HistoryArgs& h, int slot, const int32_t* ids, const float* values, int n, hipStream_t s);
 
 // Block-scaled 8-bit products (cubic_block.hip)
+constexpr int64_t kPastCacheBytes = (int64_t)300 << 20;  // weights that the 256 MB cache does not hold
 struct BlockMember {
     const uint8_t* codes;         // tiles of 16 rows, laid out by launch_block_prepare
     const float* scales;          // [ceil(n / 128), blocks]

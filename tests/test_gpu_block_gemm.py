@@ -123,10 +123,10 @@ def test_integers_are_exact(m, n, k):
     assert torch.equal(y.double(), wide(x) @ wide(w).t())
 
 
-@pytest.mark.parametrize("m", [50, 128])
-def test_weights_larger_than_the_cache(m):
-    print(f"block gemm m={m} n=65000 k=4864", flush=True)
-    x, w = activations(m, 4864, 31, column_major=m == 50), matrix(65000, 4864, 32)
+@pytest.mark.parametrize("m,n,k", [(50, 65000, 4864), (128, 65000, 4864), (1, 66001, 4864), (7, 66001, 4864), (3, 20000, 16400)])
+def test_weights_larger_than_the_cache(m, n, k):
+    print(f"block gemm m={m} n={n} k={k}", flush=True)
+    x, w = activations(m, k, 31, column_major=m == 50), matrix(n, k, 32)
     y, = product(x, [w], BF16)
     check(x, w, y)
 
