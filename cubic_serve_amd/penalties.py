@@ -53,20 +53,21 @@ class TokenHistory:
         if type(vocab) is not int or not 1 <= vocab <= 1 << 24:
             raise ValueError("history vocabulary must be an int in 1..2^24")
         self.slots, self.vocab = slots, vocab
-        self.state = torch.zeros((slots, vocab, 2), dtype=torch.int32, device=device)
-        self.listed = torch.zeros((slots, vocab), dtype=torch.int32, device=device)
-        self.sizes = torch.zeros((slots, (vocab + BUCKET - 1) // BUCKET), dtype=torch.int32, device=device)
+        # (their addresses are copied by every launch)
+        self._tables = (torch.zeros((slots, vocab, 2), dtype=torch.int32, device=device),
+                        torch.zeros((slots, vocab), dtype=torch.int32, device=device),
+                        torch.zeros((slots, (vocab + BUCKET - 1) // BUCKET), dtype=torch.int32, device=device))
+        self._storages = tuple(t.untyped_storage() for t in self._tables)
         self.device = self.state.device
-        self._held = (self.state, self.listed, self.sizes)  # whose addresses bindings copy
-        self._args = (*self._tables(), slots, vocab)
-        self._storages = tuple(t.untyped_storage() for t in self._held)
+        self._args = (*(t.data_ptr() for t in self._tables), slots, vocab)
 
-    def _tables(self) -> tuple[int, int, int]:
-        return self.state.data_ptr(), self.listed.data_ptr(), self.sizes.data_ptr()
+    state = property(lambda self: self._tables[0])
+    listed = property(lambda self: self._tables[1])
+    sizes = property(lambda self: self._tables[2])
 
     def _check_tables(self) -> None:
-        if self._tables() != self._args[:3]:
-            raise ValueError("a history's tensors were replaced")
+        if tuple(t.data_ptr() for t in self._tables) != self._args[:3]:
+            raise ValueError("a history's tensors were given other memory")
 
     def _check_slots(self, row_slots: Tensor) -> None:
         if not isinstance(row_slots, Tensor):
@@ -232,7 +233,7 @@ class LogitPenaltyPlan:
         self._call = _native.BoundCall("cubic_logit_penalties", *self._head, self.sequences, None, *self._tail[:-1])
         # what a launch looks at: whether every operand still has its memory (which is held) and size
         self._held = tuple(t.untyped_storage() for t in operands)
-        self._probes = tuple(f for t in operands for f in (t.data_ptr, t.numel))
+        self._probes = (*(f for t in operands for f in (t.data_ptr, t.numel)), *(t.data_ptr for t in history._tables))
         self._identity = [f() for f in self._probes]
         self._index = device.index
 
@@ -242,7 +243,6 @@ class LogitPenaltyPlan:
         is read when the launch runs) keep their outputs."""
         if [f() for f in self._probes] != self._identity:
             raise ValueError("penalty operands changed after binding")
-        self.history._check_tables()
         index = self._index
         live = None if live_sequences is None else _live(live_sequences, self.sequences, self.history.device, "sequence")
         if live is None and _native.current_device() == index:
