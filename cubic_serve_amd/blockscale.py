@@ -299,6 +299,8 @@ def bind_block_linear_group(operators, x: BlockScaledActivations, weights: Seque
 
     Outputs are bf16, fp16 or fp32 (one type for all) and may have padded rows.
     K has to be a multiple of 16, x 16-byte aligned with rows of whole 16 bytes.
+    Weights are laid out as they are now (bindings of the same values share the layout);
+    after a change to one, bind again.
     The binding owns its workspace, cleared on the current stream: a launch on
     another one has to follow it, and launches of one binding must not overlap.
     """

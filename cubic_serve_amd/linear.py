@@ -62,17 +62,19 @@ DTYPE_IDS = {torch.bfloat16: 0, torch.float16: 1}  # CUBIC_DTYPE_BF16 / CUBIC_DT
 
 
 def _versions(matrix: QuantizedMatrix) -> tuple:
-    return tensor_versions(matrix.payload.values())
-
-
-def tensor_versions(tensors) -> tuple:
     versions = []
-    for tensor in tensors:
+    for tensor in matrix.payload.values():
         try:
             versions.append(tensor._version)
         except RuntimeError:  # inference-mode tensors
             versions.append(None)
     return tuple(versions)
+
+
+def _same_bits(a: Tensor, b: Tensor) -> bool:
+    """Whether two contiguous tensors of 32-bit words hold the same (NaNs too)."""
+    words = lambda t: t.view(-1).view(torch.int32)
+    return a.numel() == b.numel() and a.dtype is b.dtype and torch.equal(words(a), words(b))
 
 
 def prepare_matrix(matrix: QuantizedMatrix, device: torch.device | None = None,
@@ -364,13 +366,21 @@ class PackedLinearOperators:
         return prepared
 
     def prepared_block(self, weight, device: torch.device) -> tuple[Tensor, Tensor]:
-        """A BlockScaledMatrix as its products read it: (values laid out, scales)."""
+        """A BlockScaledMatrix as its products read it now: (values laid out, scales).
+
+        Laid out at every call: nothing about a tensor tells of every write to it
+        (``.data``, inference tensors).  Where the bits are those of the last layout, that
+        one serves, so a weight's bindings share one; else it is replaced here.  (0.2 ms for
+        4096 x 4096, 1.8 for 151936 x 4096.)
+        """
         from . import blockscale
 
-        key = ("block.mi355x.v1", id(weight), tensor_versions((weight.values, weight.scales)), str(device))
+        key = ("block.mi355x.v2", id(weight), str(device))
+        laid_out = blockscale.prepare_block_matrix(weight, device)
         cached = self.prepared_weights.get(key)
-        if cached is None:  # the weight is kept, so its id cannot be reused while cached
-            cached = self.prepared_weights[key] = (weight, blockscale.prepare_block_matrix(weight, device))
+        if cached is None or not all(map(_same_bits, cached[1], laid_out)):
+            # the weight is kept, so its id cannot be reused while cached
+            cached = self.prepared_weights[key] = (weight, laid_out)
         return cached[1]
 
     # -- validation (quantized.py:348-405) ------------------------------------

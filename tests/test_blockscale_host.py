@@ -154,3 +154,35 @@ def test_bound_calls():
         norm(bound=c.addressof(memory) + 4)
     with pytest.raises(ValueError, match="epsilon"):
         norm(eps=-1.0, bound=c.addressof(memory))
+
+
+def test_layouts_follow_their_weights(monkeypatch):
+    """Writes that neither a version nor an address shows; one layout is kept per weight, and shared while it holds."""
+    monkeypatch.setattr(blockscale, "prepare_block_matrix", lambda w, device: (w.values.clone().view(torch.uint8), w.scales.clone()))
+    ops, device = linear.PackedLinearOperators(), torch.device("cpu")
+    make = lambda v: torch.full((4, 256), v).to(E4M3)
+    w = blockscale.BlockScaledMatrix(make(1.0), torch.ones((1, 2)))
+    first = ops.prepared_block(w, device)
+    assert ops.prepared_block(w, device) is first
+
+    def inference(t):
+        with torch.inference_mode():
+            return t.clone()
+
+    def write(t):
+        with torch.inference_mode():
+            t.copy_(make(6.0))
+
+    changes = [lambda: w.values.copy_(make(2.0)), lambda: w.values.data.copy_(make(3.0)),
+               lambda: setattr(w.values, "data", make(4.0)), lambda: w.scales.data.fill_(5.0),
+               lambda: setattr(w.scales, "data", torch.full((1, 2), 6.0)), lambda: w.scales.data.fill_(float("nan"))]
+    for change in changes:
+        change()
+        values, scales = ops.prepared_block(w, device)
+        assert torch.equal(values, w.values.view(torch.uint8)) and torch.equal(scales.nan_to_num(-1), w.scales.nan_to_num(-1))
+        assert ops.prepared_block(w, device)[0] is values  # NaNs too are the same
+        assert len(ops.prepared_weights) == 1
+    w = blockscale.BlockScaledMatrix(inference(make(5.0)), inference(torch.ones((1, 2))))
+    ops.prepared_block(w, device)
+    write(w.values)
+    assert torch.equal(ops.prepared_block(w, device)[0], w.values.view(torch.uint8))

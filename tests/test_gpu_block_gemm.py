@@ -268,3 +268,25 @@ def test_refusals():
     with torch.cuda.graph(torch.cuda.CUDAGraph()):
         with pytest.raises(RuntimeError, match="before graph capture"):
             ops.bind_block_linear(x, w, y)
+
+
+def test_weights_written_past_autograd_are_prepared_again():
+    """Through .data, into an inference tensor: no version counts these."""
+    x, w = activations(4, 256, 41), matrix(64, 256, 42)
+    ops = linear.PackedLinearOperators()
+    y = torch.empty((4, 64), dtype=FP32, device=DEV)
+    ops.bind_block_linear(x, w, y).launch()
+    other = matrix(64, 256, 43)
+    for change in (lambda: w.values.data.copy_(other.values), lambda: w.scales.data.mul_(2),
+                   lambda: setattr(w.values, "data", matrix(64, 256, 44).values), lambda: setattr(w.scales, "data", w.scales * 3)):
+        change()
+        ops.bind_block_linear(x, w, y).launch()
+        check(x, w, y)
+        assert len(ops.prepared_weights) == 1
+    with torch.inference_mode():
+        w = matrix(64, 256, 45)
+        ops.bind_block_linear(x, w, y).launch()
+        w.values.copy_(other.values)
+        w.scales.mul_(0.5)
+        ops.bind_block_linear(x, w, y).launch()
+    check(x, w, y)
