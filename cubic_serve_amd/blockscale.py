@@ -58,6 +58,11 @@ class BlockScaledActivations:
     scales: Tensor
 
     def __post_init__(self):
+        self.check()
+
+    def check(self) -> None:
+        """Whether the scales are those of the values' extents, which a launch reads
+        (a tensor may have been given other memory since)."""
         if not isinstance(self.values, Tensor) or not isinstance(self.scales, Tensor):
             raise TypeError("block-scaled activations are two tensors")
         if self.values.dtype is not E4M3 or not _row_major(self.values):
@@ -89,6 +94,10 @@ class BlockScaledMatrix:
     scales: Tensor
 
     def __post_init__(self):
+        self.check()
+
+    def check(self) -> None:
+        """As BlockScaledActivations.check."""
         if not isinstance(self.values, Tensor) or not isinstance(self.scales, Tensor):
             raise TypeError("a block-scaled matrix is two tensors")
         if self.values.dtype is not E4M3 or not _row_major(self.values):
@@ -217,6 +226,7 @@ def _quantized(q: BlockScaledActivations | None, shape: tuple, device: torch.dev
         return (), (None, 0, None, 0, 0)
     if not isinstance(q, BlockScaledActivations):
         raise TypeError("an 8-bit output must be BlockScaledActivations")
+    q.check()
     if q.values.shape != shape or q.values.device != device:
         raise ValueError(f"an 8-bit output must be {list(shape)} on {device}")
     return (q.values, q.scales), (q.values.data_ptr(), _stride(q.values), q.scales.data_ptr(), *q.scales.stride())
@@ -278,6 +288,7 @@ def prepare_block_matrix(weight: BlockScaledMatrix, device: torch.device | None 
     (load time, allocates)."""
     if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
         raise RuntimeError("block-scaled weights require cold preparation before capture")
+    weight.check()
     device = torch.device(device) if device is not None else weight.device
     values = weight.values.to(device)
     n, k = weight.shape
@@ -311,6 +322,8 @@ def bind_block_linear_group(operators, x: BlockScaledActivations, weights: Seque
         raise TypeError("block-scaled linear requires BlockScaledActivations and BlockScaledMatrix")
     if any(not isinstance(y, Tensor) for y in outputs):
         raise TypeError("block-scaled linear outputs must be tensors")
+    for operand in (x, *weights):
+        operand.check()
     values, device = x.values, x.values.device
     m, k = values.shape
     if device.type != "cuda":

@@ -186,3 +186,21 @@ def test_layouts_follow_their_weights(monkeypatch):
     ops.prepared_block(w, device)
     write(w.values)
     assert torch.equal(ops.prepared_block(w, device)[0], w.values.view(torch.uint8))
+
+
+def test_tensors_that_grew_after_their_check():
+    """A launch would read scales past their end."""
+    make = lambda m: blockscale.BlockScaledActivations(torch.zeros((m, 64), dtype=E4M3), torch.ones((m, 1)))
+    weight = lambda: blockscale.BlockScaledMatrix(torch.zeros((4, 64), dtype=E4M3), torch.ones((1, 1)))
+    ops, y = linear.PackedLinearOperators(), torch.zeros((2, 4))
+    for grown, other in ((lambda q: q.values, (300, 64)), (lambda q: q.scales, (1, 3))):
+        x, w = make(2), weight()
+        grown(x).data = torch.zeros(other, dtype=grown(x).dtype)
+        for refused in (lambda: ops.bind_block_linear(x, w, y), lambda: blockscale._quantized(x, tuple(x.values.shape), x.values.device)):
+            with pytest.raises(ValueError, match="scales"):
+                refused()
+        x = make(2)
+        grown(w).data = torch.zeros(other, dtype=grown(w).dtype)
+        for refused in (lambda: ops.bind_block_linear(x, w, y), lambda: blockscale.prepare_block_matrix(w)):
+            with pytest.raises(ValueError, match="scales"):
+                refused()
