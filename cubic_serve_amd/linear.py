@@ -71,6 +71,11 @@ def _versions(matrix: QuantizedMatrix) -> tuple:
     return tuple(versions)
 
 
+def operand_identity(operands: Sequence[Tensor]) -> list:
+    """What a bound call took from its operands."""
+    return [(t.data_ptr(), t.shape, t.stride(), t.dtype) for t in operands]
+
+
 def _same_bits(a: Tensor, b: Tensor) -> bool:
     """Whether two contiguous tensors of 32-bit words hold the same (NaNs too)."""
     words = lambda t: t.view(-1).view(torch.int32)

@@ -19,6 +19,7 @@ import torch
 from torch import Tensor
 
 from . import _native
+from .linear import operand_identity
 from .sampling import _CANDIDATE_DTYPES
 
 MAX_DEPTH = 8  # kMaxPenaltyDepth of the C ABI
@@ -231,17 +232,20 @@ class LogitPenaltyPlan:
                       _CANDIDATE_DTYPES[outputs.dtype], stride(outputs), None)
         # the call with all sequences live
         self._call = _native.BoundCall("cubic_logit_penalties", *self._head, self.sequences, None, *self._tail[:-1])
-        # what a launch looks at: whether every operand still has its memory (which is held) and size
+        # what a launch looks at: whether every operand still has its memory (which is held) and layout
         self._held = tuple(t.untyped_storage() for t in operands)
-        self._probes = (*(f for t in operands for f in (t.data_ptr, t.numel)), *(t.data_ptr for t in history._tables))
-        self._identity = [f() for f in self._probes]
+        self._operands = tuple(operands)
+        self._identity = self._look()
         self._index = device.index
+
+    def _look(self) -> list:
+        return [*operand_identity(self._operands), *[t.data_ptr() for t in self.history._tables]]
 
     def launch(self, live_sequences: int | Tensor | None = None) -> None:
         """Enqueue on the current stream.  The rows of sequences at or past
         ``live_sequences`` (a host int, or a device int32 tensor whose first element
         is read when the launch runs) keep their outputs."""
-        if [f() for f in self._probes] != self._identity:
+        if self._look() != self._identity:
             raise ValueError("penalty operands changed after binding")
         index = self._index
         live = None if live_sequences is None else _live(live_sequences, self.sequences, self.history.device, "sequence")

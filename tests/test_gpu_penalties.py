@@ -436,3 +436,23 @@ def test_refusals():
     logits.resize_((3, 80))
     with pytest.raises(ValueError, match="changed after binding"):
         plan.launch()
+
+
+@pytest.mark.parametrize("name", ["logits", "slots", "frequency", "drafts", "mask", "outputs"])
+def test_operands_with_another_layout_after_binding(name):
+    """The same memory and number of elements, read another way."""
+    n, vocab = 32, 64
+    h = penalties.TokenHistory(n, vocab, DEV)
+    t = dict(logits=torch.zeros((2 * n, vocab), dtype=BF16, device=DEV), slots=torch.arange(n, dtype=torch.int32, device=DEV),
+             frequency=torch.ones(n, device=DEV), drafts=torch.zeros((1, n), dtype=torch.int64, device=DEV),
+             mask=torch.full((2 * n, 2), -1, dtype=torch.int32, device=DEV), outputs=torch.zeros((2 * n, vocab), dtype=BF16, device=DEV))
+    plan = penalties.LogitPenaltyPlan(logits=t["logits"], history=h, slots=t["slots"], frequency=t["frequency"],
+                                      draft_tokens=t["drafts"], token_mask=t["mask"], outputs=t["outputs"])
+    plan.launch()
+    if t[name].ndim == 2:
+        t[name].t_()
+    else:
+        t[name].data = t[name].view(FP32 if t[name].dtype is torch.int32 else torch.int32)
+    for live in (None, 1):
+        with pytest.raises(ValueError, match="changed after binding"):
+            plan.launch(live)

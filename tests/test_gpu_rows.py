@@ -300,3 +300,35 @@ def test_refusals():
         OPS.bind_quantize(x, y)
     with pytest.raises(ValueError, match="gate"):
         OPS.bind_quantize(x, q, gate=x[:, :63])
+
+
+def transposed(t):
+    t.t_()
+
+
+def narrowed(t):
+    t.as_strided_((t.shape[0] // 2, 2 * t.shape[1]), (t.stride(0), 1)) if t.stride(0) >= 2 * t.shape[1] else t.as_strided_(
+        (2 * t.shape[0], t.shape[1] // 2), (t.shape[1] // 2, 1))
+
+
+def retyped(t):
+    t.data = t.view({BF16: FP16, torch.float32: torch.int32, blockscale.E4M3: torch.uint8}[t.dtype])
+
+
+@pytest.mark.parametrize("change", [transposed, narrowed, retyped])
+@pytest.mark.parametrize("name", ["x", "residual", "output", "values", "scales"])
+def test_operands_with_another_layout_after_binding(name, change):
+    """The same memory and number of elements, read another way."""
+    k = 64
+    t = {n: torch.ones((k, k), dtype=BF16, device=DEV) for n in ("x", "residual", "output")}
+    t["values"], t["scales"] = torch.zeros((k, k), dtype=blockscale.E4M3, device=DEV), torch.zeros((k, 4), device=DEV)[:, :1]
+    w = torch.ones(k, dtype=BF16, device=DEV)
+    if name == "scales" and change is narrowed:
+        pytest.skip("one column")
+    bindings = (OPS.bind_norm(t["x"], w, epsilon=1e-6, residual=t["residual"], output=t["output"],
+                              quantized=blockscale.BlockScaledActivations(t["values"], t["scales"])),
+                OPS.bind_quantize(t["x"], blockscale.BlockScaledActivations(t["values"], t["scales"]), gate=t["residual"]))
+    change(t[name])
+    for binding in bindings[:1] if name == "output" else bindings:
+        with pytest.raises(ValueError, match="changed after binding"):
+            binding.launch()
