@@ -308,7 +308,10 @@ def bind_block_linear_group(operators, x: BlockScaledActivations, weights: Seque
                             outputs: Sequence[Tensor]) -> PackedOperatorBinding:
     """Bind ``outputs[j] = x weights[j]^T`` in one launch.
 
-    Outputs are bf16, fp16 or fp32 (one type for all) and may have padded rows.
+    Outputs are bf16, fp16 or fp32 (one type for all) and may have padded rows.  Sums are
+    in 32 bits for fp32; for 16-bit outputs the matrix instruction adds each eight products of
+    consecutive columns at 14 bits below the largest, at most 7 * 2^-13 of the eight's largest
+    |x| times its largest |w| off (1.5e-5 of y for normal operands).
     K has to be a multiple of 16, x 16-byte aligned with rows of whole 16 bytes.
     Weights are laid out as they are now (bindings of the same values share the layout);
     after a change to one, bind again.

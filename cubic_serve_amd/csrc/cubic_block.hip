@@ -2,14 +2,20 @@
 //
 //   y[m, n] = sum_b sx[m, b] sw[n / 128, b] sum_{k in block b} xq[m, k] wq[n, k]
 //
-// over e4m3 values and blocks of 128 columns.  One v_mfma_f32_16x16x128_f8f6f4
-// (unscaled form: the plain products of its 8-bit operands, at twice the rate of
-// the K = 32 ones) is one block of a 16 x 16 tile, so each block's product
-// starts from zero and is added to the 32-bit accumulator under its scale.
-// The instruction adds eight neighbouring products at 14 bits below the largest's
+// over e4m3 values and blocks of 128 columns.  Each block's product starts from zero
+// and is added to the 32-bit accumulator under its scale.
+//
+// Outputs in 16 bits: one v_mfma_f32_16x16x128_f8f6f4 (unscaled form: the plain products
+// of its 8-bit operands, at twice the rate of the K = 32 ones) is one block of a 16 x 16
+// tile.  The instruction adds eight neighbouring products at 14 bits below the largest's
 // exponent, and those sums in 32 bits.  That is the one rounding below 32 bits here,
 // taken for its rate: of N(0, 1) operands it leaves y 1.5e-5 off (root mean
-// square), a hundredth of bf16's rounding and a fourteenth of fp16's.
+// square), a hundredth of bf16's rounding and a fourteenth of fp16's; at most 7 * 2^-13 of an
+// eight's largest |x| times its largest |w|.
+// Outputs in 32 bits (FULL): the K = 32 instructions of 8-bit operands cut in the same way (2^16 + 2^e
+// keeps 2^e to e = 3 in both, to e = -7 with 16-bit operands), so the values go to
+// fp16, which holds all of e4m3, and four v_mfma_f32_16x16x32_f16 make a block: sums in 32 bits.
+//
 // Weights are its first operand: a lane then holds four columns n of one row m, the
 // scale is one number per lane, and outputs leave four columns at a time.
 //
@@ -39,10 +45,43 @@ __device__ __forceinline__ v8i join(u32x4_dev_t a, u32x4_dev_t b) {
     return v8i{(int)a.x, (int)a.y, (int)a.z, (int)a.w, (int)b.x, (int)b.y, (int)b.z, (int)b.w};
 }
 
+// 32 values of a row in fp16, as four operands of 8.
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+struct Halves {
+    v8h c[4];
+};
+__device__ __forceinline__ Halves to_halves(v8i v) {
+    Halves h;
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const v2h p = e & 1 ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v[2 * c + e / 2], 1.0f, true)
+                                : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v[2 * c + e / 2], 1.0f, false);
+            h.c[c][2 * e] = p[0];
+            h.c[c][2 * e + 1] = p[1];
+        }
+    return h;
+}
+
 // 16 x 16 products over one block from zero: rows of w by rows of x.
+__device__ __forceinline__ v4f block_product(const Halves& w, const Halves& x) {
+    v4f p = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int c = 0; c < 4; ++c) p = __builtin_amdgcn_mfma_f32_16x16x32_f16(w.c[c], x.c[c], p, 0, 0, 0);
+    return p;
+}
 __device__ __forceinline__ v4f block_product(v8i w, v8i x) {
     const v4f zero = {0.f, 0.f, 0.f, 0.f};
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, zero, 0, 0, 0, 0, 0, 0);
+}
+
+// 32 values of a row as block_product takes them.
+template <bool FULL>
+__device__ __forceinline__ auto operand(v8i v) {
+    if constexpr (FULL) return to_halves(v);
+    else return v;
 }
 
 // Four outputs in 16 bits.
@@ -56,10 +95,10 @@ __device__ __forceinline__ v2u pack4(const BlockGemmArgs& a, v4f v) {
 // LINES: past the caches where rows of y are whole lines, which a wave then writes whole: 64 rows
 // of 151936 x 4096 in 124 and 117 us, 2048 x 24576 x 4096 185 and 179; rows that share lines
 // (333 of 1521 x 2064) lose by it, 9.1 and 9.5.
-template <bool LINES = false>
+template <bool FULL, bool LINES = false>
 __device__ __forceinline__ void store4(const BlockGemmArgs& a, const BlockMember& w, int64_t m, int n, v4f v) {
     if (n >= w.n) return;
-    if (a.out == 2) {
+    if constexpr (FULL) {
         float* y = static_cast<float*>(w.y) + m * w.ldy + n;
         if (LINES && w.lines) {
             __builtin_nontemporal_store(v, reinterpret_cast<v4f*>(y));
@@ -70,24 +109,24 @@ __device__ __forceinline__ void store4(const BlockGemmArgs& a, const BlockMember
             for (int i = 0; i < 4; ++i)
                 if (n + i < w.n) y[i] = v[i];
         }
-        return;
-    }
-    const v2u u = pack4(a, v);
-    uint16_t* y = static_cast<uint16_t*>(w.y) + m * w.ldy + n;
-    if (n + 4 <= w.n) {
-        __builtin_memcpy(y, &u, sizeof u);
     } else {
+        const v2u u = pack4(a, v);
+        uint16_t* y = static_cast<uint16_t*>(w.y) + m * w.ldy + n;
+        if (n + 4 <= w.n) {
+            __builtin_memcpy(y, &u, sizeof u);
+        } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (n + i < w.n) y[i] = (uint16_t)(u[i >> 1] >> (16 * (i & 1)));
+            for (int i = 0; i < 4; ++i)
+                if (n + i < w.n) y[i] = (uint16_t)(u[i >> 1] >> (16 * (i & 1)));
+        }
     }
 }
 
 // Eight columns in 16 bits, past the caches as above.
 __device__ __forceinline__ void store8(const BlockGemmArgs& a, const BlockMember& w, int64_t m, int n, v4f lo, v4f hi) {
     if (n + 8 > w.n) {
-        store4(a, w, m, n, lo);
-        store4(a, w, m, n + 4, hi);
+        store4<false>(a, w, m, n, lo);
+        store4<false>(a, w, m, n + 4, hi);
         return;
     }
     const v2u l = pack4(a, lo), h = pack4(a, hi);
@@ -110,7 +149,7 @@ __device__ __forceinline__ int find_member(const BlockGemmArgs& a, int group) {
 // into registers, DEPTH blocks ahead, no barrier until the waves' sums are added
 // through LDS, in the order of the waves.  1 row, 20000 x 16384: 61 us, 5.4 TB/s.
 // ---------------------------------------------------------------------------
-template <int NT, int DEPTH>
+template <int NT, int DEPTH, bool FULL>
 __global__ __launch_bounds__(kStreamWaves * 64) void block_stream_kernel(BlockGemmArgs a) {
     __shared__ v4f sums[kStreamWaves][NT][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -164,10 +203,10 @@ __global__ __launch_bounds__(kStreamWaves * 64) void block_stream_kernel(BlockGe
             if (b + d * kStreamWaves < a.blocks) {
                 Stage& s = st[d];
                 const float scale = s.sx * s.sw;
-                const v8i xv = join(s.x[0], s.x[1]);
+                const auto xv = operand<FULL>(join(s.x[0], s.x[1]));
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
-                    const v4f p = block_product(join(s.w[t][0], s.w[t][1]), xv);
+                    const v4f p = block_product(operand<FULL>(join(s.w[t][0], s.w[t][1])), xv);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) acc[t][e] = fmaf(scale, p[e], acc[t][e]);
                 }
@@ -182,7 +221,7 @@ __global__ __launch_bounds__(kStreamWaves * 64) void block_stream_kernel(BlockGe
     if (wave < NT && tile0 + wave < w.tiles && row < a.m) {
         v4f v = sums[0][wave][lane];
         for (int o = 1; o < kStreamWaves; ++o) v += sums[o][wave][lane];
-        store4(a, w, row, (tile0 + wave) * 16 + quarter * 4, v);
+        store4<FULL>(a, w, row, (tile0 + wave) * 16 + quarter * 4, v);
     }
 }
 
@@ -228,7 +267,7 @@ __device__ __forceinline__ TileAt tile_at(const BlockGemmArgs& a, int id, int ro
 }
 
 // A wave's sums, 16 rows at a time through a run of LDS of its own (`out`), to leave in whole lines.
-template <int NTW, int MTW>
+template <bool FULL, int NTW, int MTW>
 __device__ __forceinline__ void leave(const BlockGemmArgs& a, const BlockMember& w, int m_first, int n0, const v4f (&acc)[NTW][MTW], float* out) {
     constexpr int kPitch = leave_pitch(NTW);
     const int lane = threadIdx.x & 63, quarter = lane >> 4, row = lane & 15;
@@ -239,7 +278,7 @@ __device__ __forceinline__ void leave(const BlockGemmArgs& a, const BlockMember&
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-        if (a.out != 2) {  // (eight columns a lane: 2048 x 24576 x 4096 in 174 us by four, and 166)
+        if constexpr (!FULL) {  // (eight columns a lane: 2048 x 24576 x 4096 in 174 us by four, and 166)
 #pragma unroll
             for (int at = lane; at < 32 * NTW; at += 64) {
                 const int r = at / (2 * NTW), c = at % (2 * NTW) * 8, m = m_first + i * 16 + r;
@@ -250,7 +289,7 @@ __device__ __forceinline__ void leave(const BlockGemmArgs& a, const BlockMember&
 #pragma unroll 1
             for (int at = lane; at < 64 * NTW; at += 64) {
                 const int r = at / (4 * NTW), c = at % (4 * NTW) * 4, m = m_first + i * 16 + r;
-                if (m < a.m) store4<true>(a, w, m, n0 + c, *reinterpret_cast<const v4f*>(out + r * kPitch + c));
+                if (m < a.m) store4<true, true>(a, w, m, n0 + c, *reinterpret_cast<const v4f*>(out + r * kPitch + c));
             }
         }
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -259,7 +298,7 @@ __device__ __forceinline__ void leave(const BlockGemmArgs& a, const BlockMember&
     }
 }
 
-template <int NTW, int MTW, int WN, int WM, int S, int G, int EU, bool SPLIT, bool PAST>
+template <int NTW, int MTW, int WN, int WM, int S, int G, int EU, bool SPLIT, bool PAST, bool FULL>
 __global__ __launch_bounds__(G * WN * WM * 64) __attribute__((amdgpu_waves_per_eu(EU, EU)))
 void block_tile_kernel(BlockGemmArgs a) {
     constexpr int W = WN * WM, N = NTW * WN, M = MTW * WM;  // waves of a group; tiles of 16
@@ -368,7 +407,8 @@ void block_tile_kernel(BlockGemmArgs a) {
         const int b = b_first + at * G + k_group;
         const uint8_t *xs = stage_of(stage) + k_group * kStage, *ws = xs + kW;
         float scale[MTW];
-        v8i xv[MTW], wv[2];
+        v8i wv[2];
+        decltype(operand<FULL>(wv[0])) xv[MTW], of_w;
         v4f p[kLag + 1];
         // (S - 2 steps' loads may be on their way, and the scales' that step 1 of S sends)
         __builtin_amdgcn_s_waitcnt(vm_waits((S - 2) * kLoads + (P >= 2 ? 1 : 0)));
@@ -376,9 +416,9 @@ void block_tile_kernel(BlockGemmArgs a) {
         __builtin_amdgcn_sched_barrier(0);
         const float block_scale = sw[G == 1 ? b : min(b, blocks - 1)];
 #pragma unroll
-        for (int i = 0; i < MTW; ++i) 
-            xv[i] = join(*reinterpret_cast<const u32x4_dev_t*>(xs + x_slot + i * kBlockBytes),
-                         *reinterpret_cast<const u32x4_dev_t*>(xs + x_half + i * kBlockBytes));
+        for (int i = 0; i < MTW; ++i)
+            xv[i] = operand<FULL>(join(*reinterpret_cast<const u32x4_dev_t*>(xs + x_slot + i * kBlockBytes),
+                                       *reinterpret_cast<const u32x4_dev_t*>(xs + x_half + i * kBlockBytes)));
         wv[0] = fragment(ws + w_slot);
 #pragma unroll
         for (int i = 0; i < MTW; ++i) {
@@ -397,7 +437,8 @@ void block_tile_kernel(BlockGemmArgs a) {
         for (int q = 0; q < NTW * MTW + kLag; ++q) {
             const int t = q / MTW, i = q % MTW;
             if (i == 0 && t + 1 < NTW) wv[(t + 1) & 1] = fragment(ws + w_slot + (t + 1) * kBlockBytes);
-            if (t < NTW) p[q % (kLag + 1)] = block_product(wv[t & 1], xv[i]);
+            if (i == 0 && t < NTW) of_w = operand<FULL>(wv[t & 1]);
+            if (t < NTW) p[q % (kLag + 1)] = block_product(of_w, xv[i]);
             if (q >= kLag) {
                 const int of = q - kLag;
                 v4f& sum = acc[of / MTW][of % MTW];
@@ -488,7 +529,7 @@ void block_tile_kernel(BlockGemmArgs a) {
     static_assert((G > 1 ? W : W / 2) * kRun * 4 <= G * kStage, "the waves' rows fit one stage, or two");
     float* out = G > 1 ? reinterpret_cast<float*>(stage1) + wave * kRun
                        : reinterpret_cast<float*>(wave & 1 ? stage1 : stage0) + (wave >> 1) * kRun;
-    leave(a, w, m0 + wm * MTW * 16, (tile0 + wn * NTW) * 16, acc, out);
+    leave<FULL>(a, w, m0 + wm * MTW * 16, (tile0 + wn * NTW) * 16, acc, out);
 }
 
 // ---------------------------------------------------------------------------
@@ -672,7 +713,7 @@ void block_wide_kernel(BlockGemmArgs a) {
     constexpr int kRun = 16 * leave_pitch(NTW);
     static_assert(3 * kRun * 4 <= 32768 && kRun * 4 <= 16384, "three waves' rows fit x0 or x1, one's the others");
     uint8_t* const out = wave < 3 ? x0 + wave * kRun * 4 : wave < 6 ? x1 + (wave - 3) * kRun * 4 : wave < 7 ? lo0 : lo1;
-    leave(a, w, m0 + wm * MTW * 16, (tile0 + wn * NTW) * 16, acc, reinterpret_cast<float*>(out));
+    leave<false>(a, w, m0 + wm * MTW * 16, (tile0 + wn * NTW) * 16, acc, reinterpret_cast<float*>(out));
 }
 // Values [n, k] of any row stride to tiles; rows past n and columns past k are 0.
 __global__ __launch_bounds__(256) void block_prepare_kernel(const uint8_t* values, int64_t ld, int64_t n, int k,
@@ -703,16 +744,16 @@ unsigned count_groups(BlockGemmArgs& a, int tiles) {
     return groups;
 }
 
-template <int NT>
+template <int NT, bool FULL>
 hipError_t launch_stream(BlockGemmArgs a, hipStream_t s) {
-    block_stream_kernel<NT, 4><<<count_groups(a, NT), kStreamWaves * 64, 0, s>>>(a);
+    block_stream_kernel<NT, 4, FULL><<<count_groups(a, NT), kStreamWaves * 64, 0, s>>>(a);
     return hipGetLastError();
 }
 
-template <int NTW, int MTW, int WN, int WM, int S, int G, int EU, bool SPLIT = false, bool PAST = false>
+template <bool FULL, int NTW, int MTW, int WN, int WM, int S, int G, int EU, bool SPLIT = false, bool PAST = false>
 hipError_t launch_tile(BlockGemmArgs a, hipStream_t s) {
     const unsigned tiles = count_groups(a, NTW * WN) * ((a.m + 16 * MTW * WM - 1) / (16 * MTW * WM));
-    block_tile_kernel<NTW, MTW, WN, WM, S, G, EU, SPLIT, PAST><<<SPLIT ? tiles * a.split : tiles, G * WN * WM * 64, 0, s>>>(a);
+    block_tile_kernel<NTW, MTW, WN, WM, S, G, EU, SPLIT, PAST, FULL><<<SPLIT ? tiles * a.split : tiles, G * WN * WM * 64, 0, s>>>(a);
     return hipGetLastError();
 }
 
@@ -721,9 +762,8 @@ hipError_t launch_wide(BlockGemmArgs a, hipStream_t s) {
     return hipGetLastError();
 }
 
-}  // namespace
-
-hipError_t launch_block_gemm(const BlockGemmArgs& a, hipStream_t s) {
+template <bool FULL>
+hipError_t launch_any(const BlockGemmArgs& a, hipStream_t s) {
     int64_t tiles = 0;
     for (int j = 0; j < a.members; ++j) tiles += a.member[j].tiles;
     // Weights that the 256 MB cache cannot hold, read by one workgroup each, are read past
@@ -731,18 +771,24 @@ hipError_t launch_block_gemm(const BlockGemmArgs& a, hipStream_t s) {
     // it all but holds, 45 and 56; by two workgroups, 128 rows of 24576 x 4096 in 64-row tiles, 39 and 41.
     const bool large = tiles * a.blocks * kBlockBytes > kPastCacheBytes;
     switch (a.tile) {
-        case 1: return launch_tile<2, 2, 2, 2, 3, 1, 3>(a, s);
+        case 1: return launch_tile<FULL, 2, 2, 2, 2, 3, 1, 3>(a, s);
         case 2:
-            return large && a.m <= 64 ? launch_tile<4, 2, 2, 2, 3, 1, 2, false, true>(a, s) : launch_tile<4, 2, 2, 2, 3, 1, 2>(a, s);
+            return large && a.m <= 64 ? launch_tile<FULL, 4, 2, 2, 2, 3, 1, 2, false, true>(a, s) : launch_tile<FULL, 4, 2, 2, 2, 3, 1, 2>(a, s);
         case 3:
-            return large && a.m <= 128 ? launch_tile<4, 4, 4, 2, 3, 1, 2, false, true>(a, s) : launch_tile<4, 4, 4, 2, 3, 1, 2>(a, s);
-        case 4: return launch_wide(a, s);
-        case 5: return a.split > 1 ? launch_tile<2, 2, 2, 2, 4, 2, 2, true>(a, s) : launch_tile<2, 2, 2, 2, 4, 2, 2>(a, s);
+            return large && a.m <= 128 ? launch_tile<FULL, 4, 4, 4, 2, 3, 1, 2, false, true>(a, s) : launch_tile<FULL, 4, 4, 4, 2, 3, 1, 2>(a, s);
+        case 4: return FULL ? hipErrorInvalidValue : launch_wide(a, s);
+        case 5: return a.split > 1 ? launch_tile<FULL, 2, 2, 2, 2, 4, 2, 2, true>(a, s) : launch_tile<FULL, 2, 2, 2, 2, 4, 2, 2>(a, s);
         default: break;
     }
     // the more columns there are, the fewer times x is read
-    if (tiles >= 2048) return launch_stream<4>(a, s);
-    return tiles >= 1024 ? launch_stream<2>(a, s) : launch_stream<1>(a, s);
+    if (tiles >= 2048) return launch_stream<4, FULL>(a, s);
+    return tiles >= 1024 ? launch_stream<2, FULL>(a, s) : launch_stream<1, FULL>(a, s);
+}
+
+}  // namespace
+
+hipError_t launch_block_gemm(const BlockGemmArgs& a, hipStream_t s) {
+    return a.out == 2 ? launch_any<true>(a, s) : launch_any<false>(a, s);
 }
 
 hipError_t launch_block_prepare(const uint8_t* values, int64_t ld, int64_t n, int64_t k, uint8_t* out, hipStream_t s) {

@@ -1044,7 +1044,8 @@ struct BlockPlan {
 // 12288 32 and 26 us, 64 x 6144 x 4096 12.7 and 11.4, 333 x 1521 x 2048 8.8 and 8.4, x 1536 7.8
 // and 7.7, x 1024 6.4 and 6.5, x 512 4.9 and 5.3.  Rows of 6144 x 4096,
 // stream and tiles: 1 8.5 and 12.0, 8 10.8 and 10.7, 16 13.1 and 10.7.
-BlockPlan plan_block(int64_t m, int64_t k, int members, const int64_t* ns) {
+// 32-bit outputs (full) go by the same rule without the 256 x 256 tile, which has no registers for fp16 operands.
+BlockPlan plan_block(int64_t m, int64_t k, int members, const int64_t* ns, bool full) {
     BlockPlan p = {0, 1, 0, 0, 0};
     const int64_t blocks = ceil_div(k, cubic::kScaleBlock);
     auto tiles = [&](int columns, int rows) {
@@ -1062,7 +1063,7 @@ BlockPlan plan_block(int64_t m, int64_t k, int members, const int64_t* ns) {
     const int64_t small = tiles(64, 64);
     auto rounds = [&](int columns, int rows) { return ceil_div(tiles(columns, rows), 256); };
     const int64_t cost[] = {24 * rounds(64, 64), 10 + 36 * rounds(128, 64), 112 * rounds(256, 128), 180 * rounds(256, 256)};
-    p.tile = 1 + (int)(std::min_element(cost, cost + 4) - cost);
+    p.tile = 1 + (int)(std::min_element(cost, cost + (full ? 3 : 4)) - cost);
     if (p.tile != 1 || small > 256) return p;
     // K in as many parts as leave one round, at most 4 of 8 blocks and more.  One part and
     // this, weights in a cache and not: 64 rows x 4096 x 12288 25 and 15 us, 38 and 20; 64 x 1024 x 8192
@@ -1090,7 +1091,7 @@ int64_t cubic_block_gemm_workspace_bytes(int64_t m, int64_t k, int members, cons
     if (m < 1 || m >= (1 << 21) || k < 1 || k > (1 << 20) || members < 1 || members > cubic::kMaxGemmMembers || !ns) return -1;
     for (int j = 0; j < members; ++j)
         if (ns[j] < 1 || ns[j] > (1 << 24)) return -1;
-    return plan_block(m, k, members, ns).bytes;
+    return plan_block(m, k, members, ns, false).bytes;
 }
 
 int cubic_block_prepare(const void* values, int64_t ld, int64_t n, int64_t k, void* prepared, void* stream) {
@@ -1147,7 +1148,7 @@ int cubic_block_gemm(const void* x, int64_t ldx, const float* x_scales, int64_t 
     }
     if (m > 8 && ceil_div(tiles, 4) * ceil_div(m, 64) >= (1 << 22))
         return fail(CUBIC_ENOTSUP, "block gemm: more tiles than one launch holds");
-    const BlockPlan p = plan_block(m, k, members, ns);
+    const BlockPlan p = plan_block(m, k, members, ns, out_dtype == CUBIC_DTYPE_F32);
     if (workspace_bytes < p.bytes)
         return fail(CUBIC_EWORKSPACE, "block gemm workspace %lld < %lld bytes", (long long)workspace_bytes, (long long)p.bytes);
     if (p.bytes && (!workspace || !aligned16(workspace))) return fail(CUBIC_EINVAL, "workspace must be 16-byte aligned");

@@ -391,9 +391,9 @@ struct BlockGemmArgs {
     const float* x_scales;        // of block b of row r at r * scale_row + b * scale_group
     int64_t ldx, scale_row, scale_group;
     int m, k, blocks, members;
-    int out;                      // CUBIC_DTYPE_* of y
-    int tile;                     // 0: the stream kernel (up to 16 rows); tiles of 1: 64 x 64, 2: 128 x 64, 3: 256 x 128, 4: 256 x 256
-                                  // columns x rows, 5: 64 x 64 by two groups of waves
+    int out;                      // CUBIC_DTYPE_* of y; _F32: sums in 32 bits throughout
+    int tile;                     // 0: the stream kernel (up to 8 rows); tiles, columns x rows, of 1: 64 x 64, 2: 128 x 64, 3: 256 x 128,
+                                  // 4: 256 x 256 (16-bit outputs only), 5: 64 x 64 by two groups of waves
     int split, part_blocks;       // tile 5: parts of K and blocks in each, joined by the last to arrive
     uint32_t* counters;           // [tiles], zero between launches
     float* partial;               // [tiles, split, 4096]

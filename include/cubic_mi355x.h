@@ -494,8 +494,15 @@ CUBIC_API int cubic_quantize_rows(const void* x, int64_t ldx, const void* gate, 
  *   ys       [m, n_j] of out_dtype CUBIC_DTYPE_BF16, _F16 or _F32, rounded once
  * Host arrays ns, prepared, scales, ys, ldys have one entry per member and are
  * read during the call.  k % 16 == 0, x 16-byte aligned with a row stride of whole
- * 16 bytes up to 2^23, m < 2^21.  NaN values and scales propagate.  Sums are in 32
- * bits; their order depends on the sizes only.
+ * 16 bytes up to 2^23, m < 2^21.  NaN values and scales propagate.  The order of sums
+ * depends on the sizes and out_dtype only.
+ *   _F32        every sum is in 32 bits.
+ *   _BF16, _F16 the matrix instruction adds eight products of consecutive columns at 14
+ *               bits below the largest's exponent (an error of at most 7 * 2^-13 of the
+ *               eight's largest |x| times its largest |w|; 1.5e-5 of y for N(0, 1)
+ *               operands), everything else is in 32 bits.  Where large products cancel
+ *               and that is too much, take _F32: up to 2.1 times as long where the matrix cores bound it,
+ *               1.07 where the weights do.
  *   workspace  cubic_block_gemm_workspace_bytes(m, k, members, ns) bytes, 16-byte
  *            aligned, zero before the first launch; every launch leaves its
  *            counters zero.  Launches that share one must not overlap.

@@ -290,3 +290,44 @@ def test_weights_written_past_autograd_are_prepared_again():
         w.scales.mul_(0.5)
         ops.bind_block_linear(x, w, y).launch()
     check(x, w, y)
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 300, 272), (3, 17000, 400), (8, 33000, 144), (9, 300, 1168), (64, 4000, 4112), (100, 1000, 2064),
+                                   (300, 12000, 272), (1000, 8192, 144), (2050, 4000, 528), (1, 66001, 4864), (60, 65000, 4864), (130, 520, 16)])
+def test_outputs_in_32_bits_hold_every_product(m, n, k):
+    """Products of 1 to 2^16 beside each other, large ones that cancel among them; whole sums below 2^24, which
+    additions in 32 bits leave exact in any order.  (Per eight: 256 * 256, its negative, six of 1 to 225.)"""
+    print(f"block gemm in 32 bits m={m} n={n} k={k}", flush=True)
+    gen = torch.Generator(device=DEV).manual_seed(51)
+    ints = lambda rows: torch.randint(-15, 16, (rows, k), generator=gen, device=DEV).float()
+    a, b = ints(m), ints(n)
+    a[:, 2::8], a[:, 5::8] = 256.0, -256.0
+    b[:, 2::8] = b[:, 5::8] = 256.0
+    blocks = (k + 127) // 128
+    # (magnitudes: 16 * 2 * 2^16 + 96 * 225 in a block, under 2^22; the large ones cancel in pairs)
+    x = blockscale.BlockScaledActivations(a.to(E4M3), torch.ones((m, blocks), device=DEV))
+    w = blockscale.BlockScaledMatrix(b.to(E4M3), torch.full(((n + 127) // 128, blocks), 0.5, device=DEV))
+    y, = product(x, [w], FP32, pad=m % 4)
+    want = torch.cat([wide(x) @ part.t() for part in wide(w).split(8192)], 1)
+    assert torch.equal(y.double(), want)
+
+
+def check32(x, w, y):
+    """In 32 bits: 128 products of a block, each exact, added in any order (127 additions, truncated: 2^-23 of the block's
+    magnitudes each), scaled, and added to the sum block by block and wave by wave, at most blocks + 20 roundings of 2^-24."""
+    a, b = wide(x), wide(w)
+    want, size = a @ b.t(), a.abs() @ b.abs().t()
+    blocks = (x.values.shape[1] + 127) // 128
+    bound = size * (127 * 2.0 ** -23 + (blocks + 20) * 2.0 ** -24) + want.abs() * 2.0 ** -24 + LEAST[FP32]
+    off = (y.double() - want).abs()
+    assert (off <= bound).all(), (off / bound).max().item()
+    # Errors add at random: 128 of 2^-24 of partial sums near size / sqrt(128) are 2^-24 of size, a 250th of the bound.
+    assert off.square().mean().sqrt() <= 0.01 * bound.square().mean().sqrt()
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 1000, 4096), (7, 20011, 1104), (33, 3000, 2064), (64, 40000, 1024), (512, 4096, 4096), (1111, 3333, 1040),
+                                   (700, 9000, 8192), (64, 1024, 8192)])
+def test_outputs_in_32_bits(m, n, k):
+    x, w = activations(m, k, 53), matrix(n, k, 54)
+    y, = product(x, [w], FP32)
+    check32(x, w, y)
