@@ -207,7 +207,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(8, 8))
     constexpr int kChunk = kPenaltyBytes / (OUT == 2 ? 4 : 2), kTurns = kChunk / (8 * kThreads), kLists = kChunk / kHistoryBucket;
     static_assert(kChunk % kHistoryBucket == 0, "a list is one workgroup's");
     __shared__ __attribute__((aligned(16))) uint8_t staged[INPLACE ? 16 : kPenaltyBytes];
-    __shared__ int drafts[kMaxPenaltyDepth];
+    __shared__ int drafts[kMaxPenaltyDepth], taken[kLists + 1];
     // (all rows' first chunks first: vocabularies begin with the tokens that come often, so
     // those have the long lists and should not come last)
     // The rows of a sequence, eight sequences at a time, on one XCD (workgroups go round robin
@@ -269,15 +269,21 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(8, 8))
     }
     const Settings s = settings_of(a, sequence);
     const bool known = s.valid && slotted;
-    int sizes[kLists], some = known ? ahead : 0;
-#pragma unroll
-    for (int l = 0; l < kLists; ++l) {
-        const int bucket = c0 / kHistoryBucket + l;
-        sizes[l] = known && bucket < buckets ? min(a.history.sizes[(int64_t)slot * buckets + bucket], kHistoryBucket) : 0;
-        some += sizes[l];
+    // What is listed, and whether a draft is a column of this chunk, as the first wave finds it: the
+    // barriers below are met by all of a workgroup or by none, whatever becomes of memory meanwhile.
+    if ((int)threadIdx.x < kLists) {
+        const int bucket = c0 / kHistoryBucket + (int)threadIdx.x;
+        taken[threadIdx.x] = known && bucket < buckets ? min(a.history.sizes[(int64_t)slot * buckets + bucket], kHistoryBucket) : 0;
     }
+    const bool drafted = (int)threadIdx.x < ahead && known && draft >= 0 && draft < columns;
+    if ((int)threadIdx.x < ahead) drafts[threadIdx.x] = drafted ? (int)draft : -1;
+    const bool any_drafted = __ballot(drafted) != 0;
+    if (threadIdx.x == 0) taken[kLists] = any_drafted;
+    __syncthreads();
+    int sizes[kLists], some = __builtin_amdgcn_readfirstlane(taken[kLists]);
+#pragma unroll
+    for (int l = 0; l < kLists; ++l) some += sizes[l] = __builtin_amdgcn_readfirstlane(taken[l]);
     if (some || !whole) {
-        if ((int)threadIdx.x < ahead) drafts[threadIdx.x] = draft >= 0 && draft < columns ? (int)draft : -1;  // columns of this chunk
         if constexpr (!INPLACE) {
 #pragma unroll
             for (int i = 0; i < kTurns; ++i)
@@ -308,7 +314,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(8, 8))
                 if (d >= 0) change(d, of_d);
             }
         }
-        if (known && (int)threadIdx.x < ahead) {  // drafts that are new to the request
+        if ((int)threadIdx.x < ahead) {  // drafts that are new to the request
             const int c = drafts[threadIdx.x];
             bool first = c >= 0;
             for (int j = 0; j < (int)threadIdx.x; ++j) first = first && drafts[j] != c;

@@ -456,3 +456,36 @@ def test_operands_with_another_layout_after_binding(name):
     for live in (None, 1):
         with pytest.raises(ValueError, match="changed after binding"):
             plan.launch(live)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_columns_that_no_list_names_beside_an_append(dtype):
+    """Lists that grow while a launch reads them: which of the two comes first is open, token by token, but a workgroup goes
+    one way as a whole, so the columns that nobody names keep their logits.  (Presence alone, each token appended once: a
+    named column holds its logit or that minus 1, whole numbers.)"""
+    vocab, sequences, length = 50000, 16, 8
+    side = torch.cuda.Stream()
+    gen = torch.Generator().manual_seed(11)
+    slots = torch.arange(sequences, dtype=torch.int32, device=DEV)
+    logits = torch.randint(-60, 60, (sequences, vocab), generator=gen).to(dtype).to(DEV)
+    for turn in range(4):
+        h = penalties.TokenHistory(sequences, vocab, DEV)
+        plan = penalties.LogitPenaltyPlan(logits=logits, history=h, slots=slots, presence=torch.ones(sequences, device=DEV),
+                                          outputs=torch.full_like(logits, 7.0))
+        # (not token 0, which an unwritten place of a list names)
+        named = torch.stack([1 + torch.randperm(vocab - 1, generator=gen)[:20 * length] for _ in range(sequences)]).to(DEV)
+        steps = [named[:, i:i + length].contiguous() for i in range(0, 20 * length, length)]
+        torch.cuda.synchronize()
+        results = []
+        for step in steps:
+            with torch.cuda.stream(side):
+                h.append(slots, step)
+            plan.launch()
+            results.append(plan.outputs.clone())
+        torch.cuda.synchronize()
+        given = torch.zeros((sequences, vocab), dtype=torch.bool, device=DEV).scatter_(1, named, True)
+        for got in results:
+            assert torch.equal(got[~given], logits[~given])
+            assert ((got == logits) | (got == logits - 1))[given].all()
+        plan.launch()
+        assert torch.equal(plan.outputs, torch.where(given, logits - 1, logits))
