@@ -133,7 +133,7 @@ __device__ __forceinline__ float row_sum(float part, float* sums) {
 
 // One row per workgroup, or per wave (WAVE: blockDim.x == 64, four rows to a
 // workgroup); NV vectors per thread cover it.  NV = 0: any length, the row is read
-// again (from the caches) for the outputs.
+// again (from the caches) for the outputs, and a thread's many additions carry their rounding.
 template <bool F16, int NV, bool WAVE, bool PAST>
 __global__ __launch_bounds__(1024) void row_norm_kernel(RowArgs a) {
     __shared__ float sums[16];
@@ -165,11 +165,15 @@ __global__ __launch_bounds__(1024) void row_norm_kernel(RowArgs a) {
             if (a.y) store8<F16, PAST>(static_cast<uint16_t*>(a.y) + row * a.ldy, c, a.k, h);
             if (a.q) quantise8<PAST>(a, row, c, h);
         };
-        float part = 0.0f;
-        for (int i = 0; i < (NV ? 0 : turns); ++i) {
+        float part = 0.0f, rest = 0.0f;
+        for (int i = 0; i < (NV ? 0 : turns); ++i) {  // what an addition rounds off goes into the next
             read(i, v[0]);
+            float squares = 0.0f;
 #pragma unroll
-            for (int e = 0; e < kVec; ++e) part = fmaf(v[0][e], v[0][e], part);
+            for (int e = 0; e < kVec; ++e) squares = fmaf(v[0][e], v[0][e], squares);
+            const float more = squares - rest, next = part + more;
+            rest = next < __builtin_huge_valf() ? (next - part) - more : 0.0f;
+            part = next;
         }
         if constexpr (NV != 0) {
 #pragma unroll

@@ -332,3 +332,23 @@ def test_operands_with_another_layout_after_binding(name, change):
     for binding in bindings[:1] if name == "output" else bindings:
         with pytest.raises(ValueError, match="changed after binding"):
             binding.launch()
+
+
+@pytest.mark.parametrize("k", [1 << 24, (1 << 21) + 8, 1 << 17])
+def test_norm_of_the_longest_rows(k):
+    """Equal squares of 1 + 2^-6 + 2^-14, whose last part a plain running sum loses from 2^10 on; a thread of a row that is
+    read twice adds 8 squares, and these eights with the rounding carried over, so the bound above holds at any length."""
+    x = torch.full((2, k), 1 + 2.0 ** -7, dtype=BF16, device=DEV)
+    x[1] = rows(1, k, BF16, 61)[0]
+    w = torch.ones(k, dtype=BF16, device=DEV)
+    y, q = torch.empty_like(x), blockscale.BlockScaledActivations.empty(2, k, DEV)
+    for value in (float("inf"), float("nan")):  # finite / inf, inf / inf
+        other = x.clone()
+        other[0, 5] = value
+        OPS.bind_norm(other, w, epsilon=1e-6, output=y).launch()
+        assert torch.isnan(y[0, 5]) and ((y[0] == 0).sum() == k - 1 if value > 0 else torch.isnan(y[0]).all())
+        near16(y[1:], norm_exact(other[1:], None, w, 1e-6, 0.0)[1])
+    OPS.bind_norm(x, w, epsilon=1e-6, output=y, quantized=q).launch()
+    _, want = norm_exact(x, None, w, 1e-6, 0.0)
+    near16(y, want)
+    near8(q, want)
