@@ -154,44 +154,58 @@ __global__ __launch_bounds__(1024) void row_norm_kernel(RowArgs a) {
                 for (int e = 0; e < kVec; ++e) h[e] += o[e];
             }
         };
-        auto write = [&](int i, float factor, float (&h)[kVec]) {
+        auto write = [&](int i, float shift, float factor, float (&h)[kVec]) {
             const int c = (i * blockDim.x + threadIdx.x) * kVec;
             // (the sum is read again a layer later: 4096 x 8192 in 55.9 and 52.1 us past the caches)
             if (a.sum) store8<F16, true>(static_cast<uint16_t*>(a.sum) + row * a.ldsum, c, a.k, h);
             float w[kVec];
             load8<F16>(weight, c, a.k, w);
 #pragma unroll
-            for (int e = 0; e < kVec; ++e) h[e] = h[e] * factor * (a.offset + w[e]);
+            for (int e = 0; e < kVec; ++e) h[e] = h[e] * shift * factor * (a.offset + w[e]);
             if (a.y) store8<F16, PAST>(static_cast<uint16_t*>(a.y) + row * a.ldy, c, a.k, h);
             if (a.q) quantise8<PAST>(a, row, c, h);
         };
-        float part = 0.0f, rest = 0.0f;
-        for (int i = 0; i < (NV ? 0 : turns); ++i) {  // what an addition rounds off goes into the next
-            read(i, v[0]);
-            float squares = 0.0f;
-#pragma unroll
-            for (int e = 0; e < kVec; ++e) squares = fmaf(v[0][e], v[0][e], squares);
-            const float more = squares - rest, next = part + more;
-            rest = next < __builtin_huge_valf() ? (next - part) - more : 0.0f;
-            part = next;
-        }
         if constexpr (NV != 0) {
 #pragma unroll
             for (int i = 0; i < N; ++i) read(i, v[i]);
-#pragma unroll
-            for (int i = 0; i < N; ++i)
-#pragma unroll
-                for (int e = 0; e < kVec; ++e) part = fmaf(v[i][e], v[i][e], part);
         }
-        const float sum = row_sum<WAVE>(part, sums);
-        const float factor = 1.0f / sqrtf(sum / (float)a.k + a.epsilon);
+        auto squares = [&](float shift) __attribute__((always_inline)) {  // of h * shift, over the row
+            float part = 0.0f, rest = 0.0f;
+            if constexpr (NV != 0) {
+#pragma unroll
+                for (int i = 0; i < N; ++i)
+#pragma unroll
+                    for (int e = 0; e < kVec; ++e) part = fmaf(v[i][e] * shift, v[i][e] * shift, part);
+            }
+            for (int i = 0; i < (NV ? 0 : turns); ++i) {  // what an addition rounds off goes into the next
+                read(i, v[0]);
+                float eight = 0.0f;
+#pragma unroll
+                for (int e = 0; e < kVec; ++e) eight = fmaf(v[0][e] * shift, v[0][e] * shift, eight);
+                const float more = eight - rest, next = part + more;
+                rest = next < __builtin_huge_valf() ? (next - part) - more : 0.0f;
+                part = next;
+            }
+            return row_sum<WAVE>(part, sums);
+        };
+        // Where the sum leaves the 32-bit numbers the squares are taken of h times a power of two
+        // (of at most 2^48 then, 2^24 of them; of at least 2^-53).  Small ones matter beside a
+        // small epsilon only.  (4096 x 8192 to 8 bits: 48.2 us without this, and 48.6.)
+        float sum = squares(1.0f), shift = 1.0f;
+        const bool large = sum > 0x1.fffffep127f, small = sum < 0x1p-100f && a.epsilon < 0x1p-76f;
+        if (__builtin_expect(large || small, 0)) {
+            if constexpr (!WAVE) __syncthreads();  // the sums are read
+            shift = large ? 0x1p-80f : 0x1p80f;
+            sum = squares(shift);
+        }
+        const float factor = 1.0f / sqrtf(sum / (float)a.k + a.epsilon * shift * shift);
         if constexpr (NV != 0) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) write(i, factor, v[i]);
+            for (int i = 0; i < N; ++i) write(i, shift, factor, v[i]);
         } else {
             for (int i = 0; i < turns; ++i) {
                 read(i, v[0]);
-                write(i, factor, v[0]);
+                write(i, shift, factor, v[0]);
             }
         }
         if constexpr (!WAVE) __syncthreads();  // the sums are read
