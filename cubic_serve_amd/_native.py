@@ -101,6 +101,10 @@ def lib() -> ctypes.CDLL:
                 f"Cubic MI355X HIP library missing at {_LIB_PATH}; run "
                 "`python -m cubic_serve_amd.build` (hipcc --offload-arch=gfx950)")
         handle = ctypes.CDLL(str(_LIB_PATH))
+        # (entries are added without a new version: an older library lacks them)
+        missing = [name for name in SIGNATURES if not hasattr(handle, name)]
+        if missing:
+            raise RuntimeError(f"{_LIB_PATH} lacks {', '.join(missing)}: rebuild the library")
         for name, (restype, argtypes) in SIGNATURES.items():
             fn = getattr(handle, name)
             fn.restype = restype

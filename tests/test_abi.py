@@ -3,6 +3,7 @@ and its host-side planning entry points answer without a GPU."""
 from __future__ import annotations
 
 import re
+import subprocess
 from pathlib import Path
 
 import pytest
@@ -24,6 +25,22 @@ def test_library_exports_every_declared_symbol():
         assert hasattr(lib, name), name
     assert set(names) == set(_native.SIGNATURES), "ctypes signatures drift from the header"
     assert lib.cubic_abi_version() == 6
+
+
+def test_an_older_library_is_refused(tmp_path, monkeypatch):
+    """One of the same version without the entries added since, and one of another version."""
+    names = sorted(set(_native.SIGNATURES) - {"cubic_abi_version"})
+    for version, exported, match in ((_native.ABI_VERSION, names[1:], f"lacks {names[0]}: rebuild"),
+                                     (_native.ABI_VERSION - 1, names, "implements ABI")):
+        source, library = tmp_path / f"old{version}.c", tmp_path / f"libold{version}.so"
+        source.write_text(f"int cubic_abi_version(void) {{ return {version}; }}\n"
+                          + "".join(f"int {name}(void) {{ return 0; }}\n" for name in exported))
+        subprocess.run(["gcc", "-shared", "-fPIC", "-o", str(library), str(source)], check=True)
+        monkeypatch.setattr(_native, "_LIB_PATH", library)
+        monkeypatch.setattr(_native, "_lib", None)
+        with pytest.raises(RuntimeError, match=match):
+            _native.lib()
+        assert _native._lib is None
 
 
 def test_host_planning_entry_points():
