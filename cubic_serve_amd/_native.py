@@ -51,6 +51,7 @@ SIGNATURES: dict[str, tuple] = {
     "cubic_block_prepared_bytes": (I64, [I64, I64]),
     "cubic_block_prepare": (I32, [P, I64, I64, I64, P, P]),
     "cubic_block_gemm_workspace_bytes": (I64, [I64, I64, I32, P]),
+    "cubic_block_gemm_launch_plan": (I64, [I64, I64, I32, P, I32, P, P]),
     "cubic_block_gemm": (I32, [P, I64, P, I64, I64, I64, I64, I32, P, P, P, P, P, I32, P, I64, P, P]),
     "cubic_moe_pad_routes": (I32, [P, P, P, P, P, I32, I32, I32, P, P, P, P]),
     "cubic_moe_max_blocks": (I64, [I64, I32, I32]),

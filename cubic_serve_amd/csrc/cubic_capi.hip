@@ -1087,11 +1087,20 @@ int64_t cubic_block_prepared_bytes(int64_t n, int64_t k) {
     return ceil_div(n, cubic::kScaleBlock) * ceil_div(k, cubic::kScaleBlock) * cubic::kScaleBlock * cubic::kScaleBlock;
 }
 
-int64_t cubic_block_gemm_workspace_bytes(int64_t m, int64_t k, int members, const int64_t* ns) {
+int64_t cubic_block_gemm_launch_plan(int64_t m, int64_t k, int members, const int64_t* ns, int out_dtype, int* kernel, int* split) {
     if (m < 1 || m >= (1 << 21) || k < 1 || k > (1 << 20) || members < 1 || members > cubic::kMaxGemmMembers || !ns) return -1;
+    if (out_dtype != CUBIC_DTYPE_BF16 && out_dtype != CUBIC_DTYPE_F16 && out_dtype != CUBIC_DTYPE_F32) return -1;
     for (int j = 0; j < members; ++j)
         if (ns[j] < 1 || ns[j] > (1 << 24)) return -1;
-    return plan_block(m, k, members, ns, false).bytes;
+    const BlockPlan p = plan_block(m, k, members, ns, out_dtype == CUBIC_DTYPE_F32);
+    if (kernel) *kernel = p.tile;
+    if (split) *split = p.split;
+    return p.bytes;
+}
+
+int64_t cubic_block_gemm_workspace_bytes(int64_t m, int64_t k, int members, const int64_t* ns) {
+    // (the same for every type: K is split where 64 x 64 tiles of one round win, which cost less than any other tile's)
+    return cubic_block_gemm_launch_plan(m, k, members, ns, CUBIC_DTYPE_BF16, nullptr, nullptr);
 }
 
 int cubic_block_prepare(const void* values, int64_t ld, int64_t n, int64_t k, void* prepared, void* stream) {

@@ -495,7 +495,7 @@ CUBIC_API int cubic_quantize_rows(const void* x, int64_t ldx, const void* gate, 
  * Host arrays ns, prepared, scales, ys, ldys have one entry per member and are
  * read during the call.  k % 16 == 0, x 16-byte aligned with a row stride of whole
  * 16 bytes up to 2^23, m < 2^21.  NaN values and scales propagate.  The order of sums
- * depends on the sizes and out_dtype only.
+ * depends on the sizes (of all members) and out_dtype only.
  *   _F32        every sum is in 32 bits.
  *   _BF16, _F16 the matrix instruction adds eight products of consecutive columns at 14
  *               bits below the largest's exponent (an error of at most 7 * 2^-13 of the
@@ -506,9 +506,22 @@ CUBIC_API int cubic_quantize_rows(const void* x, int64_t ldx, const void* gate, 
  *   workspace  cubic_block_gemm_workspace_bytes(m, k, members, ns) bytes, 16-byte
  *            aligned, zero before the first launch; every launch leaves its
  *            counters zero.  Launches that share one must not overlap.
+ * cubic_block_gemm_launch_plan: what a launch of these sizes takes: returns its
+ *   workspace (-1 for an inadmissible argument) and stores, where the pointers are not
+ *   NULL, its kernel (CUBIC_BLOCK_*: tiles of so many columns by rows) and its number of
+ *   K partitions.  Kernels but _STREAM and _64X64_PAIRED (two groups of waves that take blocks
+ *   of K in turn) go through K in order, so their bits agree.
  * ------------------------------------------------------------------------- */
+#define CUBIC_BLOCK_STREAM 0  /* few rows, K over the waves of a workgroup */
+#define CUBIC_BLOCK_64X64 1
+#define CUBIC_BLOCK_128X64 2
+#define CUBIC_BLOCK_256X128 3
+#define CUBIC_BLOCK_256X256 4  /* 16-bit outputs */
+#define CUBIC_BLOCK_64X64_PAIRED 5
 CUBIC_API int64_t cubic_block_gemm_workspace_bytes(int64_t m, int64_t k, int members,
                                                    const int64_t* ns);
+CUBIC_API int64_t cubic_block_gemm_launch_plan(int64_t m, int64_t k, int members, const int64_t* ns,
+                                               int out_dtype, int* kernel, int* split);
 CUBIC_API int64_t cubic_block_prepared_bytes(int64_t n, int64_t k);
 CUBIC_API int cubic_block_prepare(const void* values, int64_t ld, int64_t n, int64_t k,
                                   void* prepared, void* stream);

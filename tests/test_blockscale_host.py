@@ -204,3 +204,29 @@ def test_tensors_that_grew_after_their_check():
         for refused in (lambda: ops.bind_block_linear(x, w, y), lambda: blockscale.prepare_block_matrix(w)):
             with pytest.raises(ValueError, match="scales"):
                 refused()
+
+
+def plan(m, k, ns, out=0):
+    """(workspace, kernel, K partitions) of a launch."""
+    c = _native.ctypes
+    kernel, split = c.c_int(), c.c_int()
+    need = _native.lib().cubic_block_gemm_launch_plan(m, k, len(ns), (c.c_int64 * len(ns))(*ns), out, c.byref(kernel), c.byref(split))
+    return need, kernel.value, split.value
+
+
+def test_launch_plans():
+    lib, c = _native.lib(), _native.ctypes
+    assert plan(1, 4096, [6144]) == (0, 0, 1) and plan(4096, 8192, [8192]) == (0, 4, 1)
+    assert plan(64, 12288, [4096])[1:] == (5, 4)
+    ns = (c.c_int64 * 1)(4096)
+    assert lib.cubic_block_gemm_launch_plan(64, 12288, 1, ns, 0, None, None) == plan(64, 12288, [4096])[0]
+    for bad in ((0, 128, 1, ns, 0), (64, 0, 1, ns, 0), (64, 128, 0, ns, 0), (64, 128, 9, ns, 0), (64, 128, 1, None, 0), (64, 128, 1, ns, 3),
+                (64, 128, 1, (c.c_int64 * 1)(0), 0)):
+        assert lib.cubic_block_gemm_launch_plan(*bad, None, None) == -1
+    # one workspace serves every type of output, and 32-bit ones never take the tile without registers for them
+    for m in (1, 8, 9, 64, 100, 257, 1000, 4096):
+        for k in (128, 1792, 4096, 12288):
+            for widths in ([1], [520, 1001], [4096], [8192, 1024], [24576], [151936]):
+                need, _, split = plan(m, k, widths)
+                assert all(plan(m, k, widths, out)[::2] == (need, split) for out in (1, 2)) and plan(m, k, widths, 2)[1] != 4
+                assert lib.cubic_block_gemm_workspace_bytes(m, k, len(widths), (c.c_int64 * len(widths))(*widths)) == need

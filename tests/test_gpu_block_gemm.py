@@ -18,6 +18,7 @@ import pytest
 import torch
 
 from cubic_serve_amd import blockscale, linear
+from test_blockscale_host import plan
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -331,3 +332,46 @@ def test_outputs_in_32_bits(m, n, k):
     x, w = activations(m, k, 53), matrix(n, k, 54)
     y, = product(x, [w], FP32)
     check32(x, w, y)
+
+
+STREAM, T64, T128, T256, WIDE, PAIRED = range(6)  # kernels of cubic_block_gemm_launch_plan
+OUTPUT_IDS = {BF16: 0, FP16: 1, FP32: 2}
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("m,n,k,kernel,split", [
+    (5, 640, 1040, STREAM, 1), (100, 1024, 1040, T64, 1), (1000, 2048, 528, T128, 1), (1000, 8192, 528, T256, 1), (2000, 8192, 272, WIDE, 1),
+    (100, 1024, 2064, PAIRED, 1), (100, 1024, 4112, PAIRED, 4),
+    # weights that are read past the cache
+    (5, 66048, 4864, T128, 1), (50, 65024, 4864, T128, 1), (120, 65024, 4864, T256, 1)])
+def test_every_kernel_writes_whole_lines(m, n, k, kernel, split, dtype):
+    """Rows of y that are whole lines of 128 bytes, in each type, through each kernel; the rows behind the last stay as they were."""
+    print(f"block gemm lines m={m} n={n} k={k} {dtype}", flush=True)
+    took = plan(m, k, [n], OUTPUT_IDS[dtype])[1:]
+    assert took == (T256 if kernel == WIDE and dtype is FP32 else kernel, split)
+    x, w = activations(m, k, 61, column_major=m % 2 == 0), matrix(n, k, 62)
+    y = torch.full((m + 3, n), 7.0, dtype=dtype, device=DEV)
+    linear.PackedLinearOperators().bind_block_linear(x, w, y[:m]).launch()
+    torch.cuda.synchronize()
+    assert y.data_ptr() % 128 == 0 and n * y.element_size() % 128 == 0
+    assert (y[m:] == 7).all()
+    check(x, w, y[:m], dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("m,k,ns", [(1, 1168, (1000, 24, 1, 392)), (5, 2064, (9000, 8000)), (40, 1168, (1000, 24, 392, 128)), (100, 1936, (1000, 24, 129, 77)),
+                                    (40, 4240, (1000, 520, 77)), (300, 528, (3000, 2048)), (1000, 272, (8192, 1024)), (300, 4240, (1000, 24, 3000)),
+                                    (2000, 272, (8192, 333))])
+def test_members_of_a_group_and_their_own_launches(m, k, ns, dtype):
+    """Through the same order of sums they are equal bit for bit: kernels that go through K in order, or the same one with
+    the same partitions.  (A group of many columns may take another order than a narrow member by itself.)"""
+    print(f"block gemm members m={m} k={k} ns={ns} {dtype}", flush=True)
+    order = lambda widths: (lambda need, kernel, split: (kernel if kernel in (STREAM, PAIRED) else None, split))(*plan(m, k, widths, OUTPUT_IDS[dtype]))
+    x, ws = activations(m, k, 63), [matrix(n, k, 64 + n) for n in ns]
+    equal = 0
+    for w, y in zip(ws, product(x, ws, dtype)):
+        check(x, w, y)
+        if order(ns) == order([w.shape[0]]):
+            assert torch.equal(y, product(x, [w], dtype)[0])
+            equal += 1
+    assert equal or order(ns)[0] is None
