@@ -352,8 +352,8 @@ def bind_block_linear_group(operators, x: BlockScaledActivations, weights: Seque
     if nbytes < 0:
         raise ValueError("block-scaled linear geometry not admitted")
     workspace = torch.zeros(nbytes, dtype=torch.uint8, device=device)
-    args = (values.data_ptr(), _stride(values), x.scales.data_ptr(), *x.scales.stride(), m, k, len(weights), widths, table(c.c_void_p, [p.data_ptr() for p, _ in prepared]),
-            table(c.c_void_p, [s.data_ptr() for _, s in prepared]), table(c.c_void_p, [y.data_ptr() for y in outputs]),
+    args = (values.data_ptr(), _stride(values), x.scales.data_ptr(), *x.scales.stride(), m, k, len(weights), widths,
+            table(c.c_void_p, [p.data_ptr() for p, _ in prepared]), table(c.c_void_p, [s.data_ptr() for _, s in prepared]), table(c.c_void_p, [y.data_ptr() for y in outputs]),
             table(c.c_int64, [_stride(y) for y in outputs]), OUTPUT_IDS[outputs[0].dtype], workspace.data_ptr(), nbytes)
     launch = _Launch("cubic_block_gemm", (values, x.scales, *outputs), args, held=(weights, prepared, workspace))
     return _binding(outputs, launch, device, scratch=(workspace,) if nbytes else ())

@@ -534,7 +534,7 @@ void block_tile_kernel(BlockGemmArgs a) {
 
 // ---------------------------------------------------------------------------
 // The largest tile, 256 columns by 256 rows: eight waves of 128 x 64, K block by block.
-// 4096 x 8192 x 8192 in 207 to 217 us, 2.6 P operations a second; the matrix cores are busy for 58 % of
+// 4096 x 8192 x 8192 in 207 to 223 us, 2.5 P operations a second; the matrix cores are busy for 62 % of
 // its cycles, and its loads bound it (262 us below are 180 without them, 255 without three quarters of its
 // additions), then the stores of y, two bursts of all CUs.  160 KB hold two blocks of both operands, so a place is loaded
 // again as soon as it is read: a wave has all of x in registers at a block's start, and half of the

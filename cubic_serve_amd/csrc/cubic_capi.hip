@@ -1038,13 +1038,16 @@ struct BlockPlan {
 // Up to 8 rows the stream kernel (mostly), else the tiles (columns x rows) whose rounds over 256
 // CUs are expected to end first, by what a block of K takes a round, in hundredths of a us:
 //   64 x 64 24, 128 x 64 36 and 10 more, 256 x 128 112, 256 x 256 180
-// (before outputs went past the caches) 4096 x 8192 x 8192: 432, 378, 283 and 229 us; 1024 rows x 8192 x 4096: 58, 50, 40 and 52; 512 x
-// 4096 x 4096: 17.7, 17.8, 33 and 50; 256 x 4096 x 12288: 32, 40, 82 and 126.  64 x 64 tiles that one
+// (4096 x 8192 x 8192 takes 21, 34, 102 and 170 of each: a seventh to a sixteenth less, in near
+// proportion).  In us, 4096 x 8192 x 8192: 421, 343, 260 and 217; 1024 rows x 8192 x 4096: 56, 48, 36 and 46; 512 x
+// 4096 x 4096: 16.9, 16.4, 31 and 46; 256 x 4096 x 12288: 31, 39, 80 and 122.  32-bit outputs (full), without
+// the 256 x 256 tile, which has no registers for fp16 operands: 620, 555 and 454; 82, 77 and 62; 27.1, 26.7
+// and 54; 48, 64 and 152.  64 x 64 tiles that one
 // round holds have two groups of waves from 14 blocks on, each every other block of K: 256 x 4096 x
-// 12288 32 and 26 us, 64 x 6144 x 4096 12.7 and 11.4, 333 x 1521 x 2048 8.8 and 8.4, x 1536 7.8
-// and 7.7, x 1024 6.4 and 6.5, x 512 4.9 and 5.3.  Rows of 6144 x 4096,
-// stream and tiles: 1 8.5 and 12.0, 8 10.8 and 10.7, 16 13.1 and 10.7.
-// 32-bit outputs (full) go by the same rule without the 256 x 256 tile, which has no registers for fp16 operands.
+// 12288 31 and 25 us, 64 x 6144 x 4096 12.1 and 10.9, 333 x 1521 x 2048 7.9 and 7.6, x 1536 6.5
+// and 6.5, x 1024 5.4 and 5.6, x 512 4.4 and 4.8.  Rows of 6144 x 4096,
+// stream and tiles: 1 8.3 and 9.7, 8 10.9 and 9.8 (9.4 with the stream where a block's scales of all
+// rows lie together), 16 13.3 and 9.7.
 BlockPlan plan_block(int64_t m, int64_t k, int members, const int64_t* ns, bool full) {
     BlockPlan p = {0, 1, 0, 0, 0};
     const int64_t blocks = ceil_div(k, cubic::kScaleBlock);
@@ -1055,8 +1058,8 @@ BlockPlan plan_block(int64_t m, int64_t k, int members, const int64_t* ns, bool 
     };
     if (m <= 8) {
         // Large weights in tiles that read past the cache, where every CU has two: 1 row of 151936 x
-        // 4096 114 us by the stream kernel and 100, 8 rows 129 and 113, 1 row of 80000 x 4096 61 and 59; of
-        // 20000 x 16384, 157 tiles, 61 and 71.
+        // 4096 116 us by the stream kernel and 114, 8 rows 129 and 108, 1 row of 80000 x 4096 62 and 61; of
+        // 20000 x 16384, 157 tiles, 72 and 69 (61 and 71 on another day).
         if (tiles(16, 8) * blocks * 2048 > cubic::kPastCacheBytes && tiles(128, 64) >= 512) p.tile = 2;
         return p;
     }
@@ -1066,8 +1069,8 @@ BlockPlan plan_block(int64_t m, int64_t k, int members, const int64_t* ns, bool 
     p.tile = 1 + (int)(std::min_element(cost, cost + (full ? 3 : 4)) - cost);
     if (p.tile != 1 || small > 256) return p;
     // K in as many parts as leave one round, at most 4 of 8 blocks and more.  One part and
-    // this, weights in a cache and not: 64 rows x 4096 x 12288 25 and 15 us, 38 and 20; 64 x 1024 x 8192
-    // 16 and 10, 17.6 and 10.6; 64 x 6144 x 4096 11.6 and 10.7, 15.6 and 13.9; 16 blocks 7.1 and 8.1.
+    // this, weights in a cache and not: 64 rows x 4096 x 12288 25 and 14 us, 38 and 19; 64 x 1024 x 8192
+    // 15.5 and 10, 17.2 and 10.3; 64 x 6144 x 4096 11.1 and 10.1, 15.2 and 12.4; 64 x 4096 x 2048 (16 blocks) 6.6 and 7.6.
     const int64_t split = blocks < 32 ? 1 : std::min({256 / small, blocks / 8, (int64_t)4});
     if (split > 1) {
         p.part_blocks = (int)ceil_div(ceil_div(blocks, split), 2) * 2;

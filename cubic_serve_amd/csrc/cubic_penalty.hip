@@ -17,8 +17,10 @@
 // What bounds the penalties: reading and writing the logits.  Listed tokens are a few
 // thousand of 10^5 columns, so each is looked up by itself, by the workgroup that has
 // its column: it reads the lists of its own columns only, and changes their logits in
-// LDS on their way.  256 rows of 151936, 3700 tokens listed for each: 39 us (38 under a
-// grammar, which admits 2 % of them), where a copy takes 31 and a history of no tokens 27.
+// LDS on their way.  256 rows of 151936 (64 sequences), 3700 tokens listed for each: 38 us (37
+// under a grammar, which admits 2 % of them), where a copy takes 31 and a history of no tokens 26.  In
+// place 34, and 69 under a grammar that admits half: whole vectors are written where nothing of
+// them is admitted, the masked columns one by one in the others.
 // What else was built, when this took 44 (its outputs went through the caches): listed tokens
 // changed in memory after the rest 69, one list per slot, which every workgroup of a row
 // has to search, 95, four rows of a sequence one after the other in a workgroup, for their common
@@ -211,7 +213,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(8, 8))
     // (all rows' first chunks first: vocabularies begin with the tokens that come often, so
     // those have the long lists and should not come last)
     // The rows of a sequence, eight sequences at a time, on one XCD (workgroups go round robin
-    // over the eight): its lists and marks come from one L2 (the 39 us were 42).
+    // over the eight): its lists and marks come from one L2 (38 us, and 42 without).
     int row = blockIdx.x;
     const int chunk = blockIdx.y, band = 8 * (a.depth + 1), within = row % band;
     if (row - within + band <= (int)gridDim.x) row = row - within + (within & 7) * (a.depth + 1) + (within >> 3);

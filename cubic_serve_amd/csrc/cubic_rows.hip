@@ -5,8 +5,8 @@
 //
 // y leaves in 16 bits, and / or per group of 128 columns as a 32-bit scale
 // s = max(max |y|, 2^-96) / 448 and values q = e4m3(y * (448 / max(max |y|, 2^-96))),
-// so that q s stands for y (448: the largest e4m3 value; below 2^-96 the scale's
-// reciprocal would leave the normal numbers).  h leaves in 16 bits too.  All is
+// so that q s stands for y (448: the largest e4m3 value; 2^-96, small beside any
+// activation, keeps 448 / top and what is scaled by it far from the largest number).  h leaves in 16 bits too.  All is
 // held in 32 bits and each output rounded once: y is computed from h as added, not
 // from the rounded one.  A NaN or an infinity makes all of its group NaN.
 //

@@ -49,7 +49,7 @@ CUBIC_API const char* cubic_last_error(void);
  * in the same dtype: ops/cuda/linear/quantized.py:348-405). */
 #define CUBIC_DTYPE_BF16 0
 #define CUBIC_DTYPE_F16 1
-#define CUBIC_DTYPE_F32 2  /* candidate preparation logits only */
+#define CUBIC_DTYPE_F32 2  /* logits of candidates, sampling and penalties; outputs of penalties and block-scaled products */
 
 /* ---------------------------------------------------------------------------
  * Cubic weight preparation (load time).
@@ -467,8 +467,8 @@ CUBIC_API int cubic_logit_penalties(const void* logits, int dtype, int64_t row_s
  * Per group of 128 columns (the last one may be shorter), in 32 bits:
  *   top = max(max |y|, 2^-96), scale = top / 448, q = e4m3(y * (448 / top))
  * The scale of group g of row r is at scales[r * scale_row + g * scale_group].
- * y is computed from h before its rounding.  A group that holds a NaN or an
- * infinity stands for NaNs.  Row strides in elements, at least k (any, for a
+ * y is computed from h before its rounding, also where squares of h leave the 32-bit
+ * numbers.  A group that holds a NaN or an infinity stands for NaNs.  Row strides in elements, at least k (any, for a
  * single row), of any alignment to an element.  1 <= k <= 2^24; no workspace.
  * ------------------------------------------------------------------------- */
 CUBIC_API int cubic_row_norm(const void* x, int64_t ldx, const void* residual, int64_t ldresidual,
