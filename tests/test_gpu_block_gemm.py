@@ -375,3 +375,24 @@ def test_members_of_a_group_and_their_own_launches(m, k, ns, dtype):
             assert torch.equal(y, product(x, [w], dtype)[0])
             equal += 1
     assert equal or order(ns)[0] is None
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+def test_every_code(dtype):
+    """Each of the 256 codes times 1, the numbers below the normal ones among them: exact in every type."""
+    codes = torch.arange(256, dtype=torch.uint8, device=DEV)
+    values = torch.zeros((256, 256), dtype=torch.uint8, device=DEV)
+    values[codes.long(), codes.long()] = codes
+    w = blockscale.BlockScaledMatrix(torch.ones((20, 256), device=DEV).to(E4M3), torch.ones((1, 2), device=DEV))
+    want = codes.view(E4M3).double()[:, None].expand(256, 20)
+    for m in (8, 40, 256):  # few rows, tiles
+        for first in range(0, 256 - m + 1, m):
+            x = blockscale.BlockScaledActivations(values[first:first + m].view(E4M3), torch.ones((m, 2), device=DEV))
+            y, = product(x, [w], dtype)
+            assert torch.equal(y.double().nan_to_num(1e9), want[first:first + m].nan_to_num(1e9))
+    # as weights, one code a column
+    w = blockscale.BlockScaledMatrix(values.view(E4M3), torch.ones((2, 2), device=DEV))
+    for m in (3, 70):
+        x = blockscale.BlockScaledActivations(torch.ones((m, 256), device=DEV).to(E4M3), torch.ones((m, 2), device=DEV))
+        y, = product(x, [w], dtype)
+        assert torch.equal(y.double().nan_to_num(1e9), want[:, 0].expand(m, 256).nan_to_num(1e9))
